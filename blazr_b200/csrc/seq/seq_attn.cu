@@ -663,11 +663,7 @@ static AttnPlan attn_plan(int T, int B, int H, int G, int max_keys) {
     return p;
 }
 
-}  // namespace b200seq
-
-using namespace b200seq;
-
-static int desc_check(const b200seq_attn_desc* d, const char* what) {
+int attn_desc_check(const b200seq_attn_desc* d, const char* what) {
     if (!d || d->H < 1 || d->G < 1 || d->H % d->G || d->D < 1 || d->V < 1 || d->q_col < 0 || d->k_col < 0 || d->v_col < 0)
         return fail(B200SEQ_ERR_INVALID_ARG, "%s: bad head counts, sizes or columns", what);
     if (!d->latent_v && d->v_col == d->k_col && d->V != d->D) return fail(B200SEQ_ERR_INVALID_ARG, "%s: values taken from the keys need V == D", what);
@@ -687,12 +683,16 @@ static int desc_check(const b200seq_attn_desc* d, const char* what) {
     return 0;
 }
 
+}  // namespace b200seq
+
+using namespace b200seq;
+
 extern "C" {
 
 int b200seq_attn_prep_ex(float* proj, int64_t ld, const b200seq_step* st, const b200seq_attn_desc* d, float* kpool, float* vpool, float* kpooled, float* vpooled,
                          void* stream) {
     if (!proj || !st || !d || ((!kpool || !vpool) && !d->kv_shared)) return fail(B200SEQ_ERR_INVALID_ARG, "attn_prep: bad arguments");
-    if (int rc = desc_check(d, "attn_prep")) return rc;
+    if (int rc = attn_desc_check(d, "attn_prep")) return rc;
     if (d->pool > 0 && (!kpooled || !vpooled)) return fail(B200SEQ_ERR_INVALID_ARG, "attn_prep: pooled blocks need their pools");
     if (st->T == 0) return 0;
     if (d->q_norm_w || d->k_norm_w || d->norm_full || d->rot_half || d->in_bias || d->kv_shared || d->vg > 0) {
@@ -774,7 +774,7 @@ size_t b200seq_attn_scratch_floats(int T, int B, int H, int G, int V, int max_ke
 int b200seq_attn_ex(const float* qkvg, int64_t ld, const b200seq_step* st, const b200seq_attn_desc* d, const float* kpool, const float* vpool,
                     const float* kpooled, const float* vpooled, void* out, int out_dtype, float* scratch, size_t scratch_floats, void* stream) {
     if (!qkvg || !st || !kpool || !out || !d || (!vpool && !d->latent_v)) return fail(B200SEQ_ERR_INVALID_ARG, "attn: bad arguments");
-    if (int rc = desc_check(d, "attn")) return rc;
+    if (int rc = attn_desc_check(d, "attn")) return rc;
     if (d->V > 512) return fail(B200SEQ_ERR_INVALID_ARG, "attn: value size <= 512");
     if (d->pool > 0 && (!kpooled || !vpooled)) return fail(B200SEQ_ERR_INVALID_ARG, "attn: pooled blocks need their pools");
     if (st->T == 0) return 0;

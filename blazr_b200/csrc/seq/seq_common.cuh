@@ -11,7 +11,10 @@ namespace b200seq {
 void count_launch(int n = 1);
 int fail(int code, const char* fmt, ...);
 int cuda_status(cudaError_t e, const char* what);
-int* error_flag_dev();   // device int: bit 0 = KV position outside the block table, bit 1 = bounded wait ran out, bit 2 = expert table entry out of range
+// device int: bit 0 = KV position outside the block table, bit 1 = bounded wait ran out, bit 2 = expert table entry out of range, bit 3 = a value beyond what
+// a 4-bit cache holds, bit 4 = a token id outside the vocabulary
+int* error_flag_dev();
+int attn_desc_check(const b200seq_attn_desc* d, const char* what);   // sizes, columns and combinations of an attention layer (seq_attn.cu)
 
 #define SEQ_LAUNCH_CHECK(what)                         \
     do {                                               \

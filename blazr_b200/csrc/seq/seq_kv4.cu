@@ -1,0 +1,226 @@
+// seq_kv4.cu -- keys and values into and out of a cache held in 4 bits (layout and rounding: seq_kv4.cuh).
+#include "seq_kv4.cuh"
+
+namespace b200seq {
+
+namespace {
+
+struct Kv4Rows {
+    const void *k, *v;
+    int64_t ldk, ldv;
+    uint8_t *kpool, *vpool;
+    int G, D, Gv, V, bf16, vec;
+};
+
+// position of a token in its sequence's pages; -1 (and the error flag) outside the block table
+__device__ __forceinline__ int64_t kv4_page(const b200seq_step& st, int t, int& o, int* err) {
+    const int pos = st.tok_pos[t], b = pos / st.block_size;
+    o = pos - b * st.block_size;
+    if (pos < 0 || b >= st.max_blocks) {
+        atomicOr(err, 1);
+        return -1;
+    }
+    return st.block_table[(int64_t)st.tok_ent[t] * st.max_blocks + b];
+}
+
+__device__ __forceinline__ void kv4_put(uint8_t* pool, const Kv4Row& at, bool key, int hl, int NG, uint32_t w, uint32_t param) {
+    *reinterpret_cast<uint16_t*>(pool + at.codes + kv4_place(key, hl, NG)) = (uint16_t)w;
+    if ((hl & 7) == 0) *reinterpret_cast<uint32_t*>(pool + at.params + (hl >> 3) * 4) = param;
+}
+
+// a warp per row (token, key or value head)
+__global__ void kv4_store_kernel(const Kv4Rows a, const b200seq_step st, int* err) {
+    chain_enter();
+    const int lane = threadIdx.x & 31, heads = a.G + a.Gv;
+    const int64_t unit = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    if (unit >= (int64_t)st.T * heads) return;
+    const int t = (int)(unit / heads), u = (int)(unit - (int64_t)t * heads);
+    const bool key = u < a.G;
+    const int g = key ? u : u - a.G, D = key ? a.D : a.V, G = key ? a.G : a.Gv, NG = kv4_groups(D);
+    int o;
+    const int64_t page = kv4_page(st, t, o, err);
+    if (page < 0) return;
+    const int64_t src = (int64_t)t * (key ? a.ldk : a.ldv) + (int64_t)g * D + 4 * lane;
+    const void* p = key ? a.k : a.v;
+    const int n = min(max(D - 4 * lane, 0), 4);
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (a.bf16) {
+        const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p) + src;
+        for (int i = 0; i < n; ++i) x[i] = __bfloat162float(q[i]);
+    } else {
+        const float* q = reinterpret_cast<const float*>(p) + src;
+        for (int i = 0; i < n; ++i) x[i] = q[i];
+    }
+    uint32_t param;
+    bool odd = false;
+    const uint32_t w = kv4_quantise(x, n, param, odd);
+    if (lane < NG * 8) kv4_put(key ? a.kpool : a.vpool, kv4_row(page, o, st.block_size, g, G, NG), key, lane, NG, w, param);
+    if (odd) atomicOr(err, KV4_ERR_RANGE);
+}
+
+// the same rows back, as the values they stand for
+__global__ void kv4_load_kernel(const Kv4Rows a, float* __restrict__ ko, float* __restrict__ vo, const b200seq_step st, int* err) {
+    chain_enter();
+    const int lane = threadIdx.x & 31, heads = a.G + a.Gv;
+    const int64_t unit = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    if (unit >= (int64_t)st.T * heads) return;
+    const int t = (int)(unit / heads), u = (int)(unit - (int64_t)t * heads);
+    const bool key = u < a.G;
+    const int g = key ? u : u - a.G, D = key ? a.D : a.V, G = key ? a.G : a.Gv, NG = kv4_groups(D);
+    int o;
+    const int64_t page = kv4_page(st, t, o, err);
+    if (page < 0) return;
+    const uint8_t* pool = key ? a.kpool : a.vpool;
+    const Kv4Row at = kv4_row(page, o, st.block_size, g, G, NG);
+    const int n = min(max(D - 4 * lane, 0), 4);
+    if (n == 0) return;
+    const uint32_t w = *reinterpret_cast<const uint16_t*>(pool + at.codes + kv4_place(key, lane, NG));
+    const uint32_t pr = *reinterpret_cast<const uint32_t*>(pool + at.params + (lane >> 3) * 4);
+    const float s = __half2float(__ushort_as_half((uint16_t)pr)), m = __half2float(__ushort_as_half((uint16_t)(pr >> 16)));
+    float* dst = (key ? ko + (int64_t)t * a.ldk : vo + (int64_t)t * a.ldv) + (int64_t)g * D + 4 * lane;
+    for (int i = 0; i < n; ++i) dst[i] = fmaf(s, (float)((w >> (4 * i)) & 15u), m);
+}
+
+// b200seq_attn_prep_ex over 4-bit pages: grid (T), 256 threads, a warp per head unit; the unit's values are staged in the warp's slice of shared memory, biased,
+// normed, turned, and written back (queries) or quantised into the token's row.  Shared memory: rot_dims floats (cos | sin) + 8 * Dmax + 40.
+__global__ void kv4_prep_kernel(float* __restrict__ proj, int64_t ld, const b200seq_step st, const b200seq_attn_desc a, uint8_t* __restrict__ kpool,
+                                uint8_t* __restrict__ vpool, int Dmax, int* err) {
+    chain_enter();
+    extern __shared__ float gsm[];
+    float* rot_sm = gsm;
+    float* stage = gsm + a.rot_dims;
+    float* red = stage + 8 * Dmax;
+    const int t = blockIdx.x, lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    const int pos = st.tok_pos[t];
+    const int H = a.H, G = a.G, D = a.D, V = a.V, Gv = a.vg > 0 ? a.vg : G, np = a.rot_dims >> 1;
+    int o = 0;
+    const int64_t page = a.kv_shared ? -1 : kv4_page(st, t, o, err);
+    float* base = proj + (int64_t)t * ld;
+    for (int i = threadIdx.x; i < np; i += blockDim.x) {
+        float sn, cs;
+        sincosf((float)pos * a.rot_freq[i], &sn, &cs);
+        rot_sm[i] = cs * a.rot_scale, rot_sm[np + i] = sn * a.rot_scale;
+    }
+    auto biased = [&](int col) { return base[col] + (a.in_bias ? a.in_bias[col] : 0.f); };
+    float rq = 1.f, rk = 1.f;
+    if (a.norm_full && a.qk_eps >= 0.f) {
+        float sq = 0.f, sk = 0.f;
+        for (int i = threadIdx.x; i < H * D; i += blockDim.x) sq = fmaf(biased(a.q_col + i), biased(a.q_col + i), sq);
+        rq = 1.0f / sqrtf(block_sum(sq, red) / (float)(H * D) + a.qk_eps);
+        if (!a.kv_shared) {
+            for (int i = threadIdx.x; i < G * D; i += blockDim.x) sk = fmaf(biased(a.k_col + i), biased(a.k_col + i), sk);
+            rk = 1.0f / sqrtf(block_sum(sk, red) / (float)(G * D) + a.qk_eps);
+        }
+    }
+    __syncthreads();   // rot_sm
+    float* hs = stage + wid * Dmax;
+    bool odd = false;
+    const int nu = a.kv_shared ? H : H + G + Gv;
+    for (int u = wid; u < nu; u += nw) {
+        const bool isq = u < H, isk = !isq && u < H + G;
+        const int hh = isq ? u : (isk ? u - H : u - H - G), size = isq || isk ? D : V;
+        const int col = (isq ? a.q_col : (isk ? a.k_col : a.v_col)) + hh * size;
+        float ss = 0.f;
+        for (int d = lane; d < size; d += 32) {
+            const float v = biased(col + d);
+            hs[d] = v;
+            ss = fmaf(v, v, ss);
+        }
+        if (isq || isk) {
+            const float* w = isq ? a.q_norm_w : a.k_norm_w;
+            if (a.qk_eps >= 0.f) {
+                const float rinv = a.norm_full ? (isq ? rq : rk) : 1.0f / sqrtf(warp_sum(ss) / (float)D + a.qk_eps);
+                for (int d = lane; d < D; d += 32) hs[d] = hs[d] * rinv * (w ? w[a.norm_full ? hh * D + d : d] : 1.f);
+            }
+            __syncwarp();
+            for (int i = lane; i < np; i += 32) {   // a lane turns whole pairs
+                const int d0 = a.rot_half ? i : 2 * i, d1 = a.rot_half ? i + np : 2 * i + 1;
+                const float x = hs[d0], y = hs[d1], cs = rot_sm[i], sn = rot_sm[np + i];
+                hs[d0] = fmaf(x, cs, -y * sn), hs[d1] = fmaf(y, cs, x * sn);
+            }
+        }
+        __syncwarp();
+        if (isq) {
+            for (int d = lane; d < D; d += 32) base[col + d] = hs[d];
+        } else if (page >= 0) {
+            const int n = min(max(size - 4 * lane, 0), 4), NG = kv4_groups(size);
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = i < n ? hs[4 * lane + i] : 0.f;
+            uint32_t param;
+            const uint32_t w = kv4_quantise(x, n, param, odd);
+            if (lane < NG * 8) kv4_put(isk ? kpool : vpool, kv4_row(page, o, st.block_size, hh, isk ? G : Gv, NG), isk, lane, NG, w, param);
+        }
+        __syncwarp();   // hs is used again by the warp's next unit
+    }
+    if (odd) atomicOr(err, KV4_ERR_RANGE);
+}
+
+int step_check(const b200seq_step* st, const char* what) {
+    if (!st || st->T < 0 || st->B < 0 || st->block_size < 1 || st->max_blocks < 0) return fail(B200SEQ_ERR_INVALID_ARG, "%s: bad step", what);
+    if (st->T > 0 && (!st->tok_ent || !st->tok_pos || !st->block_table)) return fail(B200SEQ_ERR_INVALID_ARG, "%s: the step lacks its arrays", what);
+    if (st->block_size > 1 << 16) return fail(B200SEQ_ERR_UNSUPPORTED, "%s: pages of up to 65536 tokens", what);
+    return 0;
+}
+
+int rows_check(const b200seq_step* st, const void* k, const void* v, int64_t ldk, int64_t ldv, int G, int D, int Gv, int V, const void* kpool, const void* vpool, const char* what) {
+    if (int rc = step_check(st, what)) return rc;
+    if (G < 1 || Gv < 1 || D < 1 || V < 1 || !kpool || !vpool || (st->T > 0 && (!k || !v))) return fail(B200SEQ_ERR_INVALID_ARG, "%s: bad sizes or null arrays", what);
+    if (D > KV4_MAX_DIM || V > KV4_MAX_DIM) return fail(B200SEQ_ERR_UNSUPPORTED, "%s: heads of up to %d values", what, KV4_MAX_DIM);
+    if (st->T > 1 && (ldk < (int64_t)G * D || ldv < (int64_t)Gv * V)) return fail(B200SEQ_ERR_INVALID_ARG, "%s: row strides below a row's length", what);
+    if ((reinterpret_cast<uintptr_t>(kpool) | reinterpret_cast<uintptr_t>(vpool)) & 15) return fail(B200SEQ_ERR_INVALID_ARG, "%s: pools start on a 16-byte boundary", what);
+    if (((int64_t)st->T * ((int64_t)G + Gv) + 7) / 8 > 0x7fffffff) return fail(B200SEQ_ERR_UNSUPPORTED, "%s: too many rows", what);
+    return 0;
+}
+
+}  // namespace
+
+}  // namespace b200seq
+
+using namespace b200seq;
+
+extern "C" {
+
+int64_t b200seq_kv4_page_bytes(int block_size, int G, int D) {
+    if (block_size < 1 || G < 1 || D < 1 || D > KV4_MAX_DIM) return 0;
+    return (int64_t)block_size * G * kv4_groups(D) * 20;
+}
+
+int b200seq_kv4_store(const void* k, int64_t ldk, const void* v, int64_t ldv, int in_dtype, const b200seq_step* st, int G, int D, int Gv, int V, void* kpool, void* vpool,
+                      void* stream) {
+    if (in_dtype != B200SEQ_F32 && in_dtype != B200SEQ_BF16) return fail(B200SEQ_ERR_INVALID_ARG, "kv4_store: rows are f32 or bf16");
+    if (int rc = rows_check(st, k, v, ldk, ldv, G, D, Gv, V, kpool, vpool, "kv4_store")) return rc;
+    if (st->T == 0) return 0;
+    const Kv4Rows a{k, v, ldk, ldv, (uint8_t*)kpool, (uint8_t*)vpool, G, D, Gv, V, in_dtype == B200SEQ_BF16, 0};
+    const int64_t rows = (int64_t)st->T * (G + Gv);
+    launch_chained(kv4_store_kernel, dim3((unsigned)((rows + 7) / 8)), 256, 0, (cudaStream_t)stream, a, *st, error_flag_dev());
+    SEQ_LAUNCH_CHECK("kv4_store");
+    return 0;
+}
+
+int b200seq_kv4_load(const void* kpool, const void* vpool, const b200seq_step* st, int G, int D, int Gv, int V, float* k, int64_t ldk, float* v, int64_t ldv, void* stream) {
+    if (int rc = rows_check(st, k, v, ldk, ldv, G, D, Gv, V, kpool, vpool, "kv4_load")) return rc;
+    if (st->T == 0) return 0;
+    const Kv4Rows a{nullptr, nullptr, ldk, ldv, (uint8_t*)kpool, (uint8_t*)vpool, G, D, Gv, V, 0, 0};
+    const int64_t rows = (int64_t)st->T * (G + Gv);
+    launch_chained(kv4_load_kernel, dim3((unsigned)((rows + 7) / 8)), 256, 0, (cudaStream_t)stream, a, k, v, *st, error_flag_dev());
+    SEQ_LAUNCH_CHECK("kv4_load");
+    return 0;
+}
+
+int b200seq_attn_prep_kv4(float* proj, int64_t ld, const b200seq_step* st, const b200seq_attn_desc* d, void* kpool, void* vpool, void* stream) {
+    if (int rc = step_check(st, "attn_prep_kv4")) return rc;
+    if (int rc = attn_desc_check(d, "attn_prep_kv4")) return rc;
+    if (!proj || ((!kpool || !vpool) && !d->kv_shared)) return fail(B200SEQ_ERR_INVALID_ARG, "attn_prep_kv4: bad arguments");
+    if (d->pool > 0 || d->latent_v || d->krot || d->ctx_rows) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_prep_kv4: a 4-bit cache holds plain keys and values (no pooled blocks, no latents)");
+    if (d->D > KV4_MAX_DIM || d->V > KV4_MAX_DIM) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_prep_kv4: heads of up to %d values", KV4_MAX_DIM);
+    if ((reinterpret_cast<uintptr_t>(kpool) | reinterpret_cast<uintptr_t>(vpool)) & 15) return fail(B200SEQ_ERR_INVALID_ARG, "attn_prep_kv4: pools start on a 16-byte boundary");
+    if (st->T == 0) return 0;
+    const int Dmax = d->D > d->V ? d->D : d->V;
+    const size_t smem = (size_t)(d->rot_dims + 8 * Dmax + 40) * sizeof(float);
+    launch_chained(kv4_prep_kernel, st->T, 256, smem, (cudaStream_t)stream, proj, ld, *st, *d, (uint8_t*)kpool, (uint8_t*)vpool, Dmax, error_flag_dev());
+    SEQ_LAUNCH_CHECK("attn_prep_kv4");
+    return 0;
+}
+
+}  // extern "C"

@@ -1,0 +1,81 @@
+// seq_kv4.cuh -- KV pages held in 4 bits: the layout of a page, and how 32 values become codes.
+//
+// A row of D values (one position, one head) is NG = 1, 2 or 4 groups of 32 (D <= 32, 64, 128; places behind D are held as zero).  A group has a minimum m and a
+// step s, both f16, and a 4-bit code per value, which stands for m + s * code:
+//   m = f16(min x),  s = (max x - m) * (1 / 15) rounded up to 7 significant bits and to a multiple of 2^-24,  code = clamp(rint((x - m) * (1 / s)), 0, 15)
+// (1 / 15 is the f32 number below it, so that a range of fifteen whole steps keeps its step).  Seven bits, because s * code is then an f16 number (7 + 4 bits): the
+// tensor cores multiply what the cache holds with no further rounding.  It costs a step that is up to 1.6 % wider; a minimum beside it
+// serves keys, whose channels do not lie around zero.  Values are limited to +-32000 (15 s stays an f16 number), NaN is held as 0; either raises bit 3 of the error flags.
+//
+// Bytes of a pool: [page][head][segment], so that one head's rows of a page are consecutive (10 NG 16-byte pieces a unit of 16 rows: one request of a warp or
+// two).  A segment is cut into units of 16 rows (block sizes that are not a multiple of 16: one unit of all rows), each unit holds its rows' codes (16 NG
+// bytes a row), then its rows' (s, m) pairs (4 NG bytes a row).  Order of a row's codes, low 4 bits first:
+//   keys    32-bit words [part c < 4][group],  eight values 32 group + 8 c + i:  thread c of a quad reads its words of all groups in one piece
+//   values  16-bit words [part r < 8][group],  four values 32 group + 4 r + i:   the eight threads that hold a column of the product each, likewise
+#pragma once
+#include <cuda_fp16.h>
+
+#include "seq_common.cuh"
+
+namespace b200seq {
+
+constexpr int KV4_MAX_DIM = 128;
+constexpr int KV4_ERR_RANGE = 8;         // error flag: a value that is not a number within +-32000 was stored
+constexpr float KV4_LIMIT = 32000.f;
+constexpr float KV4_FIFTEENTH = 0x1.11111p-4f;
+
+__host__ __device__ __forceinline__ int kv4_groups(int D) { return D <= 32 ? 1 : (D <= 64 ? 2 : 4); }
+__host__ __device__ __forceinline__ int kv4_unit(int bs) { return bs % 16 == 0 ? 16 : bs; }
+
+// row `o` of a page of `bs` rows, head g of G: offset of its codes and of its parameters in the pool
+struct Kv4Row {
+    int64_t codes, params;
+};
+__device__ __forceinline__ Kv4Row kv4_row(int64_t page, int o, int bs, int g, int G, int NG) {
+    const int unit = kv4_unit(bs), u = o / unit, ru = o - u * unit;
+    const int64_t base = (page * G + g) * (int64_t)(bs * NG * 20) + (int64_t)u * (unit * NG * 20);
+    return Kv4Row{base + ru * NG * 16, base + unit * NG * 16 + ru * NG * 4};
+}
+
+// A group of 32 values, four in each of eight neighbouring lanes (`n` of the lane's four are values of the row, the rest do not exist).  Returns the lane's four
+// codes in 16 bits and, the same in all eight lanes, the (s, m) pair.  Every lane of the warp takes part.
+__device__ __forceinline__ uint32_t kv4_quantise(float (&x)[4], int n, uint32_t& param, bool& odd) {
+    float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float y = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -KV4_LIMIT), KV4_LIMIT);
+        if (i < n) {
+            odd |= !(y == x[i]);
+            lo = fminf(lo, y), hi = fmaxf(hi, y);
+        }
+        x[i] = y;
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)), hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    if (!(lo <= hi)) {   // a group behind the row's end
+        param = 0;
+        return 0;
+    }
+    const __half mh = __float2half_rn(lo);
+    const float m = __half2float(mh);
+    float s = fmaxf((hi - m) * KV4_FIFTEENTH, 0.f);
+    s = __uint_as_float((__float_as_uint(s) + 0x1FFFFu) & ~0x1FFFFu);
+    if (s < 0x1p-18f) s = ceilf(s * 0x1p24f) * 0x1p-24f;
+    param = (uint32_t)__half_as_ushort(__float2half_rn(s)) | ((uint32_t)__half_as_ushort(mh) << 16);
+    const float inv = s > 0.f ? 1.0f / s : 0.f;
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int c = min(max(__float2int_rn((x[i] - m) * inv), 0), 15);
+        w |= (i < n ? (uint32_t)c : 0u) << (4 * i);
+    }
+    return w;
+}
+
+// place of a lane's four codes in the row: lane hl holds values 4 hl .. 4 hl + 3
+__device__ __forceinline__ int kv4_place(bool key, int hl, int NG) {
+    const int g = hl >> 3, r = hl & 7;
+    return key ? (((r >> 1) * NG + g) * 2 + (r & 1)) * 2 : (r * NG + g) * 2;
+}
+
+}  // namespace b200seq

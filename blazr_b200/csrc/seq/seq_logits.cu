@@ -1,0 +1,132 @@
+// seq_logits.cu -- what a request's sampling rules make of its logits, in one pass over the row: penalties for repeated tokens, biases, temperature, grammar mask.
+//
+// A block has a slice of one row's vocabulary.  It counts the row's history into a table in shared memory (only the tokens of its slice; whole numbers, so the order of
+// the additions does not matter), then reads, changes and writes its logits once.  Bounded by the logits' bytes, 8 a token; the history is read by every slice,
+// from L2.
+#include "seq_common.cuh"
+
+namespace b200seq {
+
+namespace {
+
+constexpr int THREADS = 256;
+constexpr int ERR_TOKEN = 16;            // error flag: a token id outside the vocabulary
+constexpr uint32_t SEEN = 0x80000000u;   // in the table: the token stands in the prompt
+
+struct LogitArgs {
+    const float* x;
+    float* out;
+    int64_t ldx, ldo;
+    int V;
+    const float* rules;                        // [R][4]: repetition, presence, frequency, temperature
+    const int32_t *hist, *hist_start, *hist_prompt;
+    const int32_t *bias_start, *bias_ids;
+    const float* bias_vals;
+    const uint32_t* mask;                      // [R][mask_ld]: bit v % 32 of word v / 32
+    int64_t mask_ld;
+    int vec;
+    int* err;
+};
+
+// grid (slices of 4 * ITEMS * THREADS tokens, rows).  Dynamic shared memory: the counts and, with biases, the number of the entry that holds for a token.
+template <int ITEMS>
+__global__ void __launch_bounds__(THREADS) process_logits_kernel(const __grid_constant__ LogitArgs a) {
+    chain_enter();
+    constexpr int S = 4 * ITEMS * THREADS;
+    extern __shared__ __align__(16) uint32_t table[];
+    uint32_t* entry = table + S;
+    const int row = blockIdx.y, v0 = blockIdx.x * S, n = min(S, a.V - v0);
+    const float* x = a.x + row * a.ldx + v0;
+    float4 v[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const int i = 4 * (k * THREADS + threadIdx.x);
+        if (a.vec && i + 3 < n) v[k] = ld4(x + i);
+        else v[k] = make_float4(i < n ? x[i] : 0.f, i + 1 < n ? x[i + 1] : 0.f, i + 2 < n ? x[i + 2] : 0.f, i + 3 < n ? x[i + 3] : 0.f);
+    }
+    for (int i = threadIdx.x; i < (a.bias_ids ? 2 * S : S) / 4; i += THREADS) reinterpret_cast<uint4*>(table)[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    bool odd = false;
+    if (a.hist) {
+        const int h0 = a.hist_start[row], h1 = a.hist_start[row + 1], prompt = h0 + a.hist_prompt[row];
+        for (int i = h0 + threadIdx.x; i < h1; i += THREADS) {
+            const int id = a.hist[i];
+            if ((unsigned)id >= (unsigned)a.V) odd = true;
+            else if ((unsigned)(id - v0) < (unsigned)n) {
+                if (i < prompt) atomicOr(table + (id - v0), SEEN);
+                else atomicAdd(table + (id - v0), 1u);
+            }
+        }
+    }
+    const int b0 = a.bias_ids ? a.bias_start[row] : 0;
+    if (a.bias_ids) {
+        const int b1 = a.bias_start[row + 1];
+        for (int i = b0 + threadIdx.x; i < b1; i += THREADS) {
+            const int id = a.bias_ids[i];
+            if ((unsigned)id >= (unsigned)a.V) odd = true;
+            else if ((unsigned)(id - v0) < (unsigned)n) atomicMax(entry + (id - v0), (uint32_t)(i - b0 + 1));
+        }
+    }
+    if (odd && blockIdx.x == 0) atomicOr(a.err, ERR_TOKEN);
+    __syncthreads();
+    const float4 rule = ld4(a.rules + 4 * (int64_t)row);   // repetition, presence, frequency, temperature
+    float* out = a.out + row * a.ldo + v0;
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        const int i = 4 * (k * THREADS + threadIdx.x);
+        if (i >= n) continue;
+        const uint4 cnt = *reinterpret_cast<const uint4*>(table + i);
+        const uint32_t cs[4] = {cnt.x, cnt.y, cnt.z, cnt.w};
+        float y[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+        uint32_t bits = 0xFu;
+        if (a.mask) bits = a.mask[row * a.mask_ld + ((v0 + i) >> 5)] >> ((v0 + i) & 31);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (cs[j]) {
+                y[j] = y[j] > 0.f ? y[j] / rule.x : y[j] * rule.x;
+                const uint32_t times = cs[j] & ~SEEN;
+                if (times) y[j] = y[j] - (float)times * rule.z - rule.y;
+            }
+            if (a.bias_ids) {
+                const uint32_t w = entry[i + j];
+                if (w) y[j] += a.bias_vals[b0 + (int)w - 1];
+            }
+            if (rule.w != 0.f) y[j] /= rule.w;
+            if (!((bits >> j) & 1u)) y[j] = -INFINITY;
+        }
+        if (a.vec && i + 3 < n) *reinterpret_cast<float4*>(out + i) = make_float4(y[0], y[1], y[2], y[3]);
+        else
+            for (int j = 0; j < 4 && i + j < n; ++j) out[i + j] = y[j];
+    }
+}
+
+template <int ITEMS>
+cudaError_t launch(const LogitArgs& a, int R, cudaStream_t cs) {
+    constexpr int S = 4 * ITEMS * THREADS;
+    launch_chained(process_logits_kernel<ITEMS>, dim3((a.V + S - 1) / S, R), THREADS, (size_t)S * 4 * (a.bias_ids ? 2 : 1), cs, a);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+}  // namespace b200seq
+
+using namespace b200seq;
+
+extern "C" int b200seq_process_logits(const float* x, int64_t ldx, int R, int V, const float* rules, const int32_t* hist, const int32_t* hist_start, const int32_t* hist_prompt,
+                                      const int32_t* bias_start, const int32_t* bias_ids, const float* bias_vals, const uint32_t* mask, int64_t mask_ld, float* out, int64_t ldo,
+                                      void* stream) {
+    if (R < 0 || V < 1 || (R > 0 && (!x || !out || !rules))) return fail(B200SEQ_ERR_INVALID_ARG, "process_logits: bad sizes or null arrays");
+    if ((hist != nullptr) != (hist_start != nullptr) || (hist != nullptr) != (hist_prompt != nullptr)) return fail(B200SEQ_ERR_INVALID_ARG, "process_logits: a history has ids, row starts and prompt lengths");
+    if ((bias_ids != nullptr) != (bias_start != nullptr) || (bias_ids != nullptr) != (bias_vals != nullptr)) return fail(B200SEQ_ERR_INVALID_ARG, "process_logits: biases have ids, values and row starts");
+    if (R > 65535) return fail(B200SEQ_ERR_UNSUPPORTED, "process_logits: up to 65535 rows");
+    if (R > 1 && (ldx < V || ldo < V || (mask && mask_ld < (V + 31) / 32))) return fail(B200SEQ_ERR_INVALID_ARG, "process_logits: row strides below a row's length");
+    if (reinterpret_cast<uintptr_t>(rules) & 15) return fail(B200SEQ_ERR_INVALID_ARG, "process_logits: rules start on a 16-byte boundary");
+    if (R == 0) return 0;
+    const LogitArgs a{x, out, ldx, ldo, V, rules, hist, hist_start, hist_prompt, bias_start, bias_ids, bias_vals, mask, mask_ld,
+                      ((ldx | ldo) & 3) == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 15) == 0, error_flag_dev()};
+    const cudaError_t e = launch<1>(a, R, (cudaStream_t)stream);
+    if (e != cudaSuccess) return cuda_status(e, "process_logits");
+    count_launch();
+    return 0;
+}

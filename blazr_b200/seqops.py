@@ -4,7 +4,7 @@ over a paged KV pool, the state-space recurrence, gated activations, the depth-a
 latent attention, per-head projections, token shift + gated post-norm, the branch sum + output norm of two-branch mixers, the bigram
 embedding, PolyNorm, soft caps, differential attention, minGRU and real-gated linear recurrences, soft-max routing with identity experts,
 the delta rule with per-channel decays, layers normed on both sides with sinusoidal positions and a token-dependent addition, the selective scan
-with a decay per channel and state, the residual of parallel layers, arg-max).
+with a decay per channel and state, the residual of parallel layers, a KV cache held in 4 bits and its attention, page copies, sampling rules, arg-max).
 
 Like blazr_b200/ops.py, PyTorch is plumbing only (device memory, streams); every compute call goes through ctypes.  The library
 is compiled on first use when it is missing (`ensure_built`): a fresh checkout needs nothing but nvcc.  There is no CPU
@@ -17,7 +17,9 @@ import fcntl
 import os
 import shutil
 import subprocess
-from typing import Optional
+from array import array
+from itertools import chain
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -44,7 +46,8 @@ EXPORTS = ["b200seq_last_error", "b200seq_version", "b200seq_launch_count", "b20
            "b200seq_moe_route_ex", "b200seq_moe_router_ex", "b200seq_moe_combine_ex", "b200seq_causal_conv_ex", "b200seq_embed_bigram", "b200seq_branch_norm", "b200seq_polynorm", "b200seq_softcap",
            "b200seq_diff_combine", "b200seq_min_gru", "b200seq_rg_lru", "b200seq_delta", "b200seq_delta_scratch_floats", "b200seq_embed_pos", "b200seq_sandwich_norm",
            "b200seq_token_gate", "b200seq_side_close", "b200seq_linear_silu", "b200seq_moe_route_rule", "b200seq_moe_router_rule", "b200seq_retention_partials",
-           "b200seq_selective_scan", "b200seq_scan_scratch_floats", "b200seq_parallel_close"]
+           "b200seq_selective_scan", "b200seq_scan_scratch_floats", "b200seq_parallel_close", "b200seq_kv4_page_bytes", "b200seq_kv4_store", "b200seq_kv4_load",
+           "b200seq_attn_prep_kv4", "b200seq_attn_kv4", "b200seq_copy_pages", "b200seq_process_logits"]
 
 # argument types of the operators' C entries (include/b200seq.h): p pointer, i int, l int64, z size_t, f float.  Declared, plain numbers are converted by ctypes
 # as they are passed; an object made for each of them and a stream object looked up for each call took half of a call's 4 - 8 us.
@@ -61,7 +64,8 @@ SIGNATURES = {
     "moe_combine_ex": "ppppipiiipplpp", "causal_conv_ex": "plpppppiiipilpilp", "embed_bigram": "pppppfiiiippip", "branch_norm": "ppppfppfpfipippipp",
     "polynorm": "pliipfpilp", "softcap": "plfp", "diff_combine": "piiiifffpip", "min_gru": "pliiipppipip", "rg_lru": "plplppfplipppiipip", "delta": "plppplppipzp",
     "embed_pos": "pppfpippppfpip", "sandwich_norm": "pppfppipippipp", "token_gate": "pliiplippip", "side_close": "pppfpppliippppipippipp",
-    "selective_scan": "piplpplppppipzp", "parallel_close": "pp", "argmax": "piipp"
+    "selective_scan": "piplpplppppipzp", "parallel_close": "pp", "argmax": "piipp", "kv4_page_bytes": "iii", "kv4_store": "plplipiiiippp", "kv4_load": "pppiiiiplplp",
+    "attn_prep_kv4": "plppppp", "attn_kv4": "plpppppip", "copy_pages": "ppiippip", "process_logits": "pliipppppppplplp"
 }
 
 
@@ -202,6 +206,7 @@ def lib() -> C.CDLL:
         L = C.CDLL(LIB_PATH)
         L.b200seq_last_error.restype = C.c_char_p
         L.b200seq_launch_count.restype = C.c_int64
+        L.b200seq_kv4_page_bytes.restype = C.c_int64
         for name, args in SIGNATURES.items():
             getattr(L, "b200seq_" + name).argtypes = [_ARG[a] for a in args]
         _lib = L
@@ -849,3 +854,166 @@ def parallel_close(x: torch.Tensor, y1: torch.Tensor, mult: float, eps: float, *
     d = ParallelDesc(ptr(x), ptr(y1), ptr(w_b1), ptr(sumsq), sumsq.shape[1] if sumsq is not None else 0, sumsq_count, s1, ptr(y2), ptr(w_b2), s2, ptr(y3), ptr(ys), ptr(wts),
                      ptr(slot_of), top, mult, ptr(add_vec), eps, W, ptr(rows), R, ptr(x_out), ptr(a_out), _DT[a_out.dtype] if a_out is not None else F32, ptr(fin_w))
     _check(lib().b200seq_parallel_close(C.byref(d), _st(x)))
+
+
+# ---- a KV cache held in 4 bits -----------------------------------------------------------------------------------------------------------------------
+KV4_MAX_DIM = 128
+
+
+def kv4_page_bytes(block_size: int, heads: int, dim: int) -> int:
+    """bytes of one page of `block_size` positions: 0.625 a value (heads of up to 32, 64 or 128 values are held as that many)"""
+    n = int(lib().b200seq_kv4_page_bytes(block_size, heads, dim))
+    if n == 0:
+        raise ValueError(f"a 4-bit cache holds heads of 1 to {KV4_MAX_DIM} values, not pages of {block_size} positions of {heads} heads of {dim}")
+    return n
+
+
+def kv4_pool(num_blocks: int, block_size: int, heads: int, dim: int, device) -> torch.Tensor:
+    """uint8 pool of zeroed pages [num_blocks, heads, bytes of a head's page] for rows of `heads` heads of `dim` values (layout: include/b200seq.h)"""
+    return torch.zeros((num_blocks, heads, kv4_page_bytes(block_size, 1, dim)), dtype=torch.uint8, device=device)
+
+
+def _on_device(name: str, fn, args: tuple, *tensors: Optional[torch.Tensor]) -> None:
+    """a library call on the one CUDA device of its tensors, on that device's current stream (the library launches on the current device)"""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if t.device.type != "cuda":
+            raise ValueError(f"{name}: Expected a cuda device, but got: {t.device}")
+        if dev is not None and t.device != dev:
+            raise ValueError(f"{name}: tensors on {dev} and {t.device}")
+        dev = t.device
+    if dev.index == torch.cuda.current_device():
+        _check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index)))
+    else:
+        with torch.cuda.device(dev):
+            _check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index)))
+
+
+def _kv4_pool_check(name: str, what: str, pool: torch.Tensor, block_size: int, heads: int, dim: int) -> None:
+    if pool.dtype != torch.uint8 or pool.dim() != 3 or not pool.is_contiguous() or pool.shape[1] != heads or pool.shape[2] != 20 * block_size * (1 if dim <= 32 else 2 if dim <= 64 else 4):
+        raise ValueError(f"{name}: the {what} pool is no contiguous uint8 [pages, {heads}, bytes] of pages of {block_size} positions and heads of {dim} values: "
+                         f"{pool.dtype} {tuple(pool.shape)}")
+
+
+def _kv4_rows(name: str, k: torch.Tensor, v: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, step: "StepDesc"):
+    G, Gv = kpool.shape[1], vpool.shape[1]
+    if k.dim() != 2 or v.dim() != 2 or k.stride(1) != 1 or v.stride(1) != 1 or k.shape[0] != step.T or v.shape[0] != step.T or k.shape[1] % G or v.shape[1] % Gv or k.dtype != v.dtype:
+        raise ValueError(f"{name}: rows {tuple(k.shape)} and {tuple(v.shape)} of {step.T} tokens do not fit {G} and {Gv} heads")
+    D, V = k.shape[1] // G, v.shape[1] // Gv
+    _kv4_pool_check(name, "key", kpool, step.block_size, G, D)
+    _kv4_pool_check(name, "value", vpool, step.block_size, Gv, V)
+    return G, D, Gv, V
+
+
+@_timed
+def kv4_store(k: torch.Tensor, v: torch.Tensor, step: "StepDesc", kpool: torch.Tensor, vpool: torch.Tensor):
+    """keys [T, G * D] and values [T, Gv * V] (f32 or bf16 rows, as they are to be cached: normed, rotated) of the step's tokens go to their pages, quantised to 4 bits"""
+    G, D, Gv, V = _kv4_rows("kv4_store", k, v, kpool, vpool, step)
+    if k.dtype not in _DT:
+        raise ValueError(f"kv4_store: rows are float32 or bfloat16, not {k.dtype}")
+    _on_device("kv4_store", lib().b200seq_kv4_store, (_p(k), k.stride(0), _p(v), v.stride(0), _DT[k.dtype], C.byref(step), G, D, Gv, V, _p(kpool), _p(vpool)),
+               k, v, kpool, vpool)
+
+
+@_timed
+def kv4_load(kpool: torch.Tensor, vpool: torch.Tensor, step: "StepDesc", k: torch.Tensor, v: torch.Tensor):
+    """the rows that the cache holds for the step's tokens, as the values they stand for: k f32 [T, G * D], v f32 [T, Gv * V]"""
+    G, D, Gv, V = _kv4_rows("kv4_load", k, v, kpool, vpool, step)
+    if k.dtype != torch.float32:
+        raise ValueError(f"kv4_load: rows are float32, not {k.dtype}")
+    _on_device("kv4_load", lib().b200seq_kv4_load, (_p(kpool), _p(vpool), C.byref(step), G, D, Gv, V, _p(k), k.stride(0), _p(v), v.stride(0)), k, v, kpool, vpool)
+
+
+def _kv4_layer(name: str, proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: Optional[torch.Tensor], vpool: Optional[torch.Tensor], need: int) -> int:
+    if proj.dim() != 2 or proj.stride(1) != 1 or proj.dtype != torch.float32 or proj.shape[0] < step.T or proj.shape[1] < need:
+        raise ValueError(f"{name}: projection rows are row-major float32 [{step.T}, {need} or more], not {proj.dtype} {tuple(proj.shape)}")
+    if kpool is not None:
+        _kv4_pool_check(name, "key", kpool, step.block_size, d.G, d.D)
+    if vpool is not None:
+        _kv4_pool_check(name, "value", vpool, step.block_size, d.vg if d.vg > 0 else d.G, d.V)
+    return proj.stride(0)
+
+
+@_timed
+def attn_prep_kv4(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: Optional[torch.Tensor], vpool: Optional[torch.Tensor]):
+    """attn_prep_ex over a 4-bit cache: queries biased, normed and rotated in place, keys and values likewise into their pages"""
+    need = max(d.q_col + d.H * d.D, 0 if d.kv_shared else max(d.k_col + d.G * d.D, d.v_col + (d.vg if d.vg > 0 else d.G) * d.V))
+    ld = _kv4_layer("attn_prep_kv4", proj, step, d, kpool, vpool, need)
+    _on_device("attn_prep_kv4", lib().b200seq_attn_prep_kv4, (_p(proj), ld, C.byref(step), C.byref(d), _p(kpool), _p(vpool)), proj, kpool, vpool)
+
+
+@_timed
+def attn_kv4(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: torch.Tensor, vpool: torch.Tensor, out: torch.Tensor, gate: Optional[torch.Tensor] = None):
+    """attn_ex over a 4-bit cache: out [T, H * V] (f32 or bf16) = softmax(q k^T * scale + mask) v, gated as the layer says.  No work area."""
+    own_gate = d.gate_col >= 0 and gate is None and not d.gate
+    need = max(d.q_col + d.H * d.D, d.gate_col + (d.H * d.V if d.gate_elem else d.H) if own_gate else 0)
+    ld = _kv4_layer("attn_kv4", proj, step, d, kpool, vpool, need)
+    if out.dtype not in _DT or not out.is_contiguous() or out.shape[0] < step.T or out[0:1].numel() != d.H * d.V:
+        raise ValueError(f"attn_kv4: results are contiguous float32 or bfloat16 [{step.T}, {d.H * d.V}], not {out.dtype} {tuple(out.shape)}")
+    if gate is not None:
+        if gate.dim() != 2 or gate.stride(1) != 1 or gate.dtype != torch.float32 or gate.shape[0] < step.T or gate.shape[1] < (d.H * d.V if d.gate_elem else d.H):
+            raise ValueError("attn_kv4: gate logits are row-major float32 rows, one for each head (or output element)")
+        d2 = AttnDesc.from_buffer_copy(d)
+        d2.gate, d2.gate_ld = gate.data_ptr(), gate.stride(0)
+        d = d2
+    _on_device("attn_kv4", lib().b200seq_attn_kv4, (_p(proj), ld, C.byref(step), C.byref(d), _p(kpool), _p(vpool), _p(out), _DT[out.dtype]), proj, kpool, vpool, out, gate)
+
+
+# ---- pages ---------------------------------------------------------------------------------------------------------------------------------------------
+@_timed
+def copy_pages(pools: Sequence[torch.Tensor], pairs: Sequence[Tuple[int, int]]):
+    """page `to` of every pool <- its page `from`, for all pairs (from, to) of host numbers, in one launch.  Pools: contiguous, the first dimension counts the
+    pages and is the same in all.  A page may be read by several pairs, but not written twice and not both read and written."""
+    if not len(pools):
+        return
+    pages = pools[0].shape[0]
+    for p in pools:
+        if not p.is_contiguous() or p.dim() < 1 or p.shape[0] != pages:
+            raise ValueError(f"copy_pages: pools are contiguous and of one number of pages, not {tuple(p.shape)} beside {pages}")
+    n, np_ = len(pairs), len(pools)
+    flat = array("i", chain.from_iterable(pairs))
+    if len(flat) != 2 * n:
+        raise ValueError("copy_pages: pairs of (from, to) expected")
+    src, dst = flat[0::2], flat[1::2]
+    ptrs = (C.c_void_p * np_)(*[p.data_ptr() for p in pools])
+    size = (C.c_int64 * np_)(*[p.numel() // pages * p.element_size() if pages else 0 for p in pools])
+    _on_device("copy_pages", lib().b200seq_copy_pages, (ptrs, size, np_, pages, src.buffer_info()[0] if n else None, dst.buffer_info()[0] if n else None, n), *pools)
+
+
+# ---- sampling rules ------------------------------------------------------------------------------------------------------------------------------------
+@_timed
+def process_logits(logits: torch.Tensor, rules: torch.Tensor, out: Optional[torch.Tensor] = None, *, hist: Optional[torch.Tensor] = None, hist_start: Optional[torch.Tensor] = None,
+                   hist_prompt: Optional[torch.Tensor] = None, bias_start: Optional[torch.Tensor] = None, bias_ids: Optional[torch.Tensor] = None,
+                   bias_vals: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out [R, V] f32 (default: `logits` in place): penalties for the tokens of each row's history, biases, temperature and a mask (include/b200seq.h has the order).
+    rules f32 [R, 4]: repetition, presence, frequency, temperature.  hist int32 [total] with hist_start int32 [R + 1] and hist_prompt int32 [R] (how many of a
+    row's ids are its prompt); bias_ids int32, bias_vals f32 with bias_start int32 [R + 1]; mask int32 [R, ceil(V / 32)], bit v % 32 of word v / 32 set: allowed."""
+    out = logits if out is None else out
+    if logits.dim() != 2 or logits.stride(1) != 1 or logits.dtype != torch.float32 or out.dim() != 2 or out.stride(1) != 1 or out.dtype != torch.float32 or out.shape != logits.shape:
+        raise ValueError(f"process_logits: row-major float32 logits and results of one shape, not {logits.dtype} {tuple(logits.shape)} and {out.dtype} {tuple(out.shape)}")
+    R, V = logits.shape
+    ld = lambda t: max(t.stride(0), V) if R == 1 else t.stride(0)
+
+    def vec(name, t, dtype, n):
+        if t is not None and (t.dtype != dtype or not t.is_contiguous() or (n is not None and t.numel() != n)):
+            raise ValueError(f"process_logits: {name} is contiguous {dtype}{'' if n is None else f' of {n} values'}, not {t.dtype} {tuple(t.shape)}")
+    vec("rules", rules, torch.float32, 4 * R)
+    vec("hist", hist, torch.int32, None)
+    vec("hist_start", hist_start, torch.int32, R + 1)
+    vec("hist_prompt", hist_prompt, torch.int32, R)
+    vec("bias_start", bias_start, torch.int32, R + 1)
+    vec("bias_ids", bias_ids, torch.int32, None)
+    vec("bias_vals", bias_vals, torch.float32, bias_ids.numel() if bias_ids is not None else None)
+    if mask is not None and (mask.dim() != 2 or mask.dtype != torch.int32 or mask.stride(1) != 1 or mask.shape[0] != R or mask.shape[1] < (V + 31) // 32):
+        raise ValueError(f"process_logits: the mask is row-major int32 [{R}, {(V + 31) // 32}], not {mask.dtype} {tuple(mask.shape)}")
+    if hist is not None and hist.numel() == 0:      # histories without a token
+        hist = hist_start = hist_prompt = None
+    if bias_ids is not None and bias_ids.numel() == 0:
+        bias_ids = bias_start = bias_vals = None
+    words = (V + 31) // 32
+    _on_device("process_logits", lib().b200seq_process_logits,
+               (_p(logits), ld(logits), R, V, _p(rules), _p(hist), _p(hist_start), _p(hist_prompt), _p(bias_start), _p(bias_ids), _p(bias_vals),
+                _p(mask), max(mask.stride(0), words) if mask is not None else 0, _p(out), ld(out)), logits, rules, out, hist, hist_start, hist_prompt, bias_start, bias_ids, bias_vals, mask)
+    return out

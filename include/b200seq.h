@@ -10,7 +10,7 @@
  * linear recurrences, PolyNorm, soft-max routing with identity experts, a hashed bigram embedding,
  * the delta rule with per-channel decays, layers normed on both sides with sinusoidal positions and a
  * token-dependent addition, the selective scan with a decay per channel and state, the residual of parallel
- * layers, arg-max sampling.
+ * layers, a KV cache held in 4 bits and its attention, page copies, sampling rules on logits, arg-max sampling.
  *
  * It sits beside libb200q (include/b200q.h), which holds the quantized linear layer; the conventions are
  * the same:
@@ -72,7 +72,8 @@ typedef struct b200seq_step {
 const char* b200seq_last_error(void);
 int b200seq_version(void);
 int64_t b200seq_launch_count(void);
-/* bit 0: a KV position fell outside its block table; bit 1: a bounded wait of the tensor-core GEMM ran out; bit 2: an expert table entry outside the experts */
+/* bit 0: a KV position fell outside its block table; bit 1: a bounded wait of the tensor-core GEMM ran out; bit 2: an expert table entry outside the experts;
+ * bit 3: a value beyond what a 4-bit cache holds; bit 4: a token id outside the vocabulary */
 int b200seq_error_flags(int* flags_out);
 
 /* X[t][s][:] = table[ids[t]][:] * scale for every stream s.  table: bf16 [V, W]; X: f32 [T, S, W]. */
@@ -488,6 +489,40 @@ typedef struct b200seq_parallel_desc {
     const float* fin_w;
 } b200seq_parallel_desc;
 int b200seq_parallel_close(const b200seq_parallel_desc* d, void* stream);
+
+/* ---- a KV cache held in 4 bits ---------------------------------------------------------------------------------------------------------------------------
+ * Pools of pages [blocks][heads][segment] bytes with b200seq_kv4_page_bytes(block_size, heads, D) bytes a page (0: sizes it does not hold; D <= 128), starting on a
+ * 16-byte boundary.  32 neighbouring values of a row (a position, a head) have a minimum m and a step s, both f16, and a 4-bit code each, which stands for m + s * code:
+ *   m = f16(min x);  s = (max x - m) / 15, rounded up to 7 significant bits and to a multiple of 2^-24;  code = clamp(rint((x - m) * (1 / s)), 0, 15)
+ * in f32 (1 / 15 as the f32 number below it).  Values beyond +-32000 are held as +-32000, NaN as 0; either raises bit 3 of the error flags.
+ * A segment is cut into units of 16 rows (block_size % 16 == 0; else one unit of block_size rows); with NG = 1, 2 or 4 groups a row (D <= 32, 64, 128) a unit holds its
+ * rows' codes (16 NG bytes each), then its rows' (s, m) pairs (4 NG bytes each).  A key row's codes are 32-bit words [part c < 4][group] of the eight values
+ * 32 group + 8 c + i, a value row's 16-bit words [part r < 8][group] of the four values 32 group + 4 r + i, the first value in the lowest bits; places behind D are 0.
+ * store: k [T, G * D], v [T, Gv * V] (f32 or bf16, row strides ldk, ldv) go to the pages of the step's tokens.
+ * load:  the same rows back in f32, as what they stand for (rows behind another owner's page or of no page are left as they are).
+ * attn_prep_kv4 is b200seq_attn_prep_ex, attn_kv4 is b200seq_attn_ex, over such pools (no pooled blocks, no latents; D, V <= 128): q and sums in 32 bits, the cache's
+ * values as they are held.  A query that is not finite gives a row of NaN.  No work area. */
+int64_t b200seq_kv4_page_bytes(int block_size, int G, int D);
+int b200seq_kv4_store(const void* k, int64_t ldk, const void* v, int64_t ldv, int in_dtype, const b200seq_step* st, int G, int D, int Gv, int V, void* kpool, void* vpool,
+                      void* stream);
+int b200seq_kv4_load(const void* kpool, const void* vpool, const b200seq_step* st, int G, int D, int Gv, int V, float* k, int64_t ldk, float* v, int64_t ldv, void* stream);
+int b200seq_attn_prep_kv4(float* proj, int64_t ld, const b200seq_step* st, const b200seq_attn_desc* d, void* kpool, void* vpool, void* stream);
+int b200seq_attn_kv4(const float* proj, int64_t ld, const b200seq_step* st, const b200seq_attn_desc* d, const void* kpool, const void* vpool, void* out, int out_dtype,
+                     void* stream);
+
+/* Page to[i] of every pool becomes a copy of its page from[i], i < n.  pools, page_bytes, from, to: HOST arrays, read during the call; every pool has `pages` pages.
+ * A page may be read by several pairs, but not written twice and not both read and written (B200SEQ_ERR_INVALID_ARG, nothing is copied). */
+int b200seq_copy_pages(void* const* pools, const int64_t* page_bytes, int npools, int pages, const int32_t* from, const int32_t* to, int n, void* stream);
+
+/* Sampling rules on rows of logits, out[r] from x[r] (f32 [R, V], out may be x), rules[r] = (repetition, presence, frequency, temperature), 16-byte aligned, in this order:
+ *   a token of the row's history (hist[hist_start[r] .. hist_start[r + 1])): x > 0 ? x / repetition : x * repetition
+ *   a token that stands n > 0 times behind the first hist_prompt[r] of them: x - n * frequency - presence
+ *   x + bias for the tokens of bias_ids[bias_start[r] .. bias_start[r + 1]) (a token named twice has the last one's)
+ *   x / temperature (0: as it is);   -inf where bit v % 32 of mask[r][v / 32] is 0
+ * History, biases and mask are each optional (null).  An id outside the vocabulary is passed over and raises bit 4 of the error flags. */
+int b200seq_process_logits(const float* x, int64_t ldx, int R, int V, const float* rules, const int32_t* hist, const int32_t* hist_start, const int32_t* hist_prompt,
+                           const int32_t* bias_start, const int32_t* bias_ids, const float* bias_vals, const uint32_t* mask, int64_t mask_ld, float* out, int64_t ldo,
+                           void* stream);
 
 /* ids[r] = argmax_v logits[r][v] (first maximum) */
 int b200seq_argmax(const float* logits, int R, int V, int32_t* ids, void* stream);
