@@ -19,6 +19,8 @@ struct Attn4Args {
     float softcap;
     void* out;                 // [T, H * V]
     int out_dtype;
+    int cluster, parts;        // CTAs of a cluster that share a row tile's keys, and clusters that do
+    float* part;               // [T][H][parts][V + 4] when parts > 1: maximum (base 2), sum, two unused, values
     int* err;
 };
 

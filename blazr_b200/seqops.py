@@ -47,7 +47,7 @@ EXPORTS = ["b200seq_last_error", "b200seq_version", "b200seq_launch_count", "b20
            "b200seq_diff_combine", "b200seq_min_gru", "b200seq_rg_lru", "b200seq_delta", "b200seq_delta_scratch_floats", "b200seq_embed_pos", "b200seq_sandwich_norm",
            "b200seq_token_gate", "b200seq_side_close", "b200seq_linear_silu", "b200seq_moe_route_rule", "b200seq_moe_router_rule", "b200seq_retention_partials",
            "b200seq_selective_scan", "b200seq_scan_scratch_floats", "b200seq_parallel_close", "b200seq_kv4_page_bytes", "b200seq_kv4_store", "b200seq_kv4_load",
-           "b200seq_attn_prep_kv4", "b200seq_attn_kv4", "b200seq_copy_pages", "b200seq_process_logits"]
+           "b200seq_attn_prep_kv4", "b200seq_attn_kv4", "b200seq_attn_kv4_scratch_floats", "b200seq_copy_pages", "b200seq_process_logits"]
 
 # argument types of the operators' C entries (include/b200seq.h): p pointer, i int, l int64, z size_t, f float.  Declared, plain numbers are converted by ctypes
 # as they are passed; an object made for each of them and a stream object looked up for each call took half of a call's 4 - 8 us.
@@ -65,7 +65,7 @@ SIGNATURES = {
     "polynorm": "pliipfpilp", "softcap": "plfp", "diff_combine": "piiiifffpip", "min_gru": "pliiipppipip", "rg_lru": "plplppfplipppiipip", "delta": "plppplppipzp",
     "embed_pos": "pppfpippppfpip", "sandwich_norm": "pppfppipippipp", "token_gate": "pliiplippip", "side_close": "pppfpppliippppipippipp",
     "selective_scan": "piplpplppppipzp", "parallel_close": "pp", "argmax": "piipp", "kv4_page_bytes": "iii", "kv4_store": "plplipiiiippp", "kv4_load": "pppiiiiplplp",
-    "attn_prep_kv4": "plppppp", "attn_kv4": "plpppppip", "copy_pages": "ppiippip", "process_logits": "pliipppppppplplp"
+    "attn_prep_kv4": "plppppp", "attn_kv4": "plpppppipzp", "attn_kv4_scratch_floats": "pp", "copy_pages": "ppiippip", "process_logits": "pliipppppppplplp"
 }
 
 
@@ -207,6 +207,7 @@ def lib() -> C.CDLL:
         L.b200seq_last_error.restype = C.c_char_p
         L.b200seq_launch_count.restype = C.c_int64
         L.b200seq_kv4_page_bytes.restype = C.c_int64
+        L.b200seq_attn_kv4_scratch_floats.restype = C.c_size_t
         for name, args in SIGNATURES.items():
             getattr(L, "b200seq_" + name).argtypes = [_ARG[a] for a in args]
         _lib = L
@@ -946,7 +947,8 @@ def attn_prep_kv4(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: Op
 
 @_timed
 def attn_kv4(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: torch.Tensor, vpool: torch.Tensor, out: torch.Tensor, gate: Optional[torch.Tensor] = None):
-    """attn_ex over a 4-bit cache: out [T, H * V] (f32 or bf16) = softmax(q k^T * scale + mask) v, gated as the layer says.  No work area."""
+    """attn_ex over a 4-bit cache: out [T, H * V] (f32 or bf16) = softmax(q k^T * scale + mask) v, gated as the layer says.
+    (The work area of few long sequences is the call's own: no two calls, streams or graphs share it.)"""
     own_gate = d.gate_col >= 0 and gate is None and not d.gate
     need = max(d.q_col + d.H * d.D, d.gate_col + (d.H * d.V if d.gate_elem else d.H) if own_gate else 0)
     ld = _kv4_layer("attn_kv4", proj, step, d, kpool, vpool, need)
@@ -958,7 +960,10 @@ def attn_kv4(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: torch.T
         d2 = AttnDesc.from_buffer_copy(d)
         d2.gate, d2.gate_ld = gate.data_ptr(), gate.stride(0)
         d = d2
-    _on_device("attn_kv4", lib().b200seq_attn_kv4, (_p(proj), ld, C.byref(step), C.byref(d), _p(kpool), _p(vpool), _p(out), _DT[out.dtype]), proj, kpool, vpool, out, gate)
+    sref, dref = C.byref(step), C.byref(d)
+    need = lib().b200seq_attn_kv4_scratch_floats(sref, dref)
+    scratch = torch.empty(need, dtype=torch.float32, device=proj.device) if need else None
+    _on_device("attn_kv4", lib().b200seq_attn_kv4, (_p(proj), ld, sref, dref, _p(kpool), _p(vpool), _p(out), _DT[out.dtype], _p(scratch), need), proj, kpool, vpool, out, gate)
 
 
 # ---- pages ---------------------------------------------------------------------------------------------------------------------------------------------
