@@ -50,13 +50,19 @@ __device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t
     const __half2 l = __floats2half2_rn(a - f.x, b - f.y);
     hi = *reinterpret_cast<const uint32_t*>(&h), lo = *reinterpret_cast<const uint32_t*>(&l);
 }
-__device__ __forceinline__ float par_s(uint32_t p) { return __half2float(__ushort_as_half((uint16_t)p)); }
-// two codes (fields at bits 0 and 16, high: at 4 and 20) and their steps -> s (u - 8), exactly: 0x6400 | u is 1024 + u, with a field of 16 u divided out
-__device__ __forceinline__ uint32_t centred(uint32_t x, uint32_t s, bool high) {
-    const uint32_t w = (x & (high ? 0x00F000F0u : 0x000F000Fu)) | 0x64006400u;
-    const __half2 h = *reinterpret_cast<const __half2*>(&w);
-    const __half2 u = high ? __hfma2(h, __floats2half2_rn(0.0625f, 0.0625f), __floats2half2_rn(-72.f, -72.f)) : __hadd2_rn(h, __floats2half2_rn(-1032.f, -1032.f));
-    const __half2 d = __hmul2_rn(u, *reinterpret_cast<const __half2*>(&s));
+__device__ __forceinline__ float par_s(uint32_t p) { return __low2float(*reinterpret_cast<const __half2*>(&p)); }
+// Two codes (fields at bits 0 and 16, high: at 4 and 20), their steps s and s72 = -72 s -> s (u - 8), exactly.  A high field in the mantissa of 64 is 64 + u: one
+// multiply-add, since -72 s is an f16 number too (7 + 4 bits).  A low one makes 1024 + u, whose -1032 s is none: the offset goes first.
+__device__ __forceinline__ uint32_t centred(uint32_t x, uint32_t s_, uint32_t s72, uint32_t magic, bool high) {
+    uint32_t w;
+    if (high) asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;" : "=r"(w) : "r"(x), "r"(magic));      // (x & mask) | magic
+    else asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(w) : "r"(x), "r"(magic));
+    const __half2 h = *reinterpret_cast<const __half2*>(&w), s = *reinterpret_cast<const __half2*>(&s_);
+    const __half2 d = high ? __hfma2(h, s, *reinterpret_cast<const __half2*>(&s72)) : __hmul2_rn(__hadd2_rn(h, __floats2half2_rn(-1032.f, -1032.f)), s);
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
+__device__ __forceinline__ uint32_t times72(uint32_t s_) {
+    const __half2 d = __hmul2_rn(*reinterpret_cast<const __half2*>(&s_), __floats2half2_rn(-72.f, -72.f));
     return *reinterpret_cast<const uint32_t*>(&d);
 }
 
@@ -84,22 +90,27 @@ __device__ __forceinline__ uint32_t lds16(uint32_t at) {
     return x;
 }
 
-// half a tile, the 16 keys from key0 on, into shared memory: codes (swizzled), then parameters.  Keys behind `hi` are read from hi's row, or, in whole units, from the
-// rest of its page.
-template <int NG, bool UNITS>
-__device__ __forceinline__ void fetch(uint32_t dst, const uint8_t* pool, const int32_t* bt, int bs, int key0, int hi, int g, int G, int lane) {
-    if (UNITS) {
-        const int pg = key0 / bs;
-        const uint8_t* src = pool + ((int64_t)bt[pg] * G + g) * (int64_t)(bs * NG * 20) + (key0 - pg * bs) * (NG * 20);
+// Half a tile, the 16 keys of a whole unit, into shared memory: codes (swizzled), then parameters, of keys and of values.  k, v: this lane's first piece of codes;
+// par: its piece of either's parameters.  dst: the half; piece: 16 * swz(lane); par_at: where the parameters' piece goes.
+template <int NK, int NV>
+__device__ __forceinline__ void fetch_unit(uint32_t dst, uint32_t piece, uint32_t par_at, const uint8_t* k, const uint8_t* v, const uint8_t* par, int lane) {
+    constexpr int KB = NK * 320;
 #pragma unroll
-        for (int i = lane; i < NG * 20; i += 32) copy16(dst + 16 * (i < NG * 16 ? swz(i) : i), src + 16 * i);
-    } else {
-        for (int i = lane; i < 16 * NG * 5; i += 32) {
-            const int row = i / (NG * 5), w = i - row * (NG * 5), key = min(key0 + row, hi), pg = key / bs;
-            const Kv4Row at = kv4_row(bt[pg], key - pg * bs, bs, g, G, NG);
-            if (w < NG * 4) copy4(dst + 16 * swz(row * NG + (w >> 2)) + 4 * (w & 3), pool + at.codes + 4 * w);
-            else copy4(dst + NG * 256 + row * NG * 4 + 4 * (w - NG * 4), pool + at.params + 4 * (w - NG * 4));
-        }
+    for (int n = 0; n < (NK + 1) / 2; ++n)      // (piece lane + 32 n: the same swizzle)
+        if (NK > 1 || lane < 16) copy16(dst + piece + 512 * n, k + 512 * n);
+#pragma unroll
+    for (int n = 0; n < (NV + 1) / 2; ++n)
+        if (NV > 1 || lane < 16) copy16(dst + KB + piece + 512 * n, v + 512 * n);
+    if (NK + NV == 8 || lane < 4 * (NK + NV)) copy16(dst + par_at, par);
+}
+// the 16 keys from key0 on of one pool, from pages that a half may cross; keys behind `hi` are read from hi's row
+template <int NG>
+__device__ __forceinline__ void fetch_rows(uint32_t dst, const uint8_t* pool, const int32_t* bt, int bs, int key0, int hi, int g, int G, int lane) {
+    for (int i = lane; i < 16 * NG * 5; i += 32) {
+        const int row = i / (NG * 5), w = i - row * (NG * 5), key = min(key0 + row, hi), pg = key / bs;
+        const Kv4Row at = kv4_row(bt[pg], key - pg * bs, bs, g, G, NG);
+        if (w < NG * 4) copy4(dst + 16 * swz(row * NG + (w >> 2)) + 4 * (w & 3), pool + at.codes + 4 * w);
+        else copy4(dst + NG * 256 + row * NG * 4 + 4 * (w - NG * 4), pool + at.params + 4 * (w - NG * 4));
     }
 }
 
@@ -129,7 +140,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
     chain_enter();
     extern __shared__ __align__(16) uint8_t smem[];
     constexpr int KB = NK * 320, HALF = (NK + NV) * 320, STAGE = 2 * HALF, MV = 32 * NV + 4;
-    __shared__ __align__(16) uint4 qfrag[NK * 2 * 32];
+    __shared__ __align__(16) uint4 qfrag[(NK * 2 + 1) * 32];
+    __shared__ float factor_sm[WARPS * ROWS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     const int D = a.D, V = a.V, R = a.H / a.G, bs = st.block_size, rank = blockIdx.z;
     const int tile_no = blockIdx.x / a.parts, seg = blockIdx.x - tile_no * a.parts;
@@ -145,41 +157,72 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
     }
     const KeySpan<KT> span(a, p0, hi);
     const int lo_last = RowSpan(a, hi).lo;
-    // ---- keys into the ring ----
+    // ---- keys into the ring: tiles me, me + walkers, ...; the first key and the pages of a tile are looked up a tile ahead of its copies ----
     const uint32_t ring = tcpair::sa(smem) + warp * (STAGES * STAGE);
     const int walkers = a.parts * a.cluster * WARPS, me = (seg * a.cluster + rank) * WARPS + warp;
     const int nt = span.total > me ? (span.total - me + walkers - 1) / walkers : 0;
-    auto issue = [&](int i) {
+    const int upp = bs >> 4, Gv = a.G / a.vdiv;                                  // units of a page
+    const uint32_t kpage = (uint32_t)(a.G * upp * (NK * 320)), vpage = (uint32_t)(Gv * upp * (NV * 320));   // (below 2^31: checked by the caller)
+    const bool kpar = lane < 4 * NK;
+    const uint8_t *kg = a.kpool + (int64_t)g * upp * (NK * 320), *vg = a.vpool + (int64_t)(g / a.vdiv) * upp * (NV * 320);
+    const uint8_t* pg = kpar ? kg + NK * 256 + 16 * lane : vg + NV * 256 + 16 * (lane - 4 * NK);
+    kg += 16 * lane, vg += 16 * lane;
+    const uint32_t ppage = kpar ? kpage : vpage, piece = 16 * swz(lane), par_at = kpar ? NK * 256 + 16 * lane : KB + NV * 256 + 16 * (lane - 4 * NK);
+    int key_n = span.key0(me), page0 = 0, page1 = 0;
+    auto lookup = [&]() {
+        if (!UNITS || key_n > hi) return;
+        const int unit = key_n >> 4;
+        page0 = bt[upp == 1 ? unit : unit / upp];
+        if (key_n + 16 <= hi) page1 = bt[upp == 1 ? unit + 1 : (unit + 1) / upp];
+    };
+    auto issue = [&](int i) {      // the i-th tile of this warp, whose first key and pages have been looked up; then the next one's
         if (i < nt) {
-            const int key0 = span.key0(me + i * walkers);
             const uint32_t dst = ring + (i & 1) * STAGE;
+            if (UNITS) {
+                const int unit = key_n >> 4;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (key0 + 16 * s > hi) break;
-                fetch<NK, UNITS>(dst + s * HALF, a.kpool, bt, bs, key0 + 16 * s, hi, g, a.G, lane);
-                fetch<NV, UNITS>(dst + s * HALF + KB, a.vpool, bt, bs, key0 + 16 * s, hi, g / a.vdiv, a.G / a.vdiv, lane);
+                for (int s = 0; s < 2; ++s) {
+                    if (key_n + 16 * s > hi) break;
+                    const uint32_t page = (uint32_t)(s ? page1 : page0);
+                    const uint8_t *k = kg + (uint64_t)page * kpage, *v = vg + (uint64_t)page * vpage, *par = pg + (uint64_t)page * ppage;
+                    if (upp != 1) {
+                        const int u = (unit + s) % upp;
+                        k += u * (NK * 320), v += u * (NV * 320), par += u * (kpar ? NK * 320 : NV * 320);
+                    }
+                    fetch_unit<NK, NV>(dst + s * HALF, piece, par_at, k, v, par, lane);
+                }
+            } else {
+                for (int s = 0; s < 2 && key_n + 16 * s <= hi; ++s) {
+                    fetch_rows<NK>(dst + s * HALF, a.kpool, bt, bs, key_n + 16 * s, hi, g, a.G, lane);
+                    fetch_rows<NV>(dst + s * HALF + KB, a.vpool, bt, bs, key_n + 16 * s, hi, g / a.vdiv, Gv, lane);
+                }
             }
+            if (i + 1 < nt) key_n = span.key0(me + (i + 1) * walkers), lookup();
         }
         copies_commit();
     };
+    lookup();
+    int key0 = key_n;
     issue(0);
-    // ---- this thread's row: q as A fragments (eight neighbouring values of every group), its factor and what it sees ----
+    // ---- the rows: q as A fragments (eight neighbouring values of every group a thread), their factors and their parts against (s, m); by the first warp ----
     const int tq = r / a.Rb, hr = r - tq * a.Rb;
     const bool live = tq < nq && hr < nh;
     const RowSpan rs(a, p0 + (live ? tq : 0));
-    float zf;
-    uint32_t qm[4] = {0u, 0u, 0u, 0u};
-    {
+    if (warp == 0) {
         const float* src = a.q + (int64_t)(t0 + tq) * a.ld + (int64_t)(h0 + hr) * D;
         float x[NK][8], mx = 0.f;
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
+            const int d = 32 * k + 8 * c;
+            if (a.vec && d < D) {       // (D a multiple of 8: eight values or none)
+                const float4 u = live ? ld4(src + d) : make_float4(0.f, 0.f, 0.f, 0.f), v = live ? ld4(src + d + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+                x[k][0] = u.x, x[k][1] = u.y, x[k][2] = u.z, x[k][3] = u.w, x[k][4] = v.x, x[k][5] = v.y, x[k][6] = v.z, x[k][7] = v.w;
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int d = 32 * k + 8 * c + i;
-                x[k][i] = live && d < D ? src[d] : 0.f;
-                mx = fmaxf(mx, fabsf(x[k][i]));
+                for (int i = 0; i < 8; ++i) x[k][i] = live && d + i < D ? src[d + i] : 0.f;
             }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[k][i]));
         }
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1)), mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         // times a power of two that puts the largest into [2^4, 2^5); a row of zeros, denormals or infinities as it is
@@ -197,20 +240,31 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
             for (int i = 0; i < 8; ++i) x[k][i] *= up, sum += x[k][i];
             sum += __shfl_xor_sync(0xffffffffu, sum, 1), sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             mine = k == c ? sum : mine;
-            if (warp == 0) {
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {   // fields 0 and 4 (2 and 6) of a word, then 1 and 5 (3 and 7), which stand four bits higher
-                    uint4 f;
-                    split16(x[k][2 * s], x[k][2 * s + 4], f.x, f.y);
-                    split16(x[k][2 * s + 1] * 0.0625f, x[k][2 * s + 5] * 0.0625f, f.z, f.w);
-                    qfrag[(k * 2 + s) * 32 + lane] = f;
-                }
+            for (int s = 0; s < 2; ++s) {   // fields 0 and 4 (2 and 6) of a word, then 1 and 5 (3 and 7), which stand four bits higher
+                uint4 f;
+                split16(x[k][2 * s], x[k][2 * s + 4], f.x, f.y);
+                split16(x[k][2 * s + 1] * 0.0625f, x[k][2 * s + 5] * 0.0625f, f.z, f.w);
+                qfrag[(k * 2 + s) * 32 + lane] = f;
             }
         }
-        split16(0.f, mine, qm[0], qm[1]);   // against (s, m) of group c
-        zf = fmaxf(fabsf(factor) * (a.softcap > 0.f ? 1.f : LOG2E) * down, 1e-37f);
+        uint4 f;
+        split16(0.f, mine, f.x, f.y);   // against (s, m) of group c
+        f.z = __float_as_uint(fmaxf(fabsf(factor) * (a.softcap > 0.f ? 1.f : LOG2E) * down, 1e-37f)), f.w = 0;
+        qfrag[NK * 64 + lane] = f;
     }
+    // where this thread's pieces lie in a half: key words of rows r and r + 8, value words and parameters of keys 2c, 2c + 1, 8 + 2c, 9 + 2c
+    uint32_t ko = NK == 4 ? 16 * swz(r * 4 + c) : (NK == 2 ? 16 * swz(r * 2 + (c >> 1)) + 8 * (c & 1) : 16 * swz(r) + 4 * c), ko8 = NK == 4 ? ko + 512 : (NK == 2 ? 16 * swz((r + 8) * 2 + (c >> 1)) + 8 * (c & 1) : 16 * swz(r + 8) + 4 * c);
+    uint32_t vo[4], magic64 = 0x54005400u, magic1024 = 0x64006400u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int row = 2 * c + (j & 1) + 8 * (j >> 1);
+        vo[j] = KB + (NV == 4 ? 16 * swz(row * 4 + (r >> 1)) + 8 * (r & 1) : (NV == 2 ? 16 * swz(row * 2 + (r >> 2)) + 4 * (r & 3) : 16 * swz(row) + 2 * r));
+    }
+    asm volatile("" : "+r"(ko), "+r"(ko8), "+r"(vo[0]), "+r"(vo[1]), "+r"(vo[2]), "+r"(vo[3]), "+r"(magic64), "+r"(magic1024));   // (kept, not made again for every tile)
     __syncthreads();
+    const uint2 qm = *reinterpret_cast<const uint2*>(&qfrag[NK * 64 + lane]);
+    const float zf = __uint_as_float(qfrag[NK * 64 + lane].z);
     float mx = -INFINITY, l = 0.f;
     uint64_t o[NV * 4], os = 0;
 #pragma unroll
@@ -220,11 +274,11 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
 
 #pragma unroll 1
     for (int i = 0; i < nt; ++i) {
+        const int key_after = key_n;      // (of the tile that is issued now)
         issue(i + 1);
         copies_wait<1>();
         __syncwarp();
         const uint32_t at = ring + (i & 1) * STAGE;
-        const int key0 = span.key0(me + i * walkers);
         // ---- scores of keys key0 + 16 s + 8 n + {2c, 2c + 1}: z[4 s + 2 n + {0, 1}] ----
         float z[8];
 #pragma unroll
@@ -232,11 +286,9 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
             const uint32_t ks = at + s * HALF;
             uint64_t zc[2] = {0, 0};
             uint32_t kw[2][NK], kp[4][NK];
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const int row = r + 8 * n;
-                lds<NK>(ks + (NK == 4 ? 16 * swz(row * 4 + c) : (NK == 2 ? 16 * swz(row * 2 + (c >> 1)) + 8 * (c & 1) : 16 * swz(row) + 4 * c)), kw[n]);
-            }
+            lds<NK>(ks + ko, kw[0]);
+            if (NK == 4) lds<NK>(ks + ko + 512, kw[1]);
+            else lds<NK>(ks + ko8, kw[1]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) lds<NK>(ks + NK * 256 + (2 * c + (j & 1) + 8 * (j >> 1)) * NK * 4, kp[j]);
 #pragma unroll
@@ -256,7 +308,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
                 uint32_t b[1] = {0};
                 if (c < NK) lds<1>(ks + NK * 256 + ((r + 8 * n) * NK + c) * 4, b);
                 float acc[4];
-                mma16816(acc, make_uint4(qm[0], qm[1], 0u, 0u), b[0], 0u, none);
+                mma16816(acc, make_uint4(qm.x, qm.y, 0u, 0u), b[0], 0u, none);
                 tcsplit::upk(tcsplit::fma2(zc[n], up24, tcsplit::add2(tcsplit::pk(acc[0], acc[1]), tcsplit::pk(acc[2], acc[3]))), z[4 * s + 2 * n], z[4 * s + 2 * n + 1]);
             }
         }
@@ -299,9 +351,9 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
                 uint32_t w1[1] = {0};
                 if (r < 2 * NV) lds<1>(vs + NV * 256 + (row * NV + (r >> 1)) * 4, w1);
                 hw[j] = w1[0];
-                if (NV == 4) lds<(NV + 1) / 2>(vs + 16 * swz(row * 4 + (r >> 1)) + 8 * (r & 1), vw[s][j]);
-                else if (NV == 2) lds<(NV + 1) / 2>(vs + 16 * swz(row * 2 + (r >> 2)) + 4 * (r & 3), vw[s][j]);
-                else vw[s][j][0] = lds16(vs + 16 * swz(row) + 2 * r);
+                if (NV == 4) lds<(NV + 1) / 2>(at + s * HALF + vo[j & 1] + 512 * (j >> 1), vw[s][j]);
+                else if (NV == 2) lds<(NV + 1) / 2>(at + s * HALF + vo[j], vw[s][j]);
+                else vw[s][j][0] = lds16(at + s * HALF + vo[j]);
             }
             if (key0 + 16 * s + 15 > hi) {   // whatever lies behind the last key
 #pragma unroll
@@ -328,24 +380,25 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int sel = (k & 1) ? 0x7632 : 0x5410;
-            uint32_t x[2][2];
+            uint32_t x[2][2], s72[2][2];
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int n = 0; n < 2; ++n) x[s][n] = __byte_perm(vw[s][2 * n][k >> 1], vw[s][2 * n + 1][k >> 1], sel);
+                for (int n = 0; n < 2; ++n) x[s][n] = __byte_perm(vw[s][2 * n][k >> 1], vw[s][2 * n + 1][k >> 1], sel), s72[s][n] = times72(sp[s][n][k]);
 #pragma unroll
             for (int i4 = 0; i4 < 4; ++i4) {
                 uint32_t b[2][2];
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) b[s][n] = centred(i4 < 2 ? x[s][n] : x[s][n] >> 8, sp[s][n][k], i4 & 1);
+                    for (int n = 0; n < 2; ++n) b[s][n] = centred(i4 < 2 ? x[s][n] : x[s][n] >> 8, sp[s][n][k], s72[s][n], (i4 & 1) ? magic64 : magic1024, i4 & 1);
                 float acc[4];
                 mma16816(acc, pa[0], b[0][0], b[0][1], none);
                 mma16816(acc, pa[1], b[1][0], b[1][1], acc);
                 o[4 * k + i4] = tcsplit::add2(o[4 * k + i4], tcsplit::add2(tcsplit::pk(acc[0], acc[1]), tcsplit::pk(acc[2], acc[3])));
             }
         }
+        key0 = key_after;
         __syncwarp();   // the stage is refilled next
     }
     copies_wait<0>();
@@ -370,53 +423,72 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
     }
     __syncthreads();
     const int rows = nq * nh, cluster = a.cluster;
-    // what several places hold for one row and column, at(w) the w-th one's (maximum, sum, value)
-    auto merge = [](int n, auto&& at, float& M, float& L, float& acc) {
-        M = -INFINITY, L = acc = 0.f;
-        for (int w = 0; w < n; ++w) M = fmaxf(M, at(w, 0));
-        for (int w = 0; w < n; ++w) {
-            const float lw = at(w, 1);
-            if (lw == 0.f) continue;          // no key that the row sees
-            const float f = tcsplit::ex2(at(w, 0) - M);
-            L = fmaf(lw, f, L), acc = fmaf(at(w, 2), f, acc);
+    // every row's maximum and sum over the warps, and the factor of each warp's values
+    float M = -INFINITY, L = 0.f;
+    if (threadIdx.x < WARPS * ROWS) {
+        const int m = threadIdx.x & (ROWS - 1), w = threadIdx.x / ROWS;
+        for (int i = 0; i < WARPS; ++i) M = fmaxf(M, all[(i * ROWS + m) * MV]);
+        for (int i = 0; i < WARPS; ++i) {
+            const float li = all[(i * ROWS + m) * MV + 1], f = li == 0.f ? 0.f : tcsplit::ex2(all[(i * ROWS + m) * MV] - M);   // (0: no key that the row sees)
+            L = fmaf(li, f, L);
+            if (i == w) factor_sm[w * ROWS + m] = f;
         }
-    };
-    if (cluster == 1 && a.parts == 1) {
+    }
+    __syncthreads();
+    if (threadIdx.x < ROWS) all[threadIdx.x * MV] = M, all[threadIdx.x * MV + 1] = L;     // (the first warp's place)
+    if (cluster > 1 || a.parts > 1) {
+        for (int i = threadIdx.x; i < ROWS * V; i += WARPS * 32) {
+            const int m = i / V, col = i - m * V;
+            float acc = 0.f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) acc = fmaf(all[(w * ROWS + m) * MV + 4 + col], factor_sm[w * ROWS + m], acc);
+            all[m * MV + 4 + col] = acc;
+        }
+        if (cluster > 1) tcpair::cluster_sync();
+    }
+    if (cluster == 1) {
+        __syncthreads();
         for (int i = threadIdx.x; i < rows * V; i += WARPS * 32) {
-            const int m = i / V, col = i - m * V, tq_ = m / nh, hr_ = m - tq_ * nh;
-            const float* pr = all + (tq_ * a.Rb + hr_) * MV;
-            float M, L, acc;
-            merge(WARPS, [&](int w, int what) { return pr[w * (ROWS * MV) + (what < 2 ? what : 4 + col)]; }, M, L, acc);
-            finish(a, t0 + tq_, h0 + hr_, col, M, L, acc);
+            const int m = i / V, col = i - m * V, tq_ = m / nh, hr_ = m - tq_ * nh, row = tq_ * a.Rb + hr_, t = t0 + tq_, h = h0 + hr_;
+            float acc = 0.f;
+            if (a.parts == 1) {
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) acc = fmaf(all[(w * ROWS + row) * MV + 4 + col], factor_sm[w * ROWS + row], acc);
+                finish(a, t, h, col, all[row * MV], all[row * MV + 1], acc);
+            } else {
+                float* pp = a.part + (((int64_t)t * a.H + h) * a.parts + seg) * (V + 4);
+                if (col == 0) pp[0] = all[row * MV], pp[1] = all[row * MV + 1];
+                pp[4 + col] = all[row * MV + 4 + col];
+            }
         }
         return;
     }
-    float* cta = all + WARPS * ROWS * MV;     // [row][maximum, sum, -, -, values]
-    for (int i = threadIdx.x; i < ROWS * V; i += WARPS * 32) {
-        const int m = i / V, col = i - m * V;
-        const float* pr = all + m * MV;
-        float M, L, acc;
-        merge(WARPS, [&](int w, int what) { return pr[w * (ROWS * MV) + (what < 2 ? what : 4 + col)]; }, M, L, acc);
-        if (col == 0) cta[m * MV] = M, cta[m * MV + 1] = L;
-        cta[m * MV + 4 + col] = acc;
-    }
-    if (cluster > 1) tcpair::cluster_sync();
-    else __syncthreads();
-    const uint32_t base = tcpair::sa(cta);
+    // and over the CTAs of the cluster, each of which has a share of the results
+    const uint32_t base = tcpair::sa(all);
     for (int i = rank * (WARPS * 32) + threadIdx.x; i < rows * V; i += cluster * (WARPS * 32)) {
         const int m = i / V, col = i - m * V, tq_ = m / nh, hr_ = m - tq_ * nh, t = t0 + tq_, h = h0 + hr_;
         const uint32_t pr = base + (tq_ * a.Rb + hr_) * MV * 4;
-        float M, L, acc;
-        merge(cluster, [&](int w, int what) { return ld_cluster(pr + 4 * (what < 2 ? what : 4 + col), w); }, M, L, acc);
+        float mw[8], lw[8], aw[8], top = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+            const bool in = w < cluster;
+            mw[w] = in ? ld_cluster(pr, w) : -INFINITY, lw[w] = in ? ld_cluster(pr + 4, w) : 0.f, aw[w] = in ? ld_cluster(pr + 16 + 4 * col, w) : 0.f;
+            top = fmaxf(top, mw[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+            const float f = lw[w] == 0.f ? 0.f : tcsplit::ex2(mw[w] - top);
+            sum = fmaf(lw[w], f, sum), acc = fmaf(aw[w], f, acc);
+        }
         if (a.parts == 1) {
-            finish(a, t, h, col, M, L, acc);
+            finish(a, t, h, col, top, sum, acc);
         } else {
             float* pp = a.part + (((int64_t)t * a.H + h) * a.parts + seg) * (V + 4);
-            if (col == 0) pp[0] = M, pp[1] = L;
+            if (col == 0) pp[0] = top, pp[1] = sum;
             pp[4 + col] = acc;
         }
     }
-    if (cluster > 1) tcpair::cluster_sync();  // nobody leaves while its shared memory is read
+    tcpair::cluster_sync();   // nobody leaves while its shared memory is read
 }
 
 // grid (T, H): the clusters' parts of one (token, head), in order
@@ -438,7 +510,7 @@ __global__ void attn4_merge_kernel(const __grid_constant__ Attn4Args a) {
 
 template <int NK, int NV, bool UNITS>
 cudaError_t launch(const Attn4Args& a, const b200seq_step& st, dim3 grid, cudaStream_t cs) {
-    constexpr int ring = WARPS * STAGES * 2 * (NK + NV) * 320, parts = (WARPS + 1) * ROWS * (32 * NV + 4) * 4, smem = ring > parts ? ring : parts;
+    constexpr int ring = WARPS * STAGES * 2 * (NK + NV) * 320, parts = WARPS * ROWS * (32 * NV + 4) * 4, smem = ring > parts ? ring : parts;
     const auto kernel = attn4_kernel<NK, NV, UNITS>;
     static bool ready[16] = {};
     int dev = 0;
@@ -512,6 +584,8 @@ int b200seq_attn_kv4(const float* proj, int64_t ld, const b200seq_step* st, cons
     if (d->D > KV4_MAX_DIM || d->V > KV4_MAX_DIM) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_kv4: heads of up to %d values", KV4_MAX_DIM);
     if ((reinterpret_cast<uintptr_t>(kpool) | reinterpret_cast<uintptr_t>(vpool)) & 15) return fail(B200SEQ_ERR_INVALID_ARG, "attn_kv4: pools start on a 16-byte boundary");
     if (st->block_size > 1 << 16) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_kv4: pages of up to 65536 tokens");
+    const int64_t page = (int64_t)20 * st->block_size * d->G * kv4_groups(d->D > d->V ? d->D : d->V);
+    if (page > 0x7fffffff) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_kv4: pages of up to 2 GiB");
     if (st->T == 0) return 0;
     if (st->B < 1) return fail(B200SEQ_ERR_INVALID_ARG, "attn_kv4: tokens without an entry");
     const bool gated = d->gate_col >= 0;
@@ -522,6 +596,7 @@ int b200seq_attn_kv4(const float* proj, int64_t ld, const b200seq_step* st, cons
     a.Rb = R < ROWS ? R : ROWS, a.HB = (R + a.Rb - 1) / a.Rb, a.QT = ROWS / a.Rb;
     a.scale = d->scale, a.chunk = d->chunk, a.window = d->window, a.keep_first = d->keep_first, a.head_scale = d->head_scale, a.sink = d->sink;
     a.gate = d->gate ? d->gate : proj + (gated ? d->gate_col : 0), a.gld = d->gate ? d->gate_ld : ld, a.gated = gated, a.gate_elem = gated && d->gate_elem;
+    a.vec = ((ld | d->q_col) & 3) == 0 && d->D % 8 == 0 && (reinterpret_cast<uintptr_t>(proj) & 15) == 0;
     a.softcap = d->softcap, a.out = out, a.out_dtype = out_dtype, a.err = error_flag_dev();
     Plan p = plan(*st, *d);
     if (p.parts > 1 && (!scratch || scratch_floats < (size_t)st->T * d->H * p.parts * (d->V + 4))) p.parts = 1;

@@ -8,6 +8,7 @@ namespace b200seq {
 struct Attn4Args {
     const float* q;            // query rows (pointer at the first head's column), stride ld
     int64_t ld;
+    int vec;                   // heads of whole 16-byte pieces
     const uint8_t *kpool, *vpool;
     int H, G, D, V, vdiv;      // key head g reads value head g / vdiv
     int Rb, HB, QT;            // query heads of a row tile, tiles a key head's query heads need, tokens of a row tile
