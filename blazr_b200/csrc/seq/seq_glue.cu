@@ -21,9 +21,13 @@ int fail(int code, const char* fmt, ...) {
 int cuda_status(cudaError_t e, const char* what) { return fail(B200SEQ_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e)); }
 
 __device__ int g_error_flags = 0;
-int* error_flag_dev() {
+int* error_flag_dev() {   // (its address is looked up once per device)
+    static std::atomic<int*> known[16];
     int* p = nullptr;
-    cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_error_flags);
+    int dev = -1;
+    if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 16 && (p = known[dev].load(std::memory_order_relaxed))) return p;
+    if (cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_error_flags) != cudaSuccess) return nullptr;
+    if (dev >= 0 && dev < 16) known[dev].store(p, std::memory_order_relaxed);
     return p;
 }
 

@@ -23,62 +23,105 @@ __device__ __forceinline__ int64_t kv4_page(const b200seq_step& st, int t, int& 
     return st.block_table[(int64_t)st.tok_ent[t] * st.max_blocks + b];
 }
 
-__device__ __forceinline__ void kv4_put(uint8_t* pool, const Kv4Row& at, bool key, int hl, int NG, uint32_t w, uint32_t param) {
-    *reinterpret_cast<uint16_t*>(pool + at.codes + kv4_place(key, hl, NG)) = (uint16_t)w;
-    if ((hl & 7) == 0) *reinterpret_cast<uint32_t*>(pool + at.params + (hl >> 3) * 4) = param;
+// A lane's eight codes and its group's parameters into a row.  Lanes of neighbouring groups change halves, so that value codes are stored as 32-bit words too.
+// All lanes of the warp take part; those with `in` store.
+__device__ __forceinline__ void kv4_put(uint8_t* pool, const Kv4Row& at, bool key, int hl, int NG, uint32_t w, uint32_t param, bool in) {
+    const bool second = hl & 4;                    // an odd group
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, second ? w & 0xFFFFu : w >> 16, 4);
+    if (!in || hl >= 4 * NG) return;
+    uint8_t* p = pool + at.codes;
+    if (key) {
+        *reinterpret_cast<uint32_t*>(p + kv4_key_place(hl, NG)) = w;
+    } else if (NG == 1) {
+        *reinterpret_cast<uint16_t*>(p + kv4_value_place(hl, NG)) = (uint16_t)w;
+        *reinterpret_cast<uint16_t*>(p + kv4_value_place(hl, NG) + 2 * NG) = (uint16_t)(w >> 16);
+    } else {                                       // the even group of a pair stores the first words of both, the odd one the second
+        *reinterpret_cast<uint32_t*>(p + kv4_value_place(hl & ~4, NG) + (second ? 2 * NG : 0)) = second ? other | (w & 0xFFFF0000u) : (w & 0xFFFFu) | (other << 16);
+    }
+    if ((hl & 3) == 0) *reinterpret_cast<uint32_t*>(pool + at.params + hl) = param;
 }
 
-// a warp per row (token, key or value head)
-__global__ void kv4_store_kernel(const Kv4Rows a, const b200seq_step st, int* err) {
+// A block has a token; LPR lanes (4 for every group of the wider of key and value heads) have a row of it at a time.  Bounded by instructions: 340 a row with
+// four values to a lane and a warp to a row (4094 tokens, 16 rows of 128 bf16: 34 us).
+template <int LPR>
+__global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4Rows a, const b200seq_step st, int* err) {
     chain_enter();
-    const int lane = threadIdx.x & 31, heads = a.G + a.Gv;
-    const int64_t unit = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (unit >= (int64_t)st.T * heads) return;
-    const int t = (int)(unit / heads), u = (int)(unit - (int64_t)t * heads);
-    const bool key = u < a.G;
-    const int g = key ? u : u - a.G, D = key ? a.D : a.V, G = key ? a.G : a.Gv, NG = kv4_groups(D);
+    const int hl = threadIdx.x & (LPR - 1), heads = a.G + a.Gv, t = blockIdx.x;
     int o;
     const int64_t page = kv4_page(st, t, o, err);
     if (page < 0) return;
-    const int64_t src = (int64_t)t * (key ? a.ldk : a.ldv) + (int64_t)g * D + 4 * lane;
-    const void* p = key ? a.k : a.v;
-    const int n = min(max(D - 4 * lane, 0), 4);
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
-    if (a.bf16) {
-        const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p) + src;
-        for (int i = 0; i < n; ++i) x[i] = __bfloat162float(q[i]);
-    } else {
-        const float* q = reinterpret_cast<const float*>(p) + src;
-        for (int i = 0; i < n; ++i) x[i] = q[i];
-    }
-    uint32_t param;
     bool odd = false;
-    const uint32_t w = kv4_quantise(x, n, param, odd);
-    if (lane < NG * 8) kv4_put(key ? a.kpool : a.vpool, kv4_row(page, o, st.block_size, g, G, NG), key, lane, NG, w, param);
+    for (int u0 = (threadIdx.x & ~31) / LPR; u0 < heads; u0 += blockDim.x / LPR) {
+        const int u = u0 + (threadIdx.x & 31) / LPR;
+        const bool in = u < heads, key = u < a.G;
+        const int g = key ? u : u - a.G, D = key ? a.D : a.V, NG = kv4_groups(D), n = in ? min(max(D - 8 * hl, 0), 8) : 0;
+        const int64_t src = (int64_t)t * (key ? a.ldk : a.ldv) + g * D + 8 * hl;
+        const void* p = key ? a.k : a.v;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = 0.f;
+        if (a.bf16) {
+            const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p) + src;
+            if (a.vec && n == 8) {
+                const uint4 w = *reinterpret_cast<const uint4*>(q);
+                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[2 * j] = __uint_as_float(ws[j] << 16), x[2 * j + 1] = __uint_as_float(ws[j] & 0xFFFF0000u);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < n) x[j] = __bfloat162float(q[j]);
+            }
+        } else {
+            const float* q = reinterpret_cast<const float*>(p) + src;
+            if (a.vec && n == 8) {
+                const float4 v = ld4(q), w = ld4(q + 4);
+                x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w, x[4] = w.x, x[5] = w.y, x[6] = w.z, x[7] = w.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < n) x[j] = q[j];
+            }
+        }
+        uint32_t param;
+        const uint32_t w = kv4_quantise(x, n, param, odd);
+        kv4_put(key ? a.kpool : a.vpool, kv4_row(page, o, st.block_size, in ? g : 0, key ? a.G : a.Gv, NG), key, hl, NG, w, param, in);
+    }
     if (odd) atomicOr(err, KV4_ERR_RANGE);
 }
 
 // the same rows back, as the values they stand for
-__global__ void kv4_load_kernel(const Kv4Rows a, float* __restrict__ ko, float* __restrict__ vo, const b200seq_step st, int* err) {
+template <int LPR>
+__global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4Rows a, float* __restrict__ ko, float* __restrict__ vo, const b200seq_step st, int* err) {
     chain_enter();
-    const int lane = threadIdx.x & 31, heads = a.G + a.Gv;
-    const int64_t unit = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    if (unit >= (int64_t)st.T * heads) return;
-    const int t = (int)(unit / heads), u = (int)(unit - (int64_t)t * heads);
-    const bool key = u < a.G;
-    const int g = key ? u : u - a.G, D = key ? a.D : a.V, G = key ? a.G : a.Gv, NG = kv4_groups(D);
+    const int hl = threadIdx.x & (LPR - 1), heads = a.G + a.Gv, t = blockIdx.x;
     int o;
     const int64_t page = kv4_page(st, t, o, err);
     if (page < 0) return;
-    const uint8_t* pool = key ? a.kpool : a.vpool;
-    const Kv4Row at = kv4_row(page, o, st.block_size, g, G, NG);
-    const int n = min(max(D - 4 * lane, 0), 4);
-    if (n == 0) return;
-    const uint32_t w = *reinterpret_cast<const uint16_t*>(pool + at.codes + kv4_place(key, lane, NG));
-    const uint32_t pr = *reinterpret_cast<const uint32_t*>(pool + at.params + (lane >> 3) * 4);
-    const float s = __half2float(__ushort_as_half((uint16_t)pr)), m = __half2float(__ushort_as_half((uint16_t)(pr >> 16)));
-    float* dst = (key ? ko + (int64_t)t * a.ldk : vo + (int64_t)t * a.ldv) + (int64_t)g * D + 4 * lane;
-    for (int i = 0; i < n; ++i) dst[i] = fmaf(s, (float)((w >> (4 * i)) & 15u), m);
+    for (int u = threadIdx.x / LPR; u < heads; u += blockDim.x / LPR) {
+        const bool key = u < a.G;
+        const int g = key ? u : u - a.G, D = key ? a.D : a.V, NG = kv4_groups(D), n = min(max(D - 8 * hl, 0), 8);
+        if (n == 0) continue;
+        const uint8_t* pool = key ? a.kpool : a.vpool;
+        const Kv4Row at = kv4_row(page, o, st.block_size, g, key ? a.G : a.Gv, NG);
+        uint32_t w;
+        if (key) w = *reinterpret_cast<const uint32_t*>(pool + at.codes + kv4_key_place(hl, NG));
+        else w = *reinterpret_cast<const uint16_t*>(pool + at.codes + kv4_value_place(hl, NG)) | ((uint32_t)*reinterpret_cast<const uint16_t*>(pool + at.codes + kv4_value_place(hl, NG) + 2 * NG) << 16);
+        const uint32_t pr = *reinterpret_cast<const uint32_t*>(pool + at.params + (hl & ~3));
+        const float s = __half2float(__ushort_as_half((uint16_t)pr)), m = __half2float(__ushort_as_half((uint16_t)(pr >> 16)));
+        float* dst = (key ? ko + (int64_t)t * a.ldk : vo + (int64_t)t * a.ldv) + g * D + 8 * hl;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = fmaf(s, __uint_as_float(((w >> (4 * j)) & 15u) | 0x4B000000u) - 8388608.f, m);   // (2^23 + code)
+        if (a.vec && n == 8) {
+            *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < n) dst[j] = x[j];
+        }
+    }
 }
 
 // b200seq_attn_prep_ex over 4-bit pages: grid (T), 256 threads, a warp per head unit; the unit's values are staged in the warp's slice of shared memory, biased,
@@ -143,13 +186,13 @@ __global__ void kv4_prep_kernel(float* __restrict__ proj, int64_t ld, const b200
         if (isq) {
             for (int d = lane; d < D; d += 32) base[col + d] = hs[d];
         } else if (page >= 0) {
-            const int n = min(max(size - 4 * lane, 0), 4), NG = kv4_groups(size);
-            float x[4];
+            const int n = min(max(size - 8 * lane, 0), 8), NG = kv4_groups(size);
+            float x[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = i < n ? hs[4 * lane + i] : 0.f;
+            for (int i = 0; i < 8; ++i) x[i] = i < n ? hs[8 * lane + i] : 0.f;
             uint32_t param;
             const uint32_t w = kv4_quantise(x, n, param, odd);
-            if (lane < NG * 8) kv4_put(isk ? kpool : vpool, kv4_row(page, o, st.block_size, hh, isk ? G : Gv, NG), isk, lane, NG, w, param);
+            kv4_put(isk ? kpool : vpool, kv4_row(page, o, st.block_size, hh, isk ? G : Gv, NG), isk, lane, NG, w, param, true);
         }
         __syncwarp();   // hs is used again by the warp's next unit
     }
@@ -169,8 +212,18 @@ int rows_check(const b200seq_step* st, const void* k, const void* v, int64_t ldk
     if (D > KV4_MAX_DIM || V > KV4_MAX_DIM) return fail(B200SEQ_ERR_UNSUPPORTED, "%s: heads of up to %d values", what, KV4_MAX_DIM);
     if (st->T > 1 && (ldk < (int64_t)G * D || ldv < (int64_t)Gv * V)) return fail(B200SEQ_ERR_INVALID_ARG, "%s: row strides below a row's length", what);
     if ((reinterpret_cast<uintptr_t>(kpool) | reinterpret_cast<uintptr_t>(vpool)) & 15) return fail(B200SEQ_ERR_INVALID_ARG, "%s: pools start on a 16-byte boundary", what);
-    if (((int64_t)st->T * ((int64_t)G + Gv) + 7) / 8 > 0x7fffffff) return fail(B200SEQ_ERR_UNSUPPORTED, "%s: too many rows", what);
+    if (((int64_t)G + Gv) * KV4_MAX_DIM > 0x7fffffff) return fail(B200SEQ_ERR_UNSUPPORTED, "%s: too many heads", what);
     return 0;
+}
+
+// threads of a block: a token's rows at once, 256 at most
+int row_threads(int heads, int lpr) {
+    const int n = (heads * lpr + 31) / 32 * 32;
+    return n < 256 ? n : 256;
+}
+// rows whose lanes' eight values are whole 16-byte pieces (align: elements of one)
+bool row_pieces(const void* k, const void* v, int64_t ldk, int64_t ldv, int D, int V, int align) {
+    return ((D | V) & 7) == 0 && ((ldk | ldv) & (align - 1)) == 0 && ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
 }
 
 }  // namespace
@@ -191,9 +244,10 @@ int b200seq_kv4_store(const void* k, int64_t ldk, const void* v, int64_t ldv, in
     if (in_dtype != B200SEQ_F32 && in_dtype != B200SEQ_BF16) return fail(B200SEQ_ERR_INVALID_ARG, "kv4_store: rows are f32 or bf16");
     if (int rc = rows_check(st, k, v, ldk, ldv, G, D, Gv, V, kpool, vpool, "kv4_store")) return rc;
     if (st->T == 0) return 0;
-    const Kv4Rows a{k, v, ldk, ldv, (uint8_t*)kpool, (uint8_t*)vpool, G, D, Gv, V, in_dtype == B200SEQ_BF16, 0};
-    const int64_t rows = (int64_t)st->T * (G + Gv);
-    launch_chained(kv4_store_kernel, dim3((unsigned)((rows + 7) / 8)), 256, 0, (cudaStream_t)stream, a, *st, error_flag_dev());
+    const bool bf16 = in_dtype == B200SEQ_BF16;
+    const Kv4Rows a{k, v, ldk, ldv, (uint8_t*)kpool, (uint8_t*)vpool, G, D, Gv, V, bf16, row_pieces(k, v, ldk, ldv, D, V, bf16 ? 8 : 4)};
+    const int lpr = 4 * kv4_groups(D > V ? D : V);
+    launch_chained(lpr == 4 ? kv4_store_kernel<4> : (lpr == 8 ? kv4_store_kernel<8> : kv4_store_kernel<16>), st->T, row_threads(G + Gv, lpr), 0, (cudaStream_t)stream, a, *st, error_flag_dev());
     SEQ_LAUNCH_CHECK("kv4_store");
     return 0;
 }
@@ -201,9 +255,10 @@ int b200seq_kv4_store(const void* k, int64_t ldk, const void* v, int64_t ldv, in
 int b200seq_kv4_load(const void* kpool, const void* vpool, const b200seq_step* st, int G, int D, int Gv, int V, float* k, int64_t ldk, float* v, int64_t ldv, void* stream) {
     if (int rc = rows_check(st, k, v, ldk, ldv, G, D, Gv, V, kpool, vpool, "kv4_load")) return rc;
     if (st->T == 0) return 0;
-    const Kv4Rows a{nullptr, nullptr, ldk, ldv, (uint8_t*)kpool, (uint8_t*)vpool, G, D, Gv, V, 0, 0};
-    const int64_t rows = (int64_t)st->T * (G + Gv);
-    launch_chained(kv4_load_kernel, dim3((unsigned)((rows + 7) / 8)), 256, 0, (cudaStream_t)stream, a, k, v, *st, error_flag_dev());
+    const Kv4Rows a{nullptr, nullptr, ldk, ldv, (uint8_t*)kpool, (uint8_t*)vpool, G, D, Gv, V, 0, row_pieces(k, v, ldk, ldv, D, V, 4)};
+    const int lpr = 4 * kv4_groups(D > V ? D : V);
+    launch_chained(lpr == 4 ? kv4_load_kernel<4> : (lpr == 8 ? kv4_load_kernel<8> : kv4_load_kernel<16>), st->T, row_threads(G + Gv, lpr), 0, (cudaStream_t)stream, a, k, v, *st,
+                   error_flag_dev());
     SEQ_LAUNCH_CHECK("kv4_load");
     return 0;
 }

@@ -32,26 +32,31 @@ struct Kv4Row {
     int64_t codes, params;
 };
 __device__ __forceinline__ Kv4Row kv4_row(int64_t page, int o, int bs, int g, int G, int NG) {
-    const int unit = kv4_unit(bs), u = o / unit, ru = o - u * unit;
+    const int unit = kv4_unit(bs), u = unit == 16 ? o >> 4 : 0, ru = unit == 16 ? o & 15 : o;   // (o < bs)
     const int64_t base = (page * G + g) * (int64_t)(bs * NG * 20) + (int64_t)u * (unit * NG * 20);
     return Kv4Row{base + ru * NG * 16, base + unit * NG * 16 + ru * NG * 4};
 }
 
-// A group of 32 values, four in each of eight neighbouring lanes (`n` of the lane's four are values of the row, the rest do not exist).  Returns the lane's four
-// codes in 16 bits and, the same in all eight lanes, the (s, m) pair.  Every lane of the warp takes part.
-__device__ __forceinline__ uint32_t kv4_quantise(float (&x)[4], int n, uint32_t& param, bool& odd) {
-    float lo = INFINITY, hi = -INFINITY;
+// A group of 32 values, eight in each of four neighbouring lanes (`n` of the lane's eight are values of the row, the rest do not exist).  Returns the lane's eight
+// codes, the first in the lowest bits, and, the same in all four lanes, the (s, m) pair.  Every lane of the warp takes part.
+__device__ __forceinline__ uint32_t kv4_quantise(float (&x)[8], int n, uint32_t& param, bool& odd) {
+    bool fine = true;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float y = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -KV4_LIMIT), KV4_LIMIT);
-        if (i < n) {
-            odd |= !(y == x[i]);
-            lo = fminf(lo, y), hi = fmaxf(hi, y);
-        }
-        x[i] = y;
+    for (int i = 0; i < 8; ++i) fine &= fabsf(x[i]) <= KV4_LIMIT;      // (places that do not exist hold zeros)
+    if (!fine) {
+        odd = true;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = x[i] != x[i] ? 0.f : fminf(fmaxf(x[i], -KV4_LIMIT), KV4_LIMIT);
     }
+    if (n < 8) {
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)), hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        for (int i = 1; i < 8; ++i) x[i] = i < n ? x[i] : x[0];
+    }
+    float lo = fminf(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])), fminf(fminf(x[4], x[5]), fminf(x[6], x[7])));
+    float hi = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    if (n == 0) lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)), hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     if (!(lo <= hi)) {   // a group behind the row's end
         param = 0;
         return 0;
@@ -63,19 +68,16 @@ __device__ __forceinline__ uint32_t kv4_quantise(float (&x)[4], int n, uint32_t&
     if (s < 0x1p-18f) s = ceilf(s * 0x1p24f) * 0x1p-24f;
     param = (uint32_t)__half_as_ushort(__float2half_rn(s)) | ((uint32_t)__half_as_ushort(mh) << 16);
     const float inv = s > 0.f ? 1.0f / s : 0.f;
+    // rint(y) for y in 0 .. 15 by adding 1.5 2^23, whose bits then end in the number; the words of eight of them add up, sixteenfold each, to the codes and a constant
     uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = min(max(__float2int_rn((x[i] - m) * inv), 0), 15);
-        w |= (i < n ? (uint32_t)c : 0u) << (4 * i);
-    }
-    return w;
+    for (int i = 7; i >= 0; --i) w = w * 16u + __float_as_uint(__fadd_rn(fminf(fmaxf(__fmul_rn(x[i] - m, inv), 0.f), 15.f), 12582912.f));
+    w -= 0x4B400000u * 0x11111111u;
+    return n < 8 ? w & ((1u << (4 * n)) - 1u) : w;
 }
 
-// place of a lane's four codes in the row: lane hl holds values 4 hl .. 4 hl + 3
-__device__ __forceinline__ int kv4_place(bool key, int hl, int NG) {
-    const int g = hl >> 3, r = hl & 7;
-    return key ? (((r >> 1) * NG + g) * 2 + (r & 1)) * 2 : (r * NG + g) * 2;
-}
+// The place of a lane's codes in a row's: lane hl holds values 8 hl .. 8 hl + 7, of group hl / 4: one word of a key row, two 16-bit words of a value row
+__device__ __forceinline__ int kv4_key_place(int hl, int NG) { return ((hl & 3) * NG + (hl >> 2)) * 4; }
+__device__ __forceinline__ int kv4_value_place(int hl, int NG) { return (2 * (hl & 3) * NG + (hl >> 2)) * 2; }   // (the second: 2 NG bytes on)
 
 }  // namespace b200seq

@@ -2,6 +2,7 @@
 //
 // A step between two steps of a serving loop: few bytes in many places.  The (from, to) pairs and the pools travel in the launch's own parameters, so a
 // copy is one launch with no upload before it; nothing of it is kept.  Bounded by the memory, 2 bytes a byte copied, or by the launch.
+#include <cstring>
 #include <vector>
 
 #include "seq_common.cuh"
@@ -17,7 +18,7 @@ template <int N>
 struct PageCopy {
     uint8_t* pool[POOLS];
     int64_t bytes[POOLS];   // of one page
-    int32_t from[N], to[N];
+    int2 pair[N];           // from, to
 };
 
 template <class V>
@@ -39,8 +40,9 @@ __global__ void __launch_bounds__(THREADS) copy_pages_kernel(const __grid_consta
     chain_enter();
     uint8_t* pool = c.pool[blockIdx.y];
     const int64_t bytes = c.bytes[blockIdx.y];
-    const uint8_t* src = pool + c.from[blockIdx.x] * bytes;
-    uint8_t* dst = pool + c.to[blockIdx.x] * bytes;
+    const int2 pair = c.pair[blockIdx.x];
+    const uint8_t* src = pool + pair.x * bytes;
+    uint8_t* dst = pool + pair.y * bytes;
     const bool wide = ((reinterpret_cast<uintptr_t>(pool) | (uintptr_t)bytes) & 15) == 0;
     for (int64_t at = (int64_t)blockIdx.z * CHUNK; at < bytes; at += (int64_t)gridDim.z * CHUNK) {
         const int64_t n = min((int64_t)CHUNK, bytes - at);
@@ -50,7 +52,7 @@ __global__ void __launch_bounds__(THREADS) copy_pages_kernel(const __grid_consta
 }
 
 template <int N>
-int run(void* const* pools, const int64_t* bytes, int npools, const int32_t* from, const int32_t* to, int n, cudaStream_t cs) {
+int run(void* const* pools, const int64_t* bytes, int npools, const int32_t* pairs, int n, cudaStream_t cs) {
     for (int p0 = 0; p0 < npools; p0 += POOLS) {
         PageCopy<N> c;
         const int np = npools - p0 < POOLS ? npools - p0 : POOLS;
@@ -62,7 +64,7 @@ int run(void* const* pools, const int64_t* bytes, int npools, const int32_t* fro
         if (most == 0) continue;
         for (int q0 = 0; q0 < n; q0 += N) {
             const int nq = n - q0 < N ? n - q0 : N;
-            for (int i = 0; i < N; ++i) c.from[i] = i < nq ? from[q0 + i] : 0, c.to[i] = i < nq ? to[q0 + i] : 0;
+            std::memcpy(c.pair, pairs + 2 * q0, (size_t)nq * 8);
             const int64_t parts = (most + CHUNK - 1) / CHUNK;
             launch_chained(copy_pages_kernel<N>, dim3(nq, np, (unsigned)(parts < 65535 ? parts : 65535)), THREADS, 0, cs, c);
             SEQ_LAUNCH_CHECK("copy_pages");
@@ -77,24 +79,25 @@ int run(void* const* pools, const int64_t* bytes, int npools, const int32_t* fro
 
 using namespace b200seq;
 
-extern "C" int b200seq_copy_pages(void* const* pools, const int64_t* page_bytes, int npools, int pages, const int32_t* from, const int32_t* to, int n, void* stream) {
-    if (npools < 0 || pages < 0 || n < 0 || (npools > 0 && (!pools || !page_bytes)) || (n > 0 && (!from || !to))) return fail(B200SEQ_ERR_INVALID_ARG, "copy_pages: bad arguments");
+extern "C" int b200seq_copy_pages(void* const* pools, const int64_t* page_bytes, int npools, int pages, const int32_t* pairs, int n, void* stream) {
+    if (npools < 0 || pages < 0 || n < 0 || (npools > 0 && (!pools || !page_bytes)) || (n > 0 && !pairs)) return fail(B200SEQ_ERR_INVALID_ARG, "copy_pages: bad arguments");
     for (int i = 0; i < npools; ++i)
         if (!pools[i] || page_bytes[i] < 0) return fail(B200SEQ_ERR_INVALID_ARG, "copy_pages: pool %d is null or its pages have no size", i);
     // A copy's result does not depend on the order of its pairs: no page is written twice, none is both read and written.
+    for (int i = 0; i < 2 * n; ++i)
+        if (pairs[i] < 0 || pairs[i] >= pages)
+            return fail(B200SEQ_ERR_INVALID_ARG, "copy_pages: pair %d names a page outside the pool's %d (%d -> %d)", i / 2, pages, pairs[i & ~1], pairs[i | 1]);
     try {
-        std::vector<uint8_t> use((size_t)pages, 0);
+        std::vector<bool> written((size_t)pages, false);
         for (int i = 0; i < n; ++i) {
-            if (from[i] < 0 || from[i] >= pages || to[i] < 0 || to[i] >= pages)
-                return fail(B200SEQ_ERR_INVALID_ARG, "copy_pages: pair %d names a page outside the pool's %d (%d -> %d)", i, pages, from[i], to[i]);
-            if (use[to[i]]) return fail(B200SEQ_ERR_INVALID_ARG, "copy_pages: page %d is written twice, or read and written, by one call", to[i]);
-            use[to[i]] = 1;
+            if (written[pairs[2 * i + 1]]) return fail(B200SEQ_ERR_INVALID_ARG, "copy_pages: page %d is written twice by one call", pairs[2 * i + 1]);
+            written[pairs[2 * i + 1]] = true;
         }
         for (int i = 0; i < n; ++i)
-            if (use[from[i]]) return fail(B200SEQ_ERR_INVALID_ARG, "copy_pages: page %d is both read and written by one call", from[i]);
+            if (written[pairs[2 * i]]) return fail(B200SEQ_ERR_INVALID_ARG, "copy_pages: page %d is both read and written by one call", pairs[2 * i]);
     } catch (const std::exception&) {
         return fail(B200SEQ_ERR_INVALID_ARG, "copy_pages: no memory for the check of %d pages", pages);
     }
     if (n == 0 || npools == 0) return 0;
-    return n <= FEW ? run<FEW>(pools, page_bytes, npools, from, to, n, (cudaStream_t)stream) : run<MANY>(pools, page_bytes, npools, from, to, n, (cudaStream_t)stream);
+    return n <= FEW ? run<FEW>(pools, page_bytes, npools, pairs, n, (cudaStream_t)stream) : run<MANY>(pools, page_bytes, npools, pairs, n, (cudaStream_t)stream);
 }

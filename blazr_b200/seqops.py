@@ -17,8 +17,8 @@ import fcntl
 import os
 import shutil
 import subprocess
-from array import array
 from itertools import chain
+from struct import error as StructError, pack
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -65,7 +65,7 @@ SIGNATURES = {
     "polynorm": "pliipfpilp", "softcap": "plfp", "diff_combine": "piiiifffpip", "min_gru": "pliiipppipip", "rg_lru": "plplppfplipppiipip", "delta": "plppplppipzp",
     "embed_pos": "pppfpippppfpip", "sandwich_norm": "pppfppipippipp", "token_gate": "pliiplippip", "side_close": "pppfpppliippppipippipp",
     "selective_scan": "piplpplppppipzp", "parallel_close": "pp", "argmax": "piipp", "kv4_page_bytes": "iii", "kv4_store": "plplipiiiippp", "kv4_load": "pppiiiiplplp",
-    "attn_prep_kv4": "plppppp", "attn_kv4": "plpppppipzp", "attn_kv4_scratch_floats": "pp", "copy_pages": "ppiippip", "process_logits": "pliipppppppplplp"
+    "attn_prep_kv4": "plppppp", "attn_kv4": "plpppppipzp", "attn_kv4_scratch_floats": "pp", "copy_pages": "ppiipip", "process_logits": "pliipppppppplplp"
 }
 
 
@@ -876,65 +876,72 @@ def kv4_pool(num_blocks: int, block_size: int, heads: int, dim: int, device) -> 
 
 def _on_device(name: str, fn, args: tuple, *tensors: Optional[torch.Tensor]) -> None:
     """a library call on the one CUDA device of its tensors, on that device's current stream (the library launches on the current device)"""
-    dev = None
+    dev = -2
     for t in tensors:
-        if t is None:
-            continue
-        if t.device.type != "cuda":
-            raise ValueError(f"{name}: Expected a cuda device, but got: {t.device}")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"{name}: tensors on {dev} and {t.device}")
-        dev = t.device
-    if dev.index == torch.cuda.current_device():
-        _check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index)))
+        if t is not None:
+            d = t.get_device()
+            if d != dev:
+                if dev != -2 or d < 0:
+                    raise ValueError(f"{name}: tensors of one cuda device expected, but got: {[str(t.device) for t in tensors if t is not None]}")
+                dev = d
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            _check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index)))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc != 0:
+        _check(rc)
 
 
 def _kv4_pool_check(name: str, what: str, pool: torch.Tensor, block_size: int, heads: int, dim: int) -> None:
-    if pool.dtype != torch.uint8 or pool.dim() != 3 or not pool.is_contiguous() or pool.shape[1] != heads or pool.shape[2] != 20 * block_size * (1 if dim <= 32 else 2 if dim <= 64 else 4):
+    shape = pool.shape
+    if pool.dtype != torch.uint8 or len(shape) != 3 or shape[1] != heads or shape[2] != 20 * block_size * (1 if dim <= 32 else 2 if dim <= 64 else 4) or not pool.is_contiguous():
         raise ValueError(f"{name}: the {what} pool is no contiguous uint8 [pages, {heads}, bytes] of pages of {block_size} positions and heads of {dim} values: "
                          f"{pool.dtype} {tuple(pool.shape)}")
 
 
 def _kv4_rows(name: str, k: torch.Tensor, v: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, step: "StepDesc"):
+    """(heads, size) of keys, the same of values, row strides"""
+    ks, vs, kt, vt, T = k.shape, v.shape, k.stride(), v.stride(), step.T
+    if kpool.dim() != 3 or vpool.dim() != 3:
+        raise ValueError(f"{name}: pools are uint8 [pages, heads, bytes], not {tuple(kpool.shape)} and {tuple(vpool.shape)}")
     G, Gv = kpool.shape[1], vpool.shape[1]
-    if k.dim() != 2 or v.dim() != 2 or k.stride(1) != 1 or v.stride(1) != 1 or k.shape[0] != step.T or v.shape[0] != step.T or k.shape[1] % G or v.shape[1] % Gv or k.dtype != v.dtype:
-        raise ValueError(f"{name}: rows {tuple(k.shape)} and {tuple(v.shape)} of {step.T} tokens do not fit {G} and {Gv} heads")
-    D, V = k.shape[1] // G, v.shape[1] // Gv
+    if len(ks) != 2 or len(vs) != 2 or kt[1] != 1 or vt[1] != 1 or ks[0] != T or vs[0] != T or ks[1] % G or vs[1] % Gv or k.dtype != v.dtype:
+        raise ValueError(f"{name}: rows {tuple(ks)} and {tuple(vs)} of {T} tokens do not fit {G} and {Gv} heads")
+    D, V = ks[1] // G, vs[1] // Gv
     _kv4_pool_check(name, "key", kpool, step.block_size, G, D)
     _kv4_pool_check(name, "value", vpool, step.block_size, Gv, V)
-    return G, D, Gv, V
+    return G, D, Gv, V, kt[0], vt[0]
 
 
 @_timed
 def kv4_store(k: torch.Tensor, v: torch.Tensor, step: "StepDesc", kpool: torch.Tensor, vpool: torch.Tensor):
     """keys [T, G * D] and values [T, Gv * V] (f32 or bf16 rows, as they are to be cached: normed, rotated) of the step's tokens go to their pages, quantised to 4 bits"""
-    G, D, Gv, V = _kv4_rows("kv4_store", k, v, kpool, vpool, step)
-    if k.dtype not in _DT:
+    G, D, Gv, V, ldk, ldv = _kv4_rows("kv4_store", k, v, kpool, vpool, step)
+    dt = _DT.get(k.dtype)
+    if dt is None:
         raise ValueError(f"kv4_store: rows are float32 or bfloat16, not {k.dtype}")
-    _on_device("kv4_store", lib().b200seq_kv4_store, (_p(k), k.stride(0), _p(v), v.stride(0), _DT[k.dtype], C.byref(step), G, D, Gv, V, _p(kpool), _p(vpool)),
-               k, v, kpool, vpool)
+    _on_device("kv4_store", lib().b200seq_kv4_store, (k.data_ptr(), ldk, v.data_ptr(), ldv, dt, C.byref(step), G, D, Gv, V, kpool.data_ptr(), vpool.data_ptr()), k, v, kpool, vpool)
 
 
 @_timed
 def kv4_load(kpool: torch.Tensor, vpool: torch.Tensor, step: "StepDesc", k: torch.Tensor, v: torch.Tensor):
     """the rows that the cache holds for the step's tokens, as the values they stand for: k f32 [T, G * D], v f32 [T, Gv * V]"""
-    G, D, Gv, V = _kv4_rows("kv4_load", k, v, kpool, vpool, step)
+    G, D, Gv, V, ldk, ldv = _kv4_rows("kv4_load", k, v, kpool, vpool, step)
     if k.dtype != torch.float32:
         raise ValueError(f"kv4_load: rows are float32, not {k.dtype}")
-    _on_device("kv4_load", lib().b200seq_kv4_load, (_p(kpool), _p(vpool), C.byref(step), G, D, Gv, V, _p(k), k.stride(0), _p(v), v.stride(0)), k, v, kpool, vpool)
+    _on_device("kv4_load", lib().b200seq_kv4_load, (kpool.data_ptr(), vpool.data_ptr(), C.byref(step), G, D, Gv, V, k.data_ptr(), ldk, v.data_ptr(), ldv), k, v, kpool, vpool)
 
 
 def _kv4_layer(name: str, proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: Optional[torch.Tensor], vpool: Optional[torch.Tensor], need: int) -> int:
-    if proj.dim() != 2 or proj.stride(1) != 1 or proj.dtype != torch.float32 or proj.shape[0] < step.T or proj.shape[1] < need:
-        raise ValueError(f"{name}: projection rows are row-major float32 [{step.T}, {need} or more], not {proj.dtype} {tuple(proj.shape)}")
+    shape, ld = proj.shape, proj.stride()
+    if len(shape) != 2 or ld[1] != 1 or proj.dtype != torch.float32 or shape[0] < step.T or shape[1] < need:
+        raise ValueError(f"{name}: projection rows are row-major float32 [{step.T}, {need} or more], not {proj.dtype} {tuple(shape)}")
     if kpool is not None:
         _kv4_pool_check(name, "key", kpool, step.block_size, d.G, d.D)
     if vpool is not None:
         _kv4_pool_check(name, "value", vpool, step.block_size, d.vg if d.vg > 0 else d.G, d.V)
-    return proj.stride(0)
+    return ld[0]
 
 
 @_timed
@@ -949,21 +956,26 @@ def attn_prep_kv4(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: Op
 def attn_kv4(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: torch.Tensor, vpool: torch.Tensor, out: torch.Tensor, gate: Optional[torch.Tensor] = None):
     """attn_ex over a 4-bit cache: out [T, H * V] (f32 or bf16) = softmax(q k^T * scale + mask) v, gated as the layer says.
     (The work area of few long sequences is the call's own: no two calls, streams or graphs share it.)"""
-    own_gate = d.gate_col >= 0 and gate is None and not d.gate
-    need = max(d.q_col + d.H * d.D, d.gate_col + (d.H * d.V if d.gate_elem else d.H) if own_gate else 0)
+    H, V, T = d.H, d.V, step.T
+    need = d.q_col + H * d.D
+    if d.gate_col >= 0 and gate is None and not d.gate:
+        need = max(need, d.gate_col + (H * V if d.gate_elem else H))
     ld = _kv4_layer("attn_kv4", proj, step, d, kpool, vpool, need)
-    if out.dtype not in _DT or not out.is_contiguous() or out.shape[0] < step.T or out[0:1].numel() != d.H * d.V:
-        raise ValueError(f"attn_kv4: results are contiguous float32 or bfloat16 [{step.T}, {d.H * d.V}], not {out.dtype} {tuple(out.shape)}")
+    dt, shape = _DT.get(out.dtype), out.shape
+    if dt is None or len(shape) < 2 or shape[0] < T or (shape[1] if len(shape) == 2 else out.numel() // max(1, shape[0])) != H * V or not out.is_contiguous():
+        raise ValueError(f"attn_kv4: results are contiguous float32 or bfloat16 [{T}, {H * V}], not {out.dtype} {tuple(shape)}")
     if gate is not None:
-        if gate.dim() != 2 or gate.stride(1) != 1 or gate.dtype != torch.float32 or gate.shape[0] < step.T or gate.shape[1] < (d.H * d.V if d.gate_elem else d.H):
+        if gate.dim() != 2 or gate.stride(1) != 1 or gate.dtype != torch.float32 or gate.shape[0] < T or gate.shape[1] < (H * V if d.gate_elem else H):
             raise ValueError("attn_kv4: gate logits are row-major float32 rows, one for each head (or output element)")
         d2 = AttnDesc.from_buffer_copy(d)
         d2.gate, d2.gate_ld = gate.data_ptr(), gate.stride(0)
         d = d2
+    L = lib()
     sref, dref = C.byref(step), C.byref(d)
-    need = lib().b200seq_attn_kv4_scratch_floats(sref, dref)
+    need = L.b200seq_attn_kv4_scratch_floats(sref, dref)
     scratch = torch.empty(need, dtype=torch.float32, device=proj.device) if need else None
-    _on_device("attn_kv4", lib().b200seq_attn_kv4, (_p(proj), ld, sref, dref, _p(kpool), _p(vpool), _p(out), _DT[out.dtype], _p(scratch), need), proj, kpool, vpool, out, gate)
+    _on_device("attn_kv4", L.b200seq_attn_kv4, (proj.data_ptr(), ld, sref, dref, kpool.data_ptr(), vpool.data_ptr(), out.data_ptr(), dt, scratch.data_ptr() if need else None, need),
+               proj, kpool, vpool, out, gate)
 
 
 # ---- pages ---------------------------------------------------------------------------------------------------------------------------------------------
@@ -971,20 +983,22 @@ def attn_kv4(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: torch.T
 def copy_pages(pools: Sequence[torch.Tensor], pairs: Sequence[Tuple[int, int]]):
     """page `to` of every pool <- its page `from`, for all pairs (from, to) of host numbers, in one launch.  Pools: contiguous, the first dimension counts the
     pages and is the same in all.  A page may be read by several pairs, but not written twice and not both read and written."""
+    n = len(pairs)
     if not len(pools):
         return
     pages = pools[0].shape[0]
+    ptrs, size = [], []
     for p in pools:
-        if not p.is_contiguous() or p.dim() < 1 or p.shape[0] != pages:
+        if p.shape[0] != pages or not p.is_contiguous():
             raise ValueError(f"copy_pages: pools are contiguous and of one number of pages, not {tuple(p.shape)} beside {pages}")
-    n, np_ = len(pairs), len(pools)
-    flat = array("i", chain.from_iterable(pairs))
-    if len(flat) != 2 * n:
-        raise ValueError("copy_pages: pairs of (from, to) expected")
-    src, dst = flat[0::2], flat[1::2]
-    ptrs = (C.c_void_p * np_)(*[p.data_ptr() for p in pools])
-    size = (C.c_int64 * np_)(*[p.numel() // pages * p.element_size() if pages else 0 for p in pools])
-    _on_device("copy_pages", lib().b200seq_copy_pages, (ptrs, size, np_, pages, src.buffer_info()[0] if n else None, dst.buffer_info()[0] if n else None, n), *pools)
+        ptrs.append(p.data_ptr())
+        size.append(p.nbytes // pages if pages else 0)
+    try:
+        flat = pack(f"{2 * n}i", *chain.from_iterable(pairs))
+    except StructError as e:
+        raise ValueError(f"copy_pages: pairs of (from, to) numbers expected: {e}") from None
+    np_ = len(ptrs)
+    _on_device("copy_pages", lib().b200seq_copy_pages, (pack(f"{np_}P", *ptrs), pack(f"{np_}q", *size), np_, pages, flat, n), *pools)
 
 
 # ---- sampling rules ------------------------------------------------------------------------------------------------------------------------------------
@@ -996,29 +1010,27 @@ def process_logits(logits: torch.Tensor, rules: torch.Tensor, out: Optional[torc
     rules f32 [R, 4]: repetition, presence, frequency, temperature.  hist int32 [total] with hist_start int32 [R + 1] and hist_prompt int32 [R] (how many of a
     row's ids are its prompt); bias_ids int32, bias_vals f32 with bias_start int32 [R + 1]; mask int32 [R, ceil(V / 32)], bit v % 32 of word v / 32 set: allowed."""
     out = logits if out is None else out
-    if logits.dim() != 2 or logits.stride(1) != 1 or logits.dtype != torch.float32 or out.dim() != 2 or out.stride(1) != 1 or out.dtype != torch.float32 or out.shape != logits.shape:
-        raise ValueError(f"process_logits: row-major float32 logits and results of one shape, not {logits.dtype} {tuple(logits.shape)} and {out.dtype} {tuple(out.shape)}")
-    R, V = logits.shape
-    ld = lambda t: max(t.stride(0), V) if R == 1 else t.stride(0)
-
-    def vec(name, t, dtype, n):
+    shape, lx, lo = logits.shape, logits.stride(), out.stride()
+    if len(shape) != 2 or out.shape != shape or lx[1] != 1 or lo[1] != 1 or logits.dtype != torch.float32 or out.dtype != torch.float32:
+        raise ValueError(f"process_logits: row-major float32 logits and results of one shape, not {logits.dtype} {tuple(shape)} and {out.dtype} {tuple(out.shape)}")
+    R, V = shape
+    words = (V + 31) // 32
+    i32, f32 = torch.int32, torch.float32
+    for name, t, dtype, n in (("rules", rules, f32, 4 * R), ("hist", hist, i32, None), ("hist_start", hist_start, i32, R + 1), ("hist_prompt", hist_prompt, i32, R),
+                              ("bias_start", bias_start, i32, R + 1), ("bias_ids", bias_ids, i32, None), ("bias_vals", bias_vals, f32, bias_ids.numel() if bias_ids is not None else None)):
         if t is not None and (t.dtype != dtype or not t.is_contiguous() or (n is not None and t.numel() != n)):
             raise ValueError(f"process_logits: {name} is contiguous {dtype}{'' if n is None else f' of {n} values'}, not {t.dtype} {tuple(t.shape)}")
-    vec("rules", rules, torch.float32, 4 * R)
-    vec("hist", hist, torch.int32, None)
-    vec("hist_start", hist_start, torch.int32, R + 1)
-    vec("hist_prompt", hist_prompt, torch.int32, R)
-    vec("bias_start", bias_start, torch.int32, R + 1)
-    vec("bias_ids", bias_ids, torch.int32, None)
-    vec("bias_vals", bias_vals, torch.float32, bias_ids.numel() if bias_ids is not None else None)
-    if mask is not None and (mask.dim() != 2 or mask.dtype != torch.int32 or mask.stride(1) != 1 or mask.shape[0] != R or mask.shape[1] < (V + 31) // 32):
-        raise ValueError(f"process_logits: the mask is row-major int32 [{R}, {(V + 31) // 32}], not {mask.dtype} {tuple(mask.shape)}")
+    lm = 0
+    if mask is not None:
+        lm = mask.stride()
+        if len(lm) != 2 or lm[1] != 1 or mask.dtype != i32 or mask.shape[0] != R or mask.shape[1] < words:
+            raise ValueError(f"process_logits: the mask is row-major int32 [{R}, {words}], not {mask.dtype} {tuple(mask.shape)}")
+        lm = max(lm[0], words) if R == 1 else lm[0]
     if hist is not None and hist.numel() == 0:      # histories without a token
         hist = hist_start = hist_prompt = None
     if bias_ids is not None and bias_ids.numel() == 0:
         bias_ids = bias_start = bias_vals = None
-    words = (V + 31) // 32
     _on_device("process_logits", lib().b200seq_process_logits,
-               (_p(logits), ld(logits), R, V, _p(rules), _p(hist), _p(hist_start), _p(hist_prompt), _p(bias_start), _p(bias_ids), _p(bias_vals),
-                _p(mask), max(mask.stride(0), words) if mask is not None else 0, _p(out), ld(out)), logits, rules, out, hist, hist_start, hist_prompt, bias_start, bias_ids, bias_vals, mask)
+               (logits.data_ptr(), lx[0] if R > 1 else V, R, V, rules.data_ptr(), _p(hist), _p(hist_start), _p(hist_prompt), _p(bias_start), _p(bias_ids), _p(bias_vals),
+                _p(mask), lm, out.data_ptr(), lo[0] if R > 1 else V), logits, rules, out, hist, hist_start, hist_prompt, bias_start, bias_ids, bias_vals, mask)
     return out

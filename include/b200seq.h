@@ -512,9 +512,9 @@ int b200seq_attn_kv4(const float* proj, int64_t ld, const b200seq_step* st, cons
                      float* scratch, size_t scratch_floats, void* stream);
 size_t b200seq_attn_kv4_scratch_floats(const b200seq_step* st, const b200seq_attn_desc* d);
 
-/* Page to[i] of every pool becomes a copy of its page from[i], i < n.  pools, page_bytes, from, to: HOST arrays, read during the call; every pool has `pages` pages.
+/* Page pairs[i][1] of every pool becomes a copy of its page pairs[i][0], i < n.  pools, page_bytes, pairs: HOST arrays, read during the call; every pool has `pages` pages.
  * A page may be read by several pairs, but not written twice and not both read and written (B200SEQ_ERR_INVALID_ARG, nothing is copied). */
-int b200seq_copy_pages(void* const* pools, const int64_t* page_bytes, int npools, int pages, const int32_t* from, const int32_t* to, int n, void* stream);
+int b200seq_copy_pages(void* const* pools, const int64_t* page_bytes, int npools, int pages, const int32_t* pairs, int n, void* stream);
 
 /* Sampling rules on rows of logits, out[r] from x[r] (f32 [R, V], out may be x), rules[r] = (repetition, presence, frequency, temperature), 16-byte aligned, in this order:
  *   a token of the row's history (hist[hist_start[r] .. hist_start[r + 1])): x > 0 ? x / repetition : x * repetition

@@ -108,13 +108,13 @@ def test_tensors_that_are_refused():
 
 def test_copies_that_are_refused():
     ptrs, size = (C.c_void_p * 1)(P), (C.c_int64 * 1)(64)
-    call = lambda pairs, pages=6: entry("copy_pages")(ptrs, size, 1, pages, (C.c_int32 * len(pairs))(*[a for a, _ in pairs]), (C.c_int32 * len(pairs))(*[b for _, b in pairs]), len(pairs), None)
+    call = lambda pairs, pages=6: entry("copy_pages")(ptrs, size, 1, pages, (C.c_int32 * (2 * len(pairs)))(*[x for p in pairs for x in p]), len(pairs), None)
     for pairs in ([(0, 1), (2, 1)], [(0, 1), (1, 2)], [(1, 2), (0, 1)], [(3, 3)], [(0, 6)], [(6, 0)], [(-1, 2)], [(2, -1)]):
         assert call(pairs) == -1, pairs
     assert call([(0, 0)], 0) == -1
-    assert entry("copy_pages")(ptrs, size, 1, 6, None, None, 0, None) == 0
-    assert entry("copy_pages")(None, None, 0, 6, None, None, 0, None) == 0
-    assert entry("copy_pages")((C.c_void_p * 1)(None), size, 1, 6, None, None, 0, None) == -1
+    assert entry("copy_pages")(ptrs, size, 1, 6, None, 0, None) == 0
+    assert entry("copy_pages")(None, None, 0, 6, None, 0, None) == 0
+    assert entry("copy_pages")((C.c_void_p * 1)(None), size, 1, 6, None, 0, None) == -1
     with pytest.raises(ValueError):
         ops.copy_pages([torch.zeros(6, 4)], [(0, 1)])
     with pytest.raises(ValueError):
