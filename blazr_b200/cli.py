@@ -1,6 +1,7 @@
 """Command line of the layer-list serving path:
 
-    python -m blazr_b200 generate --model DIR --prompt 1,2,3 [--prompt ...] [--max-new N] [--temperature T] [--top-k K] [--top-p P]
+    python -m blazr_b200 generate --model DIR --prompt 1,2,3 [--prompt ...] [--max-new N] [--temperature T] [--top-k K] [--top-p P] [--samples N]
+                                  [--repetition-penalty R] [--presence-penalty P] [--frequency-penalty F] [--logit-bias 7:-2.5,9:1] [--kv-bits 4]
     python -m blazr_b200 trace    --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N     (also bin/trace_run)
 
 `trace` replays externally scheduled steps through the engine: one JSON object per line on standard input,
@@ -29,7 +30,7 @@ def cmd_trace(a) -> int:
     from . import seqops
     from .engine import Engine
     model = _load(a.model, a.dtype)
-    eng = Engine(model, max_tokens=a.max_tokens, max_seqs=a.max_seqs, block_size=a.block_size)
+    eng = Engine(model, max_tokens=a.max_tokens, max_seqs=a.max_seqs, block_size=a.block_size, kv_bits=a.kv_bits)
     os.makedirs(a.out, exist_ok=True)
     for line in sys.stdin:
         line = line.strip()
@@ -55,11 +56,15 @@ def cmd_generate(a) -> int:
     from .engine import Engine, SamplingParams
     model = _load(a.model, a.dtype)
     prompts = [[int(t) for t in p.split(",") if t.strip()] for p in a.prompt]
-    need = sum(-(-(len(p) + a.max_new) // a.block_size) * a.block_size for p in prompts[:a.max_seqs]) if a.max_tokens <= 0 else a.max_tokens
-    eng = Engine(model, max_tokens=need, max_seqs=a.max_seqs, block_size=a.block_size)
-    outs = eng.generate(prompts, SamplingParams(temperature=a.temperature, top_k=a.top_k, top_p=a.top_p, seed=a.seed, max_new_tokens=a.max_new))
+    need = sum(-(-(len(p) + a.max_new) // a.block_size) * a.block_size for p in prompts[:a.max_seqs]) * a.samples if a.max_tokens <= 0 else a.max_tokens
+    bias = dict((int(t), float(v)) for t, v in (e.split(":") for e in a.logit_bias.split(",") if e.strip())) if a.logit_bias else None
+    eng = Engine(model, max_tokens=need, max_seqs=max(a.max_seqs, a.samples), block_size=a.block_size, kv_bits=a.kv_bits)
+    outs = eng.generate(prompts, SamplingParams(temperature=a.temperature, top_k=a.top_k, top_p=a.top_p, seed=a.seed, max_new_tokens=a.max_new, n=a.samples,
+                                                repetition_penalty=a.repetition_penalty, presence_penalty=a.presence_penalty, frequency_penalty=a.frequency_penalty,
+                                                logit_bias=bias))
     for p, o in zip(prompts, outs):
-        print(json.dumps({"prompt": p, "tokens": o}))
+        for tokens in o if a.samples > 1 else [o]:
+            print(json.dumps({"prompt": p, "tokens": tokens}))
     return 0
 
 
@@ -72,6 +77,7 @@ def main(argv=None) -> int:
         p.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
         p.add_argument("--max-seqs", type=int, default=4, help="state slots: most requests live at a time")
         p.add_argument("--block-size", type=int, default=16, help="tokens per KV page")
+        p.add_argument("--kv-bits", type=int, default=32, choices=[4, 32], help="bits of a cached key or value")
         if name == "trace":
             p.add_argument("--out", required=True)
             p.add_argument("--max-tokens", type=int, required=True, help="tokens the KV pool holds")
@@ -83,5 +89,10 @@ def main(argv=None) -> int:
             p.add_argument("--top-k", type=int, default=0)
             p.add_argument("--top-p", type=float, default=1.0)
             p.add_argument("--seed", type=int, default=0)
+            p.add_argument("--samples", type=int, default=1, help="samples of every prompt, which is run once")
+            p.add_argument("--repetition-penalty", type=float, default=1.0)
+            p.add_argument("--presence-penalty", type=float, default=0.0)
+            p.add_argument("--frequency-penalty", type=float, default=0.0)
+            p.add_argument("--logit-bias", default="", help="token:value, with commas")
     a = ap.parse_args(argv)
     return cmd_trace(a) if a.cmd == "trace" else cmd_generate(a)

@@ -290,6 +290,11 @@ def loop_runs(n: int, start: int = 0, stop: int = 0, times: int = 0) -> list:
     return runs + [(i, None, False) for i in range(stop, n)]
 
 
+# buffers of a layer whose first dimension counts KV pages / state slots
+PAGED = ("kpool", "vpool", "kpooled", "vpooled")
+SLOTTED = ("canon1_state", "canon2_state", "conv_state", "ssm_state", "shift_state", "ret_state", "rec_state", "delta_state", "scan_state")
+
+
 class _Rows:
     """rows of a layer's stacked input projection, with the bias of every row (zero where a projection has none)"""
 
@@ -604,6 +609,7 @@ class LayeredModel:
                 self.weight_bytes += (L["w_gu"].numel() + L["w_down"].numel()) * 2
             self.layers.append(L)
         self.max_seqs = self.max_blocks = self.block_size = 0
+        self.kv_bits = 32
         self._ws: Dict[int, _Workspace] = {}
         self._graphs: Dict[int, object] = {}
         self.use_graphs = True
@@ -1109,9 +1115,34 @@ class LayeredModel:
             self.max_ff_proj = max(self.max_ff_proj, 2 * f.ff)
 
     # ---- cache and state -------------------------------------------------------------------------------------------------------
-    def allocate(self, num_blocks: int, block_size: int, max_seqs: int, max_seq_tokens: int) -> None:
-        """KV pools for `num_blocks` pages, state for `max_seqs` slots; block tables hold up to max_seq_tokens positions"""
+    def attention_specs(self) -> list:
+        """the layers' attentions over KV pages, latent ones too"""
+        specs = [L["spec"].mixer.left if L["spec"].kind == "two_branch" else L["spec"].mixer for L in self.layers if L["spec"].kind in ("attention", "two_branch", "latent_attention")]
+        return [m for m in specs if isinstance(m, (AttentionSpec, LatentAttentionSpec))]
+
+    def pooled_sizes(self) -> tuple:
+        """sizes of the pooled blocks that layers keep beside their pages"""
+        return tuple(sorted({m.pool for m in self.attention_specs() if isinstance(m, AttentionSpec) and m.pool > 0}))
+
+    def _kv_pools(self, num_blocks: int, block_size: int, key_heads: int, dim: int, value_heads: int, vdim: int) -> tuple:
+        n = max(1, num_blocks)
+        if self.kv_bits == 4:
+            return seqops.kv4_pool(n, block_size, key_heads, dim, self.dev), seqops.kv4_pool(n, block_size, value_heads, vdim, self.dev)
+        f32 = dict(dtype=torch.float32, device=self.dev)
+        return torch.zeros((n, block_size, key_heads, dim), **f32), torch.zeros((n, block_size, value_heads, vdim), **f32)
+
+    def allocate(self, num_blocks: int, block_size: int, max_seqs: int, max_seq_tokens: int, kv_bits: int = 32) -> None:
+        """KV pools for `num_blocks` pages, state for `max_seqs` slots; block tables hold up to max_seq_tokens positions.  kv_bits: 32, or 4 (plain attention layers
+        with heads of up to 128 values: keys and values are held as 4-bit codes, 0.625 bytes a value)"""
         dev, cfg = self.dev, self.cfg
+        if kv_bits not in (4, 32):
+            raise ValueError(f"a KV cache holds 4 or 32 bits a value, not {kv_bits}")
+        if kv_bits == 4:
+            for m in self.attention_specs():
+                if isinstance(m, LatentAttentionSpec) or m.pool > 0 or max(m.dim, m.vdim) > seqops.KV4_MAX_DIM:
+                    raise ValueError("a 4-bit KV cache holds plain keys and values of heads of up to "
+                                     f"{seqops.KV4_MAX_DIM} values: not latents, not pooled blocks, not {max(getattr(m, 'dim', 0), m.vdim)} values")
+        self.kv_bits = kv_bits
         f32 = dict(dtype=torch.float32, device=dev)
         self.block_size, self.max_seqs = block_size, max_seqs
         self.max_blocks = max(1, -(-max_seq_tokens // block_size))
@@ -1132,8 +1163,7 @@ class LayeredModel:
                 att = m if ls.kind == "attention" else m.left
                 maps = 2 if att.diff is not None else 1
                 if att.kv_from is None:      # a layer that reads another layer's keys and values has no pool (bound below, when all pools exist)
-                    L["kpool"] = torch.zeros((max(1, num_blocks), block_size, att.kv_heads * maps, att.dim), **f32)
-                    L["vpool"] = torch.zeros((max(1, num_blocks), block_size, att.kv_heads, att.vdim), **f32)
+                    L["kpool"], L["vpool"] = self._kv_pools(num_blocks, block_size, att.kv_heads * maps, att.dim, att.kv_heads, att.vdim)
                 right = None if ls.kind == "attention" else m.right
                 if isinstance(right, MinGruSpec):
                     L["rec_state"] = torch.zeros((max_seqs, right.width), **f32)
@@ -1143,8 +1173,7 @@ class LayeredModel:
                 continue
             if cfg.layout == "parallel" and ls.kind == "two_branch":
                 att, right = m.left, m.right
-                L["kpool"] = torch.zeros((max(1, num_blocks), block_size, att.kv_heads, att.dim), **f32)
-                L["vpool"] = torch.zeros((max(1, num_blocks), block_size, att.kv_heads, att.vdim), **f32)
+                L["kpool"], L["vpool"] = self._kv_pools(num_blocks, block_size, att.kv_heads, att.dim, att.kv_heads, att.vdim)
                 L["scan_state"] = torch.zeros((max_seqs, right.inner, right.state), **f32)
                 L["conv_state"] = torch.zeros((max_seqs, max(right.conv - 1, 1), right.inner), **f32)
                 continue
@@ -1155,8 +1184,7 @@ class LayeredModel:
                 L["desc_x"] = seqops.expanded_attn_desc(m.heads, m.dim, m.rot_dim, m.vdim, m.scale, L["kpool"].view(-1, m.kv_rank + m.rot_dim)[:, m.kv_rank:],
                                                         gated=m.gated, sink=L["sink"])
             elif ls.kind == "attention":
-                L["kpool"] = torch.zeros((max(1, num_blocks), block_size, m.kv_heads, m.dim), **f32)
-                L["vpool"] = torch.zeros((max(1, num_blocks), block_size, m.kv_heads, m.vdim), **f32)
+                L["kpool"], L["vpool"] = self._kv_pools(num_blocks, block_size, m.kv_heads, m.dim, m.kv_heads, m.vdim)
                 if m.pool > 0:      # mean key / value of every block of `pool` positions, kept in the page of the block's first position
                     per_page = -(-block_size // m.pool)
                     L["kpooled"] = torch.zeros((max(1, num_blocks), per_page, m.kv_heads, m.dim), **f32)
@@ -1222,8 +1250,21 @@ class LayeredModel:
         return max([0] + [seqops.scan_scratch_floats(cap, self.max_seqs, L["spec"].mixer.right.inner, L["spec"].mixer.right.state) for L in self.layers if "scan" in L])
 
     def cache_bytes(self) -> int:
-        keys = ("canon1_state", "canon2_state", "kpool", "vpool", "kpooled", "vpooled", "conv_state", "ssm_state", "shift_state", "ret_state", "rec_state", "delta_state", "scan_state")
-        return sum(L[k].numel() * 4 for L in self.layers for k in keys if k in L)
+        return sum(L[k].nbytes for L in self.layers for k in PAGED + SLOTTED if k in L)
+
+    def has_state(self) -> bool:
+        """whether requests carry state outside their KV pages"""
+        return any(k in L for L in self.layers for k in SLOTTED)
+
+    def copy_pages(self, pairs) -> None:
+        """KV pages `to` <- `from` in every layer, for pairs (from, to)"""
+        if pairs:
+            seqops.copy_pages([L[k] for L in self.layers for k in PAGED if k in L], pairs)
+
+    def copy_slots(self, pairs) -> None:
+        """recurrent state of slots `to` <- `from` in every layer, for pairs (from, to)"""
+        if pairs:
+            seqops.copy_pages([L[k] for L in self.layers for k in SLOTTED if k in L], pairs)
 
     def _ctx_buffers(self, rows: int):
         """gathered latents (activation type) and the per-head keys | values projected out of them (f32) for `rows` context positions;
@@ -1741,18 +1782,32 @@ class LayeredModel:
         seqops.delta(proj, st, d, wz, L["delta_state"], o, ws.scratch)
         seqops.linear(o, L["w_o"], y)
 
+    def _attn_prep(self, L, st, proj: torch.Tensor) -> None:
+        """queries normed and rotated in the projection rows, keys and values into the layer's pages"""
+        if self.kv_bits == 4:
+            seqops.attn_prep_kv4(proj, st, L["desc"], L.get("kpool"), L.get("vpool"))
+        else:
+            seqops.attn_prep_ex(proj, st, L["desc"], L.get("kpool"), L.get("vpool"), L.get("kpooled"), L.get("vpooled"))
+
+    def _attend(self, L, src, ws: _Workspace, st, proj: torch.Tensor, o: torch.Tensor) -> None:
+        """attention of the prepared rows over the pages of layer `src`"""
+        if self.kv_bits == 4:
+            seqops.attn_kv4(proj, st, L["desc"], src["kpool"], src["vpool"], o)
+        else:
+            seqops.attn_ex(proj, st, L["desc"], src["kpool"], src["vpool"], o, ws.scratch, src.get("kpooled"), src.get("vpooled"))
+
     def _attention_out(self, L, m: AttentionSpec, ws: _Workspace, st, T: int, proj: torch.Tensor, y: torch.Tensor) -> None:
         """attention (prepared from the stacked projection `proj`) over the layer's own pool or the pool of the layer whose keys and values it shares"""
         src = L.get("kv_src", L)
-        seqops.attn_prep_ex(proj, st, L["desc"], L.get("kpool"), L.get("vpool"))
+        self._attn_prep(L, st, proj)
         H, V = m.heads, m.vdim
         o = ws.inner_a.view(-1)[:T * H * V].view(T, H * V)
         if m.diff is not None:      # two maps per head as 2 H plain heads, f32; then o = unit_rms(a1 - lambda a2) * (1 - diff)
             a12 = ws.inner_f.view(-1)[:T * 2 * H * V].view(T, 2 * H * V)
-            seqops.attn_ex(proj, st, L["desc"], src["kpool"], src["vpool"], a12, ws.scratch)
+            self._attend(L, src, ws, st, proj, a12)
             seqops.diff_combine(a12, H, m.kv_heads, V, L["lambda"], 1.0 - m.diff, self.cfg.eps, o)
         else:
-            seqops.attn_ex(proj, st, L["desc"], src["kpool"], src["vpool"], o, ws.scratch)
+            self._attend(L, src, ws, st, proj, o)
         seqops.linear(o, L["w_o"], y)
 
     def _recurrent_branch(self, L, r, ws: _Workspace, st, T: int, proj: torch.Tensor, y: torch.Tensor) -> None:
@@ -1847,9 +1902,9 @@ class LayeredModel:
         n_in = L["w_in"].shape[0]
         qkvg = ws.proj[:T, :n_in]
         seqops.linear(a, L["w_in"], qkvg)
-        seqops.attn_prep_ex(qkvg, st, L["desc"], L["kpool"], L["vpool"], L.get("kpooled"), L.get("vpooled"))
+        self._attn_prep(L, st, qkvg)
         o = ws.inner_a.view(-1)[:T * m.heads * m.vdim].view(T, m.heads * m.vdim)
-        seqops.attn_ex(qkvg, st, L["desc"], L["kpool"], L["vpool"], o, ws.scratch, L.get("kpooled"), L.get("vpooled"))
+        self._attend(L, L, ws, st, qkvg, o)
         seqops.linear(o, L["w_o"], y)
 
     def _ssm(self, L, m: SsmSpec, ws: _Workspace, st, T: int, a: torch.Tensor, y: torch.Tensor) -> None:
