@@ -544,14 +544,19 @@ struct Plan {
     int64_t tiles;
     int heads, cluster, parts;
 };
+// the most keys a token can see
+int64_t most_keys(const b200seq_step& st, const b200seq_attn_desc& d, int tokens) {
+    int64_t keys = (int64_t)st.max_blocks * st.block_size;
+    if (d.chunk > 0 && d.chunk < keys) keys = d.chunk;
+    if (d.window > 0 && (int64_t)d.window + d.keep_first + tokens < keys) keys = (int64_t)d.window + d.keep_first + tokens;
+    return keys;
+}
 Plan plan(const b200seq_step& st, const b200seq_attn_desc& d) {
     Plan p;
     const int R = d.H / d.G, Rb = R < ROWS ? R : ROWS, QT = ROWS / Rb;
     p.heads = d.G * ((R + Rb - 1) / Rb);
     p.tiles = st.T == st.B ? st.T : ((int64_t)st.T + QT - 1) / QT + st.B;
-    int64_t keys = (int64_t)st.max_blocks * st.block_size;
-    if (d.chunk > 0 && d.chunk < keys) keys = d.chunk;
-    if (d.window > 0 && (int64_t)d.window + d.keep_first + QT < keys) keys = (int64_t)d.window + d.keep_first + QT;
+    const int64_t keys = most_keys(st, d, QT);
     int64_t want = 2 * 148 / (p.tiles * p.heads), most = keys / (4 * KT);
     want = want < most ? want : most;
     p.cluster = want >= 8 ? 8 : (want >= 4 ? 4 : (want >= 2 ? 2 : 1));
@@ -569,8 +574,12 @@ extern "C" {
 
 size_t b200seq_attn_kv4_scratch_floats(const b200seq_step* st, const b200seq_attn_desc* d) {
     if (!st || !d || st->T < 1 || st->B < 1 || st->block_size < 1 || st->max_blocks < 1 || d->H < 1 || d->G < 1 || d->H % d->G || d->V < 1) return 0;
-    const Plan p = plan(*st, *d);
-    return p.parts > 1 ? (size_t)st->T * d->H * p.parts * (d->V + 4) : 0;
+    int parts = plan(*st, *d).parts;
+    if (attn4_tc_takes(*st, d->H, d->G, d->D, d->V)) {
+        const int tc = attn4_tc_plan(*st, d->H, d->G, d->D, d->V, most_keys(*st, *d, 0)).parts;
+        parts = tc > parts ? tc : parts;
+    }
+    return parts > 1 ? (size_t)st->T * d->H * parts * (d->V + 4) : 0;
 }
 
 int b200seq_attn_kv4(const float* proj, int64_t ld, const b200seq_step* st, const b200seq_attn_desc* d, const void* kpool, const void* vpool, void* out, int out_dtype,
@@ -598,21 +607,35 @@ int b200seq_attn_kv4(const float* proj, int64_t ld, const b200seq_step* st, cons
     a.gate = d->gate ? d->gate : proj + (gated ? d->gate_col : 0), a.gld = d->gate ? d->gate_ld : ld, a.gated = gated, a.gate_elem = gated && d->gate_elem;
     a.vec = ((ld | d->q_col) & 3) == 0 && d->D % 8 == 0 && (reinterpret_cast<uintptr_t>(proj) & 15) == 0;
     a.softcap = d->softcap, a.out = out, a.out_dtype = out_dtype, a.err = error_flag_dev();
+    cudaStream_t cs = (cudaStream_t)stream;
+    if (d->H > 65535) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_kv4: too many heads");
+    auto merge = [&]() -> int {
+        if (a.parts > 1) {
+            launch_chained(attn4_merge_kernel, dim3(st->T, d->H), d->V <= 64 ? 64 : 128, 0, cs, a);
+            SEQ_LAUNCH_CHECK("attn_kv4 merge");
+        }
+        return 0;
+    };
+    if (a.vec && attn4_tc_takes(*st, d->H, d->G, d->D, d->V)) {
+        Attn4TcPlan tp = attn4_tc_plan(*st, d->H, d->G, d->D, d->V, most_keys(*st, *d, 0));
+        if (tp.parts > 1 && (!scratch || scratch_floats < (size_t)st->T * d->H * tp.parts * (d->V + 4))) tp.parts = 1;
+        if ((int64_t)d->G * tp.HB * tp.tiles > 0x7fffffff) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_kv4: too many heads or tokens");
+        a.part = scratch, a.parts = tp.parts;
+        const cudaError_t e = attn4_tc_launch(a, *st, tp, cs);
+        if (e != cudaSuccess) return cuda_status(e, "attn_kv4");
+        count_launch();
+        return merge();
+    }
     Plan p = plan(*st, *d);
     if (p.parts > 1 && (!scratch || scratch_floats < (size_t)st->T * d->H * p.parts * (d->V + 4))) p.parts = 1;
     a.cluster = p.cluster, a.parts = p.parts, a.part = scratch;
-    if (p.heads > 65535 || p.tiles * p.parts > 0x7fffffff || d->H > 65535) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_kv4: too many heads or tokens");
+    if (p.heads > 65535 || p.tiles * p.parts > 0x7fffffff) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_kv4: too many heads or tokens");
     const dim3 grid((unsigned)(p.tiles * p.parts), (unsigned)p.heads, (unsigned)p.cluster);
     const int nk = kv4_groups(d->D), nv = kv4_groups(d->V);
-    cudaStream_t cs = (cudaStream_t)stream;
     const cudaError_t e = nk == 1 ? launch_values<1>(nv, a, *st, grid, cs) : (nk == 2 ? launch_values<2>(nv, a, *st, grid, cs) : launch_values<4>(nv, a, *st, grid, cs));
     if (e != cudaSuccess) return cuda_status(e, "attn_kv4");
     count_launch();
-    if (p.parts > 1) {
-        launch_chained(attn4_merge_kernel, dim3(st->T, d->H), d->V <= 64 ? 64 : 128, 0, cs, a);
-        SEQ_LAUNCH_CHECK("attn_kv4 merge");
-    }
-    return 0;
+    return merge();
 }
 
 }  // extern "C"

@@ -50,4 +50,13 @@ struct RowSpan {
     __device__ __forceinline__ bool sees(int j) const { return j <= p && (j >= lo || j < keep); }
 };
 
+// Attend step of many rows on the tensor cores (seq_attn4_tc.cu)
+struct Attn4TcPlan {
+    int mt, Rb, HB, QT, parts;
+    int64_t tiles, real;
+};
+bool attn4_tc_takes(const b200seq_step& st, int H, int G, int D, int V);
+Attn4TcPlan attn4_tc_plan(const b200seq_step& st, int H, int G, int D, int V, int64_t keys);
+cudaError_t attn4_tc_launch(Attn4Args a, const b200seq_step& st, const Attn4TcPlan& p, cudaStream_t cs);
+
 }  // namespace b200seq

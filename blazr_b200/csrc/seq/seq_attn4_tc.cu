@@ -1,0 +1,572 @@
+// seq_attn4_tc.cu -- the attend step of prompt portions over KV pages held in 4 bits, on the 5th-generation tensor cores.
+//
+// What the cache holds enters the products as it is: s (u - 8) is an f16 number (seq_kv4.cuh), and the m + 8 s of a row's groups are eight more values of it, as high and low
+// f16 parts, against the group sums of q (keys), or as columns of their own (values).  Only q and the weights are rounded: q to two f16 parts (22 bits), the weights to
+// two where results are f32 and to one, 2^-12 of a weight, where they are bf16 (an eighth of the result's own rounding, and averaged over keys).  So scores are two products
+// and sums of values one or two where f32 operands (seq_attn_tc.cu) take six each.  The values of 64 keys leave the tensor core and are summed over the key tiles by
+// rounded adds in registers.
+//
+// One CTA works on MT tiles of 128 (token, query head) rows of one key head against tiles of 64 keys.  MT = 2 (heads up to 64): the two row tiles alternate, one
+// in the soft-max while the other is in the tensor pipe; MT = 1 (heads up to 128): consecutive key tiles alternate.
+//   warps 0 .. 4 MT - 1    soft-max: a thread owns a row -- its maximum, sum and value sums stay in registers, nothing is shuffled
+//   next 8 warps           loaders: four threads a key; codes and parameters from its page, a tile ahead, expanded into 128-byte swizzled rows.  Keys and values lie
+//                          alike, [key][value]: K-major for the scores, mn-major for the sums
+//   last 4 warps           the first of them issues the MMAs
+// The order of a row's values is that of its code words (pairs of fields that one AND takes out): q is permuted alike, results are put back in order as they are stored.
+// Registers (setmaxnreg, per thread): launched with 96 (MT = 2) or 128 (MT = 1) for all; soft-max 160 / 240, loaders 64 / 104, issuer 32 / 64: the sums
+// (2 * 160 + 2 * 64 + 32 = 5 * 96, 240 + 2 * 104 + 64 = 4 * 128) are what the block was launched with.
+// Every wait is bounded (tc_pair.cuh): one that runs out sets bit 1 of the library's error flags and the CTA leaves through the common exit.
+#include "seq_attn4.cuh"
+#include "tc_split.cuh"
+
+namespace b200seq {
+
+namespace {
+
+using namespace tcsplit;
+
+constexpr int KT = 64;                       // keys per tile
+constexpr int PLANE = KT * 128;              // bytes of one 64-key x 64-wide block
+constexpr int SLOT_COLS = 64;                // scores f32 [64], then the weights' parts [32] [32] in the same columns
+constexpr float LOG2E = 1.4426950408889634f;
+
+__host__ __device__ constexpr int blocks_of(int groups) { return (4 * groups + 9) / 8; }   // 16-byte pieces of a row: 4 a group, m + 8 s, zeros
+__host__ __device__ constexpr int columns_of(int groups) { return 32 * groups + 16; }
+
+__device__ __forceinline__ uint32_t h2(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
+__device__ __forceinline__ __half2 h2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+__device__ __forceinline__ uint32_t field_or(uint32_t x, uint32_t mask, uint32_t magic) {
+    uint32_t w;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(w) : "r"(x), "r"(mask), "r"(magic));
+    return w;
+}
+// a word's eight codes as eight f16 s (u - 8): pairs of fields (i, i + 4), i = 0 .. 3.  s: the steps of the word's low and high half.  A field in the mantissa of 64 takes
+// one multiply-add (-72 s is an f16 number), one in that of 1024 an add first.
+__device__ __forceinline__ void expand(uint32_t w, __half2 s, __half2 s72, uint32_t (&x)[4]) {
+    const __half2 off = __floats2half2_rn(-1032.f, -1032.f);
+    const uint32_t w8 = w >> 8;
+    x[0] = h2(__hmul2_rn(__hadd2_rn(h2(field_or(w, 0x000F000Fu, 0x64006400u)), off), s));
+    x[1] = h2(__hfma2(h2(field_or(w, 0x00F000F0u, 0x54005400u)), s, s72));
+    x[2] = h2(__hmul2_rn(__hadd2_rn(h2(field_or(w8, 0x000F000Fu, 0x64006400u)), off), s));
+    x[3] = h2(__hfma2(h2(field_or(w8, 0x00F000F0u, 0x54005400u)), s, s72));
+}
+// m + 8 s of two groups, as high and low f16 parts (the low one is what rounding the high one leaves: an f16 number)
+__device__ __forceinline__ void centres(__half2 s, __half2 m, uint32_t& high, uint32_t& low) {
+    const __half2 eight = __floats2half2_rn(8.f, 8.f), d = __hfma2(s, eight, m), t = __hsub2_rn(d, m);
+    high = h2(d), low = h2(__hadd2_rn(__hsub2_rn(m, __hsub2_rn(d, t)), __hfma2(s, eight, __hneg2(t))));
+}
+__device__ __forceinline__ void sts16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void ld8(uint32_t taddr, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+// place of value d of a row in the order of its code words
+__host__ __device__ constexpr int value_place(int d, int NV) {
+    const int g = d >> 5, r = (d >> 2) & 7, i = d & 3;
+    return NV == 1 ? (r >> 1) * 8 + 2 * i + (r & 1) : (g >> 1) * 64 + ((r & 1) * 4 + (r >> 1)) * 8 + 2 * i + (g & 1);
+}
+
+template <int N>
+struct Codes {
+    uint32_t w[N], p[N];
+};
+// a thread's quarter of a row's codes and the row's parameters
+template <int N>
+__device__ __forceinline__ void load_codes(Codes<N>& c, const uint8_t* pool, const Kv4Row& at, int quarter, bool in) {
+    const uint8_t* w = pool + at.codes + 4 * N * quarter;
+    const uint8_t* p = pool + at.params;
+    if (!in) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) c.w[i] = c.p[i] = 0;
+    } else if (N == 4) {
+        const uint4 a = *reinterpret_cast<const uint4*>(w), b = *reinterpret_cast<const uint4*>(p);
+        c.w[0] = a.x, c.w[1 % N] = a.y, c.w[2 % N] = a.z, c.w[3 % N] = a.w, c.p[0] = b.x, c.p[1 % N] = b.y, c.p[2 % N] = b.z, c.p[3 % N] = b.w;
+    } else if (N == 2) {
+        const uint2 a = *reinterpret_cast<const uint2*>(w), b = *reinterpret_cast<const uint2*>(p);
+        c.w[0] = a.x, c.w[1 % N] = a.y, c.p[0] = b.x, c.p[1 % N] = b.y;
+    } else {
+        c.w[0] = *reinterpret_cast<const uint32_t*>(w), c.p[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+}
+// into shared memory: piece i of row `key` lies at block i / 8, place (i % 8) ^ (key % 8)
+template <int N, bool KEY>
+__device__ __forceinline__ void put_codes(const Codes<N>& c, uint32_t at, int key, int quarter) {
+    const uint32_t row = at + key * 128;
+    auto piece = [&](int i) { return row + (i >> 3) * PLANE + (((i & 7) ^ (key & 7)) << 4); };
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        uint32_t x[4];
+        __half2 s;
+        int to;
+        if (KEY) {            // words [part][group]: word i is group i of part `quarter`
+            s = __low2half2(h2(c.p[i])), to = i * 4 + quarter;
+        } else if (N == 1) {  // two parts of the one group
+            s = __low2half2(h2(c.p[0])), to = quarter;
+        } else {              // 16-bit words [part][group]: word i is two groups of part 2 quarter + i / (N / 2)
+            const int gp = N == 4 ? i & 1 : 0, r = N == 4 ? i >> 1 : i;
+            s = __lows2half2(h2(c.p[2 * gp]), h2(c.p[(2 * gp + 1) % N])), to = gp * 8 + r * 4 + quarter;
+        }
+        expand(c.w[i], s, __hmul2_rn(s, __floats2half2_rn(-72.f, -72.f)), x);
+        sts16(piece(to), x[0], x[1], x[2], x[3]);
+    }
+    if (quarter == 0) {       // groups 0 .. 3, high parts, then low parts
+        uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
+        const __half2 zero = __floats2half2_rn(0.f, 0.f);
+        if (N == 1) centres(__halves2half2(__low2half(h2(c.p[0])), __low2half(zero)), __halves2half2(__high2half(h2(c.p[0])), __low2half(zero)), hi[0], lo[0]);
+#pragma unroll
+        for (int i = 0; i + 1 < N; i += 2) centres(__lows2half2(h2(c.p[i]), h2(c.p[(i + 1) % N])), __highs2half2(h2(c.p[i]), h2(c.p[(i + 1) % N])), hi[i / 2], lo[i / 2]);
+        sts16(piece(4 * N), hi[0], hi[1], lo[0], lo[1]);
+    }
+}
+
+// MT row tiles; NK, NV groups of a key and a value; NP parts of a weight; CAP: scores are soft-capped
+template <int MT, int NK, int NV, int NP, bool CAP>
+__global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const __grid_constant__ Attn4Args a, const __grid_constant__ b200seq_step st) {
+    chain_enter();
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint32_t tmem_base;
+    __shared__ int abort_sh;
+    __shared__ __align__(8) uint64_t bars[16];
+    constexpr int KBYTES = blocks_of(NK) * PLANE, VBYTES = blocks_of(NV) * PLANE, STAGE = KBYTES + VBYTES, VM = 32 * NV, OCOLS = columns_of(NV), QP = columns_of(NK) / 2;
+    const uint32_t kv = (sa(smem_raw) + 1023u) & ~1023u;
+    const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // warp-uniform: the roles branch on it
+    const int D = a.D, V = a.V, H = a.H, G = a.G;
+    const uint32_t B0 = sa(bars);
+    const uint32_t k_full = B0, k_free = B0 + 16, v_full = B0 + 32, v_free = B0 + 48, s_full = B0 + 64, p_ready = B0 + 80, o_full = B0 + 96;
+    volatile int* ab = &abort_sh;
+    int e, t0, nq;
+    // the tiles with the most keys first, for all heads at once, so that the last CTAs to start are short
+    const int units = G * a.HB, n = (int)gridDim.x / units, ord = (int)blockIdx.x / units, unit = (int)blockIdx.x - ord * units;
+    int tile_no = n - 1 - ord;
+    if (a.chunk > 0 && a.chunk % a.QT == 0 && a.chunk / a.QT < n) {   // (in a step of chunks those are the last ones of every chunk)
+        const int per = a.chunk / a.QT, nc = (n + per - 1) / per, rem = n - (nc - 1) * per, longer = (per - rem) * (nc - 1);
+        if (ord < longer) tile_no = (ord % (nc - 1)) * per + per - 1 - ord / (nc - 1);
+        else tile_no = ((ord - longer) % nc) * per + rem - 1 - (ord - longer) / nc;
+    }
+    if (!attn_find_tile(st, tile_no, a.QT, e, t0, nq)) return;
+    const int g = unit / a.HB, hb = unit - g * a.HB, R = H / G;
+    const int h0 = g * R + hb * a.Rb, nh = min(a.Rb, R - hb * a.Rb);
+    const int split = blockIdx.z;
+    const int p0 = st.tok_pos[t0], hi = p0 + nq - 1, bs = st.block_size;
+    const int32_t* bt = st.block_table + (int64_t)e * st.max_blocks;
+    if (p0 < 0 || hi / bs >= st.max_blocks) {
+        if (threadIdx.x == 0) atomicOr(a.err, 1);
+        return;
+    }
+    const KeySpan<KT> span(a, p0, hi);
+    const int ntile = span.total > split ? (span.total - split + a.parts - 1) / a.parts : 0;   // tiles split, split + parts, ...
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            bar_init(k_full + 8 * i, 8), bar_init(k_free + 8 * i, 1), bar_init(v_full + 8 * i, 8), bar_init(v_free + 8 * i, 1);
+            bar_init(s_full + 8 * i, 1), bar_init(p_ready + 8 * i, 4), bar_init(o_full + 8 * i, 1);
+        }
+        bar_init(B0 + 112, 1);
+        abort_sh = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(sa(&tmem_base)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = tmem_base;
+    const uint32_t slot0 = tmem, o0 = tmem + 2 * SLOT_COLS, q0 = o0 + MT * OCOLS;   // columns: slots | value tiles | query parts
+
+    if (warp < 4 * MT) {
+        // ===================== soft-max: thread == row =====================
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MT == 2 ? 160 : 240));
+        const int m = warp >> 2, q = warp & 3;
+        const uint32_t lanes = (uint32_t)(q * 32) << 16;
+        const int r = m * 128 + q * 32 + lane;
+        const int tq = r / a.Rb, hr = r - tq * a.Rb;
+        const bool live = tq < nq && hr < nh;
+        int rlo = 0, rhi = 0x3fffffff;   // rows without a token see everything and are not stored
+        const int keep = a.window > 0 ? a.keep_first : 0;
+        float factor = a.scale;
+        if (live) {
+            const RowSpan rs(a, p0 + tq);
+            rlo = rs.lo, rhi = rs.p;
+            if (a.head_scale) factor *= a.head_scale[h0 + hr];
+        }
+        // soft-max in base 2 over raw scores: weight = 2^(c s - mb), mb = c max(s); the sign of the factor and a power of two go into the query.  With a soft cap the
+        // scores are scaled and capped first (CAP) and c is 1.
+        float c, zf;
+        {   // this row's query, in two parts and the order of the code words, and its group sums, to TMEM
+            const float* src = a.q + (int64_t)(t0 + tq) * a.ld + (int64_t)(h0 + hr) * D;
+            float top = 0.f;
+            for (int d = 0; live && d < D; d += 4) {
+                const float4 x = ld4(src + d);
+                top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
+            }
+            const int ex = (int)(__float_as_uint(top) >> 23);
+            const bool norm = ex >= 20 && ex < 255;     // the largest into [2^4, 2^5); a row of zeros, denormals or infinities as it is
+            const float up = copysignf(norm ? __uint_as_float((uint32_t)(254 - ex + 4) << 23) : 1.f, factor), down = norm ? __uint_as_float((uint32_t)(ex - 4) << 23) : 1.f;
+            zf = fmaxf(fabsf(factor) * down * (CAP ? 1.f : LOG2E), 1e-37f);
+            c = CAP ? 1.f : zf;
+            const uint32_t qa = q0 + lanes + m * 2 * QP;
+            uint32_t sh[8], sl[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sh[i] = sl[i] = 0;
+            float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+#pragma unroll 1
+                for (int c2 = 0; c2 < 4; c2 += 2) {
+                    uint32_t ph[8], pl[8];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int d = 32 * k + 8 * (c2 + u);
+                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+                        if (live && d < D) x = ld4(src + d), y = ld4(src + d + 4);     // (D a multiple of 8)
+                        const float f[8] = {x.x * up, x.y * up, x.z * up, x.w * up, y.x * up, y.y * up, y.z * up, y.w * up};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const __half2 h = __floats2half2_rn(f[i], f[i + 4]);
+                            const float2 b = __half22float2(h);
+                            ph[4 * u + i] = h2(h), pl[4 * u + i] = h2(__floats2half2_rn(f[i] - b.x, f[i + 4] - b.y));
+                            sums[k] += f[i] + f[i + 4];
+                        }
+                    }
+                    st8(qa + (4 * k + c2) * 4, ph), st8(qa + QP + (4 * k + c2) * 4, pl);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {   // the sums of q, against the high and the low parts of m + 8 s
+                const __half2 h = __floats2half2_rn(sums[2 * i], sums[2 * i + 1]);
+                const float2 b = __half22float2(h);
+                sh[i] = sh[2 + i] = h2(h), sl[i] = sl[2 + i] = h2(__floats2half2_rn(sums[2 * i] - b.x, sums[2 * i + 1] - b.y));
+            }
+            st8(qa + 16 * NK, sh), st8(qa + QP + 16 * NK, sl);
+            st_wait();
+            fence_before();
+        }
+        asm volatile("bar.sync 1, %0;" ::"n"((4 * MT + 1) * 32) : "memory");   // the queries are in place (with the MMA warp)
+        const uint64_t cc = pk(c, c);
+        float mx = -INFINITY, mb = -INFINITY, l = 0.f, rest[4] = {0.f, 0.f, 0.f, 0.f};
+        uint64_t acc[VM / 2];
+#pragma unroll
+        for (int i = 0; i < VM / 2; ++i) acc[i] = 0;
+        bool ok = true;
+        auto add_values = [&](int step) {   // acc += the value tile of a step
+            ok = bar_wait<false>(o_full + 8 * (step & 1), (step >> 1) & 1, ab);
+            if (!ok) return false;
+            fence_after();
+#pragma unroll
+            for (int i = 0; i < VM; i += 32) {
+                float o[32];
+                ld32(o0 + lanes + m * OCOLS + i, o);
+                ld_wait();
+#pragma unroll
+                for (int u = 0; u < 32; u += 2) acc[(i + u) >> 1] = add2(acc[(i + u) >> 1], pk(o[u], o[u + 1]));
+            }
+            float o[8];
+            ld8(o0 + lanes + m * OCOLS + VM, o);
+            ld_wait();
+#pragma unroll
+            for (int u = 0; u < 4; ++u) rest[u] += o[u] + o[4 + u];
+            fence_before();
+            return true;
+        };
+#pragma unroll 1
+        for (int j = 0; j < ntile && ok; ++j) {
+            const int step = j * MT + m, slot = step & 1;
+            const int k0 = span.key0(split + j * a.parts);
+            const int lo = rlo - k0, hi1 = rhi + 1 - k0, kp = keep - k0;   // visible keys of this row, relative to the tile: [lo, hi1) and those below kp
+            const bool whole = __all_sync(0xffffffffu, lo <= 0 && hi1 >= KT);
+            const uint32_t S = slot0 + lanes + slot * SLOT_COLS;
+            ok = bar_wait<false>(s_full + 8 * slot, (step >> 1) & 1, ab);
+            if (!ok) break;
+            fence_after();
+            float v[KT];
+            ld32(S, v);
+            ld32(S + 32, v + 32);
+            ld_wait();
+            if (CAP) {
+#pragma unroll
+                for (int i = 0; i < KT; ++i) v[i] = a.softcap * LOG2E * tanhf(v[i] * zf / a.softcap);
+            }
+            if (!whole) {
+                auto below = [](int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); };
+                const uint32_t s0 = below(hi1) & (~below(lo) | below(kp)), s1 = below(hi1 - 32) & (~below(lo - 32) | below(kp - 32));
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    v[i] = (s0 >> i) & 1u ? v[i] : -INFINITY;
+                    v[32 + i] = (s1 >> i) & 1u ? v[32 + i] : -INFINITY;
+                }
+            }
+            float m0 = fmaxf(v[0], v[1]), m1 = fmaxf(v[2], v[3]);
+#pragma unroll
+            for (int i = 4; i < KT; i += 4) m0 = fmaxf(m0, fmaxf(v[i], v[i + 1])), m1 = fmaxf(m1, fmaxf(v[i + 2], v[i + 3]));
+            mx = fmaxf(mx, fmaxf(m0, m1));
+            const float mbn = mx * c;
+            const float corr = mx == -INFINITY ? 1.f : ex2(mb - mbn);   // 0 at the first visible key
+            mb = mbn;
+            const float off = mx == -INFINITY ? 0.f : -mbn;
+            const uint64_t off2 = pk(off, off);
+            uint64_t sum = 0;
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4) {   // the weights' parts (over the scores, which are in registers)
+                uint32_t ph[8], pl[8];
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    float x, y;
+                    upk(fma2(pk(v[16 * q4 + i], v[16 * q4 + i + 1]), cc, off2), x, y);
+                    x = ex2(x), y = ex2(y);
+                    sum = add2(sum, pk(x, y));
+                    const __half2 h = __floats2half2_rn(x, y);
+                    ph[i >> 1] = h2(h);
+                    if (NP == 2) {
+                        const float2 b = __half22float2(h);
+                        pl[i >> 1] = h2(__floats2half2_rn(x - b.x, y - b.y));
+                    }
+                }
+                st8(S + 8 * q4, ph);
+                if (NP == 2) st8(S + 32 + 8 * q4, pl);
+            }
+            float sx, sy;
+            upk(sum, sx, sy);
+            l = fmaf(l, corr, sx + sy);
+            const uint64_t corr2 = pk(corr, corr);
+            const bool same = __all_sync(0xffffffffu, corr == 1.f);
+            // MT = 1: the value tile of the key tile before, whose product ran beside this soft-max
+            if (MT == 1 && j > 0 && !add_values(step - 1)) break;
+            if (!same) {
+#pragma unroll
+                for (int i = 0; i < VM / 2; ++i) acc[i] = mul2(acc[i], corr2);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) rest[i] *= corr;
+            }
+            st_wait();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) bar_arrive(p_ready + 8 * slot);
+            // MT = 2: this key tile's, while the next scores are made (the other row tile keeps the tensor pipe busy)
+            if (MT == 2 && !add_values(step)) break;
+        }
+        if (MT == 1 && ok && ntile > 0) add_values(ntile - 1);
+        if (ok && live) {
+            const int t = t0 + tq, h = h0 + hr;
+            float f = 1.f;
+            float* pp = nullptr;
+            if (a.parts == 1) {
+                float gate = 1.f, den = l, resc = 1.f;
+                if (a.gated && !a.gate_elem) gate = sigmoidf_acc(a.gate[(int64_t)t * a.gld + h]);
+                if (a.sink) {   // the sink's term, under the larger of the two maxima
+                    const float sk = a.sink[h] * LOG2E, top = fmaxf(mb, sk);
+                    resc = ex2(mb - top);
+                    den = fmaf(l, resc, ex2(sk - top));
+                }
+                f = gate * resc / den;
+            } else {
+                pp = a.part + (((int64_t)t * H + h) * a.parts + split) * (V + 4);
+                pp[0] = mb, pp[1] = l;
+            }
+            const bool wide = (V & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+#pragma unroll
+            for (int d = 0; d < VM; d += 4) {
+                if (d >= V) break;
+                float o[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float x, y;
+                    const int at = value_place(d + i, NV);
+                    upk(acc[at >> 1], x, y);
+                    o[i] = ((at & 1) ? y : x) + rest[d >> 5];
+                    if (!pp) o[i] *= f * (a.gate_elem && d + i < V ? sigmoidf_acc(a.gate[(int64_t)t * a.gld + (int64_t)h * V + d + i]) : 1.f);
+                }
+                if (pp) {
+                    for (int i = 0; i < 4 && d + i < V; ++i) pp[4 + d + i] = o[i];
+                } else if (wide) {
+                    store_act4(a.out, a.out_dtype, ((int64_t)t * H + h) * V + d, make_float4(o[0], o[1], o[2], o[3]));
+                } else {
+                    for (int i = 0; i < 4 && d + i < V; ++i) store_act(a.out, a.out_dtype, ((int64_t)t * H + h) * V + d + i, o[i]);
+                }
+            }
+        }
+    } else if (warp < 4 * MT + 8) {
+        // ===================== loaders: 256 threads, four a key =====================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MT == 2 ? 64 : 104));
+        // eight lanes store pieces of keys k and k + 4: their places in the swizzle fill a 128-byte line
+        const int lw = warp - 4 * MT, j8 = lane >> 2, key = lw * 8 + ((j8 & 1) << 2) + (j8 >> 1), quarter = lane & 3;
+        const int shift = (bs & (bs - 1)) == 0 ? 31 - __clz(bs) : -1;
+        const int Gv = G / a.vdiv, gv = g / a.vdiv;
+        if (quarter == 0) {   // the pieces behind m + 8 s stay zero
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const uint32_t kz = kv + s * STAGE + key * 128, vz = kz + KBYTES;
+                sts16(kz + ((4 * NK + 1) >> 3) * PLANE + ((((4 * NK + 1) & 7) ^ (key & 7)) << 4), 0, 0, 0, 0);
+                sts16(vz + ((4 * NV + 1) >> 3) * PLANE + ((((4 * NV + 1) & 7) ^ (key & 7)) << 4), 0, 0, 0, 0);
+            }
+        }
+        int page = 0, pos = 0;
+        auto lookup = [&](int j) {
+            pos = span.key0(split + j * a.parts) + key;
+            const int kp = min(pos, hi);
+            page = bt[shift >= 0 ? kp >> shift : kp / bs];
+        };
+        Codes<NK> kc;
+        Codes<NV> vc;
+        auto fetch = [&]() {   // the tile that was looked up
+            const bool in = pos <= hi;
+            const int kp = min(pos, hi), o = shift >= 0 ? kp & (bs - 1) : kp % bs;
+            load_codes<NK>(kc, a.kpool, kv4_row(page, o, bs, g, G, NK), quarter, in);
+            load_codes<NV>(vc, a.vpool, kv4_row(page, o, bs, gv, Gv, NV), quarter, in);
+        };
+        if (ntile > 0) {
+            lookup(0);
+            fetch();
+            if (ntile > 1) lookup(1);
+        }
+        bool ok = true;
+#pragma unroll 1
+        for (int j = 0; j < ntile && ok; ++j) {
+            const int s = j & 1;
+            const Codes<NK> k = kc;
+            const Codes<NV> v = vc;
+            if (j + 1 < ntile) {
+                fetch();
+                if (j + 2 < ntile) lookup(j + 2);
+            }
+            ok = bar_wait<false>(k_free + 8 * s, ((j >> 1) & 1) ^ 1, ab);
+            if (!ok) break;
+            put_codes<NK, true>(k, kv + s * STAGE, key, quarter);
+            async_fence();
+            __syncwarp();
+            if (lane == 0) bar_arrive(k_full + 8 * s);
+            ok = bar_wait<false>(v_free + 8 * s, ((j >> 1) & 1) ^ 1, ab);
+            if (!ok) break;
+            put_codes<NV, false>(v, kv + s * STAGE + KBYTES, key, quarter);
+            async_fence();
+            __syncwarp();
+            if (lane == 0) bar_arrive(v_full + 8 * s);
+        }
+    } else {
+        // ===================== MMA issuer =====================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MT == 2 ? 32 : 64));
+        if (warp == 4 * MT + 8) asm volatile("bar.sync 1, %0;" ::"n"((4 * MT + 1) * 32) : "memory");
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        if (warp == 4 * MT + 8 && elect()) {
+            fence_after();
+            constexpr uint32_t ids = (1u << 4) | ((uint32_t)(KT >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);                  // f16 x f16 -> f32
+            constexpr uint32_t ido = (1u << 4) | (1u << 16) | ((uint32_t)(OCOLS >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);   // B is mn-major
+            constexpr uint32_t O0 = 2 * SLOT_COLS, Q0 = O0 + MT * OCOLS;
+            const int steps = ntile * MT;
+            bool ok = true;
+            auto scores = [&](int step) {
+                const int j = step / MT, s = j & 1, slot = step & 1, m = MT == 2 ? slot : 0;
+                ok = bar_wait<false>(k_full + 8 * s, (j >> 1) & 1, ab);
+                if (!ok) return;
+                fence_after();
+                const uint64_t kb = desc_k128(kv + s * STAGE);
+                const uint32_t d = tm + slot * SLOT_COLS, qa = tm + Q0 + m * 2 * QP;
+#pragma unroll
+                for (int pr = 1; pr >= 0; --pr)          // the low parts of q first
+#pragma unroll
+                    for (int kk = 0; kk < 2 * NK + 1; ++kk)
+                        mma_ts(d, qa + pr * QP + kk * 8, kb + (uint64_t)(((kk >> 2) * PLANE) / 16 + 2 * (kk & 3)), ids, (pr < 1 || kk) ? 1u : 0u);
+                commit_one(s_full + 8 * slot);
+                if ((MT == 1 || slot == 1) && j + 2 < ntile) commit_one(k_free + 8 * s);   // (nobody waits for the last ones)
+            };
+            if (steps > 0) scores(0);
+#pragma unroll 1
+            for (int step = 0; step < steps && ok; ++step) {
+                if (step + 1 < steps) {
+                    if (step >= 1) ok = bar_wait<false>(o_full + 8 * ((step + 1) & 1), ((step - 1) >> 1) & 1, ab);   // the other slot's weights have been read
+                    if (ok) scores(step + 1);
+                    if (!ok) break;
+                }
+                const int j = step / MT, s = j & 1, slot = step & 1, m = MT == 2 ? slot : 0;
+                ok = bar_wait<false>(v_full + 8 * s, (j >> 1) & 1, ab) && bar_wait<false>(p_ready + 8 * slot, (step >> 1) & 1, ab);
+                if (!ok) break;
+                fence_after();
+                const uint64_t vb = desc_mn128(kv + s * STAGE + KBYTES, PLANE);
+                const uint32_t d = tm + O0 + m * OCOLS, pa = tm + slot * SLOT_COLS;
+#pragma unroll
+                for (int pr = NP - 1; pr >= 0; --pr)
+#pragma unroll
+                    for (int kk = 0; kk < KT / 16; ++kk)
+                        mma_ts(d, pa + 32 * pr + 8 * kk, vb + (uint64_t)(kk * 2048 / 16), ido, (pr < NP - 1 || kk) ? 1u : 0u);
+                commit_one(o_full + 8 * slot);
+                if ((MT == 1 || slot == 1) && j + 2 < ntile) commit_one(v_free + 8 * s);
+            }
+            if (!ok) {   // what was issued reads shared memory and TMEM: wait for it (bounded) before the CTA goes
+                commit_one(B0 + 112);
+                const unsigned long long t0_ = now_ns();
+                while (!bar_try<false>(B0 + 112, 0) && now_ns() - t0_ < WAIT_NS) {}
+            }
+        }
+        __syncwarp();
+    }
+    fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && abort_sh) atomicOr(a.err, 2);
+    if (warp == 0) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+template <int MT, int NK, int NV, int NP, bool CAP>
+cudaError_t run_one(const Attn4Args& a, const b200seq_step& st, dim3 grid, cudaStream_t cs) {
+    constexpr int need = 2 * (blocks_of(NK) + blocks_of(NV)) * PLANE + 1024, smem = need < 120 * 1024 ? 120 * 1024 : need;   // one CTA per SM: it takes all of TMEM
+    const auto kernel = attn4_tc_kernel<MT, NK, NV, NP, CAP>;
+    static bool ready[16] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 16 || !ready[dev]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        if (dev < 16) ready[dev] = true;
+    }
+    launch_chained(kernel, grid, (4 * MT + 12) * 32, smem, cs, a, st);
+    return cudaGetLastError();
+}
+template <int MT, int NK, int NV>
+cudaError_t run(const Attn4Args& a, const b200seq_step& st, dim3 grid, cudaStream_t cs) {
+    if (a.softcap > 0.f) return a.out_dtype == B200SEQ_F32 ? run_one<MT, NK, NV, 2, true>(a, st, grid, cs) : run_one<MT, NK, NV, 1, true>(a, st, grid, cs);
+    return a.out_dtype == B200SEQ_F32 ? run_one<MT, NK, NV, 2, false>(a, st, grid, cs) : run_one<MT, NK, NV, 1, false>(a, st, grid, cs);
+}
+
+}  // namespace
+
+// Steps whose portions fill a quarter of a row tile or more, with whole 16-byte pieces of queries and keys and values of as many groups.
+bool attn4_tc_takes(const b200seq_step& st, int H, int G, int D, int V) {
+    return st.T > 16 && (int64_t)st.T * (H / G) >= 32ll * st.B && D % 8 == 0 && kv4_groups(D) == kv4_groups(V);
+}
+
+// row tiles of 128 (256: two per CTA, heads of up to 64 and rows enough for all SMs)
+Attn4TcPlan attn4_tc_plan(const b200seq_step& st, int H, int G, int D, int V, int64_t keys) {
+    Attn4TcPlan p;
+    const int R = H / G;
+    p.mt = D <= 64 && V <= 64 && (int64_t)st.T * H >= 256ll * 148 ? 2 : 1;
+    const int RQ = 128 * p.mt;
+    p.Rb = R < RQ ? R : RQ, p.HB = (R + p.Rb - 1) / p.Rb, p.QT = RQ / p.Rb;
+    p.tiles = ((int64_t)st.T + p.QT - 1) / p.QT + st.B - (st.B == 1);   // upper bound of the step's query tiles (exact for one entry)
+    const int64_t each = (st.T + st.B - 1) / st.B;
+    p.real = (int64_t)st.B * ((each + p.QT - 1) / p.QT) * G * p.HB;      // row tiles, were all entries equally long
+    p.parts = 1;
+    if (2 * p.real <= 148) {   // too few tiles: deal the key tiles to several CTAs, at least four each
+        int64_t ns = 148 / p.real, most = keys / KT / 4;
+        ns = ns < most ? ns : most;
+        p.parts = (int)(ns > 32 ? 32 : (ns < 1 ? 1 : ns));
+    }
+    return p;
+}
+
+cudaError_t attn4_tc_launch(Attn4Args a, const b200seq_step& st, const Attn4TcPlan& p, cudaStream_t cs) {
+    a.Rb = p.Rb, a.HB = p.HB, a.QT = p.QT, a.parts = p.parts;
+    const dim3 grid((unsigned)(a.G * p.HB * p.tiles), 1, (unsigned)p.parts);
+    const int nk = kv4_groups(a.D);
+    if (p.mt == 2) return nk == 1 ? run<2, 1, 1>(a, st, grid, cs) : run<2, 2, 2>(a, st, grid, cs);
+    return nk == 1 ? run<1, 1, 1>(a, st, grid, cs) : (nk == 2 ? run<1, 2, 2>(a, st, grid, cs) : run<1, 4, 4>(a, st, grid, cs));
+}
+
+}  // namespace b200seq

@@ -246,6 +246,18 @@ CASES = [
     ([(130, 10)], 6, 2, 80, 48, dict(softcap=5.0), 16),
     ([(100, 0)], 4, 1, 32, 64, {}, 5),
     ([(33, 1500)], 32, 8, 128, 128, {}, 16),
+    # row tiles of 128 and of twice that on the tensor cores
+    ([(600, 0)], 64, 8, 64, 64, dict(window=130), 16),
+    ([(600, 5)], 64, 16, 32, 32, dict(chunk=128, sink=True), 32),
+    ([(450, 30), (150, 0)], 64, 1, 64, 64, dict(softcap=4.0, gated=True), 16),
+    ([(300, 0), (1, 70), (300, 17)], 64, 8, 40, 64, dict(window=64, keep_first=70, gated=True, gate_elem=True), 16),
+    ([(200, 100)], 8, 2, 128, 104, dict(window=70, keep_first=5, head_scale=True), 24),
+    ([(40, 700)], 8, 1, 32, 24, dict(scale=-0.3), 16),
+    ([(65, 190)], 12, 2, 88, 127, dict(sink=True), 5),
+    ([(40, 2000)], 8, 2, 64, 64, {}, 16),                                # keys dealt to several CTAs
+    ([(40, 2000), (35, 10)], 4, 1, 128, 128, dict(sink=True, gated=True), 16),
+    ([(20, 3000)], 96, 1, 64, 64, dict(softcap=6.0), 16),
+    ([(17, 63), (17, 64), (17, 47)], 256, 2, 32, 32, {}, 16),
 ]
 
 
