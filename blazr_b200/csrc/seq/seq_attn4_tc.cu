@@ -1,19 +1,23 @@
 // seq_attn4_tc.cu -- the attend step of prompt portions over KV pages held in 4 bits, on the 5th-generation tensor cores.
 //
 // What the cache holds enters the products as it is: s (u - 8) is an f16 number (seq_kv4.cuh), and the m + 8 s of a row's groups are eight more values of it, as high and low
-// f16 parts, against the group sums of q (keys), or as columns of their own (values).  Only q and the weights are rounded: q to two f16 parts (22 bits), the weights to
-// two where results are f32 and to one, 2^-12 of a weight, where they are bf16 (an eighth of the result's own rounding, and averaged over keys).  So scores are two products
-// and sums of values one or two where f32 operands (seq_attn_tc.cu) take six each.  The values of 64 keys leave the tensor core and are summed over the key tiles by
-// rounded adds in registers.
+// f16 parts, against the group sums of q (keys), or as columns of their own (values).  Only q and the weights are rounded: to two f16 parts (22 bits) each where results are
+// f32; to one (2^-12 of a value) where they are bf16, which is an eighth of what such a result itself and the bf16 activations behind q are rounded by.  So scores and sums
+// of values are one or two products each where f32 operands (seq_attn_tc.cu) take six.
 //
-// One CTA works on MT tiles of 128 (token, query head) rows of one key head against tiles of 64 keys.  MT = 2 (heads up to 64): the two row tiles alternate, one
-// in the soft-max while the other is in the tensor pipe; MT = 1 (heads up to 128): consecutive key tiles alternate.
-//   warps 0 .. 4 MT - 1    soft-max: a thread owns a row -- its maximum, sum and value sums stay in registers, nothing is shuffled
-//   next 8 warps           loaders: four threads a key; codes and parameters from its page, a tile ahead, expanded into 128-byte swizzled rows.  Keys and values lie
+// One CTA works on rows of 128 (token, query head) pairs of one key head against tiles of 64 keys.  A soft-max warp's thread owns a row; two groups of four such warps alternate,
+// one in the soft-max while the other's products are in the tensor pipe:
+//   MT = 2        two row tiles, a group each (heads up to 64, rows for all SMs)
+//   MT = 1, TG    one row tile, the groups take turns with the key tiles and are merged at the end
+//   MT = 1        one group, whose consecutive key tiles alternate (heads above 64 with f32 results: no registers for two)
+// The values of 64 keys leave the tensor core and are summed over the key tiles by rounded adds in registers; heads above 64 with bf16 results stay there (TA: the
+// sums' truncation, 2^-24 of them a product, is nothing to such a result) and are rescaled when a row's maximum has grown by 2^8.
+//   first 4 or 8 warps     soft-max: a row's maximum, sum and value sums stay in its thread's registers, nothing is shuffled
+//   next 8 warps           loaders, four for keys and four for values: codes and parameters from the pages, a tile ahead, expanded into 128-byte swizzled rows.  Both lie
 //                          alike, [key][value]: K-major for the scores, mn-major for the sums
 //   last 4 warps           the first of them issues the MMAs
 // The order of a row's values is that of its code words (pairs of fields that one AND takes out): q is permuted alike, results are put back in order as they are stored.
-// Registers (setmaxnreg, per thread): launched with 96 (MT = 2) or 128 (MT = 1) for all; soft-max 160 / 240, loaders 64 / 104, issuer 32 / 64: the sums
+// Registers (setmaxnreg, per thread): launched with 96 (two groups) or 128 (one) for all; soft-max 160 / 240, loaders 64 / 104, issuer 32 / 64: the sums
 // (2 * 160 + 2 * 64 + 32 = 5 * 96, 240 + 2 * 104 + 64 = 4 * 128) are what the block was launched with.
 // Every wait is bounded (tc_pair.cuh): one that runs out sets bit 1 of the library's error flags and the CTA leaves through the common exit.
 #include "seq_attn4.cuh"
@@ -29,6 +33,7 @@ constexpr int KT = 64;                       // keys per tile
 constexpr int PLANE = KT * 128;              // bytes of one 64-key x 64-wide block
 constexpr int SLOT_COLS = 64;                // scores f32 [64], then the weights' parts [32] [32] in the same columns
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr float SLACK = 8.f;
 
 __host__ __device__ constexpr int blocks_of(int groups) { return (4 * groups + 9) / 8; }   // 16-byte pieces of a row: 4 a group, m + 8 s, zeros
 __host__ __device__ constexpr int columns_of(int groups) { return 32 * groups + 16; }
@@ -124,16 +129,78 @@ __device__ __forceinline__ void put_codes(const Codes<N>& c, uint32_t at, int ke
     }
 }
 
-// MT row tiles; NK, NV groups of a key and a value; NP parts of a weight; CAP: scores are soft-capped
-template <int MT, int NK, int NV, int NP, bool CAP>
-__global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const __grid_constant__ Attn4Args a, const __grid_constant__ b200seq_step st) {
+// The key tiles of one pool, expanded into their stages: four warps, four threads a key, two keys a thread.  A tile's codes are asked for while the tile before it is
+// expanded, its pages a tile earlier.  stage: of tile 0 (tile 1's is `pitch` bytes on); full, free: the stages' barriers.
+template <int N, bool KEY>
+__device__ __forceinline__ void load_tiles(const uint8_t* pool, const int32_t* bt, int bs, int g, int G, const KeySpan<KT>& span, int split, int parts, int ntile, int hi, uint32_t stage,
+                                           uint32_t pitch, uint32_t full, uint32_t free, int lw, int lane, volatile int* ab) {
+    // eight lanes store pieces of keys k and k + 4: their places in the swizzle fill a 128-byte line
+    const int j8 = lane >> 2, key = lw * 16 + ((j8 & 1) << 2) + (j8 >> 1), quarter = lane & 3;
+    const int shift = (bs & (bs - 1)) == 0 ? 31 - __clz(bs) : -1;
+    if (quarter == 0) {   // the pieces behind m + 8 s stay zero
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int k = key + 8 * u;
+                sts16(stage + s * pitch + k * 128 + ((4 * N + 1) >> 3) * PLANE + ((((4 * N + 1) & 7) ^ (k & 7)) << 4), 0, 0, 0, 0);
+            }
+    }
+    int page[2], pos = 0;
+    auto lookup = [&](int j) {
+        pos = span.key0(split + j * parts) + key;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int kp = min(pos + 8 * u, hi);
+            page[u] = bt[shift >= 0 ? kp >> shift : kp / bs];
+        }
+    };
+    Codes<N> next[2];
+    auto fetch = [&]() {   // the tile that was looked up
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int kp = min(pos + 8 * u, hi);
+            load_codes<N>(next[u], pool, kv4_row(page[u], shift >= 0 ? kp & (bs - 1) : kp % bs, bs, g, G, N), quarter, pos + 8 * u <= hi);
+        }
+    };
+    if (ntile > 0) {
+        lookup(0);
+        fetch();
+        if (ntile > 1) lookup(1);
+    }
+#pragma unroll 1
+    for (int j = 0; j < ntile; ++j) {
+        const int s = j & 1;
+        const Codes<N> c0 = next[0], c1 = next[1];
+        if (j + 1 < ntile) {
+            fetch();
+            if (j + 2 < ntile) lookup(j + 2);
+        }
+        if (!bar_wait<false>(free + 8 * s, ((j >> 1) & 1) ^ 1, ab)) return;
+        put_codes<N, KEY>(c0, stage + s * pitch, key, quarter);
+        put_codes<N, KEY>(c1, stage + s * pitch, key + 8, quarter);
+        async_fence();
+        __syncwarp();
+        if (lane == 0) bar_arrive(full + 8 * s);
+    }
+}
+
+// MT row tiles; TG: two groups on one; NK, NV groups of 32 of a key and a value; NP parts of q and of a weight; CAP: scores are soft-capped
+template <int MT, bool TG, int NK, int NV, int NP, bool CAP>
+__global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_kernel(const __grid_constant__ Attn4Args a, const __grid_constant__ b200seq_step st) {
     chain_enter();
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint32_t tmem_base;
     __shared__ int abort_sh;
     __shared__ __align__(8) uint64_t bars[16];
+    __shared__ float row_factor[TG ? 128 : 1];
+    static_assert(!(TG && MT == 2) && (NV < 4 || (MT == 1 && (!TG || NP == 1))), "");
+    constexpr bool TA = TG && NV == 4;                 // value sums stay in TMEM
+    constexpr int GROUPS = TG ? 2 : MT, SW = 4 * GROUPS;   // soft-max warps
     constexpr int KBYTES = blocks_of(NK) * PLANE, VBYTES = blocks_of(NV) * PLANE, STAGE = KBYTES + VBYTES, VM = 32 * NV, OCOLS = columns_of(NV), QP = columns_of(NK) / 2;
+    constexpr int PITCH = 32 * (NK > NV ? NK : NV) + 4, RL = 8 * NK;   // floats of a staged row (16-byte pieces of a warp's rows in different banks); lanes a row of q takes
     const uint32_t kv = (sa(smem_raw) + 1023u) & ~1023u;
+    float* const stage_rows = reinterpret_cast<float*>(smem_raw + (kv - sa(smem_raw)) + 2 * STAGE);   // [128 MT][PITCH]: q on the way in, results on the way out
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;   // warp-uniform: the roles branch on it
     const int D = a.D, V = a.V, H = a.H, G = a.G;
     const uint32_t B0 = sa(bars);
@@ -160,9 +227,22 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
     }
     const KeySpan<KT> span(a, p0, hi);
     const int ntile = span.total > split ? (span.total - split + a.parts - 1) / a.parts : 0;   // tiles split, split + parts, ...
+    {   // the queries' rows on their way while the rest is set up: whole rows at a time (read by their threads they cost a 128-byte line a lane and load), by all warps
+        constexpr int WARPS = SW + 12, STEP = WARPS * (32 / RL);
+        const int d4 = 4 * (lane & (RL - 1));
+        const float* qrow = a.q + (int64_t)t0 * a.ld + (int64_t)h0 * D + d4;
+        const uint32_t to = sa(stage_rows) + d4 * 4;
+#pragma unroll 2
+        for (int row = warp * (32 / RL) + lane / RL; row < 128 * MT; row += STEP) {
+            const int rt = row / a.Rb, rh = row - rt * a.Rb;
+            const bool in = rt < nq && rh < nh && d4 < D;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + row * PITCH * 4), "l"(in ? qrow + (int64_t)rt * a.ld + rh * D : a.q), "r"(in ? 16 : 0)
+                         : "memory");                  // (nothing is read where there is no row; its place becomes zero)
+        }
+    }
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
-            bar_init(k_full + 8 * i, 8), bar_init(k_free + 8 * i, 1), bar_init(v_full + 8 * i, 8), bar_init(v_free + 8 * i, 1);
+            bar_init(k_full + 8 * i, 4), bar_init(k_free + 8 * i, 1), bar_init(v_full + 8 * i, 4), bar_init(v_free + 8 * i, 1);
             bar_init(s_full + 8 * i, 1), bar_init(p_ready + 8 * i, 4), bar_init(o_full + 8 * i, 1);
         }
         bar_init(B0 + 112, 1);
@@ -173,18 +253,19 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(sa(&tmem_base)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = tmem_base;
-    const uint32_t slot0 = tmem, o0 = tmem + 2 * SLOT_COLS, q0 = o0 + MT * OCOLS;   // columns: slots | value tiles | query parts
+    const uint32_t slot0 = tmem, o0 = tmem + 2 * SLOT_COLS, q0 = o0 + GROUPS * OCOLS;   // columns: slots | value tiles | query parts
 
-    if (warp < 4 * MT) {
+    if (warp < SW) {
         // ===================== soft-max: thread == row =====================
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(MT == 2 ? 160 : 240));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(GROUPS == 2 ? 160 : 240));
         const int m = warp >> 2, q = warp & 3;
         const uint32_t lanes = (uint32_t)(q * 32) << 16;
-        const int r = m * 128 + q * 32 + lane;
+        const int r = (TG ? 0 : m * 128) + q * 32 + lane;
         const int tq = r / a.Rb, hr = r - tq * a.Rb;
         const bool live = tq < nq && hr < nh;
         int rlo = 0, rhi = 0x3fffffff;   // rows without a token see everything and are not stored
@@ -197,11 +278,13 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
         }
         // soft-max in base 2 over raw scores: weight = 2^(c s - mb), mb = c max(s); the sign of the factor and a power of two go into the query.  With a soft cap the
         // scores are scaled and capped first (CAP) and c is 1.
-        float c, zf;
-        {   // this row's query, in two parts and the order of the code words, and its group sums, to TMEM
-            const float* src = a.q + (int64_t)(t0 + tq) * a.ld + (int64_t)(h0 + hr) * D;
+        float zf = 0.f;
+        float* const mine_row = stage_rows + r * PITCH;
+        if (!TG || m == 0) {   // this row's query, in the order of the code words, and its group sums, to TMEM
+            const float* src = mine_row;
             float top = 0.f;
-            for (int d = 0; live && d < D; d += 4) {
+#pragma unroll 8
+            for (int d = 0; d < 32 * NK; d += 4) {
                 const float4 x = ld4(src + d);
                 top = fmaxf(top, fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))));
             }
@@ -209,8 +292,7 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
             const bool norm = ex >= 20 && ex < 255;     // the largest into [2^4, 2^5); a row of zeros, denormals or infinities as it is
             const float up = copysignf(norm ? __uint_as_float((uint32_t)(254 - ex + 4) << 23) : 1.f, factor), down = norm ? __uint_as_float((uint32_t)(ex - 4) << 23) : 1.f;
             zf = fmaxf(fabsf(factor) * down * (CAP ? 1.f : LOG2E), 1e-37f);
-            c = CAP ? 1.f : zf;
-            const uint32_t qa = q0 + lanes + m * 2 * QP;
+            const uint32_t qa = q0 + lanes + (TG ? 0 : m * NP * QP);
             uint32_t sh[8], sl[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) sh[i] = sl[i] = 0;
@@ -223,8 +305,7 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const int d = 32 * k + 8 * (c2 + u);
-                        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-                        if (live && d < D) x = ld4(src + d), y = ld4(src + d + 4);     // (D a multiple of 8)
+                        const float4 x = ld4(src + d), y = ld4(src + d + 4);     // (zeros behind D)
                         const float f[8] = {x.x * up, x.y * up, x.z * up, x.w * up, y.x * up, y.y * up, y.z * up, y.w * up};
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
@@ -234,7 +315,8 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
                             sums[k] += f[i] + f[i + 4];
                         }
                     }
-                    st8(qa + (4 * k + c2) * 4, ph), st8(qa + QP + (4 * k + c2) * 4, pl);
+                    st8(qa + (4 * k + c2) * 4, ph);
+                    if (NP == 2) st8(qa + QP + (4 * k + c2) * 4, pl);
                 }
             }
 #pragma unroll
@@ -243,19 +325,24 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
                 const float2 b = __half22float2(h);
                 sh[i] = sh[2 + i] = h2(h), sl[i] = sl[2 + i] = h2(__floats2half2_rn(sums[2 * i] - b.x, sums[2 * i + 1] - b.y));
             }
-            st8(qa + 16 * NK, sh), st8(qa + QP + 16 * NK, sl);
+            st8(qa + 16 * NK, sh);
+            if (NP == 2) st8(qa + QP + 16 * NK, sl);
+            if (TG) row_factor[q * 32 + lane] = zf;
             st_wait();
             fence_before();
         }
-        asm volatile("bar.sync 1, %0;" ::"n"((4 * MT + 1) * 32) : "memory");   // the queries are in place (with the MMA warp)
+        asm volatile("bar.sync 1, %0;" ::"n"((SW + 1) * 32) : "memory");   // the queries are in place (with the MMA warp)
+        if (TG && m) zf = row_factor[q * 32 + lane];
+        const float c = CAP ? 1.f : zf;
         const uint64_t cc = pk(c, c);
         float mx = -INFINITY, mb = -INFINITY, l = 0.f, rest[4] = {0.f, 0.f, 0.f, 0.f};
-        uint64_t acc[VM / 2];
+        constexpr int NACC = TA ? 1 : VM / 2;
+        uint64_t acc[NACC];
 #pragma unroll
-        for (int i = 0; i < VM / 2; ++i) acc[i] = 0;
+        for (int i = 0; i < NACC; ++i) acc[i] = 0;
         bool ok = true;
         auto add_values = [&](int step) {   // acc += the value tile of a step
-            ok = bar_wait<false>(o_full + 8 * (step & 1), (step >> 1) & 1, ab);
+            ok = __all_sync(0xffffffffu, bar_wait<false>(o_full + 8 * (step & 1), (step >> 1) & 1, ab));
             if (!ok) return false;
             fence_after();
 #pragma unroll
@@ -264,7 +351,7 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
                 ld32(o0 + lanes + m * OCOLS + i, o);
                 ld_wait();
 #pragma unroll
-                for (int u = 0; u < 32; u += 2) acc[(i + u) >> 1] = add2(acc[(i + u) >> 1], pk(o[u], o[u + 1]));
+                for (int u = 0; u < 32; u += 2) acc[TA ? 0 : (i + u) >> 1] = add2(acc[TA ? 0 : (i + u) >> 1], pk(o[u], o[u + 1]));
             }
             float o[8];
             ld8(o0 + lanes + m * OCOLS + VM, o);
@@ -275,13 +362,13 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
             return true;
         };
 #pragma unroll 1
-        for (int j = 0; j < ntile && ok; ++j) {
-            const int step = j * MT + m, slot = step & 1;
+        for (int j = TG ? m : 0; j < ntile && ok; j += TG ? 2 : 1) {
+            const int step = TG ? j : j * MT + m, slot = step & 1;
             const int k0 = span.key0(split + j * a.parts);
             const int lo = rlo - k0, hi1 = rhi + 1 - k0, kp = keep - k0;   // visible keys of this row, relative to the tile: [lo, hi1) and those below kp
             const bool whole = __all_sync(0xffffffffu, lo <= 0 && hi1 >= KT);
             const uint32_t S = slot0 + lanes + slot * SLOT_COLS;
-            ok = bar_wait<false>(s_full + 8 * slot, (step >> 1) & 1, ab);
+            ok = __all_sync(0xffffffffu, bar_wait<false>(s_full + 8 * slot, (step >> 1) & 1, ab));   // (tcgen05 loads are the whole warp's)
             if (!ok) break;
             fence_after();
             float v[KT];
@@ -304,11 +391,15 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
             float m0 = fmaxf(v[0], v[1]), m1 = fmaxf(v[2], v[3]);
 #pragma unroll
             for (int i = 4; i < KT; i += 4) m0 = fmaxf(m0, fmaxf(v[i], v[i + 1])), m1 = fmaxf(m1, fmaxf(v[i + 2], v[i + 3]));
-            mx = fmaxf(mx, fmaxf(m0, m1));
-            const float mbn = mx * c;
-            const float corr = mx == -INFINITY ? 1.f : ex2(mb - mbn);   // 0 at the first visible key
-            mb = mbn;
-            const float off = mx == -INFINITY ? 0.f : -mbn;
+            const float tmax = fmaxf(m0, m1);
+            float corr = 1.f;
+            if (!TA || (tmax * c > mb + SLACK)) {      // (TA: a row's reference stays until a score passes it by 2^8)
+                mx = fmaxf(mx, tmax);
+                const float mbn = mx * c;
+                corr = mx == -INFINITY ? 1.f : ex2(mb - mbn);   // 0 at the first visible key
+                mb = mbn;
+            }
+            const float off = mx == -INFINITY ? 0.f : -mb;
             const uint64_t off2 = pk(off, off);
             uint64_t sum = 0;
 #pragma unroll
@@ -335,27 +426,98 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
             l = fmaf(l, corr, sx + sy);
             const uint64_t corr2 = pk(corr, corr);
             const bool same = __all_sync(0xffffffffu, corr == 1.f);
-            // MT = 1: the value tile of the key tile before, whose product ran beside this soft-max
-            if (MT == 1 && j > 0 && !add_values(step - 1)) break;
-            if (!same) {
+            // one group: the value tile of the key tile before, whose product ran beside this soft-max
+            if (GROUPS == 1 && j > 0 && !add_values(step - 1)) break;
+            if (!same && !TA) {
 #pragma unroll
-                for (int i = 0; i < VM / 2; ++i) acc[i] = mul2(acc[i], corr2);
+                for (int i = 0; i < NACC; ++i) acc[i] = mul2(acc[i], corr2);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) rest[i] *= corr;
+            }
+            if (!same && TA && j >= 2) {        // behind the product of this group's tile before
+                ok = __all_sync(0xffffffffu, bar_wait<false>(o_full + 8 * slot, ((step >> 1) & 1) ^ 1, ab));
+                if (!ok) break;
+                fence_after();
+                const uint32_t O = o0 + lanes + m * OCOLS;
+#pragma unroll 1
+                for (int i = 0; i < OCOLS; i += 16) {
+                    float o[16];
+                    ld16(O + i, o);
+                    ld_wait();
+                    uint32_t u[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) u[k] = __float_as_uint(o[k] * corr);
+                    st8(O + i, u), st8(O + i + 8, u + 8);
+                }
             }
             st_wait();
             fence_before();
             __syncwarp();
             if (lane == 0) bar_arrive(p_ready + 8 * slot);
-            // MT = 2: this key tile's, while the next scores are made (the other row tile keeps the tensor pipe busy)
-            if (MT == 2 && !add_values(step)) break;
+            // two groups: this key tile's, while the next scores are made (the other group keeps the tensor pipe busy)
+            if (GROUPS == 2 && !TA && !add_values(step)) break;
         }
-        if (MT == 1 && ok && ntile > 0) add_values(ntile - 1);
-        if (ok && live) {
+        if (GROUPS == 1 && ok && ntile > 0) add_values(ntile - 1);
+        const int mine = TG ? (ntile - m + 1) / 2 : ntile;    // key tiles of this group
+        if (TA && ok && mine > 0) {
+            const int last = 2 * (mine - 1) + m;
+            ok = __all_sync(0xffffffffu, bar_wait<false>(o_full + 8 * (last & 1), (last >> 1) & 1, ab));
+            fence_after();
+        }
+        // value sums of 32 columns, from registers or TMEM
+        auto values = [&](int i, float (&o)[32]) {
+            if (TA) {
+                if (mine > 0) {
+                    ld32(o0 + lanes + m * OCOLS + i, o);
+                    ld_wait();
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 32; ++u) o[u] = 0.f;
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < 32; u += 2) upk(acc[TA ? 0 : (i + u) >> 1], o[u], o[u + 1]);
+            }
+        };
+        if (TA && ok && mine > 0) {
+            float o[8];
+            ld8(o0 + lanes + m * OCOLS + VM, o);
+            ld_wait();
+#pragma unroll
+            for (int u = 0; u < 4; ++u) rest[u] = o[u] + o[4 + u];
+        }
+        float f0 = 1.f, f1 = 0.f;
+        const float* other = nullptr;
+        if (TG) {   // the second group's parts go to the first through shared memory, over the key and value stages (all that was issued has been waited for by both)
+            constexpr int XP = VM + 7;             // odd: a warp's rows lie in different banks
+            float* x = reinterpret_cast<float*>(smem_raw + (kv - sa(smem_raw))) + (q * 32 + lane) * XP;
+            asm volatile("bar.sync 2, %0;" ::"n"(SW * 32) : "memory");
+            if (m == 1) {
+                x[0] = mb, x[1] = l;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) x[2 + u] = rest[u];
+#pragma unroll
+                for (int i = 0; i < VM; i += 32) {
+                    float o[32];
+                    values(i, o);
+#pragma unroll
+                    for (int u = 0; u < 32; ++u) x[6 + i + u] = o[u];
+                }
+            }
+            asm volatile("bar.sync 2, %0;" ::"n"(SW * 32) : "memory");
+            if (m == 0) {
+                const float mb1 = x[0], l1 = x[1], top = fmaxf(mb, mb1);
+                f0 = l == 0.f ? 0.f : ex2(mb - top), f1 = l1 == 0.f ? 0.f : ex2(mb1 - top);    // (0: no key that the row sees)
+                l = l * f0 + l1 * f1, mb = top;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) rest[u] = rest[u] * f0 + x[2 + u] * f1;
+                other = x + 6;
+            }
+        }
+        if (ok && (!TG || m == 0)) {   // (all lanes: TMEM is read by whole warps)
             const int t = t0 + tq, h = h0 + hr;
             float f = 1.f;
-            float* pp = nullptr;
-            if (a.parts == 1) {
+            if (live && a.parts == 1) {
                 float gate = 1.f, den = l, resc = 1.f;
                 if (a.gated && !a.gate_elem) gate = sigmoidf_acc(a.gate[(int64_t)t * a.gld + h]);
                 if (a.sink) {   // the sink's term, under the larger of the two maxima
@@ -364,99 +526,72 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
                     den = fmaf(l, resc, ex2(sk - top));
                 }
                 f = gate * resc / den;
-            } else {
-                pp = a.part + (((int64_t)t * H + h) * a.parts + split) * (V + 4);
+            } else if (live) {
+                float* pp = a.part + (((int64_t)t * H + h) * a.parts + split) * (V + 4);
                 pp[0] = mb, pp[1] = l;
             }
+            // blocks of 64 columns in the order of the code words are the values of two groups (32 columns: of the one group); through shared memory, so that rows are
+            // stored whole
+#pragma unroll
+            for (int i0 = 0; i0 < VM; i0 += 64) {
+                constexpr int W = VM < 64 ? VM : 64;
+                float o[W];
+                __syncwarp();
+                values(i0, *reinterpret_cast<float(*)[32]>(o));
+                if (W == 64) values(i0 + 32, *reinterpret_cast<float(*)[32]>(o + W - 32));
+                if (TG) {
+#pragma unroll
+                    for (int u = 0; u < W; ++u) o[u] = f1 != 0.f || f1 != f1 ? fmaf(other[i0 + u], f1, o[u] * f0) : o[u] * f0;
+                }
+#pragma unroll
+                for (int d = 0; d < W; d += 4) {
+                    float y[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) y[i] = (o[value_place(d + i, W == 64 ? 2 : 1)] + rest[(i0 + d) >> 5]) * f;
+                    *reinterpret_cast<float4*>(mine_row + i0 + d) = make_float4(y[0], y[1], y[2], y[3]);
+                }
+            }
+            __syncwarp();
             const bool wide = (V & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
-#pragma unroll
-            for (int d = 0; d < VM; d += 4) {
-                if (d >= V) break;
-                float o[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float x, y;
-                    const int at = value_place(d + i, NV);
-                    upk(acc[at >> 1], x, y);
-                    o[i] = ((at & 1) ? y : x) + rest[d >> 5];
-                    if (!pp) o[i] *= f * (a.gate_elem && d + i < V ? sigmoidf_acc(a.gate[(int64_t)t * a.gld + (int64_t)h * V + d + i]) : 1.f);
+            const int row0 = (TG ? 0 : m * 128) + q * 32;
+            int rt = row0 / a.Rb, rh = row0 - rt * a.Rb;
+            auto each = [&](auto&& store) {     // the warp's rows: store(row in shared memory, its number among all (token, head) pairs)
+#pragma unroll 4
+                for (int i = 0; i < 32; ++i) {
+                    if (rt < nq && rh < nh) store(stage_rows + (row0 + i) * PITCH, (int64_t)(t0 + rt) * H + h0 + rh);
+                    if (++rh == a.Rb) rh = 0, ++rt;
                 }
-                if (pp) {
-                    for (int i = 0; i < 4 && d + i < V; ++i) pp[4 + d + i] = o[i];
-                } else if (wide) {
-                    store_act4(a.out, a.out_dtype, ((int64_t)t * H + h) * V + d, make_float4(o[0], o[1], o[2], o[3]));
-                } else {
-                    for (int i = 0; i < 4 && d + i < V; ++i) store_act(a.out, a.out_dtype, ((int64_t)t * H + h) * V + d + i, o[i]);
-                }
+            };
+            if (a.parts > 1) {
+                each([&](const float* y, int64_t at) {
+                    for (int d = lane; d < V; d += 32) a.part[(at * a.parts + split) * (V + 4) + 4 + d] = y[d];
+                });
+            } else if (wide && !a.gate_elem) {
+                const bool in = 4 * lane < V;
+                if (a.out_dtype == B200SEQ_F32) each([&](const float* y, int64_t at) { if (in) store_act4(a.out, B200SEQ_F32, at * V + 4 * lane, ld4(y + 4 * lane)); });
+                else each([&](const float* y, int64_t at) { if (in) store_act4(a.out, B200SEQ_BF16, at * V + 4 * lane, ld4(y + 4 * lane)); });
+            } else {
+                each([&](const float* y, int64_t at) {
+                    for (int d = lane; d < V; d += 32) store_act(a.out, a.out_dtype, at * V + d, y[d] * (a.gate_elem ? sigmoidf_acc(a.gate[at / H * a.gld + at % H * V + d]) : 1.f));
+                });
             }
         }
-    } else if (warp < 4 * MT + 8) {
-        // ===================== loaders: 256 threads, four a key =====================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MT == 2 ? 64 : 104));
-        // eight lanes store pieces of keys k and k + 4: their places in the swizzle fill a 128-byte line
-        const int lw = warp - 4 * MT, j8 = lane >> 2, key = lw * 8 + ((j8 & 1) << 2) + (j8 >> 1), quarter = lane & 3;
-        const int shift = (bs & (bs - 1)) == 0 ? 31 - __clz(bs) : -1;
-        const int Gv = G / a.vdiv, gv = g / a.vdiv;
-        if (quarter == 0) {   // the pieces behind m + 8 s stay zero
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const uint32_t kz = kv + s * STAGE + key * 128, vz = kz + KBYTES;
-                sts16(kz + ((4 * NK + 1) >> 3) * PLANE + ((((4 * NK + 1) & 7) ^ (key & 7)) << 4), 0, 0, 0, 0);
-                sts16(vz + ((4 * NV + 1) >> 3) * PLANE + ((((4 * NV + 1) & 7) ^ (key & 7)) << 4), 0, 0, 0, 0);
-            }
-        }
-        int page = 0, pos = 0;
-        auto lookup = [&](int j) {
-            pos = span.key0(split + j * a.parts) + key;
-            const int kp = min(pos, hi);
-            page = bt[shift >= 0 ? kp >> shift : kp / bs];
-        };
-        Codes<NK> kc;
-        Codes<NV> vc;
-        auto fetch = [&]() {   // the tile that was looked up
-            const bool in = pos <= hi;
-            const int kp = min(pos, hi), o = shift >= 0 ? kp & (bs - 1) : kp % bs;
-            load_codes<NK>(kc, a.kpool, kv4_row(page, o, bs, g, G, NK), quarter, in);
-            load_codes<NV>(vc, a.vpool, kv4_row(page, o, bs, gv, Gv, NV), quarter, in);
-        };
-        if (ntile > 0) {
-            lookup(0);
-            fetch();
-            if (ntile > 1) lookup(1);
-        }
-        bool ok = true;
-#pragma unroll 1
-        for (int j = 0; j < ntile && ok; ++j) {
-            const int s = j & 1;
-            const Codes<NK> k = kc;
-            const Codes<NV> v = vc;
-            if (j + 1 < ntile) {
-                fetch();
-                if (j + 2 < ntile) lookup(j + 2);
-            }
-            ok = bar_wait<false>(k_free + 8 * s, ((j >> 1) & 1) ^ 1, ab);
-            if (!ok) break;
-            put_codes<NK, true>(k, kv + s * STAGE, key, quarter);
-            async_fence();
-            __syncwarp();
-            if (lane == 0) bar_arrive(k_full + 8 * s);
-            ok = bar_wait<false>(v_free + 8 * s, ((j >> 1) & 1) ^ 1, ab);
-            if (!ok) break;
-            put_codes<NV, false>(v, kv + s * STAGE + KBYTES, key, quarter);
-            async_fence();
-            __syncwarp();
-            if (lane == 0) bar_arrive(v_full + 8 * s);
-        }
+    } else if (warp < SW + 8) {
+        // ===================== loaders: four warps for keys, four for values =====================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(GROUPS == 2 ? 64 : 104));
+        const int lw = warp - SW;
+        if (lw < 4) load_tiles<NK, true>(a.kpool, bt, bs, g, G, span, split, a.parts, ntile, hi, kv, STAGE, k_full, k_free, lw, lane, ab);
+        else load_tiles<NV, false>(a.vpool, bt, bs, g / a.vdiv, G / a.vdiv, span, split, a.parts, ntile, hi, kv + KBYTES, STAGE, v_full, v_free, lw - 4, lane, ab);
     } else {
         // ===================== MMA issuer =====================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(MT == 2 ? 32 : 64));
-        if (warp == 4 * MT + 8) asm volatile("bar.sync 1, %0;" ::"n"((4 * MT + 1) * 32) : "memory");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(GROUPS == 2 ? 32 : 64));
+        if (warp == SW + 8) asm volatile("bar.sync 1, %0;" ::"n"((SW + 1) * 32) : "memory");
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        if (warp == 4 * MT + 8 && elect()) {
+        if (warp == SW + 8 && elect()) {
             fence_after();
             constexpr uint32_t ids = (1u << 4) | ((uint32_t)(KT >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);                  // f16 x f16 -> f32
             constexpr uint32_t ido = (1u << 4) | (1u << 16) | ((uint32_t)(OCOLS >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);   // B is mn-major
-            constexpr uint32_t O0 = 2 * SLOT_COLS, Q0 = O0 + MT * OCOLS;
+            constexpr uint32_t O0 = 2 * SLOT_COLS, Q0 = O0 + GROUPS * OCOLS;
             const int steps = ntile * MT;
             bool ok = true;
             auto scores = [&](int step) {
@@ -465,12 +600,12 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
                 if (!ok) return;
                 fence_after();
                 const uint64_t kb = desc_k128(kv + s * STAGE);
-                const uint32_t d = tm + slot * SLOT_COLS, qa = tm + Q0 + m * 2 * QP;
+                const uint32_t d = tm + slot * SLOT_COLS, qa = tm + Q0 + m * NP * QP;
 #pragma unroll
-                for (int pr = 1; pr >= 0; --pr)          // the low parts of q first
+                for (int pr = NP - 1; pr >= 0; --pr)     // the low parts of q first
 #pragma unroll
                     for (int kk = 0; kk < 2 * NK + 1; ++kk)
-                        mma_ts(d, qa + pr * QP + kk * 8, kb + (uint64_t)(((kk >> 2) * PLANE) / 16 + 2 * (kk & 3)), ids, (pr < 1 || kk) ? 1u : 0u);
+                        mma_ts(d, qa + pr * QP + kk * 8, kb + (uint64_t)(((kk >> 2) * PLANE) / 16 + 2 * (kk & 3)), ids, (pr < NP - 1 || kk) ? 1u : 0u);
                 commit_one(s_full + 8 * slot);
                 if ((MT == 1 || slot == 1) && j + 2 < ntile) commit_one(k_free + 8 * s);   // (nobody waits for the last ones)
             };
@@ -482,7 +617,8 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
                     if (ok) scores(step + 1);
                     if (!ok) break;
                 }
-                const int j = step / MT, s = j & 1, slot = step & 1, m = MT == 2 ? slot : 0;
+                const int j = step / MT, s = j & 1, slot = step & 1, m = GROUPS == 2 ? slot : 0;
+                const uint32_t more = TA && j >= 2 ? 1u : 0u;          // on top of what is there
                 ok = bar_wait<false>(v_full + 8 * s, (j >> 1) & 1, ab) && bar_wait<false>(p_ready + 8 * slot, (step >> 1) & 1, ab);
                 if (!ok) break;
                 fence_after();
@@ -492,7 +628,7 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
                 for (int pr = NP - 1; pr >= 0; --pr)
 #pragma unroll
                     for (int kk = 0; kk < KT / 16; ++kk)
-                        mma_ts(d, pa + 32 * pr + 8 * kk, vb + (uint64_t)(kk * 2048 / 16), ido, (pr < NP - 1 || kk) ? 1u : 0u);
+                        mma_ts(d, pa + 32 * pr + 8 * kk, vb + (uint64_t)(kk * 2048 / 16), ido, (pr < NP - 1 || kk) ? 1u : more);
                 commit_one(o_full + 8 * slot);
                 if ((MT == 1 || slot == 1) && j + 2 < ntile) commit_one(v_free + 8 * s);
             }
@@ -513,10 +649,10 @@ __global__ void __launch_bounds__((4 * MT + 12) * 32, 1) attn4_tc_kernel(const _
     }
 }
 
-template <int MT, int NK, int NV, int NP, bool CAP>
+template <int MT, bool TG, int NK, int NV, int NP, bool CAP>
 cudaError_t run_one(const Attn4Args& a, const b200seq_step& st, dim3 grid, cudaStream_t cs) {
-    constexpr int need = 2 * (blocks_of(NK) + blocks_of(NV)) * PLANE + 1024, smem = need < 120 * 1024 ? 120 * 1024 : need;   // one CTA per SM: it takes all of TMEM
-    const auto kernel = attn4_tc_kernel<MT, NK, NV, NP, CAP>;
+    constexpr int need = 2 * (blocks_of(NK) + blocks_of(NV)) * PLANE + 128 * MT * (32 * (NK > NV ? NK : NV) + 4) * 4 + 1024, smem = need < 120 * 1024 ? 120 * 1024 : need;   // one CTA per SM: it takes all of TMEM
+    const auto kernel = attn4_tc_kernel<MT, TG, NK, NV, NP, CAP>;
     static bool ready[16] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -526,13 +662,14 @@ cudaError_t run_one(const Attn4Args& a, const b200seq_step& st, dim3 grid, cudaS
         if (e != cudaSuccess) return e;
         if (dev < 16) ready[dev] = true;
     }
-    launch_chained(kernel, grid, (4 * MT + 12) * 32, smem, cs, a, st);
+    launch_chained(kernel, grid, (4 * (TG ? 2 : MT) + 12) * 32, smem, cs, a, st);
     return cudaGetLastError();
 }
 template <int MT, int NK, int NV>
 cudaError_t run(const Attn4Args& a, const b200seq_step& st, dim3 grid, cudaStream_t cs) {
-    if (a.softcap > 0.f) return a.out_dtype == B200SEQ_F32 ? run_one<MT, NK, NV, 2, true>(a, st, grid, cs) : run_one<MT, NK, NV, 1, true>(a, st, grid, cs);
-    return a.out_dtype == B200SEQ_F32 ? run_one<MT, NK, NV, 2, false>(a, st, grid, cs) : run_one<MT, NK, NV, 1, false>(a, st, grid, cs);
+    constexpr bool two = MT == 1;   // two groups on one row tile: not with f32 results of heads above 64
+    if (a.softcap > 0.f) return a.out_dtype == B200SEQ_F32 ? run_one<MT, two && NV < 4, NK, NV, 2, true>(a, st, grid, cs) : run_one<MT, two, NK, NV, 1, true>(a, st, grid, cs);
+    return a.out_dtype == B200SEQ_F32 ? run_one<MT, two && NV < 4, NK, NV, 2, false>(a, st, grid, cs) : run_one<MT, two, NK, NV, 1, false>(a, st, grid, cs);
 }
 
 }  // namespace
