@@ -63,6 +63,7 @@ __device__ __forceinline__ void centres(__half2 s, __half2 m, uint32_t& high, ui
 __device__ __forceinline__ void sts16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ void st1(uint32_t taddr, uint32_t r) { asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r) : "memory"); }
 __device__ __forceinline__ void ld8(uint32_t taddr, float* v) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -82,9 +83,7 @@ struct Codes {
 };
 // a thread's quarter of a row's codes and the row's parameters
 template <int N>
-__device__ __forceinline__ void load_codes(Codes<N>& c, const uint8_t* pool, const Kv4Row& at, int quarter, bool in) {
-    const uint8_t* w = pool + at.codes + 4 * N * quarter;
-    const uint8_t* p = pool + at.params;
+__device__ __forceinline__ void load_codes(Codes<N>& c, const uint8_t* w, const uint8_t* p, bool in) {
     if (!in) {
 #pragma unroll
         for (int i = 0; i < N; ++i) c.w[i] = c.p[i] = 0;
@@ -98,35 +97,43 @@ __device__ __forceinline__ void load_codes(Codes<N>& c, const uint8_t* pool, con
         c.w[0] = *reinterpret_cast<const uint32_t*>(w), c.p[0] = *reinterpret_cast<const uint32_t*>(p);
     }
 }
-// into shared memory: piece i of row `key` lies at block i / 8, place (i % 8) ^ (key % 8)
+// Into shared memory: piece i of row `key` lies at block i / 8, place (i % 8) ^ (key % 8).  at: the row's first block; even, odd: where this thread's pieces `quarter` and
+// quarter + 4 of a block lie in it (the same for all blocks, and for key + 8).
 template <int N, bool KEY>
-__device__ __forceinline__ void put_codes(const Codes<N>& c, uint32_t at, int key, int quarter) {
-    const uint32_t row = at + key * 128;
-    auto piece = [&](int i) { return row + (i >> 3) * PLANE + (((i & 7) ^ (key & 7)) << 4); };
+__device__ __forceinline__ void put_codes(const Codes<N>& c, uint32_t even, uint32_t odd) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         uint32_t x[4];
         __half2 s;
-        int to;
-        if (KEY) {            // words [part][group]: word i is group i of part `quarter`
-            s = __low2half2(h2(c.p[i])), to = i * 4 + quarter;
-        } else if (N == 1) {  // two parts of the one group
-            s = __low2half2(h2(c.p[0])), to = quarter;
-        } else {              // 16-bit words [part][group]: word i is two groups of part 2 quarter + i / (N / 2)
+        uint32_t to;
+        if (KEY) {            // words [part][group]: word i is group i of part `quarter`: piece 4 i + quarter
+            s = __low2half2(h2(c.p[i])), to = ((i & 1) ? odd : even) + (i >> 1) * PLANE;
+        } else if (N == 1) {  // two parts of the one group: piece `quarter`
+            s = __low2half2(h2(c.p[0])), to = even;
+        } else {              // 16-bit words [part][group]: word i is two groups of part 2 quarter + r: piece 8 gp + 4 r + quarter
             const int gp = N == 4 ? i & 1 : 0, r = N == 4 ? i >> 1 : i;
-            s = __lows2half2(h2(c.p[2 * gp]), h2(c.p[(2 * gp + 1) % N])), to = gp * 8 + r * 4 + quarter;
+            s = __lows2half2(h2(c.p[2 * gp]), h2(c.p[(2 * gp + 1) % N])), to = (r ? odd : even) + gp * PLANE;
         }
         expand(c.w[i], s, __hmul2_rn(s, __floats2half2_rn(-72.f, -72.f)), x);
-        sts16(piece(to), x[0], x[1], x[2], x[3]);
+        sts16(to, x[0], x[1], x[2], x[3]);
     }
-    if (quarter == 0) {       // groups 0 .. 3, high parts, then low parts
-        uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};
-        const __half2 zero = __floats2half2_rn(0.f, 0.f);
-        if (N == 1) centres(__halves2half2(__low2half(h2(c.p[0])), __low2half(zero)), __halves2half2(__high2half(h2(c.p[0])), __low2half(zero)), hi[0], lo[0]);
-#pragma unroll
-        for (int i = 0; i + 1 < N; i += 2) centres(__lows2half2(h2(c.p[i]), h2(c.p[(i + 1) % N])), __highs2half2(h2(c.p[i]), h2(c.p[(i + 1) % N])), hi[i / 2], lo[i / 2]);
-        sts16(piece(4 * N), hi[0], hi[1], lo[0], lo[1]);
-    }
+}
+// group `quarter`'s m + 8 s of two keys into their rows' piece 4 N: four high parts, four low parts
+template <int N>
+__device__ __forceinline__ void put_centres(const Codes<N>& c0, const Codes<N>& c1, int quarter, uint32_t at0, uint32_t at1) {
+    auto pick = [&](const Codes<N>& c) {
+        uint32_t p = c.p[0];
+        if (N > 1) p = quarter & 1 ? c.p[1 % N] : p;
+        if (N == 4) p = quarter & 2 ? (quarter & 1 ? c.p[3 % N] : c.p[2 % N]) : p;
+        return quarter < N ? p : 0u;
+    };
+    const uint32_t a = pick(c0), b = pick(c1);
+    uint32_t hi, lo;
+    centres(__lows2half2(h2(a), h2(b)), __highs2half2(h2(a), h2(b)), hi, lo);
+    asm volatile("st.shared.b16 [%0], %1;" ::"r"(at0), "h"((uint16_t)hi) : "memory");
+    asm volatile("st.shared.b16 [%0], %1;" ::"r"(at1), "h"((uint16_t)(hi >> 16)) : "memory");
+    asm volatile("st.shared.b16 [%0], %1;" ::"r"(at0 + 8), "h"((uint16_t)lo) : "memory");
+    asm volatile("st.shared.b16 [%0], %1;" ::"r"(at1 + 8), "h"((uint16_t)(lo >> 16)) : "memory");
 }
 
 // The key tiles of one pool, expanded into their stages: four warps, four threads a key, two keys a thread.  A tile's codes are asked for while the tile before it is
@@ -136,7 +143,6 @@ __device__ __forceinline__ void load_tiles(const uint8_t* pool, const int32_t* b
                                            uint32_t pitch, uint32_t full, uint32_t free, int lw, int lane, volatile int* ab) {
     // eight lanes store pieces of keys k and k + 4: their places in the swizzle fill a 128-byte line
     const int j8 = lane >> 2, key = lw * 16 + ((j8 & 1) << 2) + (j8 >> 1), quarter = lane & 3;
-    const int shift = (bs & (bs - 1)) == 0 ? 31 - __clz(bs) : -1;
     if (quarter == 0) {   // the pieces behind m + 8 s stay zero
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -146,21 +152,35 @@ __device__ __forceinline__ void load_tiles(const uint8_t* pool, const int32_t* b
                 sts16(stage + s * pitch + k * 128 + ((4 * N + 1) >> 3) * PLANE + ((((4 * N + 1) & 7) ^ (k & 7)) << 4), 0, 0, 0, 0);
             }
     }
-    int page[2], pos = 0;
+    uint32_t even = stage + key * 128 + ((quarter ^ (key & 7)) << 4), odd = stage + key * 128 + (((4 + quarter) ^ (key & 7)) << 4);
+    uint32_t centre = stage + key * 128 + ((4 * N) >> 3) * PLANE + ((((4 * N) & 7) ^ (key & 7)) << 4) + 2 * quarter;
+    // Pages of 16: a tile's 64 keys are four whole pages, and a thread's keys (key and key + 8) lie at fixed places of one of them.  Other sizes: each key is looked up.
+    const bool whole = bs == 16;
+    const Kv4Row r0 = kv4_row(0, key & 15, 16, g, G, N), r1 = kv4_row(0, (key & 15) + 8, 16, g, G, N);      // (key % 16 < 8)
+    const uint8_t *w0 = pool + r0.codes + 4 * N * quarter, *p0 = pool + r0.params;
+    const uint32_t pitch_w = (uint32_t)(r1.codes - r0.codes), pitch_p = (uint32_t)(r1.params - r0.params), page_bytes = (uint32_t)G * (16 * N * 20);
+    int page[2] = {0, 0}, pos = 0;
     auto lookup = [&](int j) {
         pos = span.key0(split + j * parts) + key;
+        if (whole) {
+            if (pos <= hi) page[0] = bt[pos >> 4];
+        } else {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int kp = min(pos + 8 * u, hi);
-            page[u] = bt[shift >= 0 ? kp >> shift : kp / bs];
+            for (int u = 0; u < 2; ++u) page[u] = bt[min(pos + 8 * u, hi) / bs];
         }
     };
     Codes<N> next[2];
     auto fetch = [&]() {   // the tile that was looked up
+        if (whole) {
+            const uint64_t at = (uint64_t)(uint32_t)page[0] * page_bytes;
+            load_codes<N>(next[0], w0 + at, p0 + at, pos <= hi), load_codes<N>(next[1], w0 + at + pitch_w, p0 + at + pitch_p, pos + 8 <= hi);
+        } else {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int kp = min(pos + 8 * u, hi);
-            load_codes<N>(next[u], pool, kv4_row(page[u], shift >= 0 ? kp & (bs - 1) : kp % bs, bs, g, G, N), quarter, pos + 8 * u <= hi);
+            for (int u = 0; u < 2; ++u) {
+                const int kp = min(pos + 8 * u, hi);
+                const Kv4Row at = kv4_row(page[u], kp % bs, bs, g, G, N);
+                load_codes<N>(next[u], pool + at.codes + 4 * N * quarter, pool + at.params, pos + 8 * u <= hi);
+            }
         }
     };
     if (ntile > 0) {
@@ -168,6 +188,7 @@ __device__ __forceinline__ void load_tiles(const uint8_t* pool, const int32_t* b
         fetch();
         if (ntile > 1) lookup(1);
     }
+    uint32_t there = pitch;
 #pragma unroll 1
     for (int j = 0; j < ntile; ++j) {
         const int s = j & 1;
@@ -177,11 +198,13 @@ __device__ __forceinline__ void load_tiles(const uint8_t* pool, const int32_t* b
             if (j + 2 < ntile) lookup(j + 2);
         }
         if (!bar_wait<false>(free + 8 * s, ((j >> 1) & 1) ^ 1, ab)) return;
-        put_codes<N, KEY>(c0, stage + s * pitch, key, quarter);
-        put_codes<N, KEY>(c1, stage + s * pitch, key + 8, quarter);
+        put_codes<N, KEY>(c0, even, odd);
+        put_codes<N, KEY>(c1, even + 1024, odd + 1024);
+        put_centres<N>(c0, c1, quarter, centre, centre + 1024);
         async_fence();
         __syncwarp();
         if (lane == 0) bar_arrive(full + 8 * s);
+        even += there, odd += there, centre += there, there = 0u - there;      // the other stage
     }
 }
 
@@ -215,18 +238,12 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
         if (ord < longer) tile_no = (ord % (nc - 1)) * per + per - 1 - ord / (nc - 1);
         else tile_no = ((ord - longer) % nc) * per + rem - 1 - (ord - longer) / nc;
     }
-    if (!attn_find_tile(st, tile_no, a.QT, e, t0, nq)) return;
+    if (st.B == 1) e = 0, t0 = tile_no * a.QT, nq = min(a.QT, st.T - t0);
+    else if (!attn_find_tile(st, tile_no, a.QT, e, t0, nq)) return;
+    const int p0 = st.tok_pos[t0];
     const int g = unit / a.HB, hb = unit - g * a.HB, R = H / G;
     const int h0 = g * R + hb * a.Rb, nh = min(a.Rb, R - hb * a.Rb);
     const int split = blockIdx.z;
-    const int p0 = st.tok_pos[t0], hi = p0 + nq - 1, bs = st.block_size;
-    const int32_t* bt = st.block_table + (int64_t)e * st.max_blocks;
-    if (p0 < 0 || hi / bs >= st.max_blocks) {
-        if (threadIdx.x == 0) atomicOr(a.err, 1);
-        return;
-    }
-    const KeySpan<KT> span(a, p0, hi);
-    const int ntile = span.total > split ? (span.total - split + a.parts - 1) / a.parts : 0;   // tiles split, split + parts, ...
     {   // the queries' rows on their way while the rest is set up: whole rows at a time (read by their threads they cost a 128-byte line a lane and load), by all warps
         constexpr int WARPS = SW + 12, STEP = WARPS * (32 / RL);
         const int d4 = 4 * (lane & (RL - 1));
@@ -240,6 +257,15 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
                          : "memory");                  // (nothing is read where there is no row; its place becomes zero)
         }
     }
+    const int hi = p0 + nq - 1, bs = st.block_size;
+    const int32_t* bt = st.block_table + (int64_t)e * st.max_blocks;
+    if (p0 < 0 || hi / bs >= st.max_blocks) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (threadIdx.x == 0) atomicOr(a.err, 1);
+        return;
+    }
+    const KeySpan<KT> span(a, p0, hi);
+    const int ntile = span.total > split ? (span.total - split + a.parts - 1) / a.parts : 0;   // tiles split, split + parts, ...
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             bar_init(k_full + 8 * i, 4), bar_init(k_free + 8 * i, 1), bar_init(v_full + 8 * i, 4), bar_init(v_free + 8 * i, 1);
@@ -280,7 +306,8 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
         // scores are scaled and capped first (CAP) and c is 1.
         float zf = 0.f;
         float* const mine_row = stage_rows + r * PITCH;
-        if (!TG || m == 0) {   // this row's query, in the order of the code words, and its group sums, to TMEM
+        constexpr bool SPLIT = TG && NK == 4;     // both groups: two of the four groups of 32 each
+        if (!TG || SPLIT || m == 0) {   // this row's query, in the order of the code words, and its group sums, to TMEM
             const float* src = mine_row;
             float top = 0.f;
 #pragma unroll 8
@@ -293,12 +320,10 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
             const float up = copysignf(norm ? __uint_as_float((uint32_t)(254 - ex + 4) << 23) : 1.f, factor), down = norm ? __uint_as_float((uint32_t)(ex - 4) << 23) : 1.f;
             zf = fmaxf(fabsf(factor) * down * (CAP ? 1.f : LOG2E), 1e-37f);
             const uint32_t qa = q0 + lanes + (TG ? 0 : m * NP * QP);
-            uint32_t sh[8], sl[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sh[i] = sl[i] = 0;
             float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < NK; ++k) {
+            for (int k_ = 0; k_ < (SPLIT ? 2 : NK); ++k_) {
+                const int k = SPLIT ? 2 * m + k_ : k_;
 #pragma unroll 1
                 for (int c2 = 0; c2 < 4; c2 += 2) {
                     uint32_t ph[8], pl[8];
@@ -312,27 +337,36 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
                             const __half2 h = __floats2half2_rn(f[i], f[i + 4]);
                             const float2 b = __half22float2(h);
                             ph[4 * u + i] = h2(h), pl[4 * u + i] = h2(__floats2half2_rn(f[i] - b.x, f[i + 4] - b.y));
-                            sums[k] += f[i] + f[i + 4];
+                            sums[k_] += f[i] + f[i + 4];
                         }
                     }
                     st8(qa + (4 * k + c2) * 4, ph);
                     if (NP == 2) st8(qa + QP + (4 * k + c2) * 4, pl);
                 }
             }
+            // the sums of q, two groups a column, against the high and the low parts of m + 8 s
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {   // the sums of q, against the high and the low parts of m + 8 s
+            for (int i = 0; i < 2; ++i) {
+                if (SPLIT && i) break;
                 const __half2 h = __floats2half2_rn(sums[2 * i], sums[2 * i + 1]);
                 const float2 b = __half22float2(h);
-                sh[i] = sh[2 + i] = h2(h), sl[i] = sl[2 + i] = h2(__floats2half2_rn(sums[2 * i] - b.x, sums[2 * i + 1] - b.y));
+                const uint32_t hi2 = h2(h), lo2 = h2(__floats2half2_rn(sums[2 * i] - b.x, sums[2 * i + 1] - b.y)), at = qa + 16 * NK + (SPLIT ? m : i);
+                st1(at, hi2), st1(at + 2, hi2);
+                if (NP == 2) st1(at + QP, lo2), st1(at + QP + 2, lo2);
             }
-            st8(qa + 16 * NK, sh);
-            if (NP == 2) st8(qa + QP + 16 * NK, sl);
-            if (TG) row_factor[q * 32 + lane] = zf;
+            if (!SPLIT || m == 0) {
+#pragma unroll
+                for (int i = 4; i < 8; ++i) {
+                    st1(qa + 16 * NK + i, 0u);
+                    if (NP == 2) st1(qa + QP + 16 * NK + i, 0u);
+                }
+            }
+            if (TG && !SPLIT) row_factor[q * 32 + lane] = zf;
             st_wait();
             fence_before();
         }
         asm volatile("bar.sync 1, %0;" ::"n"((SW + 1) * 32) : "memory");   // the queries are in place (with the MMA warp)
-        if (TG && m) zf = row_factor[q * 32 + lane];
+        if (TG && !SPLIT && m) zf = row_factor[q * 32 + lane];
         const float c = CAP ? 1.f : zf;
         const uint64_t cc = pk(c, c);
         float mx = -INFINITY, mb = -INFINITY, l = 0.f, rest[4] = {0.f, 0.f, 0.f, 0.f};
@@ -486,35 +520,41 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
 #pragma unroll
             for (int u = 0; u < 4; ++u) rest[u] = o[u] + o[4 + u];
         }
+        // Two groups on one row tile are merged through shared memory, over the key and value stages (all that was issued has been waited for by both): each gives the
+        // other its share of the columns, a block of 64 where there are two, all to the first one where there is one.
+        constexpr int W = VM < 64 ? VM : 64, XP = W + 7;    // (odd: a warp's rows lie in different banks)
+        const int keep_block = NV == 4 && TG ? m : 0;
         float f0 = 1.f, f1 = 0.f;
         const float* other = nullptr;
-        if (TG) {   // the second group's parts go to the first through shared memory, over the key and value stages (all that was issued has been waited for by both)
-            constexpr int XP = VM + 7;             // odd: a warp's rows lie in different banks
-            float* x = reinterpret_cast<float*>(smem_raw + (kv - sa(smem_raw))) + (q * 32 + lane) * XP;
+        if (TG) {
+            float* const base = reinterpret_cast<float*>(smem_raw + (kv - sa(smem_raw)));
+            constexpr int XQ = NV == 4 ? XP : 8;            // (one block of columns: the first group gives its maximum and sums alone)
+            static_assert(128 * (XP + XQ) * 4 <= 2 * STAGE, "the stages hold both groups' parts");
+            float *const second = base + (q * 32 + lane) * XP, *const first = base + 128 * XP + (q * 32 + lane) * XQ;
+            float* const x = m ? second : first;
+            const float* const y = m ? first : second;
             asm volatile("bar.sync 2, %0;" ::"n"(SW * 32) : "memory");
-            if (m == 1) {
-                x[0] = mb, x[1] = l;
+            x[0] = mb, x[1] = l;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) x[2 + u] = rest[u];
+            for (int u = 0; u < 4; ++u) x[2 + u] = rest[u];
+            if (NV == 4 || m == 1) {
 #pragma unroll
-                for (int i = 0; i < VM; i += 32) {
+                for (int i = 0; i < W; i += 32) {
                     float o[32];
-                    values(i, o);
+                    values(NV == 4 ? (m ? i : 64 + i) : i, o);
 #pragma unroll
                     for (int u = 0; u < 32; ++u) x[6 + i + u] = o[u];
                 }
             }
             asm volatile("bar.sync 2, %0;" ::"n"(SW * 32) : "memory");
-            if (m == 0) {
-                const float mb1 = x[0], l1 = x[1], top = fmaxf(mb, mb1);
-                f0 = l == 0.f ? 0.f : ex2(mb - top), f1 = l1 == 0.f ? 0.f : ex2(mb1 - top);    // (0: no key that the row sees)
-                l = l * f0 + l1 * f1, mb = top;
+            const float mb1 = y[0], l1 = y[1], top = fmaxf(mb, mb1);
+            f0 = l == 0.f ? 0.f : ex2(mb - top), f1 = l1 == 0.f ? 0.f : ex2(mb1 - top);    // (0: no key that the row sees)
+            l = m ? fmaf(l1, f1, l * f0) : fmaf(l, f0, l1 * f1), mb = top;                 // (the first group's first: the same sum in both)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) rest[u] = rest[u] * f0 + x[2 + u] * f1;
-                other = x + 6;
-            }
+            for (int u = 0; u < 4; ++u) rest[u] = fmaf(rest[u], f0, y[2 + u] * f1);
+            other = y + 6;
         }
-        if (ok && (!TG || m == 0)) {   // (all lanes: TMEM is read by whole warps)
+        if (ok) {   // (all lanes: TMEM is read by whole warps)
             const int t = t0 + tq, h = h0 + hr;
             float f = 1.f;
             if (live && a.parts == 1) {
@@ -526,38 +566,44 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
                     den = fmaf(l, resc, ex2(sk - top));
                 }
                 f = gate * resc / den;
-            } else if (live) {
+            } else if (live && (!TG || m == 0)) {
                 float* pp = a.part + (((int64_t)t * H + h) * a.parts + split) * (V + 4);
                 pp[0] = mb, pp[1] = l;
             }
             // blocks of 64 columns in the order of the code words are the values of two groups (32 columns: of the one group); through shared memory, so that rows are
             // stored whole
 #pragma unroll
-            for (int i0 = 0; i0 < VM; i0 += 64) {
-                constexpr int W = VM < 64 ? VM : 64;
+            for (int b = 0; b < (NV == 4 && !TG ? 2 : 1); ++b) {
+                if (TG && NV < 4 && m) break;
+                const int i0 = NV == 4 && TG ? 64 * keep_block : 64 * b;
                 float o[W];
                 __syncwarp();
                 values(i0, *reinterpret_cast<float(*)[32]>(o));
                 if (W == 64) values(i0 + 32, *reinterpret_cast<float(*)[32]>(o + W - 32));
                 if (TG) {
 #pragma unroll
-                    for (int u = 0; u < W; ++u) o[u] = f1 != 0.f || f1 != f1 ? fmaf(other[i0 + u], f1, o[u] * f0) : o[u] * f0;
+                    for (int u = 0; u < W; ++u) o[u] = f1 != 0.f || f1 != f1 ? fmaf(other[u], f1, o[u] * f0) : o[u] * f0;
                 }
+                const float r0 = NV == 4 && i0 ? rest[2] : rest[0], r1 = NV == 4 && i0 ? rest[3] : rest[1];
 #pragma unroll
                 for (int d = 0; d < W; d += 4) {
                     float y[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) y[i] = (o[value_place(d + i, W == 64 ? 2 : 1)] + rest[(i0 + d) >> 5]) * f;
+                    for (int i = 0; i < 4; ++i) y[i] = (o[value_place(d + i, W == 64 ? 2 : 1)] + (d < 32 ? r0 : r1)) * f;
                     *reinterpret_cast<float4*>(mine_row + i0 + d) = make_float4(y[0], y[1], y[2], y[3]);
                 }
             }
-            __syncwarp();
+        }
+        if (TG) asm volatile("bar.sync 2, %0;" ::"n"(SW * 32) : "memory");      // both groups store rows, half of them each
+        __syncwarp();
+        if (ok) {
             const bool wide = (V & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
-            const int row0 = (TG ? 0 : m * 128) + q * 32;
+            constexpr int MINE = TG ? 16 : 32;
+            const int row0 = TG ? q * 32 + 16 * m : m * 128 + q * 32;
             int rt = row0 / a.Rb, rh = row0 - rt * a.Rb;
-            auto each = [&](auto&& store) {     // the warp's rows: store(row in shared memory, its number among all (token, head) pairs)
+            auto each = [&](auto&& store) {     // this warp's rows: store(row in shared memory, its number among all (token, head) pairs)
 #pragma unroll 4
-                for (int i = 0; i < 32; ++i) {
+                for (int i = 0; i < MINE; ++i) {
                     if (rt < nq && rh < nh) store(stage_rows + (row0 + i) * PITCH, (int64_t)(t0 + rt) * H + h0 + rh);
                     if (++rh == a.Rb) rh = 0, ++rt;
                 }
