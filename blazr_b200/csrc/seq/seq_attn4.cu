@@ -78,17 +78,20 @@ __device__ __forceinline__ uint32_t centre(uint32_t s_, uint32_t m_, bool low) {
 // reads at once lie in different banks
 __device__ __forceinline__ int swz(int i) { return i ^ (((i >> 3) & 3) << 1); }
 
+// (plain loads: the compiler may move them ahead of what they do not depend on)
 template <int N>
-__device__ __forceinline__ void lds(uint32_t at, uint32_t (&x)[N]) {
-    if (N == 4) asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[N > 2 ? 2 : 0]), "=r"(x[N > 3 ? 3 : 0]) : "r"(at) : "memory");
-    else if (N == 2) asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(x[0]), "=r"(x[N > 1 ? 1 : 0]) : "r"(at) : "memory");
-    else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x[0]) : "r"(at) : "memory");
+__device__ __forceinline__ void lds(const uint8_t* at, uint32_t (&x)[N]) {
+    if (N == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(at);
+        x[0] = v.x, x[1 % N] = v.y, x[2 % N] = v.z, x[3 % N] = v.w;
+    } else if (N == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(at);
+        x[0] = v.x, x[1 % N] = v.y;
+    } else {
+        x[0] = *reinterpret_cast<const uint32_t*>(at);
+    }
 }
-__device__ __forceinline__ uint32_t lds16(uint32_t at) {
-    uint16_t x;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(at) : "memory");
-    return x;
-}
+__device__ __forceinline__ uint32_t lds16(const uint8_t* at) { return *reinterpret_cast<const uint16_t*>(at); }
 
 // Half a tile, the 16 keys of a whole unit, into shared memory: codes (swizzled), then parameters, of keys and of values.  k, v: this lane's first piece of codes;
 // par: its piece of either's parameters.  dst: the half; piece: 16 * swz(lane); par_at: where the parameters' piece goes.
@@ -278,12 +281,12 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
         issue(i + 1);
         copies_wait<1>();
         __syncwarp();
-        const uint32_t at = ring + (i & 1) * STAGE;
+        const uint8_t* const at = smem + warp * (STAGES * STAGE) + (i & 1) * STAGE;
         // ---- scores of keys key0 + 16 s + 8 n + {2c, 2c + 1}: z[4 s + 2 n + {0, 1}] ----
         float z[8];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const uint32_t ks = at + s * HALF;
+            const uint8_t* const ks = at + s * HALF;
             uint64_t zc[2] = {0, 0};
             uint32_t kw[2][NK], kp[4][NK];
             lds<NK>(ks + ko, kw[0]);
@@ -342,7 +345,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
         uint32_t vw[2][4][(NV + 1) / 2], sp[2][2][NV], bp[2][2];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            const uint32_t vs = at + s * HALF + KB;
+            const uint8_t* const vs = at + s * HALF + KB;
             uint32_t vp[4][NV], hw[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
