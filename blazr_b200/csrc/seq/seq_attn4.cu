@@ -14,8 +14,8 @@
 // So nothing is rounded but q and the weights to 22 bits; the rest is f32.  The tensor core cuts its f32 sums off instead of rounding them, 2^-21 of a sum a product, always
 // downwards: value products are summed over 32 keys there and by rounded adds from then on (531 tokens, 2048 keys: error 1.3e-5 in one chain over all keys).
 //
-// Keys are dealt to the 8 warps of a CTA, to the CTAs of a cluster (merged through distributed shared memory) and, where that leaves SMs idle, to several clusters
-// (merged by a second kernel through the work area).
+// A CTA's 8 or 4 warps share the keys of a row tile.  Few keys: so do the CTAs of a cluster, merged through distributed shared memory.  Many: the keys of all row tiles are one
+// list that is dealt out evenly, and a second kernel merges the parts of row tiles that ended up in several CTAs.
 #include "seq_attn4.cuh"
 #include "tc_split.cuh"
 
@@ -25,8 +25,10 @@ namespace {
 
 constexpr int KT = 32;        // keys per tile: two halves of 16
 constexpr int ROWS = 8;       // rows per row tile
-constexpr int WARPS = 8;
 constexpr int STAGES = 2;
+// CTAs on every SM: two of 8 warps with 128 registers, or three of 4 with 168 (the plan says which)
+__host__ __device__ constexpr int resident(int warps) { return warps == 8 ? 2 : 3; }
+__host__ __device__ constexpr int ctas_of(int warps) { return 148 * resident(warps); }
 constexpr float SLACK = 8.f;  // a maximum is raised when a score passes it by this much (weights up to 2^8, where f16 parts are as good)
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -137,33 +139,131 @@ __device__ __forceinline__ void finish(const Attn4Args& a, int t, int h, int col
     store_act(a.out, a.out_dtype, ((int64_t)t * a.H + h) * a.V + col, acc * f / L * gate);
 }
 
-// grid (row tiles * parts, key heads * head blocks, 1), clusters along z: (row tile, part, rank) share nothing but the merge
-template <int NK, int NV, bool UNITS>
-__global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_constant__ Attn4Args a, const __grid_constant__ b200seq_step st) {
+constexpr int MAX_TILES = 1024;             // row tiles whose keys are dealt out evenly
+constexpr int HEADER = MAX_TILES + 8;       // floats of the work area in front of the parts: CTAs that have work, key tiles of a head, first key tile of every row tile
+
+// the r-th of the step's row tiles: its entry, first token and number of tokens (0: there is none, or its positions have no pages)
+__device__ __forceinline__ int row_tile(const Attn4Args& a, const b200seq_step& st, int i, int& e, int& t0, int& p0) {
+    int nq = 1;
+    if (st.T == st.B) {
+        if (i >= st.T) return 0;
+        e = t0 = i;
+    } else if (!attn_find_tile(st, i, a.QT, e, t0, nq)) {
+        return 0;
+    }
+    p0 = st.tok_pos[t0];
+    if (p0 < 0 || (p0 + nq - 1) / st.block_size >= st.max_blocks) {
+        atomicOr(a.err, 1);
+        return 0;
+    }
+    return nq;
+}
+
+// The keys of all row tiles and heads as one list of key tiles, head by head, dealt out evenly to the CTAs.
+struct Deal {
+    int64_t begin, end, total;
+    int per_head;       // key tiles of one head
+};
+__device__ __forceinline__ int64_t deal_begin(int64_t total, int ctas, int c) { return total * c / ctas; }
+__device__ __forceinline__ int deal_owner(int64_t total, int ctas, int64_t i) { return (int)(((i + 1) * ctas - 1) / total); }   // the CTA that has tile i
+
+// first[t]: key tiles of the row tiles before t (all threads; first: shared memory, MAX_TILES + 1)
+template <int WARPS>
+__device__ __forceinline__ int deal_tiles(const Attn4Args& a, const b200seq_step& st, int tiles, int* first, int* sums) {
+    constexpr int PER = (MAX_TILES + WARPS * 32 - 1) / (WARPS * 32);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int n[PER], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int tile = threadIdx.x * PER + i;
+        int e, t0, p0, nq = 0;
+        n[i] = 0;
+        if (tile < tiles) nq = row_tile(a, st, tile, e, t0, p0);
+        if (nq) n[i] = KeySpan<KT>(a, p0, p0 + nq - 1).total;
+        sum += n[i];
+    }
+    int upto = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int before = upto - sum, all = 0;
+    for (int w = 0; w < WARPS; ++w) {
+        before += w < warp ? sums[w] : 0;
+        all += sums[w];
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        if ((int)threadIdx.x * PER + i < MAX_TILES) first[threadIdx.x * PER + i] = before;
+        before += n[i];
+    }
+    if (threadIdx.x == 0) first[MAX_TILES] = all;
+    __syncthreads();
+    return all;
+}
+
+// Not STREAM: grid (row tiles, key heads * head blocks, cluster), a cluster's CTAs share a row tile's keys.  STREAM: ctas_of(warps) blocks, which share the keys of all row tiles evenly;
+// a row tile that ends up in several leaves its parts in the work area.
+template <int WARPS, int NK, int NV, bool UNITS, bool STREAM>
+__global__ void __launch_bounds__(WARPS * 32, resident(WARPS)) attn4_kernel(const __grid_constant__ Attn4Args a, const __grid_constant__ b200seq_step st) {
     chain_enter();
     extern __shared__ __align__(16) uint8_t smem[];
     constexpr int KB = NK * 320, HALF = (NK + NV) * 320, STAGE = 2 * HALF, MV = 32 * NV + 4;
+    auto both = [](const float (&x)[4]) { return tcsplit::add2(tcsplit::pk(x[0], x[1]), tcsplit::pk(x[2], x[3])); };      // a product's rows of high and of low parts
     __shared__ __align__(16) uint4 qfrag[(NK * 2 + 1) * 32];
-    __shared__ float factor_sm[WARPS * ROWS];
+    __shared__ int first[STREAM ? MAX_TILES + 1 : 1], warp_sums[STREAM ? WARPS : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     const int D = a.D, V = a.V, R = a.H / a.G, bs = st.block_size, rank = blockIdx.z;
-    const int tile_no = blockIdx.x / a.parts, seg = blockIdx.x - tile_no * a.parts;
-    int e, t0, nq;
-    if (st.T == st.B) e = t0 = tile_no, nq = 1;
-    else if (!attn_find_tile(st, tile_no, a.QT, e, t0, nq)) return;      // (all CTAs of a cluster alike)
-    const int g = blockIdx.y / a.HB, hb = blockIdx.y - g * a.HB, h0 = g * R + hb * a.Rb, nh = min(a.Rb, R - hb * a.Rb);
-    const int p0 = st.tok_pos[t0], hi = p0 + nq - 1;
-    const int32_t* bt = st.block_table + (int64_t)e * st.max_blocks;
-    if (p0 < 0 || hi / bs >= st.max_blocks) {
-        if (threadIdx.x == 0) atomicOr(a.err, 1);
-        return;
+    int64_t pos = 0, begin = 0, end = 1, total = 0;
+    int per_head = 0;
+    if (STREAM) {
+        per_head = deal_tiles<WARPS>(a, st, a.tiles, first, warp_sums);
+        total = (int64_t)per_head * a.heads;
+        const int64_t want = (total + WARPS - 1) / WARPS;
+        const int ctas = (int)(want < gridDim.x ? want : gridDim.x);
+        if (blockIdx.x == 0) {
+            int* head = reinterpret_cast<int*>(a.part);
+            for (int i = threadIdx.x; i <= a.tiles; i += WARPS * 32) head[2 + i] = first[i < MAX_TILES ? i : MAX_TILES];
+            if (threadIdx.x == 0) head[0] = ctas, head[1] = per_head;
+        }
+        if ((int)blockIdx.x >= ctas) return;
+        begin = pos = deal_begin(total, ctas, blockIdx.x), end = deal_begin(total, ctas, blockIdx.x + 1);
     }
+  do {
+    int e, t0, nq, p0, unit, from = 0, to = 0;
+    bool whole = false;
+    if (STREAM) {
+        if (pos >= end) break;
+        unit = (int)(pos / per_head);
+        const int at = (int)(pos - (int64_t)unit * per_head);
+        int lo = 0, up = a.tiles;                     // the row tile of key tile `at`
+        while (up - lo > 1) {
+            const int mid = (lo + up) >> 1;
+            if (first[mid] <= at) lo = mid;
+            else up = mid;
+        }
+        nq = row_tile(a, st, lo, e, t0, p0);
+        const int n = (lo + 1 < MAX_TILES ? first[lo + 1] : first[MAX_TILES]) - first[lo];
+        from = at - first[lo];
+        to = end - pos < n - from ? from + (int)(end - pos) : n;
+        whole = from == 0 && to == n;
+    } else {
+        unit = blockIdx.y;
+        nq = row_tile(a, st, blockIdx.x, e, t0, p0);
+        if (!nq) return;                              // (all CTAs of a cluster alike)
+    }
+    const int g = unit / a.HB, hb = unit - g * a.HB, h0 = g * R + hb * a.Rb, nh = min(a.Rb, R - hb * a.Rb);
+    const int hi = p0 + nq - 1;
+    const int32_t* bt = st.block_table + (int64_t)e * st.max_blocks;
     const KeySpan<KT> span(a, p0, hi);
     const int lo_last = RowSpan(a, hi).lo;
     // ---- keys into the ring: tiles me, me + walkers, ...; the first key and the pages of a tile are looked up a tile ahead of its copies ----
     const uint32_t ring = tcpair::sa(smem) + warp * (STAGES * STAGE);
-    const int walkers = a.parts * a.cluster * WARPS, me = (seg * a.cluster + rank) * WARPS + warp;
-    const int nt = span.total > me ? (span.total - me + walkers - 1) / walkers : 0;
+    const int walkers = STREAM ? WARPS : a.cluster * WARPS, me = STREAM ? from + warp : rank * WARPS + warp, last = STREAM ? to : span.total;
+    const int nt = last > me ? (last - me + walkers - 1) / walkers : 0;
     const int upp = bs >> 4, Gv = a.G / a.vdiv;                                  // units of a page
     const uint32_t kpage = (uint32_t)(a.G * upp * (NK * 320)), vpage = (uint32_t)(Gv * upp * (NV * 320));   // (below 2^31: checked by the caller)
     const bool kpar = lane < 4 * NK;
@@ -206,11 +306,11 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
     };
     lookup();
     int key0 = key_n;
-    issue(0);
     // ---- the rows: q as A fragments (eight neighbouring values of every group a thread), their factors and their parts against (s, m); by the first warp ----
     const int tq = r / a.Rb, hr = r - tq * a.Rb;
     const bool live = tq < nq && hr < nh;
     const RowSpan rs(a, p0 + (live ? tq : 0));
+    issue(0);
     if (warp == 0) {
         const float* src = a.q + (int64_t)(t0 + tq) * a.ld + (int64_t)(h0 + hr) * D;
         float x[NK][8], mx = 0.f;
@@ -303,7 +403,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
                     const uint32_t w = kw[n][k], w8 = w >> 8;
                     mma16816(acc, f[0], w & 0x000F000Fu, w & 0x00F000F0u, none);
                     mma16816(acc, f[1], w8 & 0x000F000Fu, w8 & 0x00F000F0u, acc);
-                    zc[n] = tcsplit::fma2(tcsplit::add2(tcsplit::pk(acc[0], acc[1]), tcsplit::pk(acc[2], acc[3])), tcsplit::pk(par_s(kp[2 * n][k]), par_s(kp[2 * n + 1][k])), zc[n]);
+                    zc[n] = tcsplit::fma2(both(acc), tcsplit::pk(par_s(kp[2 * n][k]), par_s(kp[2 * n + 1][k])), zc[n]);
                 }
             }
 #pragma unroll
@@ -312,7 +412,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
                 if (c < NK) lds<1>(ks + NK * 256 + ((r + 8 * n) * NK + c) * 4, b);
                 float acc[4];
                 mma16816(acc, make_uint4(qm.x, qm.y, 0u, 0u), b[0], 0u, none);
-                tcsplit::upk(tcsplit::fma2(zc[n], up24, tcsplit::add2(tcsplit::pk(acc[0], acc[1]), tcsplit::pk(acc[2], acc[3]))), z[4 * s + 2 * n], z[4 * s + 2 * n + 1]);
+                tcsplit::upk(tcsplit::fma2(zc[n], up24, both(acc)), z[4 * s + 2 * n], z[4 * s + 2 * n + 1]);
             }
         }
         if (a.softcap > 0.f) {
@@ -378,7 +478,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
             float acc[4];
             mma16816(acc, pa[0], bp[0][0], bp[0][1], none);
             mma16816(acc, pa[1], bp[1][0], bp[1][1], acc);
-            os = tcsplit::add2(os, tcsplit::add2(tcsplit::pk(acc[0], acc[1]), tcsplit::pk(acc[2], acc[3])));
+            os = tcsplit::add2(os, both(acc));
         }
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -398,7 +498,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
                 float acc[4];
                 mma16816(acc, pa[0], b[0][0], b[0][1], none);
                 mma16816(acc, pa[1], b[1][0], b[1][1], acc);
-                o[4 * k + i4] = tcsplit::add2(o[4 * k + i4], tcsplit::add2(tcsplit::pk(acc[0], acc[1]), tcsplit::pk(acc[2], acc[3])));
+                o[4 * k + i4] = tcsplit::add2(o[4 * k + i4], both(acc));
             }
         }
         key0 = key_after;
@@ -425,76 +525,105 @@ __global__ void __launch_bounds__(WARPS * 32, 2) attn4_kernel(const __grid_const
         }
     }
     __syncthreads();
-    const int rows = nq * nh, cluster = a.cluster;
-    // every row's maximum and sum over the warps, and the factor of each warp's values
-    float M = -INFINITY, L = 0.f;
-    if (threadIdx.x < WARPS * ROWS) {
-        const int m = threadIdx.x & (ROWS - 1), w = threadIdx.x / ROWS;
-        for (int i = 0; i < WARPS; ++i) M = fmaxf(M, all[(i * ROWS + m) * MV]);
-        for (int i = 0; i < WARPS; ++i) {
-            const float li = all[(i * ROWS + m) * MV + 1], f = li == 0.f ? 0.f : tcsplit::ex2(all[(i * ROWS + m) * MV] - M);   // (0: no key that the row sees)
-            L = fmaf(li, f, L);
-            if (i == w) factor_sm[w * ROWS + m] = f;
+    // A warp takes a row (and row + WARPS): its maximum and sum over the warps and the factor of each one's values, then the values.
+    const int cluster = STREAM ? 1 : a.cluster;
+#pragma unroll 1
+    for (int row = warp; row < ROWS; row += WARPS) {
+        const int rt = row / a.Rb, rh = row - rt * a.Rb;
+        if (rt >= nq || rh >= nh) continue;
+        const float* const at = all + row * MV;
+        float f[WARPS], M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) M = fmaxf(M, at[w * (ROWS * MV)]);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float lw = at[w * (ROWS * MV) + 1];
+            f[w] = lw == 0.f ? 0.f : tcsplit::ex2(at[w * (ROWS * MV)] - M);      // (0: no key that the row sees)
+            L = fmaf(lw, f[w], L);
         }
-    }
-    __syncthreads();
-    if (threadIdx.x < ROWS) all[threadIdx.x * MV] = M, all[threadIdx.x * MV + 1] = L;     // (the first warp's place)
-    if (cluster > 1 || a.parts > 1) {
-        for (int i = threadIdx.x; i < ROWS * V; i += WARPS * 32) {
-            const int m = i / V, col = i - m * V;
+        float* const pp = STREAM ? a.part + HEADER + ((int64_t)((int)blockIdx.x * 2 + (pos != begin)) * ROWS + row) * (V + 4) : nullptr;
+        if (STREAM && !whole && lane == 0) pp[0] = M, pp[1] = L;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int col = 32 * i + lane;
             float acc = 0.f;
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) acc = fmaf(all[(w * ROWS + m) * MV + 4 + col], factor_sm[w * ROWS + m], acc);
-            all[m * MV + 4 + col] = acc;
+            for (int w = 0; w < WARPS; ++w) acc = fmaf(at[w * (ROWS * MV) + 4 + col], f[w], acc);
+            if (col >= V) continue;
+            if (STREAM && !whole) pp[4 + col] = acc;
+            else if (cluster == 1) finish(a, t0 + rt, h0 + rh, col, M, L, acc);
+            else all[row * MV + 4 + col] = acc;                                  // (the first warp's place, whose old value this thread alone has read)
         }
-        if (cluster > 1) tcpair::cluster_sync();
+        __syncwarp();
+        if (cluster > 1 && lane == 0) all[row * MV] = M, all[row * MV + 1] = L;
     }
-    if (cluster == 1) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < rows * V; i += WARPS * 32) {
-            const int m = i / V, col = i - m * V, tq_ = m / nh, hr_ = m - tq_ * nh, row = tq_ * a.Rb + hr_, t = t0 + tq_, h = h0 + hr_;
-            float acc = 0.f;
-            if (a.parts == 1) {
+    if (cluster > 1) {   // the CTAs of the cluster, each of which has a share of the rows' values
+        tcpair::cluster_sync();
+        const uint32_t base = tcpair::sa(all);
+        const int rows = nq * nh;
+        for (int i = rank * (WARPS * 32) + threadIdx.x; i < rows * V; i += cluster * (WARPS * 32)) {
+            const int m = i / V, col = i - m * V, tq_ = m / nh, hr_ = m - tq_ * nh;
+            const uint32_t pr = base + (tq_ * a.Rb + hr_) * MV * 4;
+            float mw[8], lw[8], aw[8], top = -INFINITY, sum = 0.f, acc = 0.f;
 #pragma unroll
-                for (int w = 0; w < WARPS; ++w) acc = fmaf(all[(w * ROWS + row) * MV + 4 + col], factor_sm[w * ROWS + row], acc);
-                finish(a, t, h, col, all[row * MV], all[row * MV + 1], acc);
-            } else {
-                float* pp = a.part + (((int64_t)t * a.H + h) * a.parts + seg) * (V + 4);
-                if (col == 0) pp[0] = all[row * MV], pp[1] = all[row * MV + 1];
-                pp[4 + col] = all[row * MV + 4 + col];
+            for (int w = 0; w < 8; ++w) {
+                const bool in = w < cluster;
+                mw[w] = in ? ld_cluster(pr, w) : -INFINITY, lw[w] = in ? ld_cluster(pr + 4, w) : 0.f, aw[w] = in ? ld_cluster(pr + 16 + 4 * col, w) : 0.f;
+                top = fmaxf(top, mw[w]);
             }
-        }
-        return;
-    }
-    // and over the CTAs of the cluster, each of which has a share of the results
-    const uint32_t base = tcpair::sa(all);
-    for (int i = rank * (WARPS * 32) + threadIdx.x; i < rows * V; i += cluster * (WARPS * 32)) {
-        const int m = i / V, col = i - m * V, tq_ = m / nh, hr_ = m - tq_ * nh, t = t0 + tq_, h = h0 + hr_;
-        const uint32_t pr = base + (tq_ * a.Rb + hr_) * MV * 4;
-        float mw[8], lw[8], aw[8], top = -INFINITY, sum = 0.f, acc = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) {
-            const bool in = w < cluster;
-            mw[w] = in ? ld_cluster(pr, w) : -INFINITY, lw[w] = in ? ld_cluster(pr + 4, w) : 0.f, aw[w] = in ? ld_cluster(pr + 16 + 4 * col, w) : 0.f;
-            top = fmaxf(top, mw[w]);
+            for (int w = 0; w < 8; ++w) {
+                const float f = lw[w] == 0.f ? 0.f : tcsplit::ex2(mw[w] - top);
+                sum = fmaf(lw[w], f, sum), acc = fmaf(aw[w], f, acc);
+            }
+            finish(a, t0 + tq_, h0 + hr_, col, top, sum, acc);
         }
-#pragma unroll
-        for (int w = 0; w < 8; ++w) {
-            const float f = lw[w] == 0.f ? 0.f : tcsplit::ex2(mw[w] - top);
-            sum = fmaf(lw[w], f, sum), acc = fmaf(aw[w], f, acc);
-        }
-        if (a.parts == 1) {
-            finish(a, t, h, col, top, sum, acc);
-        } else {
-            float* pp = a.part + (((int64_t)t * a.H + h) * a.parts + seg) * (V + 4);
-            if (col == 0) pp[0] = top, pp[1] = sum;
-            pp[4 + col] = acc;
-        }
+        tcpair::cluster_sync();   // nobody leaves while its shared memory is read
     }
-    tcpair::cluster_sync();   // nobody leaves while its shared memory is read
+    if (STREAM) pos += to - from, __syncthreads();    // shared memory is the next row tile's
+  } while (STREAM);
 }
 
-// grid (T, H): the clusters' parts of one (token, head), in order
+// grid (row tiles, key heads * head blocks, blocks of 32 values), a warp a row: the parts of a row tile that several CTAs have, in order
+__global__ void __launch_bounds__(ROWS * 32) attn4_gather_kernel(const __grid_constant__ Attn4Args a, const __grid_constant__ b200seq_step st) {
+    chain_enter();
+    __shared__ float factor[ROWS][ctas_of(4)];
+    const int* head = reinterpret_cast<const int*>(a.part);
+    const int ctas = head[0], per_head = head[1], n = head[3 + blockIdx.x] - head[2 + blockIdx.x];
+    if (n == 0) return;
+    const int64_t total = (int64_t)per_head * a.heads, u0 = (int64_t)blockIdx.y * per_head + head[2 + blockIdx.x];
+    const int c0 = deal_owner(total, ctas, u0), c1 = deal_owner(total, ctas, u0 + n - 1);
+    if (c0 == c1) return;                             // one CTA had it all
+    int e, t0, p0;
+    const int nq = row_tile(a, st, blockIdx.x, e, t0, p0);
+    const int R = a.H / a.G, g = blockIdx.y / a.HB, hb = blockIdx.y - g * a.HB, h0 = g * R + hb * a.Rb, nh = min(a.Rb, R - hb * a.Rb);
+    const int row = threadIdx.x >> 5, lane = threadIdx.x & 31, tq = row / a.Rb, hr = row - tq * a.Rb, step = a.V + 4;
+    if (tq >= nq || hr >= nh) return;
+    // a CTA's part of this row tile lies in its first place if its share begins there or before, else in its second
+    const int64_t pitch = (int64_t)2 * ROWS * step;
+    const float* const parts = a.part + HEADER + c0 * pitch + (int64_t)row * step;
+    const float* const own = deal_begin(total, ctas, c0) != u0 ? parts + (int64_t)ROWS * step : parts;      // c0's
+    const int np = c1 - c0 + 1;
+    auto part = [&](int i) { return i ? parts + i * pitch : own; };
+    float M = -INFINITY, L = 0.f;
+    for (int i = lane; i < np; i += 32) M = fmaxf(M, part(i)[0]);
+    M = warp_max(M);
+    for (int i = lane; i < np; i += 32) {
+        const float l = part(i)[1], f = l == 0.f ? 0.f : tcsplit::ex2(part(i)[0] - M);      // (0: no key that the row sees)
+        factor[row][i] = f;
+        L = fmaf(l, f, L);
+    }
+    L = warp_sum(L);
+    __syncwarp();
+    const int col = blockIdx.z * 32 + lane;
+    if (col >= a.V) return;
+    float acc = own[4 + col] * factor[row][0];
+#pragma unroll 8
+    for (int i = 1; i < np; ++i) acc = fmaf(parts[i * pitch + 4 + col], factor[row][i], acc);
+    finish(a, t0 + tq, h0 + hr, col, M, L, acc);
+}
+
+// grid (T, H): the parts that the tensor-core kernel leaves of one (token, head), in order
 __global__ void attn4_merge_kernel(const __grid_constant__ Attn4Args a) {
     chain_enter();
     const int t = blockIdx.x, h = blockIdx.y, n = a.parts, step = a.V + 4;
@@ -511,10 +640,10 @@ __global__ void attn4_merge_kernel(const __grid_constant__ Attn4Args a) {
     }
 }
 
-template <int NK, int NV, bool UNITS>
+template <int WARPS, int NK, int NV, bool UNITS, bool STREAM>
 cudaError_t launch(const Attn4Args& a, const b200seq_step& st, dim3 grid, cudaStream_t cs) {
     constexpr int ring = WARPS * STAGES * 2 * (NK + NV) * 320, parts = WARPS * ROWS * (32 * NV + 4) * 4, smem = ring > parts ? ring : parts;
-    const auto kernel = attn4_kernel<NK, NV, UNITS>;
+    const auto kernel = attn4_kernel<WARPS, NK, NV, UNITS, STREAM>;
     static bool ready[16] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -532,21 +661,6 @@ cudaError_t launch(const Attn4Args& a, const b200seq_step& st, dim3 grid, cudaSt
     e = cudaLaunchKernelEx(&cfg, kernel, a, st);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
-template <int NK, int NV>
-cudaError_t launch_units(const Attn4Args& a, const b200seq_step& st, dim3 grid, cudaStream_t cs) {
-    return st.block_size % 16 == 0 ? launch<NK, NV, true>(a, st, grid, cs) : launch<NK, NV, false>(a, st, grid, cs);
-}
-template <int NK>
-cudaError_t launch_values(int nv, const Attn4Args& a, const b200seq_step& st, dim3 grid, cudaStream_t cs) {
-    return nv == 1 ? launch_units<NK, 1>(a, st, grid, cs) : (nv == 2 ? launch_units<NK, 2>(a, st, grid, cs) : launch_units<NK, 4>(a, st, grid, cs));
-}
-
-// How many CTAs share a row tile's keys: as many as put two on every SM (a CTA's 8 warps hide half of the latency), each with 4 tiles of keys or more when the block
-// table is as long as its sequence.  Up to 8 are a cluster; beyond that several clusters.
-struct Plan {
-    int64_t tiles;
-    int heads, cluster, parts;
-};
 // the most keys a token can see
 int64_t most_keys(const b200seq_step& st, const b200seq_attn_desc& d, int tokens) {
     int64_t keys = (int64_t)st.max_blocks * st.block_size;
@@ -554,18 +668,64 @@ int64_t most_keys(const b200seq_step& st, const b200seq_attn_desc& d, int tokens
     if (d.window > 0 && (int64_t)d.window + d.keep_first + tokens < keys) keys = (int64_t)d.window + d.keep_first + tokens;
     return keys;
 }
+// How the keys of a step are shared.  Row tiles and heads go to a CTA each, or to a cluster of up to 8 while there are CTAs for all and keys for all their warps.  Few of them
+// with many keys are dealt out evenly, with a second launch for those that several CTAs have; that costs about 8 us a row tile begun and 5 for the launch (32 sequences, 256
+// row tiles and heads: 65 us dealt, 55 not; one sequence of 131072 keys: 62 dealt, 110 in clusters).  CTAs have the 8 or 4 warps whose last wave is the fuller one (256 row tiles
+// and heads of 128, 3000 keys: 55 us with 8, 77 with 4; 16 x 5 tokens, 384 of 64, 1500 keys: 29 with 8, 24 with 4); the small ones for heads of up to 64 where that is the same.
+struct Plan {
+    int64_t tiles, real;     // row tiles: upper bound; as many as there are if all entries are equally long
+    int heads, cluster, warps, ctas;
+    bool dealt;
+};
 Plan plan(const b200seq_step& st, const b200seq_attn_desc& d) {
     Plan p;
     const int R = d.H / d.G, Rb = R < ROWS ? R : ROWS, QT = ROWS / Rb;
     p.heads = d.G * ((R + Rb - 1) / Rb);
     p.tiles = st.T == st.B ? st.T : ((int64_t)st.T + QT - 1) / QT + st.B;
-    const int64_t keys = most_keys(st, d, QT);
-    int64_t want = 2 * 148 / (p.tiles * p.heads), most = keys / (4 * KT);
-    want = want < most ? want : most;
-    p.cluster = want >= 8 ? 8 : (want >= 4 ? 4 : (want >= 2 ? 2 : 1));
-    p.parts = want >= 16 ? (int)(want / 8 < 16 ? want / 8 : 16) : 1;
+    const int64_t each = ((int64_t)st.T + st.B - 1) / st.B;
+    p.real = st.B * ((each + QT - 1) / QT);
+    const int64_t units = p.real * p.heads, key_tiles = (most_keys(st, d, QT) + KT - 1) / KT;
+    const bool small = d.D <= 64 && d.V <= 64;
+    double best = -1.0;
+    for (int warps : {small ? 4 : 8, small ? 8 : 4}) {
+        const int ctas = ctas_of(warps);
+        int64_t want = ctas / units, most = (key_tiles + warps - 1) / warps;
+        want = want < most ? want : most;
+        const int cluster = want >= 8 ? 8 : (want >= 4 ? 4 : (want >= 2 ? 2 : 1));
+        const int64_t n = units * cluster, waves = (n + ctas - 1) / ctas;
+        const double full = (double)n / (double)(waves * ctas);
+        if (full > best * 1.05) best = full, p.warps = warps, p.ctas = ctas, p.cluster = cluster;
+    }
+    p.dealt = st.block_size % 16 == 0 && p.tiles <= MAX_TILES && units * p.cluster * 2 <= p.ctas && key_tiles > 8ll * p.cluster * p.warps;
+    if (p.dealt) p.cluster = 1, p.warps = small ? 4 : 8, p.ctas = ctas_of(p.warps);
     return p;
 }
+template <int NK, int NV>
+cudaError_t launch_form(const Attn4Args& a, const b200seq_step& st, dim3 grid, const Plan& p, cudaStream_t cs) {
+    if (st.block_size % 16) return p.warps == 8 ? launch<8, NK, NV, false, false>(a, st, grid, cs) : launch<4, NK, NV, false, false>(a, st, grid, cs);
+    if (p.dealt) return launch<(NK == 4 || NV == 4 ? 8 : 4), NK, NV, true, true>(a, st, grid, cs);
+    return p.warps == 8 ? launch<8, NK, NV, true, false>(a, st, grid, cs) : launch<4, NK, NV, true, false>(a, st, grid, cs);
+}
+template <int NK>
+cudaError_t launch_values(int nv, const Attn4Args& a, const b200seq_step& st, dim3 grid, const Plan& p, cudaStream_t cs) {
+    return nv == 1 ? launch_form<NK, 1>(a, st, grid, p, cs) : (nv == 2 ? launch_form<NK, 2>(a, st, grid, p, cs) : launch_form<NK, 4>(a, st, grid, p, cs));
+}
+// Which kernel is the faster one, from the key tiles a CTA has at most.  us, fitted to 57 steps of 8 to 288 tokens, timed with each of the two (the choice is at most 12 % behind the faster one).  Here: a wave of
+// CTAs takes 4 (5 with heads above 64) and 1.5 (3.6) a key tile of 32 and warp; keys that are dealt out 10, and 1290 (675) key tiles a us.  On the tensor cores: 7.5 (9; f32
+// 11) a CTA and 0.8 (0.75; f32 1.4) a key tile of 64, 4 more for keys in several parts.  Measured, us, here / there, 32 query heads of 8 key heads of 64 (of 128):
+//   1 x 64 tokens                6 /  8 ( 7 / 10)     16 x 9 behind 1500   43 / 28 (66 / 31)     32 x 2 behind 2000   34 / 64 (45 / 73)
+//   1 x 32 behind 4000          22 / 22 (34 / 25)      4 x 8 behind 8000   56 / 36 (83 / 39)      4 x 64 behind 300   27 / 13 (38 / 14)
+bool tc_is_faster(const b200seq_step& st, const b200seq_attn_desc& d, const Plan& p, const Attn4TcPlan& tp, bool f32) {
+    const bool small = d.D <= 64 && d.V <= 64;
+    const double keys = (double)most_keys(st, d, 0), kt = (keys + KT - 1) / KT, units = (double)p.real * p.heads;
+    const double waves = units * p.cluster / p.ctas, share = kt / (p.warps * p.cluster);
+    const double here = p.dealt ? 10.0 + units * kt / (small ? 1290.0 : 675.0) : (waves < 1.0 ? 1.0 : waves) * ((small ? 4.0 : 5.0) + (small ? 1.5 : 3.6) * (share < 1.0 ? 1.0 : share)) + 2.0;
+    const double set_up = small ? 7.5 : (f32 ? 11.0 : 9.0), each = small ? 0.8 : (f32 ? 1.4 : 0.75);
+    const int64_t tc_waves = (tp.real * tp.parts + 147) / 148;
+    const double there = (double)tc_waves * (set_up + each * (keys / 64.0 / tp.parts + 0.5)) + 2.0 + (tp.parts > 1 ? 4.0 : 0.0);
+    return there < here;
+}
+size_t plan_floats(const Plan& p, int V) { return p.dealt ? (size_t)HEADER + (size_t)p.ctas * 2 * ROWS * (V + 4) : 0; }
 
 }  // namespace
 
@@ -577,12 +737,13 @@ extern "C" {
 
 size_t b200seq_attn_kv4_scratch_floats(const b200seq_step* st, const b200seq_attn_desc* d) {
     if (!st || !d || st->T < 1 || st->B < 1 || st->block_size < 1 || st->max_blocks < 1 || d->H < 1 || d->G < 1 || d->H % d->G || d->V < 1) return 0;
-    int parts = plan(*st, *d).parts;
-    if (attn4_tc_takes(*st, d->H, d->G, d->D, d->V)) {
-        const int tc = attn4_tc_plan(*st, d->H, d->G, d->D, d->V, most_keys(*st, *d, 0)).parts;
-        parts = tc > parts ? tc : parts;
+    size_t need = plan_floats(plan(*st, *d), d->V);
+    if (attn4_tc_takes(d->D, d->V)) {
+        const int parts = attn4_tc_plan(*st, d->H, d->G, d->D, d->V, most_keys(*st, *d, 0)).parts;
+        const size_t tc = parts > 1 ? (size_t)st->T * d->H * parts * (d->V + 4) : 0;
+        need = tc > need ? tc : need;
     }
-    return parts > 1 ? (size_t)st->T * d->H * parts * (d->V + 4) : 0;
+    return need;
 }
 
 int b200seq_attn_kv4(const float* proj, int64_t ld, const b200seq_step* st, const b200seq_attn_desc* d, const void* kpool, const void* vpool, void* out, int out_dtype,
@@ -612,33 +773,34 @@ int b200seq_attn_kv4(const float* proj, int64_t ld, const b200seq_step* st, cons
     a.softcap = d->softcap, a.out = out, a.out_dtype = out_dtype, a.err = error_flag_dev();
     cudaStream_t cs = (cudaStream_t)stream;
     if (d->H > 65535) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_kv4: too many heads");
-    auto merge = [&]() -> int {
-        if (a.parts > 1) {
-            launch_chained(attn4_merge_kernel, dim3(st->T, d->H), d->V <= 64 ? 64 : 128, 0, cs, a);
-            SEQ_LAUNCH_CHECK("attn_kv4 merge");
-        }
-        return 0;
-    };
-    if (a.vec && attn4_tc_takes(*st, d->H, d->G, d->D, d->V)) {
-        Attn4TcPlan tp = attn4_tc_plan(*st, d->H, d->G, d->D, d->V, most_keys(*st, *d, 0));
+    Plan p = plan(*st, *d);
+    Attn4TcPlan tp = attn4_tc_plan(*st, d->H, d->G, d->D, d->V, most_keys(*st, *d, 0));
+    if (a.vec && attn4_tc_takes(d->D, d->V) && tc_is_faster(*st, *d, p, tp, out_dtype == B200SEQ_F32)) {
         if (tp.parts > 1 && (!scratch || scratch_floats < (size_t)st->T * d->H * tp.parts * (d->V + 4))) tp.parts = 1;
         if ((int64_t)d->G * tp.HB * tp.tiles > 0x7fffffff) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_kv4: too many heads or tokens");
         a.part = scratch, a.parts = tp.parts;
         const cudaError_t e = attn4_tc_launch(a, *st, tp, cs);
         if (e != cudaSuccess) return cuda_status(e, "attn_kv4");
         count_launch();
-        return merge();
+        if (tp.parts > 1) {
+            launch_chained(attn4_merge_kernel, dim3(st->T, d->H), d->V <= 64 ? 64 : 128, 0, cs, a);
+            SEQ_LAUNCH_CHECK("attn_kv4 merge");
+        }
+        return 0;
     }
-    Plan p = plan(*st, *d);
-    if (p.parts > 1 && (!scratch || scratch_floats < (size_t)st->T * d->H * p.parts * (d->V + 4))) p.parts = 1;
-    a.cluster = p.cluster, a.parts = p.parts, a.part = scratch;
-    if (p.heads > 65535 || p.tiles * p.parts > 0x7fffffff) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_kv4: too many heads or tokens");
-    const dim3 grid((unsigned)(p.tiles * p.parts), (unsigned)p.heads, (unsigned)p.cluster);
+    if (p.dealt && (!scratch || scratch_floats < plan_floats(p, d->V))) p.dealt = false;
+    if (p.heads > 65535 || p.tiles > 0x7fffffff) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_kv4: too many heads or tokens");
+    a.cluster = p.cluster, a.parts = 1, a.part = scratch, a.tiles = (int)p.tiles, a.heads = p.heads;
+    const dim3 grid = p.dealt ? dim3((unsigned)p.ctas) : dim3((unsigned)p.tiles, (unsigned)p.heads, (unsigned)p.cluster);
     const int nk = kv4_groups(d->D), nv = kv4_groups(d->V);
-    const cudaError_t e = nk == 1 ? launch_values<1>(nv, a, *st, grid, cs) : (nk == 2 ? launch_values<2>(nv, a, *st, grid, cs) : launch_values<4>(nv, a, *st, grid, cs));
+    const cudaError_t e = nk == 1 ? launch_values<1>(nv, a, *st, grid, p, cs) : (nk == 2 ? launch_values<2>(nv, a, *st, grid, p, cs) : launch_values<4>(nv, a, *st, grid, p, cs));
     if (e != cudaSuccess) return cuda_status(e, "attn_kv4");
     count_launch();
-    return merge();
+    if (p.dealt) {
+        launch_chained(attn4_gather_kernel, dim3((unsigned)p.tiles, (unsigned)p.heads, (unsigned)((d->V + 31) / 32)), ROWS * 32, 0, cs, a, *st);
+        SEQ_LAUNCH_CHECK("attn_kv4 gather");
+    }
+    return 0;
 }
 
 }  // extern "C"

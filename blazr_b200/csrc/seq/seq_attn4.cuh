@@ -20,8 +20,10 @@ struct Attn4Args {
     float softcap;
     void* out;                 // [T, H * V]
     int out_dtype;
-    int cluster, parts;        // CTAs of a cluster that share a row tile's keys, and clusters that do
-    float* part;               // [T][H][parts][V + 4] when parts > 1: maximum (base 2), sum, two unused, values
+    int cluster;               // CTAs of a cluster that share a row tile's keys
+    int tiles, heads;          // row tiles (bound), key heads * head blocks
+    int parts;                 // tensor-core kernel: CTAs that share a row tile's keys
+    float* part;               // work area.  Tensor-core kernel, parts > 1: [T][H][parts][V + 4] = maximum (base 2), sum, two unused, values
     int* err;
 };
 
@@ -55,7 +57,7 @@ struct Attn4TcPlan {
     int mt, Rb, HB, QT, parts;
     int64_t tiles, real;
 };
-bool attn4_tc_takes(const b200seq_step& st, int H, int G, int D, int V);
+bool attn4_tc_takes(int D, int V);
 Attn4TcPlan attn4_tc_plan(const b200seq_step& st, int H, int G, int D, int V, int64_t keys);
 cudaError_t attn4_tc_launch(Attn4Args a, const b200seq_step& st, const Attn4TcPlan& p, cudaStream_t cs);
 

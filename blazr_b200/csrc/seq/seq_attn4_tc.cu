@@ -720,10 +720,8 @@ cudaError_t run(const Attn4Args& a, const b200seq_step& st, dim3 grid, cudaStrea
 
 }  // namespace
 
-// Steps whose portions fill a quarter of a row tile or more, with whole 16-byte pieces of queries and keys and values of as many groups.
-bool attn4_tc_takes(const b200seq_step& st, int H, int G, int D, int V) {
-    return st.T > 16 && (int64_t)st.T * (H / G) >= 32ll * st.B && D % 8 == 0 && kv4_groups(D) == kv4_groups(V);
-}
+// What this kernel can do: whole 16-byte pieces of queries (the caller looks at addresses), keys and values of as many groups.
+bool attn4_tc_takes(int D, int V) { return D % 8 == 0 && kv4_groups(D) == kv4_groups(V); }
 
 // row tiles of 128 (256: two per CTA, heads of up to 64 and rows enough for all SMs)
 Attn4TcPlan attn4_tc_plan(const b200seq_step& st, int H, int G, int D, int V, int64_t keys) {
