@@ -124,7 +124,102 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4Rows a, float* _
     }
 }
 
-// b200seq_attn_prep_ex over 4-bit pages: grid (T), 256 threads, a warp per head unit; the unit's values are staged in the warp's slice of shared memory, biased,
+// b200seq_attn_prep_ex over 4-bit pages, for rows of whole 16-byte pieces (every head size, rotation and column that is a multiple of 8; norms over single heads).
+// LPR lanes have a head's row (4 for every group of 32), eight neighbouring values in a lane's registers; the rotation's other half comes from another lane.
+// A token's rows are split over `split` blocks of 128 threads.  Bounded by a chain of loads for single tokens (position, frequencies, then sines) and by
+// instructions for prompts.  us with rotation of halves and norms, rows as here / a warp to a head through shared memory (32 query heads of 8 key heads of 128):
+//   1 token  2.9 / 8.7      32 tokens  3.3 / 9.5      512  8.9 / 14.1      2048  26.3 / 49.9  (bytes alone: 12.8)
+template <int LPR>
+__global__ void __launch_bounds__(128) kv4_prep_rows_kernel(float* proj, int64_t ld, const b200seq_step st, const b200seq_attn_desc a, uint8_t* kpool, uint8_t* vpool,
+                                                            int split, int* err) {
+    chain_enter();
+    extern __shared__ __align__(16) float rot_sm[];   // cos | sin
+    constexpr int ROWS = 128 / LPR;
+    const int t = blockIdx.x / split, part = blockIdx.x - t * split, lane = threadIdx.x & 31, hl = threadIdx.x & (LPR - 1);
+    const int pos = st.tok_pos[t];
+    const int H = a.H, G = a.G, Gv = a.vg > 0 ? a.vg : G, np = a.rot_dims >> 1, nu = a.kv_shared ? H : H + G + Gv;
+    int o = 0;
+    const int64_t page = a.kv_shared ? -1 : kv4_page(st, t, o, err);
+    float* base = proj + (int64_t)t * ld;
+    bool odd = false, first = true;
+    for (int u0 = part * ROWS; u0 < nu; u0 += split * ROWS) {
+        const int u = u0 + (int)threadIdx.x / LPR;
+        const bool in = u < nu, isq = u < H, isk = !isq && u < H + G, turned = in && (isq || isk);
+        const int hh = isq ? u : (isk ? u - H : u - H - G), size = isq || isk ? a.D : a.V, n = in && 8 * hl < size ? 8 : 0;
+        const int col = (isq ? a.q_col : (isk ? a.k_col : a.v_col)) + hh * size + 8 * hl;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = 0.f;
+        if (n) {
+            const float4 v = ld4(base + col), w = ld4(base + col + 4);
+            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w, x[4] = w.x, x[5] = w.y, x[6] = w.z, x[7] = w.w;
+            if (a.in_bias) {
+                const float4 b = ld4(a.in_bias + col), c = ld4(a.in_bias + col + 4);
+                x[0] += b.x, x[1] += b.y, x[2] += b.z, x[3] += b.w, x[4] += c.x, x[5] += c.y, x[6] += c.z, x[7] += c.w;
+            }
+        }
+        if (first) {
+            for (int i = threadIdx.x; i < np; i += 128) {
+                float sn, cs;
+                sincosf((float)pos * a.rot_freq[i], &sn, &cs);
+                rot_sm[i] = cs * a.rot_scale, rot_sm[np + i] = sn * a.rot_scale;
+            }
+            __syncthreads();
+            first = false;
+        }
+        if (a.qk_eps >= 0.f) {
+            float ss = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+#pragma unroll
+            for (int m = 1; m < LPR; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+            if (turned && n) {
+                const float* w = isq ? a.q_norm_w : a.k_norm_w;
+                const float rinv = 1.0f / sqrtf(ss / (float)a.D + a.qk_eps);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] *= rinv;
+                if (w) {
+                    const float4 b = ld4(w + 8 * hl), c = ld4(w + 8 * hl + 4);
+                    x[0] *= b.x, x[1] *= b.y, x[2] *= b.z, x[3] *= b.w, x[4] *= c.x, x[5] *= c.y, x[6] *= c.z, x[7] *= c.w;
+                }
+            }
+        }
+        if (np > 0 && a.rot_half) {
+            const bool lower = 8 * hl < np, turns = turned && 8 * hl < 2 * np;
+            const int from = 8 * hl >= 2 * np ? lane : (lower ? lane + (np >> 3) : lane - (np >> 3)), i = lower ? 8 * hl : 8 * hl - np;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float other = __shfl_sync(0xffffffffu, x[j], from);
+                if (turns) x[j] = fmaf(x[j], rot_sm[i + j], (lower ? -other : other) * rot_sm[np + i + j]);
+            }
+        } else if (turned) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int i = 4 * hl + j;
+                if (i >= np) continue;
+                const float e = x[2 * j], f = x[2 * j + 1], cs = rot_sm[i], sn = rot_sm[np + i];
+                x[2 * j] = fmaf(e, cs, -f * sn), x[2 * j + 1] = fmaf(f, cs, e * sn);
+            }
+        }
+        if (isq) {
+            if (n) {
+                *reinterpret_cast<float4*>(base + col) = make_float4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<float4*>(base + col + 4) = make_float4(x[4], x[5], x[6], x[7]);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = 0.f;   // (a query is none of the values that are held)
+        }
+        if (page >= 0 && __any_sync(0xffffffffu, in && !isq)) {
+            const int NG = kv4_groups(size);
+            uint32_t param;
+            const uint32_t w = kv4_quantise(x, isq ? 0 : n, param, odd);
+            kv4_put(isk ? kpool : vpool, kv4_row(page, o, st.block_size, in && !isq ? hh : 0, isk ? G : Gv, NG), isk, hl, NG, w, param, in && !isq);
+        }
+    }
+    if (odd) atomicOr(err, KV4_ERR_RANGE);
+}
+
+// The same for every other row: grid (T), 256 threads, a warp per head unit; the unit's values are staged in the warp's slice of shared memory, biased,
 // normed, turned, and written back (queries) or quantised into the token's row.  Shared memory: rot_dims floats (cos | sin) + 8 * Dmax + 40.
 __global__ void kv4_prep_kernel(float* __restrict__ proj, int64_t ld, const b200seq_step st, const b200seq_attn_desc a, uint8_t* __restrict__ kpool,
                                 uint8_t* __restrict__ vpool, int Dmax, int* err) {
@@ -273,6 +368,16 @@ int b200seq_attn_prep_kv4(float* proj, int64_t ld, const b200seq_step* st, const
     if (st->T == 0) return 0;
     const int Dmax = d->D > d->V ? d->D : d->V;
     const size_t smem = (size_t)(d->rot_dims + 8 * Dmax + 40) * sizeof(float);
+    const int heads = d->H + (d->kv_shared ? 0 : d->G + (d->vg > 0 ? d->vg : d->G)), lpr = 4 * kv4_groups(Dmax), np = d->rot_dims / 2;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(proj) | reinterpret_cast<uintptr_t>(d->in_bias) | reinterpret_cast<uintptr_t>(d->q_norm_w) | reinterpret_cast<uintptr_t>(d->k_norm_w);
+    if (!d->norm_full && ((d->D | d->V) & 7) == 0 && ((ld | d->q_col | d->k_col | d->v_col) & 3) == 0 && (at & 15) == 0 && (!d->rot_half || (np & 7) == 0)) {
+        // as many blocks as eight an SM allow, or as a token has rows for
+        const int most = (heads * lpr + 127) / 128, want = 148 * 8 / st->T, split = want < 1 ? 1 : (want < most ? want : most);
+        const auto kernel = lpr == 4 ? kv4_prep_rows_kernel<4> : (lpr == 8 ? kv4_prep_rows_kernel<8> : kv4_prep_rows_kernel<16>);
+        launch_chained(kernel, st->T * split, 128, (size_t)(2 * np) * sizeof(float), (cudaStream_t)stream, proj, ld, *st, *d, (uint8_t*)kpool, (uint8_t*)vpool, split, error_flag_dev());
+        SEQ_LAUNCH_CHECK("attn_prep_kv4");
+        return 0;
+    }
     launch_chained(kv4_prep_kernel, st->T, 256, smem, (cudaStream_t)stream, proj, ld, *st, *d, (uint8_t*)kpool, (uint8_t*)vpool, Dmax, error_flag_dev());
     SEQ_LAUNCH_CHECK("attn_prep_kv4");
     return 0;

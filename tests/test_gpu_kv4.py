@@ -128,23 +128,19 @@ PREP = [
 ]
 
 
-@pytest.mark.parametrize("o", PREP, ids=lambda o: "-".join(o) or "plain")
-@pytest.mark.parametrize("D,bs", [(64, 16), (80, 16), (128, 5)])
-def test_prep_is_that_of_the_f32_cache(ops, o, D, bs):
-    """queries to f32 roundings, cached rows as what the f32 pool's rows become (a value that such a rounding moves over the middle between two codes may be a step off)"""
+def prep_case(ops, o, H, G, D, V, bs, entries, spare):
+    """rows that lie `spare` values further apart than they are long"""
     rng = np.random.default_rng(11)
-    H, G, V = 4, 2, D
-    entries = [(7, 0), (1, 40), (2, 15)]
     st, keep, slots, pages = step(ops, entries, bs, rng)
     t = lambda *s: torch.from_numpy(rng.standard_normal(s).astype(np.float32)).to(DEV)
     freq = torch.from_numpy((10000.0 ** (-np.arange(o["rot"] // 2) / 32)).astype(np.float32)).to(DEV) if "rot" in o else None
     full = o.get("norm_full", False)
     qw, kw = (t(H * D if full else D), t(G * D if full else D)) if o.get("weights") else (None, None)
-    bias = t(4096) if o.get("in_bias") else None
+    bias = t(8192) if o.get("in_bias") else None
     d = ops.attn_desc(H, G, D, V, 1.0, gated=False, qk_eps=o.get("qk_eps", -1.0), rot_freq=freq, rot_half=o.get("rot_half", False), rot_scale=1.1, q_norm_w=qw, k_norm_w=kw, norm_full=full,
                       in_bias=bias, values_from_keys=o.get("values_from_keys", False), value_heads=o.get("value_heads", 0), kv_shared=o.get("kv_shared", False))
     Gv = o.get("value_heads", 0) or G
-    rows = t(st.T, d.width + 3)
+    rows = t(st.T, d.width + spare)
     a, b = rows.clone(), rows.clone()
     kf, vf = torch.zeros(pages, bs, G, D, device=DEV), torch.zeros(pages, bs, Gv, V, device=DEV)
     k4, v4 = ops.kv4_pool(pages, bs, G, D, DEV), ops.kv4_pool(pages, bs, Gv, V, DEV)
@@ -166,6 +162,28 @@ def test_prep_is_that_of_the_f32_cache(ops, o, D, bs):
         at = np.arange(w) // 32
         assert (off <= step_[..., at] * 1.05 + 1e-5).all() and (off > 1e-5).mean() < 0.01
     assert ops.error_flags() == 0
+
+
+@pytest.mark.parametrize("o", PREP, ids=lambda o: "-".join(o) or "plain")
+@pytest.mark.parametrize("D,bs", [(64, 16), (80, 16), (128, 5)])
+def test_prep_is_that_of_the_f32_cache(ops, o, D, bs):
+    """queries to f32 roundings, cached rows as what the f32 pool's rows become (a value that such a rounding moves over the middle between two codes may be a step off)"""
+    prep_case(ops, o, 4, 2, D, D, bs, [(7, 0), (1, 40), (2, 15)], 3)
+
+
+@pytest.mark.parametrize("o", PREP, ids=lambda o: "-".join(o) or "plain")
+@pytest.mark.parametrize("H,G,D,V,bs,entries", [(4, 2, 64, 64, 16, [(7, 0), (1, 40), (2, 15)]), (5, 5, 80, 80, 16, [(1, 100)]), (6, 2, 128, 72, 5, [(3, 1), (1, 9)]),
+                                                (8, 2, 64, 24, 16, [(600, 3), (700, 0)]), (32, 8, 128, 128, 16, [(1, 700)] * 33)])
+def test_prep_of_rows_in_whole_pieces(ops, o, H, G, D, V, bs, entries):
+    if o.get("values_from_keys") and D != V:
+        pytest.skip("no such layer")
+    prep_case(ops, o, H, G, D, V, bs, entries, 4)
+
+
+def test_prep_of_small_heads_in_whole_pieces(ops):
+    for o in (dict(), dict(qk_eps=1e-5, rot=16, rot_half=True, weights=True), dict(qk_eps=1e-5, rot=10)):
+        prep_case(ops, o, 9, 3, 24, 8, 16, [(5, 0), (1, 31)], 0)
+        prep_case(ops, o, 2, 1, 32, 128, 16, [(2, 14)], 8)
 
 
 # ---- attention -------------------------------------------------------------------------------------------------------------------------------
