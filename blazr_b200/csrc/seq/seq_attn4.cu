@@ -145,9 +145,9 @@ constexpr int HEADER = MAX_TILES + 8;       // floats of the work area in front 
 // the r-th of the step's row tiles: its entry, first token and number of tokens (0: there is none, or its positions have no pages)
 __device__ __forceinline__ int row_tile(const Attn4Args& a, const b200seq_step& st, int i, int& e, int& t0, int& p0) {
     int nq = 1;
-    if (st.T == st.B) {
-        if (i >= st.T) return 0;
-        e = t0 = i;
+    if (st.T == st.B) {                         // (one token each, or as many entries without tokens as others have more)
+        if (i >= st.T || i >= st.ent_start[st.B]) return 0;
+        e = st.tok_ent[i], t0 = i;
     } else if (!attn_find_tile(st, i, a.QT, e, t0, nq)) {
         return 0;
     }
@@ -624,11 +624,12 @@ __global__ void __launch_bounds__(ROWS * 32) attn4_gather_kernel(const __grid_co
 }
 
 // grid (T, H): the parts that the tensor-core kernel leaves of one (token, head), in order
-__global__ void attn4_merge_kernel(const __grid_constant__ Attn4Args a) {
+__global__ void attn4_merge_kernel(const __grid_constant__ Attn4Args a, const __grid_constant__ b200seq_step st) {
     chain_enter();
     const int t = blockIdx.x, h = blockIdx.y, n = a.parts, step = a.V + 4;
     const float* pp = a.part + ((int64_t)t * a.H + h) * n * step;
     float M = -INFINITY, L = 0.f;
+    if (t >= st.ent_start[st.B] || pp[1] < 0.f) return;      // nobody's row; a row whose positions have no pages
     for (int w = 0; w < n; ++w) M = fmaxf(M, pp[w * step]);
     for (int w = 0; w < n; ++w)
         if (pp[w * step + 1] != 0.f) L = fmaf(pp[w * step + 1], tcsplit::ex2(pp[w * step] - M), L);
@@ -710,8 +711,8 @@ template <int NK>
 cudaError_t launch_values(int nv, const Attn4Args& a, const b200seq_step& st, dim3 grid, const Plan& p, cudaStream_t cs) {
     return nv == 1 ? launch_form<NK, 1>(a, st, grid, p, cs) : (nv == 2 ? launch_form<NK, 2>(a, st, grid, p, cs) : launch_form<NK, 4>(a, st, grid, p, cs));
 }
-// Which kernel is the faster one, from the key tiles a CTA has at most.  us, fitted to 57 steps of 8 to 288 tokens, timed with each of the two (the choice is at most 12 % behind the faster one).  Here: a wave of
-// CTAs takes 4 (5 with heads above 64) and 1.5 (3.6) a key tile of 32 and warp; keys that are dealt out 10, and 1290 (675) key tiles a us.  On the tensor cores: 7.5 (9; f32
+// Which kernel is the faster one, from the key tiles a CTA has at most.  us, fitted to 57 steps of 8 to 288 tokens, timed with each of the two (the choice is at
+// most 12 % behind the faster one).  Here: a wave of CTAs takes 4 (5 with heads above 64) and 1.5 (3.6) a key tile of 32 and warp; keys that are dealt out 10, and 1290 (675) key tiles a us.  On the tensor cores: 7.5 (9; f32
 // 11) a CTA and 0.8 (0.75; f32 1.4) a key tile of 64, 4 more for keys in several parts.  Measured, us, here / there, 32 query heads of 8 key heads of 64 (of 128):
 //   1 x 64 tokens                6 /  8 ( 7 / 10)     16 x 9 behind 1500   43 / 28 (66 / 31)     32 x 2 behind 2000   34 / 64 (45 / 73)
 //   1 x 32 behind 4000          22 / 22 (34 / 25)      4 x 8 behind 8000   56 / 36 (83 / 39)      4 x 64 behind 300   27 / 13 (38 / 14)
@@ -737,11 +738,14 @@ extern "C" {
 
 size_t b200seq_attn_kv4_scratch_floats(const b200seq_step* st, const b200seq_attn_desc* d) {
     if (!st || !d || st->T < 1 || st->B < 1 || st->block_size < 1 || st->max_blocks < 1 || d->H < 1 || d->G < 1 || d->H % d->G || d->V < 1) return 0;
-    size_t need = plan_floats(plan(*st, *d), d->V);
+    const Plan p = plan(*st, *d);
+    size_t need = plan_floats(p, d->V);
     if (attn4_tc_takes(d->D, d->V)) {
-        const int parts = attn4_tc_plan(*st, d->H, d->G, d->D, d->V, most_keys(*st, *d, 0)).parts;
-        const size_t tc = parts > 1 ? (size_t)st->T * d->H * parts * (d->V + 4) : 0;
-        need = tc > need ? tc : need;
+        const Attn4TcPlan tp = attn4_tc_plan(*st, d->H, d->G, d->D, d->V, most_keys(*st, *d, 0));
+        if (tp.parts > 1 && tc_is_faster(*st, *d, p, tp, false)) {   // (chosen for f32 results: chosen for bf16 ones too)
+            const size_t tc = (size_t)st->T * d->H * tp.parts * (d->V + 4);
+            need = tc > need ? tc : need;
+        }
     }
     return need;
 }
@@ -750,7 +754,8 @@ int b200seq_attn_kv4(const float* proj, int64_t ld, const b200seq_step* st, cons
                      float* scratch, size_t scratch_floats, void* stream) {
     if (int rc = attn_desc_check(d, "attn_kv4")) return rc;
     if (!st || st->T < 0 || st->B < 0 || st->block_size < 1 || st->max_blocks < 0) return fail(B200SEQ_ERR_INVALID_ARG, "attn_kv4: bad step");
-    if (!proj || !kpool || !vpool || !out || (st->T > 0 && (!st->tok_pos || !st->ent_start || !st->block_table))) return fail(B200SEQ_ERR_INVALID_ARG, "attn_kv4: bad arguments");
+    if (!proj || !kpool || !vpool || !out || (st->T > 0 && (!st->tok_ent || !st->tok_pos || !st->ent_start || !st->block_table)))
+        return fail(B200SEQ_ERR_INVALID_ARG, "attn_kv4: bad arguments");
     if (out_dtype != B200SEQ_F32 && out_dtype != B200SEQ_BF16) return fail(B200SEQ_ERR_INVALID_ARG, "attn_kv4: results are f32 or bf16");
     if (d->pool > 0 || d->latent_v || d->krot || d->ctx_rows || d->kv_ld > 0 || (d->kd > 0 && d->kd < d->D))
         return fail(B200SEQ_ERR_UNSUPPORTED, "attn_kv4: a 4-bit cache holds plain keys and values (no pooled blocks, no latents)");
@@ -783,7 +788,7 @@ int b200seq_attn_kv4(const float* proj, int64_t ld, const b200seq_step* st, cons
         if (e != cudaSuccess) return cuda_status(e, "attn_kv4");
         count_launch();
         if (tp.parts > 1) {
-            launch_chained(attn4_merge_kernel, dim3(st->T, d->H), d->V <= 64 ? 64 : 128, 0, cs, a);
+            launch_chained(attn4_merge_kernel, dim3(st->T, d->H), d->V <= 64 ? 64 : 128, 0, cs, a, *st);
             SEQ_LAUNCH_CHECK("attn_kv4 merge");
         }
         return 0;

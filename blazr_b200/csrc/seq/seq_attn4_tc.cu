@@ -238,8 +238,10 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
         if (ord < longer) tile_no = (ord % (nc - 1)) * per + per - 1 - ord / (nc - 1);
         else tile_no = ((ord - longer) % nc) * per + rem - 1 - (ord - longer) / nc;
     }
-    if (st.B == 1) e = 0, t0 = tile_no * a.QT, nq = min(a.QT, st.T - t0);
-    else if (!attn_find_tile(st, tile_no, a.QT, e, t0, nq)) return;
+    if (st.B == 1) {
+        e = 0, t0 = tile_no * a.QT, nq = min(a.QT, min(st.T, st.ent_start[1]) - t0);
+        if (nq <= 0) return;
+    } else if (!attn_find_tile(st, tile_no, a.QT, e, t0, nq)) return;
     const int p0 = st.tok_pos[t0];
     const int g = unit / a.HB, hb = unit - g * a.HB, R = H / G;
     const int h0 = g * R + hb * a.Rb, nh = min(a.Rb, R - hb * a.Rb);
@@ -262,6 +264,8 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
     if (p0 < 0 || hi / bs >= st.max_blocks) {
         asm volatile("cp.async.wait_all;" ::: "memory");
         if (threadIdx.x == 0) atomicOr(a.err, 1);
+        if (a.parts > 1)                              // (a sum below zero: no parts of these rows)
+            for (int i = threadIdx.x; i < nq * nh; i += blockDim.x) a.part[(((int64_t)(t0 + i / nh) * H + h0 + i % nh) * a.parts + split) * (V + 4) + 1] = -1.f;
         return;
     }
     const KeySpan<KT> span(a, p0, hi);

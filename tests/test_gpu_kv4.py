@@ -372,3 +372,52 @@ def test_the_same_call_gives_the_same_bits(ops):
         for o in outs:
             ops.attn_kv4(q, st, d, kp, vp, o)
         assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2]) and (a is None or np.isfinite(a).all())
+
+
+# ---- steps that hold more than tokens ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("entries,D", [([(2, 50), (1, 30), (1, 9)], 64), ([(1, 5000)], 128), ([(1, 40)] * 6, 64), ([(70, 3000)], 64), ([(70, 3000)], 128), ([(100, 0), (37, 900)], 64),
+                                       ([(5, 700), (3, 0)], 128)])
+@pytest.mark.parametrize("odt", [torch.float32, torch.bfloat16])
+def test_entries_without_tokens_and_rows_behind_the_last(ops, entries, D, odt):
+    """entries without tokens among the others, and rows behind the last entry's, change nothing of the others' results; the latter are left as they were, and so are those of
+    positions without pages"""
+    rng = np.random.default_rng(len(entries) + D)
+    H, G = 8, 2
+    st, keep, slots, pages = step(ops, entries, 16, rng)
+    pools = [np.zeros((pages, G, ops.kv4_page_bytes(16, 1, D)), dtype=np.uint8) for _ in range(2)]
+    for pool, key in zip(pools, (True, False)):
+        for e in slots:
+            ref.put_rows(pool, 16, e, rng.standard_normal((len(e), G, D)).astype(np.float32), key)
+    kp, vp = (torch.from_numpy(p).to(DEV) for p in pools)
+    d = ops.attn_desc(H, G, D, D, 0.125, gated=False, kv_shared=True)
+    T, B = st.T, st.B
+    q = torch.from_numpy(rng.standard_normal((T + 5, d.width)).astype(np.float32)).to(DEV)
+
+    def run(tok_ent, tok_pos, ent_start, table, n, flags=0):
+        dev = [torch.tensor(x, dtype=torch.int32, device=DEV) for x in (tok_ent, tok_pos, ent_start)] + [torch.tensor(table, dtype=torch.int32, device=DEV)]
+        s = ops.StepDesc(dev[0].data_ptr(), dev[1].data_ptr(), dev[2].data_ptr(), dev[0].data_ptr(), dev[1].data_ptr(), dev[3].data_ptr(), n, len(ent_start) - 1, len(table[0]), 16)
+        out = torch.full((T + 5, H * D), 3.0, device=DEV, dtype=odt)
+        ops.attn_kv4(q, s, d, kp, vp, out)
+        assert ops.error_flags() == flags
+        return out
+
+    ent, pos, start, table = (keep[k].cpu().tolist() for k in ("tok_ent", "tok_pos", "ent_start", "block_table"))
+    plain = run(ent, pos, start, table, T)
+    assert bool((plain[T:] == 3).all()) and not bool((plain[:T] == 3).all(1).any())
+    same = lambda out: (out[:T].float() - plain[:T].float()).abs().max().item() <= (4e-6 if odt == torch.float32 else 2.0 ** -7) * plain[:T].float().abs().max().item()
+    # entries without tokens: behind the first one, and at the end as many as make it as many entries as tokens (two where that is many)
+    extra = max(T - B - 1, 0) if T <= 8 else 2
+    at = [0] + [i + 2 for i in range(B - 1)]
+    start2, table2 = [0, start[1]] + start[1:] + [T] * extra, [table[0], table[0]] + table[1:] + [table[0]] * extra
+    out = run([at[e] for e in ent], pos, start2, table2, T)
+    assert same(out) and bool((out[T:] == 3).all())
+    # rows behind the last entry's
+    out = run(ent + [0] * 5, pos + [0] * 5, start, table, T + 5)
+    assert same(out) and bool((out[T:] == 3).all())
+    if T <= 8:                                                 # (as many entries as rows)
+        out = run(ent + [0] * 5, pos + [0] * 5, start + [T] * (T + 5 - B), table + [table[0]] * (T + 5 - B), T + 5)
+        assert same(out) and bool((out[T:] == 3).all())
+    # no page for the last positions of the longest
+    w = len(table[0]) - 1
+    out = run(ent, pos, start, [r[:w] for r in table], T, flags=1)
+    assert bool((out[:T][torch.tensor([p >= 16 * w for p in pos], device=DEV)] == 3).all()) and bool((out[T:] == 3).all())
