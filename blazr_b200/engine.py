@@ -113,10 +113,13 @@ class Engine:
     def fork(self, rid: str, new_rid: str, params: Optional[SamplingParams] = None) -> Optional[Request]:
         """a second request that continues from where the live request `rid` is.  Of a request of the engine's own scheduler a Request (with the prompt and the
         output so far, and params or the same ones) that runs from the next step on; of an externally scheduled one None"""
+        rid, new_rid = str(rid), str(new_rid)
         if new_rid in self.requests or new_rid in self.cache.live:
             raise ValueError(f"request id {new_rid} is in use")
         if rid not in self.cache.live:
             raise ValueError(f"request {rid} holds nothing in the cache")
+        if self.cache.slots.free_slots <= self._promised():
+            raise CacheFull(f"no state slot for request {new_rid}: {self.cache.slots.free_slots} free, {self._promised()} kept for samples of running prompts")
         r = self.requests.get(rid)
         if r is not None:
             self._check(replace(params or r.params, n=1))
@@ -128,6 +131,10 @@ class Engine:
         self.running.append(q)
         return q
 
+    def _promised(self) -> int:
+        """slots that running requests take when their prompt is through, for its other samples"""
+        return sum(r.params.n - 1 for r in self.running if r.params.n > 1 and not r.output and not r.siblings)
+
     def _fork_cache(self, rid: str, new_rid: str) -> None:
         src, new = self.cache.live[rid], self.cache.fork(rid, new_rid)
         if hasattr(self.model, "copy_slots"):
@@ -135,6 +142,7 @@ class Engine:
 
     def truncate(self, rid: str, n_tokens: int) -> None:
         """takes back the tokens of an externally scheduled request from position n_tokens on (rejected drafts); models whose layers carry state cannot"""
+        rid = str(rid)
         if rid in self.requests:
             raise ValueError(f"request {rid} belongs to the scheduler")
         if rid not in self.cache.live:
@@ -206,8 +214,7 @@ class Engine:
         plan: List[Tuple[Request, List[int], List[int]]] = []
         budget = self.max_step_tokens
         free_pages = self.cache.pages.free_blocks
-        # slots that running requests take when their prompt is through, for its other samples
-        free_slots = self.cache.slots.free_slots - sum(r.params.n - 1 for r in self.running if r.params.n > 1 and not r.output and not r.siblings)
+        free_slots = self.cache.slots.free_slots - self._promised()
         for r in self.running:
             if r.fed < len(r.prompt):
                 continue

@@ -256,6 +256,19 @@ def test_a_prompt_is_sampled_several_times(monkeypatch):
         eng.add_request("x", [1], SamplingParams(n=0))
 
 
+def test_a_fork_leaves_the_slots_of_samples_to_come(monkeypatch):
+    fake_rules(monkeypatch)
+    eng = Engine(PagedModel(), max_tokens=400, max_seqs=3, block_size=16, prefill_chunk=2)
+    eng.add_request("a", [3, 1, 4, 1, 5], SamplingParams(max_new_tokens=4, n=3))
+    eng.step()
+    with pytest.raises(CacheFull):
+        eng.fork("a", "b")
+    r = eng.requests["a"]
+    while eng.has_work():
+        eng.step()
+    assert [q.output for q in [r] + r.siblings] == [alone([3, 1, 4, 1, 5], 4)] * 3
+
+
 def test_rules_of_a_batch(monkeypatch):
     seen = []
     fake_rules(monkeypatch, seen)

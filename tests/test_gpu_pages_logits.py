@@ -206,3 +206,14 @@ def test_empty_histories(ops):
     a = make(np.random.default_rng(6), 3, 100, 0, 0, False)
     assert a["hist"].size == 0
     same(run(ops, a), rules64(a))
+
+
+@pytest.mark.parametrize("V", [100, 128256])
+def test_temperatures_whose_reciprocal_is_no_number(ops, V):
+    a = make(np.random.default_rng(7), 64, V, 20, 0, False)
+    a["logits"][:, ::2] = 0
+    a["hist_prompt"][:] = np.diff(a["hist_start"])            # (repetitions leave zeros zero)
+    a["rules"][::2, 3] = 2.0 ** -140
+    want = rules64(a).astype(np.float32)                       # (infinities: beyond f32)
+    got = run(ops, a).cpu().numpy()
+    assert np.array_equal(np.isinf(want), np.isinf(got)) and np.array_equal(got[::2, ::2], np.zeros_like(got[::2, ::2])) and np.array_equal(np.sign(want), np.sign(got))
