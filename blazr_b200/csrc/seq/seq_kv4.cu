@@ -9,11 +9,11 @@ struct Kv4Rows {
     const void *k, *v;
     int64_t ldk, ldv;
     uint8_t *kpool, *vpool;
-    int G, D, Gv, V, bf16, vec;
+    int G, D, Gv, V, vec;
 };
 
 // position of a token in its sequence's pages; -1 (and the error flag) outside the block table
-__device__ __forceinline__ int64_t kv4_page(const b200seq_step& st, int t, int& o, int* err) {
+__device__ __forceinline__ int kv4_page(const b200seq_step& st, int t, int& o, int* err) {
     const int pos = st.tok_pos[t], b = pos / st.block_size;
     o = pos - b * st.block_size;
     if (pos < 0 || b >= st.max_blocks) {
@@ -41,29 +41,24 @@ __device__ __forceinline__ void kv4_put(uint8_t* pool, const Kv4Row& at, bool ke
     if ((hl & 3) == 0) *reinterpret_cast<uint32_t*>(pool + at.params + hl) = param;
 }
 
-// A block has a token; LPR lanes (4 for every group of the wider of key and value heads) have a row of it at a time.  Bounded by instructions: 340 a row with
-// four values to a lane and a warp to a row (4094 tokens, 16 rows of 128 bf16: 34 us).
-template <int LPR>
+// A block has a token; LPR lanes (4 for every group of the wider of key and value heads) have a row of it at a time.  WHOLE: keys and values of as many groups,
+// rows of whole 16-byte pieces, of bf16 values or not.  Bounded by instructions: about 300 a pair of rows (4094 tokens of 16 rows of 128 bf16 values, stored and loaded: 22.4 us, 26.0 with the rows asked for behind their page).
+template <int LPR, bool WHOLE, bool BF16>
 __global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4Rows a, const b200seq_step st, int* err) {
     chain_enter();
     const int hl = threadIdx.x & (LPR - 1), heads = a.G + a.Gv, t = blockIdx.x;
-    int o;
-    const int64_t page = kv4_page(st, t, o, err);
-    if (page < 0) return;
-    bool odd = false;
-    for (int u0 = (threadIdx.x & ~31) / LPR; u0 < heads; u0 += blockDim.x / LPR) {
-        const int u = u0 + (threadIdx.x & 31) / LPR;
-        const bool in = u < heads, key = u < a.G;
-        const int g = key ? u : u - a.G, D = key ? a.D : a.V, NG = kv4_groups(D), n = in ? min(max(D - 8 * hl, 0), 8) : 0;
-        const int64_t src = (int64_t)t * (key ? a.ldk : a.ldv) + g * D + 8 * hl;
+    float x[8];
+    auto fetch = [&](int u) {
+        const bool key = u < a.G;
+        const int g = key ? u : u - a.G, D = key ? a.D : a.V, n = u < heads ? min(max(D - 8 * hl, 0), 8) : 0;
+        const int64_t src = (int64_t)t * (key ? a.ldk : a.ldv) + (g * D + 8 * hl);
         const void* p = key ? a.k : a.v;
-        float x[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] = 0.f;
-        if (a.bf16) {
+        if (BF16) {
             const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p) + src;
-            if (a.vec && n == 8) {
-                const uint4 w = *reinterpret_cast<const uint4*>(q);
+            if (WHOLE) {
+                const uint4 w = n ? *reinterpret_cast<const uint4*>(q) : make_uint4(0, 0, 0, 0);
                 const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) x[2 * j] = __uint_as_float(ws[j] << 16), x[2 * j + 1] = __uint_as_float(ws[j] & 0xFFFF0000u);
@@ -74,54 +69,85 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const Kv4Rows a, const b
             }
         } else {
             const float* q = reinterpret_cast<const float*>(p) + src;
-            if (a.vec && n == 8) {
-                const float4 v = ld4(q), w = ld4(q + 4);
-                x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w, x[4] = w.x, x[5] = w.y, x[6] = w.z, x[7] = w.w;
+            if (WHOLE) {
+                if (n) {
+                    const float4 v = ld4(q), w = ld4(q + 4);
+                    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w, x[4] = w.x, x[5] = w.y, x[6] = w.z, x[7] = w.w;
+                }
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (j < n) x[j] = q[j];
             }
         }
+    };
+    fetch((int)threadIdx.x / LPR);                 // (on its way while the page is looked up)
+    int o;
+    const int page = kv4_page(st, t, o, err);
+    if (page < 0) return;
+    bool odd = false;
+    for (int u0 = (threadIdx.x & ~31) / LPR; u0 < heads; u0 += blockDim.x / LPR) {
+        const int u = u0 + (threadIdx.x & 31) / LPR;
+        const bool in = u < heads, key = u < a.G;
+        const int g = key ? u : u - a.G, D = key ? a.D : a.V, NG = WHOLE ? LPR / 4 : kv4_groups(D), n = in ? min(max(D - 8 * hl, 0), 8) : 0;
         uint32_t param;
         const uint32_t w = kv4_quantise(x, n, param, odd);
         kv4_put(key ? a.kpool : a.vpool, kv4_row(page, o, st.block_size, in ? g : 0, key ? a.G : a.Gv, NG), key, hl, NG, w, param, in);
+        if (u0 + (int)blockDim.x / LPR < heads) fetch(u + (int)blockDim.x / LPR);
     }
     if (odd) atomicOr(err, KV4_ERR_RANGE);
 }
+template <bool WHOLE, bool BF16>
+auto store_kernel(int lpr) {
+    return lpr == 4 ? kv4_store_kernel<4, WHOLE, BF16> : (lpr == 8 ? kv4_store_kernel<8, WHOLE, BF16> : kv4_store_kernel<16, WHOLE, BF16>);
+}
 
-// the same rows back, as the values they stand for
-template <int LPR>
+// The same rows back, as the values they stand for.  A block has TOK tokens: two where half the GPU's threads have work (4094 tokens of 16 rows of 128: 22.4
+// us for storing and loading with two, 23.9 with one; 300 tokens 4.9 and 4.6).
+template <int LPR, bool WHOLE, int TOK>
 __global__ void __launch_bounds__(256) kv4_load_kernel(const Kv4Rows a, float* __restrict__ ko, float* __restrict__ vo, const b200seq_step st, int* err) {
     chain_enter();
-    const int hl = threadIdx.x & (LPR - 1), heads = a.G + a.Gv, t = blockIdx.x;
-    int o;
-    const int64_t page = kv4_page(st, t, o, err);
-    if (page < 0) return;
+    const int hl = threadIdx.x & (LPR - 1), heads = a.G + a.Gv, t0 = blockIdx.x * TOK;
+    int o[TOK], page[TOK];
+#pragma unroll
+    for (int k = 0; k < TOK; ++k) page[k] = t0 + k < st.T ? kv4_page(st, t0 + k, o[k], err) : -1;
     for (int u = threadIdx.x / LPR; u < heads; u += blockDim.x / LPR) {
         const bool key = u < a.G;
-        const int g = key ? u : u - a.G, D = key ? a.D : a.V, NG = kv4_groups(D), n = min(max(D - 8 * hl, 0), 8);
+        const int g = key ? u : u - a.G, D = key ? a.D : a.V, NG = WHOLE ? LPR / 4 : kv4_groups(D), n = min(max(D - 8 * hl, 0), 8);
         if (n == 0) continue;
         const uint8_t* pool = key ? a.kpool : a.vpool;
-        const Kv4Row at = kv4_row(page, o, st.block_size, g, key ? a.G : a.Gv, NG);
-        uint32_t w;
-        if (key) w = *reinterpret_cast<const uint32_t*>(pool + at.codes + kv4_key_place(hl, NG));
-        else w = *reinterpret_cast<const uint16_t*>(pool + at.codes + kv4_value_place(hl, NG)) | ((uint32_t)*reinterpret_cast<const uint16_t*>(pool + at.codes + kv4_value_place(hl, NG) + 2 * NG) << 16);
-        const uint32_t pr = *reinterpret_cast<const uint32_t*>(pool + at.params + (hl & ~3));
-        const float s = __half2float(__ushort_as_half((uint16_t)pr)), m = __half2float(__ushort_as_half((uint16_t)(pr >> 16)));
-        float* dst = (key ? ko + (int64_t)t * a.ldk : vo + (int64_t)t * a.ldv) + g * D + 8 * hl;
-        float x[8];
+        uint32_t w[TOK], pr[TOK];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = fmaf(s, __uint_as_float(((w >> (4 * j)) & 15u) | 0x4B000000u) - 8388608.f, m);   // (2^23 + code)
-        if (a.vec && n == 8) {
-            *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<float4*>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
-        } else {
+        for (int k = 0; k < TOK; ++k) {
+            w[k] = pr[k] = 0;
+            if (page[k] < 0) continue;
+            const Kv4Row at = kv4_row(page[k], o[k], st.block_size, g, key ? a.G : a.Gv, NG);
+            if (key) w[k] = *reinterpret_cast<const uint32_t*>(pool + at.codes + kv4_key_place(hl, NG));
+            else w[k] = *reinterpret_cast<const uint16_t*>(pool + at.codes + kv4_value_place(hl, NG)) | ((uint32_t)*reinterpret_cast<const uint16_t*>(pool + at.codes + kv4_value_place(hl, NG) + 2 * NG) << 16);
+            pr[k] = *reinterpret_cast<const uint32_t*>(pool + at.params + (hl & ~3));
+        }
+        float* dst = (key ? ko + (int64_t)t0 * a.ldk : vo + (int64_t)t0 * a.ldv) + g * D + 8 * hl;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (j < n) dst[j] = x[j];
+        for (int k = 0; k < TOK; ++k, dst += key ? a.ldk : a.ldv) {
+            if (page[k] < 0) continue;
+            const float s = __half2float(__ushort_as_half((uint16_t)pr[k])), m = __half2float(__ushort_as_half((uint16_t)(pr[k] >> 16)));
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = fmaf(s, __uint_as_float(((w[k] >> (4 * j)) & 15u) | 0x4B000000u) - 8388608.f, m);   // (2^23 + code)
+            if (WHOLE) {
+                *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<float4*>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < n) dst[j] = x[j];
+            }
         }
     }
+}
+template <bool WHOLE, int TOK>
+auto load_kernel(int lpr) {
+    return lpr == 4 ? kv4_load_kernel<4, WHOLE, TOK> : (lpr == 8 ? kv4_load_kernel<8, WHOLE, TOK> : kv4_load_kernel<16, WHOLE, TOK>);
 }
 
 // b200seq_attn_prep_ex over 4-bit pages, for rows of whole 16-byte pieces (every head size, rotation and column that is a multiple of 8; norms over single heads).
@@ -139,7 +165,7 @@ __global__ void __launch_bounds__(128) kv4_prep_rows_kernel(float* proj, int64_t
     const int pos = st.tok_pos[t];
     const int H = a.H, G = a.G, Gv = a.vg > 0 ? a.vg : G, np = a.rot_dims >> 1, nu = a.kv_shared ? H : H + G + Gv;
     int o = 0;
-    const int64_t page = a.kv_shared ? -1 : kv4_page(st, t, o, err);
+    const int page = a.kv_shared ? -1 : kv4_page(st, t, o, err);
     float* base = proj + (int64_t)t * ld;
     bool odd = false, first = true;
     for (int u0 = part * ROWS; u0 < nu; u0 += split * ROWS) {
@@ -232,7 +258,7 @@ __global__ void kv4_prep_kernel(float* __restrict__ proj, int64_t ld, const b200
     const int pos = st.tok_pos[t];
     const int H = a.H, G = a.G, D = a.D, V = a.V, Gv = a.vg > 0 ? a.vg : G, np = a.rot_dims >> 1;
     int o = 0;
-    const int64_t page = a.kv_shared ? -1 : kv4_page(st, t, o, err);
+    const int page = a.kv_shared ? -1 : kv4_page(st, t, o, err);
     float* base = proj + (int64_t)t * ld;
     for (int i = threadIdx.x; i < np; i += blockDim.x) {
         float sn, cs;
@@ -307,6 +333,7 @@ int rows_check(const b200seq_step* st, const void* k, const void* v, int64_t ldk
     if (D > KV4_MAX_DIM || V > KV4_MAX_DIM) return fail(B200SEQ_ERR_UNSUPPORTED, "%s: heads of up to %d values", what, KV4_MAX_DIM);
     if (st->T > 1 && (ldk < (int64_t)G * D || ldv < (int64_t)Gv * V)) return fail(B200SEQ_ERR_INVALID_ARG, "%s: row strides below a row's length", what);
     if ((reinterpret_cast<uintptr_t>(kpool) | reinterpret_cast<uintptr_t>(vpool)) & 15) return fail(B200SEQ_ERR_INVALID_ARG, "%s: pools start on a 16-byte boundary", what);
+    if (!kv4_pages_fit(st->block_size, G, D) || !kv4_pages_fit(st->block_size, Gv, V)) return fail(B200SEQ_ERR_UNSUPPORTED, "%s: pages of up to 2 GiB", what);
     if (((int64_t)G + Gv) * KV4_MAX_DIM > 0x7fffffff) return fail(B200SEQ_ERR_UNSUPPORTED, "%s: too many heads", what);
     return 0;
 }
@@ -340,9 +367,10 @@ int b200seq_kv4_store(const void* k, int64_t ldk, const void* v, int64_t ldv, in
     if (int rc = rows_check(st, k, v, ldk, ldv, G, D, Gv, V, kpool, vpool, "kv4_store")) return rc;
     if (st->T == 0) return 0;
     const bool bf16 = in_dtype == B200SEQ_BF16;
-    const Kv4Rows a{k, v, ldk, ldv, (uint8_t*)kpool, (uint8_t*)vpool, G, D, Gv, V, bf16, row_pieces(k, v, ldk, ldv, D, V, bf16 ? 8 : 4)};
+    const Kv4Rows a{k, v, ldk, ldv, (uint8_t*)kpool, (uint8_t*)vpool, G, D, Gv, V, row_pieces(k, v, ldk, ldv, D, V, bf16 ? 8 : 4)};
     const int lpr = 4 * kv4_groups(D > V ? D : V);
-    launch_chained(lpr == 4 ? kv4_store_kernel<4> : (lpr == 8 ? kv4_store_kernel<8> : kv4_store_kernel<16>), st->T, row_threads(G + Gv, lpr), 0, (cudaStream_t)stream, a, *st, error_flag_dev());
+    const bool whole = a.vec && kv4_groups(D) == kv4_groups(V);
+    launch_chained(whole ? (bf16 ? store_kernel<true, true>(lpr) : store_kernel<true, false>(lpr)) : (bf16 ? store_kernel<false, true>(lpr) : store_kernel<false, false>(lpr)), st->T, row_threads(G + Gv, lpr), 0, (cudaStream_t)stream, a, *st, error_flag_dev());
     SEQ_LAUNCH_CHECK("kv4_store");
     return 0;
 }
@@ -350,10 +378,11 @@ int b200seq_kv4_store(const void* k, int64_t ldk, const void* v, int64_t ldv, in
 int b200seq_kv4_load(const void* kpool, const void* vpool, const b200seq_step* st, int G, int D, int Gv, int V, float* k, int64_t ldk, float* v, int64_t ldv, void* stream) {
     if (int rc = rows_check(st, k, v, ldk, ldv, G, D, Gv, V, kpool, vpool, "kv4_load")) return rc;
     if (st->T == 0) return 0;
-    const Kv4Rows a{nullptr, nullptr, ldk, ldv, (uint8_t*)kpool, (uint8_t*)vpool, G, D, Gv, V, 0, row_pieces(k, v, ldk, ldv, D, V, 4)};
+    const Kv4Rows a{nullptr, nullptr, ldk, ldv, (uint8_t*)kpool, (uint8_t*)vpool, G, D, Gv, V, row_pieces(k, v, ldk, ldv, D, V, 4)};
     const int lpr = 4 * kv4_groups(D > V ? D : V);
-    launch_chained(lpr == 4 ? kv4_load_kernel<4> : (lpr == 8 ? kv4_load_kernel<8> : kv4_load_kernel<16>), st->T, row_threads(G + Gv, lpr), 0, (cudaStream_t)stream, a, k, v, *st,
-                   error_flag_dev());
+    const bool whole = a.vec && kv4_groups(D) == kv4_groups(V);
+    const int tok = whole && (int64_t)st->T * (G + Gv) * lpr >= 148 * 1024 ? 2 : 1;
+    launch_chained(whole ? (tok == 2 ? load_kernel<true, 2>(lpr) : load_kernel<true, 1>(lpr)) : load_kernel<false, 1>(lpr), (st->T + tok - 1) / tok, row_threads(G + Gv, lpr), 0, (cudaStream_t)stream, a, k, v, *st, error_flag_dev());
     SEQ_LAUNCH_CHECK("kv4_load");
     return 0;
 }
@@ -365,6 +394,7 @@ int b200seq_attn_prep_kv4(float* proj, int64_t ld, const b200seq_step* st, const
     if (d->pool > 0 || d->latent_v || d->krot || d->ctx_rows) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_prep_kv4: a 4-bit cache holds plain keys and values (no pooled blocks, no latents)");
     if (d->D > KV4_MAX_DIM || d->V > KV4_MAX_DIM) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_prep_kv4: heads of up to %d values", KV4_MAX_DIM);
     if ((reinterpret_cast<uintptr_t>(kpool) | reinterpret_cast<uintptr_t>(vpool)) & 15) return fail(B200SEQ_ERR_INVALID_ARG, "attn_prep_kv4: pools start on a 16-byte boundary");
+    if (!kv4_pages_fit(st->block_size, d->G, d->D) || !kv4_pages_fit(st->block_size, d->vg > 0 ? d->vg : d->G, d->V)) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_prep_kv4: pages of up to 2 GiB");
     if (st->T == 0) return 0;
     const int Dmax = d->D > d->V ? d->D : d->V;
     const size_t smem = (size_t)(d->rot_dims + 8 * Dmax + 40) * sizeof(float);

@@ -27,15 +27,16 @@ constexpr float KV4_FIFTEENTH = 0x1.11111p-4f;
 __host__ __device__ __forceinline__ int kv4_groups(int D) { return D <= 32 ? 1 : (D <= 64 ? 2 : 4); }
 __host__ __device__ __forceinline__ int kv4_unit(int bs) { return bs % 16 == 0 ? 16 : bs; }
 
-// row `o` of a page of `bs` rows, head g of G: offset of its codes and of its parameters in the pool
+// row `o` of a page of `bs` rows, head g of G: offset of its codes and of its parameters in the pool (pages of less than 2 GiB: checked by the callers)
 struct Kv4Row {
     int64_t codes, params;
 };
-__device__ __forceinline__ Kv4Row kv4_row(int64_t page, int o, int bs, int g, int G, int NG) {
-    const int unit = kv4_unit(bs), u = unit == 16 ? o >> 4 : 0, ru = unit == 16 ? o & 15 : o;   // (o < bs)
-    const int64_t base = (page * G + g) * (int64_t)(bs * NG * 20) + (int64_t)u * (unit * NG * 20);
-    return Kv4Row{base + ru * NG * 16, base + unit * NG * 16 + ru * NG * 4};
+__device__ __forceinline__ Kv4Row kv4_row(int page, int o, int bs, int g, int G, int NG) {
+    const int unit = kv4_unit(bs), u = unit == 16 ? o >> 4 : 0, ru = unit == 16 ? o & 15 : o, head = bs * NG * 20;   // (o < bs)
+    const int64_t base = (int64_t)page * (G * head) + (g * head + u * (unit * NG * 20));
+    return Kv4Row{base + ru * NG * 16, base + (unit * NG * 16 + ru * NG * 4)};
 }
+inline bool kv4_pages_fit(int bs, int heads, int D) { return (int64_t)bs * heads * kv4_groups(D) * 20 <= 0x7fffffff; }
 
 // A group of 32 values, eight in each of four neighbouring lanes (`n` of the lane's eight are values of the row, the rest do not exist).  Returns the lane's eight
 // codes, the first in the lowest bits, and, the same in all four lanes, the (s, m) pair.  Every lane of the warp takes part.
