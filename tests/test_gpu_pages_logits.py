@@ -185,6 +185,7 @@ def test_temperature_zero_and_no_rules(ops):
     """rules of (1, 0, 0, 0) leave the logits, bit by bit, whatever the history"""
     a = make(np.random.default_rng(4), 2, 700, 90, 0, False)
     a["rules"][:] = [1, 0, 0, 0]
+    a["logits"][0, :3] = 3e38, -3e38, 1e-44
     assert np.array_equal(run(ops, a).cpu().numpy(), a["logits"])
     for k in ("hist", "hist_start", "hist_prompt"):
         a.pop(k)
