@@ -665,9 +665,10 @@ cudaError_t launch(const Attn4Args& a, const b200seq_step& st, dim3 grid, cudaSt
     e = cudaLaunchKernelEx(&cfg, kernel, a, st);
     return e != cudaSuccess ? e : cudaGetLastError();
 }
-// the most keys a token can see
-int64_t most_keys(const b200seq_step& st, const b200seq_attn_desc& d, int tokens) {
+// the most keys a token can see: what the block tables hold, or the fewer that the caller names (a bound to plan by; nothing goes wrong with more of them)
+int64_t most_keys(const b200seq_step& st, const b200seq_attn_desc& d, int max_keys, int tokens) {
     int64_t keys = (int64_t)st.max_blocks * st.block_size;
+    if (max_keys > 0 && max_keys < keys) keys = max_keys;
     if (d.chunk > 0 && d.chunk < keys) keys = d.chunk;
     if (d.window > 0 && (int64_t)d.window + d.keep_first + tokens < keys) keys = (int64_t)d.window + d.keep_first + tokens;
     return keys;
@@ -681,14 +682,14 @@ struct Plan {
     int heads, cluster, warps, ctas;
     bool dealt;
 };
-Plan plan(const b200seq_step& st, const b200seq_attn_desc& d) {
+Plan plan(const b200seq_step& st, const b200seq_attn_desc& d, int max_keys) {
     Plan p;
     const int R = d.H / d.G, Rb = R < ROWS ? R : ROWS, QT = ROWS / Rb;
     p.heads = d.G * ((R + Rb - 1) / Rb);
     p.tiles = st.T == st.B ? st.T : ((int64_t)st.T + QT - 1) / QT + st.B;
     const int64_t each = ((int64_t)st.T + st.B - 1) / st.B;
     p.real = st.B * ((each + QT - 1) / QT);
-    const int64_t units = p.real * p.heads, key_tiles = (most_keys(st, d, QT) + KT - 1) / KT;
+    const int64_t units = p.real * p.heads, key_tiles = (most_keys(st, d, max_keys, QT) + KT - 1) / KT;
     const bool small = d.D <= 64 && d.V <= 64;
     double best = -1.0;
     for (int warps : {small ? 4 : 8, small ? 8 : 4}) {
@@ -719,9 +720,9 @@ cudaError_t launch_values(int nv, const Attn4Args& a, const b200seq_step& st, di
 // 11) a CTA and 0.8 (0.75; f32 1.4) a key tile of 64, 4 more for keys in several parts.  Measured, us, here / there, 32 query heads of 8 key heads of 64 (of 128):
 //   1 x 64 tokens                6 /  8 ( 7 / 10)     16 x 9 behind 1500   43 / 28 (66 / 31)     32 x 2 behind 2000   34 / 64 (45 / 73)
 //   1 x 32 behind 4000          22 / 22 (34 / 25)      4 x 8 behind 8000   56 / 36 (83 / 39)      4 x 64 behind 300   27 / 13 (38 / 14)
-bool tc_is_faster(const b200seq_step& st, const b200seq_attn_desc& d, const Plan& p, const Attn4TcPlan& tp, bool f32) {
+bool tc_is_faster(const b200seq_step& st, const b200seq_attn_desc& d, int max_keys, const Plan& p, const Attn4TcPlan& tp, bool f32) {
     const bool small = d.D <= 64 && d.V <= 64;
-    const double keys = (double)most_keys(st, d, 0), kt = (keys + KT - 1) / KT, units = (double)p.real * p.heads;
+    const double keys = (double)most_keys(st, d, max_keys, 0), kt = (keys + KT - 1) / KT, units = (double)p.real * p.heads;
     const double waves = units * p.cluster / p.ctas, share = kt / (p.warps * p.cluster);
     const double here = p.dealt ? 10.0 + units * kt / (small ? 1290.0 : 675.0) : (waves < 1.0 ? 1.0 : waves) * ((small ? 4.0 : 5.0) + (small ? 1.5 : 3.6) * (share < 1.0 ? 1.0 : share)) + 2.0;
     const double set_up = small ? 7.5 : (f32 ? 11.0 : 9.0), each = small ? 0.8 : (f32 ? 1.4 : 0.75);
@@ -739,13 +740,13 @@ using namespace b200seq;
 
 extern "C" {
 
-size_t b200seq_attn_kv4_scratch_floats(const b200seq_step* st, const b200seq_attn_desc* d) {
+size_t b200seq_attn_kv4_scratch_floats(const b200seq_step* st, const b200seq_attn_desc* d, int max_keys) {
     if (!st || !d || st->T < 1 || st->B < 1 || st->block_size < 1 || st->max_blocks < 1 || d->H < 1 || d->G < 1 || d->H % d->G || d->V < 1) return 0;
-    const Plan p = plan(*st, *d);
+    const Plan p = plan(*st, *d, max_keys);
     size_t need = plan_floats(p, d->V);
     if (attn4_tc_takes(d->D, d->V)) {
-        const Attn4TcPlan tp = attn4_tc_plan(*st, d->H, d->G, d->D, d->V, most_keys(*st, *d, 0));
-        if (tp.parts > 1 && tc_is_faster(*st, *d, p, tp, false)) {   // (chosen for f32 results: chosen for bf16 ones too)
+        const Attn4TcPlan tp = attn4_tc_plan(*st, d->H, d->G, d->D, d->V, most_keys(*st, *d, max_keys, 0));
+        if (tp.parts > 1 && tc_is_faster(*st, *d, max_keys, p, tp, false)) {   // (chosen for f32 results: chosen for bf16 ones too)
             const size_t tc = (size_t)st->T * d->H * tp.parts * (d->V + 4);
             need = tc > need ? tc : need;
         }
@@ -754,7 +755,7 @@ size_t b200seq_attn_kv4_scratch_floats(const b200seq_step* st, const b200seq_att
 }
 
 int b200seq_attn_kv4(const float* proj, int64_t ld, const b200seq_step* st, const b200seq_attn_desc* d, const void* kpool, const void* vpool, void* out, int out_dtype,
-                     float* scratch, size_t scratch_floats, void* stream) {
+                     float* scratch, size_t scratch_floats, int max_keys, void* stream) {
     if (int rc = attn_desc_check(d, "attn_kv4")) return rc;
     if (!st || st->T < 0 || st->B < 0 || st->block_size < 1 || st->max_blocks < 0) return fail(B200SEQ_ERR_INVALID_ARG, "attn_kv4: bad step");
     if (!proj || !kpool || !vpool || !out || (st->T > 0 && (!st->tok_ent || !st->tok_pos || !st->ent_start || !st->block_table)))
@@ -781,9 +782,9 @@ int b200seq_attn_kv4(const float* proj, int64_t ld, const b200seq_step* st, cons
     a.softcap = d->softcap, a.out = out, a.out_dtype = out_dtype, a.err = error_flag_dev();
     cudaStream_t cs = (cudaStream_t)stream;
     if (d->H > 65535) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_kv4: too many heads");
-    Plan p = plan(*st, *d);
-    Attn4TcPlan tp = attn4_tc_plan(*st, d->H, d->G, d->D, d->V, most_keys(*st, *d, 0));
-    if (a.vec && attn4_tc_takes(d->D, d->V) && tc_is_faster(*st, *d, p, tp, out_dtype == B200SEQ_F32)) {
+    Plan p = plan(*st, *d, max_keys);
+    Attn4TcPlan tp = attn4_tc_plan(*st, d->H, d->G, d->D, d->V, most_keys(*st, *d, max_keys, 0));
+    if (a.vec && attn4_tc_takes(d->D, d->V) && tc_is_faster(*st, *d, max_keys, p, tp, out_dtype == B200SEQ_F32)) {
         if (tp.parts > 1 && (!scratch || scratch_floats < (size_t)st->T * d->H * tp.parts * (d->V + 4))) tp.parts = 1;
         if ((int64_t)d->G * tp.HB * tp.tiles > 0x7fffffff) return fail(B200SEQ_ERR_UNSUPPORTED, "attn_kv4: too many heads or tokens");
         a.part = scratch, a.parts = tp.parts;

@@ -609,7 +609,7 @@ class LayeredModel:
                 self.weight_bytes += (L["w_gu"].numel() + L["w_down"].numel()) * 2
             self.layers.append(L)
         self.max_seqs = self.max_blocks = self.block_size = 0
-        self.kv_bits = 32
+        self.kv_bits, self._keys = 32, 0
         self._ws: Dict[int, _Workspace] = {}
         self._graphs: Dict[int, object] = {}
         self.use_graphs = True
@@ -1319,12 +1319,15 @@ class LayeredModel:
             raise RuntimeError("allocate() the cache first")
         T, B, R = sa.T, sa.B, int(sa.want_rows.shape[0])
         self._ctx_rows = int(sa.ent_pos0.sum()) + T if (T > B and self.max_ctx_r) else 0
+        self._keys = int((sa.ent_pos0 + np.diff(sa.ent_start)).max()) if B else 0
         ws = self._workspace(T)
         self._upload(ws, sa)
         graphable = self.use_graphs and debug_layers is None and sa.decode_only and R == T and self.dev.type == "cuda" \
             and bool((sa.want_rows == np.arange(T)).all())
         if graphable:
-            key = (T, bool(sample))
+            if self.kv_bits == 4:       # a captured step shares its work out by the keys of its longest sequence: one for every power of two of them
+                self._keys = max(256, 1 << (self._keys - 1).bit_length())
+            key = (T, bool(sample), self._keys if self.kv_bits == 4 else 0)
             g = self._graphs.get(key)
             if g is None:
                 self._run(ws, T, B, R, sample, None)        # warm-up outside capture (module loading, attribute calls)
@@ -1792,7 +1795,7 @@ class LayeredModel:
     def _attend(self, L, src, ws: _Workspace, st, proj: torch.Tensor, o: torch.Tensor) -> None:
         """attention of the prepared rows over the pages of layer `src`"""
         if self.kv_bits == 4:
-            seqops.attn_kv4(proj, st, L["desc"], src["kpool"], src["vpool"], o)
+            seqops.attn_kv4(proj, st, L["desc"], src["kpool"], src["vpool"], o, max_keys=self._keys)
         else:
             seqops.attn_ex(proj, st, L["desc"], src["kpool"], src["vpool"], o, ws.scratch, src.get("kpooled"), src.get("vpooled"))
 

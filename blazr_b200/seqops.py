@@ -65,7 +65,7 @@ SIGNATURES = {
     "polynorm": "pliipfpilp", "softcap": "plfp", "diff_combine": "piiiifffpip", "min_gru": "pliiipppipip", "rg_lru": "plplppfplipppiipip", "delta": "plppplppipzp",
     "embed_pos": "pppfpippppfpip", "sandwich_norm": "pppfppipippipp", "token_gate": "pliiplippip", "side_close": "pppfpppliippppipippipp",
     "selective_scan": "piplpplppppipzp", "parallel_close": "pp", "argmax": "piipp", "kv4_page_bytes": "iii", "kv4_store": "plplipiiiippp", "kv4_load": "pppiiiiplplp",
-    "attn_prep_kv4": "plppppp", "attn_kv4": "plpppppipzp", "attn_kv4_scratch_floats": "pp", "copy_pages": "ppiipip", "process_logits": "pliipppppppplplp"
+    "attn_prep_kv4": "plppppp", "attn_kv4": "plpppppipzip", "attn_kv4_scratch_floats": "ppi", "copy_pages": "ppiipip", "process_logits": "pliipppppppplplp"
 }
 
 
@@ -859,6 +859,7 @@ def parallel_close(x: torch.Tensor, y1: torch.Tensor, mult: float, eps: float, *
 
 # ---- a KV cache held in 4 bits -----------------------------------------------------------------------------------------------------------------------
 KV4_MAX_DIM = 128
+_U8 = torch.uint8
 
 
 def kv4_page_bytes(block_size: int, heads: int, dim: int) -> int:
@@ -893,24 +894,23 @@ def _on_device(name: str, fn, args: tuple, *tensors: Optional[torch.Tensor]) -> 
         _check(rc)
 
 
-def _kv4_pool_check(name: str, what: str, pool: torch.Tensor, block_size: int, heads: int, dim: int) -> None:
-    shape = pool.shape
-    if pool.dtype != torch.uint8 or len(shape) != 3 or shape[1] != heads or shape[2] != 20 * block_size * (1 if dim <= 32 else 2 if dim <= 64 else 4) or not pool.is_contiguous():
+def _kv4_pool_check(name: str, what: str, pool: torch.Tensor, shape: torch.Size, block_size: int, heads: int, dim: int) -> None:
+    if pool.dtype != _U8 or len(shape) != 3 or shape[1] != heads or shape[2] != 20 * block_size * (1 if dim <= 32 else 2 if dim <= 64 else 4) or not pool.is_contiguous():
         raise ValueError(f"{name}: the {what} pool is no contiguous uint8 [pages, {heads}, bytes] of pages of {block_size} positions and heads of {dim} values: "
-                         f"{pool.dtype} {tuple(pool.shape)}")
+                         f"{pool.dtype} {tuple(shape)}")
 
 
 def _kv4_rows(name: str, k: torch.Tensor, v: torch.Tensor, kpool: torch.Tensor, vpool: torch.Tensor, step: "StepDesc"):
     """(heads, size) of keys, the same of values, row strides"""
-    ks, vs, kt, vt, T = k.shape, v.shape, k.stride(), v.stride(), step.T
-    if kpool.dim() != 3 or vpool.dim() != 3:
-        raise ValueError(f"{name}: pools are uint8 [pages, heads, bytes], not {tuple(kpool.shape)} and {tuple(vpool.shape)}")
-    G, Gv = kpool.shape[1], vpool.shape[1]
+    ks, vs, kt, vt, T, kp, vp = k.shape, v.shape, k.stride(), v.stride(), step.T, kpool.shape, vpool.shape
+    if len(kp) != 3 or len(vp) != 3 or not kp[1] or not vp[1]:
+        raise ValueError(f"{name}: pools are uint8 [pages, heads, bytes], not {tuple(kp)} and {tuple(vp)}")
+    G, Gv = kp[1], vp[1]
     if len(ks) != 2 or len(vs) != 2 or kt[1] != 1 or vt[1] != 1 or ks[0] != T or vs[0] != T or ks[1] % G or vs[1] % Gv or k.dtype != v.dtype:
         raise ValueError(f"{name}: rows {tuple(ks)} and {tuple(vs)} of {T} tokens do not fit {G} and {Gv} heads")
-    D, V = ks[1] // G, vs[1] // Gv
-    _kv4_pool_check(name, "key", kpool, step.block_size, G, D)
-    _kv4_pool_check(name, "value", vpool, step.block_size, Gv, V)
+    D, V, bs = ks[1] // G, vs[1] // Gv, step.block_size
+    _kv4_pool_check(name, "key", kpool, kp, bs, G, D)
+    _kv4_pool_check(name, "value", vpool, vp, bs, Gv, V)
     return G, D, Gv, V, kt[0], vt[0]
 
 
@@ -937,10 +937,11 @@ def _kv4_layer(name: str, proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", k
     shape, ld = proj.shape, proj.stride()
     if len(shape) != 2 or ld[1] != 1 or proj.dtype != torch.float32 or shape[0] < step.T or shape[1] < need:
         raise ValueError(f"{name}: projection rows are row-major float32 [{step.T}, {need} or more], not {proj.dtype} {tuple(shape)}")
+    G, bs = d.G, step.block_size
     if kpool is not None:
-        _kv4_pool_check(name, "key", kpool, step.block_size, d.G, d.D)
+        _kv4_pool_check(name, "key", kpool, kpool.shape, bs, G, d.D)
     if vpool is not None:
-        _kv4_pool_check(name, "value", vpool, step.block_size, d.vg if d.vg > 0 else d.G, d.V)
+        _kv4_pool_check(name, "value", vpool, vpool.shape, bs, d.vg if d.vg > 0 else G, d.V)
     return ld[0]
 
 
@@ -953,8 +954,10 @@ def attn_prep_kv4(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: Op
 
 
 @_timed
-def attn_kv4(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: torch.Tensor, vpool: torch.Tensor, out: torch.Tensor, gate: Optional[torch.Tensor] = None):
-    """attn_ex over a 4-bit cache: out [T, H * V] (f32 or bf16) = softmax(q k^T * scale + mask) v, gated as the layer says.
+def attn_kv4(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: torch.Tensor, vpool: torch.Tensor, out: torch.Tensor, gate: Optional[torch.Tensor] = None,
+             max_keys: int = 0):
+    """attn_ex over a 4-bit cache: out [T, H * V] (f32 or bf16) = softmax(q k^T * scale + mask) v, gated as the layer says.  max_keys: keys of the step's longest
+    sequence, where the block tables hold many more (0: as many as they hold); the work is shared out by it, results do not depend on it but for roundings.
     (The work area of few long sequences is the call's own: no two calls, streams or graphs share it.)"""
     H, V, T = d.H, d.V, step.T
     need = d.q_col + H * d.D
@@ -972,9 +975,9 @@ def attn_kv4(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: torch.T
         d = d2
     L = lib()
     sref, dref = C.byref(step), C.byref(d)
-    need = L.b200seq_attn_kv4_scratch_floats(sref, dref)
+    need = L.b200seq_attn_kv4_scratch_floats(sref, dref, max_keys)
     scratch = torch.empty(need, dtype=torch.float32, device=proj.device) if need else None
-    _on_device("attn_kv4", L.b200seq_attn_kv4, (proj.data_ptr(), ld, sref, dref, kpool.data_ptr(), vpool.data_ptr(), out.data_ptr(), dt, scratch.data_ptr() if need else None, need),
+    _on_device("attn_kv4", L.b200seq_attn_kv4, (proj.data_ptr(), ld, sref, dref, kpool.data_ptr(), vpool.data_ptr(), out.data_ptr(), dt, scratch.data_ptr() if need else None, need, max_keys),
                proj, kpool, vpool, out, gate)
 
 

@@ -501,16 +501,17 @@ int b200seq_parallel_close(const b200seq_parallel_desc* d, void* stream);
  * store: k [T, G * D], v [T, Gv * V] (f32 or bf16, row strides ldk, ldv) go to the pages of the step's tokens.
  * load:  the same rows back in f32, as what they stand for (rows behind another owner's page or of no page are left as they are).
  * attn_prep_kv4 is b200seq_attn_prep_ex, attn_kv4 is b200seq_attn_ex, over such pools (no pooled blocks, no latents; D, V <= 128): q and sums in 32 bits, the cache's
- * values as they are held.  A query that is not finite gives a row of NaN.  scratch: f32 work area of b200seq_attn_kv4_scratch_floats(...) floats (0 for most steps) or null:
- * with it, few sequences of many keys use the whole GPU. */
+ * values as they are held.  A query that is not finite gives a row of NaN.  scratch: f32 work area of b200seq_attn_kv4_scratch_floats(...) floats (0 for most steps) or
+ * null: with it, few sequences of many keys use the whole GPU.  max_keys: as many keys as the step's longest sequence has, or 0 for what the block tables hold; the work is shared
+ * out by it (right for any number, faster for one that is near). */
 int64_t b200seq_kv4_page_bytes(int block_size, int G, int D);
 int b200seq_kv4_store(const void* k, int64_t ldk, const void* v, int64_t ldv, int in_dtype, const b200seq_step* st, int G, int D, int Gv, int V, void* kpool, void* vpool,
                       void* stream);
 int b200seq_kv4_load(const void* kpool, const void* vpool, const b200seq_step* st, int G, int D, int Gv, int V, float* k, int64_t ldk, float* v, int64_t ldv, void* stream);
 int b200seq_attn_prep_kv4(float* proj, int64_t ld, const b200seq_step* st, const b200seq_attn_desc* d, void* kpool, void* vpool, void* stream);
 int b200seq_attn_kv4(const float* proj, int64_t ld, const b200seq_step* st, const b200seq_attn_desc* d, const void* kpool, const void* vpool, void* out, int out_dtype,
-                     float* scratch, size_t scratch_floats, void* stream);
-size_t b200seq_attn_kv4_scratch_floats(const b200seq_step* st, const b200seq_attn_desc* d);
+                     float* scratch, size_t scratch_floats, int max_keys, void* stream);
+size_t b200seq_attn_kv4_scratch_floats(const b200seq_step* st, const b200seq_attn_desc* d, int max_keys);
 
 /* Page pairs[i][1] of every pool becomes a copy of its page pairs[i][0], i < n.  pools, page_bytes, pairs: HOST arrays, read during the call; every pool has `pages` pages.
  * A page may be read by several pairs, but not written twice and not both read and written (B200SEQ_ERR_INVALID_ARG, nothing is copied). */

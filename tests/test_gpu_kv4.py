@@ -421,3 +421,24 @@ def test_entries_without_tokens_and_rows_behind_the_last(ops, entries, D, odt):
     w = len(table[0]) - 1
     out = run(ent, pos, start, [r[:w] for r in table], T, flags=1)
     assert bool((out[:T][torch.tensor([p >= 16 * w for p in pos], device=DEV)] == 3).all()) and bool((out[T:] == 3).all())
+
+
+@pytest.mark.parametrize("entries,D,keys", [([(1, 5000)], 128, 5001), ([(1, 30)] * 3, 64, 31), ([(16, 0)], 64, 16), ([(70, 3000)], 64, 3070), ([(5, 700), (3, 0)], 128, 705),
+                                            ([(300, 200)], 128, 500)])
+def test_results_for_any_number_of_keys_named(ops, entries, D, keys):
+    """the keys that a caller names share the work out and do no more: too few, as many as there are, too many"""
+    rng = np.random.default_rng(D + keys)
+    st, keep, slots, pages = step(ops, entries, 16, rng)
+    kp, vp = ops.kv4_pool(pages, 16, 2, D, DEV), ops.kv4_pool(pages, 16, 2, D, DEV)
+    fill, keep2, *_ = step(ops, [(16 * pages, 0)], 16, np.random.default_rng(0), spare=0)      # (every row of every page)
+    ops.kv4_store(torch.randn(fill.T, 2 * D, device=DEV), torch.randn(fill.T, 2 * D, device=DEV), fill, kp, vp)
+    d = ops.attn_desc(8, 2, D, D, 0.125, gated=False, kv_shared=True)
+    q = torch.randn(st.T, d.width, device=DEV)
+    outs = []
+    for named in (0, keys, 1, 64, 1 << 20):
+        out = torch.full((st.T, 8 * D), 3.0, device=DEV)
+        ops.attn_kv4(q, st, d, kp, vp, out, max_keys=named)
+        outs.append(out)
+    for o in outs[1:]:
+        assert (o - outs[0]).abs().max().item() <= 4e-6 * outs[0].abs().max().item()
+    assert ops.error_flags() == 0

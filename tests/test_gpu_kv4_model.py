@@ -177,3 +177,18 @@ def test_samples_penalties_and_masks(models):
     pushed = eng.generate([prompt(40)], SamplingParams(max_new_tokens=12, logit_bias={5: 1e4}, frequency_penalty=3e3))[0]
     assert pushed[:4] == [5] * 4 and pushed[4:].count(5) == 0            # 1e4 - 3e3 n: four times
     assert seqops.error_flags() == 0
+
+
+def test_captured_steps_of_growing_sequences(models):
+    """a captured step is made for so many keys; sequences that outgrow them go through another one"""
+    m, toks = models("Vodelix"), prompt(270)
+    got = []
+    for graphs in (True, False):
+        m.use_graphs = graphs
+        eng = engine(m, max_tokens=4096)
+        eng.run_entries([{"id": "a", "tokens": toks[:250], "want": []}, {"id": "b", "tokens": toks[:40], "want": []}])
+        got.append(np.stack([eng.run_entries([{"id": "a", "tokens": [t], "want": [0]}, {"id": "b", "tokens": [t], "want": [0]}]) for t in toks[250:]]))
+        if graphs:
+            assert {k[2] for k in m._graphs} == {256, 512}
+    m.use_graphs = True
+    near(got[0], got[1])

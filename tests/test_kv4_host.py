@@ -59,7 +59,7 @@ def layer(**o):
                                     (layer(H=7), -1), (layer(D=0), -1), (layer(keep_first=2), -1), (layer(vg=3), -1)])
 def test_layers_that_are_refused(d, code):
     st = step()
-    assert entry("attn_kv4")(P, 1024, C.byref(st), C.byref(d), P, P, P, 0, None, 0, None) == code
+    assert entry("attn_kv4")(P, 1024, C.byref(st), C.byref(d), P, P, P, 0, None, 0, 0, None) == code
     if not d.kv_ld:
         assert entry("attn_prep_kv4")(P, 1024, C.byref(st), C.byref(d), P, P, None) == code
 
@@ -68,7 +68,7 @@ def test_layers_that_are_refused(d, code):
                                 ops.StepDesc(P, P, P, P, P, 0, 2, 1, 4, 16)], ids=range(8))
 def test_steps_that_are_refused(st):
     d = layer()
-    assert entry("attn_kv4")(P, 1024, C.byref(st), C.byref(d), P, P, P, 0, None, 0, None) < 0
+    assert entry("attn_kv4")(P, 1024, C.byref(st), C.byref(d), P, P, P, 0, None, 0, 0, None) < 0
     if st.B:
         assert entry("kv4_store")(P, 128, P, 128, 0, C.byref(st), 2, 64, 2, 64, P, P, None) < 0
         assert entry("kv4_load")(P, P, C.byref(st), 2, 64, 2, 64, P, 128, P, 128, None) < 0
@@ -80,13 +80,13 @@ def test_arguments_that_are_refused():
     for bad in ((None, 1024, C.byref(st), C.byref(d), P, P, P, 0, None), (P, 1024, C.byref(st), C.byref(d), None, P, P, 0, None), (P, 1024, C.byref(st), C.byref(d), P, None, P, 0, None),
                 (P, 1024, C.byref(st), C.byref(d), P, P, None, 0, None), (P, 1024, C.byref(st), C.byref(d), P, P, P, 1, None), (P, 1024, C.byref(st), C.byref(d), P + 8, P, P, 0, None),
                 (P, 1024, None, C.byref(d), P, P, P, 0, None), (P, 1024, C.byref(st), None, P, P, P, 0, None)):
-        assert entry("attn_kv4")(*bad[:-1], None, 0, None) == -1
+        assert entry("attn_kv4")(*bad[:-1], None, 0, 0, None) == -1
     for bad in ((P, 100, P, 128, 0, C.byref(st), 2, 64, 2, 64, P, P, None), (P, 128, P, 128, 7, C.byref(st), 2, 64, 2, 64, P, P, None), (P, 128, P, 128, 0, C.byref(st), 0, 64, 2, 64, P, P, None),
                 (None, 128, P, 128, 0, C.byref(st), 2, 64, 2, 64, P, P, None), (P, 128, P, 128, 0, C.byref(st), 2, 64, 2, 64, P + 4, P, None)):
         assert entry("kv4_store")(*bad) == -1
     assert entry("kv4_store")(P, 1024, P, 128, 0, C.byref(st), 2, 129, 2, 64, P, P, None) == -2
     none = step(T=0)
-    assert entry("attn_kv4")(P, 1024, C.byref(none), C.byref(d), P, P, P, 0, None, 0, None) == 0
+    assert entry("attn_kv4")(P, 1024, C.byref(none), C.byref(d), P, P, P, 0, None, 0, 0, None) == 0
     assert entry("kv4_store")(None, 128, None, 128, 0, C.byref(none), 2, 64, 2, 64, P, P, None) == 0
 
 
