@@ -675,13 +675,20 @@ int64_t most_keys(const b200seq_step& st, const b200seq_attn_desc& d, int max_ke
 }
 // How the keys of a step are shared.  Row tiles and heads go to a CTA each, or to a cluster of up to 8 while there are CTAs for all and keys for all their warps.  Few of them
 // with many keys are dealt out evenly, with a second launch for those that several CTAs have; that costs about 8 us a row tile begun and 5 for the launch (32 sequences, 256
-// row tiles and heads: 65 us dealt, 55 not; one sequence of 131072 keys: 62 dealt, 110 in clusters).  CTAs have the 8 or 4 warps whose last wave is the fuller one (256 row tiles
+// row tiles and heads: 65 us dealt, 55 not; one sequence of 40000 keys, heads of 64: 26 dealt, 33 in a cluster; of 131072, heads of 128: 66 and 110).  CTAs have the 8 or 4 warps whose last wave is the fuller one (256 row tiles
 // and heads of 128, 3000 keys: 55 us with 8, 77 with 4; 16 x 5 tokens, 384 of 64, 1500 keys: 29 with 8, 24 with 4); the small ones for heads of up to 64 where that is the same.
 struct Plan {
     int64_t tiles, real;     // row tiles: upper bound; as many as there are if all entries are equally long
     int heads, cluster, warps, ctas;
     bool dealt;
 };
+// us of row tiles with kt key tiles each that have CTAs of their own, or whose keys are dealt out
+double shared_us(const Plan& p, bool small, double kt) {
+    const double waves = (double)p.real * p.heads * p.cluster / p.ctas, share = kt / (p.warps * p.cluster), least = p.warps == 4 ? 0.4 : (small ? 0.85 : 0.53);
+    const double tile = (small ? 1.5 : 3.6) * (waves < least ? least : (waves < 1.0 ? waves : 1.0));
+    return (waves < 1.0 ? 1.0 : waves) * ((small ? 4.0 : 5.0) + tile * (share < 1.0 ? 1.0 : share)) + 2.0;
+}
+double dealt_us(bool small, double units, double kt) { return small ? 18.0 + units * kt / 1200.0 : 15.5 + units * kt / 645.0; }
 Plan plan(const b200seq_step& st, const b200seq_attn_desc& d, int max_keys) {
     Plan p;
     const int R = d.H / d.G, Rb = R < ROWS ? R : ROWS, QT = ROWS / Rb;
@@ -701,7 +708,7 @@ Plan plan(const b200seq_step& st, const b200seq_attn_desc& d, int max_keys) {
         const double full = (double)n / (double)(waves * ctas);
         if (full > best * 1.05) best = full, p.warps = warps, p.ctas = ctas, p.cluster = cluster;
     }
-    p.dealt = st.block_size % 16 == 0 && p.tiles <= MAX_TILES && units * p.cluster * 2 <= p.ctas && key_tiles > 8ll * p.cluster * p.warps;
+    p.dealt = st.block_size % 16 == 0 && p.tiles <= MAX_TILES && units * p.cluster * 2 <= p.ctas && dealt_us(small, (double)units, (double)key_tiles) + 2.0 < shared_us(p, small, (double)key_tiles);
     if (p.dealt) p.cluster = 1, p.warps = small ? 4 : 8, p.ctas = ctas_of(p.warps);
     return p;
 }
@@ -716,15 +723,15 @@ cudaError_t launch_values(int nv, const Attn4Args& a, const b200seq_step& st, di
     return nv == 1 ? launch_form<NK, 1>(a, st, grid, p, cs) : (nv == 2 ? launch_form<NK, 2>(a, st, grid, p, cs) : launch_form<NK, 4>(a, st, grid, p, cs));
 }
 // Which kernel is the faster one, from the key tiles a CTA has at most.  us, fitted to 57 steps of 8 to 288 tokens, timed with each of the two (the choice is at
-// most 12 % behind the faster one).  Here: a wave of CTAs takes 4 (5 with heads above 64) and 1.5 (3.6) a key tile of 32 and warp; keys that are dealt out 10, and 1290 (675) key tiles a us.  On the tensor cores: 7.5 (9; f32
-// 11) a CTA and 0.8 (0.75; f32 1.4) a key tile of 64, 4 more for keys in several parts.  Measured, us, here / there, 32 query heads of 8 key heads of 64 (of 128):
+// most 13 % behind the faster one).  Here (shared_us, dealt_us): a wave of CTAs takes 4 (5 with heads above 64) and 1.5 (3.6) a key tile of 32 and warp, down to 0.6 (four
+// warps) or 1.3 (1.9) where a CTA has an SM to itself; keys that are dealt out 18 (15.5), and 1200 (645) key tiles a us.  On the tensor cores: 7.5 (9; f32 11) a CTA
+// and 0.8 (0.75; f32 1.4) a key tile of 64, 4 more for keys in several parts.  Measured, us, here / there, 32 query heads of 8 key heads of 64 (of 128):
 //   1 x 64 tokens                6 /  8 ( 7 / 10)     16 x 9 behind 1500   43 / 28 (66 / 31)     32 x 2 behind 2000   34 / 64 (45 / 73)
 //   1 x 32 behind 4000          22 / 22 (34 / 25)      4 x 8 behind 8000   56 / 36 (83 / 39)      4 x 64 behind 300   27 / 13 (38 / 14)
 bool tc_is_faster(const b200seq_step& st, const b200seq_attn_desc& d, int max_keys, const Plan& p, const Attn4TcPlan& tp, bool f32) {
     const bool small = d.D <= 64 && d.V <= 64;
-    const double keys = (double)most_keys(st, d, max_keys, 0), kt = (keys + KT - 1) / KT, units = (double)p.real * p.heads;
-    const double waves = units * p.cluster / p.ctas, share = kt / (p.warps * p.cluster);
-    const double here = p.dealt ? 10.0 + units * kt / (small ? 1290.0 : 675.0) : (waves < 1.0 ? 1.0 : waves) * ((small ? 4.0 : 5.0) + (small ? 1.5 : 3.6) * (share < 1.0 ? 1.0 : share)) + 2.0;
+    const double keys = (double)most_keys(st, d, max_keys, 0), kt = (keys + KT - 1) / KT;
+    const double here = p.dealt ? dealt_us(small, (double)p.real * p.heads, kt) : shared_us(p, small, kt);
     const double set_up = small ? 7.5 : (f32 ? 11.0 : 9.0), each = small ? 0.8 : (f32 ? 1.4 : 0.75);
     const int64_t tc_waves = (tp.real * tp.parts + 147) / 148;
     const double there = (double)tc_waves * (set_up + each * (keys / 64.0 / tp.parts + 0.5)) + 2.0 + (tp.parts > 1 ? 4.0 : 0.0);
