@@ -308,3 +308,27 @@ def test_rules_that_are_refused(monkeypatch):
     while eng.has_work():
         eng.step()
     assert eng.requests["x"].output == alone([1, 2], 3)
+
+
+def test_the_command_line_has_them(monkeypatch, capsys):
+    """options of `generate`: bits of the cache, samples, penalties, biases; a line a sample"""
+    import json
+
+    from blazr_b200 import cli
+    seen, made = [], {}
+    fake_rules(monkeypatch, seen)
+
+    class Model(PagedModel):
+        def allocate(self, *a, kv_bits=32):
+            made.update(bits=kv_bits)
+            super().allocate(*a)
+    monkeypatch.setattr(cli, "_load", lambda *a: Model())
+    assert cli.main(["generate", "--model", "x", "--prompt", "3,1,4", "--prompt", "2,7", "--max-new", "5", "--samples", "3", "--kv-bits", "4", "--repetition-penalty", "1.5",
+                     "--presence-penalty", "0.25", "--frequency-penalty", "0.5", "--logit-bias", "7:-2.5,9:1"]) == 0
+    lines = [json.loads(s) for s in capsys.readouterr().out.splitlines()]
+    assert [x["prompt"] for x in lines] == [[3, 1, 4]] * 3 + [[2, 7]] * 3 and made == {"bits": 4}
+    assert [x["tokens"] for x in lines] == [alone([3, 1, 4], 5)] * 3 + [alone([2, 7], 5)] * 3
+    _, rules, kw = seen[0]
+    assert rules[0].tolist() == [1.5, 0.25, 0.5, 0.0] and kw["bias_ids"][:2].tolist() == [7, 9] and kw["bias_vals"][:2].tolist() == [-2.5, 1.0]
+    assert cli.main(["generate", "--model", "x", "--prompt", "2,7", "--max-new", "4"]) == 0 and made == {"bits": 32}
+    assert json.loads(capsys.readouterr().out) == {"prompt": [2, 7], "tokens": alone([2, 7], 4)}
