@@ -21,6 +21,7 @@ struct LogitArgs {
     const float* rules;                        // [R][4]: repetition, presence, frequency, temperature
     const int32_t *hist, *hist_start, *hist_prompt;
     const int32_t *bias_start, *bias_ids;
+    int nhist, nbias;
     const float* bias_vals;
     const uint32_t* mask;                      // [R][mask_ld]: bit v % 32 of word v / 32
     int64_t mask_ld;
@@ -39,7 +40,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 1) process_logi
     const int row = blockIdx.y, v0 = blockIdx.x * S, n = min(S, a.V - v0);
     const float4 rule = ld4(a.rules + 4 * (int64_t)row);   // repetition, presence, frequency, temperature
     int h0 = 0, h1 = 0, prompt = 0, b0 = 0, b1 = 0;
-    if (a.hist) h0 = a.hist_start[row], h1 = a.hist_start[row + 1], prompt = h0 + a.hist_prompt[row];
+    if (a.hist) h0 = a.hist_start[row], h1 = a.hist_start[row + 1], prompt = a.hist_prompt[row];
     if (a.bias_ids) b0 = a.bias_start[row], b1 = a.bias_start[row + 1];
     const float* x = a.x + row * a.ldx + v0;
     float4 v[ITEMS];
@@ -51,10 +52,13 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 1) process_logi
         else v[k] = make_float4(i < n ? x[i] : 0.f, i + 1 < n ? x[i + 1] : 0.f, i + 2 < n ? x[i + 2] : 0.f, i + 3 < n ? x[i + 3] : 0.f);
         bits[k] = a.mask && i < n ? a.mask[row * a.mask_ld + ((v0 + i) >> 5)] >> ((v0 + i) & 31) : 0xFu;
     }
+    // a row's list that is not one: the row has none
+    bool odd = h0 < 0 || h0 > h1 || h1 > a.nhist || b0 < 0 || b0 > b1 || b1 > a.nbias;
+    if (odd) h0 = h1 = b0 = b1 = 0;
+    prompt += h0;
     const bool biased = b1 > b0;
     for (int i = threadIdx.x; i < (biased ? 2 * S : S) / 4; i += THREADS) reinterpret_cast<uint4*>(table)[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
-    bool odd = false;
 #pragma unroll 4
     for (int i = h0 + (int)threadIdx.x; i < h1; i += THREADS) {
         const int id = a.hist[i];
@@ -122,17 +126,18 @@ cudaError_t launch(const LogitArgs& a, int R, cudaStream_t cs) {
 
 using namespace b200seq;
 
-extern "C" int b200seq_process_logits(const float* x, int64_t ldx, int R, int V, const float* rules, const int32_t* hist, const int32_t* hist_start, const int32_t* hist_prompt,
-                                      const int32_t* bias_start, const int32_t* bias_ids, const float* bias_vals, const uint32_t* mask, int64_t mask_ld, float* out, int64_t ldo,
-                                      void* stream) {
+extern "C" int b200seq_process_logits(const float* x, int64_t ldx, int R, int V, const float* rules, const int32_t* hist, int nhist, const int32_t* hist_start,
+                                      const int32_t* hist_prompt, const int32_t* bias_start, const int32_t* bias_ids, const float* bias_vals, int nbias, const uint32_t* mask,
+                                      int64_t mask_ld, float* out, int64_t ldo, void* stream) {
     if (R < 0 || V < 1 || (R > 0 && (!x || !out || !rules))) return fail(B200SEQ_ERR_INVALID_ARG, "process_logits: bad sizes or null arrays");
+    if (nhist < 0 || nbias < 0) return fail(B200SEQ_ERR_INVALID_ARG, "process_logits: negative lengths");
     if ((hist != nullptr) != (hist_start != nullptr) || (hist != nullptr) != (hist_prompt != nullptr)) return fail(B200SEQ_ERR_INVALID_ARG, "process_logits: a history has ids, row starts and prompt lengths");
     if ((bias_ids != nullptr) != (bias_start != nullptr) || (bias_ids != nullptr) != (bias_vals != nullptr)) return fail(B200SEQ_ERR_INVALID_ARG, "process_logits: biases have ids, values and row starts");
     if (R > 65535) return fail(B200SEQ_ERR_UNSUPPORTED, "process_logits: up to 65535 rows");
     if (R > 1 && (ldx < V || ldo < V || (mask && mask_ld < (V + 31) / 32))) return fail(B200SEQ_ERR_INVALID_ARG, "process_logits: row strides below a row's length");
     if (reinterpret_cast<uintptr_t>(rules) & 15) return fail(B200SEQ_ERR_INVALID_ARG, "process_logits: rules start on a 16-byte boundary");
     if (R == 0) return 0;
-    const LogitArgs a{x, out, ldx, ldo, V, rules, hist, hist_start, hist_prompt, bias_start, bias_ids, bias_vals, mask, mask_ld,
+    const LogitArgs a{x, out, ldx, ldo, V, rules, hist, hist_start, hist_prompt, bias_start, bias_ids, nhist, nbias, bias_vals, mask, mask_ld,
                       ((ldx | ldo) & 3) == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 15) == 0, error_flag_dev()};
     // Every slice reads the row's whole history: slices of 8192 tokens where they fill the GPU, of 1024 otherwise.
     const cudaError_t e = (int64_t)R * ((V + 8191) / 8192) >= 2 * 148 ? launch<1024, 2>(a, R, (cudaStream_t)stream) : launch<256, 1>(a, R, (cudaStream_t)stream);

@@ -65,7 +65,7 @@ SIGNATURES = {
     "polynorm": "pliipfpilp", "softcap": "plfp", "diff_combine": "piiiifffpip", "min_gru": "pliiipppipip", "rg_lru": "plplppfplipppiipip", "delta": "plppplppipzp",
     "embed_pos": "pppfpippppfpip", "sandwich_norm": "pppfppipippipp", "token_gate": "pliiplippip", "side_close": "pppfpppliippppipippipp",
     "selective_scan": "piplpplppppipzp", "parallel_close": "pp", "argmax": "piipp", "kv4_page_bytes": "iii", "kv4_store": "plplipiiiippp", "kv4_load": "pppiiiiplplp",
-    "attn_prep_kv4": "plppppp", "attn_kv4": "plpppppipzip", "attn_kv4_scratch_floats": "ppi", "copy_pages": "ppiipip", "process_logits": "pliipppppppplplp"
+    "attn_prep_kv4": "plppppp", "attn_kv4": "plpppppipzip", "attn_kv4_scratch_floats": "ppi", "copy_pages": "ppiipip", "process_logits": "pliippipppppiplplp"
 }
 
 
@@ -1034,6 +1034,6 @@ def process_logits(logits: torch.Tensor, rules: torch.Tensor, out: Optional[torc
     if bias_ids is not None and bias_ids.numel() == 0:
         bias_ids = bias_start = bias_vals = None
     _on_device("process_logits", lib().b200seq_process_logits,
-               (logits.data_ptr(), lx[0] if R > 1 else V, R, V, rules.data_ptr(), _p(hist), _p(hist_start), _p(hist_prompt), _p(bias_start), _p(bias_ids), _p(bias_vals),
-                _p(mask), lm, out.data_ptr(), lo[0] if R > 1 else V), logits, rules, out, hist, hist_start, hist_prompt, bias_start, bias_ids, bias_vals, mask)
+               (logits.data_ptr(), lx[0] if R > 1 else V, R, V, rules.data_ptr(), _p(hist), hist.numel() if hist is not None else 0, _p(hist_start), _p(hist_prompt),
+                _p(bias_start), _p(bias_ids), _p(bias_vals), bias_ids.numel() if bias_ids is not None else 0, _p(mask), lm, out.data_ptr(), lo[0] if R > 1 else V), logits, rules, out, hist, hist_start, hist_prompt, bias_start, bias_ids, bias_vals, mask)
     return out

@@ -522,9 +522,10 @@ int b200seq_copy_pages(void* const* pools, const int64_t* page_bytes, int npools
  *   a token that stands n > 0 times behind the first hist_prompt[r] of them: x - n * frequency - presence
  *   x + bias for the tokens of bias_ids[bias_start[r] .. bias_start[r + 1]) (a token named twice has the last one's)
  *   x / temperature (0: as it is);   -inf where bit v % 32 of mask[r][v / 32] is 0
- * History, biases and mask are each optional (null).  An id outside the vocabulary is passed over and raises bit 4 of the error flags. */
-int b200seq_process_logits(const float* x, int64_t ldx, int R, int V, const float* rules, const int32_t* hist, const int32_t* hist_start, const int32_t* hist_prompt,
-                           const int32_t* bias_start, const int32_t* bias_ids, const float* bias_vals, const uint32_t* mask, int64_t mask_ld, float* out, int64_t ldo,
+ * History (nhist ids of all rows), biases (nbias) and mask are each optional (null).  An id outside the vocabulary is passed over, a row whose starts are not in order within
+ * nhist or nbias has neither history nor biases; both raise bit 4 of the error flags. */
+int b200seq_process_logits(const float* x, int64_t ldx, int R, int V, const float* rules, const int32_t* hist, int nhist, const int32_t* hist_start, const int32_t* hist_prompt,
+                           const int32_t* bias_start, const int32_t* bias_ids, const float* bias_vals, int nbias, const uint32_t* mask, int64_t mask_ld, float* out, int64_t ldo,
                            void* stream);
 
 /* ids[r] = argmax_v logits[r][v] (first maximum) */

@@ -218,3 +218,24 @@ def test_temperatures_whose_reciprocal_is_no_number(ops, V):
     want = rules64(a).astype(np.float32)                       # (infinities: beyond f32)
     got = run(ops, a).cpu().numpy()
     assert np.array_equal(np.isinf(want), np.isinf(got)) and np.array_equal(got[::2, ::2], np.zeros_like(got[::2, ::2])) and np.array_equal(np.sign(want), np.sign(got))
+
+
+@pytest.mark.parametrize("what,starts", [("hist_start", [0, 5, 99999]), ("hist_start", [-3, 5, 9]), ("hist_start", [0, 9, 5]), ("bias_start", [0, 5, 99999]), ("bias_start", [7, 5, 9])])
+@pytest.mark.parametrize("V", [300, 128256])
+def test_rows_whose_lists_are_none(ops, what, starts, V):
+    """starts that are not in order within their ids raise the flag, and the row goes without; nothing behind the ids is read"""
+    a = make(np.random.default_rng(8), 2, V, 0, 0, False)
+    a.update(hist=np.arange(9, dtype=np.int32), hist_start=np.array([0, 5, 9], np.int32), hist_prompt=np.zeros(2, np.int32), bias_ids=np.arange(9, dtype=np.int32),
+             bias_start=np.array([0, 5, 9], np.int32), bias_vals=np.ones(9, np.float32))
+    got = {True: dict(a), False: dict(a)}
+    got[True][what] = np.array(starts, np.int32)
+    bad = [starts[0] < 0 or starts[0] > starts[1], starts[1] > starts[2] or starts[2] > 9]
+    out = run(ops, got[True]).cpu().numpy()
+    assert ops.error_flags() == 16
+    plain = rules64({k: a[k] for k in ("logits", "rules")} | dict(hist=np.zeros(0, np.int32), hist_start=np.zeros(3, np.int32), hist_prompt=np.zeros(2, np.int32)))
+    full = rules64(got[False])
+    for r in range(2):
+        if bad[r]:
+            same(torch.from_numpy(out[r]), plain[r])
+        elif starts[r:r + 2] == [0, 5, 9][r:r + 2]:
+            same(torch.from_numpy(out[r]), full[r])

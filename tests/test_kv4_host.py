@@ -123,8 +123,8 @@ def test_copies_that_are_refused():
 
 def test_logit_rules_that_are_refused():
     f = entry("process_logits")
-    ok = [P, 100, 2, 100, P, P, P, P, P, P, P, P, 4, P, 100, None]
-    for i, v in ((0, None), (1, 99), (2, -1), (3, 0), (4, None), (4, P + 4), (5, None), (6, None), (7, None), (8, None), (9, None), (10, None), (12, 3), (13, None), (14, 50)):
+    ok = [P, 100, 2, 100, P, P, 8, P, P, P, P, P, 8, P, 4, P, 100, None]
+    for i, v in ((0, None), (1, 99), (2, -1), (3, 0), (4, None), (4, P + 4), (5, None), (6, -1), (7, None), (8, None), (9, None), (10, None), (11, None), (12, -1), (14, 3), (15, None), (16, 50)):
         a = list(ok)
         a[i] = v
         assert f(*a) == -1, (i, v)
