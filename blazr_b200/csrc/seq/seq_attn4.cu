@@ -113,10 +113,10 @@ __device__ __forceinline__ void fetch_unit(uint32_t dst, uint32_t piece, uint32_
 }
 // the 16 keys from key0 on of one pool, from pages that a half may cross; keys behind `hi` are read from hi's row
 template <int NG>
-__device__ __forceinline__ void fetch_rows(uint32_t dst, const uint8_t* pool, const int32_t* bt, int bs, int key0, int hi, int g, int G, int lane) {
+__device__ __forceinline__ void fetch_rows(uint32_t dst, const uint8_t* pool, const int32_t* bt, int bs, int key0, int hi, int g, int G, int lane, int* err) {
     for (int i = lane; i < 16 * NG * 5; i += 32) {
         const int row = i / (NG * 5), w = i - row * (NG * 5), key = min(key0 + row, hi), pg = key / bs;
-        const Kv4Row at = kv4_row(bt[pg], key - pg * bs, bs, g, G, NG);
+        const Kv4Row at = kv4_row(kv4_page_read(bt[pg], err), key - pg * bs, bs, g, G, NG);
         if (w < NG * 4) copy4(dst + 16 * swz(row * NG + (w >> 2)) + 4 * (w & 3), pool + at.codes + 4 * w);
         else copy4(dst + NG * 256 + row * NG * 4 + 4 * (w - NG * 4), pool + at.params + 4 * (w - NG * 4));
     }
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident(WARPS)) attn4_kernel(cons
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     if (key_n + 16 * s > hi) break;
-                    const uint32_t page = (uint32_t)(s ? page1 : page0);
+                    const uint32_t page = (uint32_t)kv4_page_read(s ? page1 : page0, a.err);
                     const uint8_t *k = kg + (uint64_t)page * kpage, *v = vg + (uint64_t)page * vpage, *par = pg + (uint64_t)page * ppage;
                     if (upp != 1) {
                         const int u = (unit + s) % upp;
@@ -299,8 +299,8 @@ __global__ void __launch_bounds__(WARPS * 32, resident(WARPS)) attn4_kernel(cons
                 }
             } else {
                 for (int s = 0; s < 2 && key_n + 16 * s <= hi; ++s) {
-                    fetch_rows<NK>(dst + s * HALF, a.kpool, bt, bs, key_n + 16 * s, hi, g, a.G, lane);
-                    fetch_rows<NV>(dst + s * HALF + KB, a.vpool, bt, bs, key_n + 16 * s, hi, g / a.vdiv, Gv, lane);
+                    fetch_rows<NK>(dst + s * HALF, a.kpool, bt, bs, key_n + 16 * s, hi, g, a.G, lane, a.err);
+                    fetch_rows<NV>(dst + s * HALF + KB, a.vpool, bt, bs, key_n + 16 * s, hi, g / a.vdiv, Gv, lane, a.err);
                 }
             }
             if (i + 1 < nt) key_n = span.key0(me + (i + 1) * walkers), lookup();

@@ -143,7 +143,7 @@ __device__ __forceinline__ void put_centres(const Codes<N>& c0, const Codes<N>& 
 // expanded, its pages a tile earlier.  stage: of tile 0 (tile 1's is `pitch` bytes on); full, free: the stages' barriers.
 template <int N, bool KEY>
 __device__ __forceinline__ void load_tiles(const uint8_t* pool, const int32_t* bt, int bs, int g, int G, const KeySpan<KT>& span, int split, int parts, int ntile, int hi, uint32_t stage,
-                                           uint32_t pitch, uint32_t full, uint32_t free, int lw, int lane, volatile int* ab) {
+                                           uint32_t pitch, uint32_t full, uint32_t free, int lw, int lane, volatile int* ab, int* err) {
     // eight lanes store pieces of keys k and k + 4: their places in the swizzle fill a 128-byte line
     const int j8 = lane >> 2, key = lw * 16 + ((j8 & 1) << 2) + (j8 >> 1), quarter = lane & 3;
     if (quarter == 0) {   // the pieces behind m + 8 s stay zero
@@ -175,13 +175,13 @@ __device__ __forceinline__ void load_tiles(const uint8_t* pool, const int32_t* b
     Codes<N> next[2];
     auto fetch = [&]() {   // the tile that was looked up
         if (whole) {
-            const uint64_t at = (uint64_t)(uint32_t)page[0] * page_bytes;
+            const uint64_t at = (uint64_t)(uint32_t)kv4_page_read(page[0], err) * page_bytes;
             load_codes<N>(next[0], w0 + at, p0 + at, pos <= hi), load_codes<N>(next[1], w0 + at + pitch_w, p0 + at + pitch_p, pos + 8 <= hi);
         } else {
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int kp = min(pos + 8 * u, hi);
-                const Kv4Row at = kv4_row(page[u], kp % bs, bs, g, G, N);
+                const Kv4Row at = kv4_row(kv4_page_read(page[u], err), kp % bs, bs, g, G, N);
                 load_codes<N>(next[u], pool + at.codes + 4 * N * quarter, pool + at.params, pos + 8 * u <= hi);
             }
         }
@@ -633,8 +633,8 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
         // ===================== loaders: four warps for keys, four for values =====================
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(GROUPS == 2 ? 64 : 104));
         const int lw = warp - SW;
-        if (lw < 4) load_tiles<NK, true>(a.kpool, bt, bs, g, G, span, split, a.parts, ntile, hi, kv, STAGE, k_full, k_free, lw, lane, ab);
-        else load_tiles<NV, false>(a.vpool, bt, bs, g / a.vdiv, G / a.vdiv, span, split, a.parts, ntile, hi, kv + KBYTES, STAGE, v_full, v_free, lw - 4, lane, ab);
+        if (lw < 4) load_tiles<NK, true>(a.kpool, bt, bs, g, G, span, split, a.parts, ntile, hi, kv, STAGE, k_full, k_free, lw, lane, ab, a.err);
+        else load_tiles<NV, false>(a.vpool, bt, bs, g / a.vdiv, G / a.vdiv, span, split, a.parts, ntile, hi, kv + KBYTES, STAGE, v_full, v_free, lw - 4, lane, ab, a.err);
     } else {
         // ===================== MMA issuer =====================
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(GROUPS == 2 ? 32 : 64));

@@ -12,7 +12,7 @@ struct Kv4Rows {
     int G, D, Gv, V, vec;
 };
 
-// position of a token in its sequence's pages; -1 (and the error flag) outside the block table
+// position of a token in its sequence's pages; negative (and the error flag) outside the block table or where the table has no page
 __device__ __forceinline__ int kv4_page(const b200seq_step& st, int t, int& o, int* err) {
     const int pos = st.tok_pos[t], b = pos / st.block_size;
     o = pos - b * st.block_size;
@@ -20,7 +20,9 @@ __device__ __forceinline__ int kv4_page(const b200seq_step& st, int t, int& o, i
         atomicOr(err, 1);
         return -1;
     }
-    return st.block_table[(int64_t)st.tok_ent[t] * st.max_blocks + b];
+    const int page = st.block_table[(int64_t)st.tok_ent[t] * st.max_blocks + b];
+    if (page < 0) atomicOr(err, 1);
+    return page;
 }
 
 // A lane's eight codes and its group's parameters into a row.  Lanes of neighbouring groups change halves, so that value codes are stored as 32-bit words too.

@@ -38,6 +38,12 @@ __device__ __forceinline__ Kv4Row kv4_row(int page, int o, int bs, int g, int G,
 }
 inline bool kv4_pages_fit(int bs, int heads, int D) { return (int64_t)bs * heads * kv4_groups(D) * 20 <= 0x7fffffff; }
 
+// an entry of a block table; a negative one is no page: the first page's memory is read in its place, and the error flag says so
+__device__ __forceinline__ int kv4_page_read(int page, int* err) {
+    if (page < 0) atomicOr(err, 1);
+    return max(page, 0);
+}
+
 // A group of 32 values, eight in each of four neighbouring lanes (`n` of the lane's eight are values of the row, the rest do not exist).  Returns the lane's eight
 // codes, the first in the lowest bits, and, the same in all four lanes, the (s, m) pair.  Every lane of the warp takes part.
 __device__ __forceinline__ uint32_t kv4_quantise(float (&x)[8], int n, uint32_t& param, bool& odd) {

@@ -499,7 +499,8 @@ int b200seq_parallel_close(const b200seq_parallel_desc* d, void* stream);
  * rows' codes (16 NG bytes each), then its rows' (s, m) pairs (4 NG bytes each).  A key row's codes are 32-bit words [part c < 4][group] of the eight values
  * 32 group + 8 c + i, a value row's 16-bit words [part r < 8][group] of the four values 32 group + 4 r + i, the first value in the lowest bits; places behind D are 0.
  * store: k [T, G * D], v [T, Gv * V] (f32 or bf16, row strides ldk, ldv) go to the pages of the step's tokens.
- * load:  the same rows back in f32, as what they stand for (rows behind another owner's page or of no page are left as they are).
+ * load:  the same rows back in f32, as what they stand for.  A position behind its block table, or whose entry there is negative, raises bit 0 of the error flags: nothing is
+ * stored or loaded for it, and attention leaves its rows as they are or (negative entries among the keys) reads the first page in its place.
  * attn_prep_kv4 is b200seq_attn_prep_ex, attn_kv4 is b200seq_attn_ex, over such pools (no pooled blocks, no latents; D, V <= 128): q and sums in 32 bits, the cache's
  * values as they are held.  A query that is not finite gives a row of NaN.  scratch: f32 work area of b200seq_attn_kv4_scratch_floats(...) floats (0 for most steps) or
  * null: with it, few sequences of many keys use the whole GPU.  max_keys: as many keys as the step's longest sequence has, or 0 for what the block tables hold; the work is shared

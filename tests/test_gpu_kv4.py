@@ -442,3 +442,24 @@ def test_results_for_any_number_of_keys_named(ops, entries, D, keys):
     for o in outs[1:]:
         assert (o - outs[0]).abs().max().item() <= 4e-6 * outs[0].abs().max().item()
     assert ops.error_flags() == 0
+
+
+@pytest.mark.parametrize("bs", [16, 5])
+@pytest.mark.parametrize("n", [1, 70])
+def test_tables_with_negative_pages(ops, n, bs):
+    """no page is written, nothing outside the pools is read, and the error flag says so"""
+    st, keep, slots, pages = step(ops, [(n, 300)], bs, np.random.default_rng(n))
+    keep["block_table"][:] = -1
+    kp, vp = ops.kv4_pool(pages, bs, 2, 64, DEV), ops.kv4_pool(pages, bs, 2, 64, DEV)
+    x = torch.randn(n, 128, device=DEV)
+    ops.kv4_store(x, x, st, kp, vp)
+    assert ops.error_flags() == 1
+    out = torch.full((n, 128), 9.0, device=DEV)
+    ops.kv4_load(kp, vp, st, out, out.clone())
+    assert ops.error_flags() == 1 and bool((out == 9).all())
+    d = ops.attn_desc(8, 2, 64, 64, 0.125, gated=False)
+    rows = torch.randn(n, d.width, device=DEV)
+    ops.attn_prep_kv4(rows, st, d, kp, vp)
+    assert ops.error_flags() == 1 and not bool(kp.any()) and not bool(vp.any())
+    ops.attn_kv4(rows, st, d, kp, vp, torch.empty(n, 512, device=DEV))
+    assert ops.error_flags() == 1
