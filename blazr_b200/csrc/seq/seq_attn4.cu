@@ -56,18 +56,14 @@ __device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t
     hi = *reinterpret_cast<const uint32_t*>(&h), lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 __device__ __forceinline__ float par_s(uint32_t p) { return __low2float(*reinterpret_cast<const __half2*>(&p)); }
-// Two codes (fields at bits 0 and 16, high: at 4 and 20), their steps s and s72 = -72 s -> s (u - 8), exactly.  A high field in the mantissa of 64 is 64 + u: one
-// multiply-add, since -72 s is an f16 number too (7 + 4 bits).  A low one makes 1024 + u, whose -1032 s is none: the offset goes first.
-__device__ __forceinline__ uint32_t centred(uint32_t x, uint32_t s_, uint32_t s72, uint32_t magic, bool high) {
+// Two codes (fields at bits 0 and 16, high: at 4 and 20) and their steps s -> s (u - 8), exactly.  A field in the mantissa of 1024 (a high one: of 64) is that number plus u; 8 and
+// the number go first, which is exact, then comes the step.  (One multiply-add with -72 s would do for a high field, were that an f16 number: from s = 912 on it is not.)
+__device__ __forceinline__ uint32_t centred(uint32_t x, uint32_t s_, uint32_t magic, bool high) {
     uint32_t w;
     if (high) asm("lop3.b32 %0, %1, 0x00F000F0, %2, 0xEA;" : "=r"(w) : "r"(x), "r"(magic));      // (x & mask) | magic
     else asm("lop3.b32 %0, %1, 0x000F000F, %2, 0xEA;" : "=r"(w) : "r"(x), "r"(magic));
-    const __half2 h = *reinterpret_cast<const __half2*>(&w), s = *reinterpret_cast<const __half2*>(&s_);
-    const __half2 d = high ? __hfma2(h, s, *reinterpret_cast<const __half2*>(&s72)) : __hmul2_rn(__hadd2_rn(h, __floats2half2_rn(-1032.f, -1032.f)), s);
-    return *reinterpret_cast<const uint32_t*>(&d);
-}
-__device__ __forceinline__ uint32_t times72(uint32_t s_) {
-    const __half2 d = __hmul2_rn(*reinterpret_cast<const __half2*>(&s_), __floats2half2_rn(-72.f, -72.f));
+    const __half2 off = high ? __floats2half2_rn(-72.f, -72.f) : __floats2half2_rn(-1032.f, -1032.f);
+    const __half2 d = __hmul2_rn(__hadd2_rn(*reinterpret_cast<const __half2*>(&w), off), *reinterpret_cast<const __half2*>(&s_));
     return *reinterpret_cast<const uint32_t*>(&d);
 }
 
@@ -486,18 +482,18 @@ __global__ void __launch_bounds__(WARPS * 32, resident(WARPS)) attn4_kernel(cons
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             const int sel = (k & 1) ? 0x7632 : 0x5410;
-            uint32_t x[2][2], s72[2][2];
+            uint32_t x[2][2];
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int n = 0; n < 2; ++n) x[s][n] = __byte_perm(vw[s][2 * n][k >> 1], vw[s][2 * n + 1][k >> 1], sel), s72[s][n] = times72(sp[s][n][k]);
+                for (int n = 0; n < 2; ++n) x[s][n] = __byte_perm(vw[s][2 * n][k >> 1], vw[s][2 * n + 1][k >> 1], sel);
 #pragma unroll
             for (int i4 = 0; i4 < 4; ++i4) {
                 uint32_t b[2][2];
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) b[s][n] = centred(i4 < 2 ? x[s][n] : x[s][n] >> 8, sp[s][n][k], s72[s][n], (i4 & 1) ? magic64 : magic1024, i4 & 1);
+                    for (int n = 0; n < 2; ++n) b[s][n] = centred(i4 < 2 ? x[s][n] : x[s][n] >> 8, sp[s][n][k], (i4 & 1) ? magic64 : magic1024, i4 & 1);
                 float acc[4];
                 mma16816(acc, pa[0], b[0][0], b[0][1], none);
                 mma16816(acc, pa[1], b[1][0], b[1][1], acc);

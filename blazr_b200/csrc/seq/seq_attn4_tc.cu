@@ -48,15 +48,15 @@ __device__ __forceinline__ uint32_t field_or(uint32_t x, uint32_t mask, uint32_t
     asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(w) : "r"(x), "r"(mask), "r"(magic));
     return w;
 }
-// a word's eight codes as eight f16 s (u - 8): pairs of fields (i, i + 4), i = 0 .. 3.  s: the steps of the word's low and high half.  A field in the mantissa of 64 takes
-// one multiply-add (-72 s is an f16 number), one in that of 1024 an add first.
-__device__ __forceinline__ void expand(uint32_t w, __half2 s, __half2 s72, uint32_t (&x)[4]) {
-    const __half2 off = __floats2half2_rn(-1032.f, -1032.f);
+// a word's eight codes as eight f16 s (u - 8): pairs of fields (i, i + 4), i = 0 .. 3.  s: the steps of the word's low and high half.  A field in the mantissa of 1024 or of
+// 64 is that number plus u; 8 and the number go first, exactly, then comes the step (72 s is no f16 number where s is large: no multiply-add).
+__device__ __forceinline__ void expand(uint32_t w, __half2 s, uint32_t (&x)[4]) {
+    const __half2 off = __floats2half2_rn(-1032.f, -1032.f), off64 = __floats2half2_rn(-72.f, -72.f);
     const uint32_t w8 = w >> 8;
     x[0] = h2(__hmul2_rn(__hadd2_rn(h2(field_or(w, 0x000F000Fu, 0x64006400u)), off), s));
-    x[1] = h2(__hfma2(h2(field_or(w, 0x00F000F0u, 0x54005400u)), s, s72));
+    x[1] = h2(__hmul2_rn(__hadd2_rn(h2(field_or(w, 0x00F000F0u, 0x54005400u)), off64), s));
     x[2] = h2(__hmul2_rn(__hadd2_rn(h2(field_or(w8, 0x000F000Fu, 0x64006400u)), off), s));
-    x[3] = h2(__hfma2(h2(field_or(w8, 0x00F000F0u, 0x54005400u)), s, s72));
+    x[3] = h2(__hmul2_rn(__hadd2_rn(h2(field_or(w8, 0x00F000F0u, 0x54005400u)), off64), s));
 }
 // m + 8 s of two groups, as high and low f16 parts (the low one is what rounding the high one leaves: an f16 number)
 __device__ __forceinline__ void centres(__half2 s, __half2 m, uint32_t& high, uint32_t& low) {
@@ -117,7 +117,7 @@ __device__ __forceinline__ void put_codes(const Codes<N>& c, uint32_t even, uint
             const int gp = N == 4 ? i & 1 : 0, r = N == 4 ? i >> 1 : i;
             s = __lows2half2(h2(c.p[2 * gp]), h2(c.p[(2 * gp + 1) % N])), to = (r ? odd : even) + gp * PLANE;
         }
-        expand(c.w[i], s, __hmul2_rn(s, __floats2half2_rn(-72.f, -72.f)), x);
+        expand(c.w[i], s, x);
         sts16(to, x[0], x[1], x[2], x[3]);
     }
 }
