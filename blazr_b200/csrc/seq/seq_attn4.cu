@@ -11,7 +11,7 @@
 //           afterwards in f32, m as one more product (the (s, m) pairs are B as they lie).
 //   values  [16 x 8 columns]: the weights are A, again in two f16 parts, from the scores' own registers.  B is s (u - 8), which is an f16 number; the columns of one more
 //           product are m + 8 s in two f16 parts.  (Centred, because sums of s u and of m are ten times the result: 500 keys, error 1.2e-6 with m and s summed apart.)
-// So nothing is rounded but q and the weights to 22 bits; the rest is f32.  The tensor core cuts its f32 sums off instead of rounding them, 2^-21 of a sum a product, always
+// So nothing is rounded but q and the weights, to 22 bits or 2^-38 of the row's largest weight, whichever is more; the rest is f32.  The tensor core cuts its f32 sums off instead of rounding them, 2^-21 of a sum a product, always
 // downwards: value products are summed over 32 keys there and by rounded adds from then on (531 tokens, 2048 keys: error 1.3e-5 in one chain over all keys).
 //
 // What bounds it is instructions, not bytes: about 900 a tile of 32 keys and warp, two a cycle and SM (32 sequences of 2000 to 4000 keys, 32 query heads of 8 key heads of 128:
@@ -32,7 +32,9 @@ constexpr int STAGES = 2;
 // CTAs on every SM: two of 8 warps with 128 registers, or three of 4 with 168 (the plan says which)
 __host__ __device__ constexpr int resident(int warps) { return warps == 8 ? 2 : 3; }
 __host__ __device__ constexpr int ctas_of(int warps) { return 148 * resident(warps); }
-constexpr float SLACK = 8.f;  // a maximum is raised when a score passes it by this much (weights up to 2^8, where f16 parts are as good)
+constexpr float SLACK = 2.f;  // a maximum is raised when a score passes it by this much (base 2: weights up to 2^2)
+// Weights become f16 parts times this: up to 2^15, and off by 2^-38 of the row's largest at most however small they are (f16 numbers end at 2^-24)
+constexpr float WEIGHT_UP = 0x1p13f, WEIGHT_DOWN = 0x1p-13f;
 constexpr float LOG2E = 1.4426950408889634f;
 
 // d = a b + c (c may be d)
@@ -439,6 +441,8 @@ __global__ void __launch_bounds__(WARPS * 32, resident(WARPS)) attn4_kernel(cons
         for (int j = 0; j < 8; ++j) z[j] = tcsplit::ex2(fmaf(z[j], zs, off));
         l += ((z[0] + z[1]) + (z[2] + z[3])) + ((z[4] + z[5]) + (z[6] + z[7]));
 #pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] *= WEIGHT_UP;
+#pragma unroll
         for (int s = 0; s < 2; ++s) split16(z[4 * s], z[4 * s + 1], pa[s].x, pa[s].y), split16(z[4 * s + 2], z[4 * s + 3], pa[s].z, pa[s].w);
         // ---- values ----
         uint32_t vw[2][4][(NV + 1) / 2], sp[2][2][NV], bp[2][2];
@@ -520,7 +524,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident(WARPS)) attn4_kernel(cons
         for (int i4 = 0; i4 < 4; ++i4) {
             float x, y;
             tcsplit::upk(o[4 * k + i4], x, y);
-            mine[4 + 32 * k + 8 * c + i4] = x + add, mine[4 + 32 * k + 8 * c + 4 + i4] = y + add;
+            mine[4 + 32 * k + 8 * c + i4] = (x + add) * WEIGHT_DOWN, mine[4 + 32 * k + 8 * c + 4 + i4] = (y + add) * WEIGHT_DOWN;
         }
     }
     __syncthreads();

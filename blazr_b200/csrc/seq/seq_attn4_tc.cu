@@ -2,8 +2,9 @@
 //
 // What the cache holds enters the products as it is: s (u - 8) is an f16 number (seq_kv4.cuh), and the m + 8 s of a row's groups are eight more values of it, as high and low
 // f16 parts, against the group sums of q (keys), or as columns of their own (values).  Only q and the weights are rounded: to two f16 parts (22 bits) each where results are
-// f32; to one (2^-12 of a value) where they are bf16, which is an eighth of what such a result itself and the bf16 activations behind q are rounded by.  So scores and sums
-// of values are one or two products each where f32 operands (seq_attn_tc.cu) take six.
+// f32; to one (11 bits, off by up to 2^-11 of a value) where they are bf16, which is an eighth of what such a result itself and the bf16 activations behind q are rounded by;
+// weights far below the row's largest keep as much of it as the kernel says.  So scores and sums of values are one or two products each where f32 operands (seq_attn_tc.cu)
+// take six.
 //
 // One CTA works on rows of 128 (token, query head) pairs of one key head against tiles of 64 keys.  A soft-max warp's thread owns a row; two groups of four such warps alternate,
 // one in the soft-max while the other's products are in the tensor pipe:
@@ -11,7 +12,7 @@
 //   MT = 1, TG    one row tile, the groups take turns with the key tiles and are merged at the end
 //   MT = 1        one group, whose consecutive key tiles alternate (heads above 64 with f32 results: no registers for two)
 // The values of 64 keys leave the tensor core and are summed over the key tiles by rounded adds in registers; heads above 64 with bf16 results stay there (TA: the
-// sums' truncation, 2^-24 of them a product, is nothing to such a result) and are rescaled when a row's maximum has grown by 2^8.
+// sums' truncation, 2^-24 of them a product, is nothing to such a result) and are rescaled when a row's maximum has grown by 2^5.
 //   first 4 or 8 warps     soft-max: a row's maximum, sum and value sums stay in its thread's registers, nothing is shuffled
 //   next 8 warps           loaders, four for keys and four for values: codes and parameters from the pages, a tile ahead, expanded into 128-byte swizzled rows.  Both lie
 //                          alike, [key][value]: K-major for the scores, mn-major for the sums
@@ -36,7 +37,7 @@ constexpr int KT = 64;                       // keys per tile
 constexpr int PLANE = KT * 128;              // bytes of one 64-key x 64-wide block
 constexpr int SLOT_COLS = 64;                // scores f32 [64], then the weights' parts [32] [32] in the same columns
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float SLACK = 8.f;
+constexpr float SLACK = 5.f;                  // TA: a row's reference is raised when a score passes it by this much (base 2: weights up to 2^5)
 
 __host__ __device__ constexpr int blocks_of(int groups) { return (4 * groups + 9) / 8; }   // 16-byte pieces of a row: 4 a group, m + 8 s, zeros
 __host__ __device__ constexpr int columns_of(int groups) { return 32 * groups + 16; }
@@ -222,6 +223,10 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
     __shared__ float row_factor[TG ? 128 : 1];
     static_assert(!(TG && MT == 2) && (NV < 4 || (MT == 1 && (!TG || NP == 1))), "");
     constexpr bool TA = TG && NV == 4;                 // value sums stay in TMEM
+    // Weights become f16 parts times a power of two: up to 2^15, so that they are off by 2^-40 (TA: 2^-35) of the row's largest at most however small they are (f16 numbers end
+    // at 2^-24).  One part: the exponent takes the power in, which rounds it at up to 2^4 (2^-21).  Two: that would show (f32 results, 600 tokens of heads of 64: rms error
+    // 4.3e-8, multiplied 3.1e-8; 26.2 us, 27.0).  TA, slack 2 instead of 5: references are raised, and sums in TMEM rescaled, too often (2048 tokens 88 us, 79).
+    constexpr float SHIFT = TA ? 10.f : 15.f, UP = TA ? 0x1p10f : 0x1p15f, DOWN = 1.f / UP;
     constexpr int GROUPS = TG ? 2 : MT, SW = 4 * GROUPS;   // soft-max warps
     constexpr int KBYTES = blocks_of(NK) * PLANE, VBYTES = blocks_of(NV) * PLANE, STAGE = KBYTES + VBYTES, VM = 32 * NV, OCOLS = columns_of(NV), QP = columns_of(NK) / 2;
     constexpr int PITCH = 32 * (NK > NV ? NK : NV) + 4, RL = 8 * NK;   // floats of a staged row (16-byte pieces of a warp's rows in different banks); lanes a row of q takes
@@ -440,7 +445,7 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
                 corr = mx == -INFINITY ? 1.f : ex2(mb - mbn);   // 0 at the first visible key
                 mb = mbn;
             }
-            const float off = mx == -INFINITY ? 0.f : -mb;
+            const float off = mx == -INFINITY ? 0.f : (NP == 1 ? SHIFT - mb : -mb);
             const uint64_t off2 = pk(off, off);
             uint64_t sum = 0;
 #pragma unroll
@@ -452,6 +457,7 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
                     upk(fma2(pk(v[16 * q4 + i], v[16 * q4 + i + 1]), cc, off2), x, y);
                     x = ex2(x), y = ex2(y);
                     sum = add2(sum, pk(x, y));
+                    if (NP == 2) upk(mul2(pk(x, y), pk(UP, UP)), x, y);
                     const __half2 h = __floats2half2_rn(x, y);
                     ph[i >> 1] = h2(h);
                     if (NP == 2) {
@@ -498,6 +504,7 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
             // two groups: this key tile's, while the next scores are made (the other group keeps the tensor pipe busy)
             if (GROUPS == 2 && !TA && !add_values(step)) break;
         }
+        if (NP == 1) l *= DOWN;                    // (the values' sums are taken down as results are made)
         if (GROUPS == 1 && ok && ntile > 0) add_values(ntile - 1);
         const int mine = TG ? (ntile - m + 1) / 2 : ntile;    // key tiles of this group
         if (TA && ok && mine > 0) {
@@ -563,7 +570,7 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
         }
         if (ok) {   // (all lanes: TMEM is read by whole warps)
             const int t = t0 + tq, h = h0 + hr;
-            float f = 1.f;
+            float f = DOWN;
             if (live && a.parts == 1) {
                 float gate = 1.f, den = l, resc = 1.f;
                 if (a.gated && !a.gate_elem) gate = sigmoidf_acc(a.gate[(int64_t)t * a.gld + h]);
@@ -572,7 +579,7 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
                     resc = ex2(mb - top);
                     den = fmaf(l, resc, ex2(sk - top));
                 }
-                f = gate * resc / den;
+                f = gate * resc / den * DOWN;
             } else if (live && (!TG || m == 0)) {
                 float* pp = a.part + (((int64_t)t * H + h) * a.parts + split) * (V + 4);
                 pp[0] = mb, pp[1] = l;

@@ -1,9 +1,11 @@
-"""Attention over 4-bit pages (csrc/seq/seq_attn4.cu, seq_attn4_tc.cu) at the ends of its range: groups as wide as the cache holds, keys far from zero.
+"""Attention over 4-bit pages (csrc/seq/seq_attn4.cu, seq_attn4_tc.cu) at the ends of its range: groups as wide as the cache holds, rows that one key dominates.
 
 Errors are bounded element by element.  With M_j the largest value that the group of value j can stand for (|m| + 15 s, larger than any of its parts) and w the soft-max weights
 in 64 bits, roundings that are relative to a weight or to a sum's terms move a result by at most their size times sum w M.  f32 results: as in test_gpu_kv4.py, 4e-6 for weights,
 powers and sums; scores: q is off by 2^-22 of a value, the products and sums of a score by 2^-22 of its terms, together 2^-21 of A = scale sum |q| (|m| + 15 s), which a weight and
-the weights' sum each take in: 2^-20 A.  bf16 results: half a step is 2^-8 of a value, and q and the weights may be f16 numbers (2^-11 of a value each): 2^-7 and 2^-10 A."""
+the weights' sum each take in: 2^-20 A.  bf16 results: half a step is 2^-8 of a value, and q and the weights may be f16 numbers (2^-11 of a value each): 2^-7 and 2^-10 A.
+Weights are f16 parts of the weight times 2^13 or more (bf16 results: 2^10 or more), whose spacing ends at 2^-24, half of which is 2^-25: each is off by up to 2^-38 (2^-35) of
+the largest weight however small it is, together that much of sum M."""
 import numpy as np
 import pytest
 import torch
@@ -49,7 +51,7 @@ def check(ops, entries, q, k, v, scale, odt, bs=16, sink=None, softcap=0.0):
     ops.attn_kv4(torch.from_numpy(q.reshape(st.T, H * D)).to(DEV), st, d, kp, vp, out)
     assert ops.error_flags() == 0
     out = out.double().cpu().numpy().reshape(st.T, H, V)
-    tol, part, r0 = (4e-6, 2.0 ** -20, 0) if odt == F32 else (2.0 ** -7, 2.0 ** -10, 0)
+    tol, part, least, r0 = (4e-6, 2.0 ** -20, 2.0 ** -38, 0) if odt == F32 else (2.0 ** -7, 2.0 ** -10, 2.0 ** -35, 0)
     for e, (n, past) in enumerate(entries):
         pos, qe = np.arange(past, past + n), q[r0:r0 + n]
         M, K = largest(v[e]), largest(k[e])
@@ -57,7 +59,9 @@ def check(ops, entries, q, k, v, scale, odt, bs=16, sink=None, softcap=0.0):
         want, near = both[..., :V], both[..., V:]
         top = np.maximum.accumulate(K, 0)[pos]                         # [n, G, D]: more than any key that a row sees
         A = np.stack([(np.abs(qe[:, h]) * top[:, h // (H // G)]).sum(1) for h in range(H)], 1) * abs(scale)
-        err, bound = np.abs(out[r0:r0 + n] - want), near * (tol + part * A[..., None])
+        far = np.cumsum(M, 0)[pos]
+        far = np.stack([far[:, h // (H // G)] for h in range(H)], 1) * least
+        err, bound = np.abs(out[r0:r0 + n] - want), near * (tol + part * A[..., None]) + far
         assert np.isfinite(out[r0:r0 + n]).all()
         assert (err <= bound).all(), (e, float((err / bound).max()), np.argwhere(err > bound)[:4].tolist())
         r0 += n
@@ -87,6 +91,41 @@ def test_groups_as_wide_as_the_cache_holds(ops, entries, H, G, D, V, odt, span, 
             x[at, :, 0], x[at, :, 1] = -span / 2, span / 2
     scale = 0.25 / D ** 0.5 / (span / 4 if which == "keys" else 1.0)
     check(ops, entries, f32(T, H, D), k, v, scale, odt)
+
+
+@pytest.mark.parametrize("entries,H,G,D", [([(1, 5000)], 8, 2, 64), ([(1, 5000)], 8, 2, 128), ([(1, 2500)] * 20, 8, 2, 64), ([(4, 3000), (1, 700)], 8, 2, 128),
+                                           ([(1, 30000)], 8, 2, 64),
+                                           ([(600, 0)], 64, 8, 64), ([(300, 200)], 32, 4, 128), ([(300, 2000)], 16, 2, 32), ([(250, 1500)], 32, 4, 64), ([(150, 2500)], 32, 4, 128)])
+@pytest.mark.parametrize("odt", [F32, BF16])
+@pytest.mark.parametrize("gap", [12.0, 15.0, 18.0])
+@pytest.mark.parametrize("first", [True, False])
+def test_rows_that_one_key_dominates(ops, entries, H, G, D, odt, gap, first):
+    """a key `gap` nats above the others, with a value of zeros: the rows are what the others leave"""
+    rng = np.random.default_rng(int(gap) + D)
+    f32 = lambda *s: rng.standard_normal(s).astype(np.float32)
+    T = sum(n for n, _ in entries)
+    e = np.ones(D, np.float32)
+    q = (e + 0.1 * f32(T, H, D)).astype(np.float32)
+    k, v = [0.3 * f32(n + p, G, D) for n, p in entries], [1 + 0.3 * f32(n + p, G, D) for n, p in entries]
+    for (n, p), x, y in zip(entries, k, v):
+        at = 0 if first else p // 2
+        x[at], y[at] = gap, 0.0
+    check(ops, entries, q, k, v, 1.0 / D, odt)
+
+
+@pytest.mark.parametrize("entries,H,G,D", [([(1, 2000)], 8, 2, 128), ([(5, 900)], 8, 2, 64), ([(600, 0)], 64, 8, 64), ([(250, 1500)], 32, 4, 64), ([(150, 2500)], 32, 4, 128)])
+@pytest.mark.parametrize("odt", [F32, BF16])
+def test_dominated_rows_with_sinks_and_caps(ops, entries, H, G, D, odt):
+    rng = np.random.default_rng(D)
+    f32 = lambda *s: rng.standard_normal(s).astype(np.float32)
+    T = sum(n for n, _ in entries)
+    q = (1 + 0.1 * f32(T, H, D)).astype(np.float32)
+    k, v = [0.3 * f32(n + p, G, D) for n, p in entries], [f32(n + p, G, D) for n, p in entries]
+    check(ops, entries, q, k, v, 1.0 / D, odt, sink=np.linspace(-20, 20, H).astype(np.float32))
+    for x, y in zip(k, v):
+        x[3], y[3] = 14.0, 0.0
+    check(ops, entries, q, k, v, 1.0 / D, odt, sink=np.linspace(-20, 20, H).astype(np.float32))
+    check(ops, entries, q, k, v, 1.0 / D, odt, softcap=30.0)
 
 
 @pytest.mark.parametrize("entries,H,G,D", [([(1, 400), (50, 30)], 8, 2, 64), ([(300, 200)], 32, 4, 128), ([(600, 0)], 64, 8, 64), ([(300, 2000)], 16, 2, 32)])
