@@ -439,7 +439,7 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
             for (int i = 4; i < KT; i += 4) m0 = fmaxf(m0, fmaxf(v[i], v[i + 1])), m1 = fmaxf(m1, fmaxf(v[i + 2], v[i + 3]));
             const float tmax = fmaxf(m0, m1);
             float corr = 1.f;
-            if (!TA || (tmax * c > mb + SLACK)) {      // (TA: a row's reference stays until a score passes it by 2^8)
+            if (!TA || (tmax * c > mb + SLACK)) {      // (TA: a row's reference stays until a score passes it by SLACK)
                 mx = fmaxf(mx, tmax);
                 const float mbn = mx * c;
                 corr = mx == -INFINITY ? 1.f : ex2(mb - mbn);   // 0 at the first visible key

@@ -82,24 +82,33 @@ class Engine:
     # ---- the one place that runs the model -----------------------------------------------------------------------------------
     def _forward(self, batch: Sequence[Tuple[str, Sequence[int], Sequence[int]]], sample: bool = False) -> torch.Tensor:
         """batch: (request id, next tokens, wanted places) per entry.  Admits unseen ids, reserves pages, runs the step, advances
-        the token counts.  Returns the f32 logits [wanted, vocab] (device; valid until the next step)."""
+        the token counts.  Returns the f32 logits [wanted, vocab] (device; valid until the next step).  Where it raises, the ids that it admitted are none again."""
         entries: List[StepEntry] = []
         copies: List[Tuple[int, int]] = []
+        admitted: List[str] = []
         seen = set()
         for rid, _, _ in batch:
             if rid in seen:
                 raise ValueError(f"request {rid} appears twice in one step")
             seen.add(rid)
         try:
-            for rid, toks, want in batch:
-                seq = self.cache.live.get(rid) or self.cache.admit(rid)
-                copies += self.cache.reserve(seq, len(toks))
-                entries.append(StepEntry(tokens=toks, pos0=seq.n_tokens, slot=seq.slot, block_table=seq.blocks, want=want, prev=seq.last_token))
-        finally:
-            if copies:      # also when the pages ran out on the way: these requests hold their copies already
-                self.model.copy_pages(copies)
-        sa = build_step(entries, self.cache.block_size)
-        logits = self.model.forward(sa, sample=sample)
+            try:
+                for rid, toks, want in batch:
+                    seq = self.cache.live.get(rid)
+                    if seq is None:
+                        seq = self.cache.admit(rid)
+                        admitted.append(rid)
+                    copies += self.cache.reserve(seq, len(toks))
+                    entries.append(StepEntry(tokens=toks, pos0=seq.n_tokens, slot=seq.slot, block_table=seq.blocks, want=want, prev=seq.last_token))
+            finally:
+                if copies:      # also when the pages ran out on the way: these requests hold their copies already
+                    self.model.copy_pages(copies)
+            sa = build_step(entries, self.cache.block_size)
+            logits = self.model.forward(sa, sample=sample)
+        except BaseException:
+            for rid in admitted:
+                self.cache.release(rid)
+            raise
         for rid, toks, _ in batch:
             self.cache.live[rid].n_tokens += len(toks)
             self.cache.live[rid].last_token = int(toks[-1])
@@ -258,13 +267,13 @@ class Engine:
             if self.has_work():
                 raise CacheFull("no request can make progress: the KV pool is too small for the live requests")
             return []
-        for r, _, _ in plan:
-            if r in self.waiting:
-                self.waiting.remove(r)
-                self.running.append(r)
         masks = {r.rid: self._mask(r) for r, _, w in plan if w and r.params.mask_fn is not None}
         greedy = all(r.params.temperature <= 0 and not r.params.ruled() and r.params.n == 1 for r, _, w in plan if w)
         logits = self._forward([(r.rid, toks, want) for r, toks, want in plan], sample=greedy)
+        for r, _, _ in plan:        # (requests run from here on: a mask that was refused, or a pass that failed, leaves them waiting)
+            if r in self.waiting:
+                self.waiting.remove(r)
+                self.running.append(r)
         sampled = [r for r, _, w in plan if w]
         ids = self.model.last_ids.cpu().tolist() if (greedy and sampled) else None
         for r, toks, _ in plan:

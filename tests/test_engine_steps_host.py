@@ -1,0 +1,79 @@
+"""Steps of the serving engine that fail, ids and slots that are spoken for, rules that are no numbers, without a GPU: what is refused leaves the engine able to go on."""
+import numpy as np
+import pytest
+import torch
+
+from blazr_b200.cache import CacheFull
+from blazr_b200.engine import Engine, SamplingParams
+from test_fork_host import VOCAB, PagedModel, alone, fake_rules
+
+PROMPT = [3, 1, 4, 1, 5]
+
+
+def engine(max_seqs=3, **kw):
+    return Engine(PagedModel(), max_tokens=400, max_seqs=max_seqs, **{"block_size": 16, **kw})
+
+
+def finish(eng):
+    while eng.has_work():
+        eng.step()
+    assert eng.cache.slots.free_slots == eng.cache.slots.n and eng.cache.pages.free_blocks == eng.cache.pages.num_blocks
+
+
+# ---- steps that fail -------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("n", [1, 2, 3])
+def test_a_refused_mask_leaves_the_request_waiting(monkeypatch, n):
+    """also one whose samples take every slot"""
+    fake_rules(monkeypatch)
+    eng = engine()
+    words = [[0, 0]]
+    r = eng.add_request("x", PROMPT, SamplingParams(max_new_tokens=4, n=n, mask_fn=lambda out: words[0]))
+    for _ in range(2):
+        with pytest.raises(ValueError):
+            eng.step()
+    assert list(eng.waiting) == [r] and not eng.running and not eng.cache.live
+    words[0] = None
+    finish(eng)
+    assert [q.output for q in [r] + r.siblings] == [alone(PROMPT, 4)] * n
+
+
+@pytest.mark.parametrize("n", [1, 3])
+@pytest.mark.parametrize("bad", [RuntimeError, CacheFull])
+def test_a_forward_pass_that_fails_once(monkeypatch, n, bad):
+    fake_rules(monkeypatch)
+    eng = engine()
+    m, fails = eng.model, [1]
+    fwd = m.forward
+
+    def forward(sa, sample=False):
+        if fails[0]:
+            fails[0] -= 1
+            raise bad("once")
+        return fwd(sa, sample)
+    m.forward = forward
+    r = eng.add_request("x", PROMPT, SamplingParams(max_new_tokens=4, n=n))
+    with pytest.raises(bad):
+        eng.step()
+    assert not eng.cache.live and list(eng.waiting) == [r] and eng.cache.slots.free_slots == 3
+    finish(eng)
+    assert [q.output for q in [r] + r.siblings] == [alone(PROMPT, 4)] * n
+    # the same for requests that run already: they stay where they are
+    r = eng.add_request("y", PROMPT, SamplingParams(max_new_tokens=4))
+    eng.step()
+    s = eng.add_request("z", PROMPT, SamplingParams(max_new_tokens=4, n=2))
+    fails[0] = 1
+    with pytest.raises(bad):
+        eng.step()
+    assert list(eng.cache.live) == ["y"] and eng.running == [r] and list(eng.waiting) == [s]
+    finish(eng)
+    assert [q.output for q in [r, s] + s.siblings] == [alone(PROMPT, 4)] * 3
+
+
+def test_an_external_step_that_fails_leaves_no_new_request():
+    eng = Engine(PagedModel(), max_tokens=32, max_seqs=2, block_size=16)               # 4 pages
+    eng.run_entries([{"id": "a", "tokens": list(range(20)), "want": []}])
+    with pytest.raises(CacheFull):
+        eng.run_entries([{"id": "b", "tokens": [1] * 10, "want": []}, {"id": "a", "tokens": [2] * 40, "want": []}])
+    assert list(eng.cache.live) == ["a"] and eng.cache.slots.free_slots == 1
+    out = eng.run_entries([{"id": "b", "tokens": [4, 5], "want": [1]}, {"id": "a", "tokens": [3], "want": [0]}])
+    assert out[0].argmax() == alone([4, 5], 1)[0] and out[1].argmax() == alone(list(range(20)) + [3], 1)[0]
