@@ -18,7 +18,7 @@ from __future__ import annotations
 
 from collections import deque
 from dataclasses import dataclass, field, replace
-from typing import Callable, Deque, Dict, List, Optional, Sequence, Tuple
+from typing import Callable, Deque, Dict, List, Optional, Sequence, Set, Tuple
 
 import numpy as np
 import torch
@@ -77,6 +77,7 @@ class Engine:
         self.waiting: Deque[Request] = deque()
         self.running: List[Request] = []
         self.requests: Dict[str, Request] = {}
+        self._sample_ids: Set[str] = set()       # of the samples that prompts which are not through will have
         self.steps = 0
 
     # ---- the one place that runs the model -----------------------------------------------------------------------------------
@@ -123,13 +124,13 @@ class Engine:
         """a second request that continues from where the live request `rid` is.  Of a request of the engine's own scheduler a Request (with the prompt and the
         output so far, and params or the same ones) that runs from the next step on; of an externally scheduled one None"""
         rid, new_rid = str(rid), str(new_rid)
-        if new_rid in self.requests or new_rid in self.cache.live:
+        if self._in_use(new_rid):
             raise ValueError(f"request id {new_rid} is in use")
         if rid not in self.cache.live:
             raise ValueError(f"request {rid} holds nothing in the cache")
         if self.cache.slots.free_slots <= self._promised():
             raise CacheFull(f"no state slot for request {new_rid}: {self.cache.slots.free_slots} free, {self._promised()} kept for samples of running prompts")
-        r = self.requests.get(rid)
+        r = self._scheduled(rid)
         if r is not None:
             self._check(replace(params or r.params, n=1))
         self._fork_cache(rid, new_rid)
@@ -139,6 +140,14 @@ class Engine:
         q.output, q.fed = list(r.output), r.fed
         self.running.append(q)
         return q
+
+    def _in_use(self, rid: str) -> bool:
+        return rid in self.requests or rid in self.cache.live or rid in self._sample_ids
+
+    def _scheduled(self, rid: str) -> Optional[Request]:
+        """the scheduler's request of that id; an id whose request is through may be an external one's"""
+        r = self.requests.get(rid)
+        return None if r is None or r.finished else r
 
     def _promised(self) -> int:
         """slots that running requests take when their prompt is through, for its other samples"""
@@ -152,7 +161,7 @@ class Engine:
     def truncate(self, rid: str, n_tokens: int) -> None:
         """takes back the tokens of an externally scheduled request from position n_tokens on (rejected drafts); models whose layers carry state cannot"""
         rid = str(rid)
-        if rid in self.requests:
+        if self._scheduled(rid):
             raise ValueError(f"request {rid} belongs to the scheduler")
         if rid not in self.cache.live:
             raise ValueError(f"request {rid} holds nothing in the cache")
@@ -171,10 +180,13 @@ class Engine:
 
     # ---- externally scheduled steps (trace replay) ----------------------------------------------------------------------------
     def run_entries(self, entries: Sequence[dict], end: Sequence[str] = ()) -> Optional[np.ndarray]:
-        """entries: [{"id", "tokens", "want"}]; end: requests whose pages and slot are given back after the step.
+        """entries: [{"id", "tokens", "want"}], of ids that are none of the scheduler's; end: requests whose pages and slot are given back after the step.
         Returns the logits of the wanted places as a host array, or None when nothing was wanted."""
         out = None
         entries = [e for e in entries if len(e.get("tokens", ()))]      # an entry that brings no token has nothing to run
+        for rid in (str(e["id"]) for e in entries):
+            if rid in self._sample_ids or self._scheduled(rid):
+                raise ValueError(f"request {rid} belongs to the scheduler")
         if entries:
             logits = self._forward([(str(e["id"]), list(e["tokens"]), list(e.get("want", ()))) for e in entries])
             if logits.shape[0]:
@@ -185,15 +197,18 @@ class Engine:
 
     # ---- own scheduler ---------------------------------------------------------------------------------------------------------
     def add_request(self, rid: str, prompt: Sequence[int], params: Optional[SamplingParams] = None) -> Request:
-        if rid in self.requests:
+        rid = str(rid)
+        if self._in_use(rid):
             raise ValueError(f"request id {rid} is in use")
         if not len(prompt):
             raise ValueError("empty prompt")
         params = params or SamplingParams()
         self._check(params)
-        if any(f"{rid}#{i}" in self.requests for i in range(1, params.n)):
+        samples = [f"{rid}#{i}" for i in range(1, params.n)]
+        if any(self._in_use(i) for i in samples):
             raise ValueError(f"request ids {rid}#1 and on are in use")
-        r = self._request(str(rid), [int(t) for t in prompt], params)
+        r = self._request(rid, [int(t) for t in prompt], params)
+        self._sample_ids.update(samples)
         self.waiting.append(r)
         return r
 
@@ -307,6 +322,7 @@ class Engine:
             if r.params.n > 1 and not r.output and not r.siblings:
                 for i in range(1, r.params.n):
                     rid = f"{r.rid}#{i}"
+                    self._sample_ids.discard(rid)
                     self._fork_cache(r.rid, rid)
                     q = self._request(rid, r.prompt, r.params, i)
                     q.fed = r.fed

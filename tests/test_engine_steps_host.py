@@ -77,3 +77,69 @@ def test_an_external_step_that_fails_leaves_no_new_request():
     assert list(eng.cache.live) == ["a"] and eng.cache.slots.free_slots == 1
     out = eng.run_entries([{"id": "b", "tokens": [4, 5], "want": [1]}, {"id": "a", "tokens": [3], "want": [0]}])
     assert out[0].argmax() == alone([4, 5], 1)[0] and out[1].argmax() == alone(list(range(20)) + [3], 1)[0]
+
+
+# ---- ids ---------------------------------------------------------------------------------------------------------------------------------
+def test_ids_of_samples_to_come_are_taken(monkeypatch):
+    fake_rules(monkeypatch)
+    eng = engine(4, prefill_chunk=2)
+    r = eng.add_request("a", PROMPT, SamplingParams(max_new_tokens=4, n=3))
+    taken = lambda: [eng.add_request, lambda i, p: eng.run_entries([{"id": i, "tokens": p, "want": []}])]
+    for _ in range(2):                                                 # while the prompt waits, and while it runs
+        for i in ("a#1", "a#2"):
+            for use in taken():
+                with pytest.raises(ValueError):
+                    use(i, [1, 2])
+        with pytest.raises(ValueError):
+            eng.add_request("a", [1])
+        eng.step()
+    for i in ("a#1", "a#2"):
+        with pytest.raises(ValueError):
+            eng.fork("a", i)
+    b = eng.add_request("a#3", [2, 7], SamplingParams(max_new_tokens=3))    # (nobody's)
+    finish(eng)
+    assert [q.output for q in [r] + r.siblings] == [alone(PROMPT, 4)] * 3 and [q.rid for q in r.siblings] == ["a#1", "a#2"] and b.output == alone([2, 7], 3)
+    with pytest.raises(ValueError):                                    # they are the finished samples' still
+        eng.add_request("a#1", [1])
+
+
+def test_samples_do_not_take_ids_in_use(monkeypatch):
+    """of requests that wait, of external ones, of samples to come"""
+    fake_rules(monkeypatch)
+    eng = engine(4)
+    eng.add_request("b#1", [2, 7], SamplingParams(max_new_tokens=3))
+    eng.run_entries([{"id": "c#2", "tokens": [5], "want": []}])
+    eng.add_request("d#1", [2, 7], SamplingParams(max_new_tokens=3, n=2))    # d#1#1 to come
+    for i, n in (("b", 2), ("c", 3), ("d", 2)):
+        with pytest.raises(ValueError):
+            eng.add_request(i, PROMPT, SamplingParams(n=n))
+    with pytest.raises(ValueError):
+        eng.add_request("d#1#1", PROMPT)
+    with pytest.raises(ValueError):
+        eng.add_request("c#2", PROMPT)                                 # an external request has it
+    with pytest.raises(ValueError):
+        eng.add_request(7, PROMPT, SamplingParams(n=0))
+    eng.add_request(7, PROMPT, SamplingParams(max_new_tokens=2))
+    with pytest.raises(ValueError):
+        eng.add_request("7", PROMPT)
+    eng.run_entries([], ["c#2"])
+    c = eng.add_request("c", PROMPT, SamplingParams(max_new_tokens=4, n=3))
+    finish(eng)
+    assert [q.output for q in [c] + c.siblings] == [alone(PROMPT, 4)] * 3 and eng.requests["b#1"].output == alone([2, 7], 3)
+
+
+def test_external_steps_leave_the_schedulers_requests_alone(monkeypatch):
+    fake_rules(monkeypatch)
+    eng = engine()
+    r = eng.add_request("a", PROMPT, SamplingParams(max_new_tokens=4))
+    for _ in range(2):                                                 # one that waits, one that runs
+        with pytest.raises(ValueError):
+            eng.run_entries([{"id": "e", "tokens": [1], "want": []}, {"id": "a", "tokens": [1, 2], "want": []}])
+        assert "e" not in eng.cache.live
+        eng.step()
+    finish(eng)
+    assert r.output == alone(PROMPT, 4)
+    out = eng.run_entries([{"id": "a", "tokens": [4, 5], "want": [1]}])     # its name is free for others when it is through
+    assert out[0].argmax() == alone([4, 5], 1)[0] and eng.fork("a", "b") is None
+    out = eng.run_entries([{"id": "b", "tokens": [6], "want": [0]}], ["a", "b"])
+    assert out[0].argmax() == alone([4, 5, 6], 1)[0] and not eng.has_work()
