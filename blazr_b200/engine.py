@@ -187,6 +187,9 @@ class Engine:
         for rid in (str(e["id"]) for e in entries):
             if rid in self._sample_ids or self._scheduled(rid):
                 raise ValueError(f"request {rid} belongs to the scheduler")
+        new, free = len({str(e["id"]) for e in entries} - self.cache.live.keys()), self.cache.slots.free_slots
+        if new and new > free - self._promised():
+            raise CacheFull(f"{new} state slots wanted, {free} free, {self._promised()} of them kept for samples of running prompts")
         if entries:
             logits = self._forward([(str(e["id"]), list(e["tokens"]), list(e.get("want", ()))) for e in entries])
             if logits.shape[0]:

@@ -143,3 +143,28 @@ def test_external_steps_leave_the_schedulers_requests_alone(monkeypatch):
     assert out[0].argmax() == alone([4, 5], 1)[0] and eng.fork("a", "b") is None
     out = eng.run_entries([{"id": "b", "tokens": [6], "want": [0]}], ["a", "b"])
     assert out[0].argmax() == alone([4, 5, 6], 1)[0] and not eng.has_work()
+
+
+# ---- slots ---------------------------------------------------------------------------------------------------------------------------------
+def test_external_requests_leave_the_slots_of_samples_to_come(monkeypatch):
+    fake_rules(monkeypatch)
+    eng = engine(3, prefill_chunk=2)
+    r = eng.add_request("a", PROMPT, SamplingParams(max_new_tokens=4, n=2))
+    eng.step()
+    eng.run_entries([{"id": "e", "tokens": [4], "want": []}])          # the third slot
+    with pytest.raises(CacheFull):
+        eng.run_entries([{"id": "e", "tokens": [5], "want": []}, {"id": "f", "tokens": [4], "want": []}])
+    assert sorted(eng.cache.live) == ["a", "e"] and eng.cache.live["e"].n_tokens == 1
+    out = eng.run_entries([{"id": "e", "tokens": [5], "want": [0]}], ["e"])
+    assert out[0].argmax() == alone([4, 5], 1)[0]
+    finish(eng)
+    assert [q.output for q in [r] + r.siblings] == [alone(PROMPT, 4)] * 2
+
+
+def test_as_many_external_requests_as_slots():
+    eng = engine(2)
+    eng.run_entries([{"id": "a", "tokens": [4], "want": []}, {"id": "b", "tokens": [4], "want": []}])
+    with pytest.raises(CacheFull):
+        eng.run_entries([{"id": "a", "tokens": [5], "want": []}, {"id": "c", "tokens": [4], "want": []}])
+    out = eng.run_entries([{"id": "a", "tokens": [5], "want": [0]}], ["a", "b"])
+    assert out[0].argmax() == alone([4, 5], 1)[0]
