@@ -28,6 +28,8 @@ from .batch import StepEntry, build_step
 from .cache import CacheFull, CacheManager
 from .layered import LayeredModel
 
+F32_MAX, F32_TINY = float(np.finfo(np.float32).max), float(np.finfo(np.float32).tiny)
+
 
 @dataclass
 class SamplingParams:
@@ -218,12 +220,29 @@ class Engine:
     def _check(self, p: SamplingParams) -> None:
         if not 1 <= p.n <= self.cache.slots.n:
             raise ValueError(f"{p.n} samples of a prompt, of {self.cache.slots.n} requests that may live at a time")
-        if not p.repetition_penalty > 0:
+        # (numbers as the kernels have them: of 32 bits)
+        if not F32_TINY <= p.repetition_penalty <= F32_MAX:
             raise ValueError(f"a repetition penalty of {p.repetition_penalty}")
+        if not (abs(p.presence_penalty) <= F32_MAX and abs(p.frequency_penalty) <= F32_MAX):
+            raise ValueError(f"presence and frequency penalties of {p.presence_penalty} and {p.frequency_penalty}")
+        if p.temperature != p.temperature or 0 < p.temperature < F32_TINY or (p.temperature > F32_MAX and p.ruled()):
+            raise ValueError(f"a temperature of {p.temperature}")
+        if p.temperature > 0 and not p.top_p > 0:
+            raise ValueError(f"a top_p of {p.top_p}")
         vocab = getattr(getattr(self.model, "cfg", None), "vocab", None)
         for t in p.logit_bias or ():
             if int(t) != t or t < 0 or (vocab is not None and t >= vocab):
                 raise ValueError(f"a bias on token {t} of {vocab}")
+        for t, v in (p.logit_bias or {}).items():
+            if not v <= F32_MAX:
+                raise ValueError(f"a bias of {v} on token {t}")
+        if vocab is not None and len(self._forbidden(p)) == vocab:
+            raise ValueError("biases that leave no token")
+
+    @staticmethod
+    def _forbidden(p: SamplingParams) -> List[int]:
+        """tokens that a bias of minus infinity (in 32 bits) takes out"""
+        return [int(t) for t, v in (p.logit_bias or {}).items() if v < -F32_MAX]
 
     def _request(self, rid: str, prompt: List[int], params: SamplingParams, place: int = 0) -> Request:
         r = Request(rid, prompt, params)
@@ -279,7 +298,8 @@ class Engine:
         return plan
 
     def step(self) -> List[Request]:
-        """one forward pass over what the scheduler picked; returns the requests that finished in it"""
+        """one forward pass over what the scheduler picked; returns the requests that finished in it.  A request whose logits leave no choice (sampled, and the
+        largest over its temperature is no number) finishes without a token; when all others have theirs, RuntimeError says so"""
         plan = self._schedule()
         if not plan:
             if self.has_work():
@@ -305,7 +325,15 @@ class Engine:
             rows = list(range(len(sampled)))
         if ids is None and any(r.params.ruled() for r in sampled):
             logits = self._apply_rules(logits[:len(sampled)], sampled, masks)
+        # largest logits of rows that are sampled: where one is no number there is nothing to choose by (and a multinomial of it would end the process)
+        tops = logits[:len(sampled)].max(1).values.tolist() if any(r.params.temperature > 0 for r in sampled) else None
+        lost: List[str] = []
         for row, r in zip(rows, sampled):
+            if r.params.temperature > 0 and not abs(tops[row] / r.params.temperature) <= F32_MAX:
+                lost.append(f"{r.rid} (its largest logit is {tops[row]}, its temperature {r.params.temperature})")
+                r.finished = True
+                done.append(r)
+                continue
             tok = ids[row] if ids is not None else self._sample(logits[row], r)
             r.output.append(int(tok))
             if len(r.output) >= r.params.max_new_tokens or int(tok) in r.params.stop_tokens:
@@ -314,6 +342,8 @@ class Engine:
         for r in done:
             self.running.remove(r)
             self.release(r.rid)
+        if lost:
+            raise RuntimeError("no token can be chosen for request " + ", ".join(lost))
         return done
 
     def _fan_out(self, sampled: List[Request]) -> Tuple[List[int], List[Request]]:
@@ -345,6 +375,11 @@ class Engine:
         vocab = getattr(getattr(self.model, "cfg", None), "vocab", 32 * m.size)
         if m.size != (vocab + 31) // 32:
             raise ValueError(f"the mask of request {r.rid} has {m.size} words, not {(vocab + 31) // 32}")
+        forbidden = [t for t in self._forbidden(r.params) if t < 32 * m.size]
+        if forbidden:
+            bits = np.unpackbits(m.astype("<u4").view(np.uint8), bitorder="little")
+            bits[forbidden] = 0
+            m = np.packbits(bits, bitorder="little").view("<u4").astype(np.uint32)
         last = m[-1] if vocab % 32 == 0 else m[-1] & np.uint32((1 << vocab % 32) - 1)
         if not (m[:-1].any() or last):
             raise ValueError(f"the mask of request {r.rid} leaves no token")
@@ -366,7 +401,7 @@ class Engine:
                 else:
                     prompt.append(0)
                 hist += r.output
-                bias += list((p.logit_bias or {}).items())
+                bias += [(t, v if v >= -F32_MAX else -np.inf) for t, v in (p.logit_bias or {}).items()]
                 m = masks.get(r.rid if r.rid in masks or not r.siblings else r.siblings[0].rid)      # (a sample's first token: the mask of its prompt's request)
                 if m is not None:
                     if mask is None:

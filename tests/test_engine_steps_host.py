@@ -168,3 +168,77 @@ def test_as_many_external_requests_as_slots():
         eng.run_entries([{"id": "a", "tokens": [5], "want": []}, {"id": "c", "tokens": [4], "want": []}])
     out = eng.run_entries([{"id": "a", "tokens": [5], "want": [0]}], ["a", "b"])
     assert out[0].argmax() == alone([4, 5], 1)[0]
+
+
+# ---- rules and logits that are no numbers ----------------------------------------------------------------------------------------------------
+NAN, INF = float("nan"), float("inf")
+
+
+@pytest.mark.parametrize("p", [
+    dict(presence_penalty=NAN), dict(presence_penalty=INF), dict(frequency_penalty=-INF), dict(frequency_penalty=NAN), dict(frequency_penalty=1e39), dict(presence_penalty=-1e300),
+    dict(repetition_penalty=INF), dict(repetition_penalty=1e39), dict(repetition_penalty=1e-40), dict(repetition_penalty=-1.0), dict(logit_bias={3: NAN}), dict(logit_bias={3: INF}),
+    dict(logit_bias={3: 1e39}), dict(logit_bias={i: -INF for i in range(VOCAB)}), dict(logit_bias={i: -1e39 for i in range(VOCAB)}), dict(temperature=NAN),
+    dict(temperature=INF, logit_bias={3: -INF}), dict(temperature=1e39, mask_fn=lambda out: None), dict(temperature=0.5, top_p=0.0), dict(temperature=0.5, top_p=NAN),
+    dict(temperature=0.5, top_p=-1.0), dict(temperature=1e-40)])
+def test_rules_that_are_no_numbers(p):
+    eng = engine()
+    with pytest.raises(ValueError):
+        eng.add_request("x", PROMPT, SamplingParams(**p))
+    assert not eng.requests and not eng.has_work()
+    eng.add_request("x", PROMPT)
+    eng.step()
+    with pytest.raises(ValueError):
+        eng.fork("x", "y", SamplingParams(**p))
+    assert list(eng.cache.live) == ["x"]
+
+
+def test_rules_at_the_ends_of_their_range(monkeypatch):
+    fake_rules(monkeypatch)
+    eng = engine()
+    for i, p in enumerate((dict(logit_bias={3: -INF}), dict(logit_bias={3: -1e300, 4: 3e38}), dict(presence_penalty=3e38, frequency_penalty=-3e38), dict(repetition_penalty=3e38),
+                           dict(repetition_penalty=1.2e-38), dict(top_p=0.0), dict(temperature=-1.0))):
+        eng.add_request(i, PROMPT, SamplingParams(max_new_tokens=1, **p))
+    with np.errstate(all="raise"):
+        finish(eng)
+
+
+def test_a_mask_of_forbidden_tokens(monkeypatch):
+    """allowed by the mask are only tokens whose bias forbids them"""
+    fake_rules(monkeypatch)
+    eng = engine()
+    words = [[0b11000, 0]]
+    r = eng.add_request("x", PROMPT, SamplingParams(max_new_tokens=2, logit_bias={3: -INF, 4: -1e39, 5: -2.0}, mask_fn=lambda out: words[0]))
+    with pytest.raises(ValueError):
+        eng.step()
+    assert list(eng.waiting) == [r]
+    words[0] = [0b110000, 0]
+    finish(eng)
+    assert len(r.output) == 2
+
+
+@pytest.mark.parametrize("bad", [NAN, INF, -INF, 3e38])
+def test_logits_that_leave_no_choice(monkeypatch, bad):
+    """the request ends without that token, the others go on, and nothing is sampled from probabilities that are none (3e38: not after the temperature)"""
+    fake_rules(monkeypatch)
+    monkeypatch.setattr("torch.multinomial", lambda p, n, generator=None: (_ for _ in ()).throw(AssertionError) if not bool((p >= 0).all()) or not float(p.sum()) > 0 else p.argmax(0, True))
+    eng = engine()
+    m, spoil = eng.model, [False]
+    fwd = m.forward
+
+    def forward(sa, sample=False):
+        z = fwd(sa, sample) * 100
+        if spoil[0]:
+            z[0, :] = bad if bad == -INF else z[0]
+            z[0, 7] = bad
+        return z
+    m.forward = forward
+    sampled = SamplingParams(max_new_tokens=4, temperature=0.5)
+    x, y = eng.add_request("x", PROMPT, sampled), eng.add_request("y", [2, 7], sampled)
+    eng.step()
+    spoil[0] = True
+    with pytest.raises(RuntimeError, match="x"):
+        eng.step()
+    spoil[0] = False
+    assert x.finished and len(x.output) == 1 and len(y.output) == 2 and list(eng.cache.live) == ["y"]
+    finish(eng)
+    assert y.output == alone([2, 7], 4)
