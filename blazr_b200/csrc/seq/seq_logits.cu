@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 1) process_logi
     if (odd && blockIdx.x == 0) atomicOr(a.err, ERR_TOKEN);
     __syncthreads();
     float* out = a.out + row * a.ldo + v0;
-    const float up = rule.w != 0.f && fabsf(rule.w) < 0x1p-126f ? 0x1p24f : 1.f, inv = rule.w != 0.f ? 1.0f / (rule.w * up) : 1.f;   // (up: a temperature whose reciprocal is no number)
+    const float heat = rule.w != 0.f ? rule.w : 1.f;
 #pragma unroll
     for (int k = 0; k < ITEMS; ++k) {
         const int i = 4 * (k * THREADS + threadIdx.x);
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 1024 ? 2 : 1) process_logi
             if (at.w) y[3] += a.bias_vals[b0 + (int)at.w - 1];
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = (bits[k] >> j) & 1u ? y[j] * up * inv : -INFINITY;
+        for (int j = 0; j < 4; ++j) y[j] = (bits[k] >> j) & 1u ? y[j] / heat : -INFINITY;
         if (a.vec && i + 3 < n) *reinterpret_cast<float4*>(out + i) = make_float4(y[0], y[1], y[2], y[3]);
         else
             for (int j = 0; j < 4 && i + j < n; ++j) out[i + j] = y[j];
