@@ -426,8 +426,9 @@ __global__ void __launch_bounds__(WARPS * 32, resident(WARPS)) attn4_kernel(cons
             for (int j = 0; j < 8; ++j)
                 if (!rs.sees(key0 + 2 * c + (j & 1) + 8 * (j >> 1))) z[j] = -INFINITY;
         }
-        float tm = fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7]))) * zs;
-        if (__any_sync(0xffffffffu, tm > mx + SLACK)) {   // (mx = -inf: the first keys a row sees)
+        // (rounded so that no exponent below exceeds SLACK, however large the scores: the weights' f16 parts end there)
+        float tm = __fmul_ru(fmaxf(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])), fmaxf(fmaxf(z[4], z[5]), fmaxf(z[6], z[7]))), zs);
+        if (__any_sync(0xffffffffu, tm > __fadd_rd(mx, SLACK))) {   // (mx = -inf: the first keys a row sees)
             tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 1)), tm = fmaxf(tm, __shfl_xor_sync(0xffffffffu, tm, 2));
             const float mn = fmaxf(mx, tm), corr = mx == -INFINITY ? 0.f : tcsplit::ex2(mx - mn);
             const uint64_t corr2 = tcsplit::pk(corr, corr);

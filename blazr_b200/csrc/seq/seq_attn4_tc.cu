@@ -439,13 +439,14 @@ __global__ void __launch_bounds__((4 * (TG ? 2 : MT) + 12) * 32, 1) attn4_tc_ker
             for (int i = 4; i < KT; i += 4) m0 = fmaxf(m0, fmaxf(v[i], v[i + 1])), m1 = fmaxf(m1, fmaxf(v[i + 2], v[i + 3]));
             const float tmax = fmaxf(m0, m1);
             float corr = 1.f;
-            if (!TA || (tmax * c > mb + SLACK)) {      // (TA: a row's reference stays until a score passes it by SLACK)
+            // (rounded so that no exponent below exceeds SLACK or 0, however large the scores: the weights' f16 parts end there)
+            if (!TA || __fmul_ru(tmax, c) > __fadd_rd(mb, SLACK)) {      // (TA: a row's reference stays until a score passes it by SLACK)
                 mx = fmaxf(mx, tmax);
-                const float mbn = mx * c;
+                const float mbn = __fmul_ru(mx, c);
                 corr = mx == -INFINITY ? 1.f : ex2(mb - mbn);   // 0 at the first visible key
                 mb = mbn;
             }
-            const float off = mx == -INFINITY ? 0.f : (NP == 1 ? SHIFT - mb : -mb);
+            const float off = mx == -INFINITY ? 0.f : (NP == 1 ? __fsub_rd(SHIFT, mb) : -mb);
             const uint64_t off2 = pk(off, off);
             uint64_t sum = 0;
 #pragma unroll

@@ -137,3 +137,33 @@ def test_keys_around_different_places(ops, entries, H, G, D, odt):
     T = sum(n for n, _ in entries)
     k, v = [f32(n + p, G, D) + 10 * f32(n + p, G, 1) for n, p in entries], [f32(n + p, G, D) for n, p in entries]
     check(ops, entries, f32(T, H, D), k, v, 0.02, odt)
+
+
+@pytest.mark.parametrize("entries,H,G,D", [([(1, 300)], 8, 2, 64), ([(1, 30000)], 8, 2, 64), ([(40, 30)], 8, 2, 128), ([(600, 0)], 64, 8, 64), ([(300, 200)], 32, 4, 128),
+                                           ([(250, 1500)], 32, 4, 64), ([(300, 2000)], 16, 2, 32)])
+@pytest.mark.parametrize("odt", [F32, BF16])
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 23, 1.3 * 2.0 ** 24, 1.3 * 2.0 ** 25, 2.0 ** 26])
+def test_scores_of_any_size(ops, entries, H, G, D, odt, size):
+    """one key of every row scores `size` (base 2: 1.44 times that), the others a tenth of it: the row is that key's value, to the roundings of one weight and of the result.
+    An f32 score of that size is a multiple of up to 8, and so is what the weight's exponent may be below 0: 2^-16 of the largest a weight can be has 11 bits and more in two
+    parts, 2^-24 / 2^-16 / 2^13 of them the last (f32 results: 2^-21); in one part half of 2^-10 (bf16 results, beside the half step of the result of 2^-8)."""
+    rng = np.random.default_rng(D)
+    f32 = lambda *s: rng.standard_normal(s).astype(np.float32)
+    (n, p), = entries
+    q = (1 + 0.02 * f32(n, H, D)).astype(np.float32)
+    k, v = 0.05 * f32(n + p, G, D), f32(n + p, G, D)
+    k[0], k[n // 2 + p] = 8.0, 16.0                                    # rows see the first, the later ones the second too
+    st, keep, slots, pages = base.step(ops, entries, 16, rng)
+    kp, vp = (torch.from_numpy(np.zeros((pages, G, ops.kv4_page_bytes(16, 1, D)), np.uint8)).to(DEV) for _ in range(2))
+    ent, pos = torch.zeros(n + p, dtype=torch.int32, device=DEV), torch.arange(n + p, dtype=torch.int32, device=DEV)
+    rows = ops.StepDesc(ent.data_ptr(), pos.data_ptr(), 0, 0, 0, keep["block_table"].data_ptr(), n + p, 1, st.max_blocks, 16)
+    ops.kv4_store(torch.from_numpy(k.reshape(n + p, -1)).to(DEV), torch.from_numpy(v.reshape(n + p, -1)).to(DEV), rows, kp, vp)
+    d = ops.attn_desc(H, G, D, D, size / (16 * D), gated=False, kv_shared=True)
+    out = torch.empty(n, H * D, device=DEV, dtype=odt)
+    ops.attn_kv4(torch.from_numpy(q.reshape(n, -1)).to(DEV), st, d, kp, vp, out)
+    got = out.double().cpu().numpy().reshape(n, G, H // G, D)
+    first, later = (ref.held(v[i]).astype(np.float64) for i in (0, n // 2 + p))
+    want = np.stack([later if i >= n // 2 else first for i in range(n)])[:, :, None]
+    M = np.stack([largest(v[n // 2 + p]) if i >= n // 2 else largest(v[0]) for i in range(n)])[:, :, None]
+    err = np.abs(got - want)
+    assert np.isfinite(got).all() and (err <= M * (4e-6 if odt == F32 else 2.0 ** -7)).all(), float((err / M).max())
