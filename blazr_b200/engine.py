@@ -124,7 +124,8 @@ class Engine:
 
     def fork(self, rid: str, new_rid: str, params: Optional[SamplingParams] = None) -> Optional[Request]:
         """a second request that continues from where the live request `rid` is.  Of a request of the engine's own scheduler a Request (with the prompt and the
-        output so far, and params or the same ones) that runs from the next step on; of an externally scheduled one None"""
+        output so far, and params or the same ones) that runs from the next step on; of an externally scheduled one None.  A sampled one draws from the beginning of its
+        seed's numbers, not from where `rid` is in them: params of another seed make another continuation"""
         rid, new_rid = str(rid), str(new_rid)
         if self._in_use(new_rid):
             raise ValueError(f"request id {new_rid} is in use")
@@ -229,6 +230,8 @@ class Engine:
             raise ValueError(f"a temperature of {p.temperature}")
         if p.temperature > 0 and not p.top_p > 0:
             raise ValueError(f"a top_p of {p.top_p}")
+        if p.temperature > 0 and p.top_k < 0:
+            raise ValueError(f"a top_k of {p.top_k}")
         vocab = getattr(getattr(self.model, "cfg", None), "vocab", None)
         for t in p.logit_bias or ():
             if int(t) != t or t < 0 or (vocab is not None and t >= vocab):
@@ -442,14 +445,22 @@ class Engine:
     def generate(self, prompts: Sequence[Sequence[int]], params: Optional[SamplingParams] = None) -> List[List[int]]:
         """runs the prompts to completion through the scheduler (more prompts than slots queue up); returns the new tokens of each (params.n > 1: a list of
         its n samples)"""
-        reqs = [self.add_request(f"g{self.steps}_{i}", p, params) for i, p in enumerate(prompts)]
-        while any(not q.finished for r in reqs for q in [r] + r.siblings):
-            self.step()
-        flags = seqops.error_flags()
-        if flags:
-            raise RuntimeError(f"device error flags {flags:#x} (1: KV position outside its block table, 2: a bounded wait ran out, 4: expert table entry out of range, "
-                               "8: a key or value beyond what a 4-bit cache holds, 16: a token id outside the vocabulary)")
-        for r in reqs:
-            for q in [r] + r.siblings:
-                del self.requests[q.rid]
+        reqs: List[Request] = []
+        try:
+            for i, p in enumerate(prompts):
+                reqs.append(self.add_request(f"g{self.steps}_{i}", p, params))
+            while any(not q.finished for r in reqs for q in [r] + r.siblings):
+                self.step()
+            flags = seqops.error_flags()
+            if flags:
+                raise RuntimeError(f"device error flags {flags:#x} (1: KV position outside its block table, 2: a bounded wait ran out, 4: expert table entry out of range, "
+                                   "8: a key or value beyond what a 4-bit cache holds, 16: a token id outside the vocabulary)")
+        finally:                    # also what is left of them where a step fails
+            for r in reqs:
+                self._sample_ids.difference_update(f"{r.rid}#{i}" for i in range(1, r.params.n))
+                for q in [r] + r.siblings:
+                    if not q.finished:
+                        (self.running if q in self.running else self.waiting).remove(q)
+                        self.release(q.rid)
+                    del self.requests[q.rid]
         return [[q.output for q in [r] + r.siblings] if r.params.n > 1 else r.output for r in reqs]

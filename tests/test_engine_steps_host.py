@@ -242,3 +242,24 @@ def test_logits_that_leave_no_choice(monkeypatch, bad):
     assert x.finished and len(x.output) == 1 and len(y.output) == 2 and list(eng.cache.live) == ["y"]
     finish(eng)
     assert y.output == alone([2, 7], 4)
+
+
+# ---- generate ------------------------------------------------------------------------------------------------------------------------------------
+def test_a_generate_that_fails_takes_its_requests_back(monkeypatch):
+    fake_rules(monkeypatch)
+    eng = engine()
+    other = eng.add_request("other", PROMPT, SamplingParams(max_new_tokens=6))
+    eng.step()
+    masked = SamplingParams(max_new_tokens=4, n=2, mask_fn=lambda out: [0, 0] if len(out) == 2 else None)
+    for _ in range(2):                                                 # (a refused mask in the middle of the output)
+        with pytest.raises(ValueError):
+            eng.generate([[2, 7], [3, 8]], masked)
+        assert list(eng.requests) == ["other"] and not eng.waiting and eng.running in ([other], []) and eng.cache.slots.free_slots == 3 - len(eng.running)
+    with pytest.raises(ValueError):
+        eng.generate([[2, 7], []])
+    with pytest.raises(ValueError):
+        eng.generate([[2, 7]], SamplingParams(temperature=0.5, top_k=-1))
+    assert not eng._sample_ids and list(eng.requests) == ["other"]
+    assert eng.generate([[2, 7], [3, 8]], SamplingParams(max_new_tokens=4)) == [alone([2, 7], 4), alone([3, 8], 4)]
+    finish(eng)
+    assert other.output == alone(PROMPT, 6)
