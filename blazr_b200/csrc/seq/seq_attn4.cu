@@ -11,11 +11,12 @@
 //           afterwards in f32, m as one more product (the (s, m) pairs are B as they lie).
 //   values  [16 x 8 columns]: the weights are A, again in two f16 parts, from the scores' own registers.  B is s (u - 8), which is an f16 number; the columns of one more
 //           product are m + 8 s in two f16 parts.  (Centred, because sums of s u and of m are ten times the result: 500 keys, error 1.2e-6 with m and s summed apart.)
-// So nothing is rounded but q and the weights, to 22 bits or 2^-38 of the row's largest weight, whichever is more; the rest is f32.  The tensor core cuts its f32 sums off instead of rounding them, 2^-21 of a sum a product, always
-// downwards: value products are summed over 32 keys there and by rounded adds from then on (531 tokens, 2048 keys: error 1.3e-5 in one chain over all keys).
+// So nothing is rounded but q and the weights, to 22 bits or 2^-38 of the row's largest weight, whichever is more; the rest is f32.  The tensor core cuts its f32 sums off
+// instead of rounding them, 2^-21 of a sum a product, always downwards: value products are summed over 32 keys there and by rounded adds from then on (531 tokens, 2048 keys:
+// error 1.3e-5 in one chain over all keys).
 //
-// What bounds it is instructions, not bytes: about 900 a tile of 32 keys and warp, two a cycle and SM (32 sequences of 2000 to 4000 keys, 32 query heads of 8 key heads of 128:
-// 57 us, 2.2 TB/s of the cache; one of 131072 keys: 64 us, 2.6 TB/s; bytes alone 19 and 26).  One token of 500 keys, heads of 64: 5.4 us.
+// What bounds it is instructions, not bytes: about 950 a tile of 32 keys and warp, two a cycle and SM (32 sequences of 2000 to 4000 keys, 32 query heads of 8 key heads of 128:
+// 59 us, 2.1 TB/s of the cache; one of 131072 keys: 67 us, 2.5 TB/s; bytes alone 19 and 26).  One token of 500 keys, heads of 64: 5.6 us.
 //
 // A CTA's 8 or 4 warps share the keys of a row tile.  Few keys: so do the CTAs of a cluster, merged through distributed shared memory.  Many: the keys of all row tiles are one
 // list that is dealt out evenly, and a second kernel merges the parts of row tiles that ended up in several CTAs.
@@ -723,12 +724,12 @@ template <int NK>
 cudaError_t launch_values(int nv, const Attn4Args& a, const b200seq_step& st, dim3 grid, const Plan& p, cudaStream_t cs) {
     return nv == 1 ? launch_form<NK, 1>(a, st, grid, p, cs) : (nv == 2 ? launch_form<NK, 2>(a, st, grid, p, cs) : launch_form<NK, 4>(a, st, grid, p, cs));
 }
-// Which kernel is the faster one, from the key tiles a CTA has at most.  us, fitted to 57 steps of 8 to 288 tokens, timed with each of the two (the choice is at
-// most 13 % behind the faster one).  Here (shared_us, dealt_us): a wave of CTAs takes 4 (5 with heads above 64) and 1.5 (3.6) a key tile of 32 and warp, down to 0.6 (four
+// Which kernel is the faster one, from the key tiles a CTA has at most.  us, fitted to measured steps.  146 steps of 1 to 288 tokens have been timed with each of the two (a table
+// in profiles/kv4_choice.txt): the choice is 18 % behind the faster one at most (8 x 16 tokens behind 1000, heads of 64), in 143 of them 3 % or less.  Here (shared_us, dealt_us): a wave of CTAs takes 4 (5 with heads above 64) and 1.5 (3.6) a key tile of 32 and warp, down to 0.6 (four
 // warps) or 1.3 (1.9) where a CTA has an SM to itself; keys that are dealt out 18 (15.5), and 1200 (645) key tiles a us.  On the tensor cores: 7.5 (9; f32 11) a CTA
 // and 0.8 (0.75; f32 1.4) a key tile of 64, 4 more for keys in several parts.  Measured, us, here / there, 32 query heads of 8 key heads of 64 (of 128):
-//   1 x 64 tokens                6 /  8 ( 7 / 10)     16 x 9 behind 1500   43 / 28 (66 / 31)     32 x 2 behind 2000   34 / 64 (45 / 73)
-//   1 x 32 behind 4000          22 / 22 (34 / 25)      4 x 8 behind 8000   56 / 36 (83 / 39)      4 x 64 behind 300   27 / 13 (38 / 14)
+//   1 x 64 tokens                6 /  8 ( 8 / 10)     16 x 9 behind 1500   45 / 29 (67 / 32)     32 x 2 behind 2000   34 / 65 (45 / 71)
+//   1 x 32 behind 4000          23 / 23 (35 / 25)      4 x 8 behind 8000   41 / 36 (62 / 41)      4 x 64 behind 300   28 / 13 (40 / 14)
 bool tc_is_faster(const b200seq_step& st, const b200seq_attn_desc& d, int max_keys, const Plan& p, const Attn4TcPlan& tp, bool f32) {
     const bool small = d.D <= 64 && d.V <= 64;
     const double keys = (double)most_keys(st, d, max_keys, 0), kt = (keys + KT - 1) / KT;

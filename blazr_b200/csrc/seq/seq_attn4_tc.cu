@@ -20,9 +20,9 @@
 // The order of a row's values is that of its code words (pairs of fields that one AND takes out): q is permuted alike, results are put back in order as they are stored.
 // Registers (setmaxnreg, per thread): launched with 96 (two groups) or 128 (one) for all; soft-max 160 / 240, loaders 64 / 104, issuer 32 / 64: the sums
 // (2 * 160 + 2 * 64 + 32 = 5 * 96, 240 + 2 * 104 + 64 = 4 * 128) are what the block was launched with.
-// Measured: 2048 tokens of 32 query heads of 8 key heads of 128, bf16 results: 78 us (440 TFLOP/s of what every row sees), f32 115; 531 tokens behind 5000, heads of 64, window 2048,
-// f32: 39 us.  A CTA takes about 9 us beside its key tiles (queries into the tensor core's memory, the first tile's way through all roles, results out) and 0.7 a key tile, which
-// the instructions of expanding and soft-max bound (tensor pipe active 21 %).
+// Measured: 2048 tokens of 32 query heads of 8 key heads of 128, bf16 results: 79 us (435 TFLOP/s of what every row sees), f32 121; 531 tokens behind 5000, heads of 64, window 2048,
+// f32: 40 us.  A CTA takes about 9 us beside its key tiles (queries into the tensor core's memory, the first tile's way through all roles, results out) and 0.7 a key tile, which
+// the instructions of expanding and soft-max bound (tensor pipe active 20 %).
 // Every wait is bounded (tc_pair.cuh): one that runs out sets bit 1 of the library's error flags and the CTA leaves through the common exit.
 #include "seq_attn4.cuh"
 #include "tc_split.cuh"

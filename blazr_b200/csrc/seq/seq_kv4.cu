@@ -154,8 +154,8 @@ auto load_kernel(int lpr) {
 
 // b200seq_attn_prep_ex over 4-bit pages, for rows of whole 16-byte pieces (every head size, rotation and column that is a multiple of 8; norms over single heads).
 // LPR lanes have a head's row (4 for every group of 32), eight neighbouring values in a lane's registers; the rotation's other half comes from another lane.
-// A token's rows are split over `split` blocks of 128 threads.  Bounded by a chain of loads for single tokens (position, frequencies, then sines) and by
-// instructions for prompts.  us with rotation of halves and norms, rows as here / a warp to a head through shared memory (32 query heads of 8 key heads of 128):
+// A token's rows are split over `split` blocks of 128 threads.  Bounded by a chain of loads for single tokens (position, frequencies, then sines); for prompts
+// by that chain and by instructions (2048 tokens: issue slots 56 % active, a warp waits 5 of 12 cycles for loads from memory, DRAM 20 %).  us with rotation of halves and norms, rows as here / a warp to a head through shared memory (32 query heads of 8 key heads of 128):
 //   1 token  2.9 / 8.7      32 tokens  3.3 / 9.5      512  8.9 / 14.1      2048  26.3 / 49.9  (bytes alone: 12.8)
 template <int LPR>
 __global__ void __launch_bounds__(128) kv4_prep_rows_kernel(float* proj, int64_t ld, const b200seq_step st, const b200seq_attn_desc a, uint8_t* kpool, uint8_t* vpool,

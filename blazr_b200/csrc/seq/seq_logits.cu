@@ -2,8 +2,8 @@
 //
 // A block has a slice of one row's vocabulary.  It counts the row's history into a table in shared memory (only the tokens of its slice; whole numbers, so the order of
 // the additions does not matter), then reads, changes and writes its logits once.  The floor is the logits' bytes, 8 a token; a block's time is a
-// chain of loads (bounds, history, counts, biases), the history is read by every slice, from L2.  64 rows of 128256: 16 us without rules (4.1 TB/s), 24 with histories of up to
-// 4000 tokens, 28 with 300 biases and a mask too; one row of 32000 with 500 tokens 2.1.
+// chain of loads (bounds, history, counts, biases), the history is read by every slice, from L2.  64 rows of 128256: 16 us without rules (4.1 TB/s), 26 with histories of up to
+// 4000 tokens, 30 with 300 biases and a mask too; one row of 32000 with 500 tokens 2.4.
 #include "seq_common.cuh"
 
 namespace b200seq {

@@ -501,8 +501,8 @@ int b200seq_parallel_close(const b200seq_parallel_desc* d, void* stream);
  * store: k [T, G * D], v [T, Gv * V] (f32 or bf16, row strides ldk, ldv) go to the pages of the step's tokens.
  * load:  the same rows back in f32, as what they stand for.  A position behind its block table, or whose entry there is negative, raises bit 0 of the error flags: nothing is
  * stored or loaded for it, and attention leaves its rows as they are or (negative entries among the keys) reads the first page in its place.
- * attn_prep_kv4 is b200seq_attn_prep_ex, attn_kv4 is b200seq_attn_ex, over such pools (no pooled blocks, no latents; D, V <= 128): q and sums in 32 bits, the cache's
- * values as they are held.  A query that is not finite gives a row of NaN.  scratch: f32 work area of b200seq_attn_kv4_scratch_floats(...) floats (0 for most steps) or
+ * attn_prep_kv4 is b200seq_attn_prep_ex, attn_kv4 is b200seq_attn_ex, over such pools (no pooled blocks, no latents; D, V <= 128): the cache's values as they are
+ * held, q and the soft-max weights to 22 bits (f32 results) or at least 11 (bf16), sums in 32 bits.  A query that is not finite gives a row of NaN.  scratch: f32 work area of b200seq_attn_kv4_scratch_floats(...) floats (0 for most steps) or
  * null: with it, few sequences of many keys use the whole GPU.  max_keys: as many keys as the step's longest sequence has, or 0 for what the block tables hold; the work is shared
  * out by it (right for any number, faster for one that is near). */
 int64_t b200seq_kv4_page_bytes(int block_size, int G, int D);
