@@ -119,6 +119,9 @@ class Engine:
         return logits
 
     def release(self, rid: str) -> None:
+        """gives an externally scheduled request's pages and slot back; of an id that holds none nothing"""
+        if self._scheduled(rid):
+            raise ValueError(f"request {rid} belongs to the scheduler")
         if rid in self.cache.live:
             self.cache.release(rid)
 
@@ -187,7 +190,7 @@ class Engine:
         Returns the logits of the wanted places as a host array, or None when nothing was wanted."""
         out = None
         entries = [e for e in entries if len(e.get("tokens", ()))]      # an entry that brings no token has nothing to run
-        for rid in (str(e["id"]) for e in entries):
+        for rid in [str(e["id"]) for e in entries] + [str(i) for i in end]:
             if rid in self._sample_ids or self._scheduled(rid):
                 raise ValueError(f"request {rid} belongs to the scheduler")
         new, free = len({str(e["id"]) for e in entries} - self.cache.live.keys()), self.cache.slots.free_slots
@@ -461,6 +464,7 @@ class Engine:
                 for q in [r] + r.siblings:
                     if not q.finished:
                         (self.running if q in self.running else self.waiting).remove(q)
+                        q.finished = True
                         self.release(q.rid)
                     del self.requests[q.rid]
         return [[q.output for q in [r] + r.siblings] if r.params.n > 1 else r.output for r in reqs]

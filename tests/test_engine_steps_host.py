@@ -263,3 +263,20 @@ def test_a_generate_that_fails_takes_its_requests_back(monkeypatch):
     assert eng.generate([[2, 7], [3, 8]], SamplingParams(max_new_tokens=4)) == [alone([2, 7], 4), alone([3, 8], 4)]
     finish(eng)
     assert other.output == alone(PROMPT, 6)
+
+
+def test_requests_of_the_scheduler_are_not_released_from_outside(monkeypatch):
+    fake_rules(monkeypatch)
+    eng = engine()
+    r = eng.add_request("a", PROMPT, SamplingParams(max_new_tokens=4, n=2))
+    for _ in range(2):
+        with pytest.raises(ValueError):
+            eng.release("a")
+        with pytest.raises(ValueError):
+            eng.run_entries([{"id": "e", "tokens": [1], "want": []}], ["e", "a"])
+        assert "e" not in eng.cache.live
+        eng.step()
+    finish(eng)
+    eng.release("a")                                                   # (through: nothing to give back)
+    eng.release("nobody")
+    assert [q.output for q in [r] + r.siblings] == [alone(PROMPT, 4)] * 2
