@@ -1,0 +1,78 @@
+// seq_weigh.cuh -- what the kernels share that add up the soft-max weight of cached keys (seq_weigh.cu, seq_weigh_tc.cu)
+#pragma once
+#include "seq_attn.cuh"
+#include "seq_kv4.cuh"
+
+namespace b200seq {
+
+struct WeighArgs {
+    const float* q;            // query rows (pointer at the first head's column), stride ld
+    int64_t ld;
+    const float* kpool;        // f32 pages [page][row][G][D], or (four) 4-bit ones
+    const uint8_t* kpool4;
+    float* acc;                // [slots][G][acc_ld]
+    int64_t acc_ld;
+    int slots, H, G, D, NG;
+    int last;                  // > 0: the last so many tokens of an entry count
+    float scale, softcap;
+    int chunk, window, keep_first;
+    const float *head_scale, *sink;
+    float* lse;                // [T][H]: base-2 logarithm of every row's sum of exponentials (minus infinity: nothing to give), or nothing (the rows' path)
+    float* part;               // work area of the path that is taken
+    int key_blocks;            // rows' path: blocks of keys that the longest sequence may need
+    int64_t most_keys;         // of a sequence
+    int* err;
+};
+
+constexpr float WEIGH_LOG2E = 1.4426950408889634f;
+
+// the keys that a token at position p sees: lo .. p and those below keep
+struct WeighSpan {
+    int lo, p, keep;
+    __device__ __forceinline__ WeighSpan(const WeighArgs& a, int pos) {
+        p = pos, lo = a.chunk > 0 ? (pos / a.chunk) * a.chunk : 0, keep = a.window > 0 ? a.keep_first : 0;
+        if (a.window > 0) lo = max(lo, pos - a.window + 1);
+    }
+    __device__ __forceinline__ bool sees(int j) const { return j <= p && (j >= lo || j < keep); }
+};
+
+// an entry as these kernels see it: its first token that counts (row of the step, place among the entry's), how many do, its keys; n = 0: none, or its keys have no place
+struct WeighEntry {
+    int t0, n, p0, keys, fresh, slot;      // p0: position of the first token that counts; keys: positions 0 .. keys - 1; fresh: the first position that this step brought
+    __device__ __forceinline__ WeighEntry(const WeighArgs& a, const b200seq_step& st, int e, bool tell) {
+        const int s0 = st.ent_start[e], s1 = st.ent_start[e + 1], len = s1 - s0;
+        fresh = st.ent_pos0[e], slot = st.ent_slot[e];
+        n = a.last > 0 && a.last < len ? a.last : len;
+        t0 = s1 - n, keys = fresh + len, p0 = keys - n;
+        const bool fine = s0 >= 0 && len >= 0 && s1 <= st.T && fresh >= 0 && slot >= 0 && slot < a.slots && keys <= a.acc_ld && keys <= a.most_keys && (keys + st.block_size - 1) / st.block_size <= st.max_blocks;
+        if (!fine) {
+            if (tell && len > 0) atomicOr(a.err, 1);
+            n = 0;
+        } else if (len == 0) {
+            n = 0;
+        }
+    }
+};
+
+// score of a dot product in base 2: scaled, soft-capped
+__device__ __forceinline__ float weigh_score(float dot, float factor, float softcap) {
+    const float z = dot * factor;
+    return softcap > 0.f ? softcap * WEIGH_LOG2E * tanhf(z / softcap) : z * WEIGH_LOG2E;
+}
+__device__ __forceinline__ float weigh_factor(const WeighArgs& a, int h) { return a.head_scale ? a.scale * a.head_scale[h] : a.scale; }
+
+// base-2 logarithm of a row's denominator from its maximum and sum (base 2), with the sink's term
+__device__ __forceinline__ float weigh_lse(const WeighArgs& a, int h, float m, float l) {
+    if (a.sink) {
+        const float sk = a.sink[h] * WEIGH_LOG2E, top = fmaxf(m, sk);
+        l = (m == -INFINITY ? 0.f : l * exp2f(m - top)) + exp2f(sk - top), m = top;
+    }
+    return m == -INFINITY ? -INFINITY : m + log2f(l);
+}
+
+// Steps of many rows on the tensor cores (seq_weigh_tc.cu): whether it takes a layer, its work area, its launches
+bool weigh_tc_takes(const WeighArgs& a, const b200seq_step& st);
+size_t weigh_tc_floats(const b200seq_step& st, int H);
+cudaError_t weigh_tc(WeighArgs a, const b200seq_step& st, int max_keys, cudaStream_t cs, int& launches);
+
+}  // namespace b200seq

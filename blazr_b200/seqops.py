@@ -4,7 +4,8 @@ over a paged KV pool, the state-space recurrence, gated activations, the depth-a
 latent attention, per-head projections, token shift + gated post-norm, the branch sum + output norm of two-branch mixers, the bigram
 embedding, PolyNorm, soft caps, differential attention, minGRU and real-gated linear recurrences, soft-max routing with identity experts,
 the delta rule with per-channel decays, layers normed on both sides with sinusoidal positions and a token-dependent addition, the selective scan
-with a decay per channel and state, the residual of parallel layers, a KV cache held in 4 bits and its attention, page copies, sampling rules, arg-max).
+with a decay per channel and state, the residual of parallel layers, a KV cache held in 4 bits and its attention, page copies, sampling rules, drafts
+verified, the weight of cached keys and their eviction, arg-max).
 
 Like blazr_b200/ops.py, PyTorch is plumbing only (device memory, streams); every compute call goes through ctypes.  The library
 is compiled on first use when it is missing (`ensure_built`): a fresh checkout needs nothing but nvcc.  There is no CPU
@@ -47,7 +48,8 @@ EXPORTS = ["b200seq_last_error", "b200seq_version", "b200seq_launch_count", "b20
            "b200seq_diff_combine", "b200seq_min_gru", "b200seq_rg_lru", "b200seq_delta", "b200seq_delta_scratch_floats", "b200seq_embed_pos", "b200seq_sandwich_norm",
            "b200seq_token_gate", "b200seq_side_close", "b200seq_linear_silu", "b200seq_moe_route_rule", "b200seq_moe_router_rule", "b200seq_retention_partials",
            "b200seq_selective_scan", "b200seq_scan_scratch_floats", "b200seq_parallel_close", "b200seq_kv4_page_bytes", "b200seq_kv4_store", "b200seq_kv4_load",
-           "b200seq_attn_prep_kv4", "b200seq_attn_kv4", "b200seq_attn_kv4_scratch_floats", "b200seq_copy_pages", "b200seq_process_logits"]
+           "b200seq_attn_prep_kv4", "b200seq_attn_kv4", "b200seq_attn_kv4_scratch_floats", "b200seq_copy_pages", "b200seq_process_logits",
+           "b200seq_verify_drafts", "b200seq_verify_scratch_bytes", "b200seq_key_weights", "b200seq_key_weights_scratch_floats", "b200seq_evict_keys"]
 
 # argument types of the operators' C entries (include/b200seq.h): p pointer, i int, l int64, z size_t, f float.  Declared, plain numbers are converted by ctypes
 # as they are passed; an object made for each of them and a stream object looked up for each call took half of a call's 4 - 8 us.
@@ -65,7 +67,9 @@ SIGNATURES = {
     "polynorm": "pliipfpilp", "softcap": "plfp", "diff_combine": "piiiifffpip", "min_gru": "pliiipppipip", "rg_lru": "plplppfplipppiipip", "delta": "plppplppipzp",
     "embed_pos": "pppfpippppfpip", "sandwich_norm": "pppfppipippipp", "token_gate": "pliiplippip", "side_close": "pppfpppliippppipippipp",
     "selective_scan": "piplpplppppipzp", "parallel_close": "pp", "argmax": "piipp", "kv4_page_bytes": "iii", "kv4_store": "plplipiiiippp", "kv4_load": "pppiiiiplplp",
-    "attn_prep_kv4": "plppppp", "attn_kv4": "plpppppipzip", "attn_kv4_scratch_floats": "ppi", "copy_pages": "ppiipip", "process_logits": "pliippipppppiplplp"
+    "attn_prep_kv4": "plppppp", "attn_kv4": "plpppppipzip", "attn_kv4_scratch_floats": "ppi", "copy_pages": "ppiipip", "process_logits": "pliippipppppiplplp",
+    "verify_scratch_bytes": "iii", "verify_drafts": "pliipippppppplpppzp", "key_weights_scratch_floats": "ppii", "key_weights": "plpppipiliipzp",
+    "evict_keys": "pppiiiiiiiilpppippiiiiipp"
 }
 
 
@@ -208,6 +212,7 @@ def lib() -> C.CDLL:
         L.b200seq_launch_count.restype = C.c_int64
         L.b200seq_kv4_page_bytes.restype = C.c_int64
         L.b200seq_attn_kv4_scratch_floats.restype = C.c_size_t
+        L.b200seq_verify_scratch_bytes.restype = L.b200seq_key_weights_scratch_floats.restype = C.c_size_t
         for name, args in SIGNATURES.items():
             getattr(L, "b200seq_" + name).argtypes = [_ARG[a] for a in args]
         _lib = L
@@ -1037,3 +1042,117 @@ def process_logits(logits: torch.Tensor, rules: torch.Tensor, out: Optional[torc
                (logits.data_ptr(), lx[0] if R > 1 else V, R, V, rules.data_ptr(), _p(hist), hist.numel() if hist is not None else 0, _p(hist_start), _p(hist_prompt),
                 _p(bias_start), _p(bias_ids), _p(bias_vals), bias_ids.numel() if bias_ids is not None else 0, _p(mask), lm, out.data_ptr(), lo[0] if R > 1 else V), logits, rules, out, hist, hist_start, hist_prompt, bias_start, bias_ids, bias_vals, mask)
     return out
+
+
+# ---- drafts, and a cache of bounded size -----------------------------------------------------------------------------------------------------------------
+def _flat(name: str, what: str, t: Optional[torch.Tensor], dtype, n: int) -> None:
+    if t is not None and (t.dtype != dtype or t.numel() != n or not t.is_contiguous()):
+        raise ValueError(f"{name}: {what} is contiguous {dtype} of {n} values, not {t.dtype} {tuple(t.shape)}")
+
+
+@_timed
+def verify_drafts(logits: torch.Tensor, start: torch.Tensor, drafts: torch.Tensor, accept_u: torch.Tensor, sample_u: torch.Tensor, temperature: torch.Tensor, *,
+                  top_k: Optional[torch.Tensor] = None, top_p: Optional[torch.Tensor] = None, draft_probs: Optional[torch.Tensor] = None,
+                  accepted: Optional[torch.Tensor] = None, tokens: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """drafted tokens against the probabilities of f32 logits [R, V], from given random numbers.  Entry e has rows start[e] .. start[e + 1] - 1 (start int32 [B + 1]): its drafts
+    (drafts int32 [R], one a row) and one row more; an entry of one row samples a token.  A draft x is accepted when accept_u * q(x) < p(x) (accept_u f32 [R], draft_probs f32 [R, V]
+    the distributions it was drawn from; None: it was certain); the token behind the accepted ones is drawn with sample_u (f32 [B]) from what p has more than q, or from the last
+    row's p.  temperature f32 [B] (0: the largest logit, always), top_k int32 [B] (0: all), top_p f32 [B] (1: all) make p as include/b200seq.h says.
+    Returns (accepted int32 [B], tokens int32 [R]: accepted drafts, the token behind them, then -1; -1 in its place: the row's logits leave no choice)."""
+    shape, lx = logits.shape, logits.stride()
+    if len(shape) != 2 or lx[1] != 1 or logits.dtype != torch.float32 or shape[1] < 1:
+        raise ValueError(f"verify_drafts: row-major float32 logits [rows, vocabulary], not {logits.dtype} {tuple(shape)}")
+    R, V = shape
+    B = temperature.numel()
+    i32, f32 = torch.int32, torch.float32
+    accepted = torch.empty(B, dtype=i32, device=logits.device) if accepted is None else accepted
+    tokens = torch.empty(R, dtype=i32, device=logits.device) if tokens is None else tokens
+    for what, t, dtype, n in (("start", start, i32, B + 1), ("drafts", drafts, i32, R), ("accept_u", accept_u, f32, R), ("sample_u", sample_u, f32, B), ("temperature", temperature, f32, B),
+                              ("top_k", top_k, i32, B), ("top_p", top_p, f32, B), ("accepted", accepted, i32, B), ("tokens", tokens, i32, R)):
+        _flat("verify_drafts", what, t, dtype, n)
+    lq = 0
+    if draft_probs is not None:
+        lq = draft_probs.stride()
+        if draft_probs.shape != shape or lq[1] != 1 or draft_probs.dtype != f32:
+            raise ValueError(f"verify_drafts: draft_probs are row-major float32 {tuple(shape)}, not {draft_probs.dtype} {tuple(draft_probs.shape)}")
+        lq = lq[0] if R > 1 else V
+    L = lib()
+    need = L.b200seq_verify_scratch_bytes(R, V, top_k is not None or top_p is not None)
+    scratch = torch.empty(need, dtype=_U8, device=logits.device)
+    _on_device("verify_drafts", L.b200seq_verify_drafts,
+               (logits.data_ptr(), lx[0] if R > 1 else V, R, V, start.data_ptr(), B, drafts.data_ptr(), accept_u.data_ptr(), sample_u.data_ptr(), temperature.data_ptr(), _p(top_k),
+                _p(top_p), _p(draft_probs), lq, accepted.data_ptr(), tokens.data_ptr(), scratch.data_ptr(), need),
+               logits, start, drafts, accept_u, sample_u, temperature, top_k, top_p, draft_probs, accepted, tokens)
+    return accepted, tokens
+
+
+@_timed
+def key_weights(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: torch.Tensor, acc: torch.Tensor, *, last: int = 0, max_keys: int = 0):
+    """adds up the soft-max weight that the step's tokens (their queries prepared in proj) give to the cached keys of their sequences: acc f32 [slots, G, room], by the entries' state
+    slots; keys that the step brought begin at zero.  kpool: the layer's f32 or 4-bit key pages.  last: only that many last tokens of every entry count (0: all).  max_keys: keys of the
+    step's longest sequence, where the block tables hold many more (0: as many as they hold; never fewer than it has)."""
+    four = kpool.dtype == _U8
+    shape, ld = proj.shape, proj.stride()
+    if len(shape) != 2 or ld[1] != 1 or proj.dtype != torch.float32 or shape[0] < step.T or shape[1] < d.q_col + d.H * d.D:
+        raise ValueError(f"key_weights: projection rows are row-major float32 [{step.T}, {d.q_col + d.H * d.D} or more], not {proj.dtype} {tuple(shape)}")
+    if four:
+        _kv4_pool_check("key_weights", "key", kpool, kpool.shape, step.block_size, d.G, d.D)
+    elif kpool.dtype != torch.float32 or kpool.dim() != 4 or tuple(kpool.shape[1:]) != (step.block_size, d.G, d.D) or not kpool.is_contiguous():
+        raise ValueError(f"key_weights: the key pool is contiguous float32 [pages, {step.block_size}, {d.G}, {d.D}], not {kpool.dtype} {tuple(kpool.shape)}")
+    if acc.dtype != torch.float32 or acc.dim() != 3 or acc.shape[1] != d.G or not acc.is_contiguous() or acc.numel() == 0:
+        raise ValueError(f"key_weights: weights are contiguous float32 [slots, {d.G}, room], not {acc.dtype} {tuple(acc.shape)}")
+    if last < 0 or max_keys < 0:
+        raise ValueError(f"key_weights: last {last} tokens of {max_keys} keys")
+    L = lib()
+    sref, dref = C.byref(step), C.byref(d)
+    need = L.b200seq_key_weights_scratch_floats(sref, dref, last, max_keys)
+    scratch = torch.empty(max(need, 4), dtype=torch.float32, device=proj.device)
+    _on_device("key_weights", L.b200seq_key_weights, (proj.data_ptr(), ld[0], sref, dref, kpool.data_ptr(), 4 if four else 32, acc.data_ptr(), acc.shape[0], acc.shape[2], last, max_keys,
+                                                      scratch.data_ptr(), need), proj, kpool, acc)
+
+
+@_timed
+def evict_keys(kpools: Sequence[torch.Tensor], vpools: Sequence[torch.Tensor], accs: Sequence[torch.Tensor], slots: torch.Tensor, rows: torch.Tensor, table: torch.Tensor, keep: int, *,
+               first: int = 0, recent: int = 0, block_size: int = 0, to_table: Optional[torch.Tensor] = None, to_slots: Optional[torch.Tensor] = None,
+               kept: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """sequences of more than `keep` cached rows are cut back, in every layer and key head for itself, to the `first` ones, the `recent` ones and those of largest weight between: rows of
+    keys, values and weights go, in order, to the places 0 .. keep - 1 of to_table and to_slots (default: where they are).  Layers: lists of pools (f32 [pages, block_size, G, D] or
+    4-bit ones, for which block_size is given) and of their weights f32 [slots, G, room]; entries: slots int32 [B], rows int32 [B] (how many each has), table int32 [B, pages].
+    No two entries write into one page or slot.  Returns kept int32 [layers, B, G, keep]: the rows that stayed, -1 behind them."""
+    n, i32 = len(kpools), torch.int32
+    if n == 0 or len(vpools) != n or len(accs) != n:
+        raise ValueError(f"evict_keys: {n} key pools, {len(vpools)} value pools and {len(accs)} weights")
+    k, v, a = kpools[0], vpools[0], accs[0]
+    four = k.dtype == _U8
+    if four:
+        if block_size < 1:
+            raise ValueError("evict_keys: 4-bit pools need their block size")
+        if k.dim() != 3 or v.dim() != 3 or any(p.shape[2] not in (20 * block_size, 40 * block_size, 80 * block_size) for p in (k, v)):
+            raise ValueError(f"evict_keys: pools {tuple(k.shape)} and {tuple(v.shape)} are not of pages of {block_size} positions")
+        bs, G, Gv = block_size, k.shape[1], v.shape[1]
+        D, V = (p.shape[2] // (20 * bs) * 32 for p in (k, v))
+    else:
+        if k.dim() != 4 or v.dim() != 4 or k.shape[1] != v.shape[1] or block_size not in (0, k.shape[1]):
+            raise ValueError(f"evict_keys: pools {tuple(k.shape)} and {tuple(v.shape)} are not of one block size")
+        bs, G, D, Gv, V = k.shape[1], k.shape[2], k.shape[3], v.shape[2], v.shape[3]
+    for what, ts, like, dtype in (("key pools", kpools, k, k.dtype if four else torch.float32), ("value pools", vpools, v, k.dtype if four else torch.float32), ("weights", accs, a, torch.float32)):
+        for t in ts:
+            if t.dtype != dtype or t.shape != like.shape or not t.is_contiguous():
+                raise ValueError(f"evict_keys: {what} are contiguous {dtype} of one shape, not {t.dtype} {tuple(t.shape)} beside {tuple(like.shape)}")
+    if k.shape[0] != v.shape[0] or a.dim() != 3 or a.shape[1] != G or a.numel() == 0 or k.numel() == 0 or v.numel() == 0:
+        raise ValueError(f"evict_keys: pools {tuple(k.shape)} and {tuple(v.shape)} with weights {tuple(a.shape)}")
+    if not (keep >= 1 and first >= 0 and recent >= 0 and first + recent <= keep):
+        raise ValueError(f"evict_keys: the first {first} and the last {recent} of {keep} rows to keep")
+    B = rows.numel()
+    to_table, to_slots = table if to_table is None else to_table, slots if to_slots is None else to_slots
+    kept = torch.empty((n, B, G, keep), dtype=i32, device=k.device) if kept is None else kept
+    for what, t, m in (("slots", slots, B), ("rows", rows, B), ("to_slots", to_slots, B), ("kept", kept, n * B * G * keep)):
+        _flat("evict_keys", what, t, i32, m)
+    for what, t in (("table", table), ("to_table", to_table)):
+        if t.dtype != i32 or t.dim() != 2 or t.shape[0] != B or t.shape[1] < 1 or not t.is_contiguous():
+            raise ValueError(f"evict_keys: {what} is contiguous int32 [{B}, pages], not {t.dtype} {tuple(t.shape)}")
+    ptrs = lambda ts: pack(f"{n}P", *[t.data_ptr() for t in ts])
+    _on_device("evict_keys", lib().b200seq_evict_keys,
+               (ptrs(kpools), ptrs(vpools), ptrs(accs), n, 4 if four else 32, bs, G, D, Gv, V, a.shape[0], a.shape[2], slots.data_ptr(), rows.data_ptr(), table.data_ptr(), table.shape[1],
+                to_slots.data_ptr(), to_table.data_ptr(), to_table.shape[1], B, keep, first, recent, kept.data_ptr()), *kpools, *vpools, *accs, slots, rows, table, to_slots, to_table, kept)
+    return kept

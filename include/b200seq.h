@@ -10,7 +10,8 @@
  * linear recurrences, PolyNorm, soft-max routing with identity experts, a hashed bigram embedding,
  * the delta rule with per-channel decays, layers normed on both sides with sinusoidal positions and a
  * token-dependent addition, the selective scan with a decay per channel and state, the residual of parallel
- * layers, a KV cache held in 4 bits and its attention, page copies, sampling rules on logits, arg-max sampling.
+ * layers, a KV cache held in 4 bits and its attention, page copies, sampling rules on logits, drafts
+ * verified, the weight of cached keys and their eviction, arg-max sampling.
  *
  * It sits beside libb200q (include/b200q.h), which holds the quantized linear layer; the conventions are
  * the same:
@@ -528,6 +529,41 @@ int b200seq_copy_pages(void* const* pools, const int64_t* page_bytes, int npools
 int b200seq_process_logits(const float* x, int64_t ldx, int R, int V, const float* rules, const int32_t* hist, int nhist, const int32_t* hist_start, const int32_t* hist_prompt,
                            const int32_t* bias_start, const int32_t* bias_ids, const float* bias_vals, int nbias, const uint32_t* mask, int64_t mask_ld, float* out, int64_t ldo,
                            void* stream);
+
+/* ---- between two steps of a serving loop: drafts, and a cache of bounded size ---------------------------------------------------------------------------
+ * Drafted tokens against the target's probabilities, from given random numbers in [0, 1).  Entry e has the rows start[e] .. start[e + 1] - 1 of logits (f32 [R, V], stride ld):
+ * its drafts drafts[row], in order, and one row more (whose draft is not read).  An entry of one row has no drafts: a token is sampled.  With its temperature T:
+ *   w = exp((z - max z) / T), kept where z >= the top_k-th largest z (top_k[e] > 0) and then where the kept weights of strictly larger z are below top_p[e] of their sum
+ *   (top_p[e] < 1; at least the largest);   p = w / sum of the kept.   T <= 0: p = 1 at the first maximum
+ * A draft x is accepted when accept_u[row] * q(x) < p(x), q(x) = draft_probs[row][x] (f32 [R, V], stride ldq; null: 1), at T <= 0 when it is the first maximum.  The token behind the
+ * accepted drafts is drawn from max(p - q, 0) of the row that rejected (null: p without the draft; where nothing is left: p), or from the last row's p: the lowest token whose
+ * cumulated weight exceeds sample_u[e] times the sum.  accepted[e]: how many drafts; tokens[start[e] ..]: the accepted drafts, the token behind them, then -1.
+ * A row without a finite maximum, or with a NaN, accepts nothing and gives -1.  A draft outside the vocabulary is not accepted; it, and starts that are not in order within R, raise
+ * bit 4 of the error flags.  top_k int32 [B], top_p f32 [B]: each optional.  scratch: b200seq_verify_scratch_bytes(R, V, top_k or top_p given) bytes, 16-byte aligned. */
+size_t b200seq_verify_scratch_bytes(int R, int V, int ruled);
+int b200seq_verify_drafts(const float* logits, int64_t ld, int R, int V, const int32_t* start, int B, const int32_t* drafts, const float* accept_u, const float* sample_u,
+                          const float* temperature, const int32_t* top_k, const float* top_p, const float* draft_probs, int64_t ldq, int32_t* accepted, int32_t* tokens,
+                          void* scratch, size_t scratch_bytes, void* stream);
+
+/* The soft-max weight that a step's tokens give to every cached key: with the queries in proj and the keys in the pool, both as b200seq_attn_prep_ex (kv_bits 32) or
+ * b200seq_attn_prep_kv4 (4) leave them, and the scores and masks of b200seq_attn_ex (no pooled blocks, latents or gathered rows),
+ *   acc[slot][g][j] += sum over the entry's tokens and the query heads of key head g of their weights for key j;   a key that this step brought gets the sum instead
+ * acc: f32 [slots][G][acc_ld].  last > 0: only the last so many tokens of every entry count.  A row that sees nothing but scores of minus infinity gives nothing.
+ * max_keys: no fewer keys than the step's longest sequence has, or 0 for what the block tables hold.  Entries whose slot is none, or whose keys go beyond acc_ld, max_keys or their
+ * block table, raise bit 0 of the error flags and are left out.  scratch: b200seq_key_weights_scratch_floats(...) floats, 16-byte aligned. */
+size_t b200seq_key_weights_scratch_floats(const b200seq_step* st, const b200seq_attn_desc* d, int last, int max_keys);
+int b200seq_key_weights(const float* proj, int64_t ld, const b200seq_step* st, const b200seq_attn_desc* d, const void* kpool, int kv_bits, float* acc, int slots, int64_t acc_ld,
+                        int last, int max_keys, float* scratch, size_t scratch_floats, void* stream);
+
+/* Sequences cut back to `keep` cached rows.  Entry e has rows[e] of them in the pages table[e] (int32 [B][max_blocks]) of every layer's pools, and their weights in slot[e] of its acc
+ * (f32 [slots][G][acc_ld]).  Where rows[e] > keep, every layer and key head keeps the first `first`, the last `recent` and, of the rest, those of largest weight (ties: the lowest
+ * row; NaN lowest); where not, all.  They go in order to the places 0, 1, .. of the pages to_table[e] and of slot to_slot[e]; both may be the entry's own (a place that is not written
+ * stays as it is), but no page or slot that is written may be another entry's, nor one of its own in another order.  kept int32 [layers][B][G][keep] receives the rows, -1 behind them.
+ * kpools, vpools, accs: HOST arrays of device pointers.  kv_bits 32: f32 pages [block_size][G][D] and [block_size][G][V]; 4: those of b200seq_kv4_store.  Gv == G.
+ * An entry whose slots are none or whose rows go beyond acc_ld or its tables, and a row whose page is negative, raise bit 0 of the error flags and stay. */
+int b200seq_evict_keys(void* const* kpools, void* const* vpools, float* const* accs, int layers, int kv_bits, int block_size, int G, int D, int Gv, int V, int slots, int64_t acc_ld,
+                       const int32_t* slot, const int32_t* rows, const int32_t* table, int max_blocks, const int32_t* to_slot, const int32_t* to_table, int to_max_blocks, int B,
+                       int keep, int first, int recent, int32_t* kept, void* stream);
 
 /* ids[r] = argmax_v logits[r][v] (first maximum) */
 int b200seq_argmax(const float* logits, int R, int V, int32_t* ids, void* stream);
