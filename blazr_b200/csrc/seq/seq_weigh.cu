@@ -340,6 +340,7 @@ struct Plan {
     bool rows;
     int blocks;        // rows path: blocks of RK keys of the longest sequence
     int tokens;        // tokens of an entry that count: a bound
+    WeighTcPlan tc;
     size_t floats;
 };
 Plan plan_of(const b200seq_step& st, const b200seq_attn_desc& d, int last, int max_keys) {
@@ -351,7 +352,8 @@ Plan plan_of(const b200seq_step& st, const b200seq_attn_desc& d, int last, int m
     p.tokens = last > 0 && last < st.T ? last : st.T;
     const int64_t floats = (int64_t)st.T * d.H * p.blocks * (RK + 2);
     p.rows = d.D <= 128 && (int64_t)tokens * (d.H / d.G) <= ROWS_MOST && floats <= ROWS_FLOATS;
-    p.floats = p.rows ? (size_t)floats : (size_t)st.T * d.H;
+    p.tc = weigh_tc_plan(st, d.H, d.G, last, (int64_t)p.blocks * RK);
+    p.floats = p.rows ? (size_t)floats : p.tc.floats;      // (more than the f32 tiles' T * H)
     return p;
 }
 
@@ -364,7 +366,7 @@ using namespace b200seq;
 extern "C" {
 
 size_t b200seq_key_weights_scratch_floats(const b200seq_step* st, const b200seq_attn_desc* d, int last, int max_keys) {
-    if (!st || !d || st->T < 1 || d->H < 1 || d->G < 1 || st->max_blocks < 1 || st->block_size < 1) return 0;
+    if (!st || !d || st->T < 1 || st->B < 1 || d->H < 1 || d->G < 1 || st->max_blocks < 1 || st->block_size < 1) return 0;
     return plan_of(*st, *d, last, max_keys).floats;
 }
 
@@ -399,6 +401,7 @@ int b200seq_key_weights(const float* proj, int64_t ld, const b200seq_step* st, c
         SEQ_LAUNCH_CHECK("key_weights");
         return 0;
     }
+    if (weigh_tc_takes(a, four)) return weigh_tc(a, *st, p.tc, scratch, four, cs);
     a.lse = scratch;
     const int64_t tiles = ((int64_t)p.tokens * (d->H / d->G) + TR - 1) / TR, key_tiles = (p.blocks * (int64_t)RK + TK - 1) / TK;
     launch_chained(weigh_tile_lse_kernel, dim3((unsigned)tiles, d->G, st->B), TT, 0, cs, a, *st, (int)four);

@@ -70,9 +70,15 @@ __device__ __forceinline__ float weigh_lse(const WeighArgs& a, int h, float m, f
     return m == -INFINITY ? -INFINITY : m + log2f(l);
 }
 
-// Steps of many rows on the tensor cores (seq_weigh_tc.cu): whether it takes a layer, its work area, its launches
-bool weigh_tc_takes(const WeighArgs& a, const b200seq_step& st);
-size_t weigh_tc_floats(const b200seq_step& st, int H);
-cudaError_t weigh_tc(WeighArgs a, const b200seq_step& st, int max_keys, cudaStream_t cs, int& launches);
+// Steps of many rows on the tensor cores (seq_weigh_tc.cu): how a step is cut up and the work area it needs (from its host sizes alone), whether a layer's rows suit it, the launches
+struct WeighTcPlan {
+    int tiles, stat_parts;     // denominators: row tiles (bound), parts of a walk
+    int key_tiles, parts;      // sums: key tiles of the longest sequence, parts of a walk
+    int64_t key_room;
+    size_t stat_floats, floats;
+};
+WeighTcPlan weigh_tc_plan(const b200seq_step& st, int H, int G, int last, int64_t keys);
+bool weigh_tc_takes(const WeighArgs& a, bool four);
+int weigh_tc(const WeighArgs& a, const b200seq_step& st, const WeighTcPlan& p, float* scratch, bool four, cudaStream_t cs);
 
 }  // namespace b200seq
