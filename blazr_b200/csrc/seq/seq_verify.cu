@@ -6,8 +6,11 @@
 //
 // What a row decides is compared with a random number, so that its sums are held in 64 bits (weights are f32, within 2^-21 of themselves; sums of four of them, then f64).
 // The floor is the logits' bytes: they are read once, in slices over the whole GPU (row_stats), with maximum, its place and sum left for every slice.  Then a cluster of eight
-// CTAs an entry puts the slices together, finds the row that rejects and reads that one again, from L2 (pick).  top_k and top_p need a threshold a row before that: a cluster a
-// row selects it by the bits of the ordered logits, eleven at a time, by counts, then by masses in whole numbers of 2^-31 (row_cut): additions whose order does not matter.
+// CTAs an entry puts the slices together, finds the row that rejects and reads that one again, from L2 (pick).
+// top_k and top_p need a threshold a row before that (row_cut, a CTA a row, which it reads twice or three times from L2): counts, or masses (whole numbers of 2^-33: additions whose
+// order does not matter), of 2048 bins of equal width below the maximum show how far down the k-th logit lies, or where the mass passes the share; the logits down to there are sorted.
+// Where those are too many (rows of equal logits, logits far apart), the threshold is selected by the bits of the ordered logits instead, eleven at a time.
+#include <cfloat>
 #include <cooperative_groups.h>
 
 #include "seq_common.cuh"
@@ -21,8 +24,9 @@ namespace cg = cooperative_groups;
 
 constexpr int ERR_TOKEN = 16;             // error flag: a token id outside the vocabulary
 constexpr int CLUSTER = 8;
-constexpr int PICK = 512, CUT = 1024;     // threads
+constexpr int STATS = 256, PICK = 256, CUT = 1024;     // threads
 constexpr int MAX_TILES = 512;            // tiles of 4 * PICK logits of one CTA's share
+constexpr int BINS = 2048, LIST = 2048;   // bins below the maximum; logits that are sorted
 constexpr int64_t MAX_V = (int64_t)CLUSTER * MAX_TILES * 4 * PICK - 64;
 
 struct Partial {      // of a slice of a row
@@ -64,14 +68,12 @@ struct Heat {
     float hi, lo;
     __device__ __forceinline__ explicit Heat(float T) {
         const double c = fmin(1.4426950408889634 / (double)T, 3e38);
-        hi = (float)c, lo = (float)(c - (double)hi);
+        hi = __double2float_rd(c), lo = (float)(c - (double)hi);      // (neither below zero: their products with d have one sign)
     }
-    // weight of z under the maximum m; NaN where either is no number
+    // weight of z under the maximum m: 1 at m, 0 at minus infinity; of a NaN, or under an infinite m, 0 (whoever sums looks for those)
     __device__ __forceinline__ float operator()(float z, float m) const {
-        if (z == m && m > -INFINITY && m < INFINITY) return 1.f;
-        if (z == -INFINITY) return 0.f;
-        const float d = z - m;
-        return tcsplit::ex2(fmaf(d, hi, d * lo));
+        const float d = fmaxf(z - m, -FLT_MAX);
+        return z == -INFINITY ? 0.f : tcsplit::ex2(fmaf(d, hi, d * lo));
     }
 };
 
@@ -89,11 +91,11 @@ __device__ __forceinline__ int entry_of(const VerifyArgs& a, int row) {
     return e;
 }
 
-// grid (slices, rows): 16 logits a thread, all asked for before anything else
-template <int THREADS>
-__global__ void __launch_bounds__(THREADS) row_stats_kernel(const __grid_constant__ VerifyArgs a) {
+// grid (slices, rows): 16 logits a thread, all asked for before anything else.  Small blocks, so that one's sums run beside another's loads (320 rows of 128256: blocks of 1024
+// threads 64 us, of 256 40: 4.1 TB/s)
+__global__ void __launch_bounds__(STATS) row_stats_kernel(const __grid_constant__ VerifyArgs a) {
     chain_enter();
-    constexpr int WARPS = THREADS / 32;
+    constexpr int THREADS = STATS, WARPS = THREADS / 32;
     __shared__ float wmax[WARPS];
     __shared__ unsigned wat[WARPS];
     __shared__ double wsum[WARPS];
@@ -126,9 +128,11 @@ __global__ void __launch_bounds__(THREADS) row_stats_kernel(const __grid_constan
     for (int w = 1; w < WARPS; ++w) top = fmaxf(top, wmax[w]);
     const unsigned first = __reduce_min_sync(0xffffffffu, m == top && top > -INFINITY ? (unsigned)at : 0x7fffffffu);
     const Heat heat(T > 0.f ? T : 1.f);
-    double sum = 0.0;
+    double sum = 0.0;      // (a slice of minus infinities: nothing)
+    if (top > -INFINITY) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) sum += (double)((heat(v[k].x, top) + heat(v[k].y, top)) + (heat(v[k].z, top) + heat(v[k].w, top)));
+        for (int k = 0; k < 4; ++k) sum += (double)((heat(v[k].x, top) + heat(v[k].y, top)) + (heat(v[k].z, top) + heat(v[k].w, top)));
+    }
     if (odd) sum = NAN;
     sum = warp_sum(sum);
     if (lane == 0) wat[warp] = first, wsum[warp] = sum;
@@ -159,7 +163,7 @@ __device__ __forceinline__ Row whole_row(const VerifyArgs& a, const Heat& heat, 
     for (int i = lane; i < a.slices; i += 32) {
         const Partial s = p[i];
         if (s.max == r.max) at = min(at, (unsigned)s.at);
-        r.sum += s.sum == 0.0 ? 0.0 : s.sum * (double)heat(s.max, r.max);
+        r.sum += s.sum * (double)heat(s.max, r.max);      // (0 or NaN stay what they are)
     }
     r.at = (int)__reduce_min_sync(0xffffffffu, at);
     r.sum = warp_sum(r.sum);
@@ -173,142 +177,261 @@ __device__ __forceinline__ uint32_t order_key(float z) {
 }
 __device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu)); }
 
-// The bin of an array of 2048 (two neighbours a thread) in which what lies above, added up from the top, passes `want`: the lowest bin with fewer than `want` above it and
-// something in it.  Every thread gets the bin and what lies above it.  sh: 34 words.
-__device__ __forceinline__ int find_bin(unsigned long long lo, unsigned long long hi, unsigned long long want, unsigned long long& above, unsigned long long* sh) {
+// the sum of a number of every thread, for all; sh: 33 words
+template <class N>
+__device__ __forceinline__ N block_total(N v, N* sh) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();                                       // (sh may still be read)
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = sh[threadIdx.x & 31];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// what lies before a thread's number, in the order of the threads (from the last on: FROM_TOP); sh: 32 words
+template <class N, bool FROM_TOP>
+__device__ __forceinline__ N block_before(N own, N* sh) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    unsigned long long s = lo + hi;                        // bins 2 t, 2 t + 1: from this thread's to the warp's last
+    N s = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long y = __shfl_down_sync(0xffffffffu, s, o);
-        if (lane + o < 32) s += y;
+        const N y = FROM_TOP ? __shfl_down_sync(0xffffffffu, s, o) : __shfl_up_sync(0xffffffffu, s, o);
+        if (FROM_TOP ? lane + o < 32 : lane >= o) s += y;
     }
     __syncthreads();                                       // (sh may still be read)
-    if (lane == 0) sh[warp] = s;
+    if (lane == (FROM_TOP ? 0 : 31)) sh[warp] = s;
     __syncthreads();
-    for (int w = warp + 1; w < CUT / 32; ++w) s += sh[w];
-    const unsigned long long over = s - lo - hi;           // above both bins
-    if (hi > 0 && over < want && over + hi >= want) sh[32] = 2 * threadIdx.x + 1, sh[33] = over;
-    if (lo > 0 && over + hi < want && over + hi + lo >= want) sh[32] = 2 * threadIdx.x, sh[33] = over + hi;
+    N w = sh[lane], all = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const N y = FROM_TOP ? __shfl_down_sync(0xffffffffu, all, o) : __shfl_up_sync(0xffffffffu, all, o);
+        if (FROM_TOP ? lane + o < 32 : lane >= o) all += y;
+    }
+    return s - own + __shfl_sync(0xffffffffu, all - w, warp);
+}
+
+// Of 2048 bins, bins 2 t and 2 t + 1 in thread t, the one in which what is added up (from the last bin on: FROM_TOP) passes `want`, and what comes before it; for all threads
+template <bool FROM_TOP>
+__device__ __forceinline__ int find_bin(unsigned long long b0, unsigned long long b1, unsigned long long want, unsigned long long& before, unsigned long long* sh) {
+    const unsigned long long first = FROM_TOP ? b1 : b0, second = FROM_TOP ? b0 : b1, s = block_before<unsigned long long, FROM_TOP>(b0 + b1, sh);
+    const int t = 2 * threadIdx.x;
+    if (s < want && s + first >= want) sh[32] = t + (FROM_TOP ? 1 : 0), sh[33] = s;
+    if (s + first < want && s + first + second >= want) sh[32] = t + (FROM_TOP ? 0 : 1), sh[33] = s + first;
     __syncthreads();
-    above = sh[33];
+    before = sh[33];
     return (int)sh[32];
 }
 
-// grid (8 rows' worth of clusters): a cluster a row
-__global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(CUT) row_cut_kernel(const __grid_constant__ VerifyArgs a) {
+// a row's logits, every thread its share of them
+template <class F>
+__device__ __forceinline__ void each_logit(const float* x, int V, F f) {
+    const int shift = quad_shift(x), quads = (V + shift + 3) / 4;
+#pragma unroll 4
+    for (int k = threadIdx.x; k < quads; k += CUT) {
+        const int i = 4 * k - shift;
+        if (i >= 0 && i + 3 < V) {
+            const float4 v = ld4(x + i);
+            f(v.x), f(v.y), f(v.z), f(v.w);
+        } else {
+            for (int j = max(i, 0); j < min(i + 4, V); ++j) f(x[j]);
+        }
+    }
+}
+
+// The smallest ordered logit that is kept, by its bits.  h: a table of 2048.
+__device__ __noinline__ uint32_t slow_cut(const float* x, int V, float top, const Heat heat, int k, bool by_count, bool by_mass, float share, unsigned long long* h, unsigned long long* sh) {
+    const int tid = threadIdx.x;
+    uint32_t least = 0;                                     // keys from here on are kept
+    for (int pass = 0; pass < 2; ++pass) {
+        if (pass == 0 ? !by_count : !by_mass) continue;
+        uint32_t prefix = 0;
+        unsigned long long want = (unsigned long long)k;
+        for (int level = 0; level < 3; ++level) {
+            const int bits = level < 2 ? 11 : 10, shift = level == 0 ? 21 : level == 1 ? 10 : 0;
+            __syncthreads();
+            h[tid] = h[tid + 1024] = 0;
+            __syncthreads();
+            each_logit(x, V, [&](float z) {
+                const uint32_t key = order_key(z);
+                if (key < least || (level > 0 && (key >> (shift + bits)) != prefix)) return;
+                unsigned long long add = 1;
+                if (pass == 1) add = (unsigned long long)__float2uint_rn(heat(z, top) * 0x1p31f);
+                if (add) atomicAdd(h + ((key >> shift) & ((1u << bits) - 1)), add);
+            });
+            __syncthreads();
+            const unsigned long long b0 = h[2 * tid], b1 = h[2 * tid + 1];
+            if (pass == 1 && level == 0) {
+                const double t = ceil((double)share * (double)block_total(b0 + b1, sh));
+                want = t >= 1.0 ? (unsigned long long)t : 1ull;
+            }
+            unsigned long long over;
+            const int bin = find_bin<true>(b0, b1, want, over, sh);
+            want -= over;
+            prefix = level == 0 ? (uint32_t)bin : (prefix << bits) | (uint32_t)bin;
+        }
+        least = prefix;
+    }
+    return least;
+}
+
+// grid (rows)
+__global__ void __launch_bounds__(CUT, 1) row_cut_kernel(const __grid_constant__ VerifyArgs a) {
     chain_enter();
-    __shared__ unsigned long long hist[2][2048];
+    __shared__ __align__(16) unsigned h32[2 * BINS * 2];    // bins: counts, coarse and fine masses; or the slow way's table
     __shared__ unsigned long long sh[34];
+    __shared__ unsigned list[LIST], many, next, cut_key;
     __shared__ Row row_sh;
-    cg::cluster_group cl = cg::this_cluster();
-    const int row = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER, tid = threadIdx.x;
+    const int row = blockIdx.x, tid = threadIdx.x;
     const int e = entry_of<CUT>(a, row);
-    if (e >= a.B) return;                                   // (the whole cluster alike, here and below)
+    if (e >= a.B) return;
     const int k = a.top_k ? a.top_k[e] : 0;
     const float share = a.top_p ? a.top_p[e] : 1.f, T = a.temp[e];
-    const bool by_count = k > 0 && k < a.V, by_mass = share < 1.f;
+    bool by_count = k > 0 && k < a.V;
+    const bool by_mass = share < 1.f;
     if (!(T > 0.f) || !(by_count || by_mass)) {
-        if (rank == 0 && tid == 0) a.cut[row] = Cut{0.0, 0.f, 0};
+        if (tid == 0) a.cut[row] = Cut{0.0, 0.f, 0};
         return;
     }
     const Heat heat(T);
+    for (int i = tid; i < 3 * BINS; i += CUT) h32[i] = 0;
     if (tid < 32) {
         const Row r = whole_row(a, heat, row);
-        if (tid == 0) row_sh = r;
+        if (tid == 0) row_sh = r, many = 0, next = 0, cut_key = 0;
     }
     __syncthreads();
     const Row r = row_sh;
     if (r.none()) {
-        if (rank == 0 && tid == 0) a.cut[row] = Cut{0.0, 0.f, 0};
+        if (tid == 0) a.cut[row] = Cut{0.0, 0.f, 0};
         return;
     }
-    const int share_v = (a.V + CLUSTER - 1) / CLUSTER, lo = min(a.V, rank * share_v), hi = min(a.V, lo + share_v);
     const float* x = a.x + row * a.ld;
-    int buf = 0;
-    uint32_t least = 0;                                     // keys from here on are kept
+    const float width = (float)BINS / (32.f * fmaxf(T, 1.f));
+    auto bin_of = [&](float z) { return (int)fminf((r.max - z) * width, (float)(BINS - 1)); };
+    // ---- counts, and masses where they are needed: with top_k, of few logits later ----
+    int finite = 0;
+    each_logit(x, a.V, [&](float z) {
+        const int b = bin_of(z);
+        finite += z > -INFINITY;
+        if (b == BINS - 1) return;                          // (the last bin has what the others have not; its masses are below 2^-34)
+        atomicAdd(h32 + b, 1u);
+        if (!by_count) {
+            const float w = heat(z, r.max) * 65536.f, c = floorf(w);
+            const unsigned f = __float2uint_rn((w - c) * 131072.f);      // (32768 of either fit 32 bits)
+            if (c > 0.f) atomicAdd(h32 + BINS + b, (unsigned)c);
+            if (f) atomicAdd(h32 + 2 * BINS + b, f);
+        }
+    });
+    if (by_count && (unsigned long long)k >= block_total((unsigned long long)finite, sh)) {      // (all but minus infinities are kept)
+        by_count = false;
+        if (!by_mass) {
+            if (tid == 0) a.cut[row] = Cut{0.0, 0.f, 0};
+            return;
+        }
+        each_logit(x, a.V, [&](float z) {
+            const int b = bin_of(z);
+            if (b == BINS - 1) return;
+            const float w = heat(z, r.max) * 65536.f, c = floorf(w);
+            const unsigned f = __float2uint_rn((w - c) * 131072.f);
+            if (c > 0.f) atomicAdd(h32 + BINS + b, (unsigned)c);
+            if (f) atomicAdd(h32 + 2 * BINS + b, f);
+        });
+    }
+    __syncthreads();
+    const int b0 = 2 * tid, b1 = b0 + 1;
+    unsigned long long c0 = h32[b0], c1 = h32[b1];
+    if (c0 > 32768 || c1 > 32768) many = 1;
+    const unsigned long long in_all = block_total(c0 + c1, sh);
+    if (b1 == BINS - 1) c1 = a.V - in_all;
+    unsigned long long want, before, all_mass = 0;
+    int b;
+    if (by_count) {
+        want = (unsigned long long)k;
+        b = find_bin<false>(c0, c1, want, before, sh);
+    } else {
+        const unsigned long long m0 = ((unsigned long long)h32[BINS + b0] << 17) + h32[2 * BINS + b0], m1 = ((unsigned long long)h32[BINS + b1] << 17) + h32[2 * BINS + b1];
+        all_mass = block_total(m0 + m1, sh);
+        const double t = ceil((double)share * (double)all_mass);
+        want = t >= 1.0 ? (unsigned long long)t : 1ull;
+        b = find_bin<false>(m0, m1, want, before, sh);
+    }
+    // the logits of this bin and of those before it, sorted; or, where top_p is all there is, of this bin alone
+    unsigned n = (unsigned)min(block_total((b0 <= b ? c0 : 0ull) + (b1 <= b ? c1 : 0ull), sh), (unsigned long long)LIST + 1);
+    const bool alone = n > LIST && !by_count;
+    if (alone) n = (unsigned)min(block_total((b0 == b ? c0 : 0ull) + (b1 == b ? c1 : 0ull), sh), (unsigned long long)LIST + 1);
+    uint32_t least;
     double total = 0.0;
-    for (int pass = 0; pass < 2; ++pass) {
-        if (pass == 0 ? !by_count : !by_mass) continue;
-        uint32_t prefix = 0;
-        unsigned long long want = (unsigned long long)k, above = 0;
-        for (int level = 0; level < 3; ++level) {
-            const int bits = level < 2 ? 11 : 10, shift = level == 0 ? 21 : level == 1 ? 10 : 0;
-            unsigned long long* h = hist[buf];
-            h[tid] = h[tid + 1024] = 0;
-            __syncthreads();
-            for (int i = lo + tid; i < hi; i += CUT) {
-                const float z = x[i];
-                const uint32_t key = order_key(z);
-                if (key < least || (level > 0 && (key >> (shift + bits)) != prefix)) continue;
-                unsigned long long add = 1;
-                if (pass == 1) add = (unsigned long long)__float2uint_rn(heat(z, r.max) * 0x1p31f);
-                if (add) atomicAdd(h + ((key >> shift) & ((1u << bits) - 1)), add);
+    if (n > LIST || many) {
+        __syncthreads();
+        least = slow_cut(x, a.V, r.max, heat, k, by_count, by_mass, share, reinterpret_cast<unsigned long long*>(h32), sh);
+        each_logit(x, a.V, [&](float z) {
+            if (order_key(z) >= least) total += (double)heat(z, r.max);
+        });
+    } else {
+        each_logit(x, a.V, [&](float z) {
+            const int at = bin_of(z);
+            if (alone ? at == b : at <= b) list[atomicAdd(&next, 1u)] = order_key(z);
+        });
+        __syncthreads();
+        int size = 32;
+        while (size < (int)n) size <<= 1;
+        for (int i = (int)n + tid; i < size; i += CUT) list[i] = 0;
+        __syncthreads();
+        for (int run = 2; run <= size; run <<= 1)           // bitonic, the largest first
+            for (int step = run >> 1; step > 0; step >>= 1) {
+                if (tid < size / 2) {
+                    const int at = 2 * step * (tid / step) + tid % step, to = at + step;
+                    const unsigned u = list[at], v = list[to];
+                    if ((u < v) == ((at & run) == 0)) list[at] = v, list[to] = u;
+                }
+                __syncthreads();
             }
-            cl.sync();
-            unsigned long long b0 = 0, b1 = 0;              // every CTA adds all eight up for itself: whole numbers, the same sums everywhere
-            for (int c = 0; c < CLUSTER; ++c) {
-                const unsigned long long* o = cl.map_shared_rank(h, c);
-                b0 += o[2 * tid], b1 += o[2 * tid + 1];
-            }
-            if (pass == 1 && level == 0) {
-                unsigned long long all = b0 + b1;
+        least = by_count ? list[k - 1] : 0;
+        double w[2];                                        // two neighbours a thread, of those that top_k leaves
+        uint32_t key[2];
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-                __syncthreads();
-                if ((tid & 31) == 0) sh[tid >> 5] = all;
-                __syncthreads();
-                all = 0;
-                for (int w = 0; w < CUT / 32; ++w) all += sh[w];
-                const double t = ceil((double)share * (double)all);
-                want = t >= 1.0 ? (unsigned long long)t : 1ull;
-            }
-            unsigned long long over;
-            const int bin = find_bin(b0, b1, want, over, sh);
-            want -= over, above += over;
-            prefix = level == 0 ? (uint32_t)bin : (prefix << bits) | (uint32_t)bin;
-            if (pass == 1 && level == 2) {                  // (the bin is one value: what it holds is kept)
-                __syncthreads();
-                if (tid == bin >> 1) sh[32] = above + (bin & 1 ? b1 : b0);
-                __syncthreads();
-                total = (double)sh[32] * 0x1p-31;
-            }
-            buf ^= 1;
+        for (int i = 0; i < 2; ++i) {
+            key[i] = 2 * tid + i < size ? list[2 * tid + i] : 0;
+            w[i] = key[i] > 0 && key[i] >= least ? (double)heat(key_value(key[i]), r.max) : 0.0;
         }
-        least = prefix;
-    }
-    // (without top_p: the sum of the k largest, in the order of the places)
-    if (!by_mass) {
-        double s = 0.0;
-        for (int i = lo + tid; i < hi; i += CUT)
-            if (order_key(x[i]) >= least) s += (double)heat(x[i], r.max);
-        s = warp_sum(s);
-        double* d = reinterpret_cast<double*>(sh);
-        __syncthreads();
-        if ((tid & 31) == 0) d[tid >> 5] = s;
-        __syncthreads();
-        if (tid == 0) {
-            s = 0.0;
-            for (int w = 0; w < CUT / 32; ++w) s += d[w];
-            d[32] = s;
+        double* const d = reinterpret_cast<double*>(sh);
+        if (by_mass) {
+            const double all = by_count ? block_total(w[0] + w[1], d) : (double)all_mass * 0x1p-33, goal = (double)share * all;
+            const double up = block_before<double, false>(w[0] + w[1], d) + (alone ? (double)before * 0x1p-33 : 0.0);
+            // the last one with less than the goal before it (the largest always)
+            uint32_t last = tid == 0 ? key[0] : 0xffffffffu;
+            if (w[0] > 0.0 && up < goal) last = key[0];
+            if (w[1] > 0.0 && up + w[0] < goal) last = key[1];
+            last = __reduce_min_sync(0xffffffffu, last);
+            if ((tid & 31) == 0 && last != 0xffffffffu) atomicMax(&cut_key, ~last);
+            __syncthreads();
+            least = max(least, ~cut_key);
         }
-        cl.sync();
-        if (rank == 0 && tid == 0)
-            for (int c = 0; c < CLUSTER; ++c) total += *cl.map_shared_rank(d + 32, c);
+        total = (key[0] >= least ? w[0] : 0.0) + (key[1] >= least ? w[1] : 0.0);
+        if (alone) {
+            total = 0.0;
+            each_logit(x, a.V, [&](float z) {
+                if (order_key(z) >= least) total += (double)heat(z, r.max);
+            });
+        }
     }
-    if (rank == 0 && tid == 0) a.cut[row] = Cut{total, key_value(least), 1};
-    cl.sync();                                              // nobody's tables go while they are read
+    total = block_total(total, reinterpret_cast<double*>(sh));
+    if (tid == 0) a.cut[row] = Cut{total, key_value(least), 1};
 }
 
 // grid: a cluster an entry
 __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_kernel(const __grid_constant__ VerifyArgs a) {
     chain_enter();
-    __shared__ double tile_sum[MAX_TILES], scan[PICK], warp_part[PICK / 32], cta_sum;
+    constexpr int WARPS = PICK / 32, ROWS = 32;
+    __shared__ double part[MAX_TILES][WARPS], tile_sum[MAX_TILES], scan[PICK], warp_part[WARPS], cta_sum;
     __shared__ int first_bad, found, last_some;
-    __shared__ Row row_sh;
+    __shared__ Row rows_sh[ROWS], row_sh;
     cg::cluster_group cl = cg::this_cluster();
     const int e = blockIdx.x / CLUSTER, rank = blockIdx.x % CLUSTER, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int s0 = a.start[e], s1 = a.start[e + 1];
+    const float T = a.temp[e], u_e = a.sample_u[e];
     if (s0 < 0 || s1 < s0 || s1 > a.R || s0 == s1) {        // no rows, or no list of rows (the whole cluster alike)
         if (rank == 0 && tid == 0) {
             a.accepted[e] = 0;
@@ -317,32 +440,37 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_ker
         return;
     }
     const int n = s1 - s0 - 1;
-    const float T = a.temp[e];
     const bool greedy = !(T > 0.f);
     const Heat heat(greedy ? 1.f : T);
     if (tid == 0) first_bad = n;
     __syncthreads();
-    for (int i = warp; i < n; i += PICK / 32) {
-        const int row = s0 + i, x = a.drafts[row];
+    for (int i = warp; i <= n; i += WARPS) {
+        const int row = s0 + i, x = i < n ? a.drafts[row] : 0;
+        const bool in = x >= 0 && x < a.V;
+        float z = 0.f, u = 0.f, q = 1.f;
+        if (i < n && in && !greedy) {      // (asked for beside the slices)
+            z = a.x[row * a.ld + x], u = a.accept_u[row];
+            if (a.q) q = a.q[row * a.ldq + x];
+        }
         const Row r = whole_row(a, heat, row);
         if (lane == 0) {
+            if (i < ROWS) rows_sh[i] = r;
             bool fine = false;
-            if (x < 0 || x >= a.V) atomicOr(a.err, ERR_TOKEN);
+            if (!in) atomicOr(a.err, ERR_TOKEN);
             else if (!r.none()) {
                 if (greedy) fine = x == r.at;
                 else {
-                    const float z = a.x[row * a.ld + x];
                     double w = (double)heat(z, r.max), sum = r.sum;
                     if (a.cut && a.cut[row].on) sum = a.cut[row].total, w = z >= a.cut[row].least ? w : 0.0;
-                    fine = (double)a.accept_u[row] * (a.q ? (double)a.q[row * a.ldq + x] : 1.0) < w / sum;
+                    fine = (double)u * (double)q < w / sum;
                 }
             }
-            if (!fine) atomicMin(&first_bad, i);
+            if (!fine && i < n) atomicMin(&first_bad, i);
         }
     }
     __syncthreads();
     const int acc = first_bad, row = s0 + acc;
-    if (warp == 0) {
+    if (acc >= ROWS && warp == 0) {
         const Row r = whole_row(a, heat, row);
         if (lane == 0) row_sh = r;
     }
@@ -351,8 +479,8 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_ker
             if (i != acc) a.tokens[s0 + i] = i < acc ? a.drafts[s0 + i] : -1;
         if (tid == 0) a.accepted[e] = acc;
     }
-    __syncthreads();
-    const Row r = row_sh;
+    if (acc >= ROWS) __syncthreads();
+    const Row r = acc < ROWS ? rows_sh[acc] : row_sh;
     if (r.none() || greedy) {
         if (rank == 0 && tid == 0) a.tokens[row] = r.none() ? -1 : r.at;
         return;
@@ -360,7 +488,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_ker
     double sum = r.sum;
     float least = -INFINITY;
     if (a.cut && a.cut[row].on) sum = a.cut[row].total, least = a.cut[row].least;
-    const double inv = 1.0 / sum;
+    const float inv = (float)(1.0 / sum);
     const float* x = a.x + row * a.ld;
     const float* q = a.q ? a.q + row * a.ldq : nullptr;
     const int drafted = a.drafts[row], shift = quad_shift(x);
@@ -368,40 +496,40 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_ker
     const int tiles_all = ((a.V + shift + 3) / 4 + PICK - 1) / PICK, per = (tiles_all + CLUSTER - 1) / CLUSTER;
     const int t0 = min(tiles_all, rank * per), t1 = min(tiles_all, t0 + per);
     bool rest = acc < n;
-    // weights of the four logits of quad k of tile t
-    auto weights = [&](int t, double (&w)[4]) {
+    // the weights of the four logits of a tile that are this thread's
+    auto weights = [&](int t, float (&w)[4]) {
         const int i = 4 * (t * PICK + tid) - shift;
         const float4 z4 = quad(x, i, a.V, -INFINITY);
-        const float z[4] = {z4.x, z4.y, z4.z, z4.w};
         float4 q4 = make_float4(0.f, 0.f, 0.f, 0.f);
         if (rest && q) {
             if (aligned_q) q4 = quad(q, i, a.V, 0.f);
             else q4 = make_float4(i >= 0 && i < a.V ? q[i] : 0.f, i + 1 >= 0 && i + 1 < a.V ? q[i + 1] : 0.f, i + 2 >= 0 && i + 2 < a.V ? q[i + 2] : 0.f,
                                   i + 3 >= 0 && i + 3 < a.V ? q[i + 3] : 0.f);
         }
-        const float qv[4] = {q4.x, q4.y, q4.z, q4.w};
+        const float z[4] = {z4.x, z4.y, z4.z, z4.w}, qv[4] = {q4.x, q4.y, q4.z, q4.w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            double p = z[j] >= least ? (double)heat(z[j], r.max) * inv : 0.0;
-            if (rest) p -= q ? (double)qv[j] : (i + j == drafted ? 1.0 : 0.0);
-            w[j] = p > 0.0 ? p : 0.0;
+            float p = z[j] >= least ? heat(z[j], r.max) * inv : 0.f;
+            if (rest) p -= q ? qv[j] : (i + j == drafted ? 1.f : 0.f);
+            w[j] = fmaxf(p, 0.f);
         }
     };
     double total;
     for (;;) {
+#pragma unroll 4
         for (int t = t0; t < t1; ++t) {
-            double w[4];
+            float w[4];
             weights(t, w);
-            const double s = warp_sum((w[0] + w[1]) + (w[2] + w[3]));
-            if (lane == 0) warp_part[warp] = s;
-            __syncthreads();
-            if (tid == 0) {
-                double y = 0.0;
-                for (int k = 0; k < PICK / 32; ++k) y += warp_part[k];
-                tile_sum[t - t0] = y;
-            }
-            __syncthreads();
+            const double s = warp_sum((double)((w[0] + w[1]) + (w[2] + w[3])));
+            if (lane == 0) part[t - t0][warp] = s;
         }
+        __syncthreads();
+        for (int t = tid; t < t1 - t0; t += PICK) {
+            double y = 0.0;
+            for (int k = 0; k < WARPS; ++k) y += part[t][k];
+            tile_sum[t] = y;
+        }
+        __syncthreads();
         if (tid == 0) {
             double y = 0.0;
             for (int t = t0; t < t1; ++t) y += tile_sum[t - t0];
@@ -414,7 +542,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_ker
         rest = false;                                       // nothing is left of the draft's excess: the target's own probabilities
         cl.sync();
     }
-    const double target = (double)a.sample_u[e] * total;
+    const double target = (double)u_e * total;
     double before = 0.0, base = 0.0;
     int owner = -1;                                         // the CTA in whose share the sum passes the target (rounding: the last that has any)
     for (int c = 0; c < CLUSTER; ++c) {
@@ -436,9 +564,10 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_ker
             }
             before += y;
         }
-        double w[4];
+        float w[4];
         weights(tile, w);
-        double s = (w[0] + w[1]) + (w[2] + w[3]), own = s;
+        const float own = (w[0] + w[1]) + (w[2] + w[3]);
+        double s = (double)own;
         const int i = 4 * (tile * PICK + tid) - shift;
         if (tid == 0) found = 0x7fffffff, last_some = -1;
 #pragma unroll
@@ -452,12 +581,12 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_ker
         scan[tid] = s;
         __syncthreads();
         double cum = base + (tid ? scan[tid - 1] : 0.0);
-        if (own > 0.0) {
+        if (own > 0.f) {
             int last = -1;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                cum += w[j];
-                if (w[j] > 0.0) {
+                cum += (double)w[j];
+                if (w[j] > 0.f) {
                     last = i + j;
                     if (cum > target) {
                         atomicMin(&found, i + j);
@@ -473,11 +602,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_ker
     cl.sync();                                              // nobody's sums go while they are read
 }
 
-int slices_of(int R, int V, int& threads) {
-    // Slices of 16384 logits where they fill the GPU twice, of 4096 otherwise
-    threads = (int64_t)R * ((V + 3 + 16383) / 16384) >= 2 * 148 ? 1024 : 256;
-    return (V + 3 + 16 * threads - 1) / (16 * threads);
-}
+int slices_of(int V) { return (V + 3 + 16 * STATS - 1) / (16 * STATS); }
 
 }  // namespace
 
@@ -489,8 +614,7 @@ extern "C" {
 
 size_t b200seq_verify_scratch_bytes(int R, int V, int ruled) {
     if (R < 1 || V < 1 || V > MAX_V) return 0;
-    int threads;
-    return (size_t)R * slices_of(R, V, threads) * sizeof(Partial) + (ruled ? (size_t)R * sizeof(Cut) : 0);
+    return (size_t)R * slices_of(V) * sizeof(Partial) + (ruled ? (size_t)R * sizeof(Cut) : 0);
 }
 
 int b200seq_verify_drafts(const float* logits, int64_t ld, int R, int V, const int32_t* start, int B, const int32_t* drafts, const float* accept_u, const float* sample_u,
@@ -505,17 +629,15 @@ int b200seq_verify_drafts(const float* logits, int64_t ld, int R, int V, const i
     if (R > 0 && B > 0 && (scratch_bytes < b200seq_verify_scratch_bytes(R, V, ruled) || (reinterpret_cast<uintptr_t>(scratch) & 15)))
         return fail(B200SEQ_ERR_INVALID_ARG, "verify_drafts: the work area is too small or not on a 16-byte boundary");
     if (B == 0) return 0;
-    int threads;
     VerifyArgs a{logits, ld, R, V, B, 0, start, drafts, accept_u, sample_u, temperature, top_k, top_p, draft_probs, ldq, accepted, tokens, (Partial*)scratch, nullptr, error_flag_dev()};
-    a.slices = slices_of(R, V, threads);
+    a.slices = slices_of(V);
     if (ruled) a.cut = reinterpret_cast<Cut*>(a.part + (size_t)R * a.slices);
     const cudaStream_t cs = (cudaStream_t)stream;
     if (R > 0) {
-        if (threads == 1024) launch_chained(row_stats_kernel<1024>, dim3(a.slices, R), 1024, 0, cs, a);
-        else launch_chained(row_stats_kernel<256>, dim3(a.slices, R), 256, 0, cs, a);
+        launch_chained(row_stats_kernel, dim3(a.slices, R), STATS, 0, cs, a);
         SEQ_LAUNCH_CHECK("verify_drafts");
         if (ruled) {
-            launch_chained(row_cut_kernel, dim3(CLUSTER * R), CUT, 0, cs, a);
+            launch_chained(row_cut_kernel, dim3(R), CUT, 0, cs, a);
             SEQ_LAUNCH_CHECK("verify_drafts");
         }
     }
