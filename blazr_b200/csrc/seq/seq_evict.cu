@@ -4,8 +4,10 @@
 // order, to the places 0 .. keep - 1.  The choice needs the weights alone: a block selects the smallest weight that stays by the bits of the ordered floats, eleven at a time, and
 // writes the list of rows.  Moving is bound by the memory: every kept row is read and written once (keys, values, f32 or 4-bit codes with their parameters).
 //
-// A row never moves to a higher place.  So a block that walks over its rows (of one head, of a slice of their bytes) in chunks, all of a chunk read before any of it is written,
-// may write into the pages that it reads: what it overwrites has been read, and nobody else touches these bytes.  That is what lets a cache be cut back where it lies.
+// A row never moves to a higher place.  So whoever walks over a head's rows in chunks, all of a chunk read before any of it is written, may write into the pages that it reads: what
+// it overwrites has been read, and nobody else touches these bytes.  That is what lets a cache be cut back where it lies.  A cluster of up to eight CTAs walks together, each with
+// whole rows of a chunk, and waits for all of them between reading and writing; the next chunks are on their way by then.  Two sequences of 32768 rows to 16384, 8 heads of 128,
+// four layers: 370 us of moving, 5.8 TB/s.  (Pages and kept rows in any order take the same time: what it cost before were instructions for addresses.)
 #include "seq_kv4.cuh"
 
 namespace b200seq {
@@ -13,9 +15,12 @@ namespace b200seq {
 namespace {
 
 constexpr int LAYERS = 32;                // of one launch
-constexpr int CHOOSE = 512;               // threads that choose
-constexpr int EACH = 8;                   // neighbouring weights a thread lists at a time
+constexpr int EACH = 8;                   // weights a thread lists at a time
+constexpr int HELD = 49152;               // weights that a block has in shared memory; longer rows are read four times
 constexpr int MOVE = 256;                 // threads that move
+// Pieces of a chunk a thread has, chunks on their way, rows looked up at a time.  Small ones, so that many CTAs share an SM: eight sequences of 2301 rows in 16 layers of 4-bit pages 143 us
+// (4, 4, 1024: 175), two of 32768 in four layers of f32 pages 410 (406)
+constexpr int ITEMS = 2, STAGES = 2, BATCH = 512;
 
 struct EvictArgs {
     uint8_t* pool[2][LAYERS];
@@ -25,8 +30,6 @@ struct EvictArgs {
     int64_t acc_ld;
     int layers, B, G, bs, mb, to_mb, slots, keep, first, recent;
     int units[2];                         // pieces of a row: keys, values
-    int per[2];                           // pieces of a row that a block takes
-    int slices;                           // blocks that share a head's rows
     int ng[2];                            // 4-bit pools: groups of a row
     int* err;
 };
@@ -49,44 +52,54 @@ __device__ __forceinline__ void entry_rows(const EvictArgs& a, int e, int& n, in
     kept = n < a.keep ? n : a.keep;
 }
 
-// grid (key heads, entries, layers)
-__global__ void __launch_bounds__(CHOOSE) evict_choose_kernel(const __grid_constant__ EvictArgs a) {
+// grid (key heads, entries, layers).  Dynamic shared memory: as many weights as a slot has room for, or HELD
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) evict_choose_kernel(const __grid_constant__ EvictArgs a) {
     chain_enter();
-    constexpr int WARPS = CHOOSE / 32;
+    constexpr int WARPS = THREADS / 32, PER = 2048 / THREADS;
+    extern __shared__ __align__(16) float held[];
     __shared__ unsigned hist[2048], wsum[WARPS], found[2];
-    __shared__ uint2 tsum[WARPS];
+    __shared__ uint2 tsum[2][WARPS];
     const int g = blockIdx.x, e = blockIdx.y, l = blockIdx.z, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int n, kept;
     entry_rows(a, e, n, kept, tid == 0 && g == 0 && l == 0);
     int32_t* list = a.kept + (((int64_t)l * a.B + e) * a.G + g) * a.keep;
-    for (int i = kept + tid; i < a.keep; i += CHOOSE) list[i] = -1;
+    for (int i = kept + tid; i < a.keep; i += THREADS) list[i] = -1;
     if (n == 0) return;
     const float* w = a.acc[l] + ((int64_t)a.slot[e] * a.G + g) * a.acc_ld;
     float* to = a.acc[l] + ((int64_t)a.to_slot[e] * a.G + g) * a.acc_ld;
     if (n <= a.keep) {
-        for (int i = tid; i < n; i += CHOOSE) {
+        for (int i = tid; i < n; i += THREADS) {
             list[i] = i;
             if (to != w) to[i] = w[i];
         }
         return;
     }
+    const bool here = n <= HELD;
+    if (here) {
+#pragma unroll 8
+        for (int i = tid; i < n; i += THREADS) held[i] = w[i];
+    }
+    const float* src = here ? held : w;
     const int lo = a.first, hi = n - a.recent;              // the rows between: more than are chosen of them
     unsigned least = 0xffffffffu, ties = 0;                 // keys above stay, and the first `ties` equal ones
     if (a.keep > a.first + a.recent) {
         unsigned want = (unsigned)(a.keep - a.first - a.recent), prefix = 0;
         for (int level = 0; level < 3; ++level) {
             const int bits = level < 2 ? 11 : 10, shift = level == 0 ? 21 : level == 1 ? 10 : 0;
-            for (int i = tid; i < 2048; i += CHOOSE) hist[i] = 0;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) hist[tid + i * THREADS] = 0;
             __syncthreads();
-            for (int i = lo + tid; i < hi; i += CHOOSE) {
-                const unsigned k = weight_key(w[i]);
+#pragma unroll 8
+            for (int i = lo + tid; i < hi; i += THREADS) {
+                const unsigned k = weight_key(src[i]);
                 if (level == 0 || (k >> (shift + bits)) == prefix) atomicAdd(hist + ((k >> shift) & ((1u << bits) - 1)), 1u);
             }
             __syncthreads();
-            // bins 4 t .. 4 t + 3 of thread t, added up from the top
-            unsigned b[4], s = 0;
+            // bins PER t .. of thread t, added up from the top
+            unsigned b[PER], s = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = hist[4 * tid + j], s += b[j];
+            for (int j = 0; j < PER; ++j) b[j] = hist[PER * tid + j], s += b[j];
             unsigned up = s;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -95,151 +108,211 @@ __global__ void __launch_bounds__(CHOOSE) evict_choose_kernel(const __grid_const
             }
             if (lane == 0) wsum[warp] = up;
             __syncthreads();
-            for (int k = warp + 1; k < WARPS; ++k) up += wsum[k];
             unsigned over = up - s;
+            for (int k = warp + 1; k < WARPS; ++k) over += wsum[k];
 #pragma unroll
-            for (int j = 3; j >= 0; --j) {
-                if (over < want && over + b[j] >= want) found[0] = 4 * tid + j, found[1] = over;
+            for (int j = PER - 1; j >= 0; --j) {
+                if (over < want && over + b[j] >= want) found[0] = PER * tid + j, found[1] = over;
                 over += b[j];
             }
             __syncthreads();
             prefix = level == 0 ? found[0] : (prefix << bits) | found[0];
             want -= found[1];
-            __syncthreads();
         }
         least = prefix, ties = want;
     }
+    __syncthreads();                                        // (the weights have been read, and held ones are in place)
     // the list, in order: a tile of rows at a time, all of it read before its places are written
-    unsigned at = 0, equal = 0;
-    for (int t0 = 0; t0 < n; t0 += CHOOSE * EACH) {
+    unsigned at = 0, equal = 0;                             // of the tiles before: rows that stay whatever their rank, rows of weight `least`
+    int buf = 0;
+    for (int t0 = 0; t0 < n; t0 += THREADS * EACH, buf ^= 1) {
+        // a warp has EACH * 32 neighbouring rows, 32 of them at a time: what stays of those goes to neighbouring places
         float x[EACH];
-        bool stay[EACH], eq[EACH];
-        unsigned above = 0, same = 0;
+        unsigned stay[EACH], eq[EACH], above = 0, same = 0;
+        const int i0 = t0 + warp * (EACH * 32) + lane;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) x[j] = i0 + 32 * j < n ? src[i0 + 32 * j] : 0.f;
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
-            const int i = t0 + tid * EACH + j;
-            x[j] = i < n ? w[i] : 0.f;
+            const int i = i0 + 32 * j;
             const unsigned k = weight_key(x[j]);
             const bool mid = i >= lo && i < hi;
-            stay[j] = i < n && (!mid || k > least), eq[j] = mid && k == least;
-            above += stay[j], same += eq[j];
+            stay[j] = __ballot_sync(0xffffffffu, i < n && (!mid || k > least)), eq[j] = __ballot_sync(0xffffffffu, mid && k == least);
+            above += __popc(stay[j]), same += __popc(eq[j]);
         }
-        uint2 s = make_uint2(above, same);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const unsigned y = __shfl_up_sync(0xffffffffu, s.x, o), z = __shfl_up_sync(0xffffffffu, s.y, o);
-            if (lane >= o) s.x += y, s.y += z;
-        }
-        if (lane == 31) tsum[warp] = s;
+        if (lane == 0) tsum[buf][warp] = make_uint2(above, same);
         __syncthreads();
         uint2 before = make_uint2(0, 0), all = make_uint2(0, 0);
         for (int k = 0; k < WARPS; ++k) {
-            const uint2 y = tsum[k];
+            const uint2 y = tsum[buf][k];
             if (k < warp) before.x += y.x, before.y += y.y;
             all.x += y.x, all.y += y.y;
         }
         // rows of equal weight stay while there is room for them: `ties` of the entry's
-        unsigned eqs = equal + before.y + s.y - same, place = at + before.x + s.x - above + min(eqs, ties);
+        unsigned over = at + before.x, eqs = equal + before.y;
+        const unsigned below = (1u << lane) - 1u;
 #pragma unroll
         for (int j = 0; j < EACH; ++j) {
-            const bool in = stay[j] || (eq[j] && eqs < ties);
-            if (in) {
-                list[place] = t0 + tid * EACH + j;
+            const unsigned my = eqs + __popc(eq[j] & below);
+            if (((stay[j] >> lane) & 1u) || (((eq[j] >> lane) & 1u) && my < ties)) {
+                const unsigned place = over + __popc(stay[j] & below) + min(my, ties);
+                list[place] = i0 + 32 * j;
                 to[place] = x[j];
-                ++place;
             }
-            eqs += eq[j];
+            over += __popc(stay[j]), eqs += __popc(eq[j]);
         }
         at += all.x, equal += all.y;
-        // (`at` counts the rows above; equal ones that stay are in `place` through eqs)
-        __syncthreads();
     }
+}
+
+// Where a row begins in a pool.  f32: pieces of sizeof(V) of rows [page][row][head]; 4 bits: five pieces of 4 NG bytes, four of codes, and one of parameters `params` further on
+struct RowAt {
+    int64_t at;
+    int params;
+};
+template <class V, bool FOUR>
+__device__ __forceinline__ RowAt row_at(const EvictArgs& a, int kv, int page, int o, int g) {
+    if (FOUR) {
+        const Kv4Row r = kv4_row(page, o, a.bs, g, a.G, a.ng[kv]);
+        return RowAt{r.codes, (int)(r.params - r.codes)};
+    }
+    return RowAt{(((int64_t)page * a.bs + o) * a.G + g) * (a.units[kv] * (int64_t)sizeof(V)), 0};
 }
 
 template <class V>
-__device__ __forceinline__ V load_piece(const uint8_t* p) { return *reinterpret_cast<const V*>(p); }
-
-// where piece u of row o of page p of head g begins.  f32: pieces of sizeof(V) of rows [page][row][head]; 4 bits: five pieces of 4 NG bytes, four of codes, one of parameters
-template <class V, bool FOUR>
-__device__ __forceinline__ int64_t piece_at(const EvictArgs& a, int kv, int page, int o, int g, int u) {
-    if (FOUR) {
-        const Kv4Row r = kv4_row(page, o, a.bs, g, a.G, a.ng[kv]);
-        return u < 4 ? r.codes + u * 4 * a.ng[kv] : r.params;
-    }
-    return ((((int64_t)page * a.bs + o) * a.G + g) * a.units[kv] + u) * (int64_t)sizeof(V);
+__device__ __forceinline__ void copy_in(V* dst, const uint8_t* src) {
+    const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+    if (sizeof(V) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(sizeof(V)) : "memory");
 }
 
-// grid (slices of a row, entries * key heads, layers): one block moves its pieces of all rows, in chunks
-template <class V, bool FOUR>
-__global__ void __launch_bounds__(MOVE) evict_move_kernel(const __grid_constant__ EvictArgs a, int kv) {
+// grid (cluster, entries * key heads, layers [* keys and values]).  BOTH: keys and values are of one size
+template <class V, bool FOUR, bool BOTH>
+__global__ void __launch_bounds__(MOVE) evict_move_kernel(const __grid_constant__ EvictArgs a, int which) {
     chain_enter();
-    constexpr int ITEMS = 4, SPAN = MOVE * ITEMS, ROWS = SPAN / 2;
-    // (page, row of the page) of a chunk's rows; page < 0: the row stays where it is.  Three of each: the next chunk's are looked up while slower warps still write the last one.
-    __shared__ int2 from[3][ROWS], dest[3][ROWS];
-    const int u0 = blockIdx.x * a.per[kv], per = min(a.per[kv], a.units[kv] - u0), e = blockIdx.y / a.G, g = blockIdx.y - e * a.G, l = blockIdx.z, tid = threadIdx.x;
-    if (per <= 0) return;
+    constexpr int SPAN = MOVE * ITEMS;
+    extern __shared__ __align__(16) uint8_t ring_raw[];
+    V* const ring = reinterpret_cast<V*>(ring_raw);
+    // Where the rows of two batches lie and go (from < 0: the row stays where it is).  Looked up a batch ahead, four chunks or more: the chain list, page takes as long as two of
+    // them; and as addresses, since made again for every piece they were what the kernel spent its time on (2.3 us a chunk of 16 KB, whatever the rows' order)
+    __shared__ int64_t from[2 * BATCH], dest[2 * BATCH];
+    __shared__ int from_par[FOUR ? 2 * BATCH : 1], dest_par[FOUR ? 2 * BATCH : 1];
+    const int kv = BOTH ? (int)blockIdx.z & 1 : which, l = BOTH ? (int)blockIdx.z >> 1 : blockIdx.z;
+    const int per = a.units[kv], e = blockIdx.y / a.G, g = blockIdx.y - e * a.G, tid = threadIdx.x, rank = blockIdx.x, ranks = gridDim.x;
     int n, kept;
     entry_rows(a, e, n, kept, false);
     const int32_t* list = a.kept + (((int64_t)l * a.B + e) * a.G + g) * a.keep;
     const int32_t *bt = a.bt + (int64_t)e * a.mb, *to = a.to_bt + (int64_t)e * a.to_mb;
     uint8_t* pool = a.pool[kv][l];
-    const int rows = min(SPAN / per, ROWS);                 // of a chunk
-    auto look = [&](int r0, int b) {
-        for (int i = tid; i < rows && r0 + i < kept; i += MOVE) {
-            const int src = list[r0 + i], dst = r0 + i;
+    // a chunk is `rows` rows of every CTA of the cluster, a batch K chunks; rows of more than SPAN pieces go in several runs over them
+    const int span = min(per, SPAN), rows = min(SPAN / span, BATCH / STAGES), K = BATCH / rows, step = rows * ranks;
+    auto look = [&](int batch, int at) {
+        for (int i = tid; i < K * rows; i += MOVE) {
+            const int c = i / rows, dst = (batch * K + c) * step + rank * rows + i - c * rows;
+            if (dst >= kept) continue;
+            const int src = list[dst];
             int sp = -1, dp = -1;
             if (src >= 0 && src < n) {
                 sp = bt[src / a.bs], dp = to[dst / a.bs];
                 if (sp < 0 || dp < 0) {
-                    if (l == 0 && kv == 0 && blockIdx.x == 0) atomicOr(a.err, 1);
+                    if (l == 0 && kv == 0) atomicOr(a.err, 1);
                     sp = -1;
                 }
             }
-            if (sp == dp && src == dst) sp = -1;
-            from[b][i] = make_int2(sp, src % a.bs), dest[b][i] = make_int2(dp, dst % a.bs);
+            const RowAt f = row_at<V, FOUR>(a, kv, max(sp, 0), src < 0 ? 0 : src % a.bs, g), t = row_at<V, FOUR>(a, kv, max(dp, 0), dst % a.bs, g);
+            from[at + i] = sp < 0 || f.at == t.at ? -1 : f.at, dest[at + i] = t.at;
+            if (FOUR) from_par[at + i] = f.params, dest_par[at + i] = t.params;
         }
     };
-    look(0, 0);
-    __syncthreads();
-    int b = 0;
-    for (int r0 = 0; r0 < kept; r0 += rows, b = b == 2 ? 0 : b + 1) {
-        const int m = min(rows, kept - r0) * per;
-        V x[ITEMS];
-        bool go[ITEMS];
+    const int chunks = (kept + step - 1) / step;
+    for (int u0 = 0; u0 < per; u0 += span) {
+        int pr[ITEMS], pu[ITEMS];                           // a thread's pieces of a chunk: row, byte (FOUR: piece) of the row
 #pragma unroll
         for (int k = 0; k < ITEMS; ++k) {
             const int i = k * MOVE + tid;
-            go[k] = false;
-            if (i < m) {
-                const int r = i / per, u = u0 + i - r * per;
-                const int2 s = from[b][r];
-                go[k] = s.x >= 0;
-                if (go[k]) x[k] = load_piece<V>(pool + piece_at<V, FOUR>(a, kv, s.x, s.y, g, u));
-            }
+            pr[k] = i / span;
+            const int u = u0 + i - pr[k] * span;
+            if (pr[k] >= rows || u >= per) pr[k] = 0x3fffffff;
+            pu[k] = FOUR && u == 4 ? -1 : u * (int)sizeof(V);
         }
-        if (r0 + rows < kept) look(r0 + rows, b == 2 ? 0 : b + 1);
-        __syncthreads();                                    // all of the chunk has been read
+        // a thread's pieces of a chunk go through its own places of the ring
+        auto load = [&](int at, int left, int stage) {      // at: the chunk's first place in the tables; left: rows from this CTA's first one on
+            V* const to_ring = ring + stage * SPAN + tid;
 #pragma unroll
-        for (int k = 0; k < ITEMS; ++k) {
-            if (!go[k]) continue;
-            const int i = k * MOVE + tid, r = i / per, u = u0 + i - r * per;
-            const int2 d = dest[b][r];
-            *reinterpret_cast<V*>(pool + piece_at<V, FOUR>(a, kv, d.x, d.y, g, u)) = x[k];
+            for (int k = 0; k < ITEMS; ++k) {
+                if (pr[k] >= left) continue;
+                const int64_t f = from[at + pr[k]];
+                if (f >= 0) copy_in(to_ring + k * MOVE, pool + f + (FOUR && pu[k] < 0 ? from_par[at + pr[k]] : pu[k]));
+            }
+        };
+        auto store = [&](int at, int left, int stage) {
+            const V* const of_ring = ring + stage * SPAN + tid;
+#pragma unroll
+            for (int k = 0; k < ITEMS; ++k) {
+                if (pr[k] >= left || from[at + pr[k]] < 0) continue;
+                *reinterpret_cast<V*>(pool + dest[at + pr[k]] + (FOUR && pu[k] < 0 ? dest_par[at + pr[k]] : pu[k])) = of_ring[k * MOVE];
+            }
+        };
+        const int mine = kept - rank * rows;
+        int load_at = 0, store_at = 0, load_stage = 0, store_stage = 0, in_batch = 0, batch = 0;
+        auto load_next = [&](int c) {
+            if (c < chunks) load(load_at, mine - c * step, load_stage);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            load_at += rows, load_stage = load_stage + 1 == STAGES ? 0 : load_stage + 1;
+            if (load_at >= 2 * K * rows) load_at = 0;
+        };
+        __syncthreads();
+        look(0, 0);
+        __syncthreads();
+        for (int c = 0; c < STAGES - 1; ++c) load_next(c);
+        for (int c = 0; c < chunks; ++c) {
+            load_next(c + STAGES - 1);                      // rows from the end of this chunk on: nothing that this one or an earlier one writes
+            // All of this chunk has been read, by all CTAs, before any of it is written.  (No order of memory is asked for but that: the values have arrived, and what is written now is
+            // read by nobody's later load.  With a release there the CTAs would wait for their stores, too.)
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+            asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+            store(store_at, mine - c * step, store_stage);
+            store_at += rows, store_stage = store_stage + 1 == STAGES ? 0 : store_stage + 1;
+            if (store_at >= 2 * K * rows) store_at = 0;
+            if (in_batch == 0) {                            // (whoever wrote by the batch before this one is through)
+                look(batch + 1, (batch + 1) & 1 ? K * rows : 0);
+                __syncthreads();
+            }
+            if (++in_batch == K) in_batch = 0, ++batch;
         }
     }
 }
 
+template <class V, bool FOUR, bool BOTH>
+cudaError_t move_as(const EvictArgs& a, int kv, cudaStream_t cs) {
+    const int64_t heads = (int64_t)a.B * a.G * a.layers * (BOTH ? 2 : 1);
+    // Three CTAs an SM, where a head's rows are enough for so many (128 heads: clusters of 1, 2, 4 took 785, 542, 411 us; 2048 heads: 143, 143, 157)
+    int cluster = 1;
+    while (cluster < 8 && heads * cluster < 3 * 148) cluster *= 2;
+    const int smem = STAGES * MOVE * ITEMS * (int)sizeof(V);
+    const cudaError_t e = cudaFuncSetAttribute(evict_move_kernel<V, FOUR, BOTH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension, attr[1].val.clusterDim.x = cluster, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(cluster, a.B * a.G, a.layers * (BOTH ? 2 : 1)), cfg.blockDim = MOVE, cfg.dynamicSmemBytes = smem, cfg.stream = cs, cfg.attrs = attr, cfg.numAttrs = 2;
+    cudaLaunchKernelEx(&cfg, evict_move_kernel<V, FOUR, BOTH>, a, kv);
+    return cudaGetLastError();
+}
 template <class V, bool FOUR>
-cudaError_t move(EvictArgs& a, int kv, int piece, cudaStream_t cs) {
-    // Blocks walk over their rows one chunk after another, so that the more of them share a row's bytes the sooner they are through: down to 32 bytes of a row each.
-    const int64_t heads = (int64_t)a.B * a.G * a.layers;
-    const int least = piece >= 32 ? 1 : 32 / piece, most = FOUR ? 1 : (a.units[kv] + least - 1) / least;
-    int64_t slices = (4 * 148 + heads - 1) / heads;
-    slices = slices < most ? slices : most;
-    a.per[kv] = FOUR ? a.units[kv] : (int)((a.units[kv] + slices - 1) / slices);
-    if (a.per[kv] > MOVE) a.per[kv] = MOVE;
-    const int blocks = (a.units[kv] + a.per[kv] - 1) / a.per[kv];
-    launch_chained(evict_move_kernel<V, FOUR>, dim3(blocks, a.B * a.G, a.layers), MOVE, 0, cs, a, kv);
+cudaError_t move(const EvictArgs& a, int kv, bool both, cudaStream_t cs) {
+    return both ? move_as<V, FOUR, true>(a, kv, cs) : move_as<V, FOUR, false>(a, kv, cs);
+}
+
+template <int THREADS>
+cudaError_t choose(const EvictArgs& a, cudaStream_t cs) {
+    const int smem = (int)(a.acc_ld < HELD ? (a.acc_ld + 7) / 8 * 8 : HELD) * 4;
+    if (smem > 36 * 1024) {      // (beside the block's own tables)
+        const cudaError_t e = cudaFuncSetAttribute(evict_choose_kernel<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, HELD * 4);
+        if (e != cudaSuccess) return e;
+    }
+    launch_chained(evict_choose_kernel<THREADS>, dim3(a.G, a.B, a.layers), THREADS, smem, cs, a);
     return cudaGetLastError();
 }
 
@@ -275,18 +348,19 @@ extern "C" int b200seq_evict_keys(void* const* kpools, void* const* vpools, floa
         a.kept = kept + (int64_t)l0 * B * G * keep;
         a.slot = slot, a.rows = rows, a.bt = table, a.to_slot = to_slot, a.to_bt = to_table, a.acc_ld = acc_ld;
         a.B = B, a.G = G, a.bs = block_size, a.mb = max_blocks, a.to_mb = to_max_blocks, a.slots = slots, a.keep = keep, a.first = first, a.recent = recent, a.err = error_flag_dev();
-        launch_chained(evict_choose_kernel, dim3(G, B, a.layers), CHOOSE, 0, cs, a);
-        SEQ_LAUNCH_CHECK("evict_keys");
+        // (a slot of up to 8192 weights: eight blocks an SM; more: one or two)
+        cudaError_t err = acc_ld <= 8192 ? choose<256>(a, cs) : choose<1024>(a, cs);
+        if (err != cudaSuccess) return cuda_status(err, "evict_keys");
+        count_launch();
         for (int kv = 0; kv < 2; ++kv) {
             const int size = kv ? V : D;
-            cudaError_t err;
-            if (kv_bits == 4) {
-                a.ng[kv] = kv4_groups(size), a.units[kv] = 5;
-                err = a.ng[kv] == 4 ? move<uint4, true>(a, kv, 16, cs) : a.ng[kv] == 2 ? move<uint2, true>(a, kv, 8, cs) : move<uint32_t, true>(a, kv, 4, cs);
-            } else {
-                a.units[kv] = wide[kv] ? size / 4 : size;
-                err = wide[kv] ? move<uint4, false>(a, kv, 16, cs) : move<uint32_t, false>(a, kv, 4, cs);
-            }
+            if (kv_bits == 4) a.ng[kv] = kv4_groups(size), a.units[kv] = 5;
+            else a.units[kv] = wide[kv] ? size / 4 : size;
+        }
+        const bool both = a.units[0] == a.units[1] && a.ng[0] == a.ng[1] && wide[0] == wide[1];
+        for (int kv = 0; kv < (both ? 1 : 2); ++kv) {
+            if (kv_bits == 4) err = a.ng[kv] == 4 ? move<uint4, true>(a, kv, both, cs) : a.ng[kv] == 2 ? move<uint2, true>(a, kv, both, cs) : move<uint32_t, true>(a, kv, both, cs);
+            else err = wide[kv] ? move<uint4, false>(a, kv, both, cs) : move<uint32_t, false>(a, kv, both, cs);
             if (err != cudaSuccess) return cuda_status(err, "evict_keys");
             count_launch();
         }
