@@ -3,10 +3,11 @@
 // acc[slot][g][j] += sum over the entry's tokens t (all, or its last few) and the query heads h of key head g of  p_thj = exp(z_thj) / (sum_j' exp(z_thj') + exp(sink_h)),
 // z = softcap(scale * head_scale_h * q_th . k_j) over the keys that t sees; a key that the step itself brought gets the sum instead of having it added.
 //
-// Few rows a key head (rows path): bound by the keys' bytes.  A block has 128 keys, a warp 16 of them in registers (8 lanes to a key, so that a product of a row with 16 keys
-// needs four shuffles), and goes through the rows, which lie in shared memory in the lanes' order; f32 multiply-adds.  It leaves 2^(z - its maximum), the maximum and the sum for
-// every row in the work area; a second launch has every row's denominator from the blocks' and adds the weights up, key by key, the rows in their order: no atomics.  The work
-// area's traffic is a row's 4 bytes a key against the key's 4 D bytes.
+// Few rows a key head (rows path): bound by the keys' bytes.  Eight rows are too few for a tcgen05 product of 128: a warp takes eight keys at a time into registers, a lane a quarter of one,
+// splits them there into two f16 parts (k = h + l, l times 2^11) and multiplies with m16n8k16 products, whose rows 0 - 7 are the high parts of eight rows of queries and 8 - 15 their
+// low parts (times 2^11), so that two products a step give all four: 22 bits, at any size of the keys that f16 has.  What has no such parts gives no number and is made again in f32.  The scores
+// go to the work area (4 bytes a row and key against the key's 4 D), with every block's maximum and sum a row; a second launch has every row's denominator from the blocks' and
+// adds the weights up, key by key, the rows in their order: no atomics.
 // Many rows: seq_weigh_tc.cu.  What neither takes (heads above 128 or of odd sizes) goes through f32 tiles here, twice: once for the denominators, once for the sums.
 #include "seq_weigh.cuh"
 #include "tc_split.cuh"
@@ -18,177 +19,260 @@ namespace {
 using tcsplit::ex2;
 
 // ---- rows path ------------------------------------------------------------------------------------------------------------------------------
-constexpr int RT = 256;                // threads
-constexpr int RK = 128;                // keys of a block
-constexpr int RROWS = 32;              // rows in shared memory at a time
+constexpr int RT = 256, RW = RT / 32;  // threads, warps
 constexpr int FT = 256, FK = 4 * FT;   // second launch: threads, keys of a block
+constexpr float LOW = 0x1p11f, UNLOW = 0x1p-11f;
 
-// work area of the rows path: [T][H][blocks][RK] weights relative to the block's maximum, then [T][H][blocks] (maximum, sum)
-__device__ __forceinline__ float* rows_weights(const WeighArgs& a, int64_t row) { return a.part + row * a.key_blocks * RK; }
-__device__ __forceinline__ float2* rows_stats(const WeighArgs& a, int T, int64_t row) {
-    return reinterpret_cast<float2*>(a.part + (int64_t)T * a.H * a.key_blocks * RK) + row * a.key_blocks;
+// work area of the rows path: [T][H][key_room] scores in base 2, then [T][H][key_blocks] (maximum, sum)
+__device__ __forceinline__ float* rows_scores(const WeighArgs& a, int64_t row) { return a.part + row * a.key_room; }
+__device__ __forceinline__ float2* rows_stats(const WeighArgs& a, int T, int64_t row) { return reinterpret_cast<float2*>(a.part + (int64_t)T * a.H * a.key_room) + row * a.key_blocks; }
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+// two values -> f16 pair of their high parts and f16 pair of what is left times 2^11 (low half = a)
+__device__ __forceinline__ void split_up(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    float x, y;
+    tcsplit::upk(tcsplit::mul2(tcsplit::pk(a - f.x, b - f.y), tcsplit::pk(LOW, LOW)), x, y);
+    const __half2 l = __floats2half2_rn(x, y);
+    hi = *reinterpret_cast<const uint32_t*>(&h), lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// grid (blocks of keys, key heads, entries).  VPL: values of a key in a lane (8 lanes to a key); FOUR: 4-bit pages
-template <int VPL, bool FOUR>
-__global__ void __launch_bounds__(RT, 2) weigh_rows_kernel(const __grid_constant__ WeighArgs a, const __grid_constant__ b200seq_step st) {
-    chain_enter();
-    constexpr int Q = VPL / 4;          // 16-byte pieces of a lane
-    __shared__ __align__(16) float qs[RROWS][VPL * 8];
-    __shared__ float zs[RROWS][RK];
-    __shared__ float factor[RROWS];
-    const int e = blockIdx.z, g = blockIdx.y, k0 = blockIdx.x * RK, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const WeighEntry en(a, st, e, blockIdx.x == 0 && g == 0 && tid == 0);
-    if (en.n == 0 || k0 >= en.keys) return;
-    const int R = a.H / a.G, rows = en.n * R, bs = st.block_size, l8 = lane & 7, hi = en.keys - 1;
-    const int32_t* bt = st.block_table + (int64_t)e * st.max_blocks;
-    float k[4][VPL];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int key = min(k0 + warp * 16 + j * 4 + (lane >> 3), hi), page = kv4_page_read(bt[key / bs], a.err), o = key % bs;
-        if (FOUR) {
-            const Kv4Row r = kv4_row(page, o, bs, g, a.G, a.NG);
-            constexpr int W = VPL / 8;  // words of a lane; a row has 4 NG of them, so that lanes behind NG / W * 4 have none
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const int word = l8 * W + w, grp = word % a.NG;
-                uint32_t c = 0, par = 0;
-                if (word < 4 * a.NG) {
-                    c = *reinterpret_cast<const uint32_t*>(a.kpool4 + r.codes + 4 * word);
-                    par = *reinterpret_cast<const uint32_t*>(a.kpool4 + r.params + 4 * grp);
-                }
-                const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&par));
-#pragma unroll
-                for (int i = 0; i < 8; ++i) k[j][w * 8 + i] = fmaf((float)((c >> (4 * i)) & 15u), sm.x, sm.y);
+// What a lane has of a key: of every group of 32 values the eight from 8 c on (c: lane & 3)
+template <int NG, bool FOUR>
+struct KeyPart {
+    float4 x[FOUR ? 1 : 2 * NG];
+    uint32_t code[FOUR ? NG : 1], par[FOUR ? NG : 1];
+    __device__ __forceinline__ void fetch(const WeighArgs& a, int page, int o, int bs, int g, int c) {
+        if constexpr (FOUR) {
+            const Kv4Row r = kv4_row(page, o, bs, g, a.G, NG);
+            const uint8_t *k = a.kpool4 + r.codes + c * NG * 4, *p = a.kpool4 + r.params;
+            if constexpr (NG == 4) {
+                const uint4 u = *reinterpret_cast<const uint4*>(k), v = *reinterpret_cast<const uint4*>(p);
+                code[0] = u.x, code[1] = u.y, code[2] = u.z, code[3] = u.w, par[0] = v.x, par[1] = v.y, par[2] = v.z, par[3] = v.w;
+            } else if constexpr (NG == 2) {
+                const uint2 u = *reinterpret_cast<const uint2*>(k), v = *reinterpret_cast<const uint2*>(p);
+                code[0] = u.x, code[1] = u.y, par[0] = v.x, par[1] = v.y;
+            } else {
+                code[0] = *reinterpret_cast<const uint32_t*>(k), par[0] = *reinterpret_cast<const uint32_t*>(p);
             }
         } else {
-            const float* row = a.kpool + (((int64_t)page * bs + o) * a.G + g) * a.D;
+            const float* row = a.kpool + (((int64_t)page * bs + o) * a.G + g) * a.D + 8 * c;
 #pragma unroll
-            for (int i = 0; i < Q; ++i) {
-                const int d = (i * 8 + l8) * 4;
-                const float4 x = d < a.D ? ld4(row + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-                k[j][4 * i] = x.x, k[j][4 * i + 1] = x.y, k[j][4 * i + 2] = x.z, k[j][4 * i + 3] = x.w;
+            for (int i = 0; i < 2 * NG; ++i) {
+                const int d = 32 * (i >> 1) + 4 * (i & 1);
+                x[i] = d + 8 * c < a.D ? ld4(row + d) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
         }
     }
-    for (int r0 = 0; r0 < rows; r0 += RROWS) {
-        const int nr = min(RROWS, rows - r0);
-        __syncthreads();
-        // queries in the lanes' order: piece i of lane l at [(i * 8 + l) * 4]
-        for (int i = tid; i < nr * VPL * 8; i += RT) {
-            const int r = i / (VPL * 8), s = i - r * (VPL * 8), x = s & 3, piece = s >> 2, l = piece & 7, pc = piece >> 3;
-            int d;
-            if (FOUR) {
-                const int v = pc * 4 + x, word = l * (VPL / 8) + v / 8;
-                d = word < 4 * a.NG ? 32 * (word % a.NG) + 8 * (word / a.NG) + v % 8 : a.D;
-            } else {
-                d = piece * 4 + x;
-            }
-            const int row = r0 + r, t = en.t0 + row / R, h = g * R + row % R;
-            qs[r][s] = d < a.D ? a.q[(int64_t)t * a.ld + (int64_t)h * a.D + d] : 0.f;
+    // the four values of step kk (two steps a group)
+    __device__ __forceinline__ float4 step(int kk) const {
+        if constexpr (FOUR) {
+            const uint32_t w = code[kk >> 1] >> (16 * (kk & 1)), p = par[kk >> 1];
+            const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&p));
+            // (a code in the mantissa of 2^23: that number more)
+            auto val = [&](uint32_t u) { return fmaf(__uint_as_float(u | 0x4B000000u) - 8388608.f, sm.x, sm.y); };
+            return make_float4(val(w & 15u), val((w >> 4) & 15u), val((w >> 8) & 15u), val((w >> 12) & 15u));
+        } else {
+            return x[kk];
         }
-        if (tid < nr) factor[tid] = weigh_factor(a, g * R + (r0 + tid) % R);
+    }
+};
+
+// grid (blocks of 64 * tiles keys, key heads, entries).  NRT: tiles of eight rows that are gone through at a time
+template <int NRT, int NG, bool FOUR>
+__global__ void __launch_bounds__(RT, 2) weigh_rows_kernel(const __grid_constant__ WeighArgs a, const __grid_constant__ b200seq_step st, int tiles) {
+    chain_enter();
+    __shared__ uint4 frag[NRT][2 * NG][32];
+    __shared__ float2 part[RW][NRT * 8];
+    const int e = blockIdx.z, g = blockIdx.y, k0 = blockIdx.x * 64 * tiles, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = lane & 3, r8 = lane >> 2;
+    const WeighEntry en(a, st, e, blockIdx.x == 0 && g == 0 && tid == 0);
+    if (en.n == 0 || k0 >= en.keys) return;
+    const int R = a.H / a.G, rows = en.n * R, bs = st.block_size, hi = en.keys - 1;
+    const int32_t* bt = st.block_table + (int64_t)e * st.max_blocks;
+    // a warp's keys: k0 + 8 (warp + 8 i), of which a lane has key lane / 4
+    auto key_of = [&](int i) { return min(k0 + 8 * (warp + RW * i) + r8, hi); };
+    auto page_of = [&](int i) { return kv4_page_read(bt[key_of(i) / bs], a.err); };
+    const bool cap = a.softcap > 0.f;
+    for (int r0 = 0; r0 < rows; r0 += NRT * 8) {
+        KeyPart<NG, FOUR> nxt, cur;
+        int page = page_of(0);
+        nxt.fetch(a, page, key_of(0) % bs, bs, g, c);
+        page = tiles > 1 ? page_of(1) : 0;
         __syncthreads();
+        for (int i = tid; i < NRT * 2 * NG * 32; i += RT) {
+            const int ln = i & 31, kk = (i >> 5) % (2 * NG), rt = i / (64 * NG), row = r0 + 8 * rt + (ln >> 2), d = 32 * (kk >> 1) + 8 * (ln & 3) + 4 * (kk & 1);
+            uint4 f = make_uint4(0, 0, 0, 0);
+            if (row < rows) {
+                const int h = g * R + row % R;
+                const float* q = a.q + (int64_t)(en.t0 + row / R) * a.ld + (int64_t)h * a.D;
+                const float fac = weigh_factor(a, h) * (cap ? 1.f : WEIGH_LOG2E);
+                float x[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = d + j < a.D ? q[d + j] * fac : 0.f;
+                split_up(x[0], x[1], f.x, f.y), split_up(x[2], x[3], f.z, f.w);
+            }
+            frag[rt][kk][ln] = f;
+        }
+        __syncthreads();
+        float m[NRT], l[NRT];
+        int pos[NRT], lo[NRT];
+        float* out[NRT];
+#pragma unroll
+        for (int rt = 0; rt < NRT; ++rt) {
+            const int row = r0 + 8 * rt + r8;
+            const bool live = row < rows;
+            const WeighSpan span(a, en.p0 + (live ? row / R : 0));
+            m[rt] = -INFINITY, l[rt] = 0.f, pos[rt] = live ? span.p : -1, lo[rt] = span.lo;
+            out[rt] = rows_scores(a, live ? (int64_t)(en.t0 + row / R) * a.H + g * R + row % R : 0);
+        }
+        const int keep = a.window > 0 ? a.keep_first : 0, pos_least = en.p0 + r0 / R;
+        const WeighSpan last(a, en.p0 + min(rows - 1, r0 + NRT * 8 - 1) / R);
+        const int lo_most = last.lo;
 #pragma unroll 1
-        for (int r = 0; r < nr; ++r) {
-            uint64_t s[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < Q; ++i) {
-                const float4 x = ld4(&qs[r][(i * 8 + l8) * 4]);
-                const uint64_t x0 = tcsplit::pk(x.x, x.y), x1 = tcsplit::pk(x.z, x.w);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    s[j] = tcsplit::fma2(tcsplit::pk(k[j][4 * i], k[j][4 * i + 1]), x0, s[j]), s[j] = tcsplit::fma2(tcsplit::pk(k[j][4 * i + 2], k[j][4 * i + 3]), x1, s[j]);
+        for (int i = 0; i < tiles; ++i) {
+            const int key0 = k0 + 8 * (warp + RW * i);
+            if (key0 > hi) break;
+            cur = nxt;
+            if (i + 1 < tiles) {
+                nxt.fetch(a, page, key_of(i + 1) % bs, bs, g, c);
+                if (i + 2 < tiles) page = page_of(i + 2);
             }
-            float p[4];
+            float ah[NRT][4], al[NRT][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float u, v;
-                tcsplit::upk(s[j], u, v);
-                p[j] = u + v;
+            for (int rt = 0; rt < NRT; ++rt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) ah[rt][j] = al[rt][j] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < 2 * NG; ++kk) {
+                const float4 x = cur.step(kk);
+                uint32_t h0, h1, l0, l1;
+                split_up(x.x, x.y, h0, l0), split_up(x.z, x.w, h1, l1);
+#pragma unroll
+                for (int rt = 0; rt < NRT; ++rt) {
+                    const uint4 f = frag[rt][kk][lane];
+                    mma16816(al[rt], f, l0, l1), mma16816(ah[rt], f, h0, h1);
+                }
             }
-            // four sums over eight lanes: lanes with bits (b2, b1) end up with key 2 b2 + b1's
-            const bool b2 = lane & 4, b1 = lane & 2;
-            float v0 = (b2 ? p[2] : p[0]) + __shfl_xor_sync(0xffffffffu, b2 ? p[0] : p[2], 4);
-            float v1 = (b2 ? p[3] : p[1]) + __shfl_xor_sync(0xffffffffu, b2 ? p[1] : p[3], 4);
-            float w = (b1 ? v1 : v0) + __shfl_xor_sync(0xffffffffu, b1 ? v0 : v1, 2);
-            w += __shfl_xor_sync(0xffffffffu, w, 1);
-            if (!(lane & 1)) zs[r][warp * 16 + ((lane >> 1) & 3) * 4 + (lane >> 3)] = weigh_score(w, factor[r], a.softcap);
+            const int key = key0 + 2 * c;
+            const bool whole = key0 >= lo_most && key0 + 7 <= pos_least;      // (every row sees all of the tile)
+#pragma unroll
+            for (int rt = 0; rt < NRT; ++rt) {
+                float z[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    z[j] = fmaf(fmaf(al[rt][2 + j], UNLOW, al[rt][j] + ah[rt][2 + j]), UNLOW, ah[rt][j]);
+                    if (cap) z[j] = a.softcap * WEIGH_LOG2E * tanhf(z[j] / a.softcap);
+                }
+                const bool odd = !(fabsf(z[0]) + fabsf(z[1]) < INFINITY);
+                if (!whole || odd) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const bool sees = key + j <= pos[rt] && (key + j >= lo[rt] || key + j < keep);
+                        if (!sees) z[j] = -INFINITY;
+                        else if (odd) z[j] = plain_score(a, st, en, e, g, r0 + 8 * rt + r8, key + j, FOUR);
+                    }
+                }
+                const float top = fmaxf(m[rt], fmaxf(z[0], z[1]));
+                if (top > m[rt]) l[rt] *= ex2(m[rt] - top), m[rt] = top;
+                const float off = m[rt] == -INFINITY ? 0.f : m[rt];      // (minus infinities give nothing)
+                l[rt] += ex2(z[0] - off) + ex2(z[1] - off);
+                if (pos[rt] >= 0) *reinterpret_cast<float2*>(out[rt] + key) = make_float2(z[0], z[1]);
+            }
+        }
+#pragma unroll
+        for (int rt = 0; rt < NRT; ++rt) {      // a row's four lanes, then the warps
+            float top = m[rt];
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1)), top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            float s = m[rt] == -INFINITY ? l[rt] : l[rt] * ex2(m[rt] - top);
+            s += __shfl_xor_sync(0xffffffffu, s, 1), s += __shfl_xor_sync(0xffffffffu, s, 2);
+            if (c == 0) part[warp][8 * rt + r8] = make_float2(top, s);
         }
         __syncthreads();
-        for (int r = warp; r < nr; r += RT / 32) {
-            const int row = r0 + r, t = en.t0 + row / R, h = g * R + row % R;
-            const WeighSpan span(a, en.p0 + row / R);
-            float z[4], m = -INFINITY, l = 0.f;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                z[i] = zs[r][4 * lane + i];
-                if (!span.sees(k0 + 4 * lane + i)) z[i] = -INFINITY;
-                m = fmaxf(m, z[i]);
+        if (tid < NRT * 8 && r0 + tid < rows) {
+            const int row = r0 + tid;
+            float top = -INFINITY, s = 0.f;
+            for (int w = 0; w < RW; ++w) top = fmaxf(top, part[w][tid].x);
+            for (int w = 0; w < RW; ++w) {
+                const float2 x = part[w][tid];
+                s += x.x == -INFINITY ? x.y : x.y * ex2(x.x - top);
             }
-            m = warp_max(m);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) z[i] = z[i] == -INFINITY ? 0.f : ex2(z[i] - m), l += z[i];
-            l = warp_sum(l);
-            const int64_t at = (int64_t)t * a.H + h;
-            *reinterpret_cast<float4*>(rows_weights(a, at) + k0 + 4 * lane) = make_float4(z[0], z[1], z[2], z[3]);
-            if (lane == 0) rows_stats(a, st.T, at)[blockIdx.x] = make_float2(m, l);
+            rows_stats(a, st.T, (int64_t)(en.t0 + row / R) * a.H + g * R + row % R)[blockIdx.x] = make_float2(top, s);
         }
     }
 }
 
 // grid (blocks of FK keys, key heads, entries)
-__global__ void __launch_bounds__(FT) weigh_join_kernel(const __grid_constant__ WeighArgs a, const __grid_constant__ b200seq_step st) {
+__global__ void __launch_bounds__(FT) weigh_join_kernel(const __grid_constant__ WeighArgs a, const __grid_constant__ b200seq_step st, int block_keys) {
     chain_enter();
-    constexpr int PER = FK / RK;
-    __shared__ float f[RROWS][PER];
+    constexpr int ROWS = 32;
+    __shared__ float den[ROWS];
     const int e = blockIdx.z, g = blockIdx.y, k0 = blockIdx.x * FK, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const WeighEntry en(a, st, e, false);
     if (en.n == 0 || k0 >= en.keys) return;
-    const int R = a.H / a.G, rows = en.n * R, nb = (en.keys + RK - 1) / RK, b0 = blockIdx.x * PER;
+    const int R = a.H / a.G, rows = en.n * R, nb = (en.keys + block_keys - 1) / block_keys;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     const int key = k0 + 4 * tid;
-    for (int r0 = 0; r0 < rows; r0 += RROWS) {
-        const int nr = min(RROWS, rows - r0);
+    auto score = [&](int row) { return ld4(rows_scores(a, (int64_t)(en.t0 + row / R) * a.H + g * R + row % R) + key); };
+    // (the first rows' scores and the weights so far are on their way while the denominators are made)
+    constexpr int AHEAD = 8;
+    float* acc = a.acc + ((int64_t)en.slot * a.G + g) * a.acc_ld;
+    float4 ahead[AHEAD];
+    float old[4];
+#pragma unroll
+    for (int r = 0; r < AHEAD; ++r)
+        if (key < en.keys && r < rows) ahead[r] = score(r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) old[i] = key + i < en.fresh ? acc[key + i] : 0.f;
+    for (int r0 = 0; r0 < rows; r0 += ROWS) {
+        const int nr = min(ROWS, rows - r0);
         __syncthreads();
-        for (int r = warp; r < nr; r += FT / 32) {      // factors of the blocks' weights: 2^(the block's maximum - lse)
+        for (int r = warp; r < nr; r += FT / 32) {      // the rows' denominators (base-2 logarithms)
             const int row = r0 + r, h = g * R + row % R;
             const float2* s = rows_stats(a, st.T, (int64_t)(en.t0 + row / R) * a.H + h);
             float m = -INFINITY, l = 0.f;
+#pragma unroll 8
             for (int i = lane; i < nb; i += 32) m = fmaxf(m, s[i].x);
-            m = warp_max(m);
+            const float top = warp_max(m);
+#pragma unroll 8
             for (int i = lane; i < nb; i += 32) {
                 const float2 x = s[i];
-                l += x.x == -INFINITY ? x.y : x.y * ex2(x.x - m);      // (a block without a key to see: 0, or no number)
+                l += x.x == -INFINITY ? x.y : x.y * ex2(x.x - top);      // (a block without a key to see: 0, or no number)
             }
             l = warp_sum(l);
-            float den = l, top = m;
-            if (a.sink) {
-                const float sk = a.sink[h] * WEIGH_LOG2E;
-                top = fmaxf(m, sk);
-                den = (m == -INFINITY ? l : l * ex2(m - top)) + ex2(sk - top);
-            }
-            if (lane < PER && b0 + lane < nb) {
-                const float bm = s[b0 + lane].x;
-                f[r][lane] = bm == -INFINITY ? (l == l ? 0.f : l) : ex2(bm - top) / den;
+            if (lane == 0) {
+                const float v = weigh_lse(a, h, top, l);
+                den[r] = l != l ? l : v == -INFINITY ? INFINITY : v;
             }
         }
         __syncthreads();
         if (key < en.keys) {
-#pragma unroll 4
-            for (int r = 0; r < nr; ++r) {
-                const int row = r0 + r;
-                const float4 w = ld4(rows_weights(a, (int64_t)(en.t0 + row / R) * a.H + g * R + row % R) + key);
-                const float x = f[r][4 * tid / RK];
-                sum.x = fmaf(w.x, x, sum.x), sum.y = fmaf(w.y, x, sum.y), sum.z = fmaf(w.z, x, sum.z), sum.w = fmaf(w.w, x, sum.w);
+            auto add = [&](const float4& z, float x) { sum.x += ex2(z.x - x), sum.y += ex2(z.y - x), sum.z += ex2(z.z - x), sum.w += ex2(z.w - x); };
+            if (r0 == 0) {
+#pragma unroll
+                for (int r = 0; r < AHEAD; ++r)
+                    if (r < nr) add(ahead[r], den[r]);
             }
+#pragma unroll 4
+            for (int r = r0 == 0 ? AHEAD : 0; r < nr; ++r) add(score(r0 + r), den[r]);
         }
     }
-    float* acc = a.acc + ((int64_t)en.slot * a.G + g) * a.acc_ld;
     const float s[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        if (key + i < en.keys) acc[key + i] = key + i < en.fresh ? acc[key + i] + s[i] : s[i];
+        if (key + i < en.keys) acc[key + i] = old[i] + s[i];
+}
+
+template <int NG, bool FOUR>
+void launch_rows(const WeighArgs& a, const b200seq_step& st, dim3 grid, int row_tiles, int tiles, cudaStream_t cs) {
+    if (row_tiles == 1) launch_chained(weigh_rows_kernel<1, NG, FOUR>, grid, RT, 0, cs, a, st, tiles);
+    else if (row_tiles == 2) launch_chained(weigh_rows_kernel<2, NG, FOUR>, grid, RT, 0, cs, a, st, tiles);
+    else if (row_tiles == 3) launch_chained(weigh_rows_kernel<3, NG, FOUR>, grid, RT, 0, cs, a, st, tiles);
+    else launch_chained(weigh_rows_kernel<4, NG, FOUR>, grid, RT, 0, cs, a, st, tiles);
 }
 
 // ---- f32 tiles ------------------------------------------------------------------------------------------------------------------------------
@@ -333,12 +417,13 @@ int check(const b200seq_step* st, const b200seq_attn_desc* d, int kv_bits) {
     return 0;
 }
 
-// How a step is run.  Rows that share a key head in one entry: up to ROWS_MOST go through the rows path, whose time grows with them, if its weights fit the work area that it may have.
+// How a step is run.  Rows that share a key head in one entry: up to ROWS_MOST go through the rows path, whose time grows with them, if its scores fit the work area that it may have.
 constexpr int ROWS_MOST = 64;
 constexpr int64_t ROWS_FLOATS = 64 << 20;
 struct Plan {
     bool rows;
-    int blocks;        // rows path: blocks of RK keys of the longest sequence
+    int row_tiles, tiles, blocks;      // rows path: tiles of eight rows at a time, tiles of eight keys of a warp, blocks of keys of the longest sequence
+    int64_t keys;      // of a sequence: a bound, a multiple of 128
     int tokens;        // tokens of an entry that count: a bound
     WeighTcPlan tc;
     size_t floats;
@@ -347,12 +432,18 @@ Plan plan_of(const b200seq_step& st, const b200seq_attn_desc& d, int last, int m
     Plan p;
     const int64_t held = (int64_t)st.max_blocks * st.block_size;
     const int64_t keys = max_keys > 0 && max_keys < held ? max_keys : held;
-    p.blocks = (int)((keys + RK - 1) / RK);
+    p.keys = (keys + 127) / 128 * 128;
     const int each = (st.T + st.B - 1) / (st.B > 0 ? st.B : 1), tokens = last > 0 && last < each ? last : each;      // (were all entries equally long)
     p.tokens = last > 0 && last < st.T ? last : st.T;
-    const int64_t floats = (int64_t)st.T * d.H * p.blocks * (RK + 2);
-    p.rows = d.D <= 128 && (int64_t)tokens * (d.H / d.G) <= ROWS_MOST && floats <= ROWS_FLOATS;
-    p.tc = weigh_tc_plan(st, d.H, d.G, last, (int64_t)p.blocks * RK);
+    const int64_t rows = (int64_t)tokens * (d.H / d.G);
+    p.row_tiles = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 || (rows > 32 && rows <= 48) ? 3 : 4;
+    // a warp goes through as many tiles, up to eight, as leave four blocks an SM
+    p.tiles = 1;
+    while (p.tiles < 8 && p.keys * d.G * st.B / (128 * p.tiles) >= 4 * 148) p.tiles *= 2;
+    p.blocks = (int)((p.keys + 64 * p.tiles - 1) / (64 * p.tiles));
+    const int64_t floats = (int64_t)st.T * d.H * p.blocks * (64 * p.tiles + 2);
+    p.rows = d.D <= 128 && rows <= ROWS_MOST && floats <= ROWS_FLOATS;
+    p.tc = weigh_tc_plan(st, d.H, d.G, last, p.keys);
     p.floats = p.rows ? (size_t)floats : p.tc.floats;      // (more than the f32 tiles' T * H)
     return p;
 }
@@ -384,26 +475,24 @@ int b200seq_key_weights(const float* proj, int64_t ld, const b200seq_step* st, c
     WeighArgs a = {};
     a.q = proj + d->q_col, a.ld = ld, a.kpool = (const float*)kpool, a.kpool4 = (const uint8_t*)kpool, a.acc = acc, a.acc_ld = acc_ld, a.slots = slots;
     a.H = d->H, a.G = d->G, a.D = d->D, a.NG = four ? kv4_groups(d->D) : 0, a.last = last, a.scale = d->scale, a.softcap = d->softcap;
-    a.chunk = d->chunk, a.window = d->window, a.keep_first = d->keep_first, a.head_scale = d->head_scale, a.sink = d->sink, a.most_keys = (int64_t)p.blocks * RK, a.err = error_flag_dev();
+    a.chunk = d->chunk, a.window = d->window, a.keep_first = d->keep_first, a.head_scale = d->head_scale, a.sink = d->sink, a.most_keys = p.keys, a.err = error_flag_dev();
     const bool wide = four || ((d->D & 3) == 0 && (reinterpret_cast<uintptr_t>(kpool) & 15) == 0);
     if (p.rows && wide) {
-        a.part = scratch, a.key_blocks = p.blocks;
+        a.part = scratch, a.key_blocks = p.blocks, a.key_room = (int64_t)p.blocks * 64 * p.tiles;
         const dim3 grid(p.blocks, d->G, st->B);
-        if (four) {
-            if (d->D <= 64) launch_chained(weigh_rows_kernel<8, true>, grid, RT, 0, cs, a, *st);
-            else launch_chained(weigh_rows_kernel<16, true>, grid, RT, 0, cs, a, *st);
-        } else {
-            if (d->D <= 64) launch_chained(weigh_rows_kernel<8, false>, grid, RT, 0, cs, a, *st);
-            else launch_chained(weigh_rows_kernel<16, false>, grid, RT, 0, cs, a, *st);
-        }
+        if (four && a.NG == 1) launch_rows<1, true>(a, *st, grid, p.row_tiles, p.tiles, cs);
+        else if (four && a.NG == 2) launch_rows<2, true>(a, *st, grid, p.row_tiles, p.tiles, cs);
+        else if (four) launch_rows<4, true>(a, *st, grid, p.row_tiles, p.tiles, cs);
+        else if (d->D <= 64) launch_rows<2, false>(a, *st, grid, p.row_tiles, p.tiles, cs);
+        else launch_rows<4, false>(a, *st, grid, p.row_tiles, p.tiles, cs);
         SEQ_LAUNCH_CHECK("key_weights");
-        launch_chained(weigh_join_kernel, dim3((p.blocks * RK + FK - 1) / FK, d->G, st->B), FT, 0, cs, a, *st);
+        launch_chained(weigh_join_kernel, dim3((unsigned)((a.key_room + FK - 1) / FK), d->G, st->B), FT, 0, cs, a, *st, 64 * p.tiles);
         SEQ_LAUNCH_CHECK("key_weights");
         return 0;
     }
     if (weigh_tc_takes(a, four)) return weigh_tc(a, *st, p.tc, scratch, four, cs);
     a.lse = scratch;
-    const int64_t tiles = ((int64_t)p.tokens * (d->H / d->G) + TR - 1) / TR, key_tiles = (p.blocks * (int64_t)RK + TK - 1) / TK;
+    const int64_t tiles = ((int64_t)p.tokens * (d->H / d->G) + TR - 1) / TR, key_tiles = (p.keys + TK - 1) / TK;
     launch_chained(weigh_tile_lse_kernel, dim3((unsigned)tiles, d->G, st->B), TT, 0, cs, a, *st, (int)four);
     SEQ_LAUNCH_CHECK("key_weights");
     launch_chained(weigh_tile_sum_kernel, dim3((unsigned)key_tiles, d->G, st->B), TT, 0, cs, a, *st, (int)four);

@@ -19,7 +19,8 @@ struct WeighArgs {
     const float *head_scale, *sink;
     float* lse;                // [T][H]: base-2 logarithm of every row's sum of exponentials (minus infinity: nothing to give), or nothing (the rows' path)
     float* part;               // work area of the path that is taken
-    int key_blocks;            // rows' path: blocks of keys that the longest sequence may need
+    int key_blocks;            // rows' path: blocks of keys that the longest sequence may need, and as keys
+    int64_t key_room;
     int64_t most_keys;         // of a sequence
     int* err;
 };
@@ -68,6 +69,22 @@ __device__ __forceinline__ float weigh_lse(const WeighArgs& a, int h, float m, f
         l = (m == -INFINITY ? 0.f : l * exp2f(m - top)) + exp2f(sk - top), m = top;
     }
     return m == -INFINITY ? -INFINITY : m + log2f(l);
+}
+
+// one score by plain f32 products, for those that the split operands have no numbers for
+__device__ __forceinline__ float weigh_key_at(const WeighArgs& a, int64_t row, const Kv4Row& r, int g, int d, bool four) {
+    if (!four) return a.kpool[(row * a.G + g) * a.D + d];
+    const uint32_t c = *reinterpret_cast<const uint32_t*>(a.kpool4 + r.codes + 4 * ((d % 32 / 8) * a.NG + d / 32)), par = *reinterpret_cast<const uint32_t*>(a.kpool4 + r.params + 4 * (d / 32));
+    const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&par));
+    return fmaf((float)((c >> (4 * (d % 8))) & 15u), sm.x, sm.y);
+}
+static __device__ __noinline__ float plain_score(const WeighArgs& a, const b200seq_step& st, const WeighEntry& en, int e, int g, int row, int key, bool four) {
+    const int R = a.H / a.G, h = g * R + row % R, page = max(0, st.block_table[(int64_t)e * st.max_blocks + key / st.block_size]), o = key % st.block_size;
+    const float* q = a.q + (int64_t)(en.t0 + row / R) * a.ld + (int64_t)h * a.D;
+    const Kv4Row r = four ? kv4_row(page, o, st.block_size, g, a.G, a.NG) : Kv4Row{0, 0};
+    float s = 0.f;
+    for (int d = 0; d < a.D; ++d) s = fmaf(q[d], weigh_key_at(a, (int64_t)page * st.block_size + o, r, g, d, four), s);
+    return weigh_score(s, weigh_factor(a, h), a.softcap);
 }
 
 // Steps of many rows on the tensor cores (seq_weigh_tc.cu): how a step is cut up and the work area it needs (from its host sizes alone), whether a layer's rows suit it, the launches

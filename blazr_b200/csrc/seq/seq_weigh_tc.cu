@@ -93,21 +93,7 @@ __device__ __forceinline__ void split16(float a, float b, uint32_t& hi, uint32_t
     hi = *reinterpret_cast<const uint32_t*>(&h), lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// ---- plain forms, for sums that are no numbers -------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float key_at(const WeighArgs& a, int64_t row, const Kv4Row& r, int g, int d, bool four) {
-    if (!four) return a.kpool[(row * a.G + g) * a.D + d];
-    const uint32_t c = *reinterpret_cast<const uint32_t*>(a.kpool4 + r.codes + 4 * ((d % 32 / 8) * a.NG + d / 32)), par = *reinterpret_cast<const uint32_t*>(a.kpool4 + r.params + 4 * (d / 32));
-    const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&par));
-    return fmaf((float)((c >> (4 * (d % 8))) & 15u), sm.x, sm.y);
-}
-__device__ __noinline__ float plain_score(const WeighArgs& a, const b200seq_step& st, const WeighEntry& en, int e, int g, int row, int key, bool four) {
-    const int R = a.H / a.G, h = g * R + row % R, page = max(0, st.block_table[(int64_t)e * st.max_blocks + key / st.block_size]), o = key % st.block_size;
-    const float* q = a.q + (int64_t)(en.t0 + row / R) * a.ld + (int64_t)h * a.D;
-    const Kv4Row r = four ? kv4_row(page, o, st.block_size, g, a.G, a.NG) : Kv4Row{0, 0};
-    float s = 0.f;
-    for (int d = 0; d < a.D; ++d) s = fmaf(q[d], key_at(a, (int64_t)page * st.block_size + o, r, g, d, four), s);
-    return weigh_score(s, weigh_factor(a, h), a.softcap);
-}
+// ---- plain forms, for sums that are no numbers ---------------------------------------------------------------------------------------------------
 __device__ __noinline__ float2 plain_row(const WeighArgs& a, const b200seq_step& st, const WeighEntry& en, int e, int g, int row, const KeyWalk walk, int part, int parts, bool four) {
     const WeighSpan span(a, en.p0 + row / (a.H / a.G));
     float m = -INFINITY, l = 0.f;
