@@ -83,6 +83,11 @@ class StepEntry:
     block_table: Sequence[int]  # KV pages of the request (must cover pos0 + len(tokens) positions)
     want: Sequence[int] = ()    # indices into `tokens` whose logits are wanted
     prev: int = -1              # the request's last token before this portion (-1: none yet); models with a bigram embedding read it
+    row0: Optional[int] = None  # cached row of tokens[0], where that is not its position (a request that rows were evicted from)
+
+    @property
+    def first_row(self) -> int:
+        return self.pos0 if self.row0 is None else self.row0
 
 
 @dataclass
@@ -99,6 +104,7 @@ class StepArrays:
     T: int
     B: int
     ent_prev: Optional[np.ndarray] = None   # the token before each entry's first one (carried per request; unused at position 0)
+    tok_abs: Optional[np.ndarray] = None    # positions of the tokens, where tok_pos and ent_pos0 count cached rows (None: they are the same)
 
     @property
     def decode_only(self) -> bool:
@@ -111,7 +117,7 @@ def build_step(entries: Sequence[StepEntry], block_size: int, max_blocks: Option
     if any(n < 1 for n in lens):
         raise ValueError("an entry without tokens")
     T = int(sum(lens))
-    need = [-(-(e.pos0 + n) // block_size) for e, n in zip(entries, lens)]
+    need = [-(-(e.first_row + n) // block_size) for e, n in zip(entries, lens)]
     for e, nb in zip(entries, need):
         if len(e.block_table) < nb:
             raise ValueError(f"block table of {len(e.block_table)} pages does not cover {nb} pages")
@@ -131,7 +137,8 @@ def build_step(entries: Sequence[StepEntry], block_size: int, max_blocks: Option
     return StepArrays(
         tok_ids=np.concatenate([np.asarray(e.tokens, dtype=np.int32) for e in entries]) if B else np.zeros(0, np.int32),
         tok_ent=np.repeat(np.arange(B, dtype=np.int32), lens),
-        tok_pos=np.concatenate([np.arange(e.pos0, e.pos0 + n, dtype=np.int32) for e, n in zip(entries, lens)]) if B else np.zeros(0, np.int32),
+        tok_pos=np.concatenate([np.arange(e.first_row, e.first_row + n, dtype=np.int32) for e, n in zip(entries, lens)]) if B else np.zeros(0, np.int32),
         ent_start=start, ent_slot=np.asarray([e.slot for e in entries], dtype=np.int32),
-        ent_pos0=np.asarray([e.pos0 for e in entries], dtype=np.int32), block_table=bt, want_rows=np.asarray(want, dtype=np.int32), T=T, B=B,
-        ent_prev=np.asarray([max(int(e.prev), 0) for e in entries], dtype=np.int32))
+        ent_pos0=np.asarray([e.first_row for e in entries], dtype=np.int32), block_table=bt, want_rows=np.asarray(want, dtype=np.int32), T=T, B=B,
+        ent_prev=np.asarray([max(int(e.prev), 0) for e in entries], dtype=np.int32),
+        tok_abs=np.concatenate([np.arange(e.pos0, e.pos0 + n, dtype=np.int32) for e, n in zip(entries, lens)]) if any(e.first_row != e.pos0 for e in entries) else None)

@@ -9,12 +9,13 @@ are written before they are read.
 
 Requests may share pages (`fork`): a page has as many owners as requests hold it, and a request that is about to write into a page
 with other owners gets a copy of its own first (`reserve` names the copies to make).  `truncate` takes a request's last tokens back,
-`compact` moves the pages in use to the front of the pool.
+`compact` moves the pages in use to the front of the pool.  `evict` cuts a request's cached rows back: from then on it has fewer rows
+than tokens, and its next token's row is not its position.
 """
 from __future__ import annotations
 
 from dataclasses import dataclass, field
-from typing import Dict, List, Sequence, Tuple
+from typing import Dict, List, Optional, Sequence, Tuple
 
 
 class CacheFull(RuntimeError):
@@ -98,6 +99,12 @@ class SeqState:
     blocks: List[int] = field(default_factory=list)
     n_tokens: int = 0          # tokens already in the cache / folded into the state
     last_token: int = -1       # the last token fed (state of embeddings that hash the previous token with the current one)
+    gone: int = 0              # tokens whose rows have left the cache
+    whole_from: int = 0        # the rows of its tokens from here on are all there, in order
+
+    @property
+    def rows(self) -> int:
+        return self.n_tokens - self.gone
 
 
 class CacheManager:
@@ -123,7 +130,7 @@ class CacheManager:
 
     def _first_written(self, seq: SeqState) -> int:
         """index of the first page that the request's next tokens write into"""
-        return min([seq.n_tokens] + [seq.n_tokens // p * p for p in self.pooled]) // self.block_size
+        return min([seq.rows] + [seq.rows // p * p for p in self.pooled]) // self.block_size
 
     def _shared(self, seq: SeqState) -> List[int]:
         return [i for i in range(self._first_written(seq), len(seq.blocks)) if self.pages.owners(seq.blocks[i]) > 1]
@@ -134,7 +141,7 @@ class CacheManager:
 
     def pages_needed(self, seq: SeqState, n_new: int) -> int:
         """free pages that n_new more tokens take: new ones, and copies of shared ones that would be written"""
-        grow = max(0, -(-(seq.n_tokens + n_new) // self.block_size) - len(seq.blocks))
+        grow = max(0, -(-(seq.rows + n_new) // self.block_size) - len(seq.blocks))
         return grow + (len(self._shared(seq)) if n_new > 0 else 0)
 
     def reserve(self, seq: SeqState, n_new: int) -> List[Tuple[int, int]]:
@@ -156,6 +163,7 @@ class CacheManager:
         s = self.admit(new_rid)
         self.pages.share(src.blocks)
         s.blocks, s.n_tokens, s.last_token = list(src.blocks), src.n_tokens, src.last_token
+        s.gone, s.whole_from = src.gone, src.whole_from
         return s
 
     def truncate(self, rid: str, n_tokens: int, last_token: int) -> None:
@@ -163,10 +171,32 @@ class CacheManager:
         s = self.live[rid]
         if not 0 <= n_tokens <= s.n_tokens:
             raise ValueError(f"request {rid} holds {s.n_tokens} tokens, not {n_tokens}")
-        keep = -(-n_tokens // self.block_size)
+        if s.gone and n_tokens < s.whole_from:
+            raise ValueError(f"request {rid} has lost rows before its token {s.whole_from}: it cannot be taken back to {n_tokens}")
+        keep = -(-(n_tokens - s.gone) // self.block_size)
         self.pages.free(s.blocks[keep:])
         s.blocks = s.blocks[:keep]
         s.n_tokens, s.last_token = n_tokens, last_token
+
+    def evict(self, rid: str, keep: int, recent: int) -> Optional[Tuple[List[int], List[int], int]]:
+        """the request's rows are cut back to `keep`, its last `recent` ones among them.  Returns (pages it had, pages that the rows go to, rows it had): shared pages are replaced
+        by free ones, the rest stay; or None where there are not enough free ones.  The caller moves the rows and then gives back what `evicted` names."""
+        s = self.live[rid]
+        assert 0 < recent <= keep < s.rows
+        had, n = list(s.blocks), s.rows
+        to = had[:-(-keep // self.block_size)]
+        shared = [i for i, b in enumerate(to) if self.pages.owners(b) > 1]
+        if len(shared) > self.pages.free_blocks:
+            return None
+        for i, b in zip(shared, self.pages.alloc(len(shared))):
+            to[i] = b
+        s.blocks, s.gone, s.whole_from = list(to), s.gone + n - keep, s.n_tokens - recent
+        return had, to, n
+
+    def evicted(self, had: Sequence[int], to: Sequence[int]) -> None:
+        """the pages that an eviction has emptied lose an owner"""
+        kept = set(to)
+        self.pages.free([b for b in had if b not in kept])
 
     def compact(self) -> List[Tuple[int, int]]:
         """moves the pages in use to the front of the pool; returns the page copies (from, to) to make"""

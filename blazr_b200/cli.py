@@ -2,6 +2,7 @@
 
     python -m blazr_b200 generate --model DIR --prompt 1,2,3 [--prompt ...] [--max-new N] [--temperature T] [--top-k K] [--top-p P] [--samples N]
                                   [--repetition-penalty R] [--presence-penalty P] [--frequency-penalty F] [--logit-bias 7:-2.5,9:1] [--kv-bits 4]
+                                  [--drafts N] [--max-keys N]
     python -m blazr_b200 trace    --model DIR --dtype bfloat16|float32 --out DIR --max-tokens N     (also bin/trace_run)
 
 `trace` replays externally scheduled steps through the engine: one JSON object per line on standard input,
@@ -53,15 +54,15 @@ def cmd_trace(a) -> int:
 
 
 def cmd_generate(a) -> int:
-    from .engine import Engine, SamplingParams
+    from .engine import Engine, SamplingParams, lookup_drafts
     model = _load(a.model, a.dtype)
     prompts = [[int(t) for t in p.split(",") if t.strip()] for p in a.prompt]
     need = sum(-(-(len(p) + a.max_new) // a.block_size) * a.block_size for p in prompts[:a.max_seqs]) * a.samples if a.max_tokens <= 0 else a.max_tokens
     bias = dict((int(t), float(v)) for t, v in (e.split(":") for e in a.logit_bias.split(",") if e.strip())) if a.logit_bias else None
-    eng = Engine(model, max_tokens=need, max_seqs=max(a.max_seqs, a.samples), block_size=a.block_size, kv_bits=a.kv_bits)
+    eng = Engine(model, max_tokens=need, max_seqs=max(a.max_seqs, a.samples), block_size=a.block_size, kv_bits=a.kv_bits, max_keys=a.max_keys)
     outs = eng.generate(prompts, SamplingParams(temperature=a.temperature, top_k=a.top_k, top_p=a.top_p, seed=a.seed, max_new_tokens=a.max_new, n=a.samples,
                                                 repetition_penalty=a.repetition_penalty, presence_penalty=a.presence_penalty, frequency_penalty=a.frequency_penalty,
-                                                logit_bias=bias))
+                                                logit_bias=bias, draft_fn=lookup_drafts(a.drafts) if a.drafts > 0 else None))
     for p, o in zip(prompts, outs):
         for tokens in o if a.samples > 1 else [o]:
             print(json.dumps({"prompt": p, "tokens": tokens}))
@@ -94,5 +95,7 @@ def main(argv=None) -> int:
             p.add_argument("--presence-penalty", type=float, default=0.0)
             p.add_argument("--frequency-penalty", type=float, default=0.0)
             p.add_argument("--logit-bias", default="", help="token:value, with commas")
+            p.add_argument("--drafts", type=int, default=0, help="guesses a step, looked up in the text so far and verified together (models without recurrent state)")
+            p.add_argument("--max-keys", type=int, default=0, help="cached rows a request may hold; beyond them the least attended leave (0: all stay)")
     a = ap.parse_args(argv)
     return cmd_trace(a) if a.cmd == "trace" else cmd_generate(a)

@@ -53,7 +53,7 @@ __global__ void attn_prep_kernel(float* __restrict__ proj, int64_t ld, b200seq_s
     if (a.rot_dims > 0) {
         for (int i = threadIdx.x; i < (a.rot_dims >> 1); i += blockDim.x) {
             float sn, cs;
-            sincosf((float)pos * a.rot_freq[i], &sn, &cs);
+            sincosf((float)(a.rot_pos ? a.rot_pos[t] : pos) * a.rot_freq[i], &sn, &cs);
             rot_sm[2 * i] = cs * a.rot_scale, rot_sm[2 * i + 1] = sn * a.rot_scale;
         }
         __syncthreads();
@@ -171,7 +171,7 @@ __global__ void attn_prep_gen_kernel(float* __restrict__ proj, int64_t ld, b200s
     float* base = proj + (int64_t)t * ld;
     for (int i = threadIdx.x; i < np; i += blockDim.x) {
         float sn, cs;
-        sincosf((float)pos * a.rot_freq[i], &sn, &cs);
+        sincosf((float)(a.rot_pos ? a.rot_pos[t] : pos) * a.rot_freq[i], &sn, &cs);
         rot_sm[i] = cs * a.rot_scale, rot_sm[np + i] = sn * a.rot_scale;
     }
     float rq = 1.f, rk = 1.f;

@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(128) kv4_prep_rows_kernel(float* proj, int64_t
         if (first) {
             for (int i = threadIdx.x; i < np; i += 128) {
                 float sn, cs;
-                sincosf((float)pos * a.rot_freq[i], &sn, &cs);
+                sincosf((float)(a.rot_pos ? a.rot_pos[t] : pos) * a.rot_freq[i], &sn, &cs);
                 rot_sm[i] = cs * a.rot_scale, rot_sm[np + i] = sn * a.rot_scale;
             }
             __syncthreads();
@@ -264,7 +264,7 @@ __global__ void kv4_prep_kernel(float* __restrict__ proj, int64_t ld, const b200
     float* base = proj + (int64_t)t * ld;
     for (int i = threadIdx.x; i < np; i += blockDim.x) {
         float sn, cs;
-        sincosf((float)pos * a.rot_freq[i], &sn, &cs);
+        sincosf((float)(a.rot_pos ? a.rot_pos[t] : pos) * a.rot_freq[i], &sn, &cs);
         rot_sm[i] = cs * a.rot_scale, rot_sm[np + i] = sn * a.rot_scale;
     }
     auto biased = [&](int col) { return base[col] + (a.in_bias ? a.in_bias[col] : 0.f); };

@@ -13,12 +13,16 @@ touches the model.
 `fork()` lets a second request continue from where another is: KV pages are shared and copied when one of the two is about to write
 into them, recurrent state is copied at once.  `SamplingParams.n` samples a prompt several times that way.  Penalties, biases and
 masks of a request are applied to its logits on the GPU before its token is chosen (seqops.process_logits).
+
+Drafts (`SamplingParams.draft_fn`): a decoded request brings its last token and guesses of the next ones in one step, and keeps those that the
+model's own probabilities bear out (seqops.verify_drafts).  A cache of bounded size (`max_keys`): the weight that every cached key is given is added up as the
+steps run (seqops.key_weights), and a request that holds more rows is cut back to those of largest weight (seqops.evict_keys).
 """
 from __future__ import annotations
 
 from collections import deque
 from dataclasses import dataclass, field, replace
-from typing import Callable, Deque, Dict, List, Optional, Sequence, Set, Tuple
+from typing import Any, Callable, Deque, Dict, List, Optional, Sequence, Set, Tuple
 
 import numpy as np
 import torch
@@ -36,7 +40,9 @@ class SamplingParams:
     """temperature 0 = greedy (arg-max kernel); otherwise soft-max sampling, optionally among the top_k / top_p tokens.
     repetition_penalty: the logits of tokens of the prompt and the output are divided by it (multiplied where negative); frequency_penalty times how often, and
     presence_penalty once if, a token stands in the output is subtracted; logit_bias: added per token; mask_fn(output so far) -> int32 words, bit v % 32 of word
-    v / 32 set where token v is allowed, or None (all).  n: samples of the prompt, which is run once (Request.siblings holds the others)"""
+    v / 32 set where token v is allowed, or None (all).  n: samples of the prompt, which is run once (Request.siblings holds the others).
+    draft_fn(prompt and output so far) -> guesses of the next tokens, which one step verifies together, or (guesses, f32 [guesses, vocab] probabilities they were drawn from);
+    what comes out has the distribution that temperature, top_k and top_p give without them (tokens of equal logits are kept or left out together)"""
     temperature: float = 0.0
     top_k: int = 0
     top_p: float = 1.0
@@ -49,10 +55,26 @@ class SamplingParams:
     logit_bias: Optional[Dict[int, float]] = None
     mask_fn: Optional[Callable[[List[int]], Optional[Sequence[int]]]] = None
     n: int = 1
+    draft_fn: Optional[Callable[[List[int]], Any]] = None
 
     def ruled(self) -> bool:
         """whether the logits are changed before the token is chosen"""
         return bool(self.repetition_penalty != 1.0 or self.presence_penalty or self.frequency_penalty or self.logit_bias or self.mask_fn)
+
+
+def lookup_drafts(most: int, match: int = 3) -> Callable[[List[int]], List[int]]:
+    """a draft_fn that looks the last `match` tokens (or fewer, down to one) up in the text before them and guesses the up to `most` tokens that followed there last"""
+    if most < 0 or match < 1:
+        raise ValueError(f"{most} drafts by {match} tokens")
+
+    def drafts(tokens: List[int]) -> List[int]:
+        for m in range(min(match, len(tokens) - 1), 0, -1):
+            tail = tokens[-m:]
+            for i in range(len(tokens) - m - 1, -1, -1):
+                if tokens[i:i + m] == tail:
+                    return tokens[i + m:i + m + most]
+        return []
+    return drafts
 
 
 @dataclass
@@ -65,16 +87,29 @@ class Request:
     finished: bool = False
     siblings: List["Request"] = field(default_factory=list)   # the other samples of params.n
     _gen: Optional[torch.Generator] = None
+    _probs: Optional[torch.Tensor] = None    # of the drafts that the step verifies
 
 
 class Engine:
     def __init__(self, model: LayeredModel, max_tokens: int, max_seqs: int = 4, block_size: int = 16, max_step_tokens: int = 2048,
-                 prefill_chunk: int = 512, kv_bits: int = 32):
+                 prefill_chunk: int = 512, kv_bits: int = 32, max_keys: int = 0, first_keys: int = 4, recent_keys: int = 0, weigh_last: int = 0):
         """max_tokens: tokens all live requests may hold together (the KV pool is made for this many, rounded up to pages);
-        max_seqs: state slots = most requests live at a time; kv_bits: bits of a cached key or value, 32 or 4"""
+        max_seqs: state slots = most requests live at a time; kv_bits: bits of a cached key or value, 32 or 4.
+        max_keys: > 0: a request that holds more cached rows between two steps is cut back to seven eighths of them: the first first_keys, the last recent_keys (0: a quarter of
+        max_keys) and, in every layer and key head, those that were given the most attention since they came.  weigh_last: only the attention of that many last tokens of
+        a step's portion counts (0: of all)"""
         self.model = model
         self.cache = CacheManager(max_tokens, max_seqs, block_size, model.pooled_sizes() if hasattr(model, "pooled_sizes") else ())
-        model.allocate(self.cache.pages.num_blocks, block_size, max_seqs, self.cache.pages.num_blocks * block_size, **({} if kv_bits == 32 else {"kv_bits": kv_bits}))
+        room = self.cache.pages.num_blocks * block_size
+        self.max_keys, self.first_keys, self.recent_keys = max_keys, first_keys, recent_keys or max_keys // 4
+        self.keep_keys = max_keys - max_keys // 8
+        if max_keys < 0 or weigh_last < 0 or (max_keys > 0 and (first_keys < 0 or self.recent_keys < 1 or first_keys + self.recent_keys > self.keep_keys)):
+            raise ValueError(f"the first {first_keys} and the last {self.recent_keys} of {self.keep_keys} rows to keep")
+        # (a slot's weights have room for what a request may hold when a step ends)
+        self.weighed_rows = min(room, max_keys + max_step_tokens) if max_keys > 0 else 0
+        model.allocate(self.cache.pages.num_blocks, block_size, max_seqs, room, **({} if kv_bits == 32 else {"kv_bits": kv_bits}), **({"weighed_rows": self.weighed_rows} if max_keys > 0 else {}))
+        if max_keys > 0:
+            model.weigh_last = weigh_last
         self.max_step_tokens, self.prefill_chunk = max_step_tokens, prefill_chunk
         self.waiting: Deque[Request] = deque()
         self.running: List[Request] = []
@@ -101,8 +136,10 @@ class Engine:
                     if seq is None:
                         seq = self.cache.admit(rid)
                         admitted.append(rid)
+                    if self.max_keys > 0 and seq.rows + len(toks) > self.weighed_rows:
+                        raise CacheFull(f"request {rid} would hold {seq.rows + len(toks)} cached rows, {self.weighed_rows} have room for their weights")
                     copies += self.cache.reserve(seq, len(toks))
-                    entries.append(StepEntry(tokens=toks, pos0=seq.n_tokens, slot=seq.slot, block_table=seq.blocks, want=want, prev=seq.last_token))
+                    entries.append(StepEntry(tokens=toks, pos0=seq.n_tokens, slot=seq.slot, block_table=seq.blocks, want=want, prev=seq.last_token, row0=seq.rows))
             finally:
                 if copies:      # also when the pages ran out on the way: these requests hold their copies already
                     self.model.copy_pages(copies)
@@ -177,6 +214,22 @@ class Engine:
             raise ValueError("this model's embedding reads the token before the next one, which a truncated request has lost")
         self.cache.truncate(rid, n_tokens, -1)
 
+    def _cut(self, rids: Sequence[str]) -> None:
+        """cuts those of the live requests back that hold more than max_keys cached rows (a request whose shared pages cannot be replaced yet: after a later step)"""
+        if self.max_keys <= 0:
+            return
+        cut = []
+        for rid in rids:
+            s = self.cache.live.get(rid)
+            if s is not None and s.rows > self.max_keys:
+                pages = self.cache.evict(rid, self.keep_keys, self.recent_keys)
+                if pages is not None:
+                    cut.append((s.slot, pages))
+        if cut:
+            self.model.evict([s for s, _ in cut], [p[2] for _, p in cut], [p[0] for _, p in cut], [p[1] for _, p in cut], self.keep_keys, self.first_keys, self.recent_keys)
+            for _, (had, to, _) in cut:
+                self.cache.evicted(had, to)
+
     def compact(self) -> int:
         """moves the KV pages in use to the front of the pool; returns how many moved"""
         pairs = self.cache.compact()
@@ -202,6 +255,7 @@ class Engine:
                 out = logits.cpu().numpy()
         for rid in end:
             self.release(str(rid))
+        self._cut([str(e["id"]) for e in entries])
         return out
 
     # ---- own scheduler ---------------------------------------------------------------------------------------------------------
@@ -235,6 +289,11 @@ class Engine:
             raise ValueError(f"a top_p of {p.top_p}")
         if p.temperature > 0 and p.top_k < 0:
             raise ValueError(f"a top_k of {p.top_k}")
+        if p.draft_fn is not None:
+            if p.ruled():
+                raise ValueError("drafts go with temperature, top_k and top_p: not with penalties, biases or masks")
+            if hasattr(self.model, "has_state") and self.model.has_state():
+                raise ValueError("layers of this model carry state that rejected drafts cannot be taken out of")
         vocab = getattr(getattr(self.model, "cfg", None), "vocab", None)
         for t in p.logit_bias or ():
             if int(t) != t or t < 0 or (vocab is not None and t >= vocab):
@@ -271,12 +330,15 @@ class Engine:
             if r.fed < len(r.prompt):
                 continue
             seq = self.cache.live[r.rid]
-            need = self.cache.pages_needed(seq, 1)
-            if budget < 1 or need > free_pages:
+            if budget < 1 or self.cache.pages_needed(seq, 1) > free_pages:
                 continue
-            plan.append((r, [r.output[-1]], [0]))
-            budget -= 1
-            free_pages -= need
+            most = min(budget, r.params.max_new_tokens - len(r.output), self.weighed_rows - seq.rows if self.max_keys > 0 else budget) if r.params.draft_fn is not None else 1
+            guess = self._drafts(r, most - 1) if most > 1 else []
+            while guess and self.cache.pages_needed(seq, 1 + len(guess)) > free_pages:
+                guess = guess[:-1]
+            plan.append((r, [r.output[-1]] + guess, list(range(1 + len(guess)))))
+            budget -= 1 + len(guess)
+            free_pages -= self.cache.pages_needed(seq, 1 + len(guess))
         prefilling = [r for r in self.running if r.fed < len(r.prompt)]
         for r in prefilling + list(self.waiting):
             if budget < 1:
@@ -288,10 +350,12 @@ class Engine:
                 free_slots -= r.params.n
             n = min(len(r.prompt) - r.fed, self.prefill_chunk, budget)
             have = len(seq.blocks) if seq else 0
-            held = seq.n_tokens if seq else 0
+            held = seq.rows if seq else 0
             own = self.cache.pages_to_copy(seq) if seq else 0       # shared pages that the portion would write into
             room = (have + free_pages - own) * self.cache.block_size - held if free_pages >= own else 0
             n = min(n, room)
+            if self.max_keys > 0:
+                n = min(n, self.weighed_rows - held)
             if n < 1:
                 if seq is None:
                     free_slots += r.params.n
@@ -312,13 +376,23 @@ class Engine:
                 raise CacheFull("no request can make progress: the KV pool is too small for the live requests")
             return []
         masks = {r.rid: self._mask(r) for r, _, w in plan if w and r.params.mask_fn is not None}
-        greedy = all(r.params.temperature <= 0 and not r.params.ruled() and r.params.n == 1 for r, _, w in plan if w)
+        greedy = all(r.params.temperature <= 0 and not r.params.ruled() and r.params.n == 1 and r.params.draft_fn is None for r, _, w in plan if w)
         logits = self._forward([(r.rid, toks, want) for r, toks, want in plan], sample=greedy)
         for r, _, _ in plan:        # (requests run from here on: a mask that was refused, or a pass that failed, leaves them waiting)
             if r in self.waiting:
                 self.waiting.remove(r)
                 self.running.append(r)
-        sampled = [r for r, _, w in plan if w]
+        drafted, sampled, others, row = [], [], [], 0      # requests whose drafts are verified (request, tokens, first row of logits); requests that get one token, and their rows
+        for r, toks, w in plan:
+            if w and r.params.draft_fn is not None and r.output:
+                drafted.append((r, toks, row))
+            elif w:
+                sampled.append(r)
+                others.append(row)
+            row += len(w)
+        chosen = self._verify(logits, drafted) if drafted else []
+        if drafted and sampled:
+            logits = logits[torch.tensor(others, device=logits.device)]
         ids = self.model.last_ids.cpu().tolist() if (greedy and sampled) else None
         for r, toks, _ in plan:
             if r.fed < len(r.prompt):
@@ -334,6 +408,18 @@ class Engine:
         # largest logits of rows that are sampled: where one is no number there is nothing to choose by (and a multinomial of it would end the process)
         tops = logits[:len(sampled)].max(1).values.tolist() if any(r.params.temperature > 0 for r in sampled) else None
         lost: List[str] = []
+        for (r, _, _), tokens in zip(drafted, chosen):
+            if tokens[-1] < 0:
+                lost.append(f"{r.rid} (a row of its logits has no largest number)")
+                tokens.pop()
+                r.finished = True
+            for tok in tokens:
+                r.output.append(tok)
+                if len(r.output) >= r.params.max_new_tokens or tok in r.params.stop_tokens:
+                    r.finished = True
+                    break
+            if r.finished:
+                done.append(r)
         for row, r in zip(rows, sampled):
             if r.params.temperature > 0 and not abs(tops[row] / r.params.temperature) <= F32_MAX:
                 lost.append(f"{r.rid} (its largest logit is {tops[row]}, its temperature {r.params.temperature})")
@@ -348,9 +434,63 @@ class Engine:
         for r in done:
             self.running.remove(r)
             self.release(r.rid)
+        self._cut([r.rid for r in self.running])
         if lost:
             raise RuntimeError("no token can be chosen for request " + ", ".join(lost))
         return done
+
+    def _drafts(self, r: Request, most: int) -> List[int]:
+        """up to `most` guesses of the request's next tokens (and the probabilities they were drawn from, kept for the step)"""
+        got = r.params.draft_fn(r.prompt + r.output)
+        probs = None
+        if isinstance(got, tuple):
+            got, probs = got
+        tokens = [int(t) for t in got][:max(0, most)]
+        vocab = getattr(getattr(self.model, "cfg", None), "vocab", None)
+        if any(t < 0 or (vocab is not None and t >= vocab) for t in tokens):
+            raise ValueError(f"drafts of request {r.rid} outside the vocabulary: {tokens}")
+        if probs is not None and (probs.dim() != 2 or probs.shape[0] < len(tokens) or (vocab is not None and probs.shape[1] != vocab)):
+            raise ValueError(f"the draft probabilities of request {r.rid} are a row for each of {len(tokens)} drafts, not {tuple(probs.shape)}")
+        r._probs = probs
+        return tokens
+
+    def _verify(self, logits: torch.Tensor, drafted: Sequence[Tuple[Request, List[int], int]]) -> List[List[int]]:
+        """the tokens that come behind the last one of every request (-1: a row without a choice); rejected drafts leave the cache"""
+        dev, out = logits.device, {}
+        for known in (False, True):        # certain guesses, and guesses with the probabilities they were drawn from
+            part = [d for d in drafted if (d[0]._probs is not None and len(d[1]) > 1) == known]
+            if not part:
+                continue
+            lens = [len(toks) for _, toks, _ in part]
+            start = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+            rows = np.concatenate([np.arange(row, row + n) for (_, _, row), n in zip(part, lens)])
+            z = logits[int(rows[0]):int(rows[-1]) + 1] if (np.diff(rows) == 1).all() else logits[torch.from_numpy(rows).to(dev)]
+            up = lambda x, dt: torch.from_numpy(np.asarray(x, dt)).to(dev)
+            drafts = up(np.concatenate([toks[1:] + [0] for _, toks, _ in part]), np.int32)
+            # a request draws as many numbers as it brought rows, and one more
+            u = [torch.rand(n + 1, device=dev, generator=r._gen) if r._gen is not None else torch.zeros(n + 1, device=dev) for (r, _, _), n in zip(part, lens)]
+            kw: Dict[str, torch.Tensor] = {}
+            if any(r.params.top_k for r, _, _ in part):
+                kw["top_k"] = up([r.params.top_k for r, _, _ in part], np.int32)
+            if any(r.params.top_p < 1.0 for r, _, _ in part):
+                kw["top_p"] = up([r.params.top_p for r, _, _ in part], np.float32)
+            if known:
+                q = torch.zeros((int(start[-1]), logits.shape[1]), dtype=torch.float32, device=dev)
+                for (r, _, _), s, n in zip(part, start, lens):
+                    q[int(s):int(s) + n - 1] = r._probs[:n - 1].to(dev, torch.float32)
+                kw["draft_probs"] = q
+            accepted, tokens = seqops.verify_drafts(z, up(start, np.int32), drafts, torch.cat([x[:-1] for x in u]), torch.stack([x[-1] for x in u]),
+                                             up([max(r.params.temperature, 0.0) for r, _, _ in part], np.float32), **kw)
+            both = torch.cat([accepted, tokens]).cpu().tolist()
+            got = both[len(part):]
+            for (r, _, _), s, a in zip(part, start, both):
+                out[r.rid] = got[int(s):int(s) + a + 1]
+        for r, toks, _ in drafted:
+            a = len(out[r.rid]) - 1
+            if a + 1 < len(toks):
+                seq = self.cache.live[r.rid]
+                self.cache.truncate(r.rid, seq.n_tokens - (len(toks) - 1 - a), toks[a])
+        return [out[r.rid] for r, _, _ in drafted]
 
     def _fan_out(self, sampled: List[Request]) -> Tuple[List[int], List[Request]]:
         """forks requests whose prompt is through into their params.n samples; (row of the step's logits, request) of every sample, in order"""

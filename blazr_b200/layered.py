@@ -293,6 +293,7 @@ def loop_runs(n: int, start: int = 0, stop: int = 0, times: int = 0) -> list:
 # buffers of a layer whose first dimension counts KV pages / state slots
 PAGED = ("kpool", "vpool", "kpooled", "vpooled")
 SLOTTED = ("canon1_state", "canon2_state", "conv_state", "ssm_state", "shift_state", "ret_state", "rec_state", "delta_state", "scan_state")
+WEIGHED = ("key_weight",)       # by slot too, but of the cache, not of the sequence
 
 
 class _Rows:
@@ -411,11 +412,11 @@ class _Workspace:
                                          order=torch.empty(n, **i32), slot=torch.empty(n, **i32))
         self.scratch = torch.empty(max(1, model.scratch_floats(cap)), **f32)      # work area: segmented state-space scan, key-split attention
         self.next_ids = torch.empty((cap,), dtype=torch.int32, device=dev)
-        # int32 step arrays in one buffer: ids | ent | pos | want | start | slot | pos0 | prev | block_table
+        # int32 step arrays in one buffer: ids | ent | pos | want | start | slot | pos0 | prev | abs | block_table
         B, mb = model.max_seqs, model.max_blocks
         self.off = {}
         o = 0
-        for k, n in (("ids", cap), ("ent", cap), ("pos", cap), ("want", cap), ("start", B + 1), ("slot", B), ("pos0", B), ("prev", B), ("bt", B * mb)):
+        for k, n in (("ids", cap), ("ent", cap), ("pos", cap), ("want", cap), ("start", B + 1), ("slot", B), ("pos0", B), ("prev", B), ("abs", cap), ("bt", B * mb)):
             self.off[k] = (o, n)
             o += -(-n // 4) * 4
         self.meta = torch.zeros(o, dtype=torch.int32, device=dev)
@@ -609,7 +610,7 @@ class LayeredModel:
                 self.weight_bytes += (L["w_gu"].numel() + L["w_down"].numel()) * 2
             self.layers.append(L)
         self.max_seqs = self.max_blocks = self.block_size = 0
-        self.kv_bits, self._keys = 32, 0
+        self.kv_bits, self._keys, self.weighed_rows, self.weigh_last = 32, 0, 0, 0
         self._ws: Dict[int, _Workspace] = {}
         self._graphs: Dict[int, object] = {}
         self.use_graphs = True
@@ -1131,9 +1132,18 @@ class LayeredModel:
         f32 = dict(dtype=torch.float32, device=self.dev)
         return torch.zeros((n, block_size, key_heads, dim), **f32), torch.zeros((n, block_size, value_heads, vdim), **f32)
 
-    def allocate(self, num_blocks: int, block_size: int, max_seqs: int, max_seq_tokens: int, kv_bits: int = 32) -> None:
+    def check_evictable(self) -> None:
+        """raises ValueError where rows cannot leave the cache: layers whose masks or pooled blocks go by positions, that share another layer's rows, that hold latents"""
+        for m in self.attention_specs():
+            if isinstance(m, LatentAttentionSpec) or m.window > 0 or m.chunk > 0 or m.pool > 0 or m.diff is not None or m.kv_from is not None:
+                raise ValueError("rows leave the cache of plain attention over all positions: not of windows, chunks, pooled blocks, latents, differential attention or shared rows")
+        if not self.attention_specs():
+            raise ValueError("no layer of this model has a KV cache")
+
+    def allocate(self, num_blocks: int, block_size: int, max_seqs: int, max_seq_tokens: int, kv_bits: int = 32, weighed_rows: int = 0) -> None:
         """KV pools for `num_blocks` pages, state for `max_seqs` slots; block tables hold up to max_seq_tokens positions.  kv_bits: 32, or 4 (plain attention layers
-        with heads of up to 128 values: keys and values are held as 4-bit codes, 0.625 bytes a value)"""
+        with heads of up to 128 values: keys and values are held as 4-bit codes, 0.625 bytes a value).  weighed_rows: > 0: every slot's attention weights are added up for
+        so many cached rows (`evict` goes by them)"""
         dev, cfg = self.dev, self.cfg
         if kv_bits not in (4, 32):
             raise ValueError(f"a KV cache holds 4 or 32 bits a value, not {kv_bits}")
@@ -1142,7 +1152,9 @@ class LayeredModel:
                 if isinstance(m, LatentAttentionSpec) or m.pool > 0 or max(m.dim, m.vdim) > seqops.KV4_MAX_DIM:
                     raise ValueError("a 4-bit KV cache holds plain keys and values of heads of up to "
                                      f"{seqops.KV4_MAX_DIM} values: not latents, not pooled blocks, not {max(getattr(m, 'dim', 0), m.vdim)} values")
-        self.kv_bits = kv_bits
+        if weighed_rows > 0:
+            self.check_evictable()
+        self.kv_bits, self.weighed_rows, self.weigh_last = kv_bits, weighed_rows, 0
         f32 = dict(dtype=torch.float32, device=dev)
         self.block_size, self.max_seqs = block_size, max_seqs
         self.max_blocks = max(1, -(-max_seq_tokens // block_size))
@@ -1196,6 +1208,10 @@ class LayeredModel:
             for L in self.layers:
                 att = L["spec"].mixer if L["spec"].kind == "attention" else L["spec"].mixer.left
                 L["kv_src"] = self.layers[att.kv_from] if att.kv_from is not None else L
+        for L in self.layers:
+            L.pop("key_weight", None)
+            if weighed_rows > 0 and "vpool" in L:
+                L["key_weight"] = torch.zeros((max_seqs, L["desc"].G, weighed_rows), **f32)
         self._ws.clear()
         self._graphs.clear()
 
@@ -1250,7 +1266,7 @@ class LayeredModel:
         return max([0] + [seqops.scan_scratch_floats(cap, self.max_seqs, L["spec"].mixer.right.inner, L["spec"].mixer.right.state) for L in self.layers if "scan" in L])
 
     def cache_bytes(self) -> int:
-        return sum(L[k].nbytes for L in self.layers for k in PAGED + SLOTTED if k in L)
+        return sum(L[k].nbytes for L in self.layers for k in PAGED + SLOTTED + WEIGHED if k in L)
 
     def has_state(self) -> bool:
         """whether requests carry state outside their KV pages"""
@@ -1264,7 +1280,21 @@ class LayeredModel:
     def copy_slots(self, pairs) -> None:
         """recurrent state of slots `to` <- `from` in every layer, for pairs (from, to)"""
         if pairs:
-            seqops.copy_pages([L[k] for L in self.layers for k in SLOTTED if k in L], pairs)
+            seqops.copy_pages([L[k] for L in self.layers for k in SLOTTED + WEIGHED if k in L], pairs)
+
+    def evict(self, slots, rows, tables, to_tables, keep: int, first: int, recent: int) -> None:
+        """cuts the cached rows of requests (their slots, rows, pages and the pages that the rows go to) back to `keep` in every layer and key head"""
+        wide = max(len(t) for t in tables)
+        i32 = lambda x: torch.from_numpy(np.asarray(x, dtype=np.int32)).to(self.dev)
+        full = lambda ts: i32([list(t) + [-1] * (wide - len(t)) for t in ts])
+        s, n, src, dst = i32(slots), i32(rows), full(tables), full(to_tables)
+        groups = {}
+        for L in self.layers:       # layers of one shape go together
+            if "key_weight" in L:
+                groups.setdefault((tuple(L["kpool"].shape), tuple(L["vpool"].shape)), []).append(L)
+        for ls in groups.values():
+            seqops.evict_keys([L["kpool"] for L in ls], [L["vpool"] for L in ls], [L["key_weight"] for L in ls], s, n, src, keep, first=first, recent=recent,
+                              block_size=self.block_size, to_table=dst)
 
     def _ctx_buffers(self, rows: int):
         """gathered latents (activation type) and the per-head keys | values projected out of them (f32) for `rows` context positions;
@@ -1296,7 +1326,7 @@ class LayeredModel:
         hn = h.numpy()
         prev = sa.ent_prev if sa.ent_prev is not None else np.zeros(sa.B, dtype=np.int32)
         for k, arr in (("ids", sa.tok_ids), ("ent", sa.tok_ent), ("pos", sa.tok_pos), ("want", sa.want_rows), ("start", sa.ent_start), ("slot", sa.ent_slot),
-                       ("pos0", sa.ent_pos0), ("prev", prev)):
+                       ("pos0", sa.ent_pos0), ("prev", prev), ("abs", sa.tok_pos if sa.tok_abs is None else sa.tok_abs)):
             o, _ = ws.off[k]
             hn[o:o + arr.shape[0]] = arr
         o, _ = ws.off["bt"]
@@ -1308,9 +1338,10 @@ class LayeredModel:
             ws.copied = torch.cuda.Event()
             ws.copied.record(torch.cuda.current_stream(self.dev))
 
-    def _desc(self, ws: _Workspace, T: int, B: int) -> seqops.StepDesc:
+    def _desc(self, ws: _Workspace, T: int, B: int, positions: str = "pos") -> seqops.StepDesc:
+        """the step's arrays; positions: "pos", cached rows, or "abs", places in the sequences (for what has no cache)"""
         ptr = lambda k: ws.view(k).data_ptr()
-        return seqops.StepDesc(ptr("ent"), ptr("pos"), ptr("start"), ptr("slot"), ptr("pos0"), ptr("bt"), T, B, self.max_blocks, self.block_size)
+        return seqops.StepDesc(ptr("ent"), ptr(positions), ptr("start"), ptr("slot"), ptr("pos0"), ptr("bt"), T, B, self.max_blocks, self.block_size)
 
     def forward(self, sa: StepArrays, sample: bool = False, debug_layers: Optional[list] = None) -> torch.Tensor:
         """runs one step; returns f32 logits [R, vocab] of the wanted rows (a view of a buffer the next step overwrites);
@@ -1325,9 +1356,10 @@ class LayeredModel:
         graphable = self.use_graphs and debug_layers is None and sa.decode_only and R == T and self.dev.type == "cuda" \
             and bool((sa.want_rows == np.arange(T)).all())
         if graphable:
-            if self.kv_bits == 4:       # a captured step shares its work out by the keys of its longest sequence: one for every power of two of them
+            by_keys = self.kv_bits == 4 or self.weighed_rows > 0
+            if by_keys:       # a captured step shares its work out by the keys of its longest sequence: one for every power of two of them
                 self._keys = max(256, 1 << (self._keys - 1).bit_length())
-            key = (T, bool(sample), self._keys if self.kv_bits == 4 else 0)
+            key = (T, bool(sample), self._keys if by_keys else 0)
             g = self._graphs.get(key)
             if g is None:
                 self._run(ws, T, B, R, sample, None)        # warm-up outside capture (module loading, attribute calls)
@@ -1621,7 +1653,7 @@ class LayeredModel:
 
         reads_x0 = any(L["spec"].enter is not None and L["spec"].enter[0] for L in self.layers)
         first = entering(0) if n else {}
-        ops.embed_pos(self.embed, ids, st, cfg.embed_scale, self.pos_freq, x, cfg.eps, x0=x0 if reads_x0 else None, add_vec=first.get("add_vec"),
+        ops.embed_pos(self.embed, ids, self._desc(ws, T, B, "abs"), cfg.embed_scale, self.pos_freq, x, cfg.eps, x0=x0 if reads_x0 else None, add_vec=first.get("add_vec"),
                       fin_w=self.layers[0]["norm1"] if n else None, a=a if n else None)
         fused_side = T <= 8 and cfg.token_side * cfg.width <= self.SIDE_FUSED_ELEMS
         for i, L in enumerate(self.layers):
@@ -1785,12 +1817,15 @@ class LayeredModel:
         seqops.delta(proj, st, d, wz, L["delta_state"], o, ws.scratch)
         seqops.linear(o, L["w_o"], y)
 
-    def _attn_prep(self, L, st, proj: torch.Tensor) -> None:
-        """queries normed and rotated in the projection rows, keys and values into the layer's pages"""
+    def _attn_prep(self, L, ws: _Workspace, st, proj: torch.Tensor) -> None:
+        """queries normed and rotated in the projection rows, keys and values into the layer's pages (and, where rows may leave those, the weights of the cached keys)"""
+        turned = ws.view("abs") if self.weighed_rows > 0 else None
         if self.kv_bits == 4:
-            seqops.attn_prep_kv4(proj, st, L["desc"], L.get("kpool"), L.get("vpool"))
+            seqops.attn_prep_kv4(proj, st, L["desc"], L.get("kpool"), L.get("vpool"), rot_pos=turned)
         else:
-            seqops.attn_prep_ex(proj, st, L["desc"], L.get("kpool"), L.get("vpool"), L.get("kpooled"), L.get("vpooled"))
+            seqops.attn_prep_ex(proj, st, L["desc"], L.get("kpool"), L.get("vpool"), L.get("kpooled"), L.get("vpooled"), rot_pos=turned)
+        if "key_weight" in L:
+            seqops.key_weights(proj, st, L["desc"], L["kpool"], L["key_weight"], last=self.weigh_last, max_keys=self._keys)
 
     def _attend(self, L, src, ws: _Workspace, st, proj: torch.Tensor, o: torch.Tensor) -> None:
         """attention of the prepared rows over the pages of layer `src`"""
@@ -1802,7 +1837,7 @@ class LayeredModel:
     def _attention_out(self, L, m: AttentionSpec, ws: _Workspace, st, T: int, proj: torch.Tensor, y: torch.Tensor) -> None:
         """attention (prepared from the stacked projection `proj`) over the layer's own pool or the pool of the layer whose keys and values it shares"""
         src = L.get("kv_src", L)
-        self._attn_prep(L, st, proj)
+        self._attn_prep(L, ws, st, proj)
         H, V = m.heads, m.vdim
         o = ws.inner_a.view(-1)[:T * H * V].view(T, H * V)
         if m.diff is not None:      # two maps per head as 2 H plain heads, f32; then o = unit_rms(a1 - lambda a2) * (1 - diff)
@@ -1905,7 +1940,7 @@ class LayeredModel:
         n_in = L["w_in"].shape[0]
         qkvg = ws.proj[:T, :n_in]
         seqops.linear(a, L["w_in"], qkvg)
-        self._attn_prep(L, st, qkvg)
+        self._attn_prep(L, ws, st, qkvg)
         o = ws.inner_a.view(-1)[:T * m.heads * m.vdim].view(T, m.heads * m.vdim)
         self._attend(L, L, ws, st, qkvg, o)
         seqops.linear(o, L["w_o"], y)

@@ -91,7 +91,7 @@ class AttnDesc(C.Structure):
                 ("gate_col", C.c_int32), ("scale", C.c_float), ("chunk", C.c_int32), ("window", C.c_int32), ("pool", C.c_int32), ("qk_eps", C.c_float),
                 ("rot_dims", C.c_int32), ("rot_freq", C.c_void_p), ("rot_scale", C.c_float), ("sink", C.c_void_p), ("latent_v", C.c_int32), ("gate", C.c_void_p), ("gate_ld", C.c_int64), ("ctx_rows", C.c_int32), ("kd", C.c_int32), ("kv_ld", C.c_int64), ("krot", C.c_void_p), ("krot_ld", C.c_int64),
                 ("q_norm_w", C.c_void_p), ("k_norm_w", C.c_void_p), ("norm_full", C.c_int32), ("rot_half", C.c_int32), ("in_bias", C.c_void_p), ("kv_shared", C.c_int32),
-                ("vg", C.c_int32), ("softcap", C.c_float), ("head_scale", C.c_void_p), ("keep_first", C.c_int32), ("gate_elem", C.c_int32)]
+                ("vg", C.c_int32), ("softcap", C.c_float), ("head_scale", C.c_void_p), ("keep_first", C.c_int32), ("gate_elem", C.c_int32), ("rot_pos", C.c_void_p)]
 
 
 class RetentionDesc(C.Structure):
@@ -380,9 +380,20 @@ def depth_norm(x_cur: torch.Tensor, out1: Optional[torch.Tensor], w1: Optional[t
 
 @_timed
 def attn_prep_ex(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: Optional[torch.Tensor], vpool: Optional[torch.Tensor],
-                 kpooled: Optional[torch.Tensor] = None, vpooled: Optional[torch.Tensor] = None):
+                 kpooled: Optional[torch.Tensor] = None, vpooled: Optional[torch.Tensor] = None, rot_pos: Optional[torch.Tensor] = None):
+    """rot_pos: int32 [T], the positions by which q and k turn, where the step's count cached rows"""
     _, _, ld = _rows2d(proj)
+    if rot_pos is not None:
+        d = _turned("attn_prep_ex", step, d, rot_pos)
     _check(lib().b200seq_attn_prep_ex(_p(proj), ld, C.byref(step), C.byref(d), _p(kpool), _p(vpool), _p(kpooled), _p(vpooled), _st(proj)))
+
+
+def _turned(name: str, step: "StepDesc", d: "AttnDesc", rot_pos: torch.Tensor) -> "AttnDesc":
+    if rot_pos.dtype != torch.int32 or rot_pos.numel() < step.T or not rot_pos.is_contiguous():
+        raise ValueError(f"{name}: rot_pos is contiguous int32 of {step.T} positions, not {rot_pos.dtype} {tuple(rot_pos.shape)}")
+    d2 = AttnDesc.from_buffer_copy(d)
+    d2.rot_pos = rot_pos.data_ptr()
+    return d2
 
 
 @_timed
@@ -951,8 +962,10 @@ def _kv4_layer(name: str, proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", k
 
 
 @_timed
-def attn_prep_kv4(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: Optional[torch.Tensor], vpool: Optional[torch.Tensor]):
+def attn_prep_kv4(proj: torch.Tensor, step: "StepDesc", d: "AttnDesc", kpool: Optional[torch.Tensor], vpool: Optional[torch.Tensor], rot_pos: Optional[torch.Tensor] = None):
     """attn_prep_ex over a 4-bit cache: queries biased, normed and rotated in place, keys and values likewise into their pages"""
+    if rot_pos is not None:
+        d = _turned("attn_prep_kv4", step, d, rot_pos)
     need = max(d.q_col + d.H * d.D, 0 if d.kv_shared else max(d.k_col + d.G * d.D, d.v_col + (d.vg if d.vg > 0 else d.G) * d.V))
     ld = _kv4_layer("attn_prep_kv4", proj, step, d, kpool, vpool, need)
     _on_device("attn_prep_kv4", lib().b200seq_attn_prep_kv4, (_p(proj), ld, C.byref(step), C.byref(d), _p(kpool), _p(vpool)), proj, kpool, vpool)

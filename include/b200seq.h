@@ -219,6 +219,7 @@ typedef struct b200seq_attn_desc {
     const float* head_scale; /* attend: device f32 [H] or null: the score of head h is also multiplied by head_scale[h] */
     int32_t keep_first;    /* attend (window > 0): positions j < keep_first stay visible to every later position, at their true positions */
     int32_t gate_elem;     /* attend (gate_col >= 0): 1 = one gate logit per output element, H * V of them at gate_col (or in `gate`), instead of one per head */
+    const int32_t* rot_pos; /* prep: device int32 [T] or null: the positions by which q and k turn, where tok_pos counts cached rows (a sequence that rows were evicted from) */
 } b200seq_attn_desc;
 int b200seq_attn_prep_ex(float* proj, int64_t ld, const b200seq_step* st, const b200seq_attn_desc* d, float* kpool, float* vpool, float* kpooled, float* vpooled,
                          void* stream);
