@@ -92,7 +92,7 @@ struct WeighTcPlan {
     int tiles, stat_parts;     // denominators: row tiles (bound), parts of a walk
     int key_tiles, parts;      // sums: key tiles of the longest sequence, parts of a walk
     int64_t key_room;
-    size_t stat_floats, floats;
+    size_t lse_floats, stat_floats, floats;
 };
 WeighTcPlan weigh_tc_plan(const b200seq_step& st, int H, int G, int last, int64_t keys);
 bool weigh_tc_takes(const WeighArgs& a, bool four);

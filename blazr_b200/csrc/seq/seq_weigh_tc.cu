@@ -32,7 +32,7 @@ struct TcArgs {
     WeighArgs w;
     int parts, stat_parts;     // of this launch's walk; of the denominators' walk
     int tiles;                 // denominators: row tiles (bound); sums: key tiles
-    float2* stat;              // [T * H][stat_parts]: (maximum, sum) in base 2
+    float2* stat;              // [T * H][stat_parts]: (maximum, sum) in base 2, where a walk has parts
     float* psum;               // sums, parts > 1: [part][B][G][key_room]
     int64_t key_room;
     int B;
@@ -107,18 +107,27 @@ __device__ __noinline__ float2 plain_row(const WeighArgs& a, const b200seq_step&
     return make_float2(m, l);
 }
 
-// a row's denominator (base-2 logarithm), from the parts of its walk; infinite where the row gives nothing
-__device__ __forceinline__ float lse_of(const TcArgs& a, int t, int h) {
-    const float2* s = a.stat + ((int64_t)t * a.w.H + h) * a.stat_parts;
+// a row's denominator (base-2 logarithm) from its maximum and sum; infinite where the row gives nothing
+__device__ __forceinline__ float lse_of(const WeighArgs& w, int h, float m, float l) {
+    if (l != l) return l;
+    const float v = weigh_lse(w, h, m, l);
+    return v == -INFINITY ? INFINITY : v;
+}
+// a thread a row: the parts of its walk (rows that do not count have none, and nobody reads theirs)
+__global__ void __launch_bounds__(128) weigh_lse_kernel(const __grid_constant__ TcArgs a, int rows) {
+    chain_enter();
+    const int row = blockIdx.x * 128 + threadIdx.x;
+    if (row >= rows) return;
+    const float2* s = a.stat + (int64_t)row * a.stat_parts;
     float m = -INFINITY, l = 0.f;
+#pragma unroll 8
     for (int i = 0; i < a.stat_parts; ++i) m = fmaxf(m, s[i].x);
+#pragma unroll 8
     for (int i = 0; i < a.stat_parts; ++i) {
         const float2 x = s[i];
         l += x.x == -INFINITY ? x.y : x.y * ex2(x.x - m);
     }
-    if (l != l) return l;
-    const float v = weigh_lse(a.w, h, m, l);
-    return v == -INFINITY ? INFINITY : v;
+    a.w.lse[row] = lse_of(a.w, row % a.w.H, m, l);
 }
 
 __device__ __noinline__ float plain_key(const TcArgs& a, const b200seq_step& st, const WeighEntry& en, int e, int g, int key, int tile0, int tiles, int part, bool four) {
@@ -128,7 +137,7 @@ __device__ __noinline__ float plain_key(const TcArgs& a, const b200seq_step& st,
         for (int r = (tile0 + i) * NT; r < min(rows, (tile0 + i + 1) * NT); ++r) {
             const WeighSpan span(a.w, en.p0 + r / R);
             if (!span.sees(key)) continue;
-            const float lse = lse_of(a, en.t0 + r / R, g * R + r % R);
+            const float lse = a.w.lse[(int64_t)(en.t0 + r / R) * a.w.H + g * R + r % R];
             sum += ex2(plain_score(a.w, st, en, e, g, r, key, four) - lse);
         }
     return sum;
@@ -143,6 +152,9 @@ __global__ void __launch_bounds__(THREADS, 2) weigh_tc_kernel(const __grid_const
     __shared__ int abort_sh;
     __shared__ __align__(8) uint64_t bars[2 * STAGES + 5];
     __shared__ __align__(16) float lse_sh[STAGES][NT];
+    __shared__ int64_t row_sh[3][NT];                                   // loaders: where the rows of three tiles lie,
+    __shared__ float fac_sh[SUMS ? 3 : 1][NT];                          // their factors,
+    __shared__ int par_sh[FOUR ? 3 : 1][NT];                            // their parameters behind their codes
     const WeighArgs& w = a.w;
     const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int D = w.D, G = w.G, R = w.H / w.G, KB = (D + 63) >> 6, KK = (D + 15) >> 4;
@@ -215,30 +227,42 @@ __global__ void __launch_bounds__(THREADS, 2) weigh_tc_kernel(const __grid_const
                 src = w.q + (int64_t)(en.t0 + at / R) * w.ld + (int64_t)h * D;
                 f = weigh_factor(w, h) * fold;
             }
-#pragma unroll 1
-            for (int kk = 0; kk < KK; ++kk) {
-                float x[16];
-                if (SUMS && FOUR) {
+            if (!live) f = 0.f;
+            if (SUMS && FOUR) {
+#pragma unroll 2
+                for (int kk = 0; kk < KK; ++kk) {
                     const int grp = kk >> 1;
                     const uint32_t par = *reinterpret_cast<const uint32_t*>(w.kpool4 + k4.params + 4 * grp);
                     const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&par));
+                    uint32_t hi[8], lo[8];
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         const uint32_t word = *reinterpret_cast<const uint32_t*>(w.kpool4 + k4.codes + 4 * ((2 * (kk & 1) + c) * w.NG + grp));
+                        float x[8];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) x[8 * c + i] = 16 * kk + 8 * c + i < D ? fmaf((float)((word >> (4 * i)) & 15u), sm.x, sm.y) : 0.f;
+                        for (int i = 0; i < 8; ++i) x[i] = live && 16 * kk + 8 * c + i < D ? fmaf((float)((word >> (4 * i)) & 15u), sm.x, sm.y) * f : 0.f;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) split16(x[2 * i], x[2 * i + 1], hi[4 * c + i], lo[4 * c + i]);
                     }
-                } else {
+                    st8(res + lanes + kk * 8, hi), st8(res + lanes + rplane + kk * 8, lo);
+                }
+            } else {
+                for (int k0 = 0; k0 < KK; k0 += 4) {       // (the loads of 64 values at once: a chain of them is what a short walk would wait for)
+                    float4 v[16];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float4 v = 16 * kk + 4 * i < D ? ld4(src + 16 * kk + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
+                    for (int i = 0; i < 16; ++i) v[i] = live && 16 * k0 + 4 * i < D ? ld4(src + 16 * k0 + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        if (k0 + kk >= KK) break;
+                        uint32_t hi[8], lo[8];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float4 x = v[4 * kk + i];
+                            split16(x.x * f, x.y * f, hi[2 * i], lo[2 * i]), split16(x.z * f, x.w * f, hi[2 * i + 1], lo[2 * i + 1]);
+                        }
+                        st8(res + lanes + (k0 + kk) * 8, hi), st8(res + lanes + rplane + (k0 + kk) * 8, lo);
                     }
                 }
-                uint32_t hi[8], lo[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) split16(live ? x[2 * i] * f : 0.f, live ? x[2 * i + 1] * f : 0.f, hi[i], lo[i]);
-                st8(res + lanes + kk * 8, hi), st8(res + lanes + rplane + kk * 8, lo);
             }
             st_wait();
             fence_before();
@@ -317,7 +341,10 @@ __global__ void __launch_bounds__(THREADS, 2) weigh_tc_kernel(const __grid_const
             if (!SUMS) {
                 float2 r = make_float2(m, l);
                 if (l != l) r = plain_row(w, st, en, e, g, mine, walk, part, a.parts, FOUR);
-                a.stat[((int64_t)(en.t0 + mine / R) * w.H + g * R + mine % R) * a.stat_parts + part] = r;
+                const int h = g * R + mine % R;
+                const int64_t row = (int64_t)(en.t0 + mine / R) * w.H + h;
+                if (a.parts > 1) a.stat[row * a.parts + part] = r;
+                else w.lse[row] = lse_of(w, h, r.x, r.y);
             } else {
                 if (l != l) l = plain_key(a, st, en, e, g, mine, tile0, all, part, FOUR);
                 if (a.parts > 1) {
@@ -331,104 +358,111 @@ __global__ void __launch_bounds__(THREADS, 2) weigh_tc_kernel(const __grid_const
     } else if (warp < 8) {
         // ===================== loaders: 128 threads =====================
         // A unit is a 64-wide block of a tile: eight 16-byte pieces a thread, 16 lanes to a row's 64 values.  The next unit's loads are in flight while this one is split and
-        // stored; a lane looks rows lane and lane + 32 of a tile up, handed round by shuffles.
-        const int lw = warp - 4, hw = lw * 2 + (lane >> 4), c4 = lane & 15;
-        struct Look {
-            int64_t at;      // f32: first value; 4 bits: (page, row in page); -1: no row
-            float f;
+        // stored.  Where a tile's rows lie stands in a table in shared memory that 64 threads write a tile ahead, from pages asked for a tile before that.  (Looked up by every lane and
+        // handed round by shuffles it was what the kernel spent its time on.)
+        const int lw = warp - 4, lt = threadIdx.x - 128, hw = lw * 2 + (lane >> 4), c4 = lane & 15;
+        auto row_of = [&](int j) { return (SUMS ? (tile0 + part + j * a.parts) * NT : walk.key0(part + j * a.parts)) + lt; };
+        auto page_of = [&](int j) {      // (keys: the page of row lt of tile j)
+            const int n = row_of(j);
+            return !SUMS && n < en.keys ? kv4_page_read(bt[n / bs], w.err) : 0;
         };
-        auto look = [&](int j, int i) {
-            const int t = part + j * a.parts, n = (SUMS ? (tile0 + t) * NT : walk.key0(t)) + i;
-            Look x{-1, UP};
+        auto note = [&](int j, int page) {
+            const int n = row_of(j), at = j % 3;
+            int64_t x = -1;
             if (SUMS) {
                 if (n < rows) {
                     const int h = g * R + n % R;
-                    x.at = (int64_t)(en.t0 + n / R) * w.ld + (int64_t)h * D, x.f = weigh_factor(w, h) * fold;
+                    x = (int64_t)(en.t0 + n / R) * w.ld + (int64_t)h * D;
+                    fac_sh[at][lt] = weigh_factor(w, h) * fold;
                 }
             } else if (n < en.keys) {
-                const int page = kv4_page_read(bt[n / bs], w.err), o = n % bs;
-                x.at = FOUR ? ((int64_t)page << 32) | (uint32_t)o : (((int64_t)page * bs + o) * G + g) * D;
+                const int o = n % bs;
+                if (FOUR) {
+                    const Kv4Row k = kv4_row(page, o, bs, g, G, w.NG);
+                    x = k.codes, par_sh[at][lt] = (int)(k.params - k.codes);
+                } else {
+                    x = (((int64_t)page * bs + o) * G + g) * D;
+                }
             }
-            return x;
+            row_sh[at][lt] = x;
         };
-        auto from = [&](const Look& ra, const Look& rb, int i) {      // row i of the tile, from the lane that looked it up
-            Look x;
-            x.at = __shfl_sync(0xffffffffu, i < 32 ? ra.at : rb.at, i & 31), x.f = SUMS ? __shfl_sync(0xffffffffu, i < 32 ? ra.f : rb.f, i & 31) : UP;
-            return x;
-        };
-        auto fetch = [&](const Look& ra, const Look& rb, int u, float4 (&x)[8]) {
-            const int d = u * 64 + c4 * 4;
+        auto fetch = [&](int j, int u, float4 (&x)[8]) {
+            const int d = u * 64 + c4 * 4, at = j % 3;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const Look r = from(ra, rb, hw + 8 * i);
+                const int64_t r = row_sh[at][hw + 8 * i];
                 x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r.at < 0 || d >= D) continue;
+                if (r < 0 || d >= D) continue;
                 if (!SUMS && FOUR) {
-                    const Kv4Row k = kv4_row((int)(r.at >> 32), (int)(uint32_t)r.at, bs, g, G, w.NG);
-                    const uint32_t word = *reinterpret_cast<const uint32_t*>(w.kpool4 + k.codes + 4 * ((d % 32 / 8) * w.NG + d / 32));
-                    x[i].x = __uint_as_float(word >> (4 * (d % 8))), x[i].y = __uint_as_float(*reinterpret_cast<const uint32_t*>(w.kpool4 + k.params + 4 * (d / 32)));
+                    const uint8_t* k = w.kpool4 + r;
+                    const uint32_t word = *reinterpret_cast<const uint32_t*>(k + 4 * ((d % 32 / 8) * w.NG + d / 32)) >> (4 * (d % 8));
+                    const uint32_t par = *reinterpret_cast<const uint32_t*>(k + par_sh[at][hw + 8 * i] + 4 * (d / 32));
+                    // (kept as they are until the values are needed; a word of a row that is one is told apart by bit 16)
+                    x[i].x = __uint_as_float((word & 0xFFFFu) | 0x10000u), x[i].y = __uint_as_float(par);
                 } else {
-                    x[i] = ld4((SUMS ? w.q : w.kpool) + r.at + d);
+                    x[i] = ld4((SUMS ? w.q : w.kpool) + r + d);
                 }
             }
         };
-        Look ra{-1, 0.f}, rb{-1, 0.f}, na, nb;
+        int page = 0;
         float4 cur[8], nxt[8];
-        if (ntile > 0) {
-            ra = look(0, lane), rb = look(0, lane + 32);
-            fetch(ra, rb, 0, nxt);
-        }
+        if (lt < 64 && ntile > 0) note(0, page_of(0));
+        if (lt < 64 && ntile > 1) page = page_of(1);
+        asm volatile("bar.sync 2, 128;" ::: "memory");
+        if (ntile > 0) fetch(0, 0, nxt);
         bool ok = true;
 #pragma unroll 1
-        for (int j = 0; j < ntile && ok; ++j) {
+        for (int j = 0; j < ntile; ++j) {      // (a wait that ran out: the warps meet at their barrier all the same, to the end)
             const int s = j % STAGES;
             const bool more = j + 1 < ntile;
-            na = nb = Look{-1, 0.f};
-            if (more) na = look(j + 1, lane), nb = look(j + 1, lane + 32);
             float lse = INFINITY;
-            if (SUMS && lw < 2) {
-                const int n = (tile0 + part + j * a.parts) * NT + lw * 32 + lane;
-                if (n < rows) lse = lse_of(a, en.t0 + n / R, g * R + n % R);
+            if (lt < 64) {
+                if (more) note(j + 1, page);
+                if (j + 2 < ntile) page = page_of(j + 2);
+                if (SUMS) {
+                    const int n = row_of(j);
+                    if (n < rows) lse = w.lse[(int64_t)(en.t0 + n / R) * w.H + g * R + n % R];
+                }
             }
+            asm volatile("bar.sync 2, 128;" ::: "memory");      // (three tables: nobody reads the one that is written next but one)
+            if (!ok) continue;
 #pragma unroll 1
             for (int u = 0; u < KB; ++u) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) cur[i] = nxt[i];
                 const bool here = u + 1 < KB;
-                if (here || more) fetch(here ? ra : na, here ? rb : nb, here ? u + 1 : 0, nxt);
+                if (here || more) fetch(here ? j : j + 1, here ? u + 1 : 0, nxt);
                 if (u == 0) {
                     ok = bar_wait<false>(b_free + 8 * s, ((j / STAGES) & 1) ^ 1, ab);
+                    ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    if (SUMS && lw < 2) lse_sh[s][lw * 32 + lane] = lse;
+                    if (SUMS && lt < 64) lse_sh[s][lt] = lse;
                 }
-                const int d = u * 64 + c4 * 4;
                 uint32_t at = ring + s * stage + u * (2 * PLANE) + hw * 128 + (((c4 >> 1) ^ (hw & 7)) << 4) + ((c4 & 1) << 3);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const Look r = from(ra, rb, hw + 8 * i);
                     float4 x = cur[i];
                     if (!SUMS && FOUR) {
                         const uint32_t word = __float_as_uint(x.x), par = __float_as_uint(x.y);
                         const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&par));
-                        x = make_float4(fmaf((float)(word & 15u), sm.x, sm.y), fmaf((float)((word >> 4) & 15u), sm.x, sm.y), fmaf((float)((word >> 8) & 15u), sm.x, sm.y),
-                                        fmaf((float)((word >> 12) & 15u), sm.x, sm.y));
-                        if (r.at < 0 || d >= D) x = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (d + 1 >= D) x.y = 0.f;
-                        if (d + 2 >= D) x.z = 0.f;
-                        if (d + 3 >= D) x.w = 0.f;
+                        auto val = [&](uint32_t c) { return fmaf(__uint_as_float(c | 0x4B000000u) - 8388608.f, sm.x, sm.y); };
+                        x = word & 0x10000u ? make_float4(val(word & 15u), val((word >> 4) & 15u), val((word >> 8) & 15u), val((word >> 12) & 15u)) : make_float4(0.f, 0.f, 0.f, 0.f);
                     }
+                    const float f = SUMS ? fac_sh[j % 3][hw + 8 * i] : UP;
+                    const uint64_t f2 = pk(f, f);
+                    float a0, a1, a2, a3;
+                    upk(mul2(pk(x.x, x.y), f2), a0, a1), upk(mul2(pk(x.z, x.w), f2), a2, a3);
                     uint32_t h0, h1, l0, l1;
-                    split16(x.x * r.f, x.y * r.f, h0, l0);
-                    split16(x.z * r.f, x.w * r.f, h1, l1);
+                    split16(a0, a1, h0, l0);
+                    split16(a2, a3, h1, l1);
                     sts8(at, h0, h1), sts8(at + PLANE, l0, l1);
                     at += 8 * 128;
                 }
             }
-            if (!ok) break;
+            if (!ok) continue;
             async_fence();
             __syncwarp();
             if (lane == 0) bar_arrive(b_full + 8 * s);
-            ra = na, rb = nb;
         }
     } else {
         // ===================== issuer =====================
@@ -518,8 +552,9 @@ WeighTcPlan weigh_tc_plan(const b200seq_step& st, int H, int G, int last, int64_
     const int64_t row_tiles = (rows + NT - 1) / NT, by_rows = row_tiles / 8, cells = (int64_t)st.B * G * p.key_tiles;
     p.parts = clamp(4 * sms / cells, by_rows < 8 ? by_rows : 8);
     p.key_room = (int64_t)p.key_tiles * MT;
-    p.stat_floats = ((size_t)st.T * H * p.stat_parts * 2 + 3) / 4 * 4;
-    p.floats = p.stat_floats + (p.parts > 1 ? (size_t)p.parts * st.B * G * p.key_room : 0);
+    p.lse_floats = ((size_t)st.T * H + 3) / 4 * 4;
+    p.stat_floats = p.stat_parts > 1 ? ((size_t)st.T * H * p.stat_parts * 2 + 3) / 4 * 4 : 0;
+    p.floats = p.lse_floats + p.stat_floats + (p.parts > 1 ? (size_t)p.parts * st.B * G * p.key_room : 0);
     return p;
 }
 
@@ -532,11 +567,15 @@ int weigh_tc(const WeighArgs& w, const b200seq_step& st, const WeighTcPlan& p, f
     const int64_t g0 = (int64_t)p.tiles * w.G, g1 = (int64_t)p.key_tiles * p.parts * w.G * st.B;
     if (g0 > 0x7fffffff || g1 > 0x7fffffff) return fail(B200SEQ_ERR_UNSUPPORTED, "key_weights: too many tiles for one launch");
     TcArgs a = {};
-    a.w = w, a.stat = reinterpret_cast<float2*>(scratch), a.psum = scratch + p.stat_floats, a.stat_parts = p.stat_parts, a.key_room = p.key_room, a.B = st.B;
+    a.w = w, a.w.lse = scratch, a.stat = reinterpret_cast<float2*>(scratch + p.lse_floats), a.psum = scratch + p.lse_floats + p.stat_floats, a.stat_parts = p.stat_parts, a.key_room = p.key_room, a.B = st.B;
     a.parts = p.stat_parts, a.tiles = p.tiles;
     cudaError_t e = run<false>(a, st, dim3((unsigned)g0, 1, p.stat_parts), four, cs);
     if (e != cudaSuccess) return cuda_status(e, "key_weights");
     count_launch();
+    if (p.stat_parts > 1) {
+        launch_chained(weigh_lse_kernel, dim3((unsigned)(((int64_t)st.T * w.H + 127) / 128)), 128, 0, cs, a, st.T * w.H);
+        SEQ_LAUNCH_CHECK("key_weights");
+    }
     a.parts = p.parts, a.tiles = p.key_tiles;
     e = run<true>(a, st, dim3((unsigned)g1), four, cs);
     if (e != cudaSuccess) return cuda_status(e, "key_weights");
