@@ -443,8 +443,9 @@ Plan plan_of(const b200seq_step& st, const b200seq_attn_desc& d, int last, int m
     p.blocks = (int)((p.keys + 64 * p.tiles - 1) / (64 * p.tiles));
     const int64_t floats = (int64_t)st.T * d.H * p.blocks * (64 * p.tiles + 2);
     p.rows = d.D <= 128 && rows <= ROWS_MOST && floats <= ROWS_FLOATS;
-    p.tc = weigh_tc_plan(st, d.H, d.G, last, p.keys);
-    p.floats = p.rows ? (size_t)floats : p.tc.floats;      // (more than the f32 tiles' T * H)
+    p.tc = weigh_tc_plan(st, d.H, d.G, d.D, last, p.keys);
+    const size_t lse = ((size_t)st.T * d.H + 3) / 4 * 4;      // (of the f32 tiles)
+    p.floats = p.rows ? (size_t)floats : d.D <= 128 && p.tc.floats > lse ? p.tc.floats : lse;
     return p;
 }
 

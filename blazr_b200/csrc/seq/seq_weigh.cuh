@@ -17,7 +17,7 @@ struct WeighArgs {
     float scale, softcap;
     int chunk, window, keep_first;
     const float *head_scale, *sink;
-    float* lse;                // [T][H]: base-2 logarithm of every row's sum of exponentials (minus infinity: nothing to give), or nothing (the rows' path)
+    float* lse;                // f32 tiles: [T][H], base-2 logarithm of every row's sum of exponentials (minus infinity: nothing to give)
     float* part;               // work area of the path that is taken
     int key_blocks;            // rows' path: blocks of keys that the longest sequence may need, and as keys
     int64_t key_room;
@@ -89,12 +89,14 @@ static __device__ __noinline__ float plain_score(const WeighArgs& a, const b200s
 
 // Steps of many rows on the tensor cores (seq_weigh_tc.cu): how a step is cut up and the work area it needs (from its host sizes alone), whether a layer's rows suit it, the launches
 struct WeighTcPlan {
-    int tiles, stat_parts;     // denominators: row tiles (bound), parts of a walk
-    int key_tiles, parts;      // sums: key tiles of the longest sequence, parts of a walk
-    int64_t key_room;
-    size_t lse_floats, stat_floats, floats;
+    int qtiles, stage;         // tiles of 64 split rows of a key head (bound), bytes of one
+    int tiles, stat_parts;     // denominators: row tiles of 128 (bound), parts of a walk
+    int key_tiles, parts;      // key tiles of 64 of the longest sequence; sums: parts of a walk
+    int ne, ng;                // entries and key heads of a run
+    int64_t key_room, q_floats, k_floats, lse_floats, stat_floats;
+    size_t floats;
 };
-WeighTcPlan weigh_tc_plan(const b200seq_step& st, int H, int G, int last, int64_t keys);
+WeighTcPlan weigh_tc_plan(const b200seq_step& st, int H, int G, int D, int last, int64_t keys);
 bool weigh_tc_takes(const WeighArgs& a, bool four);
 int weigh_tc(const WeighArgs& a, const b200seq_step& st, const WeighTcPlan& p, float* scratch, bool four, cudaStream_t cs);
 

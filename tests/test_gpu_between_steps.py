@@ -478,6 +478,34 @@ def test_weights_captured_and_on_another_stream(ops):
         assert torch.equal(acc, want[0])
 
 
+@pytest.mark.parametrize("n,past,last,D", [(700, 0, 0, 128), (100, 6000, 60, 64), (3, 5000, 0, 128)])
+def test_calls_behind_one_another(ops, n, past, last, D):
+    """steps of other sequences before and after, with nothing waited for: bit by bit what a call alone gives"""
+    g = torch.Generator(device=DEV)
+    g.manual_seed(n)
+    H, G, keys = 32, 8, past + n
+    pages = -(-keys // 16)
+    layer = ops.attn_desc(H, G, D, D, D ** -0.5, gated=False, kv_shared=True)
+    i32 = lambda x: up(x, np.int32)
+    t = dict(ent=i32(np.zeros(n)), pos=i32(np.arange(past, keys)), start=i32([0, n]), slot=i32([0]), pos0=i32([past]), bt=i32(np.arange(pages)[None]))
+    st = ops.StepDesc(t["ent"].data_ptr(), t["pos"].data_ptr(), t["start"].data_ptr(), t["slot"].data_ptr(), t["pos0"].data_ptr(), t["bt"].data_ptr(), n, 1, pages, 16)
+    sets = [(torch.randn(n, H * D, device=DEV, generator=g), torch.randn(pages, 16, G, D, device=DEV, generator=g)) for _ in range(3)]
+    want = []
+    for q, k in sets:
+        acc = torch.zeros(1, G, keys, device=DEV)
+        ops.key_weights(q, st, layer, k, acc, last=last)
+        torch.cuda.synchronize()
+        want.append(acc)
+    rows = (min(last, n) if last else n) * H // G
+    for acc in want:
+        assert abs(float(acc.double().sum()) - rows * G) < 1e-4 * rows * G
+    for _ in range(25):
+        accs = [torch.zeros(1, G, keys, device=DEV) for _ in sets]
+        for (q, k), acc in zip(sets, accs):
+            ops.key_weights(q, st, layer, k, acc, last=last)
+        assert all(torch.equal(a, b) for a, b in zip(accs, want))
+
+
 # ---- eviction ------------------------------------------------------------------------------------------------------------------------------------
 def bytes_of(pool, bits, bs, G, page, o, g):
     if bits == 32:
