@@ -7,7 +7,7 @@
 // What a row decides is compared with a random number, so that its sums are held in 64 bits (weights are f32, within 2^-21 of themselves; sums of four of them, then f64).
 // The floor is the logits' bytes: they are read once, in slices over the whole GPU (row_stats), with maximum, its place and sum left for every slice.  Then a cluster of eight
 // CTAs an entry puts the slices together, finds the row that rejects and reads that one again, from L2 (pick).
-// top_k and top_p need a threshold a row before that (row_cut, a CTA a row, which it reads twice or three times from L2): counts, or masses (whole numbers of 2^-33: additions whose
+// top_k and top_p need a threshold a row before that (row_cut, a CTA a row, which it reads twice or three times from L2): counts, or masses (whole numbers of 2^-32: additions whose
 // order does not matter), of 2048 bins of equal width below the maximum show how far down the k-th logit lies, or where the mass passes the share; the logits down to there are sorted.
 // Where those are too many (rows of equal logits, logits far apart), the threshold is selected by the bits of the ordered logits instead, eleven at a time.
 #include <cfloat>
@@ -24,6 +24,7 @@ namespace cg = cooperative_groups;
 
 constexpr int ERR_TOKEN = 16;             // error flag: a token id outside the vocabulary
 constexpr int CLUSTER = 8;
+constexpr int QUADS = 8;                  // 16-byte pieces of a slice of a row a thread has
 constexpr int STATS = 256, PICK = 256, CUT = 1024;     // threads
 constexpr int MAX_TILES = 512;            // tiles of 4 * PICK logits of one CTA's share
 constexpr int BINS = 2048, LIST = 2048;   // bins below the maximum; logits that are sorted
@@ -91,7 +92,7 @@ __device__ __forceinline__ int entry_of(const VerifyArgs& a, int row) {
     return e;
 }
 
-// grid (slices, rows): 16 logits a thread, all asked for before anything else.  Small blocks, so that one's sums run beside another's loads (320 rows of 128256: blocks of 1024
+// grid (slices, rows): 4 QUADS logits a thread, all asked for before anything else.  Small blocks, so that one's sums run beside another's loads (320 rows of 128256: blocks of 1024
 // threads 64 us, of 256 40: 4.1 TB/s)
 __global__ void __launch_bounds__(STATS) row_stats_kernel(const __grid_constant__ VerifyArgs a) {
     chain_enter();
@@ -101,10 +102,10 @@ __global__ void __launch_bounds__(STATS) row_stats_kernel(const __grid_constant_
     __shared__ double wsum[WARPS];
     const int row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float* x = a.x + row * a.ld;
-    const int i0 = 4 * (blockIdx.x * 4 * THREADS + threadIdx.x) - quad_shift(x);
-    float4 v[4];
+    const int i0 = 4 * (blockIdx.x * QUADS * THREADS + threadIdx.x) - quad_shift(x);
+    float4 v[QUADS];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = quad(x, i0 + 4 * k * THREADS, a.V, -INFINITY);
+    for (int k = 0; k < QUADS; ++k) v[k] = quad(x, i0 + 4 * k * THREADS, a.V, -INFINITY);
     const int e = entry_of<THREADS>(a, row);
     if (e >= a.B) return;
     const float T = a.temp[e];
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(STATS) row_stats_kernel(const __grid_constant_
     int at = 0x7fffffff;
     bool odd = false;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < QUADS; ++k) {
         const float z[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(STATS) row_stats_kernel(const __grid_constant_
     double sum = 0.0;      // (a slice of minus infinities: nothing)
     if (top > -INFINITY) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) sum += (double)((heat(v[k].x, top) + heat(v[k].y, top)) + (heat(v[k].z, top) + heat(v[k].w, top)));
+        for (int k = 0; k < QUADS; ++k) sum += (double)((heat(v[k].x, top) + heat(v[k].y, top)) + (heat(v[k].z, top) + heat(v[k].w, top)));
     }
     if (odd) sum = NAN;
     sum = warp_sum(sum);
@@ -229,7 +230,7 @@ __device__ __forceinline__ int find_bin(unsigned long long b0, unsigned long lon
 template <class F>
 __device__ __forceinline__ void each_logit(const float* x, int V, F f) {
     const int shift = quad_shift(x), quads = (V + shift + 3) / 4;
-#pragma unroll 4
+#pragma unroll 2
     for (int k = threadIdx.x; k < quads; k += CUT) {
         const int i = 4 * k - shift;
         if (i >= 0 && i + 3 < V) {
@@ -309,35 +310,34 @@ __global__ void __launch_bounds__(CUT, 1) row_cut_kernel(const __grid_constant__
     }
     const float* x = a.x + row * a.ld;
     const float width = (float)BINS / (32.f * fmaxf(T, 1.f));
-    auto bin_of = [&](float z) { return (int)fminf((r.max - z) * width, (float)(BINS - 1)); };
+    bool masses_only = false;                               // (the counts are there)
+    // (numbers made whole by adding 2^23: conversions, like the exponential, go through a unit of a quarter of the rate)
+    auto bin_of = [&](float z) { return (int)(__float_as_uint(fminf((r.max - z) * width, (float)(BINS - 1)) + 8388608.f) & (2 * BINS - 1)); };
     // ---- counts, and masses where they are needed: with top_k, of few logits later ----
     int finite = 0;
-    each_logit(x, a.V, [&](float z) {
-        const int b = bin_of(z);
-        finite += z > -INFINITY;
-        if (b == BINS - 1) return;                          // (the last bin has what the others have not; its masses are below 2^-34)
-        atomicAdd(h32 + b, 1u);
-        if (!by_count) {
-            const float w = heat(z, r.max) * 65536.f, c = floorf(w);
-            const unsigned f = __float2uint_rn((w - c) * 131072.f);      // (32768 of either fit 32 bits)
-            if (c > 0.f) atomicAdd(h32 + BINS + b, (unsigned)c);
-            if (f) atomicAdd(h32 + 2 * BINS + b, f);
-        }
-    });
-    if (by_count && (unsigned long long)k >= block_total((unsigned long long)finite, sh)) {      // (all but minus infinities are kept)
-        by_count = false;
-        if (!by_mass) {
-            if (tid == 0) a.cut[row] = Cut{0.0, 0.f, 0};
-            return;
-        }
+    for (bool again = true; again;) {
         each_logit(x, a.V, [&](float z) {
             const int b = bin_of(z);
-            if (b == BINS - 1) return;
-            const float w = heat(z, r.max) * 65536.f, c = floorf(w);
-            const unsigned f = __float2uint_rn((w - c) * 131072.f);
-            if (c > 0.f) atomicAdd(h32 + BINS + b, (unsigned)c);
-            if (f) atomicAdd(h32 + 2 * BINS + b, f);
+            finite += z > -INFINITY;
+            if (b == BINS - 1) return;                      // (the last bin has what the others have not; its masses are below 2^-34)
+            if (by_count || !masses_only) atomicAdd(h32 + b, 1u);
+            if (!by_count) {
+                const float w = heat(z, r.max) * 65536.f, c = w + 8388608.f;
+                const unsigned whole = __float_as_uint(c) & 0x1ffffu;
+                const int part = (int)(__float_as_uint((w - (c - 8388608.f)) * 65536.f + 12582912.f) - 0x4B400000u);      // (-32768 .. 32768: 32768 of either fit 32 bits)
+                if (whole) atomicAdd(h32 + BINS + b, whole);
+                if (part) atomicAdd(reinterpret_cast<int*>(h32) + 2 * BINS + b, part);
+            }
         });
+        again = false;
+        if (by_count && !masses_only && (unsigned long long)k >= block_total((unsigned long long)finite, sh)) {      // (all but minus infinities are kept)
+            by_count = false;
+            if (!by_mass) {
+                if (tid == 0) a.cut[row] = Cut{0.0, 0.f, 0};
+                return;
+            }
+            again = masses_only = true;
+        }
     }
     __syncthreads();
     const int b0 = 2 * tid, b1 = b0 + 1;
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(CUT, 1) row_cut_kernel(const __grid_constant__
         want = (unsigned long long)k;
         b = find_bin<false>(c0, c1, want, before, sh);
     } else {
-        const unsigned long long m0 = ((unsigned long long)h32[BINS + b0] << 17) + h32[2 * BINS + b0], m1 = ((unsigned long long)h32[BINS + b1] << 17) + h32[2 * BINS + b1];
+        const unsigned long long m0 = ((unsigned long long)h32[BINS + b0] << 16) + (long long)(int)h32[2 * BINS + b0], m1 = ((unsigned long long)h32[BINS + b1] << 16) + (long long)(int)h32[2 * BINS + b1];
         all_mass = block_total(m0 + m1, sh);
         const double t = ceil((double)share * (double)all_mass);
         want = t >= 1.0 ? (unsigned long long)t : 1ull;
@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(CUT, 1) row_cut_kernel(const __grid_constant__
     }
     // the logits of this bin and of those before it, sorted; or, where top_p is all there is, of this bin alone
     unsigned n = (unsigned)min(block_total((b0 <= b ? c0 : 0ull) + (b1 <= b ? c1 : 0ull), sh), (unsigned long long)LIST + 1);
-    const bool alone = n > LIST && !by_count;
+    const bool alone = n > LIST / 4 && !by_count;           // (a pass over the row takes less than sorting so many)
     if (alone) n = (unsigned)min(block_total((b0 == b ? c0 : 0ull) + (b1 == b ? c1 : 0ull), sh), (unsigned long long)LIST + 1);
     uint32_t least;
     double total = 0.0;
@@ -382,12 +382,15 @@ __global__ void __launch_bounds__(CUT, 1) row_cut_kernel(const __grid_constant__
         for (int run = 2; run <= size; run <<= 1)           // bitonic, the largest first
             for (int step = run >> 1; step > 0; step >>= 1) {
                 if (tid < size / 2) {
-                    const int at = 2 * step * (tid / step) + tid % step, to = at + step;
+                    const int at = ((tid & ~(step - 1)) << 1) | (tid & (step - 1)), to = at + step;
                     const unsigned u = list[at], v = list[to];
                     if ((u < v) == ((at & run) == 0)) list[at] = v, list[to] = u;
                 }
-                __syncthreads();
+                // (a warp has 64 neighbours to itself: shorter steps stay within them)
+                if (step > 32 || (step == 1 && run >= 64)) __syncthreads();
+                else __syncwarp();
             }
+        __syncthreads();
         least = by_count ? list[k - 1] : 0;
         double w[2];                                        // two neighbours a thread, of those that top_k leaves
         uint32_t key[2];
@@ -398,8 +401,8 @@ __global__ void __launch_bounds__(CUT, 1) row_cut_kernel(const __grid_constant__
         }
         double* const d = reinterpret_cast<double*>(sh);
         if (by_mass) {
-            const double all = by_count ? block_total(w[0] + w[1], d) : (double)all_mass * 0x1p-33, goal = (double)share * all;
-            const double up = block_before<double, false>(w[0] + w[1], d) + (alone ? (double)before * 0x1p-33 : 0.0);
+            const double all = by_count ? block_total(w[0] + w[1], d) : (double)all_mass * 0x1p-32, goal = (double)share * all;
+            const double up = block_before<double, false>(w[0] + w[1], d) + (alone ? (double)before * 0x1p-32 : 0.0);
             // the last one with less than the goal before it (the largest always)
             uint32_t last = tid == 0 ? key[0] : 0xffffffffu;
             if (w[0] > 0.0 && up < goal) last = key[0];
@@ -602,7 +605,7 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_ker
     cl.sync();                                              // nobody's sums go while they are read
 }
 
-int slices_of(int V) { return (V + 3 + 16 * STATS - 1) / (16 * STATS); }
+int slices_of(int V) { return (V + 3 + 4 * QUADS * STATS - 1) / (4 * QUADS * STATS); }
 
 }  // namespace
 
