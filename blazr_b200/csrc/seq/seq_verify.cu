@@ -5,6 +5,8 @@
 // rejected (from p where that is nothing), or from the last row's p: the lowest one whose cumulated weight exceeds u times the sum.  T <= 0: p = 1 at the first maximum.
 //
 // What a row decides is compared with a random number, so that its sums are held in 64 bits (weights are f32, within 2^-21 of themselves; sums of four of them, then f64).
+// Measured: 64 entries of 4 drafts, 128256 logits a row, 58 us (35 + 27; the logits' bytes alone 25, the draft's probabilities of a row an entry 5); one of 32000 logits 18.6, a chain of
+// loads and of the clusters' barriers; 16 entries of 3 drafts with top_k and top_p 52 to 55 (thresholds 40).
 // The floor is the logits' bytes: they are read once, in slices over the whole GPU (row_stats), with maximum, its place and sum left for every slice.  Then a cluster of eight
 // CTAs an entry puts the slices together, finds the row that rejects and reads that one again, from L2 (pick).
 // top_k and top_p need a threshold a row before that (row_cut, a CTA a row, which it reads twice or three times from L2): counts, or masses (whole numbers of 2^-32: additions whose

@@ -8,7 +8,11 @@
 // low parts (times 2^11), so that two products a step give all four: 22 bits, at any size of the keys that f16 has.  What has no such parts gives no number and is made again in f32.  The scores
 // go to the work area (4 bytes a row and key against the key's 4 D), with every block's maximum and sum a row; a second launch has every row's denominator from the blocks' and
 // adds the weights up, key by key, the rows in their order: no atomics.
+// Measured: 32 sequences of 2000 to 4000 keys, 32 query heads of 8 key heads of 128, 88 to 91 us (75 and 11, 5.4 TB/s of keys in the first), one of 131072 keys 116 to 121 (100
+// and 15; 4.5 TB/s over both); what the first launch spends are instructions: 364 of a warp for eight keys, two a cycle and SM.  (In f32 multiply-adds: 123 and 149.)
 // Many rows: seq_weigh_tc.cu.  What neither takes (heads above 128 or of odd sizes) goes through f32 tiles here, twice: once for the denominators, once for the sums.
+#include <cooperative_groups.h>
+
 #include "seq_weigh.cuh"
 #include "tc_split.cuh"
 
@@ -21,7 +25,15 @@ using tcsplit::ex2;
 // ---- rows path ------------------------------------------------------------------------------------------------------------------------------
 constexpr int RT = 256, RW = RT / 32;  // threads, warps
 constexpr int FT = 256, FK = 4 * FT;   // second launch: threads, keys of a block
+constexpr int MOST_TILES = 16;         // of eight keys of a warp
 constexpr float LOW = 0x1p11f, UNLOW = 0x1p-11f;
+
+// the base-2 logarithm of a row's denominator from its maximum and sum; infinite where the row gives nothing
+__device__ __forceinline__ float denominator(const WeighArgs& a, int h, float m, float l) {
+    if (l != l) return l;
+    const float v = weigh_lse(a, h, m, l);
+    return v == -INFINITY ? INFINITY : v;
+}
 
 // work area of the rows path: [T][H][key_room] scores in base 2, then [T][H][key_blocks] (maximum, sum)
 __device__ __forceinline__ float* rows_scores(const WeighArgs& a, int64_t row) { return a.part + row * a.key_room; }
@@ -36,76 +48,111 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t
 __device__ __forceinline__ void split_up(float a, float b, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(a, b);
     const float2 f = __half22float2(h);
-    float x, y;
-    tcsplit::upk(tcsplit::mul2(tcsplit::pk(a - f.x, b - f.y), tcsplit::pk(LOW, LOW)), x, y);
+    float x, y;      // (x - h) 2^11: both products are exact
+    tcsplit::upk(tcsplit::fma2(tcsplit::pk(f.x, f.y), tcsplit::pk(-LOW, -LOW), tcsplit::mul2(tcsplit::pk(a, b), tcsplit::pk(LOW, LOW))), x, y);
     const __half2 l = __floats2half2_rn(x, y);
     hi = *reinterpret_cast<const uint32_t*>(&h), lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 
-// What a lane has of a key: of every group of 32 values the eight from 8 c on (c: lane & 3)
+// What a lane has of a key (c: lane & 3).  4-bit keys: of every group of 32 values the eight from 8 c on, codes and parameters in registers, a tile ahead.  f32 ones: of every 16 values the
+// four from 4 c on, on their way to the lane's own places of a ring in shared memory, two tiles ahead (in registers there was room for one: with eight tiles a warp 32 sequences 97 us, now 93; one of 131072
+// keys 119 either way).
+constexpr int RING = 3;
 template <int NG, bool FOUR>
 struct KeyPart {
-    float4 x[FOUR ? 1 : 2 * NG];
     uint32_t code[FOUR ? NG : 1], par[FOUR ? NG : 1];
     __device__ __forceinline__ void fetch(const WeighArgs& a, int page, int o, int bs, int g, int c) {
-        if constexpr (FOUR) {
-            const Kv4Row r = kv4_row(page, o, bs, g, a.G, NG);
-            const uint8_t *k = a.kpool4 + r.codes + c * NG * 4, *p = a.kpool4 + r.params;
-            if constexpr (NG == 4) {
-                const uint4 u = *reinterpret_cast<const uint4*>(k), v = *reinterpret_cast<const uint4*>(p);
-                code[0] = u.x, code[1] = u.y, code[2] = u.z, code[3] = u.w, par[0] = v.x, par[1] = v.y, par[2] = v.z, par[3] = v.w;
-            } else if constexpr (NG == 2) {
-                const uint2 u = *reinterpret_cast<const uint2*>(k), v = *reinterpret_cast<const uint2*>(p);
-                code[0] = u.x, code[1] = u.y, par[0] = v.x, par[1] = v.y;
-            } else {
-                code[0] = *reinterpret_cast<const uint32_t*>(k), par[0] = *reinterpret_cast<const uint32_t*>(p);
-            }
+        const Kv4Row r = kv4_row(page, o, bs, g, a.G, NG);
+        const uint8_t *k = a.kpool4 + r.codes + c * NG * 4, *p = a.kpool4 + r.params;
+        if constexpr (NG == 4) {
+            const uint4 u = *reinterpret_cast<const uint4*>(k), v = *reinterpret_cast<const uint4*>(p);
+            code[0] = u.x, code[1] = u.y, code[2] = u.z, code[3] = u.w, par[0] = v.x, par[1] = v.y, par[2] = v.z, par[3] = v.w;
+        } else if constexpr (NG == 2) {
+            const uint2 u = *reinterpret_cast<const uint2*>(k), v = *reinterpret_cast<const uint2*>(p);
+            code[0] = u.x, code[1] = u.y, par[0] = v.x, par[1] = v.y;
         } else {
-            const float* row = a.kpool + (((int64_t)page * bs + o) * a.G + g) * a.D + 8 * c;
-#pragma unroll
-            for (int i = 0; i < 2 * NG; ++i) {
-                const int d = 32 * (i >> 1) + 4 * (i & 1);
-                x[i] = d + 8 * c < a.D ? ld4(row + d) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
+            code[0] = *reinterpret_cast<const uint32_t*>(k), par[0] = *reinterpret_cast<const uint32_t*>(p);
         }
     }
     // the four values of step kk (two steps a group)
     __device__ __forceinline__ float4 step(int kk) const {
-        if constexpr (FOUR) {
-            const uint32_t w = code[kk >> 1] >> (16 * (kk & 1)), p = par[kk >> 1];
-            const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&p));
-            // (a code in the mantissa of 2^23: that number more)
-            auto val = [&](uint32_t u) { return fmaf(__uint_as_float(u | 0x4B000000u) - 8388608.f, sm.x, sm.y); };
-            return make_float4(val(w & 15u), val((w >> 4) & 15u), val((w >> 8) & 15u), val((w >> 12) & 15u));
-        } else {
-            return x[kk];
-        }
+        const uint32_t w = code[kk >> 1] >> (16 * (kk & 1)), p = par[kk >> 1];
+        const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(&p));
+        // (a code in the mantissa of 2^23: that number more)
+        auto val = [&](uint32_t u) { return fmaf(__uint_as_float(u | 0x4B000000u) - 8388608.f, sm.x, sm.y); };
+        return make_float4(val(w & 15u), val((w >> 4) & 15u), val((w >> 8) & 15u), val((w >> 12) & 15u));
     }
 };
+// pieces of an f32 key to `dst` + 512 i (places behind the head's values: zeros)
+template <int NG>
+__device__ __forceinline__ void fetch_key(const WeighArgs& a, uint32_t dst, int page, int o, int bs, int g, int c) {
+    const float* row = a.kpool + (((int64_t)page * bs + o) * a.G + g) * a.D + 4 * c;
+#pragma unroll
+    for (int i = 0; i < 2 * NG; ++i) {
+        const int d = 16 * i;
+        const bool in = d + 4 * c < a.D;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 512 * i), "l"(in ? row + d : a.kpool), "r"(in ? 16 : 0) : "memory");
+    }
+}
 
-// grid (blocks of 64 * tiles keys, key heads, entries).  NRT: tiles of eight rows that are gone through at a time
-template <int NRT, int NG, bool FOUR>
+// grid (blocks of 64 * tiles keys, key heads, entries).  NRT: tiles of eight rows that are gone through at a time.  JOINED: a sequence's blocks are one cluster, which joins their
+// maxima and sums itself and adds the weights up at once.  (For steps whose blocks are all on the GPU together: one token of 500 keys 14.2 -> 11.7 us; in several waves the blocks
+// that wait for one another keep others out, 32 sequences 88 -> 137.)
+template <int NRT, int NG, bool FOUR, bool JOINED>
 __global__ void __launch_bounds__(RT, 2) weigh_rows_kernel(const __grid_constant__ WeighArgs a, const __grid_constant__ b200seq_step st, int tiles) {
     chain_enter();
+    extern __shared__ __align__(16) float4 ring[];      // f32: [warp][RING][2 NG][lane]
     __shared__ uint4 frag[NRT][2 * NG][32];
-    __shared__ float2 part[RW][NRT * 8];
+    __shared__ float2 part[RW][NRT * 8], fin[NRT * 8];
+    __shared__ float den[NRT * 8];
     const int e = blockIdx.z, g = blockIdx.y, k0 = blockIdx.x * 64 * tiles, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, c = lane & 3, r8 = lane >> 2;
     const WeighEntry en(a, st, e, blockIdx.x == 0 && g == 0 && tid == 0);
-    if (en.n == 0 || k0 >= en.keys) return;
+    if (en.n == 0 || (k0 >= en.keys && !JOINED)) return;      // (a cluster's blocks stay together)
     const int R = a.H / a.G, rows = en.n * R, bs = st.block_size, hi = en.keys - 1;
+    float total[MOST_TILES / 4];                             // JOINED: the weights of keys k0 + tid + 256 q
+#pragma unroll
+    for (int q = 0; q < MOST_TILES / 4; ++q) total[q] = 0.f;
     const int32_t* bt = st.block_table + (int64_t)e * st.max_blocks;
-    // a warp's keys: k0 + 8 (warp + 8 i), of which a lane has key lane / 4
-    auto key_of = [&](int i) { return min(k0 + 8 * (warp + RW * i) + r8, hi); };
-    auto page_of = [&](int i) { return kv4_page_read(bt[key_of(i) / bs], a.err); };
+    // a warp's keys: k0 + 8 (warp + 8 i) ..., of which a lane has key lane / 4
+    // (place in the table and row of the page of the next one that is looked up, and of the next one that is fetched: 64 keys on each time, without a division)
+    const int key_first = k0 + 8 * warp + r8, on_pages = 64 / bs, on_rows = 64 - on_pages * bs, hi_page = hi / bs, hi_row = hi - hi_page * bs;
+    int look_page, look_row, row_page, row_row;
+    auto restart = [&]() { look_page = row_page = key_first / bs, look_row = row_row = key_first - look_page * bs; };
+    auto next_page = [&]() {      // pages in the order of the tiles (behind the last key: its page)
+        const int page = kv4_page_read(bt[min(look_page, hi_page)], a.err);
+        look_page += on_pages, look_row += on_rows;
+        if (look_row >= bs) look_row -= bs, ++look_page;
+        return page;
+    };
+    auto next_row = [&]() {       // and rows
+        const int row = row_page > hi_page || (row_page == hi_page && row_row > hi_row) ? hi_row : row_row;
+        row_page += on_pages, row_row += on_rows;
+        if (row_row >= bs) row_row -= bs, ++row_page;
+        return row;
+    };
     const bool cap = a.softcap > 0.f;
     for (int r0 = 0; r0 < rows; r0 += NRT * 8) {
+        restart();
         KeyPart<NG, FOUR> nxt, cur;
-        int page = page_of(0);
-        nxt.fetch(a, page, key_of(0) % bs, bs, g, c);
-        page = tiles > 1 ? page_of(1) : 0;
+        const float4* const mine = ring + warp * (RING * 2 * NG * 32) + lane;
+        const uint32_t mine_at = tcpair::sa(mine);
+        int page;
+        if constexpr (FOUR) {
+            page = next_page();
+            nxt.fetch(a, page, next_row(), bs, g, c);
+            page = tiles > 1 ? next_page() : 0;
+        } else {
+            const int first = next_page(), second = tiles > 1 ? next_page() : 0;
+            page = tiles > 2 ? next_page() : 0;
+            fetch_key<NG>(a, mine_at, first, next_row(), bs, g, c);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (tiles > 1) fetch_key<NG>(a, mine_at + 1024 * NG, second, next_row(), bs, g, c);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
         __syncthreads();
         for (int i = tid; i < NRT * 2 * NG * 32; i += RT) {
-            const int ln = i & 31, kk = (i >> 5) % (2 * NG), rt = i / (64 * NG), row = r0 + 8 * rt + (ln >> 2), d = 32 * (kk >> 1) + 8 * (ln & 3) + 4 * (kk & 1);
+            const int ln = i & 31, kk = (i >> 5) % (2 * NG), rt = i / (64 * NG), row = r0 + 8 * rt + (ln >> 2);
+            const int d = FOUR ? 32 * (kk >> 1) + 8 * (ln & 3) + 4 * (kk & 1) : 16 * kk + 4 * (ln & 3);
             uint4 f = make_uint4(0, 0, 0, 0);
             if (row < rows) {
                 const int h = g * R + row % R;
@@ -133,14 +180,26 @@ __global__ void __launch_bounds__(RT, 2) weigh_rows_kernel(const __grid_constant
         const int keep = a.window > 0 ? a.keep_first : 0, pos_least = en.p0 + r0 / R;
         const WeighSpan last(a, en.p0 + min(rows - 1, r0 + NRT * 8 - 1) / R);
         const int lo_most = last.lo;
+        int slot = 0;
 #pragma unroll 1
         for (int i = 0; i < tiles; ++i) {
             const int key0 = k0 + 8 * (warp + RW * i);
             if (key0 > hi) break;
-            cur = nxt;
-            if (i + 1 < tiles) {
-                nxt.fetch(a, page, key_of(i + 1) % bs, bs, g, c);
-                if (i + 2 < tiles) page = page_of(i + 2);
+            const float4* const now = mine + slot * (2 * NG * 32);
+            if constexpr (FOUR) {
+                cur = nxt;
+                if (i + 1 < tiles) {
+                    nxt.fetch(a, page, next_row(), bs, g, c);
+                    if (i + 2 < tiles) page = next_page();
+                }
+            } else {
+                if (i + 2 < tiles) {
+                    fetch_key<NG>(a, mine_at + (slot == 0 ? 2 : slot - 1) * (1024 * NG), page, next_row(), bs, g, c);
+                    if (i + 3 < tiles) page = next_page();
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                asm volatile("cp.async.wait_group 2;" ::: "memory");
+                slot = slot == 2 ? 0 : slot + 1;
             }
             float ah[NRT][4], al[NRT][4];
 #pragma unroll
@@ -149,7 +208,9 @@ __global__ void __launch_bounds__(RT, 2) weigh_rows_kernel(const __grid_constant
                 for (int j = 0; j < 4; ++j) ah[rt][j] = al[rt][j] = 0.f;
 #pragma unroll
             for (int kk = 0; kk < 2 * NG; ++kk) {
-                const float4 x = cur.step(kk);
+                float4 x;
+                if constexpr (FOUR) x = cur.step(kk);
+                else x = now[kk * 32];
                 uint32_t h0, h1, l0, l1;
                 split_up(x.x, x.y, h0, l0), split_up(x.z, x.w, h1, l1);
 #pragma unroll
@@ -201,13 +262,48 @@ __global__ void __launch_bounds__(RT, 2) weigh_rows_kernel(const __grid_constant
                 const float2 x = part[w][tid];
                 s += x.x == -INFINITY ? x.y : x.y * ex2(x.x - top);
             }
-            rows_stats(a, st.T, (int64_t)(en.t0 + row / R) * a.H + g * R + row % R)[blockIdx.x] = make_float2(top, s);
+            if constexpr (JOINED) fin[tid] = make_float2(top, s);
+            else rows_stats(a, st.T, (int64_t)(en.t0 + row / R) * a.H + g * R + row % R)[blockIdx.x] = make_float2(top, s);
+        }
+        if constexpr (JOINED) {
+            auto cl = cooperative_groups::this_cluster();
+            cl.sync();                                      // (and this block's scores are written)
+            if (tid < NRT * 8 && r0 + tid < rows) {
+                float2 x[8];
+                float top = -INFINITY, s = 0.f;
+#pragma unroll
+                for (int b = 0; b < 8; ++b) {
+                    x[b] = b < (int)gridDim.x ? *cl.map_shared_rank(fin + tid, b) : make_float2(-INFINITY, 0.f);
+                    top = fmaxf(top, x[b].x);
+                }
+#pragma unroll
+                for (int b = 0; b < 8; ++b) s += x[b].x == -INFINITY ? x[b].y : x[b].y * ex2(x[b].x - top);
+                den[tid] = denominator(a, g * R + (r0 + tid) % R, top, s);
+            }
+            __syncthreads();
+            const int nr = min(NRT * 8, rows - r0);
+#pragma unroll
+            for (int q = 0; q < MOST_TILES / 4; ++q) {
+                const int at = tid + RT * q, key = k0 + at;
+                if (at >= 64 * tiles || key > hi) continue;
+#pragma unroll 8
+                for (int r = 0; r < nr; ++r) total[q] += ex2(rows_scores(a, (int64_t)(en.t0 + (r0 + r) / R) * a.H + g * R + (r0 + r) % R)[key] - den[r]);
+            }
+            cl.sync();                                      // nobody's sums go while they are read
+        }
+    }
+    if constexpr (JOINED) {
+        float* acc = a.acc + ((int64_t)en.slot * a.G + g) * a.acc_ld;
+#pragma unroll
+        for (int q = 0; q < MOST_TILES / 4; ++q) {
+            const int at = tid + RT * q, key = k0 + at;
+            if (at < 64 * tiles && key <= hi) acc[key] = key < en.fresh ? acc[key] + total[q] : total[q];
         }
     }
 }
 
 // grid (blocks of FK keys, key heads, entries)
-__global__ void __launch_bounds__(FT) weigh_join_kernel(const __grid_constant__ WeighArgs a, const __grid_constant__ b200seq_step st, int block_keys) {
+__global__ void __launch_bounds__(FT, 3) weigh_join_kernel(const __grid_constant__ WeighArgs a, const __grid_constant__ b200seq_step st, int block_keys) {
     chain_enter();
     constexpr int ROWS = 32;
     __shared__ float den[ROWS];
@@ -244,10 +340,7 @@ __global__ void __launch_bounds__(FT) weigh_join_kernel(const __grid_constant__ 
                 l += x.x == -INFINITY ? x.y : x.y * ex2(x.x - top);      // (a block without a key to see: 0, or no number)
             }
             l = warp_sum(l);
-            if (lane == 0) {
-                const float v = weigh_lse(a, h, top, l);
-                den[r] = l != l ? l : v == -INFINITY ? INFINITY : v;
-            }
+            if (lane == 0) den[r] = denominator(a, h, top, l);
         }
         __syncthreads();
         if (key < en.keys) {
@@ -267,12 +360,42 @@ __global__ void __launch_bounds__(FT) weigh_join_kernel(const __grid_constant__ 
         if (key + i < en.keys) acc[key + i] = old[i] + s[i];
 }
 
+// How a step is run.  Rows that share a key head in one entry: up to ROWS_MOST go through the rows path, whose time grows with them, if its scores fit the work area that it may have.
+constexpr int ROWS_MOST = 64;
+constexpr int64_t ROWS_FLOATS = 64 << 20;
+struct Plan {
+    bool rows, joined;                 // rows path; in one launch
+    int row_tiles, tiles, blocks;      // rows path: tiles of eight rows at a time, tiles of eight keys of a warp, blocks of keys of the longest sequence
+    int64_t keys;      // of a sequence: a bound, a multiple of 128
+    int tokens;        // tokens of an entry that count: a bound
+    WeighTcPlan tc;
+    size_t floats;
+};
+template <int NRT, int NG, bool FOUR, bool JOINED>
+cudaError_t launch_rows(const WeighArgs& a, const b200seq_step& st, dim3 grid, int tiles, cudaStream_t cs) {
+    const int smem = FOUR ? 0 : RW * RING * 2 * NG * 512;
+    if (smem > 36 * 1024) {      // (beside the fragments)
+        const cudaError_t e = cudaFuncSetAttribute(weigh_rows_kernel<NRT, NG, FOUR, JOINED>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension, attr[1].val.clusterDim.x = JOINED ? grid.x : 1, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+    cfg.gridDim = grid, cfg.blockDim = RT, cfg.dynamicSmemBytes = smem, cfg.stream = cs, cfg.attrs = attr, cfg.numAttrs = JOINED ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, weigh_rows_kernel<NRT, NG, FOUR, JOINED>, a, st, tiles);
+    return cudaGetLastError();
+}
+template <int NRT, int NG, bool FOUR>
+cudaError_t launch_rows(const WeighArgs& a, const b200seq_step& st, dim3 grid, int tiles, bool joined, cudaStream_t cs) {
+    return joined ? launch_rows<NRT, NG, FOUR, true>(a, st, grid, tiles, cs) : launch_rows<NRT, NG, FOUR, false>(a, st, grid, tiles, cs);
+}
 template <int NG, bool FOUR>
-void launch_rows(const WeighArgs& a, const b200seq_step& st, dim3 grid, int row_tiles, int tiles, cudaStream_t cs) {
-    if (row_tiles == 1) launch_chained(weigh_rows_kernel<1, NG, FOUR>, grid, RT, 0, cs, a, st, tiles);
-    else if (row_tiles == 2) launch_chained(weigh_rows_kernel<2, NG, FOUR>, grid, RT, 0, cs, a, st, tiles);
-    else if (row_tiles == 3) launch_chained(weigh_rows_kernel<3, NG, FOUR>, grid, RT, 0, cs, a, st, tiles);
-    else launch_chained(weigh_rows_kernel<4, NG, FOUR>, grid, RT, 0, cs, a, st, tiles);
+cudaError_t launch_rows(const WeighArgs& a, const b200seq_step& st, dim3 grid, const Plan& p, cudaStream_t cs) {
+    if (p.row_tiles == 1) return launch_rows<1, NG, FOUR>(a, st, grid, p.tiles, p.joined, cs);
+    if (p.row_tiles == 2) return launch_rows<2, NG, FOUR>(a, st, grid, p.tiles, p.joined, cs);
+    if (p.row_tiles == 3) return launch_rows<3, NG, FOUR>(a, st, grid, p.tiles, p.joined, cs);
+    return launch_rows<4, NG, FOUR>(a, st, grid, p.tiles, p.joined, cs);
 }
 
 // ---- f32 tiles ------------------------------------------------------------------------------------------------------------------------------
@@ -417,17 +540,6 @@ int check(const b200seq_step* st, const b200seq_attn_desc* d, int kv_bits) {
     return 0;
 }
 
-// How a step is run.  Rows that share a key head in one entry: up to ROWS_MOST go through the rows path, whose time grows with them, if its scores fit the work area that it may have.
-constexpr int ROWS_MOST = 64;
-constexpr int64_t ROWS_FLOATS = 64 << 20;
-struct Plan {
-    bool rows;
-    int row_tiles, tiles, blocks;      // rows path: tiles of eight rows at a time, tiles of eight keys of a warp, blocks of keys of the longest sequence
-    int64_t keys;      // of a sequence: a bound, a multiple of 128
-    int tokens;        // tokens of an entry that count: a bound
-    WeighTcPlan tc;
-    size_t floats;
-};
 Plan plan_of(const b200seq_step& st, const b200seq_attn_desc& d, int last, int max_keys) {
     Plan p;
     const int64_t held = (int64_t)st.max_blocks * st.block_size;
@@ -437,10 +549,11 @@ Plan plan_of(const b200seq_step& st, const b200seq_attn_desc& d, int last, int m
     p.tokens = last > 0 && last < st.T ? last : st.T;
     const int64_t rows = (int64_t)tokens * (d.H / d.G);
     p.row_tiles = rows <= 8 ? 1 : rows <= 16 ? 2 : rows <= 24 || (rows > 32 && rows <= 48) ? 3 : 4;
-    // a warp goes through as many tiles, up to eight, as leave four blocks an SM
+    // a warp goes through as many tiles, up to sixteen, as leave four blocks an SM
     p.tiles = 1;
-    while (p.tiles < 8 && p.keys * d.G * st.B / (128 * p.tiles) >= 4 * 148) p.tiles *= 2;
+    while (p.tiles < MOST_TILES && p.keys * d.G * st.B / (128 * p.tiles) >= 4 * 148) p.tiles *= 2;
     p.blocks = (int)((p.keys + 64 * p.tiles - 1) / (64 * p.tiles));
+    p.joined = p.blocks <= 8 && (int64_t)p.blocks * d.G * st.B <= 2 * 148;
     const int64_t floats = (int64_t)st.T * d.H * p.blocks * (64 * p.tiles + 2);
     p.rows = d.D <= 128 && rows <= ROWS_MOST && floats <= ROWS_FLOATS;
     p.tc = weigh_tc_plan(st, d.H, d.G, d.D, last, p.keys);
@@ -481,12 +594,15 @@ int b200seq_key_weights(const float* proj, int64_t ld, const b200seq_step* st, c
     if (p.rows && wide) {
         a.part = scratch, a.key_blocks = p.blocks, a.key_room = (int64_t)p.blocks * 64 * p.tiles;
         const dim3 grid(p.blocks, d->G, st->B);
-        if (four && a.NG == 1) launch_rows<1, true>(a, *st, grid, p.row_tiles, p.tiles, cs);
-        else if (four && a.NG == 2) launch_rows<2, true>(a, *st, grid, p.row_tiles, p.tiles, cs);
-        else if (four) launch_rows<4, true>(a, *st, grid, p.row_tiles, p.tiles, cs);
-        else if (d->D <= 64) launch_rows<2, false>(a, *st, grid, p.row_tiles, p.tiles, cs);
-        else launch_rows<4, false>(a, *st, grid, p.row_tiles, p.tiles, cs);
-        SEQ_LAUNCH_CHECK("key_weights");
+        cudaError_t e;
+        if (four && a.NG == 1) e = launch_rows<1, true>(a, *st, grid, p, cs);
+        else if (four && a.NG == 2) e = launch_rows<2, true>(a, *st, grid, p, cs);
+        else if (four) e = launch_rows<4, true>(a, *st, grid, p, cs);
+        else if (d->D <= 64) e = launch_rows<2, false>(a, *st, grid, p, cs);
+        else e = launch_rows<4, false>(a, *st, grid, p, cs);
+        if (e != cudaSuccess) return cuda_status(e, "key_weights");
+        count_launch();
+        if (p.joined) return 0;
         launch_chained(weigh_join_kernel, dim3((unsigned)((a.key_room + FK - 1) / FK), d->G, st->B), FT, 0, cs, a, *st, 64 * p.tiles);
         SEQ_LAUNCH_CHECK("key_weights");
         return 0;

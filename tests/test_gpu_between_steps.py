@@ -215,6 +215,18 @@ def test_many_entries(ops):
     assert same(run_verify(ops, z, start, drafts, ua, us, T), want, start) > B - 40
 
 
+def test_no_rows_and_no_entries(ops):
+    e = lambda n, t=torch.float32: torch.zeros(n, dtype=t, device=DEV)
+    i32 = torch.int32
+    acc, tok = ops.verify_drafts(torch.zeros(0, 50, device=DEV), e(4, i32), e(0, i32), e(0), e(3), torch.ones(3, device=DEV))
+    assert acc.tolist() == [0, 0, 0] and tok.numel() == 0
+    tok = torch.full((2,), 7, dtype=i32, device=DEV)
+    acc, tok = ops.verify_drafts(torch.zeros(2, 50, device=DEV), e(1, i32), e(2, i32), e(2), e(0), e(0), tokens=tok)
+    assert acc.numel() == 0 and tok.tolist() == [7, 7]
+    acc, tok = ops.verify_drafts(torch.zeros(2, 50, device=DEV), torch.tensor([1, 2], dtype=i32, device=DEV), e(2, i32), e(2), e(1), e(1), tokens=tok)      # a row of nobody's
+    assert acc.tolist() == [0] and tok.tolist() == [7, 0] and ops.error_flags() == 0
+
+
 def captured(run):
     run()
     torch.cuda.synchronize()
