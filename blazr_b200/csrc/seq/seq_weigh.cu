@@ -245,6 +245,8 @@ __global__ void __launch_bounds__(RT, 2) weigh_rows_kernel(const __grid_constant
                 if (pos[rt] >= 0) *reinterpret_cast<float2*>(out[rt] + key) = make_float2(z[0], z[1]);
             }
         }
+        // (a warp that ran out of keys has copies on their way, to places that the next rows' copies go to as well: two copies to one place have no order)
+        if constexpr (!FOUR) asm volatile("cp.async.wait_all;" ::: "memory");
 #pragma unroll
         for (int rt = 0; rt < NRT; ++rt) {      // a row's four lanes, then the warps
             float top = m[rt];

@@ -360,6 +360,13 @@ def test_weights_of_few_rows(ops, case, bits):
     weigh(ops, s, 14, wide=8)
 
 
+def test_rows_that_take_several_passes_over_a_short_last_block(ops):
+    """48 rows an entry go in two passes over its keys; most warps run out of keys before the last block's end"""
+    rng = np.random.default_rng(31)
+    s = Step(ops, rng, [12] * 32, [int(k) for k in rng.integers(500, 620, 32)], 32, 8, 128)
+    weigh(ops, s, 128 + 14)
+
+
 @pytest.mark.parametrize("kw", [dict(window=50), dict(window=50, keep_first=4), dict(chunk=64), dict(softcap=5.0), dict(sink=True), dict(head_scale=True), dict(scale=-0.3), dict(window=1), dict(last=2),
                                 dict(softcap=2.0, sink=True, head_scale=True, window=40, keep_first=3)], ids=str)
 @pytest.mark.parametrize("bits", [32, 4])
