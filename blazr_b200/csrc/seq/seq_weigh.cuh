@@ -47,7 +47,7 @@ struct WeighEntry {
         t0 = s1 - n, keys = fresh + len, p0 = keys - n;
         const bool fine = s0 >= 0 && len >= 0 && s1 <= st.T && fresh >= 0 && slot >= 0 && slot < a.slots && keys <= a.acc_ld && keys <= a.most_keys && (keys + st.block_size - 1) / st.block_size <= st.max_blocks;
         if (!fine) {
-            if (tell && len > 0) atomicOr(a.err, 1);
+            if (tell && len != 0) atomicOr(a.err, 1);
             n = 0;
         } else if (len == 0) {
             n = 0;

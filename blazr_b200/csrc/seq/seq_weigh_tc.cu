@@ -77,6 +77,9 @@ __device__ __forceinline__ int first_qtile(const WeighArgs& a, const b200seq_ste
     return before * a.G + g * ((n * R + NT - 1) / NT);
 }
 
+// whether the split tiles of an entry's key heads lie within the work area (not all do where the entries' tokens overlap: its size is that of tokens of one entry each); q0: of head g
+__device__ __forceinline__ bool tiles_fit(const TcArgs& a, int q0, int g, int n, int R) { return q0 + (int64_t)(a.w.G - g) * ((n * R + NT - 1) / NT) <= a.qrows / NT; }
+
 // the key tiles that a tile of rows (tokens at p_first .. p_last) sees, in their order
 struct KeyWalk {
     int first, main0, total;
@@ -172,6 +175,7 @@ __global__ void __launch_bounds__(256) weigh_split_kernel(const __grid_constant_
         if (!find_rows(w, st, 0, st.B, NT, blockIdx.x / G, e, tile)) return;
         const WeighEntry en(w, st, e, false);
         const int q0 = first_qtile(w, st, e, en.n, g);
+        if (!tiles_fit(a, q0, g, en.n, R)) return;
         out = a.qtiles + (int64_t)(q0 + tile) * a.stage;
         if (tid < NT) {
             const int row = tile * NT + tid;
@@ -280,6 +284,7 @@ __global__ void __launch_bounds__(THREADS, 2) weigh_tc_kernel(const __grid_const
     const int rows = en.n * R;
     if (en.n == 0 || (SUMS ? res0 >= en.keys : res0 >= rows)) return;
     const int q0 = first_qtile(w, st, e, en.n, g);
+    if (!tiles_fit(a, q0, g, en.n, R)) return;
     const uint8_t *qt = a.qtiles + (int64_t)q0 * stage, *kt = a.ktiles + (int64_t)((e - a.e0) * a.ng + g - a.g0) * a.key_tiles * stage;
     const int last_row = min(rows, res0 + MT) - 1;
     const KeyWalk walk(w, SUMS ? 0 : en.p0 + res0 / R, SUMS ? 0 : en.p0 + last_row / R);

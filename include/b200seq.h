@@ -551,7 +551,7 @@ int b200seq_verify_drafts(const float* logits, int64_t ld, int R, int V, const i
  *   acc[slot][g][j] += sum over the entry's tokens and the query heads of key head g of their weights for key j;   a key that this step brought gets the sum instead
  * acc: f32 [slots][G][acc_ld]; the entries of a step have slots of their own.  last > 0: only the last so many tokens of every entry count.  A row that sees nothing but scores of minus infinity gives nothing.
  * max_keys: no fewer keys than the step's longest sequence has, or 0 for what the block tables hold.  Entries whose slot is none, or whose keys go beyond acc_ld, max_keys or their
- * block table, raise bit 0 of the error flags and are left out.  scratch: b200seq_key_weights_scratch_floats(...) floats, 16-byte aligned. */
+ * block table, and starts that are not in order, raise bit 0 of the error flags; the former are left out.  scratch: b200seq_key_weights_scratch_floats(...) floats, 16-byte aligned. */
 size_t b200seq_key_weights_scratch_floats(const b200seq_step* st, const b200seq_attn_desc* d, int last, int max_keys);
 int b200seq_key_weights(const float* proj, int64_t ld, const b200seq_step* st, const b200seq_attn_desc* d, const void* kpool, int kv_bits, float* acc, int slots, int64_t acc_ld,
                         int last, int max_keys, float* scratch, size_t scratch_floats, void* stream);

@@ -470,6 +470,23 @@ def test_entries_that_are_none(ops):
             assert not torch.equal(acc[s2], torch.ones_like(acc[s2])), what
 
 
+@pytest.mark.parametrize("n", [4, 80, 300])
+def test_starts_out_of_order(ops, n):
+    """entries of overlapping tokens: flagged, and nothing beyond the entries' own rows is written"""
+    rng = np.random.default_rng(8)
+    s = Step(ops, rng, [n, 0, 0, 0, 0], [60, 0, 0, 0, 0], 16, 2, 64)
+    layer = ops.attn_desc(16, 2, 64, 64, 0.125, gated=False, kv_shared=True)
+    s.t["start"].copy_(up([0, n, 0, n, 0, n], np.int32))
+    s.t["bt"].copy_(s.t["bt"][:1].expand(5, -1).contiguous())
+    s.t["pos0"].fill_(60)
+    acc = torch.ones(7, 2, n + 80, device=DEV)
+    ops.key_weights(s.proj(), s.desc, layer, s.kpool, acc)
+    assert ops.error_flags() == 1
+    assert torch.equal(acc[:, :, n + 60:], torch.ones_like(acc[:, :, n + 60:]))
+    spare = [i for i in range(7) if i not in s.slots[[0, 2, 4]]]
+    assert torch.equal(acc[spare], torch.ones_like(acc[spare]))
+
+
 def test_weights_captured_and_on_another_stream(ops):
     rng = np.random.default_rng(11)
     layer = ops.attn_desc(8, 2, 64, 64, 0.125, gated=False, kv_shared=True)
