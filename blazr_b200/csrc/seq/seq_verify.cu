@@ -634,6 +634,7 @@ int b200seq_verify_drafts(const float* logits, int64_t ld, int R, int V, const i
     if (R > 0 && B > 0 && (scratch_bytes < b200seq_verify_scratch_bytes(R, V, ruled) || (reinterpret_cast<uintptr_t>(scratch) & 15)))
         return fail(B200SEQ_ERR_INVALID_ARG, "verify_drafts: the work area is too small or not on a 16-byte boundary");
     if (B == 0) return 0;
+    if (R > 0 && tokens < drafts + R && drafts < tokens + R) return fail(B200SEQ_ERR_INVALID_ARG, "verify_drafts: tokens and drafts share memory");      // (read by other blocks than write them)
     VerifyArgs a{logits, ld, R, V, B, 0, start, drafts, accept_u, sample_u, temperature, top_k, top_p, draft_probs, ldq, accepted, tokens, (Partial*)scratch, nullptr, error_flag_dev()};
     a.slices = slices_of(V);
     if (ruled) a.cut = reinterpret_cast<Cut*>(a.part + (size_t)R * a.slices);

@@ -538,7 +538,7 @@ int b200seq_process_logits(const float* x, int64_t ldx, int R, int V, const floa
  *   (top_p[e] < 1; at least the largest);   p = w / sum of the kept.   T <= 0: p = 1 at the first maximum
  * A draft x is accepted when accept_u[row] * q(x) < p(x), q(x) = draft_probs[row][x] (f32 [R, V], stride ldq; null: 1), at T <= 0 when it is the first maximum.  The token behind the
  * accepted drafts is drawn from max(p - q, 0) of the row that rejected (null: p without the draft; where nothing is left: p), or from the last row's p: the lowest token whose
- * cumulated weight exceeds sample_u[e] times the sum.  accepted[e]: how many drafts; tokens[start[e] ..]: the accepted drafts, the token behind them, then -1.
+ * cumulated weight exceeds sample_u[e] times the sum.  accepted[e]: how many drafts; tokens[start[e] ..]: the accepted drafts, the token behind them, then -1 (not written over drafts).
  * A row without a finite maximum, or with a NaN, accepts nothing and gives -1.  A draft outside the vocabulary is not accepted; it, and starts that are not in order within R, raise
  * bit 4 of the error flags.  top_k int32 [B], top_p f32 [B]: each optional.  scratch: b200seq_verify_scratch_bytes(R, V, top_k or top_p given) bytes, 16-byte aligned. */
 size_t b200seq_verify_scratch_bytes(int R, int V, int ruled);

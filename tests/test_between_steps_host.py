@@ -113,3 +113,10 @@ def test_evict_keys_c_refuses(L):
         assert call(**kw) < 0, kw
         assert b"evict_keys" in L.b200seq_last_error()
     assert call(layers=0) == 0 and call(B=0) == 0
+
+
+def test_verify_drafts_refuses_tokens_over_drafts(L):
+    p = C.c_void_p(16)
+    for d, t in ((64, 64), (64, 72), (72, 64)):
+        assert L.b200seq_verify_drafts(p, 10, 3, 10, p, 2, C.c_void_p(d), p, p, p, None, None, None, 10, p, C.c_void_p(t), p, 1 << 20, None) == -1
+        assert b"share memory" in L.b200seq_last_error()
