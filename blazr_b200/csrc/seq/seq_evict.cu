@@ -336,6 +336,11 @@ extern "C" int b200seq_evict_keys(void* const* kpools, void* const* vpools, floa
     for (int i = 0; i < layers; ++i)
         if (!kpools[i] || !vpools[i] || !accs[i] || (kv_bits == 4 && ((reinterpret_cast<uintptr_t>(kpools[i]) | reinterpret_cast<uintptr_t>(vpools[i])) & 15)))
             return fail(B200SEQ_ERR_INVALID_ARG, "evict_keys: a pool of layer %d is null or not on a 16-byte boundary", i);
+    for (int i = 0; i < 2 * layers && B > 0; ++i) {      // (every one is moved within itself, all at the same time)
+        void* const p = i < layers ? kpools[i] : vpools[i - layers];
+        for (int j = 0; j < i; ++j)
+            if (p == (j < layers ? kpools[j] : vpools[j - layers]) || (i < layers && accs[i] == accs[j])) return fail(B200SEQ_ERR_INVALID_ARG, "evict_keys: a pool, or weights, given twice");
+    }
     const cudaStream_t cs = (cudaStream_t)stream;
     for (int l0 = 0; l0 < layers && B > 0; l0 += LAYERS) {
         EvictArgs a = {};

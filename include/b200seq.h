@@ -560,7 +560,7 @@ int b200seq_key_weights(const float* proj, int64_t ld, const b200seq_step* st, c
  * (f32 [slots][G][acc_ld]).  Where rows[e] > keep, every layer and key head keeps the first `first`, the last `recent` and, of the rest, those of largest weight (ties: the lowest
  * row; NaN lowest); where not, all.  They go in order to the places 0, 1, .. of the pages to_table[e] and of slot to_slot[e]; both may be the entry's own (a place that is not written
  * stays as it is), but no page or slot that is written may be another entry's, nor one of its own in another order.  kept int32 [layers][B][G][keep] receives the rows, -1 behind them.
- * kpools, vpools, accs: HOST arrays of device pointers.  kv_bits 32: f32 pages [block_size][G][D] and [block_size][G][V]; 4: those of b200seq_kv4_store.  Gv == G.
+ * kpools, vpools, accs: HOST arrays of device pointers, none of them twice.  kv_bits 32: f32 pages [block_size][G][D] and [block_size][G][V]; 4: those of b200seq_kv4_store.  Gv == G.
  * An entry whose slots are none or whose rows go beyond acc_ld or its tables, and a row whose page is negative, raise bit 0 of the error flags and stay. */
 int b200seq_evict_keys(void* const* kpools, void* const* vpools, float* const* accs, int layers, int kv_bits, int block_size, int G, int D, int Gv, int V, int slots, int64_t acc_ld,
                        const int32_t* slot, const int32_t* rows, const int32_t* table, int max_blocks, const int32_t* to_slot, const int32_t* to_table, int to_max_blocks, int B,

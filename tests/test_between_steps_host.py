@@ -120,3 +120,11 @@ def test_verify_drafts_refuses_tokens_over_drafts(L):
     for d, t in ((64, 64), (64, 72), (72, 64)):
         assert L.b200seq_verify_drafts(p, 10, 3, 10, p, 2, C.c_void_p(d), p, p, p, None, None, None, 10, p, C.c_void_p(t), p, 1 << 20, None) == -1
         assert b"share memory" in L.b200seq_last_error()
+
+
+@pytest.mark.parametrize("k,v,a", [((64, 64), (128, 192), (256, 512)), ((64, 320), (128, 128), (256, 512)), ((64, 320), (64, 192), (256, 512)), ((64, 320), (128, 64), (256, 512)),
+                                   ((64, 320), (128, 192), (256, 256))])
+def test_evict_keys_refuses_what_is_given_twice(L, k, v, a):
+    p, arr = C.c_void_p(16), lambda x: (C.c_void_p * 2)(*x)
+    assert L.b200seq_evict_keys(arr(k), arr(v), arr(a), 2, 32, 16, 2, 64, 2, 64, 3, 64, p, p, p, 3, p, p, 3, 1, 20, 2, 4, p, None) == -1
+    assert b"given twice" in L.b200seq_last_error()
