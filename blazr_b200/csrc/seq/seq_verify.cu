@@ -5,8 +5,8 @@
 // rejected (from p where that is nothing), or from the last row's p: the lowest one whose cumulated weight exceeds u times the sum.  T <= 0: p = 1 at the first maximum.
 //
 // What a row decides is compared with a random number, so that its sums are held in 64 bits (weights are f32, within 2^-21 of themselves; sums of four of them, then f64).
-// Measured: 64 entries of 4 drafts, 128256 logits a row, 58 us (35 + 27; the logits' bytes alone 25, the draft's probabilities of a row an entry 5); one of 32000 logits 18.6, a chain of
-// loads and of the clusters' barriers; 16 entries of 3 drafts with top_k and top_p 52 to 55 (thresholds 40).
+// Measured: 64 entries of 4 drafts, 128256 logits a row, 55 us (33.5 + 28; the logits' bytes alone 25, the draft's probabilities of a row an entry 5); one of 32000 logits 18.6, a chain of
+// loads and of the clusters' barriers; 16 entries of 3 drafts with top_k and top_p 52 to 56 (thresholds 42).
 // The floor is the logits' bytes: they are read once, in slices over the whole GPU (row_stats), with maximum, its place and sum left for every slice.  Then a cluster of eight
 // CTAs an entry puts the slices together, finds the row that rejects and reads that one again, from L2 (pick).
 // top_k and top_p need a threshold a row before that (row_cut, a CTA a row, which it reads twice or three times from L2): counts, or masses (whole numbers of 2^-32: additions whose
@@ -95,7 +95,8 @@ __device__ __forceinline__ int entry_of(const VerifyArgs& a, int row) {
 }
 
 // grid (slices, rows): 4 QUADS logits a thread, all asked for before anything else.  Small blocks, so that one's sums run beside another's loads (320 rows of 128256: blocks of 1024
-// threads 64 us, of 256 40: 4.1 TB/s)
+// threads 64 us, of 256 40, with 32 logits a thread instead of 16 35; with the maximum's place looked up by those that have it and the weights two at a time 33.5: 4.9 TB/s, 13 instructions
+// a logit for 21)
 __global__ void __launch_bounds__(STATS) row_stats_kernel(const __grid_constant__ VerifyArgs a) {
     chain_enter();
     constexpr int THREADS = STATS, WARPS = THREADS / 32;
@@ -112,31 +113,46 @@ __global__ void __launch_bounds__(STATS) row_stats_kernel(const __grid_constant_
     if (e >= a.B) return;
     const float T = a.temp[e];
     float m = -INFINITY;
-    int at = 0x7fffffff;
-    bool odd = false;
 #pragma unroll
-    for (int k = 0; k < QUADS; ++k) {
-        const float z[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (z[j] > m) m = z[j], at = i0 + 4 * k * THREADS + j;
-            odd |= z[j] != z[j];
-        }
-    }
+    for (int k = 0; k < QUADS; ++k) m = fmaxf(m, fmaxf(fmaxf(v[k].x, v[k].y), fmaxf(v[k].z, v[k].w)));
     const float wm = warp_max(m);
     if (lane == 0) wmax[warp] = wm;
     __syncthreads();
     float top = wmax[0];
 #pragma unroll
     for (int w = 1; w < WARPS; ++w) top = fmaxf(top, wmax[w]);
-    const unsigned first = __reduce_min_sync(0xffffffffu, m == top && top > -INFINITY ? (unsigned)at : 0x7fffffffu);
+    unsigned at = 0x7fffffff;
+    if (m == top && top > -INFINITY) {      // (few threads have it)
+#pragma unroll
+        for (int k = QUADS - 1; k >= 0; --k) {
+            const int i = i0 + 4 * k * THREADS;
+            at = v[k].x == top ? i : v[k].y == top ? i + 1 : v[k].z == top ? i + 2 : v[k].w == top ? i + 3 : at;
+        }
+    }
+    const unsigned first = __reduce_min_sync(0xffffffffu, at);
     const Heat heat(T > 0.f ? T : 1.f);
     double sum = 0.0;      // (a slice of minus infinities: nothing)
-    if (top > -INFINITY) {
+    // the weights two at a time, with the roundings that heat() has; a sum that is no number has met one, or an infinity: heat() and a look at each.  (A difference beyond the type is
+    // minus infinity here, the least number there: the same nothing, but for temperatures that make something of it.)
+    const uint64_t off = tcsplit::pk(-top, -top), hi = tcsplit::pk(heat.hi, heat.hi), lo = tcsplit::pk(heat.lo, heat.lo);
+    auto two = [&](float x, float y) {
+        const uint64_t d = tcsplit::add2(tcsplit::pk(x, y), off);
+        float a0, a1;
+        tcsplit::upk(tcsplit::fma2(d, hi, tcsplit::mul2(d, lo)), a0, a1);
+        return tcsplit::ex2(a0) + tcsplit::ex2(a1);
+    };
 #pragma unroll
-        for (int k = 0; k < QUADS; ++k) sum += (double)((heat(v[k].x, top) + heat(v[k].y, top)) + (heat(v[k].z, top) + heat(v[k].w, top)));
+    for (int k = 0; k < QUADS; ++k) sum += (double)(two(v[k].x, v[k].y) + two(v[k].z, v[k].w));
+    if (!(sum >= 0.0) || T > 1e30f) {
+        bool odd = false;
+        sum = 0.0;
+#pragma unroll
+        for (int k = 0; k < QUADS; ++k) {
+            odd |= v[k].x != v[k].x || v[k].y != v[k].y || v[k].z != v[k].z || v[k].w != v[k].w;
+            if (top > -INFINITY) sum += (double)((heat(v[k].x, top) + heat(v[k].y, top)) + (heat(v[k].z, top) + heat(v[k].w, top)));
+        }
+        if (odd) sum = NAN;
     }
-    if (odd) sum = NAN;
     sum = warp_sum(sum);
     if (lane == 0) wat[warp] = first, wsum[warp] = sum;
     __syncthreads();

@@ -164,6 +164,26 @@ def test_temperatures_and_numbers_at_their_ends(ops):
         assert go(0.37, 1.0, top_p=[p]) == go(0.37, 1.0)
 
 
+@pytest.mark.parametrize("T", [0.0, 1e-30, 0.7, 3e29, 1e38])
+def test_logits_at_the_ends_of_their_type(ops, T):
+    """differences beyond the type, minus infinities in some slices, one equal maximum a slice, a NaN in the last place"""
+    V, rng = 30011, np.random.default_rng(12)
+    z = (2 * rng.standard_normal((6, V))).astype(np.float32)
+    z[0, ::3] = -np.inf
+    z[1, 100:20000] = -np.inf
+    z[2, :] = -np.inf
+    z[2, 17000:17003] = 0.5
+    z[3, ::2], z[3, 1::2] = 3e38, -3e38
+    z[4, [5, 9000, 29999]] = 50.0
+    z[5, V - 1] = np.nan
+    start, n = np.arange(7), 6
+    us = np.array([0.1, 0.35, 0.5, 0.83, 0.6, 0.2], np.float32)
+    got = run_verify(ops, z, start, np.zeros(n), np.zeros(n), us, np.full(n, T))
+    want = oracle.verify(z, start, np.zeros(n, np.int32), np.zeros(n), us, np.full(n, T, np.float32))
+    assert same(got, want, start) >= 3
+    assert got[1][5] == -1
+
+
 def test_what_is_drawn_has_the_target_s_distribution(ops):
     """drafts from q, verified against p: tokens as often as p says.  Random numbers from an even grid in both places: counts are off by the grid's steps alone"""
     V, n = 5, 64
