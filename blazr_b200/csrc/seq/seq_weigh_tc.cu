@@ -7,7 +7,8 @@
 // operand is off by 2^-23 of itself or 2^-29, whichever is more; the queries carry the scale, so that a tile is scores in base 2.  Beyond 4094 an operand has no such parts:
 // they make a row's or a key's sum NaN, and such a sum is made again by plain f32 products (plain_row, plain_key).
 //
-// What bounds it is the tensor pipe, three products a pass: 6.3 MFLOP a tile of 128 x 64 at heads of 128, 0.55 us at the rate of an SM.  So that nothing else takes as long, rows and
+// Its floor is the tensor pipe, three products a pass: 6.3 MFLOP a tile of 128 x 64 at heads of 128, 0.55 us at the rate of an SM.  2047 tokens of 32 heads of 128 (8 key heads): 123 us,
+// 15 of splitting and passes of 57 and 55, in which the pipe is active 54 and 57 % (31 a pass at its rate); where the rest of a pass goes has not been taken apart.  So that nothing else takes as long, rows and
 // keys are split once, ahead of the two passes: tiles of 64 of them in the work area, two planes of f16 in the swizzled order of shared memory, so that a tile is one bulk copy.  (Split by
 // loader warps each time a tile was needed: 4850 instructions of warps a tile, 90 us a pass of 2047 tokens.)  The operand that stays lies in TMEM (128 columns at most), the one that
 // streams in three stages; 256 columns of TMEM and under 100 KB of shared memory: two CTAs an SM, so that one's beginning and end run beside the other's tiles.
