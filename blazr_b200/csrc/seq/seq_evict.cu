@@ -6,8 +6,10 @@
 //
 // A row never moves to a higher place.  So whoever walks over a head's rows in chunks, all of a chunk read before any of it is written, may write into the pages that it reads: what
 // it overwrites has been read, and nobody else touches these bytes.  That is what lets a cache be cut back where it lies.  A cluster of up to eight CTAs walks together, each with
-// whole rows of a chunk, and waits for all of them between reading and writing; the next chunks are on their way by then.  Two sequences of 32768 rows to 16384, 8 heads of 128,
-// four layers: 370 us of moving, 5.8 TB/s.  (Pages and kept rows in any order take the same time: what it cost before were instructions for addresses.)
+// whole rows of a chunk, and waits for all of them between reading and writing; the next chunks are on their way by then.  The wait orders those reads before those writes: a barrier of the
+// block where it is alone, else a barrier of the cluster with release and acquire.  A release waits for all that its thread has under way, so that one warp that moves nothing does it
+// for its block (two sequences of 32768 rows in place, in all: 415 us; with a release of every thread that reads 436 to 590, with none, so in no order that memory promises, 397).  Two
+// sequences of 32768 rows to 16384, 8 heads of 128, four layers: 390 us of moving, 5.5 TB/s.  (Pages and kept rows in any order take the same time: what it cost before were instructions for addresses.)
 #include "seq_kv4.cuh"
 
 namespace b200seq {
@@ -17,10 +19,10 @@ namespace {
 constexpr int LAYERS = 32;                // of one launch
 constexpr int EACH = 8;                   // weights a thread lists at a time
 constexpr int HELD = 49152;               // weights that a block has in shared memory; longer rows are read four times
-constexpr int MOVE = 256;                 // threads that move
-// Pieces of a chunk a thread has, chunks on their way, rows looked up at a time.  Small ones, so that many CTAs share an SM: eight sequences of 2301 rows in 16 layers of 4-bit pages 143 us
-// (4, 4, 1024: 175), two of 32768 in four layers of f32 pages 410 (406)
-constexpr int ITEMS = 2, STAGES = 2, BATCH = 512;
+constexpr int MOVE = 256;                 // threads that move (and a warp that arrives for them, in clusters)
+// Pieces of a chunk a thread has, chunks on their way, rows looked up at a time.  Small ones, so that many CTAs share an SM; in clusters larger ones, as each costs a barrier.  Eight
+// sequences of 2301 rows in 16 layers of 4-bit pages (blocks alone) 160 us, with four pieces 172; two of 32768 in four layers of f32 pages (clusters of four) 415, with two pieces 447
+constexpr int ITEMS_ALONE = 2, ITEMS_CLUSTER = 4, STAGES = 2, BATCH = 512;
 
 struct EvictArgs {
     uint8_t* pool[2][LAYERS];
@@ -186,11 +188,11 @@ __device__ __forceinline__ void copy_in(V* dst, const uint8_t* src) {
     else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(sizeof(V)) : "memory");
 }
 
-// grid (cluster, entries * key heads, layers [* keys and values]).  BOTH: keys and values are of one size
-template <class V, bool FOUR, bool BOTH>
-__global__ void __launch_bounds__(MOVE) evict_move_kernel(const __grid_constant__ EvictArgs a, int which) {
+// grid (cluster, entries * key heads, layers [* keys and values]).  BOTH: keys and values are of one size.  ALONE: the cluster is one block
+template <class V, bool FOUR, bool BOTH, bool ALONE>
+__global__ void __launch_bounds__(ALONE ? MOVE : MOVE + 32) evict_move_kernel(const __grid_constant__ EvictArgs a, int which) {
     chain_enter();
-    constexpr int SPAN = MOVE * ITEMS;
+    constexpr int ITEMS = ALONE ? ITEMS_ALONE : ITEMS_CLUSTER, SPAN = MOVE * ITEMS;
     extern __shared__ __align__(16) uint8_t ring_raw[];
     V* const ring = reinterpret_cast<V*>(ring_raw);
     // Where the rows of two batches lie and go (from < 0: the row stays where it is).  Looked up a batch ahead, four chunks or more: the chain list, page takes as long as two of
@@ -225,6 +227,15 @@ __global__ void __launch_bounds__(MOVE) evict_move_kernel(const __grid_constant_
         }
     };
     const int chunks = (kept + step - 1) / step;
+    if (!ALONE && tid >= MOVE) {      // (a warp of its own)
+        for (int u0 = 0; u0 < per; u0 += span)
+            for (int c = 0; c < chunks; ++c) {
+                asm volatile("bar.sync 2, %0;" ::"n"(MOVE + 32) : "memory");
+                asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+            }
+        return;
+    }
+    auto movers = []() { asm volatile("bar.sync 1, %0;" ::"n"(MOVE) : "memory"); };
     for (int u0 = 0; u0 < per; u0 += span) {
         int pr[ITEMS], pu[ITEMS];                           // a thread's pieces of a chunk: row, byte (FOUR: piece) of the row
 #pragma unroll
@@ -261,44 +272,53 @@ __global__ void __launch_bounds__(MOVE) evict_move_kernel(const __grid_constant_
             load_at += rows, load_stage = load_stage + 1 == STAGES ? 0 : load_stage + 1;
             if (load_at >= 2 * K * rows) load_at = 0;
         };
-        __syncthreads();
+        movers();
         look(0, 0);
-        __syncthreads();
+        movers();
         for (int c = 0; c < STAGES - 1; ++c) load_next(c);
         for (int c = 0; c < chunks; ++c) {
             load_next(c + STAGES - 1);                      // rows from the end of this chunk on: nothing that this one or an earlier one writes
-            // All of this chunk has been read, by all CTAs, before any of it is written.  (No order of memory is asked for but that: the values have arrived, and what is written now is
-            // read by nobody's later load.  With a release there the CTAs would wait for their stores, too.)
+            // all of this chunk has been read, by all CTAs, before any of it is written
             asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-            asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+            if (ALONE) {
+                movers();
+            } else {
+                asm volatile("bar.arrive 2, %0;" ::"n"(MOVE + 32) : "memory");
+                asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+            }
             store(store_at, mine - c * step, store_stage);
             store_at += rows, store_stage = store_stage + 1 == STAGES ? 0 : store_stage + 1;
             if (store_at >= 2 * K * rows) store_at = 0;
             if (in_batch == 0) {                            // (whoever wrote by the batch before this one is through)
                 look(batch + 1, (batch + 1) & 1 ? K * rows : 0);
-                __syncthreads();
+                movers();
             }
             if (++in_batch == K) in_batch = 0, ++batch;
         }
     }
 }
 
-template <class V, bool FOUR, bool BOTH>
-cudaError_t move_as(const EvictArgs& a, int kv, cudaStream_t cs) {
-    const int64_t heads = (int64_t)a.B * a.G * a.layers * (BOTH ? 2 : 1);
-    // Three CTAs an SM, where a head's rows are enough for so many (128 heads: clusters of 1, 2, 4 took 785, 542, 411 us; 2048 heads: 143, 143, 157)
-    int cluster = 1;
-    while (cluster < 8 && heads * cluster < 3 * 148) cluster *= 2;
-    const int smem = STAGES * MOVE * ITEMS * (int)sizeof(V);
-    const cudaError_t e = cudaFuncSetAttribute(evict_move_kernel<V, FOUR, BOTH>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <class V, bool FOUR, bool BOTH, bool ALONE>
+cudaError_t move_as(const EvictArgs& a, int kv, int cluster, cudaStream_t cs) {
+    const int smem = STAGES * MOVE * (ALONE ? ITEMS_ALONE : ITEMS_CLUSTER) * (int)sizeof(V);
+    const cudaError_t e = cudaFuncSetAttribute(evict_move_kernel<V, FOUR, BOTH, ALONE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization, attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension, attr[1].val.clusterDim.x = cluster, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
-    cfg.gridDim = dim3(cluster, a.B * a.G, a.layers * (BOTH ? 2 : 1)), cfg.blockDim = MOVE, cfg.dynamicSmemBytes = smem, cfg.stream = cs, cfg.attrs = attr, cfg.numAttrs = 2;
-    cudaLaunchKernelEx(&cfg, evict_move_kernel<V, FOUR, BOTH>, a, kv);
+    cfg.gridDim = dim3(cluster, a.B * a.G, a.layers * (BOTH ? 2 : 1)), cfg.blockDim = ALONE ? MOVE : MOVE + 32, cfg.dynamicSmemBytes = smem, cfg.stream = cs, cfg.attrs = attr;
+    cfg.numAttrs = ALONE ? 1 : 2;
+    cudaLaunchKernelEx(&cfg, evict_move_kernel<V, FOUR, BOTH, ALONE>, a, kv);
     return cudaGetLastError();
+}
+template <class V, bool FOUR, bool BOTH>
+cudaError_t move_as(const EvictArgs& a, int kv, cudaStream_t cs) {
+    const int64_t heads = (int64_t)a.B * a.G * a.layers * (BOTH ? 2 : 1);
+    // Three CTAs an SM, where a head's rows are enough for so many (128 heads: clusters of 1, 2, 4 took 785, 542, 411 us; 2048 heads: 143, 143, 157; before the blocks' order was asked for)
+    int cluster = 1;
+    while (cluster < 8 && heads * cluster < 3 * 148) cluster *= 2;
+    return cluster == 1 ? move_as<V, FOUR, BOTH, true>(a, kv, 1, cs) : move_as<V, FOUR, BOTH, false>(a, kv, cluster, cs);
 }
 template <class V, bool FOUR>
 cudaError_t move(const EvictArgs& a, int kv, bool both, cudaStream_t cs) {
