@@ -9,8 +9,8 @@
 // loads and of the clusters' barriers; 16 entries of 3 drafts with top_k and top_p 52 to 56 (thresholds 42).
 // The floor is the logits' bytes: they are read once, in slices over the whole GPU (row_stats), with maximum, its place and sum left for every slice.  Then a cluster of eight
 // CTAs an entry puts the slices together, finds the row that rejects and reads that one again, from L2 (pick).
-// top_k and top_p need a threshold a row before that (row_cut, a CTA a row, which it reads twice or three times from L2): counts, or masses (whole numbers of 2^-32: additions whose
-// order does not matter), of 2048 bins of equal width below the maximum show how far down the k-th logit lies, or where the mass passes the share; the logits down to there are sorted.
+// top_k and top_p need a threshold a row before that (row_cut, a CTA a row, which it reads twice or three times from L2): counts, or masses (whole numbers of 2^-42: additions whose
+// order does not matter, off by 2^-43 a token: 2^-26 of the largest weight for 128 k), of 2048 bins of equal width below the maximum show how far down the k-th logit lies, or where the mass passes the share; the logits down to there are sorted.
 // Where those are too many (rows of equal logits, logits far apart), the threshold is selected by the bits of the ordered logits instead, eleven at a time.
 #include <cfloat>
 #include <cooperative_groups.h>
@@ -30,6 +30,7 @@ constexpr int QUADS = 8;                  // 16-byte pieces of a slice of a row 
 constexpr int STATS = 256, PICK = 256, CUT = 1024;     // threads
 constexpr int MAX_TILES = 512;            // tiles of 4 * PICK logits of one CTA's share
 constexpr int BINS = 2048, LIST = 2048;   // bins below the maximum; logits that are sorted
+constexpr float MASS = 0x1p42f;           // masses as whole numbers: MAX_V weights of one fit 64 bits
 constexpr int64_t MAX_V = (int64_t)CLUSTER * MAX_TILES * 4 * PICK - 64;
 
 struct Partial {      // of a slice of a row
@@ -277,7 +278,7 @@ __device__ __noinline__ uint32_t slow_cut(const float* x, int V, float top, cons
                 const uint32_t key = order_key(z);
                 if (key < least || (level > 0 && (key >> (shift + bits)) != prefix)) return;
                 unsigned long long add = 1;
-                if (pass == 1) add = (unsigned long long)__float2uint_rn(heat(z, top) * 0x1p31f);
+                if (pass == 1) add = __float2ull_rn(heat(z, top) * MASS);
                 if (add) atomicAdd(h + ((key >> shift) & ((1u << bits) - 1)), add);
             });
             __syncthreads();
@@ -299,7 +300,7 @@ __device__ __noinline__ uint32_t slow_cut(const float* x, int V, float top, cons
 // grid (rows)
 __global__ void __launch_bounds__(CUT, 1) row_cut_kernel(const __grid_constant__ VerifyArgs a) {
     chain_enter();
-    __shared__ __align__(16) unsigned h32[2 * BINS * 2];    // bins: counts, coarse and fine masses; or the slow way's table
+    __shared__ __align__(16) unsigned h32[4 * BINS];        // bins: counts, masses in three parts; or the slow way's table
     __shared__ unsigned long long sh[34];
     __shared__ unsigned list[LIST], many, next, cut_key;
     __shared__ Row row_sh;
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(CUT, 1) row_cut_kernel(const __grid_constant__
         return;
     }
     const Heat heat(T);
-    for (int i = tid; i < 3 * BINS; i += CUT) h32[i] = 0;
+    for (int i = tid; i < 4 * BINS; i += CUT) h32[i] = 0;
     if (tid < 32) {
         const Row r = whole_row(a, heat, row);
         if (tid == 0) row_sh = r, many = 0, next = 0, cut_key = 0;
@@ -337,14 +338,17 @@ __global__ void __launch_bounds__(CUT, 1) row_cut_kernel(const __grid_constant__
         each_logit(x, a.V, [&](float z) {
             const int b = bin_of(z);
             finite += z > -INFINITY;
-            if (b == BINS - 1) return;                      // (the last bin has what the others have not; its masses are below 2^-34)
+            if (b == BINS - 1) return;                      // (the last bin has what the others have not; a weight in it is below 2^-46)
             if (by_count || !masses_only) atomicAdd(h32 + b, 1u);
             if (!by_count) {
                 const float w = heat(z, r.max) * 65536.f, c = w + 8388608.f;
                 const unsigned whole = __float_as_uint(c) & 0x1ffffu;
-                const int part = (int)(__float_as_uint((w - (c - 8388608.f)) * 65536.f + 12582912.f) - 0x4B400000u);      // (-32768 .. 32768: 32768 of either fit 32 bits)
+                const float x1 = (w - (c - 8388608.f)) * 65536.f, c1 = x1 + 12582912.f;
+                const int part = (int)(__float_as_uint(c1) - 0x4B400000u);      // (-32768 .. 32768: 32768 of either fit 32 bits)
+                const int low = (int)(__float_as_uint((x1 - (c1 - 12582912.f)) * 1024.f + 12582912.f) - 0x4B400000u);
                 if (whole) atomicAdd(h32 + BINS + b, whole);
                 if (part) atomicAdd(reinterpret_cast<int*>(h32) + 2 * BINS + b, part);
+                if (low) atomicAdd(reinterpret_cast<int*>(h32) + 3 * BINS + b, low);
             }
         });
         again = false;
@@ -369,7 +373,10 @@ __global__ void __launch_bounds__(CUT, 1) row_cut_kernel(const __grid_constant__
         want = (unsigned long long)k;
         b = find_bin<false>(c0, c1, want, before, sh);
     } else {
-        const unsigned long long m0 = ((unsigned long long)h32[BINS + b0] << 16) + (long long)(int)h32[2 * BINS + b0], m1 = ((unsigned long long)h32[BINS + b1] << 16) + (long long)(int)h32[2 * BINS + b1];
+        auto mass = [&](int i) {      // (never below zero: a sum of numbers that are not)
+            return ((unsigned long long)h32[BINS + i] << 26) + (unsigned long long)((long long)(int)h32[2 * BINS + i] * 1024 + (int)h32[3 * BINS + i]);
+        };
+        const unsigned long long m0 = mass(b0), m1 = mass(b1);
         all_mass = block_total(m0 + m1, sh);
         const double t = ceil((double)share * (double)all_mass);
         want = t >= 1.0 ? (unsigned long long)t : 1ull;
@@ -419,8 +426,8 @@ __global__ void __launch_bounds__(CUT, 1) row_cut_kernel(const __grid_constant__
         }
         double* const d = reinterpret_cast<double*>(sh);
         if (by_mass) {
-            const double all = by_count ? block_total(w[0] + w[1], d) : (double)all_mass * 0x1p-32, goal = (double)share * all;
-            const double up = block_before<double, false>(w[0] + w[1], d) + (alone ? (double)before * 0x1p-32 : 0.0);
+            const double all = by_count ? block_total(w[0] + w[1], d) : (double)all_mass * (1.0 / MASS), goal = (double)share * all;
+            const double up = block_before<double, false>(w[0] + w[1], d) + (alone ? (double)before * (1.0 / MASS) : 0.0);
             // the last one with less than the goal before it (the largest always)
             uint32_t last = tid == 0 ? key[0] : 0xffffffffu;
             if (w[0] > 0.0 && up < goal) last = key[0];

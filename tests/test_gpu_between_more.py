@@ -2,9 +2,52 @@
 import numpy as np
 import pytest
 
-from test_gpu_between_steps import evict, ops  # noqa: F401
+from test_gpu_between_steps import evict, ops, run_verify, up  # noqa: F401
 
 pytestmark = pytest.mark.gpu
+
+
+# ---- drafts: shares near one ---------------------------------------------------------------------------------------------------------------
+# A token that top_p keeps is accepted at accept_u = 0, one that it does not keep is not.  The mass before a token is known to the roundings of the tail's weights (2^-19 of the tail,
+# in that mass and in the whole), to those of the whole numbers that masses are added up in (2^-43 a weight) and to the weights that are left out (2^-46 each).  Tokens whose
+# mass before them is within that of the share may go either way.
+TAILS = {
+    "flat": lambda r, n: np.full(n, -23.0),
+    "one bin": lambda r, n: -23.0 - r.random(n) / 80,
+    "two units": lambda r, n: -22.0 - 2 * r.random(n),
+    "two units, cold": lambda r, n: 0.25 * (-22.0 - 2 * r.random(n)),
+    "far": lambda r, n: -24.5 - 4 * r.random(n),
+}
+
+
+@pytest.mark.parametrize("tail", TAILS)
+@pytest.mark.parametrize("top_k", [0, 60000])
+@pytest.mark.parametrize("V", [50257, 128256])
+def test_shares_near_one_keep_their_tail(ops, tail, top_k, V):
+    rng = np.random.default_rng(V)
+    z = np.empty(V, np.float32)
+    z[0] = 0.0
+    z[1:] = TAILS[tail](rng, V - 1)
+    T = 0.25 if "cold" in tail else 1.0
+    w = np.exp(z.astype(np.float64) / T)
+    if 0 < top_k < V:
+        w[z < np.sort(z)[::-1][top_k - 1]] = 0.0
+    total = w.sum()
+    order = np.argsort(-z, kind="stable")
+    before = np.cumsum(w[order]) - w[order]
+    before = before[np.searchsorted(-z[order], -z[order], side="left")]        # (equal ones together)
+    share = np.float32(1.0 - 0.3 * (1.0 - w[0] / total))
+    x = order[np.unique(np.linspace(1, V - 1, 60).astype(int))]
+    rank = np.argsort(order)[x]
+    near = V * (2.0 ** -43 + 2.0 ** -46) + 2.0 ** -18 * (1.0 - w[0] / total)
+    sure = np.abs(before[rank] - float(share) * total) > near * total
+    keep = (before[rank] < float(share) * total) & (w[x] > 0)
+    B = len(x)
+    rows, two = up(z).expand(2 * B, V).contiguous(), lambda a: np.stack([a, 0 * a], 1).reshape(-1)
+    got, _ = run_verify(ops, rows, np.arange(0, 2 * B + 1, 2), two(x), np.zeros(2 * B), np.full(B, 0.5), np.full(B, T), [top_k] * B if top_k else None, [share] * B)
+    assert sure.sum() >= B // 2 and keep[sure].any()
+    np.testing.assert_array_equal(got[sure], keep[sure].astype(int))
+    assert ops.error_flags() == 0
 
 
 # ---- eviction in place -------------------------------------------------------------------------------------------------------------------------
