@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(THREADS, 2) weigh_tc_kernel(const __grid_const
                     else if (l != l) r = plain_row(w, st, en, e, g, mine, walk, part, a.parts, four);
                     if (live && w.sink && part == 0) {                  // the sink's term, once
                         const float sk = w.sink[g * R + mine % R] * WEIGH_LOG2E, top = fmaxf(r.x, sk);
-                        r = make_float2(top, (r.x == -INFINITY ? r.y : r.y * ex2(r.x - top)) + ex2(sk - top));
+                        if (top != -INFINITY) r = make_float2(top, (r.x == -INFINITY ? r.y : r.y * ex2(r.x - top)) + ex2(sk - top));      // (else neither has anything yet)
                     }
                     const int64_t row = (int64_t)q0 * NT + mine;
                     if (a.parts > 1) a.stat[part * a.qrows + row] = r;

@@ -1,8 +1,9 @@
 """Drafts verified, the weight of cached keys and eviction at places that test_gpu_between_steps.py does not reach (its docstring has the roundings that the bounds count)."""
 import numpy as np
 import pytest
+import torch
 
-from test_gpu_between_steps import evict, ops, run_verify, up  # noqa: F401
+from test_gpu_between_steps import DEV, Step, evict, ops, run_verify, up, weigh  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -48,6 +49,31 @@ def test_shares_near_one_keep_their_tail(ops, tail, top_k, V):
     assert sure.sum() >= B // 2 and keep[sure].any()
     np.testing.assert_array_equal(got[sure], keep[sure].astype(int))
     assert ops.error_flags() == 0
+
+
+# ---- weights: heads whose sink is none -------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kw", [dict(window=50), dict(chunk=64), dict(window=50, keep_first=3), dict(softcap=3.0, window=50), dict()], ids=str)
+@pytest.mark.parametrize("lens,past,H,G", [([300], [700], 4, 4), ([3], [700], 4, 4), ([130, 1], [0, 400], 8, 2), ([40], [900], 8, 1)])
+@pytest.mark.parametrize("bits", [32, 4])
+def test_sinks_of_minus_infinity(ops, kw, lens, past, H, G, bits):
+    """such a head has no sink: also where a part of the walk over the keys has none that the row sees"""
+    s = Step(ops, np.random.default_rng(H), lens, past, H, G, 64, bits)
+    sink = np.where(np.arange(H) % 2 == 0, -np.inf, 0.7).astype(np.float32)
+    weigh(ops, s, 64 + 14, sink=sink, **kw)
+
+
+@pytest.mark.parametrize("n", [1, 90])
+@pytest.mark.parametrize("sink", [None, -np.inf, 0.5])
+def test_rows_that_see_nothing_but_minus_infinity(ops, n, sink):
+    s = Step(ops, np.random.default_rng(5), [n], [400], 2, 2, 64)
+    s.kpool[:] = float("-inf")
+    s.q = [np.abs(q) + 0.1 for q in s.q]
+    acc = torch.ones(3, 2, 500, device=DEV)
+    dev = None if sink is None else torch.full((2,), sink, device=DEV)
+    ops.key_weights(s.proj(), s.desc, ops.attn_desc(2, 2, 64, 64, 0.125, gated=False, kv_shared=True, sink=dev), s.kpool, acc)
+    want = torch.ones(3, 2, 500, device=DEV)
+    want[int(s.slots[0]), :, 400:400 + n] = 0.0
+    assert torch.equal(acc, want) and ops.error_flags() == 0
 
 
 # ---- eviction in place -------------------------------------------------------------------------------------------------------------------------
