@@ -29,7 +29,7 @@ import torch
 
 from . import seqops
 from .batch import StepEntry, build_step
-from .cache import CacheFull, CacheManager
+from .cache import CacheFull, CacheManager, SeqState
 from .layered import LayeredModel
 
 F32_MAX, F32_TINY = float(np.finfo(np.float32).max), float(np.finfo(np.float32).tiny)
@@ -129,6 +129,8 @@ class Engine:
             if rid in seen:
                 raise ValueError(f"request {rid} appears twice in one step")
             seen.add(rid)
+        if self.max_keys > 0:       # (requests that could not be cut back when it was their turn)
+            self._cut([rid for rid, toks, _ in batch if rid in self.cache.live and self.cache.live[rid].rows + len(toks) > self.weighed_rows])
         try:
             try:
                 for rid, toks, want in batch:
@@ -216,16 +218,16 @@ class Engine:
 
     def _cut(self, rids: Sequence[str]) -> None:
         """cuts those of the live requests back that hold more than max_keys cached rows (a request whose shared pages cannot be replaced yet: after a later step)"""
-        if self.max_keys <= 0:
-            return
-        cut = []
-        for rid in rids:
-            s = self.cache.live.get(rid)
-            if s is not None and s.rows > self.max_keys:
-                pages = self.cache.evict(rid, self.keep_keys, self.recent_keys)
-                if pages is not None:
-                    cut.append((s.slot, pages))
-        if cut:
+        while self.max_keys > 0:        # (a request that is cut back leaves pages, and pages that it shared to those that it shared them with)
+            cut = []
+            for rid in rids:
+                s = self.cache.live.get(rid)
+                if s is not None and s.rows > self.max_keys:
+                    pages = self.cache.evict(rid, self.keep_keys, self.recent_keys)
+                    if pages is not None:
+                        cut.append((s.slot, pages))
+            if not cut:
+                return
             self.model.evict([s for s, _ in cut], [p[2] for _, p in cut], [p[0] for _, p in cut], [p[1] for _, p in cut], self.keep_keys, self.first_keys, self.recent_keys)
             for _, (had, to, _) in cut:
                 self.cache.evicted(had, to)
@@ -330,9 +332,9 @@ class Engine:
             if r.fed < len(r.prompt):
                 continue
             seq = self.cache.live[r.rid]
-            if budget < 1 or self.cache.pages_needed(seq, 1) > free_pages:
+            if budget < 1 or self.cache.pages_needed(seq, 1) > free_pages or self._weight_room(seq) < 1:
                 continue
-            most = min(budget, r.params.max_new_tokens - len(r.output), self.weighed_rows - seq.rows if self.max_keys > 0 else budget) if r.params.draft_fn is not None else 1
+            most = min(budget, r.params.max_new_tokens - len(r.output), self._weight_room(seq)) if r.params.draft_fn is not None else 1
             guess = self._drafts(r, most - 1) if most > 1 else []
             while guess and self.cache.pages_needed(seq, 1 + len(guess)) > free_pages:
                 guess = guess[:-1]
@@ -353,9 +355,9 @@ class Engine:
             held = seq.rows if seq else 0
             own = self.cache.pages_to_copy(seq) if seq else 0       # shared pages that the portion would write into
             room = (have + free_pages - own) * self.cache.block_size - held if free_pages >= own else 0
-            n = min(n, room)
-            if self.max_keys > 0:
-                n = min(n, self.weighed_rows - held)
+            if seq is not None and self._weight_room(seq) < 1:
+                continue                # (it waits to be cut back: nobody waits for it)
+            n = min(n, room, self._weight_room(seq))
             if n < 1:
                 if seq is None:
                     free_slots += r.params.n
@@ -367,10 +369,17 @@ class Engine:
             plan.append((r, r.prompt[r.fed:r.fed + n], [n - 1] if last else []))
         return plan
 
+    def _weight_room(self, seq: Optional[SeqState]) -> int:
+        """rows that a request may still bring before it is cut back (what its weights have room for)"""
+        return self.weighed_rows - (seq.rows if seq is not None else 0) if self.max_keys > 0 else self.max_step_tokens
+
     def step(self) -> List[Request]:
         """one forward pass over what the scheduler picked; returns the requests that finished in it.  A request whose logits leave no choice (sampled, and the
         largest over its temperature is no number) finishes without a token; when all others have theirs, RuntimeError says so"""
         plan = self._schedule()
+        if not plan and self.max_keys > 0:      # (pages that were given back since the last step may let a request be cut back)
+            self._cut([r.rid for r in self.running])
+            plan = self._schedule()
         if not plan:
             if self.has_work():
                 raise CacheFull("no request can make progress: the KV pool is too small for the live requests")

@@ -1,0 +1,88 @@
+"""Requests of a bounded cache and of drafts beside one another, without a GPU (test_drafts_evict_host.py has the stand-in models)."""
+import pytest
+
+from blazr_b200.cache import CacheFull
+from blazr_b200.engine import Engine, SamplingParams
+from test_drafts_evict_host import PROMPT, RowModel, alone, host_argmax, oracle_drafts, verified  # noqa: F401
+
+
+def test_requests_that_cannot_be_cut_back_do_not_stop_others():
+    """two samples share pages that there are no free ones for: they wait when the room of their weights is full, others go on, and so do they when pages are given back"""
+    eng = Engine(RowModel(), max_tokens=36, max_seqs=4, block_size=4, max_keys=16, first_keys=1, max_step_tokens=4)      # 13 pages
+    eng.run_entries([{"id": "x", "tokens": [1] * 4, "want": []}])
+    for _ in range(3):
+        eng.run_entries([{"id": "x", "tokens": [1] * 4, "want": []}])
+    a = eng.add_request("a", PROMPT + PROMPT[:7], SamplingParams(max_new_tokens=30, n=2))
+    for _ in range(12):
+        if eng.cache.live["a"].rows == 20 if "a" in eng.cache.live else False:
+            break
+        eng.step()
+    assert eng.cache.live["a"].rows == eng.cache.live["a#1"].rows == eng.weighed_rows == 20 and eng.cache.pages.free_blocks == 2 and not eng.model.cut
+    c = eng.add_request("c", PROMPT[:2], SamplingParams(max_new_tokens=6))
+    while not c.finished:
+        eng.step()
+    assert c.output == alone(PROMPT[:2], 6) and len(a.output) == 6
+    with pytest.raises(CacheFull):
+        eng.step()
+    eng.release("x")
+    while eng.has_work():
+        eng.step()
+        assert all(s.rows <= 16 for s in eng.cache.live.values())
+    want = alone(PROMPT + PROMPT[:7], 30)
+    assert a.output == a.siblings[0].output == want and eng.model.cut
+    assert eng.cache.pages.free_blocks == eng.cache.pages.num_blocks
+
+
+def test_prompts_that_cannot_be_cut_back_do_not_stop_others():
+    """a prompt and its fork share eight pages, of which a cut would have to replace seven; five are free"""
+    eng = Engine(RowModel(), max_tokens=48, max_seqs=3, block_size=4, max_keys=32, first_keys=1, max_step_tokens=4)      # 15 pages
+    r = eng.add_request("a", PROMPT * 8, SamplingParams(max_new_tokens=3))
+    for _ in range(8):
+        eng.step()
+    q = eng.fork("a", "b")
+    others = eng.cache.pages.alloc(2)
+    assert eng.cache.pages.free_blocks == 5
+    eng.step()
+    eng.step()
+    assert eng.cache.live["a"].rows == eng.cache.live["b"].rows == eng.weighed_rows == 36 and not eng.model.cut
+    c = eng.add_request("c", PROMPT[:2], SamplingParams(max_new_tokens=2))
+    while not c.finished:
+        eng.step()
+    assert c.output == alone(PROMPT[:2], 2)
+    with pytest.raises(CacheFull):
+        eng.step()
+    eng.cache.pages.free(others)
+    with pytest.raises(CacheFull):              # five are free and seven wanted
+        eng.step()
+    eng.cache.release("b")
+    eng.running.remove(q)
+    while eng.has_work():
+        eng.step()
+    assert r.output == alone(PROMPT * 8, 3)
+
+
+def test_sharers_are_cut_back_in_one_step():
+    """the first one takes free pages, the last one keeps those that they shared"""
+    m = RowModel()
+    eng = Engine(m, max_tokens=16, max_seqs=2, block_size=4, max_keys=8, first_keys=1)      # 6 pages
+    eng.run_entries([{"id": "a", "tokens": [1, 2, 3, 4, 5, 6, 7, 8], "want": []}])
+    eng.fork("a", "b")
+    eng.run_entries([{"id": "a", "tokens": [2, 4, 6, 8], "want": []}, {"id": "b", "tokens": [4, 4, 6, 6], "want": []}])
+    a, b = eng.cache.live["a"], eng.cache.live["b"]
+    assert a.rows == b.rows == 7 and m.cut == [(12, 7), (12, 7)] and not set(a.blocks) & set(b.blocks) and eng.cache.pages.free_blocks == 2
+    row = lambda s: [int(m.pages[s.blocks[i // 4], i % 4]) for i in range(7)]
+    assert row(a) == [1, 2, 4, 6, 8, 6, 8] and row(b) == [1, 2, 4, 6, 8, 6, 6]
+
+
+def test_a_request_is_cut_back_before_it_is_refused():
+    m = RowModel()
+    eng = Engine(m, max_tokens=16, max_seqs=2, block_size=4, max_keys=8, first_keys=1)      # 6 pages
+    eng.run_entries([{"id": "a", "tokens": [1] * 8, "want": []}])
+    eng.fork("a", "b")
+    eng.run_entries([{"id": "a", "tokens": [2] * 12, "want": []}])
+    with pytest.raises(CacheFull):
+        eng.run_entries([{"id": "a", "tokens": [3] * 5, "want": []}])
+    assert eng.cache.live["a"].rows == 20 and not m.cut
+    eng.release("b")
+    eng.run_entries([{"id": "a", "tokens": [3] * 5, "want": []}])
+    assert eng.cache.live["a"].n_tokens == 25 and m.cut == [(20, 7), (12, 7)]
