@@ -323,8 +323,9 @@ class Engine:
         return bool(self.waiting or self.running)
 
     def _schedule(self) -> List[Tuple[Request, List[int], List[int]]]:
-        """decoded tokens of running requests first, then prompt portions while the token budget, the slots and the pages last"""
+        """decoded tokens of running requests first, then prompt portions while the token budget, the slots and the pages last, then guesses: no request waits for another's"""
         plan: List[Tuple[Request, List[int], List[int]]] = []
+        guessing: List[int] = []       # places in the plan
         budget = self.max_step_tokens
         free_pages = self.cache.pages.free_blocks
         free_slots = self.cache.slots.free_slots - self._promised()
@@ -334,13 +335,11 @@ class Engine:
             seq = self.cache.live[r.rid]
             if budget < 1 or self.cache.pages_needed(seq, 1) > free_pages or self._weight_room(seq) < 1:
                 continue
-            most = min(budget, r.params.max_new_tokens - len(r.output), self._weight_room(seq)) if r.params.draft_fn is not None else 1
-            guess = self._drafts(r, most - 1) if most > 1 else []
-            while guess and self.cache.pages_needed(seq, 1 + len(guess)) > free_pages:
-                guess = guess[:-1]
-            plan.append((r, [r.output[-1]] + guess, list(range(1 + len(guess)))))
-            budget -= 1 + len(guess)
-            free_pages -= self.cache.pages_needed(seq, 1 + len(guess))
+            if r.params.draft_fn is not None:
+                guessing.append(len(plan))
+            plan.append((r, [r.output[-1]], [0]))
+            budget -= 1
+            free_pages -= self.cache.pages_needed(seq, 1)
         prefilling = [r for r in self.running if r.fed < len(r.prompt)]
         for r in prefilling + list(self.waiting):
             if budget < 1:
@@ -367,6 +366,17 @@ class Engine:
             budget -= n
             last = r.fed + n == len(r.prompt)
             plan.append((r, r.prompt[r.fed:r.fed + n], [n - 1] if last else []))
+        for i in guessing:
+            r, toks, _ = plan[i]
+            seq = self.cache.live[r.rid]
+            most = min(budget, r.params.max_new_tokens - len(r.output) - 1, self._weight_room(seq) - 1)
+            guess = self._drafts(r, most) if most > 0 else []
+            more = lambda n: self.cache.pages_needed(seq, 1 + n) - self.cache.pages_needed(seq, 1)
+            while guess and more(len(guess)) > free_pages:
+                guess = guess[:-1]
+            plan[i] = (r, toks + guess, list(range(1 + len(guess))))
+            budget -= len(guess)
+            free_pages -= more(len(guess))
         return plan
 
     def _weight_room(self, seq: Optional[SeqState]) -> int:

@@ -86,3 +86,40 @@ def test_a_request_is_cut_back_before_it_is_refused():
     eng.release("b")
     eng.run_entries([{"id": "a", "tokens": [3] * 5, "want": []}])
     assert eng.cache.live["a"].n_tokens == 25 and m.cut == [(20, 7), (12, 7)]
+
+
+# ---- guesses take what is left --------------------------------------------------------------------------------------------------------------
+def run_until(eng, done, most):
+    for _ in range(most):
+        if done():
+            return
+        eng.step()
+    assert done()
+
+
+@pytest.mark.parametrize("wrong", [0, 1])
+def test_guesses_take_no_tokens_from_other_requests(verified, wrong):
+    """a step of four tokens, a request that brings nine guesses: others decode in every step, and prompts go on"""
+    eng = Engine(RowModel(), max_tokens=400, max_seqs=4, block_size=4, max_step_tokens=4)
+    a = eng.add_request("a", PROMPT, SamplingParams(max_new_tokens=60, draft_fn=oracle_drafts(9, wrong)))
+    b = eng.add_request("b", PROMPT[:3], SamplingParams(max_new_tokens=9))
+    run_until(eng, lambda: len(a.output) > 2 and b.output, 8)
+    n, m = eng.steps, len(b.output)
+    run_until(eng, lambda: b.finished, 9)
+    assert eng.steps - n == 9 - m and not a.finished
+    c = eng.add_request("c", PROMPT[2:], SamplingParams(max_new_tokens=1))
+    run_until(eng, lambda: c.finished, 3)
+    assert not a.finished
+    run_until(eng, lambda: a.finished, 60)
+    assert (a.output, b.output, c.output) == (alone(PROMPT, 60), alone(PROMPT[:3], 9), alone(PROMPT[2:], 1))
+
+
+def test_guesses_take_no_pages_from_other_requests(verified):
+    """eleven pages of one token are left: the second request needs one in every step, the first one's guesses take the others"""
+    eng = Engine(RowModel(), max_tokens=20, max_seqs=2, block_size=1)
+    a = eng.add_request("a", PROMPT, SamplingParams(max_new_tokens=14, draft_fn=oracle_drafts(30, 1)))
+    b = eng.add_request("b", PROMPT[:3], SamplingParams(max_new_tokens=4))
+    run_until(eng, lambda: b.finished, 4)
+    assert len(a.output) == 4 and not a.finished
+    run_until(eng, lambda: a.finished, 10)
+    assert (a.output, b.output) == (alone(PROMPT, 14), alone(PROMPT[:3], 4))
