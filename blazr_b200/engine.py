@@ -462,7 +462,7 @@ class Engine:
         """up to `most` guesses of the request's next tokens (and the probabilities they were drawn from, kept for the step)"""
         got = r.params.draft_fn(r.prompt + r.output)
         probs = None
-        if isinstance(got, tuple):
+        if isinstance(got, tuple) and len(got) == 2 and np.ndim(got[0]) > 0:      # (two guesses are a tuple of two, too)
             got, probs = got
         tokens = [int(t) for t in got][:max(0, most)]
         vocab = getattr(getattr(self.model, "cfg", None), "vocab", None)

@@ -1,5 +1,7 @@
 """Requests of a bounded cache and of drafts beside one another, without a GPU (test_drafts_evict_host.py has the stand-in models)."""
+import numpy as np
 import pytest
+import torch
 
 from blazr_b200.cache import CacheFull
 from blazr_b200.engine import Engine, SamplingParams
@@ -123,3 +125,14 @@ def test_guesses_take_no_pages_from_other_requests(verified):
     assert len(a.output) == 4 and not a.finished
     run_until(eng, lambda: a.finished, 10)
     assert (a.output, b.output) == (alone(PROMPT, 14), alone(PROMPT[:3], 4))
+
+
+def test_guesses_in_other_containers(verified):
+    """tuples of one, two and three guesses, arrays, tensors; with None for the probabilities of certain ones"""
+    want = alone(PROMPT, 13)
+    for make in (tuple, np.array, torch.tensor, lambda g: tuple(torch.tensor(g)), lambda g: (g, None), lambda g: (torch.tensor(g), None), lambda g: tuple(np.array(g))):
+        for n in (1, 2, 3):
+            fn = oracle_drafts(n)
+            eng = Engine(RowModel(), max_tokens=100, max_seqs=1, block_size=4)
+            assert eng.generate([PROMPT], SamplingParams(max_new_tokens=13, draft_fn=lambda t: make(fn(t))))[0] == want
+            assert eng.steps == 1 + 12 // (n + 1)
