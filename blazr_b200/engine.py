@@ -490,7 +490,7 @@ class Engine:
             u = [torch.rand(n + 1, device=dev, generator=r._gen) if r._gen is not None else torch.zeros(n + 1, device=dev) for (r, _, _), n in zip(part, lens)]
             kw: Dict[str, torch.Tensor] = {}
             if any(r.params.top_k for r, _, _ in part):
-                kw["top_k"] = up([r.params.top_k for r, _, _ in part], np.int32)
+                kw["top_k"] = up([min(max(r.params.top_k, 0), logits.shape[1]) for r, _, _ in part], np.int32)      # (as many as there are: all)
             if any(r.params.top_p < 1.0 for r, _, _ in part):
                 kw["top_p"] = up([r.params.top_p for r, _, _ in part], np.float32)
             if known:

@@ -5,7 +5,7 @@ import torch
 
 from blazr_b200.cache import CacheFull
 from blazr_b200.engine import Engine, SamplingParams
-from test_drafts_evict_host import PROMPT, RowModel, alone, host_argmax, oracle_drafts, verified  # noqa: F401
+from test_drafts_evict_host import PROMPT, VOCAB, RowModel, alone, host_argmax, oracle_drafts, verified  # noqa: F401
 
 
 def test_requests_that_cannot_be_cut_back_do_not_stop_others():
@@ -136,3 +136,11 @@ def test_guesses_in_other_containers(verified):
             eng = Engine(RowModel(), max_tokens=100, max_seqs=1, block_size=4)
             assert eng.generate([PROMPT], SamplingParams(max_new_tokens=13, draft_fn=lambda t: make(fn(t))))[0] == want
             assert eng.steps == 1 + 12 // (n + 1)
+
+
+@pytest.mark.parametrize("top_k,T", [(2 ** 31, 0.5), (10 ** 12, 0.0), (-5, 0.0), (-2 ** 40, 0.0), (VOCAB, 0.5)])
+def test_drafts_with_a_top_k_of_any_size(verified, top_k, T):
+    """numbers that 32 bits do not hold, and negative ones beside a temperature of zero, choose among all tokens, as without drafts"""
+    kw = dict(max_new_tokens=10, temperature=T, seed=1)
+    eng = Engine(RowModel(), max_tokens=100, max_seqs=1, block_size=4)
+    assert eng.generate([PROMPT], SamplingParams(top_k=top_k, draft_fn=oracle_drafts(3), **kw))[0] == alone(PROMPT, 10)
