@@ -1767,7 +1767,7 @@ class LayeredModel:
                 if m.norm == "joint":
                     P = ops.retention_partials(T, B, H, V)
                     close.update(sumsq=ws.sumsq.view(-1)[:T * P].view(T, P), sumsq_count=H * V)
-                ops.retention(proj, st, L["desc"], L["ret_state"], o, ws.scratch, sumsq=close.get("sumsq"))
+                ops.retention(proj, self._desc(ws, T, B, "abs"), L["desc"], L["ret_state"], o, ws.scratch, sumsq=close.get("sumsq"))
                 ops.linear(o, L["w_o"], y)
             elif ls.kind == "attention":
                 self._attention_out(L, m, ws, st, T, proj, y)
@@ -1867,7 +1867,7 @@ class LayeredModel:
         proj = ws.proj[:T, :L["w_in"].shape[0]]
         seqops.linear(a, L["w_in"], proj)
         o = ws.inner_a.view(-1)[:T * m.heads * m.vdim].view(T, m.heads * m.vdim)
-        seqops.retention(proj, st, L["desc"], L["ret_state"], o, ws.scratch)
+        seqops.retention(proj, self._desc(ws, T, st.B, "abs"), L["desc"], L["ret_state"], o, ws.scratch)
         seqops.linear(o, L["w_o"], y)
 
     def _latent_attention(self, L, m: LatentAttentionSpec, ws: _Workspace, st, T: int, a: torch.Tensor, y: torch.Tensor) -> None:
