@@ -417,7 +417,7 @@ using namespace b200seq;
 extern "C" {
 
 const char* b200seq_last_error(void) { return g_err; }
-int b200seq_version(void) { return 1; }
+int b200seq_version(void) { return B200SEQ_VERSION; }
 int64_t b200seq_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }
 
 int b200seq_error_flags(int* flags_out) {

@@ -201,6 +201,7 @@ def ensure_built(force: bool = False) -> str:
 
 
 _lib = None
+VERSION = 2      # of the structs above (include/b200seq.h)
 
 
 def lib() -> C.CDLL:
@@ -208,6 +209,8 @@ def lib() -> C.CDLL:
     if _lib is None:
         ensure_built()
         L = C.CDLL(LIB_PATH)
+        if L.b200seq_version() != VERSION:
+            raise SeqError(-1, f"{LIB_PATH} is of version {L.b200seq_version()}, its structs are not those of version {VERSION}")
         L.b200seq_last_error.restype = C.c_char_p
         L.b200seq_launch_count.restype = C.c_int64
         L.b200seq_kv4_page_bytes.restype = C.c_int64

@@ -60,6 +60,9 @@ extern "C" {
 #define B200SEQ_PATH_TILED 2  /* float32 FMA tiles (any M, exact 32-bit arithmetic) */
 #define B200SEQ_PATH_TC 3     /* tcgen05 tensor-core tiles (bf16 activations) */
 
+/* Goes up when one of the structs below changes: a caller and a library of different versions do not go together.  2: b200seq_attn_desc ends with rot_pos. */
+#define B200SEQ_VERSION 2
+
 typedef struct b200seq_step {
     const int32_t* tok_ent;
     const int32_t* tok_pos;
@@ -71,7 +74,7 @@ typedef struct b200seq_step {
 } b200seq_step;
 
 const char* b200seq_last_error(void);
-int b200seq_version(void);
+int b200seq_version(void);      /* the B200SEQ_VERSION that the library was built with */
 int64_t b200seq_launch_count(void);
 /* bit 0: a KV position fell outside its block table; bit 1: a bounded wait of the tensor-core GEMM ran out; bit 2: an expert table entry outside the experts;
  * bit 3: a value beyond what a 4-bit cache holds; bit 4: a token id outside the vocabulary */
