@@ -96,8 +96,10 @@ __device__ __forceinline__ void fetch_key(const WeighArgs& a, uint32_t dst, int 
 }
 
 // grid (blocks of 64 * tiles keys, key heads, entries).  NRT: tiles of eight rows that are gone through at a time.  JOINED: a sequence's blocks are one cluster, which joins their
-// maxima and sums itself and adds the weights up at once.  (For steps whose blocks are all on the GPU together: one token of 500 keys 14.2 -> 11.7 us; in several waves the blocks
-// that wait for one another keep others out, 32 sequences 88 -> 137.)
+// maxima and sums itself and adds the weights up at once.  (For steps whose blocks are all on the GPU together, two an SM: one token of 500 keys 14.2 -> 11.7 us; in several waves the
+// blocks that wait for one another keep others out, 32 sequences 88 -> 137.  With four tiles of rows and f32 keys of more than 64 values a block has 117 KB of shared memory and
+// an SM one block; joined steps are then the faster ones up to two waves.  Waves of clusters leave SMs idle: 30 clusters of eight, 40 of six, 64 of four and 144 of two take 22 us for
+// 25 to 26 in two launches, 32, 48 and 72 of the first three 31, 57 for 46 (64 rows) and 31.)
 template <int NRT, int NG, bool FOUR, bool JOINED>
 __global__ void __launch_bounds__(RT, 2) weigh_rows_kernel(const __grid_constant__ WeighArgs a, const __grid_constant__ b200seq_step st, int tiles) {
     chain_enter();
@@ -583,9 +585,10 @@ int b200seq_key_weights(const float* proj, int64_t ld, const b200seq_step* st, c
     if (!proj || !kpool || !acc || slots < 1 || acc_ld < 1 || last < 0 || max_keys < 0) return fail(B200SEQ_ERR_INVALID_ARG, "key_weights: bad arguments");
     if (st->T == 0 || st->B == 0) return 0;
     if (ld < (int64_t)d->q_col + (int64_t)d->H * d->D && st->T > 1) return fail(B200SEQ_ERR_INVALID_ARG, "key_weights: row stride below the queries' columns");
-    const Plan p = plan_of(*st, *d, last, max_keys);
+    Plan p = plan_of(*st, *d, last, max_keys);
     if (!scratch || scratch_floats < p.floats || (reinterpret_cast<uintptr_t>(scratch) & 15)) return fail(B200SEQ_ERR_INVALID_ARG, "key_weights: the work area is too small or not on a 16-byte boundary");
     const bool four = kv_bits == 4;
+    if (p.joined && !four && d->D > 64 && p.row_tiles == 4) p.joined = (int64_t)p.blocks * d->G * st->B <= (p.blocks <= 2 ? 2 * 148 : p.blocks <= 4 ? 256 : 240);
     if (four && (reinterpret_cast<uintptr_t>(kpool) & 15)) return fail(B200SEQ_ERR_INVALID_ARG, "key_weights: 4-bit pools start on a 16-byte boundary");
     const cudaStream_t cs = (cudaStream_t)stream;
     WeighArgs a = {};

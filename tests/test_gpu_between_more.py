@@ -76,6 +76,16 @@ def test_rows_that_see_nothing_but_minus_infinity(ops, n, sink):
     assert torch.equal(acc, want) and ops.error_flags() == 0
 
 
+@pytest.mark.parametrize("B,n,past,G,D,bits,launches", [(4, 8, 500, 8, 128, 32, 2), (3, 8, 500, 8, 128, 32, 1), (9, 8, 240, 8, 128, 32, 2), (18, 8, 100, 8, 128, 32, 1), (6, 16, 250, 8, 128, 32, 2),
+                                                        (4, 8, 500, 8, 64, 32, 1), (4, 8, 500, 8, 128, 4, 1), (4, 6, 500, 8, 128, 32, 1)])
+def test_steps_are_joined_where_their_blocks_fit(ops, B, n, past, G, D, bits, launches):
+    """four tiles of rows with f32 keys above 64 values: one block an SM instead of two, and one launch up to two waves of clusters"""
+    s = Step(ops, np.random.default_rng(B), [n] * B, [past] * B, 4 * G, G, D, bits)
+    before = ops.launch_count()
+    weigh(ops, s, D + 14)
+    assert ops.launch_count() - before == launches
+
+
 # ---- eviction in place -------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("kw", [dict(rows=[9000], keep=8000, L=1, G=4, D=128), dict(rows=[7000, 6500], keep=3000, L=2, G=2, D=80), dict(rows=[6000], keep=5990, L=1, G=1, D=600),
                                 dict(rows=[5000] * 3, keep=4900, L=2, G=2, D=128, bits=4), dict(rows=[4000], keep=3999, L=1, G=3, D=7)], ids=str)
