@@ -613,6 +613,7 @@ class LayeredModel:
         self.kv_bits, self._keys, self.weighed_rows, self.weigh_last = 32, 0, 0, 0
         self._ws: Dict[int, _Workspace] = {}
         self._graphs: Dict[int, object] = {}
+        self._graph_pool = None
         self.use_graphs = True
         self.overlap_branches = True     # depth layout: mixer and feed-forward of a layer on two streams
         self._side = self._side2 = None
@@ -1214,6 +1215,7 @@ class LayeredModel:
                 L["key_weight"] = torch.zeros((max_seqs, L["desc"].G, weighed_rows), **f32)
         self._ws.clear()
         self._graphs.clear()
+        self._graph_pool = None
 
     def scratch_floats(self, cap: int) -> int:
         """floats of the largest work area any layer wants for a step of up to `cap` tokens"""
@@ -1370,7 +1372,9 @@ class LayeredModel:
                 s = torch.cuda.Stream(self.dev)
                 s.wait_stream(torch.cuda.current_stream(self.dev))
                 with torch.cuda.stream(s):
-                    with torch.cuda.graph(g, stream=s):
+                    # (captured steps run one after the other: one pool has the work areas of all of them, not each its own)
+                    self._graph_pool = self._graph_pool or torch.cuda.graph_pool_handle()
+                    with torch.cuda.graph(g, pool=self._graph_pool, stream=s):
                         self._run(ws, T, B, R, sample, None)
                 torch.cuda.current_stream(self.dev).wait_stream(s)
                 self._graphs[key] = g
