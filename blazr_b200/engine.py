@@ -20,6 +20,7 @@ steps run (seqops.key_weights), and a request that holds more rows is cut back t
 """
 from __future__ import annotations
 
+from array import array
 from collections import deque
 from dataclasses import dataclass, field, replace
 from typing import Any, Callable, Deque, Dict, List, Optional, Sequence, Set, Tuple
@@ -68,12 +69,14 @@ def lookup_drafts(most: int, match: int = 3) -> Callable[[List[int]], List[int]]
         raise ValueError(f"{most} drafts by {match} tokens")
 
     def drafts(tokens: List[int]) -> List[int]:
-        for m in range(min(match, len(tokens) - 1), 0, -1):
-            tail = tokens[-m:]
-            for i in range(len(tokens) - m - 1, -1, -1):
-                if tokens[i:i + m] == tail:
-                    return tokens[i + m:i + m + most]
-        return []
+        text, hits = np.frombuffer(array("q", tokens), dtype=np.int64), None
+        for m in range(min(match, len(tokens) - 1)):       # places whose last m + 1 tokens are the text's
+            ends = np.nonzero(text[:-1] == text[-1])[0] if m == 0 else hits[hits >= m]
+            ends = ends[text[ends - m] == text[-1 - m]]
+            if not ends.size:
+                break
+            hits = ends
+        return tokens[hits[-1] + 1:hits[-1] + 1 + most] if hits is not None else []
     return drafts
 
 

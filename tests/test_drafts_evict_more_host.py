@@ -1,10 +1,12 @@
 """Requests of a bounded cache and of drafts beside one another, without a GPU (test_drafts_evict_host.py has the stand-in models)."""
+import time
+
 import numpy as np
 import pytest
 import torch
 
 from blazr_b200.cache import CacheFull
-from blazr_b200.engine import Engine, SamplingParams
+from blazr_b200.engine import Engine, SamplingParams, lookup_drafts
 from test_drafts_evict_host import PROMPT, VOCAB, RowModel, alone, host_argmax, oracle_drafts, verified  # noqa: F401
 
 
@@ -144,3 +146,31 @@ def test_drafts_with_a_top_k_of_any_size(verified, top_k, T):
     kw = dict(max_new_tokens=10, temperature=T, seed=1)
     eng = Engine(RowModel(), max_tokens=100, max_seqs=1, block_size=4)
     assert eng.generate([PROMPT], SamplingParams(top_k=top_k, draft_fn=oracle_drafts(3), **kw))[0] == alone(PROMPT, 10)
+
+
+def plain_lookup(tokens, most, match):
+    for m in range(min(match, len(tokens) - 1), 0, -1):
+        for i in range(len(tokens) - m - 1, -1, -1):
+            if tokens[i:i + m] == tokens[-m:]:
+                return tokens[i + m:i + m + most]
+    return []
+
+
+def test_lookups_in_long_texts():
+    """the same guesses as one place after the other gives, without the time that takes (a text of 32000 tokens without a match: 20 ms, several steps of a model)"""
+    rng = np.random.default_rng(0)
+    for n in list(range(0, 12)) + [50, 300]:
+        for vocab in (1, 2, 5, 40, 2 ** 40):
+            for most, match in ((0, 3), (1, 1), (4, 3), (9, 7)):
+                text = [int(x) for x in rng.integers(0, vocab, n)]
+                assert lookup_drafts(most, match)(text) == plain_lookup(text, most, match)
+    text = [int(x) for x in rng.integers(0, 1000, 32000)] + [5000]
+
+    def least(f):
+        times = []
+        for _ in range(5):
+            t = time.perf_counter()
+            assert f(text) == []
+            times.append(time.perf_counter() - t)
+        return min(times)
+    assert least(lookup_drafts(4)) < least(lambda x: plain_lookup(x, 4, 3)) / 4
