@@ -99,8 +99,9 @@ class Engine:
         """max_tokens: tokens all live requests may hold together (the KV pool is made for this many, rounded up to pages);
         max_seqs: state slots = most requests live at a time; kv_bits: bits of a cached key or value, 32 or 4.
         max_keys: > 0: a request that holds more cached rows between two steps is cut back to seven eighths of them: the first first_keys, the last recent_keys (0: a quarter of
-        max_keys) and, in every layer and key head, those that were given the most attention since they came.  weigh_last: only the attention of that many last tokens of
-        a step's portion counts (0: of all)"""
+        max_keys) and, in every layer and key head, those that were given the most attention since they came (by guesses that were rejected, too).  weigh_last: only the attention
+        of that many last tokens of a step's portion counts (0: of all).  Beside the cache, steps of many tokens or long sequences take a work area for the weights of up to
+        256 MB of scores or keys, and some for the tokens"""
         self.model = model
         self.cache = CacheManager(max_tokens, max_seqs, block_size, model.pooled_sizes() if hasattr(model, "pooled_sizes") else ())
         room = self.cache.pages.num_blocks * block_size
