@@ -4,11 +4,12 @@
 // strictly larger z are below top_p of their sum;  p = w / sum.  Draft x of row i is accepted when u_i q(x) < p(x).  The next token comes from max(p - q, 0) of the row that
 // rejected (from p where that is nothing), or from the last row's p: the lowest one whose cumulated weight exceeds u times the sum.  T <= 0: p = 1 at the first maximum.
 //
-// What a row decides is compared with a random number, so that its sums are held in 64 bits (weights are f32, within 2^-21 of themselves; sums of four of them, then f64).
-// Measured: 64 entries of 4 drafts, 128256 logits a row, 55 us (33.5 + 28; the logits' bytes alone 25, the draft's probabilities of a row an entry 5); one of 32000 logits 18.6, a chain of
-// loads and of the clusters' barriers; 16 entries of 3 drafts with top_k and top_p 52 to 56 (thresholds 42).
+// What a row decides is compared with a random number, so that its sums are held in 64 bits.  The weights behind one comparison (a draft, the end of top_p) are f32, within 2^-21 of
+// themselves; a draw is a comparison with 10^5 sums, and its weights are made in 64 bits, within 2^-34.
+// Measured: 64 entries of 4 drafts, 128256 logits a row, 61 us (33.5 + 35; with draws of f32 weights 55, 28 of them; the logits' bytes alone 25, the draft's probabilities of a row an
+// entry 5); one of 32000 logits 19, a chain of loads and of the clusters' barriers; 16 entries of 3 drafts with top_k and top_p 52 to 57 (thresholds 42 to 45).
 // The floor is the logits' bytes: they are read once, in slices over the whole GPU (row_stats), with maximum, its place and sum left for every slice.  Then a cluster of eight
-// CTAs an entry puts the slices together, finds the row that rejects and reads that one again, from L2 (pick).
+// CTAs an entry puts the slices together, finds the row that rejects and reads that one again, from L2, every warp a run of it (pick).
 // top_k and top_p need a threshold a row before that (row_cut, a CTA a row, which it reads twice or three times from L2): counts, or masses (whole numbers of 2^-42: additions whose
 // order does not matter, off by 2^-43 a token: 2^-26 of the largest weight for 128 k), of 2048 bins of equal width below the maximum show how far down the k-th logit lies, or where the mass passes the share; the logits down to there are sorted.
 // Where those are too many (rows of equal logits, logits far apart), the threshold is selected by the bits of the ordered logits instead, eleven at a time.
@@ -28,10 +29,9 @@ constexpr int ERR_TOKEN = 16;             // error flag: a token id outside the 
 constexpr int CLUSTER = 8;
 constexpr int QUADS = 8;                  // 16-byte pieces of a slice of a row a thread has
 constexpr int STATS = 256, PICK = 256, CUT = 1024;     // threads
-constexpr int MAX_TILES = 512;            // tiles of 4 * PICK logits of one CTA's share
 constexpr int BINS = 2048, LIST = 2048;   // bins below the maximum; logits that are sorted
 constexpr float MASS = 0x1p42f;           // masses as whole numbers: MAX_V weights of one fit 64 bits
-constexpr int64_t MAX_V = (int64_t)CLUSTER * MAX_TILES * 4 * PICK - 64;
+constexpr int64_t MAX_V = (1 << 22) - 64;
 
 struct Partial {      // of a slice of a row
     double sum;       // of exp((z - max) / T)
@@ -80,6 +80,30 @@ struct Heat {
         return z == -INFINITY ? 0.f : tcsplit::ex2(fmaf(d, hi, d * lo));
     }
 };
+
+// The same weight to 2^-34 of itself: 2^u, u = (z - m) log2(e) / T, as 2^n 2^f with n whole and |f| <= 1/2, 2^f by the polynomial of the seventh degree that equals it at the Chebyshev
+// nodes of that interval.  Logits below `least`, and those of weights below 2^-1000, have none.
+struct FineHeat {
+    double m, c;
+    float lowest;
+    __device__ __forceinline__ FineHeat(float T, float max, float least) {
+        m = (double)max, c = 1.4426950408889634 / (double)T;
+        lowest = fmaxf(fmaxf(__fsub_ru(max, __double2float_rd(1000.0 / c)), -FLT_MAX), least);
+    }
+    __device__ __forceinline__ double operator()(float z) const {
+        const double d = (double)z - m, k = fma(d, c, 6755399441055744.0), f = fma(d, c, -(k - 6755399441055744.0));      // (1.5 2^52: the last digits are n)
+        double p = 1.5303700711232177e-05;
+        p = fma(p, f, 1.5469729214116396e-04), p = fma(p, f, 1.3333478473686084e-03), p = fma(p, f, 9.6180256133180427e-03), p = fma(p, f, 5.5504109063258658e-02);
+        p = fma(p, f, 2.4022651213498092e-01), p = fma(p, f, 6.9314718055683244e-01), p = fma(p, f, 9.9999999995956179e-01);
+        const int hi = __double2hiint(p) + (__double2loint(k) << 20);
+        return z >= lowest ? __hiloint2double(hi, __double2loint(p)) : 0.0;
+    }
+};
+// a finite number of normal size in 64 bits, by its bits (conversions go through a unit of a quarter of the rate); 0 as 2^-127, infinities and NaN as 2^128 or more
+__device__ __forceinline__ double widened(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return __hiloint2double((int)((b & 0x80000000u) | (((b & 0x7fffffffu) >> 3) + (896u << 20))), (int)(b << 29));
+}
 
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
@@ -449,11 +473,19 @@ __global__ void __launch_bounds__(CUT, 1) row_cut_kernel(const __grid_constant__
     if (tid == 0) a.cut[row] = Cut{total, key_value(least), 1};
 }
 
+// what a warp or a block has of a row: the weights to draw from, all weights, and the draft's probabilities where weights are left
+struct Share {
+    double draw, all;
+    float off;
+    __device__ __forceinline__ void add(const Share& o) { draw += o.draw, all += o.all, off += o.off; }
+};
+
 // grid: a cluster an entry
 __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_kernel(const __grid_constant__ VerifyArgs a) {
     chain_enter();
     constexpr int WARPS = PICK / 32, ROWS = 32;
-    __shared__ double part[MAX_TILES][WARPS], tile_sum[MAX_TILES], scan[PICK], warp_part[WARPS], cta_sum;
+    __shared__ double scan[PICK], warp_part[WARPS];
+    __shared__ Share warp_share[WARPS], cta_share;
     __shared__ int first_bad, found, last_some;
     __shared__ Row rows_sh[ROWS], row_sh;
     cg::cluster_group cl = cg::this_cluster();
@@ -513,118 +545,137 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_ker
         if (rank == 0 && tid == 0) a.tokens[row] = r.none() ? -1 : r.at;
         return;
     }
-    double sum = r.sum;
     float least = -INFINITY;
-    if (a.cut && a.cut[row].on) sum = a.cut[row].total, least = a.cut[row].least;
-    const float inv = (float)(1.0 / sum);
+    double about = r.sum;                                   // the row's sum, to the digits of 32-bit weights
+    if (a.cut && a.cut[row].on) about = a.cut[row].total, least = a.cut[row].least;
     const float* x = a.x + row * a.ld;
-    const float* q = a.q ? a.q + row * a.ldq : nullptr;
-    const int drafted = a.drafts[row], shift = quad_shift(x);
+    const float* q = a.q && acc < n ? a.q + row * a.ldq : nullptr;
+    const int certain = acc < n && !q ? a.drafts[row] : -1, shift = quad_shift(x);
     const bool aligned_q = q && (quad_shift(q) == shift);
-    const int tiles_all = ((a.V + shift + 3) / 4 + PICK - 1) / PICK, per = (tiles_all + CLUSTER - 1) / CLUSTER;
-    const int t0 = min(tiles_all, rank * per), t1 = min(tiles_all, t0 + per);
-    bool rest = acc < n;
-    // the weights of the four logits of a tile that are this thread's
-    auto weights = [&](int t, float (&w)[4]) {
-        const int i = 4 * (t * PICK + tid) - shift;
+    // Weights in 64 bits: which of 10^5 sums is the first beyond the target is known only to their own digits (in 32 bits one draw in 10^4 was the neighbour's).  Drawn from is what
+    // w has more than S q, S the sum of all w.  That is known only behind the walk over the row, which takes `about` for S: where weights are left, sums of q tell what that changes.
+    const FineHeat weight(T, r.max, least);
+    // the four weights of a lane at quad k, and q; false: the whole warp has none
+    auto weights = [&](int k, double (&w)[4], float (&qv)[4]) {
+        const int i = 4 * k - shift;
         const float4 z4 = quad(x, i, a.V, -INFINITY);
+        const float z[4] = {z4.x, z4.y, z4.z, z4.w};
         float4 q4 = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (rest && q) {
+        if (q) {
             if (aligned_q) q4 = quad(q, i, a.V, 0.f);
             else q4 = make_float4(i >= 0 && i < a.V ? q[i] : 0.f, i + 1 >= 0 && i + 1 < a.V ? q[i + 1] : 0.f, i + 2 >= 0 && i + 2 < a.V ? q[i + 2] : 0.f,
                                   i + 3 >= 0 && i + 3 < a.V ? q[i + 3] : 0.f);
         }
-        const float z[4] = {z4.x, z4.y, z4.z, z4.w}, qv[4] = {q4.x, q4.y, q4.z, q4.w};
+        qv[0] = q4.x, qv[1] = q4.y, qv[2] = q4.z, qv[3] = q4.w;
+        const bool some = __any_sync(0xffffffffu, fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])) >= weight.lowest);
+        if (some) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = weight(z[j]);
+        }
+        return some;
+    };
+    auto left = [&](double w, float qv, double all) {      // (a q that is no number takes all)
+        if (!q) return w;
+        const double l = fma(-all, widened(qv), w);
+        return __double2hiint(l) < 0 ? 0.0 : l;
+    };
+    // every warp a run of neighbouring quads, every lane its sums
+    const int quads = (a.V + shift + 3) / 4, run = ((quads + CLUSTER * WARPS - 1) / (CLUSTER * WARPS) + 31) & ~31;
+    Share mine{0.0, 0.0, 0.f};
+    const int k0 = (rank * WARPS + warp) * run;
+#pragma unroll 4
+    for (int k = k0 + lane; k < min(k0 + run, (quads + 31) & ~31); k += 32) {
+        double w[4];
+        float qv[4];
+        if (!weights(k, w, qv)) continue;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            float p = z[j] >= least ? heat(z[j], r.max) * inv : 0.f;
-            if (rest) p -= q ? qv[j] : (i + j == drafted ? 1.f : 0.f);
-            w[j] = fmaxf(p, 0.f);
+            mine.all += w[j];
+            const double l = 4 * k - shift + j == certain ? 0.0 : left(w[j], qv[j], about);
+            mine.draw += l;
+            if (q && __double2hiint(l) > 0) mine.off += qv[j];
         }
-    };
-    double total;
-    for (;;) {
-#pragma unroll 4
-        for (int t = t0; t < t1; ++t) {
-            float w[4];
-            weights(t, w);
-            const double s = warp_sum((double)((w[0] + w[1]) + (w[2] + w[3])));
-            if (lane == 0) part[t - t0][warp] = s;
-        }
-        __syncthreads();
-        for (int t = tid; t < t1 - t0; t += PICK) {
-            double y = 0.0;
-            for (int k = 0; k < WARPS; ++k) y += part[t][k];
-            tile_sum[t] = y;
-        }
-        __syncthreads();
-        if (tid == 0) {
-            double y = 0.0;
-            for (int t = t0; t < t1; ++t) y += tile_sum[t - t0];
-            cta_sum = y;
-        }
-        cl.sync();
-        total = 0.0;
-        for (int c = 0; c < CLUSTER; ++c) total += *cl.map_shared_rank(&cta_sum, c);
-        if (!rest || total > 0.0) break;
-        rest = false;                                       // nothing is left of the draft's excess: the target's own probabilities
-        cl.sync();
     }
-    const double target = (double)u_e * total;
+    mine.draw = warp_sum(mine.draw), mine.all = warp_sum(mine.all);
+    if (q) mine.off = warp_sum(mine.off);
+    if (lane == 0) warp_share[warp] = mine;
+    __syncthreads();
+    if (tid == 0) {
+        Share y = warp_share[0];
+        for (int k = 1; k < WARPS; ++k) y.add(warp_share[k]);
+        cta_share = y;
+    }
+    cl.sync();
+    Share row_share{0.0, 0.0, 0.f}, share[CLUSTER];
+#pragma unroll
+    for (int k = 0; k < CLUSTER; ++k) share[k] = *cl.map_shared_rank(&cta_share, k), row_share.add(share[k]);
+    const double more = q ? row_share.all - about : 0.0;
+    const bool rest = row_share.draw - more * (double)row_share.off > 0.0;      // (else nothing is left of the draft's excess: the target's own probabilities)
+    auto drawn = [&](const Share& y) { return rest ? y.draw - more * (double)y.off : y.all; };
+    const double target = (double)u_e * drawn(row_share);
     double before = 0.0, base = 0.0;
+    bool passed = false;
     int owner = -1;                                         // the CTA in whose share the sum passes the target (rounding: the last that has any)
-    for (int c = 0; c < CLUSTER; ++c) {
-        const double y = *cl.map_shared_rank(&cta_sum, c);
-        if (y > 0.0) {
-            owner = c, base = before;
-            if (before + y > target) break;
-        }
+#pragma unroll
+    for (int k = 0; k < CLUSTER; ++k) {
+        const double y = drawn(share[k]);
+        if (y > 0.0 && !passed) owner = k, base = before, passed = before + y > target;
         before += y;
     }
     if (rank == owner) {
-        int tile = t0;
+        int of = 0;
         before = base;
-        for (int t = t0; t < t1; ++t) {
-            const double y = tile_sum[t - t0];
+        for (int k = 0; k < WARPS; ++k) {
+            const double y = drawn(warp_share[k]);
             if (y > 0.0) {
-                tile = t, base = before;
+                of = k, base = before;
                 if (before + y > target) break;
             }
             before += y;
         }
-        float w[4];
-        weights(tile, w);
-        const float own = (w[0] + w[1]) + (w[2] + w[3]);
-        double s = (double)own;
-        const int i = 4 * (tile * PICK + tid) - shift;
         if (tid == 0) found = 0x7fffffff, last_some = -1;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double y = __shfl_up_sync(0xffffffffu, s, o);
-            if (lane >= o) s += y;
-        }
-        if (lane == 31) warp_part[warp] = s;
         __syncthreads();
-        for (int k = 0; k < warp; ++k) s += warp_part[k];
-        scan[tid] = s;
-        __syncthreads();
-        double cum = base + (tid ? scan[tid - 1] : 0.0);
-        if (own > 0.f) {
-            int last = -1;
+        // that warp's run, by the block: a tile of its quads at a time
+        const int from = (rank * WARPS + of) * run, to = min(from + run, quads);
+        for (int t = from; t < to; t += PICK) {
+            double w[4];
+            float qv[4];
+            const int k = t + tid;
+            if (!weights(min(k, quads), w, qv)) w[0] = w[1] = w[2] = w[3] = 0.0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                cum += (double)w[j];
-                if (w[j] > 0.f) {
-                    last = i + j;
-                    if (cum > target) {
-                        atomicMin(&found, i + j);
-                        break;
+            for (int j = 0; j < 4; ++j) w[j] = k >= to ? 0.0 : rest ? (4 * k - shift + j == certain ? 0.0 : left(w[j], qv[j], row_share.all)) : w[j];
+            const double own = (w[0] + w[1]) + (w[2] + w[3]);
+            double s = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double y = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += y;
+            }
+            if (lane == 31) warp_part[warp] = s;
+            __syncthreads();
+            for (int v = 0; v < warp; ++v) s += warp_part[v];
+            scan[tid] = s;
+            __syncthreads();
+            double cum = base + (tid ? scan[tid - 1] : 0.0);
+            if (own > 0.0) {
+                int last = -1;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    cum += w[j];
+                    if (w[j] > 0.0) {
+                        last = 4 * k - shift + j;
+                        if (cum > target) {
+                            atomicMin(&found, last);
+                            break;
+                        }
                     }
                 }
+                atomicMax(&last_some, last);
             }
-            atomicMax(&last_some, last);
+            base += scan[PICK - 1];
+            __syncthreads();
+            if (found != 0x7fffffff) break;
         }
-        __syncthreads();
         if (tid == 0) a.tokens[row] = found != 0x7fffffff ? found : last_some;
     }
     cl.sync();                                              // nobody's sums go while they are read

@@ -539,7 +539,7 @@ int b200seq_process_logits(const float* x, int64_t ldx, int R, int V, const floa
  * its drafts drafts[row], in order, and one row more (whose draft is not read).  An entry of one row has no drafts: a token is sampled.  With its temperature T:
  *   w = exp((z - max z) / T), kept where z >= the top_k-th largest z (top_k[e] > 0) and then where the kept weights of strictly larger z are below top_p[e] of their sum
  *   (top_p[e] < 1; at least the largest);   p = w / sum of the kept.   T <= 0: p = 1 at the first maximum
- *   (sums are within 2^-19 of themselves, and what lies before a token in them for top_p within V 2^-43 + V 2^-46 more, of the largest weight)
+ *   (w is within 2^-19 of itself where a draft is accepted and where top_p ends, for the latter with V 2^-43 + V 2^-46 of the largest weight; within 2^-34 where a token is drawn)
  * A draft x is accepted when accept_u[row] * q(x) < p(x), q(x) = draft_probs[row][x] (f32 [R, V], stride ldq; null: 1), at T <= 0 when it is the first maximum.  The token behind the
  * accepted drafts is drawn from max(p - q, 0) of the row that rejected (null: p without the draft; where nothing is left: p), or from the last row's p: the lowest token whose
  * cumulated weight exceeds sample_u[e] times the sum.  accepted[e]: how many drafts; tokens[start[e] ..]: the accepted drafts, the token behind them, then -1 (not written over drafts).

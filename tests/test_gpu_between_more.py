@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 import torch
 
+import between_oracle as oracle
 from test_gpu_between_steps import DEV, Step, evict, ops, run_verify, up, weigh  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -49,6 +50,40 @@ def test_shares_near_one_keep_their_tail(ops, tail, top_k, V):
     assert sure.sum() >= B // 2 and keep[sure].any()
     np.testing.assert_array_equal(got[sure], keep[sure].astype(int))
     assert ops.error_flags() == 0
+
+
+# ---- drafts: draws beside the border of two tokens ---------------------------------------------------------------------------------------------
+# sample_u is the f32 number next to the share of the weights up to some token, so that the target is 2^-25 of the whole from a border at most.  Weights are known to 2^-34 of themselves and so is
+# their sum up to any token; where a draft's distribution is taken off them, to 2^-33 of the target's whole.  Entries nearer than 2^-32 of the whole may go either way.
+@pytest.mark.parametrize("form", ["sampled", "certain draft", "drafted", "top_p"])
+@pytest.mark.parametrize("V,T", [(128256, 1.0), (50257, 0.6), (131072, 3.0), (1000, 1.0)])
+def test_draws_beside_a_border(ops, form, V, T):
+    rng = np.random.default_rng(V)
+    B, z = 120, (2 * rng.standard_normal(V)).astype(np.float32)
+    p = oracle.probabilities(z, float(np.float32(T)), 0, float(np.float32(0.9)) if form == "top_p" else 1.0)      # (of the numbers that the call gets)
+    n, q, x = (1 if "draft" in form else 0), None, int(z.argmin())
+    w = np.array(p)
+    if form == "certain draft":
+        w[x] = 0.0
+    elif form == "drafted":
+        y = z / T + 0.5 * rng.standard_normal(V)
+        y[x] += 12.0
+        q = np.exp(y - y.max())
+        q = (q / q.sum()).astype(np.float32)
+        w = np.maximum(p - q, 0.0)
+    cum = np.cumsum(w) / w.sum()
+    some = np.nonzero(w)[0][:-1]
+    us = cum[some[(np.arange(B) * (len(some) / B)).astype(int)]].astype(np.float32)
+    R = B * (n + 1)
+    start = np.arange(B + 1) * (n + 1)
+    args = (start, np.full(R, x), np.full(R, 1 - 2.0 ** -24, np.float32), us, np.full(B, T, np.float32), None, np.full(B, 0.9, np.float32) if form == "top_p" else None)
+    got = run_verify(ops, up(z).expand(R, V).contiguous(), *args, None if q is None else up(q).expand(R, V).contiguous())
+    near = np.abs(cum[None, some] - us[:, None].astype(np.float64)).min(1) * w.sum()
+    want = np.minimum(np.searchsorted(cum, us.astype(np.float64), side="right"), some[-1] + 1)
+    sure = near > 2.0 ** -32
+    assert sure.sum() >= B // 2 and (near < 2.0 ** -20).all()
+    np.testing.assert_array_equal(got[0], 0)
+    np.testing.assert_array_equal(got[1][::n + 1][sure], want[sure])
 
 
 # ---- weights: heads whose sink is none -------------------------------------------------------------------------------------------------------
