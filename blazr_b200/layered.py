@@ -1345,6 +1345,10 @@ class LayeredModel:
         ptr = lambda k: ws.view(k).data_ptr()
         return seqops.StepDesc(ptr("ent"), ptr(positions), ptr("start"), ptr("slot"), ptr("pos0"), ptr("bt"), T, B, self.max_blocks, self.block_size)
 
+    def _turned(self, ws: _Workspace, st: seqops.StepDesc) -> seqops.StepDesc:
+        """the step by places in the sequences (where no rows leave the cache, its rows are those)"""
+        return self._desc(ws, st.T, st.B, "abs") if self.weighed_rows > 0 else st
+
     def forward(self, sa: StepArrays, sample: bool = False, debug_layers: Optional[list] = None) -> torch.Tensor:
         """runs one step; returns f32 logits [R, vocab] of the wanted rows (a view of a buffer the next step overwrites);
         sample: also leaves the greedy token of every wanted row in `self.last_ids` (int32 [R], device)"""
@@ -1771,7 +1775,7 @@ class LayeredModel:
                 if m.norm == "joint":
                     P = ops.retention_partials(T, B, H, V)
                     close.update(sumsq=ws.sumsq.view(-1)[:T * P].view(T, P), sumsq_count=H * V)
-                ops.retention(proj, self._desc(ws, T, B, "abs"), L["desc"], L["ret_state"], o, ws.scratch, sumsq=close.get("sumsq"))
+                ops.retention(proj, self._turned(ws, st), L["desc"], L["ret_state"], o, ws.scratch, sumsq=close.get("sumsq"))
                 ops.linear(o, L["w_o"], y)
             elif ls.kind == "attention":
                 self._attention_out(L, m, ws, st, T, proj, y)
@@ -1871,7 +1875,7 @@ class LayeredModel:
         proj = ws.proj[:T, :L["w_in"].shape[0]]
         seqops.linear(a, L["w_in"], proj)
         o = ws.inner_a.view(-1)[:T * m.heads * m.vdim].view(T, m.heads * m.vdim)
-        seqops.retention(proj, self._desc(ws, T, st.B, "abs"), L["desc"], L["ret_state"], o, ws.scratch)
+        seqops.retention(proj, self._turned(ws, st), L["desc"], L["ret_state"], o, ws.scratch)
         seqops.linear(o, L["w_o"], y)
 
     def _latent_attention(self, L, m: LatentAttentionSpec, ws: _Workspace, st, T: int, a: torch.Tensor, y: torch.Tensor) -> None:
