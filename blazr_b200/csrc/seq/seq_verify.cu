@@ -6,8 +6,8 @@
 //
 // What a row decides is compared with a random number, so that its sums are held in 64 bits.  The weights behind one comparison (a draft, the end of top_p) are f32, within 2^-21 of
 // themselves; a draw is a comparison with 10^5 sums, and its weights are made in 64 bits, within 2^-34.
-// Measured: 64 entries of 4 drafts, 128256 logits a row, 61 us (33.5 + 35; with draws of f32 weights 55, 28 of them; the logits' bytes alone 25, the draft's probabilities of a row an
-// entry 5); one of 32000 logits 19, a chain of loads and of the clusters' barriers; 16 entries of 3 drafts with top_k and top_p 52 to 57 (thresholds 42 to 45).
+// Measured: 64 entries of 4 drafts, 128256 logits a row, 58 us (33.5 + 31; with draws of f32 weights 55, 28 of them; the logits' bytes alone 25, the draft's probabilities of a row an
+// entry 5); one of 32000 logits 18.5, a chain of loads and of the clusters' barriers; 16 entries of 3 drafts with top_k and top_p 52 to 57 (thresholds 42 to 45).
 // The floor is the logits' bytes: they are read once, in slices over the whole GPU (row_stats), with maximum, its place and sum left for every slice.  Then a cluster of eight
 // CTAs an entry puts the slices together, finds the row that rejects and reads that one again, from L2, every warp a run of it (pick).
 // top_k and top_p need a threshold a row before that (row_cut, a CTA a row, which it reads twice or three times from L2): counts, or masses (whole numbers of 2^-42: additions whose
@@ -483,7 +483,7 @@ struct Share {
 // grid: a cluster an entry
 __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_kernel(const __grid_constant__ VerifyArgs a) {
     chain_enter();
-    constexpr int WARPS = PICK / 32, ROWS = 32;
+    constexpr int WARPS = PICK / 32, ROWS = 32, AHEAD = 4;
     __shared__ double scan[PICK], warp_part[WARPS];
     __shared__ Share warp_share[WARPS], cta_share;
     __shared__ int first_bad, found, last_some;
@@ -555,23 +555,19 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_ker
     // Weights in 64 bits: which of 10^5 sums is the first beyond the target is known only to their own digits (in 32 bits one draw in 10^4 was the neighbour's).  Drawn from is what
     // w has more than S q, S the sum of all w.  That is known only behind the walk over the row, which takes `about` for S: where weights are left, sums of q tell what that changes.
     const FineHeat weight(T, r.max, least);
-    // the four weights of a lane at quad k, and q; false: the whole warp has none
-    auto weights = [&](int k, double (&w)[4], float (&qv)[4]) {
+    auto load = [&](int k, float4& z, float4& qv) {
         const int i = 4 * k - shift;
-        const float4 z4 = quad(x, i, a.V, -INFINITY);
-        const float z[4] = {z4.x, z4.y, z4.z, z4.w};
-        float4 q4 = make_float4(0.f, 0.f, 0.f, 0.f);
+        z = quad(x, i, a.V, -INFINITY), qv = make_float4(0.f, 0.f, 0.f, 0.f);
         if (q) {
-            if (aligned_q) q4 = quad(q, i, a.V, 0.f);
-            else q4 = make_float4(i >= 0 && i < a.V ? q[i] : 0.f, i + 1 >= 0 && i + 1 < a.V ? q[i + 1] : 0.f, i + 2 >= 0 && i + 2 < a.V ? q[i + 2] : 0.f,
+            if (aligned_q) qv = quad(q, i, a.V, 0.f);
+            else qv = make_float4(i >= 0 && i < a.V ? q[i] : 0.f, i + 1 >= 0 && i + 1 < a.V ? q[i + 1] : 0.f, i + 2 >= 0 && i + 2 < a.V ? q[i + 2] : 0.f,
                                   i + 3 >= 0 && i + 3 < a.V ? q[i + 3] : 0.f);
         }
-        qv[0] = q4.x, qv[1] = q4.y, qv[2] = q4.z, qv[3] = q4.w;
-        const bool some = __any_sync(0xffffffffu, fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])) >= weight.lowest);
-        if (some) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = weight(z[j]);
-        }
+    };
+    // the four weights of a lane; false: the whole warp has none
+    auto weights = [&](const float4& z, double (&w)[4]) {
+        const bool some = __any_sync(0xffffffffu, fmaxf(fmaxf(z.x, z.y), fmaxf(z.z, z.w)) >= weight.lowest);
+        if (some) w[0] = weight(z.x), w[1] = weight(z.y), w[2] = weight(z.z), w[3] = weight(z.w);
         return some;
     };
     auto left = [&](double w, float qv, double all) {      // (a q that is no number takes all)
@@ -579,21 +575,27 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_ker
         const double l = fma(-all, widened(qv), w);
         return __double2hiint(l) < 0 ? 0.0 : l;
     };
-    // every warp a run of neighbouring quads, every lane its sums
+    // every warp a run of neighbouring quads, every lane its sums, AHEAD quads asked for at a time (64 entries with drafts' probabilities, in all: one 61.8 us, two 60.9, four 58.0)
     const int quads = (a.V + shift + 3) / 4, run = ((quads + CLUSTER * WARPS - 1) / (CLUSTER * WARPS) + 31) & ~31;
     Share mine{0.0, 0.0, 0.f};
     const int k0 = (rank * WARPS + warp) * run;
-#pragma unroll 4
-    for (int k = k0 + lane; k < min(k0 + run, (quads + 31) & ~31); k += 32) {
-        double w[4];
-        float qv[4];
-        if (!weights(k, w, qv)) continue;
+    const int k1 = min(k0 + run, (quads + 31) & ~31);
+    for (int kk = k0 + lane; kk < k1; kk += 32 * AHEAD) {
+        float4 z[AHEAD], qv[AHEAD];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            mine.all += w[j];
-            const double l = 4 * k - shift + j == certain ? 0.0 : left(w[j], qv[j], about);
-            mine.draw += l;
-            if (q && __double2hiint(l) > 0) mine.off += qv[j];
+        for (int u = 0; u < AHEAD; ++u) load(kk + 32 * u < k1 ? kk + 32 * u : quads, z[u], qv[u]);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            double w[4];
+            if (!weights(z[u], w)) continue;
+            const float qs[4] = {qv[u].x, qv[u].y, qv[u].z, qv[u].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                mine.all += w[j];
+                const double l = 4 * (kk + 32 * u) - shift + j == certain ? 0.0 : left(w[j], qs[j], about);
+                mine.draw += l;
+                if (q && __double2hiint(l) > 0) mine.off += qs[j];
+            }
         }
     }
     mine.draw = warp_sum(mine.draw), mine.all = warp_sum(mine.all);
@@ -638,12 +640,15 @@ __global__ void __cluster_dims__(CLUSTER, 1, 1) __launch_bounds__(PICK) pick_ker
         // that warp's run, by the block: a tile of its quads at a time
         const int from = (rank * WARPS + of) * run, to = min(from + run, quads);
         for (int t = from; t < to; t += PICK) {
-            double w[4];
-            float qv[4];
+            double w[4] = {0.0, 0.0, 0.0, 0.0};
+            float4 z, qv;
             const int k = t + tid;
-            if (!weights(min(k, quads), w, qv)) w[0] = w[1] = w[2] = w[3] = 0.0;
+            load(k < to ? k : quads, z, qv);                // (behind the last quad: minus infinities)
+            weights(z, w);
+            const float qs[4] = {qv.x, qv.y, qv.z, qv.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = k >= to ? 0.0 : rest ? (4 * k - shift + j == certain ? 0.0 : left(w[j], qv[j], row_share.all)) : w[j];
+            for (int j = 0; j < 4; ++j)
+                if (rest) w[j] = 4 * k - shift + j == certain ? 0.0 : left(w[j], qs[j], row_share.all);
             const double own = (w[0] + w[1]) + (w[2] + w[3]);
             double s = own;
 #pragma unroll
